@@ -48,6 +48,8 @@ extern "C" {
 #define ST_F16 1
 #define ST_BF16 2
 #define ST_I32 3
+#define ST_E4M3 4 /* 8-bit floats: st_quantize_fp8, st_matmul_fp8 and the norms' 8-bit output only */
+#define ST_E5M2 5
 
 /* ---- binding kinds of st_param ---- */
 #define ST_PARAM_BUFFER 0 /* data pointer of one array (spirv StorageBuffer f32[]) */
@@ -241,6 +243,69 @@ int st_vector_fma(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
 /* C = A converted to C's dtype (ST_F32 / ST_F16 / ST_BF16; round to nearest
  * even when narrowing) -- the lowering's ftof (tileops.hpp:257-258). */
 int st_cast(st_ctx *ctx, const st_tensor *a, const st_tensor *c, const st_exec *exec);
+
+/* ---- 8-bit operands with a scale for each block of 128 ----
+ * No counterpart in the reference.  Device memory only.
+ *
+ * st_quantize_fp8: for each block_rows x block_cols block of A (1 x 128,
+ * 128 x 1 or 128 x 128; the last ones may be cut by A's edge)
+ *   scale = max(max|a| / limit, 2^-126)   limit 448 for ST_E4M3, 57344 for ST_E5M2
+ *   q     = fp8(a * (1 / scale))          round to nearest even, saturating
+ * each step one fp32 operation.  A NaN or infinity makes its block's scale
+ * NaN or infinite, and what is computed from the block NaN.  A is f32, f16 or
+ * bf16, Q ST_E4M3 or ST_E5M2 of A's shape, scale f32 of one element per
+ * block; any strides (Q's fastest rows are those on 8-byte boundaries, and
+ * st_matmul_fp8 reads without a copy those on 16-byte boundaries). */
+int st_quantize_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *q, const st_tensor *scale,
+                    int32_t block_rows, int32_t block_cols, const st_exec *exec);
+/* C[m, n] = sum_b a_scale[m, b] b_scale[b, n] sum_{k in block b of 128} A[m, k] B[k, n]  (+ bias[n])
+ *   A [M, K], B [K, N]    ST_E4M3 or ST_E5M2, each of its own; any strides
+ *   a_scale               f32 [M, ceil(K/128)] or, one scale for 128 rows, [ceil(M/128), ceil(K/128)]
+ *   b_scale               f32 [ceil(K/128), N] or [ceil(K/128), ceil(N/128)]
+ *   C                     f32, f16 or bf16, unit column stride;  bias: f32 or C's dtype
+ * The sum over blocks is kept in fp32.  Gradients are calls of the same kind:
+ * with dY in blocks of 1 x 128, dX = dY @ W reads W [N, K] as it is stored;
+ * with dY and X in blocks of 128 x 1 (tokens), dW = dY^T @ X reads both as
+ * they are stored, through transposed views.  The same inputs give the same
+ * bits.  An operand that neither starts on a 16-byte boundary nor has its
+ * rows (or columns) 16 bytes apart is copied first, into `workspace`:
+ * st_matmul_fp8_workspace gives the bytes, 0 where none is needed. */
+int st_matmul_fp8_workspace(const st_tensor *a, const st_tensor *b, uint64_t *bytes);
+int st_matmul_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_tensor *a_scale,
+                  const st_tensor *b_scale, const st_tensor *bias, const st_tensor *c, void *workspace,
+                  uint64_t workspace_bytes, const st_exec *exec);
+
+/* ---- the norms after and before a block, its gate and residual scale ----
+ * No counterpart in the reference.  Device memory only; tensors [rows, cols]
+ * with unit column stride, 1 to 16384 columns.
+ *   u            = x * rsqrt(mean(x^2) + eps) * (post + weight_offset)     (x where post is NULL)
+ *   residual_out = residual + alpha * gate * u                             (residual where x is NULL)
+ *   normed       = r * rsqrt(mean(r^2) + eps) * (pre + weight_offset)      r: residual_out before its rounding
+ * x, normed: one type T (f32, f16 or bf16); residual, residual_out: T or f32;
+ * post, pre [cols] and gate: T or f32.  gate: [cols] or [1, cols], [rows, 1]
+ * or [rows, cols]; NULL for 1.  normed may be ST_E4M3 or ST_E5M2: then in
+ * blocks of 1 x 128 as st_quantize_fp8 makes them, their scales in
+ * normed_scale [rows, ceil(cols/128)].  residual_out may be residual itself. */
+typedef struct {
+    float alpha, eps, weight_offset;
+} st_norm_options;
+int st_residual_norm(st_ctx *ctx, const st_tensor *x, const st_tensor *residual, const st_tensor *post,
+                     const st_tensor *gate, const st_tensor *pre, const st_tensor *residual_out,
+                     const st_tensor *normed, const st_tensor *normed_scale, const st_norm_options *options,
+                     const st_exec *exec);
+/* The gradients of the call above at `residual`, its residual_out as stored:
+ * d_residual and d_normed (either may be NULL) to dx, dr (the incoming
+ * stream's; may be NULL), dpost, dpre (f32 [cols]; may be NULL) and dgate (the gate's shape: f32, or T where it is
+ * [rows, cols]).  `workspace` holds partial sums over rows:
+ * st_residual_norm_backward_workspace gives its bytes.  The same inputs give
+ * the same bits. */
+int st_residual_norm_backward_workspace(int64_t rows, int64_t cols, uint64_t *bytes);
+int st_residual_norm_backward(st_ctx *ctx, const st_tensor *d_residual, const st_tensor *d_normed,
+                              const st_tensor *x, const st_tensor *residual, const st_tensor *post,
+                              const st_tensor *gate, const st_tensor *pre, const st_tensor *dx, const st_tensor *dr,
+                              const st_tensor *dpost, const st_tensor *dgate, const st_tensor *dpre,
+                              void *workspace, uint64_t workspace_bytes, const st_norm_options *options,
+                              const st_exec *exec);
 
 /* ---- typed calls on host memory: copy in, compute, copy out, all on the
  *      context's stream; returns once C is back in host memory. ---- */

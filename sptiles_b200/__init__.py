@@ -16,6 +16,8 @@ from .runtime import (  # noqa: F401
     run_tile_kernel,
     shard_range, shutdown, stream_k_split, sync, tensor_1d_descriptor, tensor_2d_descriptor, tile_raster,
 )
+from .fp8 import matmul_fp8, quantize_fp8  # noqa: F401
+from .norm import ResidualNorm, ResidualNormGrads, residual_norm, residual_norm_backward  # noqa: F401
 from .module import ModuleEntry, TileModule  # noqa: F401
 from ._native import DeviceAbort, NativeError, lib  # noqa: F401
 

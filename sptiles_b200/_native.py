@@ -25,6 +25,7 @@ ST_ERR_TIMEOUT = 7
 ST_ERR_DEVICE_ABORT = 8
 
 ST_F32, ST_F16, ST_BF16, ST_I32 = 0, 1, 2, 3
+ST_E4M3, ST_E5M2 = 4, 5
 ST_PARAM_BUFFER, ST_PARAM_I32 = 0, 1
 ST_MODULE_PARAM_BUFFER, ST_MODULE_PARAM_I32, ST_MODULE_PARAM_OTHER = 0, 1, 2
 ST_EXEC_SYNC, ST_EXEC_HOST_BUFFERS, ST_EXEC_DETERMINISTIC, ST_EXEC_ALL_DEVICES = 1, 2, 4, 8
@@ -35,6 +36,8 @@ EXPORTED = (
     "st_alloc", "st_free", "st_upload", "st_download", "st_launch", "st_grid_from_dispatch",
     "st_vector_add", "st_matmul", "st_vector_add_host", "st_matmul_host", "st_tile_raster",
     "st_matmul_plan", "st_stream_k_split", "st_shard_range", "st_matmul_static_scratch", "st_vector_fma", "st_cast",
+    "st_quantize_fp8", "st_matmul_fp8_workspace", "st_matmul_fp8", "st_residual_norm",
+    "st_residual_norm_backward_workspace", "st_residual_norm_backward",
     "st_ipc_handle", "st_ipc_open", "st_ipc_close", "st_matmul_allgather",
     "st_module_load", "st_module_load_file", "st_module_free", "st_module_version", "st_module_entry_count",
     "st_module_entry", "st_module_param", "st_launch_module", "st_check_device_wait",
@@ -59,6 +62,10 @@ class StExec(ctypes.Structure):
     _fields_ = [("stream", ctypes.c_void_p), ("device", ctypes.c_int32), ("flags", ctypes.c_int32),
                 ("timeout_ms", ctypes.c_uint32), ("output_indices", ctypes.POINTER(ctypes.c_int32)),
                 ("n_outputs", ctypes.c_int32)]
+
+
+class StNormOptions(ctypes.Structure):
+    _fields_ = [("alpha", ctypes.c_float), ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float)]
 
 
 class StModuleEntryInfo(ctypes.Structure):
@@ -111,6 +118,12 @@ def _declare(L: ctypes.CDLL) -> None:
         "st_matmul_host": ([vp, _P(StTensor), _P(StTensor), _P(StTensor), _P(StTensor), _P(StExec)], _c.c_int),
         "st_vector_fma": ([vp, _P(StTensor), _P(StTensor), _P(StTensor), _P(StTensor), _P(StExec)], _c.c_int),
         "st_cast": ([vp, _P(StTensor), _P(StTensor), _P(StExec)], _c.c_int),
+        "st_quantize_fp8": ([vp, _P(StTensor), _P(StTensor), _P(StTensor), i32, i32, _P(StExec)], _c.c_int),
+        "st_matmul_fp8_workspace": ([_P(StTensor), _P(StTensor), _P(u64)], _c.c_int),
+        "st_matmul_fp8": ([vp] + [_P(StTensor)] * 6 + [vp, u64, _P(StExec)], _c.c_int),
+        "st_residual_norm": ([vp] + [_P(StTensor)] * 8 + [_P(StNormOptions), _P(StExec)], _c.c_int),
+        "st_residual_norm_backward_workspace": ([i64, i64, _P(u64)], _c.c_int),
+        "st_residual_norm_backward": ([vp] + [_P(StTensor)] * 12 + [vp, u64, _P(StNormOptions), _P(StExec)], _c.c_int),
         "st_ipc_handle": ([vp, i32, vp, _P(_c.c_uint8)], _c.c_int),
         "st_ipc_open": ([vp, i32, _P(_c.c_uint8), _P(vp)], _c.c_int),
         "st_ipc_close": ([vp, i32, vp], _c.c_int),

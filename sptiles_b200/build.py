@@ -18,7 +18,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libsptiles_b200.so"
-SOURCES = ["runtime.cu", "vecadd.cu", "elementwise.cu", "gemm.cu", "pack.cu", "noalloc.cu", "module.cu", "diag.cu"]
+SOURCES = ["runtime.cu", "vecadd.cu", "elementwise.cu", "gemm.cu", "pack.cu", "noalloc.cu", "module.cu", "diag.cu",
+           "quantize.cu", "gemm_fp8.cu", "norm.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

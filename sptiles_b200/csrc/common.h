@@ -227,4 +227,79 @@ int launch_pack_ab_tf32(const float *a, int64_t sa0, int64_t sa1, int64_t m, con
 int launch_repack_16(const uint16_t *src, int64_t s0, int64_t s1, int64_t rows, int64_t cols, uint16_t *dst,
                      int64_t ld, cudaStream_t stream);
 
+// ---- 8-bit operands with a scale per block of 128 along K (gemm_fp8.cu)
+// One operand as [rows, k]: A's rows are M, B's rows are N.  Element (i, b)
+// of `scale` belongs to rows [i << scale_shift, (i + 1) << scale_shift) and
+// to K block b.
+struct Fp8Operand {
+    const void *data;
+    int64_t rows, k;
+    int64_t s_row, s_k;  // element strides
+    uint32_t e5m2;       // 0: e4m3
+    const void *scale;
+    int64_t scale_row, scale_k;
+    int scale_shift;  // 0 or 7
+};
+
+struct GemmFp8Args {
+    Fp8Operand a, b;
+    void *c;
+    int64_t ldc;
+    int c_dtype;
+    const void *bias;
+    int bias_dtype;
+};
+
+// Bytes of workspace for copies of the operands that TMA cannot address.
+int64_t gemm_fp8_workspace_bytes(const Fp8Operand &a, const Fp8Operand &b);
+int launch_gemm_fp8(const GemmFp8Args &args, void *workspace, int sm_count, int *dev_err, uint64_t timeout_ns,
+                    cudaStream_t stream);
+
+// q = fp8(a / scale) with one scale per block_rows x block_cols block (quantize.cu).
+struct QuantizeArgs {
+    const void *a;
+    int a_dtype;
+    int64_t sa0, sa1;
+    void *q;
+    bool e5m2;
+    int64_t sq0, sq1;
+    float *scale;
+    int64_t ss0, ss1;
+    int64_t rows, cols;
+    int block_rows, block_cols;  // 1 x 128, 128 x 1 or 128 x 128
+};
+int launch_quantize_fp8(const QuantizeArgs &args, cudaStream_t stream);
+
+// Norms around a block (norm.cu).  Strides in elements; unit column strides.
+struct NormView {
+    void *p = nullptr;
+    int dtype = ST_F32;
+    int64_t ld = 0;
+};
+enum : int { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateFull = 3 };
+struct NormArgs {
+    int64_t rows, cols;
+    float alpha, eps, offset;
+    NormView x, r, r_out, h;
+    NormView post, pre, gate;  // post, pre and a channel gate: one row; a token gate: ld per row
+    int gate_mode = kGateNone;
+    float *h_scale = nullptr;  // h is 8-bit: its scales per 1 x 128 block
+    int64_t hs0 = 0, hs1 = 0;
+    bool h_e5m2 = false, h_fp8 = false;
+};
+int launch_residual_norm(const NormArgs &args, int sm_count, cudaStream_t stream);
+
+struct NormBackwardArgs {
+    int64_t rows, cols;
+    float alpha, eps, offset;
+    NormView d_residual, d_normed;  // p null: absent
+    NormView x, r;                  // the branch and the updated stream
+    NormView post, pre, gate;
+    int gate_mode = kGateNone;
+    NormView dx, dr, dgate;  // dgate: rows x cols (full) or float per row / column
+    float *dpost = nullptr, *dpre = nullptr;
+};
+int64_t residual_norm_backward_workspace(int64_t rows, int64_t cols);
+int launch_residual_norm_backward(const NormBackwardArgs &args, void *workspace, int sm_count, cudaStream_t stream);
+
 }  // namespace st

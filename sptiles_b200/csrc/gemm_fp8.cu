@@ -1,0 +1,654 @@
+// gemm_fp8.cu -- matrix product of 8-bit operands with a scale for each
+// block of 128 along the contraction.
+//
+//   C[m, n] = sum_b sa[m, b] * sb[b, n] * sum_{k in block b} A[m, k] * B[k, n]  (+ bias[n])
+//
+// A and B are e4m3 or e5m2, sa and sb float32.  The inner sum of a block is
+// one K = 128 chain of tcgen05.mma (kind::f8f6f4) into a fresh TMEM
+// accumulator; the epilogue warps read each block's accumulator, multiply by
+// the block's two scales and add onto running sums in fp32 registers, while
+// the tensor core works on the next blocks in the other TMEM accumulators.
+// So the sum over blocks is a plain fp32 sum, whatever the scales are.
+//
+//   warp 0      TMA producer: one 128-byte-swizzled box of each operand per block
+//   warp 1      MMA issuer (owns the TMEM allocation)
+//   warps 2-5   scaling: TMEM -> registers, scale, add; then bias and the store
+//
+// The kernel knows a row operand (128 rows a tile, the MMA's M) and a column
+// operand (BN columns, the MMA's N).  A call with few tokens makes the
+// weights the row operand and the tokens the columns, so that a tile reads
+// 128 rows of weights against 16 to 64 tokens and nothing is padded to 128
+// tokens.  When tiles alone would leave SMs idle, a cluster of up to 8 CTAs
+// splits the blocks of one tile and adds its parts in a fixed order through
+// distributed shared memory.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <mutex>
+
+#include "common.h"
+#include "sm100.cuh"
+
+namespace st {
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kBlockK = 128;  // bytes = elements: one scale block, one 128-byte swizzle span
+constexpr int kThreads = 192;
+constexpr int kScaleWarps = 4;
+constexpr int kMmaK = 32;
+constexpr int kBarBytes = 1024;
+
+struct Fp8Params {
+    int rows, cols, k_blocks;  // row operand x column operand
+    int tiles_r, tiles_c, split;
+    const float *rs, *cs;        // scales of the row and the column operand
+    int64_t rs_i, rs_b, cs_i, cs_b;  // strides: per index (row / column or their block of 128), per K block
+    int rs_shift, cs_shift;      // 7: one scale for 128 rows / columns
+    void *c;
+    int64_t c_r, c_c;  // strides of C along the row and the column operand
+    int c_dtype;
+    const void *bias;
+    int bias_dtype;
+    int bias_on_rows;
+    uint32_t idesc;
+    int *err;
+    unsigned long long timeout_ns;
+};
+
+template <int BN>
+struct Fp8Cfg {
+    static constexpr int kRowBytes = kTileRows * kBlockK;
+    static constexpr int kColBytes = BN * kBlockK;
+    static constexpr int kStageBytes = kRowBytes + kColBytes;
+    // BN 128 fills an SM's TMEM (4 x 128 columns) and shared memory alone;
+    // narrower tiles leave room for two CTAs per SM
+    static constexpr int kStages = BN == 128 ? 6 : (BN == 64 ? 4 : (BN == 32 ? 5 : 6));
+    static constexpr int kAccs = 4;
+    static constexpr int kTmemCols = kAccs * BN;
+    static constexpr int kColScaleBytes = kScaleWarps * 2 * BN * 4;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kColScaleBytes + 1024;
+    static_assert(kSmemBytes <= (BN == 128 ? 232448 : 115712), "shared memory of one (two) CTAs per SM");
+    static_assert(kStages * kStageBytes >= kTileRows * BN * 4, "the ring holds a tile's partial sums");
+};
+
+__device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
+    if (dtype == ST_F32) return static_cast<const float *>(p)[i];
+    if (dtype == ST_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+
+__device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v) {
+    if (dtype == ST_F32) static_cast<float *>(p)[i] = v;
+    else if (dtype == ST_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// acc (two fp32) += v * s, one packed instruction
+__device__ __forceinline__ void fma2(uint64_t &acc, uint32_t v0, uint32_t v1, uint64_t s) {
+    asm("{\n\t.reg .b64 v;\n\t"
+        "mov.b64 v, {%1, %2};\n\t"
+        "fma.rn.f32x2 %0, v, %3, %0;\n\t}"
+        : "+l"(acc)
+        : "r"(v0), "r"(v1), "l"(s));
+}
+
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    return static_cast<uint64_t>(__float_as_uint(a)) | (static_cast<uint64_t>(__float_as_uint(b)) << 32);
+}
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+
+// Load 16 consecutive f32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+// Wait for the loads above; the registers pass through, so that nothing reads
+// them before it.
+__device__ __forceinline__ void tmem_load_wait_16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
+// R_MN / C_MN: the operand is stored with its rows (columns) contiguous
+// instead of K.  CVEC: the column scale differs inside the tile.
+template <int BN, bool R_MN, bool C_MN, bool CVEC>
+__global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
+    gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
+                    const Fp8Params p) {
+    using Cfg = Fp8Cfg<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::kStages * Cfg::kStageBytes);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * Cfg::kStages + 2 * Cfg::kAccs + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    float *col_scale = reinterpret_cast<float *>(smem + Cfg::kStages * Cfg::kStageBytes + kBarBytes);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t bar0 = smem_addr(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };
+    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + a); };
+    auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + Cfg::kAccs + a); };
+    const uint32_t drain_bar = bar0 + 8u * (2 * Cfg::kStages + 2 * Cfg::kAccs);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Cfg::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int a = 0; a < Cfg::kAccs; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), kScaleWarps);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_map(&tmap_r);
+        tma_prefetch_map(&tmap_c);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_addr(tmem_slot), Cfg::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_begin();  // nothing above touches global memory
+
+    const int split = p.split;
+    const int part = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int tile = static_cast<int>(blockIdx.x) / split;
+    // neighbouring CTAs walk the row tiles of one column tile
+    const int r0 = (tile % p.tiles_r) * kTileRows;
+    const int c0 = (tile / p.tiles_r) * BN;
+    const int b0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * part / split);
+    const int b1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / split);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint64_t pol = l2_policy_evict_last();
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int b = b0; b < b1; ++b, ++issued) {
+                if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
+                    ok = false;
+                    break;
+                }
+                mbar_arrive_expect_tx(full_bar(s), Cfg::kStageBytes);
+                const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
+                const uint32_t sc = sr + Cfg::kRowBytes;
+                const int k0 = b * kBlockK;
+                if constexpr (R_MN) tma_load_2d(sr, &tmap_r, full_bar(s), r0, k0, pol);
+                else tma_load_2d(sr, &tmap_r, full_bar(s), k0, r0, pol);
+                if constexpr (C_MN) tma_load_2d(sc, &tmap_c, full_bar(s), c0, k0, pol);
+                else tma_load_2d(sc, &tmap_c, full_bar(s), k0, c0, pol);
+                if (++s == Cfg::kStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                atomicExch(p.err, kDevAbortGemmProducer);
+            }
+            // no copy is in flight when the CTA leaves, also after an abort
+            const volatile int never = 0;
+            for (int i = issued > Cfg::kStages ? issued - Cfg::kStages : 0; i < issued; ++i)
+                (void)mbar_wait(full_bar(i % Cfg::kStages), static_cast<uint32_t>(i / Cfg::kStages) & 1u, &never,
+                                p.timeout_ns);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int s = 0, a = 0;
+            uint32_t ph = 0, aph = 0;
+            bool ok = true;
+            for (int b = b0; b < b1; ++b) {
+                if (!mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns) ||
+                    !mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+                const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
+                const uint32_t sc = sr + Cfg::kRowBytes;
+#pragma unroll
+                for (int ks = 0; ks < kBlockK / kMmaK; ++ks) {
+                    // K-major: 32 bytes further along the 128-byte span; otherwise 32 K rows of 128 bytes
+                    const uint64_t dr = smem_desc_sw128(sr + ks * (R_MN ? kMmaK * 128 : kMmaK), R_MN ? 128 * 128 : 16, 1024);
+                    const uint64_t dc = smem_desc_sw128(sc + ks * (C_MN ? kMmaK * 128 : kMmaK), C_MN ? 128 * 128 : 16, 1024);
+                    tc_mma_f8(tmem_base + static_cast<uint32_t>(a * BN), dr, dc, p.idesc, ks != 0 ? 1u : 0u);
+                }
+                tc_commit(empty_bar(s));
+                tc_commit(tfull_bar(a));
+                if (++s == Cfg::kStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+                if (++a == Cfg::kAccs) {
+                    a = 0;
+                    aph ^= 1u;
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                atomicExch(p.err, kDevAbortGemmMma);
+            }
+            tc_commit(drain_bar);
+            (void)mbar_wait(drain_bar, 0, abort_flag, p.timeout_ns);
+        }
+    }
+
+    // ------------------------------------------------ scaling warps
+    const int g = warp & 3;
+    const int row_in_tile = g * 32 + lane;
+    const int row = r0 + row_in_tile;
+    uint64_t acc[BN / 2];
+    if (warp >= 2) {
+#pragma unroll
+        for (int j = 0; j < BN / 2; ++j) acc[j] = 0;
+        const bool row_ok = row < p.rows;
+        const float *rs = p.rs + static_cast<int64_t>(row_ok ? row >> p.rs_shift : 0) * p.rs_i;
+        const float *cs = p.cs + static_cast<int64_t>(c0 >> p.cs_shift) * p.cs_i;
+        float *my_cols = col_scale + g * 2 * BN;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(g * 32) << 16);
+        int a = 0;
+        uint32_t aph = 0;
+        for (int b = b0; b < b1; ++b) {
+            const float r_scale = row_ok ? rs[b * p.rs_b] : 0.0f;
+            float c_scale = 0.0f;
+            if constexpr (CVEC) {
+                float *buf = my_cols + (b & 1) * BN;
+#pragma unroll
+                for (int j = lane; j < BN; j += 32)
+                    buf[j] = c0 + j < p.cols
+                                 ? p.cs[static_cast<int64_t>((c0 + j) >> p.cs_shift) * p.cs_i + b * p.cs_b]
+                                 : 0.0f;
+                __syncwarp();
+            } else {
+                c_scale = cs[b * p.cs_b];
+            }
+            const bool ready = mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns);
+            if (!__all_sync(0xffffffffu, ready)) {
+                *abort_flag = 1;
+                if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
+                break;
+            }
+            tc_fence_after_sync();
+            const uint32_t t = t_lane + static_cast<uint32_t>(a * BN);
+            const float both = r_scale * c_scale;
+            const uint64_t s2 = CVEC ? pack2(r_scale, r_scale) : pack2(both, both);
+#pragma unroll
+            for (int j = 0; j < BN; j += 16) {
+                uint32_t v[16];
+                tmem_load_16(t + j, v);
+                tmem_load_wait_16(v);
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    if constexpr (CVEC) {
+                        const float4 c = *reinterpret_cast<const float4 *>(my_cols + (b & 1) * BN + j + i);
+                        fma2(acc[(j + i) / 2], v[i], v[i + 1], mul2(s2, pack2(c.x, c.y)));
+                        fma2(acc[(j + i) / 2 + 1], v[i + 2], v[i + 3], mul2(s2, pack2(c.z, c.w)));
+                    } else {
+                        fma2(acc[(j + i) / 2], v[i], v[i + 1], s2);
+                        fma2(acc[(j + i) / 2 + 1], v[i + 2], v[i + 3], s2);
+                    }
+                }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty_bar(a));
+            if (++a == Cfg::kAccs) {
+                a = 0;
+                aph ^= 1u;
+            }
+        }
+    }
+
+    // ------------------------------------------------ bias, conversion and the store
+    auto put = [&](int j, float v) {  // column j of the tile
+        const int col = c0 + j;
+        if (row >= p.rows || col >= p.cols) return;
+        if (p.bias != nullptr) v += load_any(p.bias, p.bias_dtype, p.bias_on_rows ? row : col);
+        store_any(p.c, p.c_dtype, row * p.c_r + col * p.c_c, v);
+    };
+    if (split == 1) {
+        if (warp >= 2) {
+            const int es = p.c_dtype == ST_F32 ? 4 : 2;
+            const bool wide = p.c_c == 1 && c0 + BN <= p.cols && p.bias == nullptr &&
+                              (reinterpret_cast<uintptr_t>(p.c) & 15u) == 0 && (p.c_r * es) % 16 == 0;
+            if (wide && row < p.rows) {
+                uint8_t *dst = static_cast<uint8_t *>(p.c) + (row * p.c_r + c0) * es;
+                if (p.c_dtype == ST_F32) {
+#pragma unroll
+                    for (int j = 0; j < BN / 2; j += 2)
+                        reinterpret_cast<float4 *>(dst)[j / 2] =
+                            make_float4(lo2(acc[j]), hi2(acc[j]), lo2(acc[j + 1]), hi2(acc[j + 1]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < BN / 2; j += 4) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (p.c_dtype == ST_F16) {
+                                const __half2 h = __floats2half2_rn(lo2(acc[j + i]), hi2(acc[j + i]));
+                                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                            } else {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(lo2(acc[j + i]), hi2(acc[j + i]));
+                                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                            }
+                        }
+                        reinterpret_cast<uint4 *>(dst)[j / 4] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            } else if (!wide) {
+#pragma unroll
+                for (int j = 0; j < BN / 2; ++j) {
+                    put(2 * j, lo2(acc[j]));
+                    put(2 * j + 1, hi2(acc[j]));
+                }
+            }
+        }
+    } else {
+        // every CTA's partial sums into its own ring (all of its MMAs have
+        // read it), [column][row]; then part q adds columns q, q + split, ...
+        // over the parts in order
+        float *mine = reinterpret_cast<float *>(smem);
+        if (warp >= 2) {
+#pragma unroll
+            for (int j = 0; j < BN / 2; ++j) {
+                mine[(2 * j) * kTileRows + row_in_tile] = lo2(acc[j]);
+                mine[(2 * j + 1) * kTileRows + row_in_tile] = hi2(acc[j]);
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 2) {
+            uint32_t part_addr[8];
+            for (int q = 0; q < 8; ++q) part_addr[q] = q < split ? map_to_rank(smem_addr(smem), q) : 0;
+            for (int j = part; j < BN; j += split) {
+                float v = 0.0f;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q < split) v += ld_cluster_f32(part_addr[q] + 4u * (j * kTileRows + row_in_tile));
+                put(j, v);
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // the others have read this CTA's part
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    }
+}
+
+// Dense copy of a strided 8-bit [rows, cols] matrix, rows of `ld` bytes (a
+// multiple of 16; the padding is not written).  Unit column stride: 16 bytes
+// a thread, put together from the aligned words that hold them.
+__global__ void __launch_bounds__(256) repack_8_kernel(const uint8_t *__restrict__ src, int64_t s0, int64_t s1,
+                                                       int64_t rows, int64_t cols, uint8_t *__restrict__ dst, int64_t ld) {
+    pdl_wait();
+    const int64_t per_row = ld / 16, total = rows * per_row;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / per_row, c = (i - r * per_row) * 16;
+        const int n = cols - c < 16 ? static_cast<int>(cols - c) : 16;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (s1 == 1) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(src + r * s0 + c);
+            const uint32_t *words = reinterpret_cast<const uint32_t *>(at & ~uintptr_t(3));
+            const int shift = static_cast<int>(at & 3) * 8, have = (static_cast<int>(at & 3) + n + 3) / 4;
+            uint32_t x[5];
+#pragma unroll
+            for (int j = 0; j < 5; ++j) x[j] = j < have ? words[j] : 0u;  // only words with a byte of the row
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(x[j], x[j + 1], shift);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (j < n) w[j / 4] |= static_cast<uint32_t>(src[r * s0 + (c + j) * s1]) << (8 * (j % 4));
+        }
+        *reinterpret_cast<uint4 *>(dst + r * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    pdl_trigger();
+}
+
+__global__ void __launch_bounds__(256) fill_bias_kernel(void *c, int64_t ldc, int c_dtype, const void *bias,
+                                                        int bias_dtype, int64_t m, int64_t n) {
+    pdl_wait();
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < m * n;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / n, q = i - r * n;
+        store_any(c, c_dtype, r * ldc + q, bias ? load_any(bias, bias_dtype, q) : 0.0f);
+    }
+    pdl_trigger();
+}
+
+// ---------------------------------------------------------------- host side
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
+}
+
+// 128-byte-swizzled box of 128 bytes x `box_rows` of a byte matrix whose rows are `ld` bytes apart
+int make_map_8(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld, int box_rows) {
+    auto fn = encode_fn();
+    if (!fn) return fail(ST_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+    cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(ST_ERR_INVALID_ARGUMENT, "cuTensorMapEncodeTiled rejected an 8-bit operand (error " +
+                                                 std::to_string(static_cast<int>(r)) + ")");
+    return ST_OK;
+}
+
+template <int BN, bool R_MN, bool C_MN, bool CVEC>
+int launch_instance(const CUtensorMap &mr, const CUtensorMap &mc, const Fp8Params &p, cudaStream_t stream) {
+    using Cfg = Fp8Cfg<BN>;
+    auto kern = gemm_fp8_kernel<BN, R_MN, C_MN, CVEC>;
+    static uint64_t attr_set = 0;  // one bit per device ordinal
+    int dev = 0;
+    ST_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !(attr_set & (1ull << dev))) {
+        ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
+        if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.tiles_r) * p.tiles_c * p.split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (p.split > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = static_cast<unsigned>(p.split);
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    ST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mr, mc, p));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "gemm_fp8_kernel launch");
+}
+
+template <int BN>
+int launch_narrow(const CUtensorMap &mr, const CUtensorMap &mc, const Fp8Params &p, bool r_mn, cudaStream_t stream) {
+    return r_mn ? launch_instance<BN, true, false, true>(mr, mc, p, stream)
+                : launch_instance<BN, false, false, true>(mr, mc, p, stream);
+}
+
+template <bool CVEC>
+int launch_wide(const CUtensorMap &mr, const CUtensorMap &mc, const Fp8Params &p, bool r_mn, bool c_mn,
+                cudaStream_t stream) {
+    if (r_mn)
+        return c_mn ? launch_instance<128, true, true, CVEC>(mr, mc, p, stream)
+                    : launch_instance<128, true, false, CVEC>(mr, mc, p, stream);
+    return c_mn ? launch_instance<128, false, true, CVEC>(mr, mc, p, stream)
+                : launch_instance<128, false, false, CVEC>(mr, mc, p, stream);
+}
+
+// How TMA can read a [rows, k] operand: directly along K or along its rows,
+// or after a copy (the strides 0 of a broadcast among the copies).
+struct Access {
+    bool mn;     // rows contiguous
+    bool copy;   // through the workspace
+    int64_t ld;  // bytes between rows (K-major) or between K indices (mn)
+};
+
+Access access_of(const Fp8Operand &o) {
+    const bool base = (reinterpret_cast<uintptr_t>(o.data) & 15u) == 0;
+    auto fits = [&](int64_t unit, int64_t unit_extent, int64_t ld, int64_t outer) {
+        return base && (unit == 1 || unit_extent == 1) &&
+               (outer == 1 || (ld > 0 && ld % 16 == 0 && ld < (int64_t(1) << 40)));
+    };
+    auto stride = [](int64_t ld, int64_t outer, int64_t extent) { return outer == 1 ? (extent + 15) / 16 * 16 : ld; };
+    if (fits(o.s_k, o.k, o.s_row, o.rows)) return {false, false, stride(o.s_row, o.rows, o.k)};
+    if (fits(o.s_row, o.rows, o.s_k, o.k)) return {true, false, stride(o.s_k, o.k, o.rows)};
+    const bool mn = o.s_row == 1 && o.s_k != 1;
+    return {mn, true, ((mn ? o.rows : o.k) + 15) / 16 * 16};
+}
+
+int64_t copy_bytes(const Fp8Operand &o, const Access &a) {
+    return a.copy ? ((a.mn ? o.k : o.rows) * a.ld + 255) / 256 * 256 : 0;
+}
+
+int launch_repack_8(const Fp8Operand &o, const Access &a, uint8_t *dst, int sm_count, cudaStream_t stream) {
+    const int64_t outer = a.mn ? o.k : o.rows, inner = a.mn ? o.rows : o.k;
+    const int64_t s0 = a.mn ? o.s_k : o.s_row, s1 = a.mn ? o.s_row : o.s_k;
+    int64_t grid = cdiv(outer * (a.ld / 16), 256);
+    if (grid > static_cast<int64_t>(sm_count) * 8) grid = static_cast<int64_t>(sm_count) * 8;
+    ST_CUDA_TRY(launch_kernel(repack_8_kernel, static_cast<unsigned>(grid), 256, 0, stream,
+                              static_cast<const uint8_t *>(o.data), s0, inner == 1 ? int64_t(1) : s1, outer, inner, dst, a.ld));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "repack_8_kernel");
+}
+
+}  // namespace
+
+int64_t gemm_fp8_workspace_bytes(const Fp8Operand &a, const Fp8Operand &b) {
+    if (a.rows == 0 || b.rows == 0 || a.k == 0) return 0;
+    return copy_bytes(a, access_of(a)) + copy_bytes(b, access_of(b));
+}
+
+int launch_gemm_fp8(const GemmFp8Args &g, void *workspace, int sm_count, int *dev_err, uint64_t timeout_ns,
+                    cudaStream_t stream) {
+    const int64_t m = g.a.rows, n = g.b.rows, k = g.a.k;
+    if (m == 0 || n == 0) return ST_OK;
+    if (k == 0) {
+        ST_CUDA_TRY(launch_kernel(fill_bias_kernel, static_cast<unsigned>(sm_count), 256, 0, stream, g.c, g.ldc,
+                                  g.c_dtype, g.bias, g.bias_dtype, m, n));
+        note_launch();
+        const cudaError_t e = cudaPeekAtLastError();
+        return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "fill_bias_kernel");
+    }
+    Fp8Operand op[2] = {g.a, g.b};
+    Access acc[2] = {access_of(g.a), access_of(g.b)};
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    for (int i = 0; i < 2; ++i) {
+        if (!acc[i].copy) continue;
+        ST_TRY(launch_repack_8(op[i], acc[i], ws, sm_count, stream));
+        op[i].data = ws;
+        ws += copy_bytes(op[i], acc[i]);
+    }
+    // The smaller of M and N becomes the column operand where a tile of up
+    // to 64 columns covers it; its boxes are K-major.
+    const bool swap = m <= 64 && m <= n && !acc[0].mn;
+    const int ri = swap ? 1 : 0, ci = swap ? 0 : 1;
+    const Fp8Operand &r = op[ri], &c = op[ci];
+    int bn = 128;
+    if (!acc[ci].mn) bn = c.rows <= 16 ? 16 : c.rows <= 32 ? 32 : c.rows <= 64 ? 64 : 128;
+    Fp8Params p{};
+    p.rows = static_cast<int>(r.rows);
+    p.cols = static_cast<int>(c.rows);
+    p.k_blocks = static_cast<int>(cdiv(k, kBlockK));
+    p.tiles_r = static_cast<int>(cdiv(r.rows, kTileRows));
+    p.tiles_c = static_cast<int>(cdiv(c.rows, bn));
+    const int64_t tiles = static_cast<int64_t>(p.tiles_r) * p.tiles_c;
+    const int64_t slots = static_cast<int64_t>(sm_count) * (bn == 128 ? 1 : 2);
+    p.split = 1;
+    while (p.split < 8 && tiles * p.split * 2 <= slots && p.k_blocks >= p.split * 2 * 2) p.split *= 2;
+    if (tiles * p.split > INT32_MAX) return fail(ST_ERR_UNSUPPORTED, "matmul_fp8: too many output tiles");
+    p.rs = static_cast<const float *>(r.scale);
+    p.rs_i = r.scale_row;
+    p.rs_b = r.scale_k;
+    p.rs_shift = r.scale_shift;
+    p.cs = static_cast<const float *>(c.scale);
+    p.cs_i = c.scale_row;
+    p.cs_b = c.scale_k;
+    p.cs_shift = c.scale_shift;
+    p.c = g.c;
+    p.c_r = swap ? 1 : g.ldc;
+    p.c_c = swap ? g.ldc : 1;
+    p.c_dtype = g.c_dtype;
+    p.bias = g.bias;
+    p.bias_dtype = g.bias_dtype;
+    p.bias_on_rows = swap;
+    p.idesc = mma_idesc_f8(r.e5m2, c.e5m2, acc[ri].mn, acc[ci].mn, kTileRows, static_cast<uint32_t>(bn));
+    p.err = dev_err;
+    p.timeout_ns = timeout_ns;
+    CUtensorMap mr, mc;
+    if (acc[ri].mn) ST_TRY(make_map_8(&mr, r.data, r.rows, k, acc[ri].ld, kBlockK));
+    else ST_TRY(make_map_8(&mr, r.data, k, r.rows, acc[ri].ld, kTileRows));
+    if (acc[ci].mn) ST_TRY(make_map_8(&mc, c.data, c.rows, k, acc[ci].ld, kBlockK));
+    else ST_TRY(make_map_8(&mc, c.data, k, c.rows, acc[ci].ld, bn));
+    switch (bn) {
+    case 16: return launch_narrow<16>(mr, mc, p, acc[ri].mn, stream);
+    case 32: return launch_narrow<32>(mr, mc, p, acc[ri].mn, stream);
+    case 64: return launch_narrow<64>(mr, mc, p, acc[ri].mn, stream);
+    default: break;
+    }
+    return p.cs_shift == 7 ? launch_wide<false>(mr, mc, p, acc[ri].mn, acc[ci].mn, stream)
+                           : launch_wide<true>(mr, mc, p, acc[ri].mn, acc[ci].mn, stream);
+}
+
+}  // namespace st

@@ -1,0 +1,646 @@
+// norm.cu -- the norms after and before a block, fused with the block's gate
+// and residual scale, forward and backward.
+//
+//   u  = x * rsqrt(mean(x^2) + eps) * (post + offset)      (u = x without post)
+//   r' = r + alpha * gate * u
+//   h  = r' * rsqrt(mean(r'^2) + eps) * (pre + offset)     (as 8-bit blocks of 128 if asked)
+//
+// One pass: a row of x and r is read once into registers, both means are
+// reduced over the row's warps, r' and h are written once.  h comes from r'
+// before its rounding to the stream's type.
+//
+// The way back takes r' and x, not the forward call's statistics: their sums
+// come with the same read.  With t = dh * (pre + offset), R = r' * inv_r:
+//
+//   dpre  = sum_rows dh * R
+//   dr    = dr' + inv_r * (t - R * mean(t * R))
+//   du    = alpha * gate * dr,  dgate = alpha * dr * u (summed over what the gate was broadcast over)
+//   dx    = the same with x, post and du in the place of r', pre and dh;  dpost likewise
+//
+// The sums over rows are kept in registers by a fixed set of row groups, each
+// taking every G-th row, written once to a workspace and added in a fixed
+// order by a second launch: no atomics, the same bits on every run.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "common.h"
+#include "fp8.cuh"
+
+namespace st {
+namespace {
+
+constexpr int kChunk = 256;     // elements of a row that a warp takes at a time, 8 a lane
+constexpr int kRowsPerCta = 4;  // rows (warps) of a CTA when a warp covers a row
+constexpr int kMaxThreads = 512;  // 128 registers a thread
+constexpr int64_t kMaxCols = 4 * kMaxThreads * 8;
+
+// Where a lane's 8 elements of a chunk lie.  VEC: next to each other;
+// otherwise 32 apart, so that a warp's scalar loads are contiguous.
+template <bool VEC>
+__device__ __forceinline__ int64_t element(int64_t base, int lane, int j) {
+    return VEC ? base + lane * 8 + j : base + lane + 32 * j;
+}
+
+// 8 elements as stored.
+template <typename T>
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ float operator[](int j) const { return to_float(reinterpret_cast<const T *>(w)[j]); }
+};
+
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw8<T> load_raw(const NormView &view, int64_t r, int64_t base, int lane, int64_t cols) {
+    Raw8<T> out;
+    const T *row = static_cast<const T *>(view.p) + r * view.ld;
+    if (VEC && base + lane * 8 + 8 <= cols) {
+        const uint4 *src = reinterpret_cast<const uint4 *>(row + base + lane * 8);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) out.w[i] = src[i];
+    } else {
+        T *e = reinterpret_cast<T *>(out.w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t c = element<VEC>(base, lane, j);
+            if (c < cols) e[j] = row[c];
+            else from_float(0.0f, e[j]);
+        }
+    }
+    return out;
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T *row, int64_t base, int lane, int64_t cols, float (&f)[8]) {
+    if (VEC && base + lane * 8 + 8 <= cols) {
+        uint4 w[sizeof(T) / 2];
+        const uint4 *src = reinterpret_cast<const uint4 *>(row + base + lane * 8);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = src[i];
+        const T *e = reinterpret_cast<const T *>(w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = to_float(e[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t c = element<VEC>(base, lane, j);
+            f[j] = c < cols ? to_float(row[c]) : 0.0f;
+        }
+    }
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T *row, int64_t base, int lane, int64_t cols, const float (&f)[8]) {
+    if (VEC && base + lane * 8 + 8 <= cols) {
+        uint4 w[sizeof(T) / 2];
+        T *e = reinterpret_cast<T *>(w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) from_float(f[j], e[j]);
+        uint4 *dst = reinterpret_cast<uint4 *>(row + base + lane * 8);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) dst[i] = w[i];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t c = element<VEC>(base, lane, j);
+            if (c < cols) from_float(f[j], row[c]);
+        }
+    }
+}
+
+// A weight or gate of type T or fp32.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8_of(const NormView &v, int64_t row, int64_t base, int lane, int64_t cols,
+                                         float (&f)[8]) {
+    if (v.dtype == ST_F32) load8<float, VEC>(static_cast<const float *>(v.p) + row * v.ld, base, lane, cols, f);
+    else load8<T, VEC>(static_cast<const T *>(v.p) + row * v.ld, base, lane, cols, f);
+}
+
+template <typename T>
+__device__ __forceinline__ float load1_of(const NormView &v, int64_t row) {
+    if (v.dtype == ST_F32) return static_cast<const float *>(v.p)[row * v.ld];
+    return to_float(static_cast<const T *>(v.p)[row * v.ld]);
+}
+
+// Sums of N values over the warps of a row.  `slot` alternates between two
+// buffers, so that one barrier a call is enough.
+template <int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int warps, int warp, int lane, float *slots, int &slot) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if (warps == 1) return;
+    float *s = slots + slot * 3 * 32;
+    slot ^= 1;
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i * 32 + warp] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = lane < warps ? s[i * 32 + lane] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+}
+
+// One row: the warps of the CTA (warps > 1), or one warp of it.
+struct RowGroup {
+    int warps, warp, lane;
+    int64_t first, step;
+    __device__ __forceinline__ RowGroup(int warps_) : warps(warps_), lane(threadIdx.x & 31) {
+        const int w = threadIdx.x >> 5;
+        const int per_cta = warps == 1 ? static_cast<int>(blockDim.x >> 5) : 1;
+        warp = warps == 1 ? 0 : w;
+        first = static_cast<int64_t>(blockIdx.x) * per_cta + (warps == 1 ? w : 0);
+        step = static_cast<int64_t>(gridDim.x) * per_cta;
+    }
+    __device__ __forceinline__ int64_t base(int v) const { return static_cast<int64_t>(v * warps + warp) * kChunk; }
+};
+
+template <typename TX, typename TR, int VPT, bool VEC>
+__global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormArgs p, int warps) {
+    pdl_wait();
+    __shared__ float slots[2 * 3 * 32];
+    const RowGroup g(warps);
+    const float inv_cols = 1.0f / static_cast<float>(p.cols);
+    int slot = 0;
+    for (int64_t row = g.first; row < p.rows; row += g.step) {
+        float r[VPT][8];
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+            load8<TR, VEC>(static_cast<const TR *>(p.r.p) + row * p.r.ld, g.base(v), g.lane, p.cols, r[v]);
+        if (p.x.p != nullptr) {
+            float x[VPT][8];
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+                load8<TX, VEC>(static_cast<const TX *>(p.x.p) + row * p.x.ld, g.base(v), g.lane, p.cols, x[v]);
+            if (p.post.p != nullptr) {
+                float s[1] = {0.0f};
+#pragma unroll
+                for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) s[0] += x[v][j] * x[v][j];
+                row_sum(s, g.warps, g.warp, g.lane, slots, slot);
+                const float inv = 1.0f / sqrtf(s[0] * inv_cols + p.eps);
+#pragma unroll
+                for (int v = 0; v < VPT; ++v) {
+                    float w[8];
+                    load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[v][j] *= inv * (w[j] + p.offset);
+                }
+            }
+            float token = p.alpha;
+            if (p.gate_mode == kGateToken) token *= load1_of<TX>(p.gate, row);
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                if (p.gate_mode == kGateChannel || p.gate_mode == kGateFull) {
+                    float w[8];
+                    load8_of<TX, VEC>(p.gate, p.gate_mode == kGateFull ? row : 0, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[v][j] *= w[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[v][j] += token * x[v][j];
+            }
+        }
+        if (p.r_out.p != nullptr) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+                store8<TR, VEC>(static_cast<TR *>(p.r_out.p) + row * p.r_out.ld, g.base(v), g.lane, p.cols, r[v]);
+        }
+        if (p.pre.p == nullptr) continue;
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[0] += r[v][j] * r[v][j];
+        row_sum(s, g.warps, g.warp, g.lane, slots, slot);
+        const float inv = 1.0f / sqrtf(s[0] * inv_cols + p.eps);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int64_t base = g.base(v);
+            float w[8];
+            load8_of<TX, VEC>(p.pre, 0, base, g.lane, p.cols, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[v][j] *= inv * (w[j] + p.offset);
+            if (!p.h_fp8) {
+                store8<TX, VEC>(static_cast<TX *>(p.h.p) + row * p.h.ld, base, g.lane, p.cols, r[v]);
+                continue;
+            }
+            // a chunk is two blocks of 128: VEC, 16 lanes each; otherwise the lanes' first and last four elements
+            const float limit = p.h_e5m2 ? 57344.0f : 448.0f;
+            uint32_t m[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m[VEC ? 0 : j / 4] = max(m[VEC ? 0 : j / 4], abs_bits(r[v][j]));
+            float inverse[2];
+#pragma unroll
+            for (int b = 0; b < (VEC ? 1 : 2); ++b) {
+#pragma unroll
+                for (int o = VEC ? 8 : 16; o > 0; o >>= 1) m[b] = max(m[b], __shfl_xor_sync(0xffffffffu, m[b], o));
+                const float scale = fp8_scale(m[b], limit);
+                inverse[b] = __fdiv_rn(1.0f, scale);
+                const int64_t block = base / 128 + (VEC ? g.lane / 16 : b);
+                if ((VEC ? g.lane % 16 : g.lane) == 0 && block * 128 < p.cols)
+                    p.h_scale[row * p.hs0 + block * p.hs1] = scale;
+            }
+            if constexpr (VEC) inverse[1] = inverse[0];
+            uint32_t q[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+                q[b] = to_fp8x4(__fmul_rn(r[v][4 * b], inverse[b]), __fmul_rn(r[v][4 * b + 1], inverse[b]),
+                                __fmul_rn(r[v][4 * b + 2], inverse[b]), __fmul_rn(r[v][4 * b + 3], inverse[b]), p.h_e5m2);
+            uint8_t *h = static_cast<uint8_t *>(p.h.p) + row * p.h.ld;
+            if (VEC && base + g.lane * 8 + 8 <= p.cols) {
+                *reinterpret_cast<uint2 *>(h + base + g.lane * 8) = make_uint2(q[0], q[1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t c = element<VEC>(base, g.lane, j);
+                    if (c < p.cols) h[c] = static_cast<uint8_t>(q[j / 4] >> (8 * (j % 4)));
+                }
+            }
+        }
+    }
+    pdl_trigger();
+}
+
+// The sums over a group's rows, in shared memory: thread t's 8 elements of
+// (plane, v) are two float4 at [plane][v][half][t], its own and free of bank
+// conflicts.  The traffic is 8 bytes an element and plane beside the 12 of a
+// 16-bit row's six streams, and shared memory moves five times what HBM
+// does; in registers the sums would halve the rows in flight.
+template <int VPT>
+struct Sums {
+    float4 *mine;
+    __device__ __forceinline__ Sums(float4 *smem) : mine(smem + threadIdx.x) {}
+    __device__ __forceinline__ float4 &at(int plane, int v, int half) {
+        return mine[((plane * VPT + v) * 2 + half) * blockDim.x];
+    }
+    __device__ __forceinline__ void add(int plane, int v, const float (&f)[8]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float4 &a = at(plane, v, h);
+            float4 s = a;
+            s.x += f[4 * h];
+            s.y += f[4 * h + 1];
+            s.z += f[4 * h + 2];
+            s.w += f[4 * h + 3];
+            a = s;
+        }
+    }
+};
+
+// planes: which sums are kept, and in what order (-1: not kept).
+struct Planes {
+    int pre, post, gate, count;
+};
+
+// out: [planes.count][groups][cols], one row a group.
+template <typename TX, typename TR, int VPT, bool VEC>
+__global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(const NormBackwardArgs p, int warps,
+                                                                             const Planes planes, float *out) {
+    extern __shared__ float4 sums_smem[];
+    __shared__ float slots[2 * 3 * 32];
+    const RowGroup g(warps);
+    const float inv_cols = 1.0f / static_cast<float>(p.cols);
+    const bool has_x = p.x.p != nullptr, has_post = p.post.p != nullptr, has_pre = p.pre.p != nullptr;
+    int slot = 0;
+    Sums<VPT> sums(sums_smem);
+    for (int i = 0; i < planes.count; ++i)
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) sums.at(i, v, h) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    pdl_wait();
+
+    for (int64_t row = g.first; row < p.rows; row += g.step) {
+        Raw8<TX> x[VPT];
+        float d[VPT][8];  // dr', then dr, then du
+        if (has_x) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) x[v] = load_raw<TX, VEC>(p.x, row, g.base(v), g.lane, p.cols);
+        }
+        Raw8<TR> dres[VPT];
+        if (p.d_residual.p != nullptr) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) dres[v] = load_raw<TR, VEC>(p.d_residual, row, g.base(v), g.lane, p.cols);
+        }
+        float s[3] = {0.0f, 0.0f, 0.0f};
+        if (has_x && has_post) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[2] += x[v][j] * x[v][j];
+        }
+        float inv_x = 1.0f;
+        if (has_pre) {
+            Raw8<TR> r[VPT];
+            Raw8<TX> dh[VPT];
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                r[v] = load_raw<TR, VEC>(p.r, row, g.base(v), g.lane, p.cols);
+                dh[v] = load_raw<TX, VEC>(p.d_normed, row, g.base(v), g.lane, p.cols);
+            }
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                float w[8];
+                load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float rj = r[v][j];
+                    s[0] += rj * rj;
+                    s[1] += rj * (dh[v][j] * (w[j] + p.offset));
+                }
+            }
+            row_sum(s, g.warps, g.warp, g.lane, slots, slot);
+            const float inv = 1.0f / sqrtf(s[0] * inv_cols + p.eps);
+            const float mean = inv * s[1] * inv_cols;  // of t * R
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                float w[8], dw[8];
+                load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float hat = r[v][j] * inv, dhj = dh[v][j];
+                    dw[j] = dhj * hat;
+                    d[v][j] = inv * (dhj * (w[j] + p.offset) - hat * mean);
+                }
+                if (planes.pre >= 0) sums.add(planes.pre, v, dw);
+            }
+        } else {
+            if (has_x && has_post) row_sum(s, g.warps, g.warp, g.lane, slots, slot);
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[v][j] = 0.0f;
+        }
+        if (has_post) inv_x = 1.0f / sqrtf(s[2] * inv_cols + p.eps);
+        if (p.d_residual.p != nullptr) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[v][j] += dres[v][j];
+        }
+        if (p.dr.p != nullptr) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+                store8<TR, VEC>(static_cast<TR *>(p.dr.p) + row * p.dr.ld, g.base(v), g.lane, p.cols, d[v]);
+        }
+        if (!has_x) continue;
+
+        float token = p.alpha;
+        if (p.gate_mode == kGateToken) token *= load1_of<TX>(p.gate, row);
+        // with X = x * inv_x, t = du * (post + offset): sums of t * X and of dgate
+        float e[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            float w[8], gt[8], dw[8], dg[8];
+            if (has_post) {
+                load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] += p.offset;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = 1.0f;
+            }
+            if (p.gate_mode == kGateChannel || p.gate_mode == kGateFull) {
+                load8_of<TX, VEC>(p.gate, p.gate_mode == kGateFull ? row : 0, g.base(v), g.lane, p.cols, gt);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) gt[j] = 1.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float hat = x[v][j] * inv_x;
+                dg[j] = p.alpha * d[v][j] * (hat * w[j]);
+                d[v][j] *= token * gt[j];
+                dw[j] = d[v][j] * hat;
+                e[0] += dw[j] * w[j];
+                e[1] += dg[j];
+            }
+            if (planes.post >= 0) sums.add(planes.post, v, dw);
+            if (planes.gate >= 0) sums.add(planes.gate, v, dg);
+            if (p.gate_mode == kGateFull) {
+                if (p.dgate.dtype == ST_F32)
+                    store8<float, VEC>(static_cast<float *>(p.dgate.p) + row * p.dgate.ld, g.base(v), g.lane, p.cols, dg);
+                else
+                    store8<TX, VEC>(static_cast<TX *>(p.dgate.p) + row * p.dgate.ld, g.base(v), g.lane, p.cols, dg);
+            }
+        }
+        if (has_post || p.gate_mode == kGateToken) row_sum(e, g.warps, g.warp, g.lane, slots, slot);
+        if (p.gate_mode == kGateToken && g.warp == 0 && g.lane == 0)
+            static_cast<float *>(p.dgate.p)[row * p.dgate.ld] = e[1];
+        const float mean = e[0] * inv_cols;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            if (has_post) {
+                float w[8];
+                load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    d[v][j] = inv_x * (d[v][j] * (w[j] + p.offset) - x[v][j] * inv_x * mean);
+            }
+            store8<TX, VEC>(static_cast<TX *>(p.dx.p) + row * p.dx.ld, g.base(v), g.lane, p.cols, d[v]);
+        }
+    }
+
+    for (int i = 0; i < planes.count; ++i) {
+        float *to = out + (i * g.step + g.first) * p.cols;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const float4 a = sums.at(i, v, 0), b = sums.at(i, v, 1);
+            const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            store8<float, VEC>(to, g.base(v), g.lane, p.cols, f);
+        }
+    }
+    pdl_trigger();
+}
+
+// out[c] = sum over groups of sums[g][c], in a fixed order; blockIdx.y picks the plane.
+__global__ void __launch_bounds__(256) column_sums_kernel(const float *sums, int64_t groups, int64_t cols, float *out0,
+                                                          float *out1, float *out2) {
+    pdl_wait();
+    float *out = blockIdx.y == 0 ? out0 : blockIdx.y == 1 ? out1 : out2;
+    __shared__ float part[8][33];
+    {
+        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+        const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
+        const float *src = sums + blockIdx.y * groups * cols + c;
+        float s = 0.0f;
+        if (c < cols)
+            for (int64_t i = ty; i < groups; i += 8) s += src[i * cols];
+        part[ty][tx] = s;
+        __syncthreads();
+        if (ty == 0 && c < cols) {
+#pragma unroll
+            for (int i = 1; i < 8; ++i) s += part[i][tx];
+            out[c] = s;
+        }
+    }
+    pdl_trigger();
+}
+
+// Row groups of the backward kernel: each leaves one row of partial sums.
+int64_t backward_groups(int64_t rows, int64_t cols) {
+    const int64_t most = cols <= 2 * kChunk ? 148 * 16 : 148 * 2;
+    return rows < most ? rows : most;
+}
+
+bool aligned_rows(const NormView &v, int64_t rows, size_t size, size_t to) {
+    if (v.p == nullptr) return true;
+    return reinterpret_cast<uintptr_t>(v.p) % to == 0 && (rows == 1 || v.ld * static_cast<int64_t>(size) % to == 0);
+}
+
+struct Shape {
+    int vpt, warps, ctas, threads;
+};
+
+// `rows` rows of `cols` on up to `most` row groups.
+Shape shape_of(int64_t rows, int64_t cols, int64_t most, bool latency) {
+    Shape s;
+    const int64_t chunks = cdiv(cols, kChunk);
+    if (chunks <= 2) {
+        s.vpt = static_cast<int>(chunks);
+    } else {
+        s.vpt = latency && chunks <= 16 ? 1 : chunks <= 32 ? 2 : 4;
+    }
+    s.warps = static_cast<int>(cdiv(chunks, s.vpt));
+    const int64_t groups = rows < most ? rows : most;
+    if (s.warps == 1) {
+        s.threads = 32 * kRowsPerCta;
+        s.ctas = static_cast<int>(cdiv(groups, kRowsPerCta));
+    } else {
+        s.threads = 32 * s.warps;
+        s.ctas = static_cast<int>(groups);
+    }
+    return s;
+}
+
+template <typename TX, typename TR, int VPT>
+int forward_vpt(const NormArgs &p, const Shape &s, bool vec, cudaStream_t stream) {
+    if (vec)
+        ST_CUDA_TRY(launch_kernel(residual_norm_kernel<TX, TR, VPT, true>, s.ctas, s.threads, 0, stream, p, s.warps));
+    else
+        ST_CUDA_TRY(launch_kernel(residual_norm_kernel<TX, TR, VPT, false>, s.ctas, s.threads, 0, stream, p, s.warps));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "residual_norm_kernel");
+}
+
+template <typename TX, typename TR>
+int forward_typed(const NormArgs &p, int sm_count, cudaStream_t stream) {
+    auto side = [](const NormView &v) { return v.dtype == ST_F32 ? sizeof(float) : sizeof(TX); };
+    const bool vec = aligned_rows(p.x, p.rows, sizeof(TX), 16) && aligned_rows(p.r, p.rows, sizeof(TR), 16) &&
+                     aligned_rows(p.r_out, p.rows, sizeof(TR), 16) &&
+                     (p.h_fp8 ? aligned_rows(p.h, p.rows, 1, 8) : aligned_rows(p.h, p.rows, sizeof(TX), 16)) &&
+                     aligned_rows(p.post, 1, side(p.post), 16) && aligned_rows(p.pre, 1, side(p.pre), 16) &&
+                     (p.gate_mode == kGateToken ||
+                      aligned_rows(p.gate, p.gate_mode == kGateFull ? p.rows : 1, side(p.gate), 16));
+    const Shape s = shape_of(p.rows, p.cols, int64_t(1) << 30, p.rows < sm_count);
+    if (s.vpt == 1) return forward_vpt<TX, TR, 1>(p, s, vec, stream);
+    if (s.vpt == 2) return forward_vpt<TX, TR, 2>(p, s, vec, stream);
+    return forward_vpt<TX, TR, 4>(p, s, vec, stream);
+}
+
+template <typename TX, typename TR, int VPT, bool VEC>
+int backward_launch(const NormBackwardArgs &p, const Shape &s, const Planes &planes, float *sums, cudaStream_t stream) {
+    auto kern = residual_norm_backward_kernel<TX, TR, VPT, VEC>;
+    static uint64_t attr_set = 0;  // one bit per device ordinal
+    int dev = 0;
+    ST_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !(attr_set & (1ull << dev))) {
+        ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         3 * VPT * 8 * kMaxThreads * static_cast<int>(sizeof(float))));
+        if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
+    }
+    const size_t smem = static_cast<size_t>(planes.count) * VPT * 8 * s.threads * sizeof(float);
+    ST_CUDA_TRY(launch_kernel(kern, s.ctas, s.threads, smem, stream, p, s.warps, planes, sums));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "residual_norm_backward_kernel");
+}
+
+template <typename TX, typename TR, int VPT>
+int backward_vpt(const NormBackwardArgs &p, const Shape &s, bool vec, const Planes &planes, float *sums,
+                 cudaStream_t stream) {
+    return vec ? backward_launch<TX, TR, VPT, true>(p, s, planes, sums, stream)
+               : backward_launch<TX, TR, VPT, false>(p, s, planes, sums, stream);
+}
+
+template <typename TX, typename TR>
+int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) {
+    auto side = [](const NormView &v) { return v.dtype == ST_F32 ? sizeof(float) : sizeof(TX); };
+    const bool vec =
+        aligned_rows(p.d_residual, p.rows, sizeof(TR), 16) && aligned_rows(p.d_normed, p.rows, sizeof(TX), 16) &&
+        aligned_rows(p.x, p.rows, sizeof(TX), 16) && aligned_rows(p.r, p.rows, sizeof(TR), 16) &&
+        aligned_rows(p.dx, p.rows, sizeof(TX), 16) && aligned_rows(p.dr, p.rows, sizeof(TR), 16) &&
+        aligned_rows(p.post, 1, side(p.post), 16) && aligned_rows(p.pre, 1, side(p.pre), 16) &&
+        (p.gate_mode == kGateToken || p.gate_mode == kGateNone ||
+         aligned_rows(p.gate, p.gate_mode == kGateFull ? p.rows : 1, side(p.gate), 16)) &&
+        (p.gate_mode != kGateFull || aligned_rows(p.dgate, p.rows, side(p.dgate), 16)) && p.cols % 4 == 0;
+    Shape s = shape_of(p.rows, p.cols, backward_groups(p.rows, p.cols), false);
+    const int64_t groups = s.warps == 1 ? static_cast<int64_t>(s.ctas) * kRowsPerCta : s.ctas;
+    Planes planes{-1, -1, -1, 0};
+    float *dst[3] = {nullptr, nullptr, nullptr};
+    auto keep = [&](int &plane, float *to) {
+        if (to == nullptr) return;
+        plane = planes.count;
+        dst[planes.count++] = to;
+    };
+    keep(planes.pre, p.dpre);
+    keep(planes.post, p.dpost);
+    if (p.gate_mode == kGateChannel) keep(planes.gate, static_cast<float *>(p.dgate.p));
+    if (s.vpt == 1) ST_TRY((backward_vpt<TX, TR, 1>(p, s, vec, planes, sums, stream)));
+    else if (s.vpt == 2) ST_TRY((backward_vpt<TX, TR, 2>(p, s, vec, planes, sums, stream)));
+    else ST_TRY((backward_vpt<TX, TR, 4>(p, s, vec, planes, sums, stream)));
+    if (planes.count == 0) return ST_OK;
+    ST_CUDA_TRY(launch_kernel(column_sums_kernel,
+                              dim3(static_cast<unsigned>(cdiv(p.cols, 32)), static_cast<unsigned>(planes.count)), 256, 0,
+                              stream, sums, groups, p.cols, dst[0], dst[1], dst[2]));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "column_sums_kernel");
+}
+
+}  // namespace
+
+int launch_residual_norm(const NormArgs &p, int sm_count, cudaStream_t stream) {
+    if (p.rows == 0) return ST_OK;
+    if (p.cols > kMaxCols) return fail(ST_ERR_UNSUPPORTED, "residual_norm: at most 16384 columns");
+    const int tx = p.x.p != nullptr ? p.x.dtype : (p.h.p != nullptr && !p.h_fp8 ? p.h.dtype : p.r.dtype);
+    const bool wide = p.r.dtype == ST_F32;
+    if (tx == ST_F32) return forward_typed<float, float>(p, sm_count, stream);
+    if (tx == ST_F16)
+        return wide ? forward_typed<__half, float>(p, sm_count, stream) : forward_typed<__half, __half>(p, sm_count, stream);
+    return wide ? forward_typed<__nv_bfloat16, float>(p, sm_count, stream)
+                : forward_typed<__nv_bfloat16, __nv_bfloat16>(p, sm_count, stream);
+}
+
+int64_t residual_norm_backward_workspace(int64_t rows, int64_t cols) {
+    // a CTA of single-warp rows may hold up to three groups without a row
+    const int64_t groups = cdiv(backward_groups(rows, cols), kRowsPerCta) * kRowsPerCta;
+    return 3 * groups * cols * static_cast<int64_t>(sizeof(float));
+}
+
+int launch_residual_norm_backward(const NormBackwardArgs &p, void *workspace, int sm_count, cudaStream_t stream) {
+    (void)sm_count;
+    if (p.cols > kMaxCols) return fail(ST_ERR_UNSUPPORTED, "residual_norm_backward: at most 16384 columns");
+    float *sums = static_cast<float *>(workspace);
+    if (p.rows == 0) {  // the sums over no rows
+        float *dgate = p.gate_mode == kGateChannel ? static_cast<float *>(p.dgate.p) : nullptr;
+        for (float *out : {p.dpre, p.dpost, dgate})
+            if (out != nullptr) ST_CUDA_TRY(cudaMemsetAsync(out, 0, p.cols * sizeof(float), stream));
+        return ST_OK;
+    }
+    const int tx = p.x.p != nullptr ? p.x.dtype : (p.d_normed.p != nullptr ? p.d_normed.dtype : p.r.dtype);
+    const bool wide = (p.r.p != nullptr ? p.r.dtype : p.d_residual.dtype) == ST_F32;
+    if (tx == ST_F32) return backward_typed<float, float>(p, sums, stream);
+    if (tx == ST_F16)
+        return wide ? backward_typed<__half, float>(p, sums, stream) : backward_typed<__half, __half>(p, sums, stream);
+    return wide ? backward_typed<__nv_bfloat16, float>(p, sums, stream)
+                : backward_typed<__nv_bfloat16, __nv_bfloat16>(p, sums, stream);
+}
+
+}  // namespace st

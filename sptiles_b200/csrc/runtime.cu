@@ -15,11 +15,14 @@
 #include <algorithm>
 #include <atomic>
 #include <chrono>
+#include <cmath>
 #include <cstdint>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <string>
 #include <thread>
+#include <utility>
 #include <vector>
 
 #include "common.h"
@@ -873,6 +876,156 @@ int matmul_host_split(st_ctx *ctx, const ExecCtx &x, const st_tensor &a, const s
     });
 }
 
+// ------------------------------------------------------------ 8-bit blocks and norms
+constexpr int64_t kScaleBlock = 128;
+
+int check_matrix(const st_tensor *t, const char *name) {
+    if (!t) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " is null");
+    if (t->rank != 2)
+        return fail(ST_ERR_INVALID_ARGUMENT,
+                    std::string(name) + " must be rank 2, got " + std::to_string(t->rank));
+    for (int i = 0; i < 2; ++i) {
+        if (t->shape[i] < 0) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " has a negative extent");
+        if (t->strides[i] < 0) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " has a negative stride");
+        if (t->shape[i] > INT32_MAX) return fail(ST_ERR_UNSUPPORTED, std::string(name) + ": extents must fit in int32");
+    }
+    if (t->shape[0] > 0 && t->shape[1] > 0 && !t->data)
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " has a null data pointer");
+    return ST_OK;
+}
+
+// An output: no two of its elements may share an address.
+int check_output(const st_tensor &t, const char *name) {
+    const int64_t a = t.shape[0], b = t.shape[1], sa = t.strides[0], sb = t.strides[1];
+    if (a == 0 || b == 0) return ST_OK;
+    const bool ok = (a == 1 && b == 1) || (a == 1 && sb >= 1) || (b == 1 && sa >= 1) ||
+                    (sb >= 1 && sa >= (b - 1) * sb + 1) || (sa >= 1 && sb >= (a - 1) * sa + 1);
+    return ok ? ST_OK : fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " has overlapping elements");
+}
+
+bool is_fp8(int dtype) { return dtype == ST_E4M3 || dtype == ST_E5M2; }
+bool is_float(int dtype) { return dtype == ST_F32 || dtype == ST_F16 || dtype == ST_BF16; }
+// element (0, 1) of a row lies next to (0, 0)
+bool unit_columns(const st_tensor &t) { return t.shape[1] <= 1 || t.strides[1] == 1; }
+
+int check_fp8_operands(const st_tensor *a, const st_tensor *b) {
+    ST_TRY(check_matrix(a, "A"));
+    ST_TRY(check_matrix(b, "B"));
+    if (!is_fp8(a->dtype) || !is_fp8(b->dtype))
+        return fail(ST_ERR_INVALID_ARGUMENT, "matmul_fp8: A and B must be ST_E4M3 or ST_E5M2");
+    if (a->shape[1] != b->shape[0])
+        return fail(ST_ERR_INVALID_ARGUMENT, "Incompatible matrices: K dimension of A (" + std::to_string(a->shape[1]) +
+                                                 ") must match K dimension of B (" + std::to_string(b->shape[0]) + ")");
+    return ST_OK;
+}
+
+Fp8Operand fp8_operand(const st_tensor &t, bool is_b) {
+    Fp8Operand o{};
+    o.data = t.data;
+    o.rows = t.shape[is_b ? 1 : 0];
+    o.k = t.shape[is_b ? 0 : 1];
+    o.s_row = t.strides[is_b ? 1 : 0];
+    o.s_k = t.strides[is_b ? 0 : 1];
+    o.e5m2 = t.dtype == ST_E5M2 ? 1 : 0;
+    return o;
+}
+
+// Scales of an operand: [rows or their blocks of 128, K blocks] for A, the transpose for B.
+int set_scale(const st_tensor *t, const char *name, bool is_b, Fp8Operand *o) {
+    ST_TRY(check_matrix(t, name));
+    if (t->dtype != ST_F32) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be ST_F32");
+    const int ri = is_b ? 1 : 0;
+    const int64_t rows = t->shape[ri], blocks = t->shape[1 - ri];
+    if (blocks != cdiv(o->k, kScaleBlock) || (rows != o->rows && rows != cdiv(o->rows, kScaleBlock)))
+        return fail(ST_ERR_INVALID_ARGUMENT,
+                    std::string(name) + " must have one scale for each 128 elements along K (" +
+                        std::to_string(cdiv(o->k, kScaleBlock)) + ") and for each " + (is_b ? "column (" : "row (") +
+                        std::to_string(o->rows) + ") or 128 of them (" + std::to_string(cdiv(o->rows, kScaleBlock)) +
+                        "), got [" + std::to_string(t->shape[0]) + ", " + std::to_string(t->shape[1]) + "]");
+    o->scale = t->data;
+    o->scale_row = t->strides[ri];
+    o->scale_k = t->strides[1 - ri];
+    o->scale_shift = rows == o->rows ? 0 : 7;
+    return ST_OK;
+}
+
+// A tensor of the norms: [rows, cols] with unit column stride.
+int norm_view(const st_tensor *t, const char *name, int64_t rows, int64_t cols, bool output, NormView *out) {
+    if (!t) return ST_OK;
+    ST_TRY(check_matrix(t, name));
+    if (t->shape[0] != rows || t->shape[1] != cols)
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be [" + std::to_string(rows) + ", " +
+                                                 std::to_string(cols) + "], got [" + std::to_string(t->shape[0]) + ", " +
+                                                 std::to_string(t->shape[1]) + "]");
+    if (!unit_columns(*t)) return fail(ST_ERR_UNSUPPORTED, std::string(name) + " must have unit column stride");
+    if (output) ST_TRY(check_output(*t, name));
+    out->p = rows > 0 ? t->data : const_cast<char *>("");  // present, though without rows
+    out->dtype = t->dtype;
+    out->ld = t->strides[0];
+    return ST_OK;
+}
+
+int norm_weight(const st_tensor *t, const char *name, int64_t cols, NormView *out) {
+    if (!t) return ST_OK;
+    if (t->rank != 1 || t->shape[0] != cols)
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must have one element per column (" +
+                                                 std::to_string(cols) + ")");
+    if (!t->data) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " has a null data pointer");
+    if (cols > 1 && t->strides[0] != 1) return fail(ST_ERR_UNSUPPORTED, std::string(name) + " must be contiguous");
+    out->p = t->data;
+    out->dtype = t->dtype;
+    out->ld = 0;
+    return ST_OK;
+}
+
+// gate: [cols] or [1, cols] (channel), [rows, 1] (token), [rows, cols] (full)
+int norm_gate(const st_tensor *t, int64_t rows, int64_t cols, NormView *out, int *mode) {
+    *mode = kGateNone;
+    if (!t) return ST_OK;
+    if (t->rank == 1) {
+        *mode = kGateChannel;
+        return norm_weight(t, "gate", cols, out);
+    }
+    ST_TRY(check_matrix(t, "gate"));
+    const int64_t r = t->shape[0], c = t->shape[1];
+    if (r == rows && c == cols) *mode = kGateFull;
+    else if (r == 1 && c == cols) *mode = kGateChannel;
+    else if (r == rows && c == 1) *mode = kGateToken;
+    else
+        return fail(ST_ERR_INVALID_ARGUMENT, "gate must be [" + std::to_string(cols) + "], [1, " + std::to_string(cols) +
+                                                 "], [" + std::to_string(rows) + ", 1] or [" + std::to_string(rows) + ", " +
+                                                 std::to_string(cols) + "], got [" + std::to_string(r) + ", " +
+                                                 std::to_string(c) + "]");
+    if (*mode != kGateToken && !unit_columns(*t)) return fail(ST_ERR_UNSUPPORTED, "gate must have unit column stride");
+    out->p = t->data;
+    out->dtype = t->dtype;
+    out->ld = *mode == kGateChannel ? 0 : t->strides[0];
+    return ST_OK;
+}
+
+int check_norm_options(const char *what, const st_norm_options *o, int64_t cols) {
+    if (!o) return fail(ST_ERR_INVALID_ARGUMENT, std::string(what) + ": null options");
+    if (!std::isfinite(o->alpha) || !std::isfinite(o->weight_offset) || !std::isfinite(o->eps) || o->eps < 0.0f)
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(what) + ": alpha, weight_offset and eps must be finite, eps >= 0");
+    if (cols < 1) return fail(ST_ERR_INVALID_ARGUMENT, std::string(what) + ": rows must have at least one element");
+    return ST_OK;
+}
+
+// The branch's type T (x, h, their gradients) and the stream's S: S is T or ST_F32.
+int check_norm_types(const char *what, int t, int s) {
+    if (!is_float(t) || !is_float(s) || (s != t && s != ST_F32))
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(what) + ": tensors must be ST_F32, ST_F16 or ST_BF16, and the "
+                                                                 "residual stream of the branch's type or ST_F32");
+    return ST_OK;
+}
+
+int check_side_types(const char *what, int t, std::initializer_list<std::pair<const NormView *, const char *>> views) {
+    for (const auto &v : views)
+        if (v.first->p && v.first->dtype != ST_F32 && v.first->dtype != t)
+            return fail(ST_ERR_INVALID_ARGUMENT, std::string(what) + ": " + v.second + " must be ST_F32 or of the branch's type");
+    return ST_OK;
+}
+
 // ------------------------------------------------------------ entry registry
 enum class Kind { VectorAdd1D, VectorAdd2D, Matmul, Fma1D, Fma2D, Cast1D, Cast2D };
 
@@ -1374,6 +1527,224 @@ int st_vector_fma(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
     ST_TRY(launch_vector_fma(static_cast<const float *>(a->data), s[0], static_cast<const float *>(b->data), s[1],
                              static_cast<const float *>(d->data), s[2], static_cast<float *>(c->data), s[3], rows, cols,
                              x.dev->sm_count, x.stream));
+    return finish(x);
+}
+
+int st_quantize_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *q, const st_tensor *scale, int32_t block_rows,
+                    int32_t block_cols, const st_exec *exec) {
+    ST_TRY(check_matrix(a, "A"));
+    ST_TRY(check_matrix(q, "Q"));
+    ST_TRY(check_matrix(scale, "scale"));
+    const bool known = (block_rows == 1 && block_cols == 128) || (block_rows == 128 && block_cols == 1) ||
+                       (block_rows == 128 && block_cols == 128);
+    if (!known) return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp8: blocks are 1 x 128, 128 x 1 or 128 x 128");
+    if (!is_float(a->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp8: A must be ST_F32, ST_F16 or ST_BF16");
+    if (!is_fp8(q->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp8: Q must be ST_E4M3 or ST_E5M2");
+    if (scale->dtype != ST_F32) return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp8: scale must be ST_F32");
+    if (q->shape[0] != a->shape[0] || q->shape[1] != a->shape[1])
+        return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp8: A and Q must have the same shape");
+    if (scale->shape[0] != cdiv(a->shape[0], block_rows) || scale->shape[1] != cdiv(a->shape[1], block_cols))
+        return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp8: scale must be [" +
+                                                 std::to_string(cdiv(a->shape[0], block_rows)) + ", " +
+                                                 std::to_string(cdiv(a->shape[1], block_cols)) + "]");
+    ST_TRY(check_output(*q, "Q"));
+    ST_TRY(check_output(*scale, "scale"));
+    QuantizeArgs g{};
+    g.a = a->data;
+    g.a_dtype = a->dtype;
+    g.sa0 = a->strides[0];
+    g.sa1 = a->strides[1];
+    g.q = q->data;
+    g.e5m2 = q->dtype == ST_E5M2;
+    g.sq0 = q->strides[0];
+    g.sq1 = q->strides[1];
+    g.scale = static_cast<float *>(scale->data);
+    g.ss0 = scale->strides[0];
+    g.ss1 = scale->strides[1];
+    g.rows = a->shape[0];
+    g.cols = a->shape[1];
+    g.block_rows = block_rows;
+    g.block_cols = block_cols;
+    ExecCtx x;
+    ST_TRY(resolve_exec(ctx, exec, &x));
+    DeviceGuard guard(x.dev->ordinal);
+    ST_TRY(launch_quantize_fp8(g, x.stream));
+    return finish(x);
+}
+
+int st_matmul_fp8_workspace(const st_tensor *a, const st_tensor *b, uint64_t *bytes) {
+    if (!bytes) return fail(ST_ERR_INVALID_ARGUMENT, "bytes is null");
+    ST_TRY(check_fp8_operands(a, b));
+    *bytes = static_cast<uint64_t>(gemm_fp8_workspace_bytes(fp8_operand(*a, false), fp8_operand(*b, true)));
+    return ST_OK;
+}
+
+int st_matmul_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_tensor *a_scale,
+                  const st_tensor *b_scale, const st_tensor *bias, const st_tensor *c, void *workspace,
+                  uint64_t workspace_bytes, const st_exec *exec) {
+    ST_TRY(check_fp8_operands(a, b));
+    ST_TRY(check_matrix(c, "C"));
+    GemmFp8Args g{};
+    g.a = fp8_operand(*a, false);
+    g.b = fp8_operand(*b, true);
+    ST_TRY(set_scale(a_scale, "a_scale", false, &g.a));
+    ST_TRY(set_scale(b_scale, "b_scale", true, &g.b));
+    if (c->shape[0] != g.a.rows || c->shape[1] != g.b.rows)
+        return fail(ST_ERR_INVALID_ARGUMENT, "C must be [M, N] = [" + std::to_string(g.a.rows) + ", " +
+                                                 std::to_string(g.b.rows) + "]");
+    if (!is_float(c->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, "C must be ST_F32, ST_F16 or ST_BF16");
+    if (!unit_columns(*c)) return fail(ST_ERR_UNSUPPORTED, "C must have unit column stride");
+    ST_TRY(check_output(*c, "C"));
+    if (bias) {
+        if (bias->rank != 1 || bias->shape[0] != g.b.rows)
+            return fail(ST_ERR_INVALID_ARGUMENT, "bias must have N elements");
+        if (bias->dtype != ST_F32 && (bias->dtype != c->dtype || !is_float(bias->dtype)))
+            return fail(ST_ERR_INVALID_ARGUMENT, "bias must be ST_F32 or C's dtype");
+        if (bias->shape[0] > 1 && bias->strides[0] != 1) return fail(ST_ERR_UNSUPPORTED, "bias must be contiguous");
+        if (bias->shape[0] > 0 && !bias->data) return fail(ST_ERR_INVALID_ARGUMENT, "bias has a null data pointer");
+        g.bias = bias->data;
+        g.bias_dtype = bias->dtype;
+    }
+    const int64_t need = gemm_fp8_workspace_bytes(g.a, g.b);
+    if (need > 0 && (!workspace || workspace_bytes < static_cast<uint64_t>(need)))
+        return fail(ST_ERR_INVALID_ARGUMENT, "matmul_fp8 needs a workspace of " + std::to_string(need) +
+                                                 " bytes for operands that are not on 16-byte boundaries");
+    if (need > 0 && !aligned16(workspace)) return fail(ST_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    g.c = c->data;
+    g.ldc = c->strides[0];
+    g.c_dtype = c->dtype;
+    ExecCtx x;
+    ST_TRY(resolve_exec(ctx, exec, &x));
+    DeviceGuard guard(x.dev->ordinal);
+    ST_TRY(launch_gemm_fp8(g, workspace, x.dev->sm_count, x.dev->dev_err, kDeviceWaitLimitNs, x.stream));
+    return finish(x);
+}
+
+int st_residual_norm(st_ctx *ctx, const st_tensor *x_in, const st_tensor *residual, const st_tensor *post,
+                     const st_tensor *gate, const st_tensor *pre, const st_tensor *residual_out,
+                     const st_tensor *normed, const st_tensor *normed_scale, const st_norm_options *options,
+                     const st_exec *exec) {
+    ST_TRY(check_matrix(residual, "residual"));
+    NormArgs g{};
+    g.rows = residual->shape[0];
+    g.cols = residual->shape[1];
+    ST_TRY(check_norm_options("residual_norm", options, g.cols));
+    g.alpha = options->alpha;
+    g.eps = options->eps;
+    g.offset = options->weight_offset;
+    ST_TRY(norm_view(residual, "residual", g.rows, g.cols, false, &g.r));
+    ST_TRY(norm_view(x_in, "x", g.rows, g.cols, false, &g.x));
+    ST_TRY(norm_view(residual_out, "residual_out", g.rows, g.cols, true, &g.r_out));
+    ST_TRY(norm_view(normed, "normed", g.rows, g.cols, true, &g.h));
+    ST_TRY(norm_weight(post, "post_weight", g.cols, &g.post));
+    ST_TRY(norm_weight(pre, "pre_weight", g.cols, &g.pre));
+    ST_TRY(norm_gate(gate, g.rows, g.cols, &g.gate, &g.gate_mode));
+    if (!x_in && (post || gate)) return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm: post_weight and gate need x");
+    if ((pre != nullptr) != (normed != nullptr))
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm: pre_weight and normed come together");
+    if (!residual_out && !normed) return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm: nothing to compute");
+    g.h_fp8 = normed && is_fp8(normed->dtype);
+    g.h_e5m2 = normed && normed->dtype == ST_E5M2;
+    const int t = x_in ? x_in->dtype : (normed && !g.h_fp8 ? normed->dtype : residual->dtype);
+    ST_TRY(check_norm_types("residual_norm", t, residual->dtype));
+    if (residual_out && residual_out->dtype != residual->dtype)
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm: residual and residual_out must have the same dtype");
+    if (normed && !g.h_fp8 && normed->dtype != t)
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm: normed must have x's dtype, ST_E4M3 or ST_E5M2");
+    ST_TRY(check_side_types("residual_norm", t, {{&g.post, "post_weight"}, {&g.pre, "pre_weight"}, {&g.gate, "gate"}}));
+    if (g.h_fp8 != (normed_scale != nullptr))
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm: 8-bit blocks come with their scales, and only they do");
+    if (g.h_fp8) {
+        ST_TRY(check_matrix(normed_scale, "normed_scale"));
+        if (normed_scale->dtype != ST_F32 || normed_scale->shape[0] != g.rows ||
+            normed_scale->shape[1] != cdiv(g.cols, kScaleBlock))
+            return fail(ST_ERR_INVALID_ARGUMENT, "normed_scale must be ST_F32 [" + std::to_string(g.rows) + ", " +
+                                                     std::to_string(cdiv(g.cols, kScaleBlock)) + "]");
+        ST_TRY(check_output(*normed_scale, "normed_scale"));
+        g.h_scale = static_cast<float *>(normed_scale->data);
+        g.hs0 = normed_scale->strides[0];
+        g.hs1 = normed_scale->strides[1];
+    }
+    ExecCtx x;
+    ST_TRY(resolve_exec(ctx, exec, &x));
+    DeviceGuard guard(x.dev->ordinal);
+    ST_TRY(launch_residual_norm(g, x.dev->sm_count, x.stream));
+    return finish(x);
+}
+
+int st_residual_norm_backward_workspace(int64_t rows, int64_t cols, uint64_t *bytes) {
+    if (!bytes) return fail(ST_ERR_INVALID_ARGUMENT, "bytes is null");
+    if (rows < 0 || cols < 1 || rows > INT32_MAX || cols > INT32_MAX)
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: bad extents");
+    *bytes = static_cast<uint64_t>(residual_norm_backward_workspace(rows, cols));
+    return ST_OK;
+}
+
+int st_residual_norm_backward(st_ctx *ctx, const st_tensor *d_residual, const st_tensor *d_normed,
+                              const st_tensor *x_in, const st_tensor *residual, const st_tensor *post,
+                              const st_tensor *gate, const st_tensor *pre, const st_tensor *dx, const st_tensor *dr,
+                              const st_tensor *dpost, const st_tensor *dgate, const st_tensor *dpre, void *workspace,
+                              uint64_t workspace_bytes, const st_norm_options *options, const st_exec *exec) {
+    const char *const what = "residual_norm_backward";
+    if (!d_residual && !d_normed) return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: no gradient to take back");
+    const st_tensor *like = d_residual ? d_residual : d_normed;
+    ST_TRY(check_matrix(like, d_residual ? "d_residual" : "d_normed"));
+    NormBackwardArgs g{};
+    g.rows = like->shape[0];
+    g.cols = like->shape[1];
+    ST_TRY(check_norm_options(what, options, g.cols));
+    g.alpha = options->alpha;
+    g.eps = options->eps;
+    g.offset = options->weight_offset;
+    ST_TRY(norm_view(d_residual, "d_residual", g.rows, g.cols, false, &g.d_residual));
+    ST_TRY(norm_view(d_normed, "d_normed", g.rows, g.cols, false, &g.d_normed));
+    ST_TRY(norm_view(x_in, "x", g.rows, g.cols, false, &g.x));
+    ST_TRY(norm_view(residual, "residual", g.rows, g.cols, false, &g.r));
+    ST_TRY(norm_view(dx, "dx", g.rows, g.cols, true, &g.dx));
+    ST_TRY(norm_view(dr, "dr", g.rows, g.cols, true, &g.dr));
+    ST_TRY(norm_weight(post, "post_weight", g.cols, &g.post));
+    ST_TRY(norm_weight(pre, "pre_weight", g.cols, &g.pre));
+    ST_TRY(norm_gate(gate, g.rows, g.cols, &g.gate, &g.gate_mode));
+    if (!x_in && (post || gate)) return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: post_weight and gate need x");
+    if ((x_in != nullptr) != (dx != nullptr)) return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: x and dx come together");
+    if ((pre != nullptr) != (d_normed != nullptr))
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: pre_weight and d_normed come together");
+    if (pre && !residual) return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: pre_weight needs the updated residual");
+    if (!pre) g.r = NormView{};
+    const int t = x_in ? x_in->dtype : (d_normed ? d_normed->dtype : d_residual->dtype);
+    const int s = residual && pre ? residual->dtype : (d_residual ? d_residual->dtype : t);
+    ST_TRY(check_norm_types(what, t, s));
+    if ((d_residual && d_residual->dtype != s) || (dr && dr->dtype != s) || (d_normed && d_normed->dtype != t) ||
+        (dx && dx->dtype != t))
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: a gradient must have the dtype of its tensor");
+    ST_TRY(check_side_types(what, t, {{&g.post, "post_weight"}, {&g.pre, "pre_weight"}, {&g.gate, "gate"}}));
+    NormView sum;
+    if ((dpost && !post) || (dpre && !pre) || (dgate != nullptr) != (gate != nullptr))
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: dpost, dpre and dgate go with their tensors");
+    ST_TRY(norm_weight(dpost, "dpost", g.cols, &sum));
+    ST_TRY(norm_weight(dpre, "dpre", g.cols, &sum));
+    if ((dpost && dpost->dtype != ST_F32) || (dpre && dpre->dtype != ST_F32))
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: dpost and dpre must be ST_F32");
+    g.dpost = dpost ? static_cast<float *>(dpost->data) : nullptr;
+    g.dpre = dpre ? static_cast<float *>(dpre->data) : nullptr;
+    if (dgate) {
+        int mode = kGateNone;
+        ST_TRY(norm_gate(dgate, g.rows, g.cols, &g.dgate, &mode));
+        if (mode != g.gate_mode) return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: dgate must have the gate's shape");
+        if (dgate->rank == 2) ST_TRY(check_output(*dgate, "dgate"));
+        if (dgate->dtype != ST_F32 && (mode != kGateFull || dgate->dtype != t))
+            return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: dgate must be ST_F32, or the branch's type where "
+                                                 "the gate is [rows, cols]");
+    }
+    const uint64_t need = static_cast<uint64_t>(residual_norm_backward_workspace(g.rows, g.cols));
+    const bool sums = dpost || dpre || g.gate_mode == kGateChannel;
+    if (sums && g.rows > 0 && (!workspace || workspace_bytes < need))
+        return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward needs a workspace of " + std::to_string(need) + " bytes");
+    if (sums && g.rows > 0 && !aligned16(workspace)) return fail(ST_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    ExecCtx x;
+    ST_TRY(resolve_exec(ctx, exec, &x));
+    DeviceGuard guard(x.dev->ordinal);
+    ST_TRY(launch_residual_norm_backward(g, workspace, x.dev->sm_count, x.stream));
     return finish(x);
 }
 

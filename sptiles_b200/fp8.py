@@ -1,0 +1,171 @@
+"""8-bit blocks and their matrix product on CUDA tensors.
+
+``quantize_fp8`` makes 8-bit blocks of 128 with one float32 scale each,
+``matmul_fp8`` multiplies them.  A layer y = x @ W.t(), its gradients among
+its calls:
+
+    Wq, Ws = quantize_fp8(W, block=(128, 128))             # W [N, K], once
+    xq, xs = quantize_fp8(x)                               # x [M, K], blocks of 1 x 128
+    y = matmul_fp8(xq, Wq.t(), xs, Ws.t())
+
+    gq, gs = quantize_fp8(dy, dtype=torch.float8_e5m2)     # dx = dy @ W: W as it is stored
+    dx = matmul_fp8(gq, Wq, gs, Ws)
+    gq, gs = quantize_fp8(dy, block=(128, 1))              # dW = dy.t() @ x: blocks along the tokens
+    xq, xs = quantize_fp8(x, block=(128, 1))
+    dW = matmul_fp8(gq.t(), xq, gs.t(), xs, out_dtype=torch.float32)
+
+Neither call takes part in autograd.  Both run on torch's current stream of
+the tensors' device, keep nothing between calls and can be captured into a
+CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _native as N
+from .api import _CODES, _TENSOR_DESC, _exec_desc
+from .runtime import context
+
+BLOCK = 128
+_BLOCKS = ((1, BLOCK), (BLOCK, 1), (BLOCK, BLOCK))
+_FP8 = {torch.float8_e4m3fn: N.ST_E4M3, torch.float8_e5m2: N.ST_E5M2}
+_ALL_CODES = {**_CODES, **_FP8}
+
+_vp, _cp, _i32, _u64 = ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int32, ctypes.c_uint64
+_fns: dict = {}
+
+
+def _fn(name: str, *args):
+    """`name` from the native library; descriptors are passed as packed bytes."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = ctypes.CFUNCTYPE(ctypes.c_int, *args)((name, N.lib()))
+    return fn
+
+
+def _desc(t: torch.Tensor) -> bytes:
+    """The st_tensor descriptor of `t`, 8-bit types among them."""
+    shape, strides = t.shape, t.stride()
+    code = _ALL_CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"unsupported dtype {t.dtype}")
+    if len(shape) == 2:
+        return _TENSOR_DESC.pack(t.data_ptr() if shape[0] and shape[1] else 0, code, 2, shape[0], shape[1],
+                                 strides[0], strides[1])
+    if len(shape) == 1:
+        return _TENSOR_DESC.pack(t.data_ptr() if shape[0] else 0, code, 1, shape[0], 0, strides[0], 0)
+    raise ValueError("tensors must be rank 1 or 2")
+
+
+def _device_of(*tensors: torch.Tensor | None) -> int:
+    """The one CUDA device of every tensor given."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        d = t.get_device()
+        if d < 0:
+            raise ValueError("Input tensors must be on a CUDA device.")
+        if dev is not None and d != dev:
+            raise ValueError("Input tensors must be on the same CUDA device.")
+        dev = d
+    return dev
+
+
+def _empty_rows(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """[rows, cols] 8-bit codes, each row on a 16-byte boundary, where the tensor core's loads can start."""
+    ld = -(-cols // 16) * 16
+    t = torch.empty((rows, ld), dtype=dtype, device=device)
+    return t if ld == cols else t[:, :cols]
+
+
+def _empty_scales(rows: int, cols: int, block: tuple[int, int], device: torch.device) -> torch.Tensor:
+    """One scale per block, lying along the rows (columns) that have one each, as the product reads them."""
+    r, c = -(-rows // block[0]), -(-cols // block[1])
+    if block[0] == 1:
+        return torch.empty((c, r), dtype=torch.float32, device=device).t()
+    return torch.empty((r, c), dtype=torch.float32, device=device)
+
+
+def quantize_fp8(A: torch.Tensor, *, block: tuple[int, int] = (1, BLOCK), dtype: torch.dtype = torch.float8_e4m3fn,
+                 out: torch.Tensor | None = None, scale_out: torch.Tensor | None = None
+                 ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(Q, scale): A (rank 2; float32, float16 or bfloat16; any strides) as 8-bit blocks.
+
+    For each block, (1, 128), (128, 1) or (128, 128), cut at A's edges:
+    scale = max(max|a| / limit, 2^-126), Q = fp8(a * (1 / scale)) rounded to
+    nearest even, with limit 448 for float8_e4m3fn and 57344 for float8_e5m2.
+    scale is float32 [ceil(rows / block[0]), ceil(cols / block[1])].  Q is
+    laid out in A's order (by rows, or by columns for a transposed A) on
+    16-byte boundaries, so it need not be contiguous.  A block with a NaN or
+    an infinity gets a scale that is one, and a product that reads it is NaN.
+    """
+    if A.dim() != 2:
+        raise ValueError("A must be a 2D tensor.")
+    if tuple(block) not in _BLOCKS:
+        raise ValueError(f"block must be one of {_BLOCKS}, got {tuple(block)}")
+    if dtype not in _FP8:
+        raise ValueError(f"dtype must be torch.float8_e4m3fn or torch.float8_e5m2, got {dtype}")
+    if out is not None and out.dtype != dtype:
+        raise ValueError(f"out must have dtype {dtype}, got {out.dtype}")
+    dev = _device_of(A, out, scale_out)
+    rows, cols = A.shape
+    if out is None:
+        by_columns = A.stride(0) == 1 and A.stride(1) != 1 and cols > 1
+        out = _empty_rows(cols, rows, dtype, A.device).t() if by_columns else _empty_rows(rows, cols, dtype, A.device)
+    if scale_out is None:
+        scale_out = _empty_scales(rows, cols, block, A.device)
+    rc = _fn("st_quantize_fp8", _vp, _cp, _cp, _cp, _i32, _i32, _cp)(
+        context(dev), _desc(A), _desc(out), _desc(scale_out), block[0], block[1], _exec_desc(dev))
+    if rc != N.ST_OK:
+        N.check(rc, "quantize_fp8")
+    return out, scale_out
+
+
+def _on_16_bytes(t: torch.Tensor) -> bool:
+    """Whether the tensor core's loads address `t` in place (a copy is made otherwise)."""
+    s0, s1 = t.stride()
+    return t.data_ptr() % 16 == 0 and ((s1 == 1 and s0 > 0 and s0 % 16 == 0) or (s0 == 1 and s1 > 0 and s1 % 16 == 0))
+
+
+def matmul_fp8(A: torch.Tensor, B: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
+               bias: torch.Tensor | None = None, *, out_dtype: torch.dtype = torch.bfloat16,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """C = A @ B (+ bias) for 8-bit A [M, K] and B [K, N] with a scale for each block of 128 along K.
+
+    A, B: float8_e4m3fn or float8_e5m2, each of its own type and any strides
+    (rows or columns on 16-byte boundaries, as quantize_fp8 lays them out,
+    are read in place; anything else is copied first).  a_scale: float32
+    [M, ceil(K/128)], or [ceil(M/128), ceil(K/128)] with one scale for 128
+    rows; b_scale: float32 [ceil(K/128), N] or [ceil(K/128), ceil(N/128)];
+    any strides.  Products are summed in fp32, block by block.  C is
+    bfloat16, float16 or float32; bias (length N) is float32 or C's dtype.
+    The same inputs give the same bits.
+    """
+    sa, sb = A.shape, B.shape
+    if len(sa) != 2 or len(sb) != 2:
+        raise ValueError("A and B must be 2D tensors.")
+    if sa[1] != sb[0]:
+        raise ValueError(f"Incompatible matrices: K dimension of A ({sa[1]}) "
+                         f"must match K dimension of B ({sb[0]})")
+    dev = _device_of(A, B, a_scale, b_scale, bias, out)
+    if out is None:
+        out = torch.empty((sa[0], sb[1]), dtype=out_dtype, device=A.device)
+    da, db = _desc(A), _desc(B)
+    workspace, need = None, 0
+    if not (_on_16_bytes(A) and _on_16_bytes(B)):
+        size = ctypes.c_uint64(0)
+        rc = _fn("st_matmul_fp8_workspace", _cp, _cp, _vp)(da, db, ctypes.addressof(size))
+        if rc != N.ST_OK:
+            N.check(rc, "matmul_fp8")
+        need = size.value
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=A.device)
+    rc = _fn("st_matmul_fp8", _vp, _cp, _cp, _cp, _cp, _cp, _cp, _vp, _u64, _cp)(
+        context(dev), da, db, _desc(a_scale), _desc(b_scale), None if bias is None else _desc(bias), _desc(out),
+        None if workspace is None else workspace.data_ptr(), need, _exec_desc(dev))
+    if rc != N.ST_OK:
+        N.check(rc, "matmul_fp8")
+    return out

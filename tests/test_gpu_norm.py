@@ -1,0 +1,323 @@
+"""residual_norm and its backward on the GPU against float64.
+
+Bounds.  A row's sum of n squares is added in a tree of depth below 64 (8
+elements a lane at most four times, 5 shuffles, 5 more over warps), so it is
+within 64 * 2^-24 relative, its root half of that; with the handful of fp32
+products around it a value u, h, t or dx before its rounding is within
+2^-16 of the sum of the magnitudes it is made of.  A rounding to type T adds
+eps(T) / 2 relative.  A sum over rows adds at most rows + 64 fp32 additions,
+each 2^-24 of the sum of magnitudes."""
+import pytest
+import torch
+
+import sptiles_b200 as st
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+REL = 2.0 ** -16
+EPS = 1e-5
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def close(got, want, mass, dtype, rel=REL):
+    assert got is not None and got.dtype == dtype and got.shape == want.shape, (got.dtype, got.shape, want.shape)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    off = (got.double().cpu() - want).abs() - rel * mass - half(dtype) * (want.abs() + rel * mass) - tiny
+    assert not torch.isnan(off).any()
+    assert off.numel() == 0 or off.max().item() <= 0, off.max().item()
+
+
+def rms(v, w):
+    return v / torch.sqrt(v.square().mean(1, keepdim=True) + EPS) * w
+
+
+def inputs(rows, cols, tx, tr, gate, post, pre, seed=0, with_x=True):
+    g = gen(seed)
+    r = {"x": (torch.randn(rows, cols, generator=g) * 2).to(tx) if with_x else None,
+         "r": torch.randn(rows, cols, generator=g).to(tr),
+         "post": (1 + 0.3 * torch.randn(cols, generator=g)).to(tx) if post else None,
+         "pre": (1 + 0.3 * torch.randn(cols, generator=g)).to(F32 if seed % 2 else tx) if pre else None}
+    shape = {"none": None, "channel": (cols,), "row": (1, cols), "token": (rows, 1), "full": (rows, cols)}[gate]
+    r["gate"] = torch.randn(*shape, generator=g).to(tx) if shape else None
+    return r
+
+
+def dev(d):
+    return {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+
+
+def dbl(d):
+    return {k: v.double() if isinstance(v, torch.Tensor) else v for k, v in d.items()}
+
+
+def forward64(d, alpha, offset):
+    r, mass = d["r"], d["r"].abs()
+    if d["x"] is not None:
+        u = d["x"] if d["post"] is None else rms(d["x"], d["post"] + offset)
+        u = u * alpha * (1 if d["gate"] is None else d["gate"])
+        r, mass = r + u, mass + u.abs()
+    h = None if d["pre"] is None else rms(r, d["pre"] + offset)
+    return r, mass, h
+
+
+def check_forward(d, alpha=0.7, offset=0.0, **kw):
+    g = dev(d)
+    got = st.residual_norm(g["x"], g["r"], g["post"], g["gate"], g["pre"], alpha=alpha, eps=EPS, weight_offset=offset, **kw)
+    r, mass, h = forward64(dbl(d), alpha, offset)
+    if d["x"] is not None:
+        close(got.residual, r, mass, d["r"].dtype)
+    else:
+        assert got.residual is g["r"]
+    if h is None:
+        assert got.normed is None
+        return got
+    w = (d["pre"].double() + offset).abs()
+    hmass = mass / torch.sqrt(r.square().mean(1, keepdim=True) + EPS) * w + h.abs()
+    tx = d["x"].dtype if d["x"] is not None else d["r"].dtype
+    if got.scale is None:
+        close(got.normed, h, hmass, tx)
+        return got
+    # 8-bit blocks: the scale within the bound of the block's largest value; the codes within half a step of the
+    # value, or of the smallest one (2^-9 for e4m3, 2^-16 for e5m2)
+    rows, cols = h.shape
+    e5 = got.normed.dtype == torch.float8_e5m2
+    pad = -cols % 128
+    blocks = torch.nn.functional.pad(h, (0, pad)).view(rows, -1, 128)
+    mblocks = torch.nn.functional.pad(hmass, (0, pad)).view(rows, -1, 128)
+    limit = 57344.0 if e5 else 448.0
+    assert got.scale.shape == (rows, blocks.shape[1]) and got.scale.dtype == F32
+    want = blocks.abs().amax(2) / limit
+    s = got.scale.cpu().double()
+    assert ((s - want).abs() <= REL * mblocks.amax(2) / limit + 2.0 ** -23 * want + 2.0 ** -125).all()
+    back = got.normed.cpu().double() * s.repeat_interleave(128, 1)[:, :cols]
+    step = 2.0 ** -3 if e5 else 2.0 ** -4
+    least = (2.0 ** -17 if e5 else 2.0 ** -10) * s.repeat_interleave(128, 1)[:, :cols]
+    assert ((back - h).abs() <= step * h.abs() + least + 4 * REL * hmass).all()
+    return got
+
+
+SHAPES = [(1, 1), (1, 4096), (2, 5), (3, 32), (5, 255), (7, 256), (6, 300), (9, 512), (4, 513), (3, 2049), (130, 1024),
+          (2, 8192), (2, 8200), (1, 16384), (3, 12001)]
+
+
+@pytest.mark.parametrize("quantize", [False, True], ids=["plain", "fp8"])
+@pytest.mark.parametrize("tx,tr", [(F32, F32), (F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)],
+                         ids=["f32", "f16", "bf16", "f16_f32", "bf16_f32"])
+@pytest.mark.parametrize("rows,cols", SHAPES, ids=lambda v: str(v))
+def test_forward(rows, cols, tx, tr, quantize):
+    check_forward(inputs(rows, cols, tx, tr, "channel", True, True, seed=rows + cols), quantize=quantize)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "row", "token", "full"])
+@pytest.mark.parametrize("post", [True, False], ids=["post", "nopost"])
+@pytest.mark.parametrize("pre", [True, False], ids=["pre", "nopre"])
+@pytest.mark.parametrize("rows,cols", [(5, 96), (4, 1100)], ids=lambda v: str(v))
+def test_forward_parts(rows, cols, pre, post, gate):
+    check_forward(inputs(rows, cols, BF16, F32, gate, post, pre, seed=2), offset=1.0)
+
+
+def test_forward_first_norm():
+    for tr, out in [(F32, None), (F32, BF16), (BF16, None)]:
+        d = inputs(6, 700, tr if out is None else out, tr, "none", False, True, with_x=False)
+        d["pre"] = d["pre"].to(F32)
+        g = dev(d)
+        got = st.residual_norm(None, g["r"], pre_weight=g["pre"], eps=EPS, out_dtype=out)
+        want = rms(d["r"].double(), d["pre"].double())
+        close(got.normed, want, 2 * want.abs(), out or tr)
+        assert got.residual is g["r"]
+    check_forward(inputs(6, 700, BF16, BF16, "none", False, True, with_x=False), quantize=torch.float8_e5m2)
+
+
+def test_forward_in_place_strided_and_zero_rows():
+    d = inputs(20, 640, BF16, BF16, "token", True, True)
+    d["x"][3], d["r"][3] = 0, 0  # a row of zeros: normed to zeros
+    want = check_forward(d)
+    room = torch.full((22, 700), 9.0, dtype=BF16, device=DEV)
+    for shift in (8, 3):  # 16-byte rows, and not
+        v = room[1:21, shift:shift + 640]
+        v.copy_(d["r"])
+        g = dev(d)
+        got = st.residual_norm(g["x"], v, g["post"], g["gate"], g["pre"], alpha=0.7, eps=EPS, out=v)
+        assert got.residual.data_ptr() == v.data_ptr()
+        close(v, want.residual.cpu().double(), 2 * want.residual.cpu().double().abs(), BF16, rel=2.0 ** -8)
+        keep = room.clone()
+        keep[1:21, shift:shift + 640] = 9.0
+        assert (keep == 9.0).all()
+        room.fill_(9.0)
+    empty = st.residual_norm(torch.empty(0, 64, device=DEV), torch.empty(0, 64, device=DEV), pre_weight=torch.ones(64, device=DEV))
+    assert empty.residual.shape == (0, 64) and empty.normed.shape == (0, 64)
+
+
+def test_forward_nan_stays_in_its_row():
+    d = inputs(5, 300, F32, F32, "none", True, True)
+    d["x"][2, 7] = float("nan")
+    g = dev(d)
+    got = st.residual_norm(g["x"], g["r"], g["post"], None, g["pre"], eps=EPS, quantize=True)
+    assert torch.isnan(got.residual[2]).all() and torch.isnan(got.scale[2]).all()
+    for r in (0, 1, 3, 4):
+        assert torch.isfinite(got.residual[r]).all() and torch.isfinite(got.scale[r]).all()
+
+
+# ------------------------------------------------------------------ backward
+def backward64(d, dr, dh, alpha, offset):
+    """Gradients and, for each, the sum of the magnitudes it is made of."""
+    out, mass = {}, {}
+    total = dr if dr is not None else torch.zeros_like(dh)
+    tmass = total.abs()
+    if d["pre"] is not None:
+        r, w = d["r"], d["pre"] + offset
+        inv = 1 / torch.sqrt(r.square().mean(1, keepdim=True) + EPS)
+        hat, t = r * inv, dh * w
+        out["pre"], mass["pre"] = (dh * hat).sum(0), (dh * hat).abs().sum(0)
+        total = total + inv * (t - hat * (t * hat).mean(1, keepdim=True))
+        tmass = tmass + inv * (t.abs() + hat.abs() * (t * hat).abs().mean(1, keepdim=True))
+    out["residual"], mass["residual"] = total, tmass
+    if d["x"] is None:
+        return out, mass
+    gate = 1 if d["gate"] is None else d["gate"]
+    agate = 1 if d["gate"] is None else d["gate"].abs()
+    x, w = d["x"], 1.0 if d["post"] is None else d["post"] + offset
+    aw = 1.0 if d["post"] is None else w.abs()
+    inv = 1.0 if d["post"] is None else 1 / torch.sqrt(x.square().mean(1, keepdim=True) + EPS)
+    hat = x * inv
+    du, dumass = alpha * gate * total, alpha * agate * tmass
+    if d["post"] is None:
+        out["x"], mass["x"] = du, dumass
+    else:
+        t, tm = du * w, dumass * aw
+        out["x"] = inv * (t - hat * (t * hat).mean(1, keepdim=True))
+        mass["x"] = inv * (tm + hat.abs() * (tm * hat.abs()).mean(1, keepdim=True))
+        out["post"], mass["post"] = (du * hat).sum(0), (dumass * hat.abs()).sum(0)
+    if d["gate"] is not None:
+        g, gm = alpha * total * hat * w, alpha * tmass * hat.abs() * aw
+        if d["gate"].dim() == 1 or (d["gate"].shape[0] == 1 and g.shape[0] != 1):
+            g, gm = (v.sum(0).view(d["gate"].shape) for v in (g, gm))
+        elif d["gate"].shape[1] == 1 and g.shape[1] != 1:
+            g, gm = (v.sum(1, keepdim=True) for v in (g, gm))
+        out["gate"], mass["gate"] = g, gm
+    return out, mass
+
+
+def check_backward(d, rows, cols, tx, tr, alpha=0.7, offset=0.0, d_residual=True):
+    g = gen(99)
+    dr = torch.randn(rows, cols, generator=g).to(tr) if d_residual else None
+    dh = torch.randn(rows, cols, generator=g).to(tx) if d["pre"] is not None else None
+    c = dev(d)
+    args = [None if t is None else t.to(DEV) for t in (dr, dh)]
+    got = st.residual_norm_backward(*args, c["x"], c["r"] if d["pre"] is not None else None, c["post"], c["gate"], c["pre"],
+                                    alpha=alpha, eps=EPS, weight_offset=offset)
+    want, mass = backward64(dbl(d), *[None if t is None else t.double() for t in (dr, dh)], alpha, offset)
+    over_rows = REL + (rows + 64) * 2.0 ** -24
+    close(got.residual, want["residual"], mass["residual"], tr)
+    for name, dtype, value in [("x", tx, got.x), ("post", F32, got.post_weight), ("pre", F32, got.pre_weight),
+                               ("gate", None, got.gate)]:
+        if name not in want:
+            assert value is None
+            continue
+        if name == "gate":
+            full = d["gate"].dim() == 2 and d["gate"].shape == (rows, cols)
+            dtype = tx if full else F32
+        close(value, want[name], mass[name], dtype, rel=REL if name == "x" else over_rows)
+    return got
+
+
+@pytest.mark.parametrize("tx,tr", [(F32, F32), (F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)],
+                         ids=["f32", "f16", "bf16", "f16_f32", "bf16_f32"])
+@pytest.mark.parametrize("rows,cols", SHAPES + [(700, 512), (1300, 96), (333, 2048)], ids=lambda v: str(v))
+def test_backward(rows, cols, tx, tr):
+    check_backward(inputs(rows, cols, tx, tr, "channel", True, True, seed=rows), rows, cols, tx, tr)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "row", "token", "full"])
+@pytest.mark.parametrize("post", [True, False], ids=["post", "nopost"])
+@pytest.mark.parametrize("pre", [True, False], ids=["pre", "nopre"])
+@pytest.mark.parametrize("rows,cols", [(5, 96), (40, 1100), (1, 64)], ids=lambda v: str(v))
+def test_backward_parts(rows, cols, pre, post, gate):
+    check_backward(inputs(rows, cols, BF16, F32, gate, post, pre, seed=2), rows, cols, BF16, F32, offset=1.0)
+
+
+def test_backward_first_norm_and_missing_gradients():
+    check_backward(inputs(33, 600, F32, F32, "none", False, True, with_x=False), 33, 600, F32, F32, d_residual=False)
+    check_backward(inputs(33, 600, BF16, BF16, "none", True, True), 33, 600, BF16, BF16, d_residual=False)
+    e = torch.empty(0, 64, device=DEV)
+    w = torch.ones(64, device=DEV)
+    got = st.residual_norm_backward(e, e, e, e, w, w, w)
+    for s in (got.post_weight, got.gate, got.pre_weight):
+        assert s.shape == (64,) and (s == 0).all()
+
+
+def test_backward_against_differences():
+    """The gradients times a direction against the forward call's own differences, in float32 with float64 quotients."""
+    rows, cols = 6, 80
+    d = dbl(inputs(rows, cols, F32, F32, "channel", True, True, seed=4))
+    g = gen(5)
+    dr, dh = torch.randn(rows, cols, generator=g).double(), torch.randn(rows, cols, generator=g).double()
+
+    def loss(v):
+        r, _, h = forward64(v, 0.7, 0.0)
+        return (r * dr).sum() + (h * dh).sum()
+
+    r_out = forward64(d, 0.7, 0.0)[0]
+    f = {k: v.float().to(DEV) for k, v in d.items()}
+    got = st.residual_norm_backward(dr.float().to(DEV), dh.float().to(DEV), f["x"], r_out.float().to(DEV), f["post"], f["gate"],
+                                    f["pre"], alpha=0.7, eps=EPS)
+    for name, grad in [("x", got.x), ("r", got.residual), ("post", got.post_weight), ("gate", got.gate), ("pre", got.pre_weight)]:
+        way = torch.randn(d[name].shape, generator=g).double()
+        step = 1e-5  # central differences in float64: off by about step^2 and 1e-16 / step, both below 1e-9
+        up, down = ({**d, name: d[name] + s * step * way} for s in (1, -1))
+        slope = (loss(up) - loss(down)) / (2 * step)
+        mine = grad.double().cpu()
+        assert abs((mine * way).sum() - slope) <= 2.0 ** -14 * (mine.abs() * way.abs()).sum() + 1e-6, name
+
+
+def test_backward_same_bits_and_graph():
+    rows, cols = 500, 1024
+    d = dev(inputs(rows, cols, BF16, BF16, "channel", True, True))
+    dr = torch.randn(rows, cols, generator=gen(1)).to(BF16).to(DEV)
+    dh = torch.randn(rows, cols, generator=gen(2)).to(BF16).to(DEV)
+
+    def step():
+        f = st.residual_norm(d["x"], d["r"], d["post"], d["gate"], d["pre"])
+        return [f.normed, *st.residual_norm_backward(dr, dh, d["x"], f.residual, d["post"], d["gate"], d["pre"])]
+
+    first = step()
+    for a, b in zip(first, step()):
+        assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            again = step()
+    torch.cuda.synchronize()
+    for t in again:
+        t.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(first, again):
+        assert torch.equal(a, b)
+
+
+def test_norm_into_product():
+    """The 8-bit copy between two blocks goes straight into matmul_fp8."""
+    rows, cols, n = 70, 512, 200
+    d = dev(inputs(rows, cols, BF16, F32, "none", True, True))
+    W = torch.randn(n, cols, generator=gen(8)).to(BF16).to(DEV)
+    Wq, Ws = st.quantize_fp8(W, block=(128, 128))
+    f = st.residual_norm(d["x"], d["r"], d["post"], None, d["pre"], eps=EPS, quantize=True)
+    y = st.matmul_fp8(f.normed, Wq.t(), f.scale, Ws.t(), out_dtype=F32)
+    a = f.normed.double() * f.scale.double().repeat_interleave(128, 1)[:, :cols]
+    b = Wq.double() * Ws.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :cols]
+    want, mass = a @ b.t(), a.abs() @ b.abs().t()
+    assert ((y.double() - want).abs() <= (128 + 4 + 5) * 2.0 ** -23 * mass).all()
+    z = st.residual_norm(y[:, :n].to(BF16), torch.zeros(rows, n, device=DEV), torch.ones(n, device=DEV))
+    assert torch.isfinite(z.residual).all() and z.normed is None
