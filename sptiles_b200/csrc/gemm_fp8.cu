@@ -55,6 +55,7 @@ struct Fp8Params {
     const void *bias;
     int bias_dtype;
     int bias_on_rows;
+    int staged;  // CTA pairs: C leaves by TMA stores
     uint32_t idesc;
     int *err;
     unsigned long long timeout_ns;
@@ -411,6 +412,371 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     }
 }
 
+// ---------------------------------------------------------------- CTA pairs, 256 x 256 tiles
+// The large products.  A pair of CTAs (cta_group::2) computes 256 x 256 of C:
+// each holds 128 rows of the row operand and 128 columns of the column
+// operand, so a block of K costs an SM 32 KB of loads for 512 cycles of its
+// tensor core, half of what 128 x 128 tiles of one CTA take.  A block's
+// accumulator is 256 TMEM columns, two of them alternate.  Eight scaling
+// warps per CTA, two for each quarter of the lanes, hold 128 columns of
+// running sums each in registers: 64 packed multiply-adds and 128 columns
+// of tcgen05.ld a block, under half of the 512 cycles.
+//
+// full[s] lives in the even CTA and counts both CTAs' loads; the even CTA's
+// MMA thread commits empty[s] and tfull[a] to both CTAs; tempty[a] lives in
+// the even CTA and counts the pair's 16 scaling warps.
+constexpr int kPairScaleWarps = 8;
+constexpr int kPairThreads = 128 + 32 * kPairScaleWarps;  // warps 0 and 1 feed, 2 and 3 idle, 4.. scale
+// 128 running sums and their temporaries do not fit the 168 registers that
+// 384 threads get each: the feeding warpgroup hands its own over,
+// 56 + 2 * 224 = 3 * 168.
+constexpr int kPairFeedRegs = 56, kPairScaleRegs = 224;
+constexpr int kPairCols = 256;
+constexpr int kPairWarpCols = 128;  // columns of a scaling warp
+constexpr int kBoxBytes = 32 * 128;
+
+struct PairCfg {
+    static constexpr int kRowBytes = kTileRows * kBlockK;
+    static constexpr int kColBytes = 128 * kBlockK;
+    static constexpr int kStageBytes = kRowBytes + kColBytes;
+    static constexpr int kStages = 4;
+    static constexpr int kAccs = 2;
+    static constexpr int kTmemCols = kAccs * kPairCols;
+    static constexpr int kStoreBytes = kPairScaleWarps * 2 * kBoxBytes;
+    static constexpr int kColScaleBytes = kPairScaleWarps * 2 * kPairWarpCols * 4;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kStoreBytes + kColScaleBytes + 1024;
+    static_assert(kSmemBytes <= 232448, "over the per-block shared memory limit");
+};
+
+// One lane's 128-byte row of a 32-row box in the 128-byte swizzle.
+__device__ __forceinline__ void put_box_row(uint32_t box, int lane, const uint32_t (&w)[32]) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const uint32_t at = box + static_cast<uint32_t>(lane * 128 + ((q ^ (lane & 7)) << 4));
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[4 * q]), "r"(w[4 * q + 1]),
+                     "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
+                     : "memory");
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_16(float a, float b, int dtype) {
+    if (dtype == ST_F16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Row and column tile of tile t: 8 row tiles of a column tile after another,
+// so that the tiles in flight share their operands in L2.
+__device__ __forceinline__ void pair_tile(const Fp8Params &p, int t, int &tr, int &tc) {
+    constexpr int kGroup = 8;
+    const int in_group = kGroup * p.tiles_c;
+    const int first = t / in_group * kGroup;
+    const int rows = p.tiles_r - first < kGroup ? p.tiles_r - first : kGroup;
+    tr = first + (t % in_group) % rows;
+    tc = (t % in_group) / rows;
+}
+
+template <bool R_MN, bool C_MN, bool CVEC>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
+                         const __grid_constant__ CUtensorMap tmap_out, const Fp8Params p) {
+    using Cfg = PairCfg;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *boxes = smem + Cfg::kStages * Cfg::kStageBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(boxes + Cfg::kStoreBytes);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * Cfg::kStages + 2 * Cfg::kAccs + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    float *col_scale = reinterpret_cast<float *>(boxes + Cfg::kStoreBytes + kBarBytes);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
+    const int tiles = p.tiles_r * p.tiles_c;
+    const uint32_t bar0 = smem_addr(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };
+    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + a); };
+    auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + Cfg::kAccs + a); };
+    const uint32_t drain_bar = bar0 + 8u * (2 * Cfg::kStages + 2 * Cfg::kAccs);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Cfg::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int a = 0; a < Cfg::kAccs; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), 2 * kPairScaleWarps);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_map(&tmap_r);
+        tma_prefetch_map(&tmap_c);
+        tma_prefetch_map(&tmap_out);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_addr(tmem_slot), Cfg::kTmemCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    cluster_sync();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_begin();  // nothing above touches global memory
+
+    if (warp < 4) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairFeedRegs));
+      if (warp == 0) {
+        // ------------------------------------------------ TMA producer (both CTAs)
+        if (lane == 0) {
+            const uint64_t pol = l2_policy_evict_last();
+            const uint32_t even_full0 = map_to_rank(full_bar(0), 0);
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                int tr, tc;
+                pair_tile(p, t, tr, tc);
+                const int r0 = tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows;
+                const int c0 = tc * kPairCols + static_cast<int>(rank) * 128;
+                for (int b = 0; b < p.k_blocks; ++b, ++issued) {
+                    if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * Cfg::kStageBytes);
+                    const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
+                    const uint32_t sc = sr + Cfg::kRowBytes;
+                    const uint32_t fb = even_full0 + 8u * s;
+                    const int k0 = b * kBlockK;
+                    if constexpr (R_MN) tma_load_2d_pair(sr, &tmap_r, fb, r0, k0, pol);
+                    else tma_load_2d_pair(sr, &tmap_r, fb, k0, r0, pol);
+                    if constexpr (C_MN) tma_load_2d_pair(sc, &tmap_c, fb, c0, k0, pol);
+                    else tma_load_2d_pair(sc, &tmap_c, fb, k0, c0, pol);
+                    if (++s == Cfg::kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                atomicExch(p.err, kDevAbortGemmProducer);
+            }
+            if (rank == 0) {  // the pair's copies have landed before it leaves, also after an abort
+                const volatile int never = 0;
+                for (int i = issued > Cfg::kStages ? issued - Cfg::kStages : 0; i < issued; ++i)
+                    (void)mbar_wait(full_bar(i % Cfg::kStages), static_cast<uint32_t>(i / Cfg::kStages) & 1u, &never,
+                                    p.timeout_ns);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issuer (even CTA)
+        if (rank == 0 && lane == 0) {
+            int s = 0, a = 0;
+            uint32_t ph = 0, aph = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                for (int b = 0; b < p.k_blocks; ++b) {
+                    if (!mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns) ||
+                        !mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
+                    const uint32_t sc = sr + Cfg::kRowBytes;
+#pragma unroll
+                    for (int ks = 0; ks < kBlockK / kMmaK; ++ks) {
+                        const uint64_t dr =
+                            smem_desc_sw128(sr + ks * (R_MN ? kMmaK * 128 : kMmaK), R_MN ? 128 * 128 : 16, 1024);
+                        const uint64_t dc =
+                            smem_desc_sw128(sc + ks * (C_MN ? kMmaK * 128 : kMmaK), C_MN ? 128 * 128 : 16, 1024);
+                        tc_mma_f8_pair(tmem_base + static_cast<uint32_t>(a * kPairCols), dr, dc, p.idesc, ks != 0 ? 1u : 0u);
+                    }
+                    tc_commit_pair_multicast(empty_bar(s), 3);
+                    tc_commit_pair_multicast(tfull_bar(a), 3);
+                    if (++s == Cfg::kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                    if (++a == Cfg::kAccs) {
+                        a = 0;
+                        aph ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                atomicExch(p.err, kDevAbortGemmMma);
+            }
+            tc_commit_pair(drain_bar);
+            (void)mbar_wait(drain_bar, 0, abort_flag, p.timeout_ns);
+        }
+      }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairScaleRegs));
+        // ------------------------------------------------ scaling warps (both CTAs)
+        const int g = warp & 3, e = warp - 4;
+        const int half = e >> 2;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(half * kPairWarpCols);
+        const uint32_t even_tempty0 = map_to_rank(tempty_bar(0), 0);
+        const uint32_t box0 = smem_addr(boxes) + static_cast<uint32_t>(e * 2 * kBoxBytes);
+        float *my_cols = col_scale + e * 2 * kPairWarpCols;
+        int a = 0, box = 0;
+        uint32_t aph = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < tiles; t += pairs) {
+            int tr, tc;
+            pair_tile(p, t, tr, tc);
+            const int row0 = tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows + g * 32;
+            const int row = row0 + lane;
+            const int col0 = tc * kPairCols + half * kPairWarpCols;
+            const bool row_ok = row < p.rows;
+            const float *rs = p.rs + static_cast<int64_t>(row_ok ? row >> p.rs_shift : 0) * p.rs_i;
+            // the warp's column scale, or lane l's four (columns l, l + 32, ...)
+            const float *cs[4];
+            bool col_ok[4];
+#pragma unroll
+            for (int i = 0; i < (CVEC ? 4 : 1); ++i) {
+                const int c = col0 + lane + 32 * i;
+                col_ok[i] = CVEC ? c < p.cols : col0 < p.cols;
+                cs[i] = p.cs + static_cast<int64_t>(col_ok[i] ? (CVEC ? c : col0) >> p.cs_shift : 0) * p.cs_i;
+            }
+            uint64_t acc[kPairWarpCols / 2];
+#pragma unroll
+            for (int j = 0; j < kPairWarpCols / 2; ++j) acc[j] = 0;
+            float r_next = row_ok ? rs[0] : 0.0f, c_next[4];
+#pragma unroll
+            for (int i = 0; i < (CVEC ? 4 : 1); ++i) c_next[i] = col_ok[i] ? cs[i][0] : 0.0f;
+            for (int b = 0; b < p.k_blocks; ++b) {
+                const float r_scale = r_next, c_scale = c_next[0];
+                float *buf = my_cols + (b & 1) * kPairWarpCols;
+                if constexpr (CVEC) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) buf[lane + 32 * i] = c_next[i];
+                    __syncwarp();
+                }
+                if (b + 1 < p.k_blocks) {  // the next block's scales arrive during this one
+                    r_next = row_ok ? rs[(b + 1) * p.rs_b] : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < (CVEC ? 4 : 1); ++i) c_next[i] = col_ok[i] ? cs[i][(b + 1) * p.cs_b] : 0.0f;
+                }
+                const bool ready = mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, ready)) {
+                    *abort_flag = 1;
+                    if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+                const uint32_t tm = t_lane + static_cast<uint32_t>(a * kPairCols);
+                const float both = r_scale * c_scale;
+                const uint64_t s2 = CVEC ? pack2(r_scale, r_scale) : pack2(both, both);
+                // 16 columns are multiplied while the next 16 are read
+                uint32_t v[2][16];
+                tmem_load_16(tm, v[0]);
+#pragma unroll
+                for (int j = 0; j < kPairWarpCols / 16; ++j) {
+                    tmem_load_wait_16(v[j & 1]);
+                    if (j + 1 < kPairWarpCols / 16) tmem_load_16(tm + (j + 1) * 16, v[(j + 1) & 1]);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const uint32_t(&x)[16] = v[j & 1];
+                        uint64_t &a0 = acc[8 * j + i / 2], &a1 = acc[8 * j + i / 2 + 1];
+                        if constexpr (CVEC) {
+                            const float4 c = *reinterpret_cast<const float4 *>(buf + 16 * j + i);
+                            fma2(a0, x[i], x[i + 1], mul2(s2, pack2(c.x, c.y)));
+                            fma2(a1, x[i + 2], x[i + 3], mul2(s2, pack2(c.z, c.w)));
+                        } else {
+                            fma2(a0, x[i], x[i + 1], s2);
+                            fma2(a1, x[i + 2], x[i + 3], s2);
+                        }
+                    }
+                }
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if (rank == 0) mbar_arrive(tempty_bar(a));
+                    else mbar_arrive_cluster(even_tempty0 + 8u * a);
+                }
+                if (++a == Cfg::kAccs) {
+                    a = 0;
+                    aph ^= 1u;
+                }
+            }
+            if (!ok) break;
+            // ---- bias, conversion, and out through two 32-row boxes of 128 bytes (TMA clips rows and 16-byte pieces at C's extents)
+            if (p.bias != nullptr) {
+#pragma unroll
+                for (int j = 0; j < kPairWarpCols / 2; ++j) {
+                    const int c = col0 + 2 * j;
+                    const float b0 = c < p.cols ? load_any(p.bias, p.bias_dtype, c) : 0.0f;
+                    const float b1 = c + 1 < p.cols ? load_any(p.bias, p.bias_dtype, c + 1) : 0.0f;
+                    acc[j] = pack2(lo2(acc[j]) + b0, hi2(acc[j]) + b1);
+                }
+            }
+            if (p.staged) {
+#pragma unroll
+                for (int h = 0; h < kPairWarpCols / 32; ++h) {  // 32 columns a step
+                    uint32_t w[32];
+                    if (p.c_dtype == ST_F32) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            w[2 * i] = static_cast<uint32_t>(acc[16 * h + i]);
+                            w[2 * i + 1] = static_cast<uint32_t>(acc[16 * h + i] >> 32);
+                        }
+                    } else {
+                        if (h & 1) continue;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            w[i] = pack_16(lo2(acc[(16 * h + i) % (kPairWarpCols / 2)]), hi2(acc[(16 * h + i) % (kPairWarpCols / 2)]),
+                                           p.c_dtype);
+                    }
+                    const int c = col0 + 32 * h;
+                    if (c >= p.cols || row0 >= p.rows) continue;
+                    if (lane == 0) bulk_wait_group_read<1>();  // the store that last used this box has read it
+                    __syncwarp();
+                    const uint32_t at = box0 + static_cast<uint32_t>(box * kBoxBytes);
+                    put_box_row(at, lane, w);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmap_out, at, c, row0);
+                        bulk_commit_group();
+                    }
+                    box ^= 1;
+                }
+            } else if (row_ok) {
+#pragma unroll
+                for (int j = 0; j < kPairWarpCols / 2; ++j) {
+                    const int c = col0 + 2 * j;
+                    if (c < p.cols) store_any(p.c, p.c_dtype, row * p.c_r + c, lo2(acc[j]));
+                    if (c + 1 < p.cols) store_any(p.c, p.c_dtype, row * p.c_r + c + 1, hi2(acc[j]));
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_group_all();  // every store of C has landed
+    }
+
+    tc_fence_before_sync();
+    __syncwarp();
+    cluster_sync();  // all MMAs retired, all TMEM reads done, no remote arrival pending
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    }
+}
+
 // Dense copy of a strided 8-bit [rows, cols] matrix, rows of `ld` bytes (a
 // multiple of 16; the padding is not written).  Unit column stride: 16 bytes
 // a thread, put together from the aligned words that hold them.
@@ -536,6 +902,55 @@ int launch_wide(const CUtensorMap &mr, const CUtensorMap &mc, const Fp8Params &p
                 : launch_instance<128, false, false, CVEC>(mr, mc, p, stream);
 }
 
+template <bool R_MN, bool C_MN, bool CVEC>
+int launch_pair_instance(const CUtensorMap &mr, const CUtensorMap &mc, const CUtensorMap &mo, const Fp8Params &p,
+                         int sm_count, cudaStream_t stream) {
+    auto kern = gemm_fp8_pair_kernel<R_MN, C_MN, CVEC>;
+    static uint64_t attr_set = 0;  // one bit per device ordinal
+    int dev = 0;
+    ST_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !(attr_set & (1ull << dev))) {
+        ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmemBytes));
+        if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
+    }
+    const int64_t tiles = static_cast<int64_t>(p.tiles_r) * p.tiles_c;
+    const int64_t pairs = tiles < sm_count / 2 ? tiles : sm_count / 2;
+    ST_CUDA_TRY(launch_kernel(kern, static_cast<unsigned>(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream, mr, mc, mo, p));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "gemm_fp8_pair_kernel launch");
+}
+
+template <bool CVEC>
+int launch_pair(const CUtensorMap &mr, const CUtensorMap &mc, const CUtensorMap &mo, const Fp8Params &p, bool r_mn,
+                bool c_mn, int sm_count, cudaStream_t stream) {
+    if (r_mn)
+        return c_mn ? launch_pair_instance<true, true, CVEC>(mr, mc, mo, p, sm_count, stream)
+                    : launch_pair_instance<true, false, CVEC>(mr, mc, mo, p, sm_count, stream);
+    return c_mn ? launch_pair_instance<false, true, CVEC>(mr, mc, mo, p, sm_count, stream)
+                : launch_pair_instance<false, false, CVEC>(mr, mc, mo, p, sm_count, stream);
+}
+
+// 32-row box of 128 bytes of C
+int make_map_out(CUtensorMap *map, const GemmFp8Args &g) {
+    auto fn = encode_fn();
+    if (!fn) return fail(ST_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const int es = static_cast<int>(dtype_size(g.c_dtype));
+    const CUtensorMapDataType dt = g.c_dtype == ST_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : g.c_dtype == ST_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(g.b.rows), static_cast<cuuint64_t>(g.a.rows)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(g.ldc) * es};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / es), 32};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, dt, 2, g.c, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(ST_ERR_INVALID_ARGUMENT, "cuTensorMapEncodeTiled rejected C (error " +
+                                                 std::to_string(static_cast<int>(r)) + ")");
+    return ST_OK;
+}
+
 // How TMA can read a [rows, k] operand: directly along K or along its rows,
 // or after a copy (the strides 0 of a broadcast among the copies).
 struct Access {
@@ -605,18 +1020,20 @@ int launch_gemm_fp8(const GemmFp8Args &g, void *workspace, int sm_count, int *de
     const bool swap = m <= 64 && m <= n && !acc[0].mn;
     const int ri = swap ? 1 : 0, ci = swap ? 0 : 1;
     const Fp8Operand &r = op[ri], &c = op[ci];
+    // 256 x 256 tiles of CTA pairs once they fill most of the pairs
+    const bool pair = !swap && n > 64 && cdiv(m, 256) * cdiv(n, 256) * 4 >= sm_count / 2 * 3;
     int bn = 128;
-    if (!acc[ci].mn) bn = c.rows <= 16 ? 16 : c.rows <= 32 ? 32 : c.rows <= 64 ? 64 : 128;
+    if (!pair && !acc[ci].mn) bn = c.rows <= 16 ? 16 : c.rows <= 32 ? 32 : c.rows <= 64 ? 64 : 128;
     Fp8Params p{};
     p.rows = static_cast<int>(r.rows);
     p.cols = static_cast<int>(c.rows);
     p.k_blocks = static_cast<int>(cdiv(k, kBlockK));
-    p.tiles_r = static_cast<int>(cdiv(r.rows, kTileRows));
-    p.tiles_c = static_cast<int>(cdiv(c.rows, bn));
+    p.tiles_r = static_cast<int>(cdiv(r.rows, pair ? 2 * kTileRows : kTileRows));
+    p.tiles_c = static_cast<int>(cdiv(c.rows, pair ? kPairCols : bn));
     const int64_t tiles = static_cast<int64_t>(p.tiles_r) * p.tiles_c;
     const int64_t slots = static_cast<int64_t>(sm_count) * (bn == 128 ? 1 : 2);
     p.split = 1;
-    while (p.split < 8 && tiles * p.split * 2 <= slots && p.k_blocks >= p.split * 2 * 2) p.split *= 2;
+    while (!pair && p.split < 8 && tiles * p.split * 2 <= slots && p.k_blocks >= p.split * 2 * 2) p.split *= 2;
     if (tiles * p.split > INT32_MAX) return fail(ST_ERR_UNSUPPORTED, "matmul_fp8: too many output tiles");
     p.rs = static_cast<const float *>(r.scale);
     p.rs_i = r.scale_row;
@@ -633,7 +1050,8 @@ int launch_gemm_fp8(const GemmFp8Args &g, void *workspace, int sm_count, int *de
     p.bias = g.bias;
     p.bias_dtype = g.bias_dtype;
     p.bias_on_rows = swap;
-    p.idesc = mma_idesc_f8(r.e5m2, c.e5m2, acc[ri].mn, acc[ci].mn, kTileRows, static_cast<uint32_t>(bn));
+    p.idesc = mma_idesc_f8(r.e5m2, c.e5m2, acc[ri].mn, acc[ci].mn, pair ? 2 * kTileRows : kTileRows,
+                           static_cast<uint32_t>(pair ? kPairCols : bn));
     p.err = dev_err;
     p.timeout_ns = timeout_ns;
     CUtensorMap mr, mc;
@@ -641,6 +1059,15 @@ int launch_gemm_fp8(const GemmFp8Args &g, void *workspace, int sm_count, int *de
     else ST_TRY(make_map_8(&mr, r.data, k, r.rows, acc[ri].ld, kTileRows));
     if (acc[ci].mn) ST_TRY(make_map_8(&mc, c.data, c.rows, k, acc[ci].ld, kBlockK));
     else ST_TRY(make_map_8(&mc, c.data, k, c.rows, acc[ci].ld, bn));
+    if (pair) {
+        CUtensorMap mo = mr;  // unused where C leaves by plain stores
+        // a TMA store writes whole 16-byte pieces: not where a row of C ends inside one
+        const int64_t es = static_cast<int64_t>(dtype_size(g.c_dtype));
+        p.staged = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc * es % 16 == 0 && n * es % 16 == 0;
+        if (p.staged) ST_TRY(make_map_out(&mo, g));
+        return p.cs_shift == 7 ? launch_pair<false>(mr, mc, mo, p, acc[ri].mn, acc[ci].mn, sm_count, stream)
+                               : launch_pair<true>(mr, mc, mo, p, acc[ri].mn, acc[ci].mn, sm_count, stream);
+    }
     switch (bn) {
     case 16: return launch_narrow<16>(mr, mc, p, acc[ri].mn, stream);
     case 32: return launch_narrow<32>(mr, mc, p, acc[ri].mn, stream);

@@ -293,3 +293,32 @@ def test_layer_forward_and_gradients():
     for got, want, mass in [(dx, dy.double() @ w.double(), dy.double().abs() @ w.double().abs()),
                             (dw, dy.double().t() @ x.double(), dy.double().abs().t() @ x.double().abs())]:
         assert ((got.cpu().double() - want).abs() <= (2 ** -4 + 2 ** -3 + 2 ** -7 + 2 ** -8) * mass).all()
+
+
+# 256 x 256 tiles of CTA pairs: enough of them, ragged at every edge, one and many blocks of K
+LARGE = [(2048, 1800, 100), (1793, 2100, 384), (3000, 1300, 1111), (2047, 2049, 2048)]
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("b_square", [True, False], ids=["b128", "b1"])
+@pytest.mark.parametrize("m,n,k", LARGE, ids=lambda v: str(v))
+def test_matmul_large(m, n, k, b_square, out):
+    a, b, sa, sb = make(m, n, k, E5, E4, b_square=b_square)
+    bias = torch.randn(n, generator=gen(9)) if k < 1000 else None
+    A, B, SA, SB = put(a), put(b).t(), sa.to(DEV), sb.t().to(DEV)
+    ld = -(-n // 8) * 8
+    for room in (torch.full((m, ld), 3.0, dtype=out, device=DEV), torch.full((m, n + 1), 3.0, dtype=out, device=DEV)):
+        C = room[:, :n]  # rows on 16-byte boundaries, and (for odd n) not
+        st.matmul_fp8(A, B, SA, SB, None if bias is None else bias.to(DEV), out=C)
+        check_product(C, a, b, sa, sb, bias, out)
+        assert (room[:, n:] == 3.0).all()
+
+
+@pytest.mark.parametrize("a_rows", [True, False], ids=["aK", "aM"])
+@pytest.mark.parametrize("b_rows", [True, False], ids=["bK", "bN"])
+@pytest.mark.parametrize("b_square", [True, False], ids=["b128", "b1"])
+def test_matmul_large_layouts(b_square, b_rows, a_rows):
+    m, n, k = 2050, 1810, 900
+    a, b, sa, sb = make(m, n, k, a_square=b_rows, b_square=b_square)
+    C = st.matmul_fp8(put(a, a_rows), put(b, b_rows, aligned=a_rows).t(), sa.to(DEV), sb.t().contiguous().to(DEV), out_dtype=torch.float32)
+    check_product(C, a, b, sa, sb, None, torch.float32)
