@@ -38,19 +38,17 @@ namespace {
 
 constexpr int kTileRows = 128;
 constexpr int kBlockK = 128;  // bytes = elements: one scale block, one 128-byte swizzle span
-constexpr int kThreads = 192;
-constexpr int kScaleWarps = 4;
 constexpr int kMmaK = 32;
 constexpr int kBarBytes = 1024;
 
 struct Fp8Params {
     int rows, cols, k_blocks;  // row operand x column operand
     int tiles_r, tiles_c, split;
-    const float *rs, *cs;        // scales of the row and the column operand
+    const float *rs, *cs;            // scales of the row and the column operand
     int64_t rs_i, rs_b, cs_i, cs_b;  // strides: per index (row / column or their block of 128), per K block
-    int rs_shift, cs_shift;      // 7: one scale for 128 rows / columns
+    int rs_shift, cs_shift;          // 7: one scale for 128 rows / columns
     void *c;
-    int64_t c_r, c_c;  // strides of C along the row and the column operand
+    int64_t c_r, c_c;  // strides of C along the row and the column operand; one of them is 1
     int c_dtype;
     const void *bias;
     int bias_dtype;
@@ -59,22 +57,6 @@ struct Fp8Params {
     uint32_t idesc;
     int *err;
     unsigned long long timeout_ns;
-};
-
-template <int BN>
-struct Fp8Cfg {
-    static constexpr int kRowBytes = kTileRows * kBlockK;
-    static constexpr int kColBytes = BN * kBlockK;
-    static constexpr int kStageBytes = kRowBytes + kColBytes;
-    // BN 128 fills an SM's TMEM (4 x 128 columns) and shared memory alone;
-    // narrower tiles leave room for two CTAs per SM
-    static constexpr int kStages = BN == 128 ? 6 : (BN == 64 ? 4 : (BN == 32 ? 5 : 6));
-    static constexpr int kAccs = 4;
-    static constexpr int kTmemCols = kAccs * BN;
-    static constexpr int kColScaleBytes = kScaleWarps * 2 * BN * 4;
-    static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kColScaleBytes + 1024;
-    static_assert(kSmemBytes <= (BN == 128 ? 232448 : 115712), "shared memory of one (two) CTAs per SM");
-    static_assert(kStages * kStageBytes >= kTileRows * BN * 4, "the ring holds a tile's partial sums");
 };
 
 __device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
@@ -87,6 +69,15 @@ __device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v
     if (dtype == ST_F32) static_cast<float *>(p)[i] = v;
     else if (dtype == ST_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
     else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ uint32_t pack_16(float a, float b, int dtype) {
+    if (dtype == ST_F16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // acc (two fp32) += v * s, one packed instruction
@@ -112,7 +103,7 @@ __device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float(static
 __device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
 
 // Load 16 consecutive f32 columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t *r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -121,9 +112,9 @@ __device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t (&r)[16]) 
         : "r"(taddr));
 }
 
-// Wait for the loads above; the registers pass through, so that nothing reads
-// them before it.
-__device__ __forceinline__ void tmem_load_wait_16(uint32_t (&r)[16]) {
+// Wait for every load so far; the registers pass through, so that nothing
+// reads them before it.
+__device__ __forceinline__ void tmem_load_wait_16(uint32_t *r) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
@@ -131,19 +122,154 @@ __device__ __forceinline__ void tmem_load_wait_16(uint32_t (&r)[16]) {
                  : "memory");
 }
 
+// acc[0..COLS) += accumulator columns at tm, times r_scale and the column
+// scales: cols[0] or, CVEC, one
+// of cols[] for each column.  STEP columns are multiplied while the next STEP
+// are read; `release` is called once the accumulator has been read.
+template <int COLS, bool CVEC, int STEP, typename Release>
+__device__ __forceinline__ void scale_and_add(uint64_t (&acc)[COLS / 2], uint32_t tm, float r_scale, const float *cols,
+                                              Release release) {
+    static_assert(COLS % STEP == 0 && STEP % 16 == 0, "whole steps");
+    constexpr int kSteps = COLS / STEP;
+    const float both = CVEC ? r_scale : r_scale * cols[0];
+    const uint64_t s2 = pack2(both, both);
+    uint32_t v[2][STEP];
+#pragma unroll
+    for (int i = 0; i < STEP; i += 16) tmem_load_16(tm + i, v[0] + i);
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        uint32_t *x = v[j & 1];
+#pragma unroll
+        for (int i = 0; i < STEP; i += 16) tmem_load_wait_16(x + i);
+        if (j + 1 < kSteps) {
+#pragma unroll
+            for (int i = 0; i < STEP; i += 16) tmem_load_16(tm + (j + 1) * STEP + i, v[(j + 1) & 1] + i);
+        } else {
+            release();
+        }
+#pragma unroll
+        for (int i = 0; i < STEP; i += 4) {
+            uint64_t &a0 = acc[(j * STEP + i) / 2], &a1 = acc[(j * STEP + i) / 2 + 1];
+            if constexpr (CVEC) {
+                const float4 c = *reinterpret_cast<const float4 *>(cols + j * STEP + i);
+                fma2(a0, x[i], x[i + 1], mul2(s2, pack2(c.x, c.y)));
+                fma2(a1, x[i + 2], x[i + 3], mul2(s2, pack2(c.z, c.w)));
+            } else {
+                fma2(a0, x[i], x[i + 1], s2);
+                fma2(a1, x[i + 2], x[i + 3], s2);
+            }
+        }
+    }
+}
+
+// One warp brings the scales of a tile's blocks, ROWS for its rows and COLS
+// for its columns (CVEC), or one for each 128 columns, into a ring of shared
+// memory DEPTH blocks ahead of their use: a load by the scaling warps
+// themselves would cost them its latency in every block (92 us against 76 at
+// 4096^3, measured with one block of look-ahead).
+__device__ __forceinline__ void copy_4_async(uint32_t dst, const float *src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+
+template <int ROWS, int COLS, bool CVEC, int DEPTH>
+struct ScaleRing {
+    static constexpr int kCols = CVEC ? COLS : (COLS + 127) / 128;
+    static constexpr int kSlot = ROWS + (kCols + 3) / 4 * 4;  // floats; 16-byte aligned columns
+    static constexpr int kBytes = DEPTH * kSlot * 4;
+    static constexpr int kBars = 2 * DEPTH;
+    float *slots;
+    uint32_t bar0;  // full[DEPTH], empty[DEPTH]
+    __device__ __forceinline__ uint32_t full(int d) const { return bar0 + 8u * d; }
+    __device__ __forceinline__ uint32_t empty(int d) const { return bar0 + 8u * (DEPTH + d); }
+    __device__ __forceinline__ void init(int readers) const {
+        for (int d = 0; d < DEPTH; ++d) {
+            mbar_init(full(d), 32);
+            mbar_init(empty(d), readers);
+        }
+    }
+    __device__ __forceinline__ const float *rows(int d) const { return slots + d * kSlot; }
+    __device__ __forceinline__ const float *cols(int d) const { return slots + d * kSlot + ROWS; }
+    // The scales of blocks [b0, b1) of the tile at row r0, column c0; false after an abort.
+    __device__ __forceinline__ bool load(const Fp8Params &p, int r0, int c0, int b0, int b1, int lane, int &d, uint32_t &ph,
+                                         const volatile int *abort_flag) const {
+        const float *src_r[ROWS / 32], *src_c[(kCols + 31) / 32];
+        bool ok_r[ROWS / 32], ok_c[(kCols + 31) / 32];
+#pragma unroll
+        for (int i = 0; i < ROWS / 32; ++i) {
+            const int r = r0 + lane + 32 * i;
+            ok_r[i] = r < p.rows;
+            src_r[i] = p.rs + static_cast<int64_t>(ok_r[i] ? r >> p.rs_shift : 0) * p.rs_i;
+        }
+#pragma unroll
+        for (int i = 0; i < (kCols + 31) / 32; ++i) {
+            const int j = lane + 32 * i, c = c0 + (CVEC ? j : 128 * j);
+            ok_c[i] = j < kCols && c < p.cols;
+            src_c[i] = p.cs + static_cast<int64_t>(ok_c[i] ? c >> p.cs_shift : 0) * p.cs_i;
+        }
+        for (int b = b0; b < b1; ++b) {
+            if (!__all_sync(0xffffffffu, mbar_wait(empty(d), ph ^ 1u, abort_flag, p.timeout_ns))) return false;
+            const uint32_t to_r = smem_addr(slots + d * kSlot) + 4u * lane, to_c = to_r + 4u * ROWS;
+#pragma unroll
+            for (int i = 0; i < ROWS / 32; ++i) copy_4_async(to_r + 128u * i, src_r[i] + b * p.rs_b, ok_r[i]);
+#pragma unroll
+            for (int i = 0; i < (kCols + 31) / 32; ++i)
+                if (lane + 32 * i < kCols) copy_4_async(to_c + 128u * i, src_c[i] + b * p.cs_b, ok_c[i]);
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(d)) : "memory");
+            if (++d == DEPTH) {
+                d = 0;
+                ph ^= 1u;
+            }
+        }
+        return true;
+    }
+};
+
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Bulk copies still in flight after `issued` of them through a ring of
+// barriers: wait (bounded, whatever the abort flag says) before leaving.
+template <typename Bar>
+__device__ __forceinline__ void drain_ring(int issued, int stages, Bar bar, uint64_t limit_ns) {
+    const volatile int never = 0;
+    for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+        (void)mbar_wait(bar(i % stages), static_cast<uint32_t>(i / stages) & 1u, &never, limit_ns);
+}
+
+// ---------------------------------------------------------------- one CTA, 128 x BN tiles
+constexpr int kScaleWarps = 4;
+constexpr int kThreads = 32 * (3 + kScaleWarps);  // warps 0 TMA, 1 MMA, 2..5 scaling, 6 scales
+constexpr int kPadRows = kTileRows + 1;           // odd: a column's and a row's elements lie in different banks
+
+template <int BN, bool CVEC>
+struct Fp8Cfg {
+    static constexpr int kRowBytes = kTileRows * kBlockK;
+    static constexpr int kColBytes = BN * kBlockK;
+    static constexpr int kStageBytes = kRowBytes + kColBytes;
+    // BN 128 fills an SM's TMEM (4 x 128 columns) and shared memory alone;
+    // narrower tiles leave room for two CTAs per SM
+    static constexpr int kStages = BN == 128 ? 6 : (BN == 64 ? 4 : (BN == 32 ? 5 : 6));
+    static constexpr int kAccs = 4;
+    static constexpr int kTmemCols = kAccs * BN;
+    using Ring = ScaleRing<kTileRows, BN, CVEC, 4>;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + Ring::kBytes + 1024;
+    static_assert(kSmemBytes <= (BN == 128 ? 232448 : 115712), "shared memory of one (two) CTAs per SM");
+    static_assert(kStages * kStageBytes >= kPadRows * BN * 4, "the ring holds a tile's partial sums");
+};
+
 // R_MN / C_MN: the operand is stored with its rows (columns) contiguous
 // instead of K.  CVEC: the column scale differs inside the tile.
 template <int BN, bool R_MN, bool C_MN, bool CVEC>
 __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
                     const Fp8Params p) {
-    using Cfg = Fp8Cfg<BN>;
+    using Cfg = Fp8Cfg<BN, CVEC>;
+    using Ring = typename Cfg::Ring;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::kStages * Cfg::kStageBytes);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * Cfg::kStages + 2 * Cfg::kAccs + 1);
+    constexpr int kBars = 2 * Cfg::kStages + 2 * Cfg::kAccs + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars + Ring::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    float *col_scale = reinterpret_cast<float *>(smem + Cfg::kStages * Cfg::kStageBytes + kBarBytes);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -152,7 +278,8 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     auto empty_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };
     auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + a); };
     auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + Cfg::kAccs + a); };
-    const uint32_t drain_bar = bar0 + 8u * (2 * Cfg::kStages + 2 * Cfg::kAccs);
+    const uint32_t drain_bar = bar0 + 8u * (kBars - 1);
+    const Ring ring{reinterpret_cast<float *>(smem + Cfg::kStages * Cfg::kStageBytes + kBarBytes), bar0 + 8u * kBars};
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
@@ -164,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
             mbar_init(tempty_bar(a), kScaleWarps);
         }
         mbar_init(drain_bar, 1);
+        ring.init(kScaleWarps);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -190,7 +318,13 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     const int b0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * part / split);
     const int b1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / split);
 
+    // scaling warps: TMEM lane = row of the tile
+    const int g = warp & 3;
+    const int row_in_tile = g * 32 + lane;
+    uint64_t acc[BN / 2];
+
     if (warp == 0) {
+        // ------------------------------------------------ TMA producer
         if (lane == 0) {
             const uint64_t pol = l2_policy_evict_last();
             int s = 0, issued = 0;
@@ -218,26 +352,24 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
                 *abort_flag = 1;
                 atomicExch(p.err, kDevAbortGemmProducer);
             }
-            // no copy is in flight when the CTA leaves, also after an abort
-            const volatile int never = 0;
-            for (int i = issued > Cfg::kStages ? issued - Cfg::kStages : 0; i < issued; ++i)
-                (void)mbar_wait(full_bar(i % Cfg::kStages), static_cast<uint32_t>(i / Cfg::kStages) & 1u, &never,
-                                p.timeout_ns);
+            drain_ring(issued, Cfg::kStages, full_bar, p.timeout_ns);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            int s = 0, a = 0;
-            uint32_t ph = 0, aph = 0;
-            bool ok = true;
-            for (int b = b0; b < b1; ++b) {
-                if (!mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns) ||
-                    !mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after_sync();
-                const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
-                const uint32_t sc = sr + Cfg::kRowBytes;
+        // ------------------------------------------------ MMA issuer
+        int s = 0, a = 0;
+        uint32_t ph = 0, aph = 0;
+        bool ok = true;
+        for (int b = b0; b < b1; ++b) {
+            const bool ready = mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns) &&
+                               mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns);
+            if (!__all_sync(0xffffffffu, ready)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after_sync();
+            const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
+            const uint32_t sc = sr + Cfg::kRowBytes;
+            if (elect_one()) {
 #pragma unroll
                 for (int ks = 0; ks < kBlockK / kMmaK; ++ks) {
                     // K-major: 32 bytes further along the 128-byte span; otherwise 32 K rows of 128 bytes
@@ -247,161 +379,133 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
                 }
                 tc_commit(empty_bar(s));
                 tc_commit(tfull_bar(a));
-                if (++s == Cfg::kStages) {
-                    s = 0;
-                    ph ^= 1u;
-                }
-                if (++a == Cfg::kAccs) {
-                    a = 0;
-                    aph ^= 1u;
-                }
             }
-            if (!ok) {
-                *abort_flag = 1;
-                atomicExch(p.err, kDevAbortGemmMma);
+            __syncwarp();
+            if (++s == Cfg::kStages) {
+                s = 0;
+                ph ^= 1u;
             }
-            tc_commit(drain_bar);
-            (void)mbar_wait(drain_bar, 0, abort_flag, p.timeout_ns);
+            if (++a == Cfg::kAccs) {
+                a = 0;
+                aph ^= 1u;
+            }
         }
-    }
-
-    // ------------------------------------------------ scaling warps
-    const int g = warp & 3;
-    const int row_in_tile = g * 32 + lane;
-    const int row = r0 + row_in_tile;
-    uint64_t acc[BN / 2];
-    if (warp >= 2) {
+        if (!ok) {
+            *abort_flag = 1;
+            atomicExch(p.err, kDevAbortGemmMma);
+        }
+        if (elect_one()) tc_commit(drain_bar);
+        __syncwarp();
+        (void)mbar_wait(drain_bar, 0, abort_flag, p.timeout_ns);
+    } else if (warp == 2 + kScaleWarps) {
+        // ------------------------------------------------ scales
+        int d = 0;
+        uint32_t dph = 0;
+        if (!ring.load(p, r0, c0, b0, b1, lane, d, dph, abort_flag)) *abort_flag = 1;
+        copies_done();
+    } else {
+        // ------------------------------------------------ scaling
 #pragma unroll
         for (int j = 0; j < BN / 2; ++j) acc[j] = 0;
-        const bool row_ok = row < p.rows;
-        const float *rs = p.rs + static_cast<int64_t>(row_ok ? row >> p.rs_shift : 0) * p.rs_i;
-        const float *cs = p.cs + static_cast<int64_t>(c0 >> p.cs_shift) * p.cs_i;
-        float *my_cols = col_scale + g * 2 * BN;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(g * 32) << 16);
-        int a = 0;
-        uint32_t aph = 0;
+        int a = 0, d = 0;
+        uint32_t aph = 0, dph = 0;
         for (int b = b0; b < b1; ++b) {
-            const float r_scale = row_ok ? rs[b * p.rs_b] : 0.0f;
-            float c_scale = 0.0f;
-            if constexpr (CVEC) {
-                float *buf = my_cols + (b & 1) * BN;
-#pragma unroll
-                for (int j = lane; j < BN; j += 32)
-                    buf[j] = c0 + j < p.cols
-                                 ? p.cs[static_cast<int64_t>((c0 + j) >> p.cs_shift) * p.cs_i + b * p.cs_b]
-                                 : 0.0f;
-                __syncwarp();
-            } else {
-                c_scale = cs[b * p.cs_b];
-            }
-            const bool ready = mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns);
+            const bool ready = mbar_wait(ring.full(d), dph, abort_flag, p.timeout_ns) &&
+                               mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns);
             if (!__all_sync(0xffffffffu, ready)) {
                 *abort_flag = 1;
                 if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
                 break;
             }
             tc_fence_after_sync();
-            const uint32_t t = t_lane + static_cast<uint32_t>(a * BN);
-            const float both = r_scale * c_scale;
-            const uint64_t s2 = CVEC ? pack2(r_scale, r_scale) : pack2(both, both);
-#pragma unroll
-            for (int j = 0; j < BN; j += 16) {
-                uint32_t v[16];
-                tmem_load_16(t + j, v);
-                tmem_load_wait_16(v);
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    if constexpr (CVEC) {
-                        const float4 c = *reinterpret_cast<const float4 *>(my_cols + (b & 1) * BN + j + i);
-                        fma2(acc[(j + i) / 2], v[i], v[i + 1], mul2(s2, pack2(c.x, c.y)));
-                        fma2(acc[(j + i) / 2 + 1], v[i + 2], v[i + 3], mul2(s2, pack2(c.z, c.w)));
-                    } else {
-                        fma2(acc[(j + i) / 2], v[i], v[i + 1], s2);
-                        fma2(acc[(j + i) / 2 + 1], v[i + 2], v[i + 3], s2);
-                    }
-                }
-            }
-            tc_fence_before_sync();
+            scale_and_add<BN, CVEC, (BN >= 64 ? 32 : 16)>(acc, t_lane + static_cast<uint32_t>(a * BN),
+                                                          ring.rows(d)[row_in_tile], ring.cols(d), [&] {
+                                                              tc_fence_before_sync();
+                                                              __syncwarp();
+                                                              if (lane == 0) mbar_arrive(tempty_bar(a));
+                                                          });
             __syncwarp();
-            if (lane == 0) mbar_arrive(tempty_bar(a));
+            if (lane == 0) mbar_arrive(ring.empty(d));
             if (++a == Cfg::kAccs) {
                 a = 0;
                 aph ^= 1u;
             }
+            if (++d == 4) {
+                d = 0;
+                dph ^= 1u;
+            }
         }
     }
 
-    // ------------------------------------------------ bias, conversion and the store
-    auto put = [&](int j, float v) {  // column j of the tile
-        const int col = c0 + j;
-        if (row >= p.rows || col >= p.cols) return;
-        if (p.bias != nullptr) v += load_any(p.bias, p.bias_dtype, p.bias_on_rows ? row : col);
-        store_any(p.c, p.c_dtype, row * p.c_r + col * p.c_c, v);
-    };
-    if (split == 1) {
-        if (warp >= 2) {
-            const int es = p.c_dtype == ST_F32 ? 4 : 2;
-            const bool wide = p.c_c == 1 && c0 + BN <= p.cols && p.bias == nullptr &&
-                              (reinterpret_cast<uintptr_t>(p.c) & 15u) == 0 && (p.c_r * es) % 16 == 0;
-            if (wide && row < p.rows) {
-                uint8_t *dst = static_cast<uint8_t *>(p.c) + (row * p.c_r + c0) * es;
-                if (p.c_dtype == ST_F32) {
+    // ------------------------------------------------ C
+    const bool scaler = warp >= 2 && warp < 2 + kScaleWarps;
+    const int es = p.c_dtype == ST_F32 ? 4 : 2;
+    const bool wide = split == 1 && p.c_c == 1 && c0 + BN <= p.cols && p.bias == nullptr &&
+                      (reinterpret_cast<uintptr_t>(p.c) & 15u) == 0 && (p.c_r * es) % 16 == 0;
+    if (wide) {  // whole 16-byte pieces of each row, straight from registers
+        const int row = r0 + row_in_tile;
+        if (scaler && row < p.rows) {
+            uint8_t *dst = static_cast<uint8_t *>(p.c) + (row * p.c_r + c0) * es;
+            if (p.c_dtype == ST_F32) {
 #pragma unroll
-                    for (int j = 0; j < BN / 2; j += 2)
-                        reinterpret_cast<float4 *>(dst)[j / 2] =
-                            make_float4(lo2(acc[j]), hi2(acc[j]), lo2(acc[j + 1]), hi2(acc[j + 1]));
-                } else {
+                for (int j = 0; j < BN / 2; j += 2)
+                    reinterpret_cast<float4 *>(dst)[j / 2] =
+                        make_float4(lo2(acc[j]), hi2(acc[j]), lo2(acc[j + 1]), hi2(acc[j + 1]));
+            } else {
 #pragma unroll
-                    for (int j = 0; j < BN / 2; j += 4) {
-                        uint32_t w[4];
+                for (int j = 0; j < BN / 2; j += 4) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (p.c_dtype == ST_F16) {
-                                const __half2 h = __floats2half2_rn(lo2(acc[j + i]), hi2(acc[j + i]));
-                                w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                            } else {
-                                const __nv_bfloat162 h = __floats2bfloat162_rn(lo2(acc[j + i]), hi2(acc[j + i]));
-                                w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                            }
-                        }
-                        reinterpret_cast<uint4 *>(dst)[j / 4] = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                }
-            } else if (!wide) {
-#pragma unroll
-                for (int j = 0; j < BN / 2; ++j) {
-                    put(2 * j, lo2(acc[j]));
-                    put(2 * j + 1, hi2(acc[j]));
+                    for (int i = 0; i < 4; ++i) w[i] = pack_16(lo2(acc[j + i]), hi2(acc[j + i]), p.c_dtype);
+                    reinterpret_cast<uint4 *>(dst)[j / 4] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
     } else {
-        // every CTA's partial sums into its own ring (all of its MMAs have
-        // read it), [column][row]; then part q adds columns q, q + split, ...
-        // over the parts in order
+        // Every CTA's (partial) sums go into its own ring, which its MMAs have
+        // read, as [column][row]; then its share of the tile is added over the
+        // parts in order, with a warp's lanes along C's contiguous dimension.
         float *mine = reinterpret_cast<float *>(smem);
-        if (warp >= 2) {
+        if (scaler) {
 #pragma unroll
             for (int j = 0; j < BN / 2; ++j) {
-                mine[(2 * j) * kTileRows + row_in_tile] = lo2(acc[j]);
-                mine[(2 * j + 1) * kTileRows + row_in_tile] = hi2(acc[j]);
+                mine[(2 * j) * kPadRows + row_in_tile] = lo2(acc[j]);
+                mine[(2 * j + 1) * kPadRows + row_in_tile] = hi2(acc[j]);
             }
         }
         __syncwarp();
-        cluster_sync();
-        if (warp >= 2) {
-            uint32_t part_addr[8];
-            for (int q = 0; q < 8; ++q) part_addr[q] = q < split ? map_to_rank(smem_addr(smem), q) : 0;
-            for (int j = part; j < BN; j += split) {
-                float v = 0.0f;
+        if (split > 1) cluster_sync();
+        else __syncthreads();
+        if (scaler) {
+            uint32_t at[8];
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (q < split) v += ld_cluster_f32(part_addr[q] + 4u * (j * kTileRows + row_in_tile));
-                put(j, v);
+            for (int q = 0; q < 8; ++q)
+                at[q] = split == 1 ? smem_addr(smem) : (q < split ? map_to_rank(smem_addr(smem), q) : 0);
+            auto put = [&](int r, int j) {  // row r, column j of the tile
+                if (r0 + r >= p.rows || c0 + j >= p.cols) return;
+                const uint32_t off = 4u * static_cast<uint32_t>(j * kPadRows + r);
+                float v = 0.0f;
+                if (split == 1) {
+                    v = mine[j * kPadRows + r];
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        if (q < split) v += ld_cluster_f32(at[q] + off);
+                }
+                if (p.bias != nullptr) v += load_any(p.bias, p.bias_dtype, p.bias_on_rows ? r0 + r : c0 + j);
+                store_any(p.c, p.c_dtype, (r0 + r) * p.c_r + (c0 + j) * p.c_c, v);
+            };
+            if (p.c_c == 1) {
+                for (int r = part * kScaleWarps + g; r < kTileRows; r += split * kScaleWarps)
+#pragma unroll
+                    for (int j = lane; j < BN; j += 32) put(r, j);
+            } else {
+                for (int j = part; j < BN; j += split) put(row_in_tile, j);
             }
         }
         __syncwarp();
-        cluster_sync();  // the others have read this CTA's part
+        if (split > 1) cluster_sync();  // the others have read this CTA's part
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -417,16 +521,17 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
 // each holds 128 rows of the row operand and 128 columns of the column
 // operand, so a block of K costs an SM 32 KB of loads for 512 cycles of its
 // tensor core, half of what 128 x 128 tiles of one CTA take.  A block's
-// accumulator is 256 TMEM columns, two of them alternate.  Eight scaling
-// warps per CTA, two for each quarter of the lanes, hold 128 columns of
-// running sums each in registers: 64 packed multiply-adds and 128 columns
-// of tcgen05.ld a block, under half of the 512 cycles.
+// accumulator is 256 TMEM columns, two of them alternate.  (Two halves of 128
+// columns with four buffers would be handed over more finely, but an MMA of
+// 128 columns is bound by its operands' shared-memory reads: 369 cycles for
+// the 256 of its arithmetic.)  Eight scaling warps per CTA, two for each
+// quarter of the lanes, hold 128 columns of running sums each in registers.
 //
 // full[s] lives in the even CTA and counts both CTAs' loads; the even CTA's
-// MMA thread commits empty[s] and tfull[a] to both CTAs; tempty[a] lives in
+// MMA warp commits empty[s] and tfull[a] to both CTAs; tempty[a] lives in
 // the even CTA and counts the pair's 16 scaling warps.
 constexpr int kPairScaleWarps = 8;
-constexpr int kPairThreads = 128 + 32 * kPairScaleWarps;  // warps 0 and 1 feed, 2 and 3 idle, 4.. scale
+constexpr int kPairThreads = 128 + 32 * kPairScaleWarps;  // warps 0 TMA, 1 MMA, 2 scales, 3 idle, 4.. scaling
 // 128 running sums and their temporaries do not fit the 168 registers that
 // 384 threads get each: the feeding warpgroup hands its own over,
 // 56 + 2 * 224 = 3 * 168.
@@ -434,7 +539,9 @@ constexpr int kPairFeedRegs = 56, kPairScaleRegs = 224;
 constexpr int kPairCols = 256;
 constexpr int kPairWarpCols = 128;  // columns of a scaling warp
 constexpr int kBoxBytes = 32 * 128;
+constexpr int kPairRingDepth = 8;
 
+template <bool CVEC>
 struct PairCfg {
     static constexpr int kRowBytes = kTileRows * kBlockK;
     static constexpr int kColBytes = 128 * kBlockK;
@@ -443,8 +550,8 @@ struct PairCfg {
     static constexpr int kAccs = 2;
     static constexpr int kTmemCols = kAccs * kPairCols;
     static constexpr int kStoreBytes = kPairScaleWarps * 2 * kBoxBytes;
-    static constexpr int kColScaleBytes = kPairScaleWarps * 2 * kPairWarpCols * 4;
-    static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kStoreBytes + kColScaleBytes + 1024;
+    using Ring = ScaleRing<kTileRows, kPairCols, CVEC, kPairRingDepth>;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + kStoreBytes + Ring::kBytes + 1024;
     static_assert(kSmemBytes <= 232448, "over the per-block shared memory limit");
 };
 
@@ -457,15 +564,6 @@ __device__ __forceinline__ void put_box_row(uint32_t box, int lane, const uint32
                      "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
                      : "memory");
     }
-}
-
-__device__ __forceinline__ uint32_t pack_16(float a, float b, int dtype) {
-    if (dtype == ST_F16) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // Row and column tile of tile t: 8 row tiles of a column tile after another,
@@ -483,14 +581,15 @@ template <bool R_MN, bool C_MN, bool CVEC>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
                          const __grid_constant__ CUtensorMap tmap_out, const Fp8Params p) {
-    using Cfg = PairCfg;
+    using Cfg = PairCfg<CVEC>;
+    using Ring = typename Cfg::Ring;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *boxes = smem + Cfg::kStages * Cfg::kStageBytes;
     uint64_t *bars = reinterpret_cast<uint64_t *>(boxes + Cfg::kStoreBytes);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * Cfg::kStages + 2 * Cfg::kAccs + 1);
+    constexpr int kBars = 2 * Cfg::kStages + 2 * Cfg::kAccs + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars + Ring::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    float *col_scale = reinterpret_cast<float *>(boxes + Cfg::kStoreBytes + kBarBytes);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -502,7 +601,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     auto empty_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };
     auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + a); };
     auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + Cfg::kAccs + a); };
-    const uint32_t drain_bar = bar0 + 8u * (2 * Cfg::kStages + 2 * Cfg::kAccs);
+    const uint32_t drain_bar = bar0 + 8u * (kBars - 1);
+    const Ring ring{reinterpret_cast<float *>(boxes + Cfg::kStoreBytes + kBarBytes), bar0 + 8u * kBars};
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
@@ -514,6 +614,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             mbar_init(tempty_bar(a), 2 * kPairScaleWarps);
         }
         mbar_init(drain_bar, 1);
+        ring.init(kPairScaleWarps);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -533,95 +634,110 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     pdl_begin();  // nothing above touches global memory
 
     if (warp < 4) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairFeedRegs));
-      if (warp == 0) {
-        // ------------------------------------------------ TMA producer (both CTAs)
-        if (lane == 0) {
-            const uint64_t pol = l2_policy_evict_last();
-            const uint32_t even_full0 = map_to_rank(full_bar(0), 0);
-            int s = 0, issued = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int t = pair; ok && t < tiles; t += pairs) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairFeedRegs));
+        if (warp == 0) {
+            // -------------------------------------------- TMA producer (both CTAs)
+            if (lane == 0) {
+                const uint64_t pol = l2_policy_evict_last();
+                const uint32_t even_full0 = map_to_rank(full_bar(0), 0);
+                int s = 0, issued = 0;
+                uint32_t ph = 0;
+                bool ok = true;
+                for (int t = pair; ok && t < tiles; t += pairs) {
+                    int tr, tc;
+                    pair_tile(p, t, tr, tc);
+                    const int r0 = tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows;
+                    const int c0 = tc * kPairCols + static_cast<int>(rank) * 128;
+                    for (int b = 0; b < p.k_blocks; ++b, ++issued) {
+                        if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
+                            ok = false;
+                            break;
+                        }
+                        if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * Cfg::kStageBytes);
+                        const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
+                        const uint32_t sc = sr + Cfg::kRowBytes;
+                        const uint32_t fb = even_full0 + 8u * s;
+                        const int k0 = b * kBlockK;
+                        if constexpr (R_MN) tma_load_2d_pair(sr, &tmap_r, fb, r0, k0, pol);
+                        else tma_load_2d_pair(sr, &tmap_r, fb, k0, r0, pol);
+                        if constexpr (C_MN) tma_load_2d_pair(sc, &tmap_c, fb, c0, k0, pol);
+                        else tma_load_2d_pair(sc, &tmap_c, fb, k0, c0, pol);
+                        if (++s == Cfg::kStages) {
+                            s = 0;
+                            ph ^= 1u;
+                        }
+                    }
+                }
+                if (!ok) {
+                    *abort_flag = 1;
+                    atomicExch(p.err, kDevAbortGemmProducer);
+                }
+                if (rank == 0) drain_ring(issued, Cfg::kStages, full_bar, p.timeout_ns);  // both CTAs' copies
+            }
+        } else if (warp == 1) {
+            // -------------------------------------------- MMA issuer (even CTA)
+            if (rank == 0) {
+                int s = 0, a = 0;
+                uint32_t ph = 0, aph = 0;
+                bool ok = true;
+                for (int t = pair; ok && t < tiles; t += pairs) {
+                    for (int b = 0; b < p.k_blocks; ++b) {
+                        const bool ready = mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns) &&
+                                           mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns);
+                        if (!__all_sync(0xffffffffu, ready)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after_sync();
+                        const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
+                        const uint32_t sc = sr + Cfg::kRowBytes;
+                        if (elect_one()) {
+#pragma unroll
+                            for (int ks = 0; ks < kBlockK / kMmaK; ++ks) {
+                                const uint64_t dr =
+                                    smem_desc_sw128(sr + ks * (R_MN ? kMmaK * 128 : kMmaK), R_MN ? 128 * 128 : 16, 1024);
+                                const uint64_t dc =
+                                    smem_desc_sw128(sc + ks * (C_MN ? kMmaK * 128 : kMmaK), C_MN ? 128 * 128 : 16, 1024);
+                                tc_mma_f8_pair(tmem_base + static_cast<uint32_t>(a * kPairCols), dr, dc, p.idesc,
+                                               ks != 0 ? 1u : 0u);
+                            }
+                            tc_commit_pair_multicast(empty_bar(s), 3);
+                            tc_commit_pair_multicast(tfull_bar(a), 3);
+                        }
+                        __syncwarp();
+                        if (++s == Cfg::kStages) {
+                            s = 0;
+                            ph ^= 1u;
+                        }
+                        if (++a == Cfg::kAccs) {
+                            a = 0;
+                            aph ^= 1u;
+                        }
+                    }
+                }
+                if (!ok) {
+                    *abort_flag = 1;
+                    atomicExch(p.err, kDevAbortGemmMma);
+                }
+                if (elect_one()) tc_commit_pair(drain_bar);
+                __syncwarp();
+                (void)mbar_wait(drain_bar, 0, abort_flag, p.timeout_ns);
+            }
+        } else if (warp == 2) {
+            // -------------------------------------------- scales (both CTAs)
+            int d = 0;
+            uint32_t dph = 0;
+            for (int t = pair; t < tiles; t += pairs) {
                 int tr, tc;
                 pair_tile(p, t, tr, tc);
-                const int r0 = tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows;
-                const int c0 = tc * kPairCols + static_cast<int>(rank) * 128;
-                for (int b = 0; b < p.k_blocks; ++b, ++issued) {
-                    if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
-                        ok = false;
-                        break;
-                    }
-                    if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * Cfg::kStageBytes);
-                    const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
-                    const uint32_t sc = sr + Cfg::kRowBytes;
-                    const uint32_t fb = even_full0 + 8u * s;
-                    const int k0 = b * kBlockK;
-                    if constexpr (R_MN) tma_load_2d_pair(sr, &tmap_r, fb, r0, k0, pol);
-                    else tma_load_2d_pair(sr, &tmap_r, fb, k0, r0, pol);
-                    if constexpr (C_MN) tma_load_2d_pair(sc, &tmap_c, fb, c0, k0, pol);
-                    else tma_load_2d_pair(sc, &tmap_c, fb, k0, c0, pol);
-                    if (++s == Cfg::kStages) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
+                if (!ring.load(p, tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows, tc * kPairCols, 0, p.k_blocks,
+                               lane, d, dph, abort_flag)) {
+                    *abort_flag = 1;
+                    break;
                 }
             }
-            if (!ok) {
-                *abort_flag = 1;
-                atomicExch(p.err, kDevAbortGemmProducer);
-            }
-            if (rank == 0) {  // the pair's copies have landed before it leaves, also after an abort
-                const volatile int never = 0;
-                for (int i = issued > Cfg::kStages ? issued - Cfg::kStages : 0; i < issued; ++i)
-                    (void)mbar_wait(full_bar(i % Cfg::kStages), static_cast<uint32_t>(i / Cfg::kStages) & 1u, &never,
-                                    p.timeout_ns);
-            }
+            copies_done();
         }
-    } else if (warp == 1) {
-        // ------------------------------------------------ MMA issuer (even CTA)
-        if (rank == 0 && lane == 0) {
-            int s = 0, a = 0;
-            uint32_t ph = 0, aph = 0;
-            bool ok = true;
-            for (int t = pair; ok && t < tiles; t += pairs) {
-                for (int b = 0; b < p.k_blocks; ++b) {
-                    if (!mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns) ||
-                        !mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after_sync();
-                    const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
-                    const uint32_t sc = sr + Cfg::kRowBytes;
-#pragma unroll
-                    for (int ks = 0; ks < kBlockK / kMmaK; ++ks) {
-                        const uint64_t dr =
-                            smem_desc_sw128(sr + ks * (R_MN ? kMmaK * 128 : kMmaK), R_MN ? 128 * 128 : 16, 1024);
-                        const uint64_t dc =
-                            smem_desc_sw128(sc + ks * (C_MN ? kMmaK * 128 : kMmaK), C_MN ? 128 * 128 : 16, 1024);
-                        tc_mma_f8_pair(tmem_base + static_cast<uint32_t>(a * kPairCols), dr, dc, p.idesc, ks != 0 ? 1u : 0u);
-                    }
-                    tc_commit_pair_multicast(empty_bar(s), 3);
-                    tc_commit_pair_multicast(tfull_bar(a), 3);
-                    if (++s == Cfg::kStages) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
-                    if (++a == Cfg::kAccs) {
-                        a = 0;
-                        aph ^= 1u;
-                    }
-                }
-            }
-            if (!ok) {
-                *abort_flag = 1;
-                atomicExch(p.err, kDevAbortGemmMma);
-            }
-            tc_commit_pair(drain_bar);
-            (void)mbar_wait(drain_bar, 0, abort_flag, p.timeout_ns);
-        }
-      }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairScaleRegs));
         // ------------------------------------------------ scaling warps (both CTAs)
@@ -629,48 +745,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const int half = e >> 2;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(half * kPairWarpCols);
         const uint32_t even_tempty0 = map_to_rank(tempty_bar(0), 0);
-        const uint32_t box0 = smem_addr(boxes) + static_cast<uint32_t>(e * 2 * kBoxBytes);
-        float *my_cols = col_scale + e * 2 * kPairWarpCols;
-        int a = 0, box = 0;
-        uint32_t aph = 0;
+        uint8_t *my_boxes = boxes + e * 2 * kBoxBytes;
+        int a = 0, box = 0, d = 0;
+        uint32_t aph = 0, dph = 0;
         bool ok = true;
         for (int t = pair; ok && t < tiles; t += pairs) {
-            int tr, tc;
-            pair_tile(p, t, tr, tc);
-            const int row0 = tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows + g * 32;
-            const int row = row0 + lane;
-            const int col0 = tc * kPairCols + half * kPairWarpCols;
-            const bool row_ok = row < p.rows;
-            const float *rs = p.rs + static_cast<int64_t>(row_ok ? row >> p.rs_shift : 0) * p.rs_i;
-            // the warp's column scale, or lane l's four (columns l, l + 32, ...)
-            const float *cs[4];
-            bool col_ok[4];
-#pragma unroll
-            for (int i = 0; i < (CVEC ? 4 : 1); ++i) {
-                const int c = col0 + lane + 32 * i;
-                col_ok[i] = CVEC ? c < p.cols : col0 < p.cols;
-                cs[i] = p.cs + static_cast<int64_t>(col_ok[i] ? (CVEC ? c : col0) >> p.cs_shift : 0) * p.cs_i;
-            }
             uint64_t acc[kPairWarpCols / 2];
 #pragma unroll
             for (int j = 0; j < kPairWarpCols / 2; ++j) acc[j] = 0;
-            float r_next = row_ok ? rs[0] : 0.0f, c_next[4];
-#pragma unroll
-            for (int i = 0; i < (CVEC ? 4 : 1); ++i) c_next[i] = col_ok[i] ? cs[i][0] : 0.0f;
             for (int b = 0; b < p.k_blocks; ++b) {
-                const float r_scale = r_next, c_scale = c_next[0];
-                float *buf = my_cols + (b & 1) * kPairWarpCols;
-                if constexpr (CVEC) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) buf[lane + 32 * i] = c_next[i];
-                    __syncwarp();
-                }
-                if (b + 1 < p.k_blocks) {  // the next block's scales arrive during this one
-                    r_next = row_ok ? rs[(b + 1) * p.rs_b] : 0.0f;
-#pragma unroll
-                    for (int i = 0; i < (CVEC ? 4 : 1); ++i) c_next[i] = col_ok[i] ? cs[i][(b + 1) * p.cs_b] : 0.0f;
-                }
-                const bool ready = mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns);
+                const bool ready = mbar_wait(ring.full(d), dph, abort_flag, p.timeout_ns) &&
+                                   mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns);
                 if (!__all_sync(0xffffffffu, ready)) {
                     *abort_flag = 1;
                     if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
@@ -678,55 +763,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     break;
                 }
                 tc_fence_after_sync();
-                const uint32_t tm = t_lane + static_cast<uint32_t>(a * kPairCols);
-                const float both = r_scale * c_scale;
-                const uint64_t s2 = CVEC ? pack2(r_scale, r_scale) : pack2(both, both);
-                // 16 columns are multiplied while the next 16 are read
-                uint32_t v[2][16];
-                tmem_load_16(tm, v[0]);
-#pragma unroll
-                for (int j = 0; j < kPairWarpCols / 16; ++j) {
-                    tmem_load_wait_16(v[j & 1]);
-                    if (j + 1 < kPairWarpCols / 16) tmem_load_16(tm + (j + 1) * 16, v[(j + 1) & 1]);
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const uint32_t(&x)[16] = v[j & 1];
-                        uint64_t &a0 = acc[8 * j + i / 2], &a1 = acc[8 * j + i / 2 + 1];
-                        if constexpr (CVEC) {
-                            const float4 c = *reinterpret_cast<const float4 *>(buf + 16 * j + i);
-                            fma2(a0, x[i], x[i + 1], mul2(s2, pack2(c.x, c.y)));
-                            fma2(a1, x[i + 2], x[i + 3], mul2(s2, pack2(c.z, c.w)));
-                        } else {
-                            fma2(a0, x[i], x[i + 1], s2);
-                            fma2(a1, x[i + 2], x[i + 3], s2);
+                scale_and_add<kPairWarpCols, CVEC, 32>(
+                    acc, t_lane + static_cast<uint32_t>(a * kPairCols), ring.rows(d)[g * 32 + lane],
+                    ring.cols(d) + half * (CVEC ? kPairWarpCols : 1), [&] {
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (rank == 0) mbar_arrive(tempty_bar(a));
+                            else mbar_arrive_cluster(even_tempty0 + 8u * a);
                         }
-                    }
-                }
-                tc_fence_before_sync();
+                    });
                 __syncwarp();
-                if (lane == 0) {
-                    if (rank == 0) mbar_arrive(tempty_bar(a));
-                    else mbar_arrive_cluster(even_tempty0 + 8u * a);
-                }
+                if (lane == 0) mbar_arrive(ring.empty(d));
                 if (++a == Cfg::kAccs) {
                     a = 0;
                     aph ^= 1u;
                 }
-            }
-            if (!ok) break;
-            // ---- bias, conversion, and out through two 32-row boxes of 128 bytes (TMA clips rows and 16-byte pieces at C's extents)
-            if (p.bias != nullptr) {
-#pragma unroll
-                for (int j = 0; j < kPairWarpCols / 2; ++j) {
-                    const int c = col0 + 2 * j;
-                    const float b0 = c < p.cols ? load_any(p.bias, p.bias_dtype, c) : 0.0f;
-                    const float b1 = c + 1 < p.cols ? load_any(p.bias, p.bias_dtype, c + 1) : 0.0f;
-                    acc[j] = pack2(lo2(acc[j]) + b0, hi2(acc[j]) + b1);
+                if (++d == kPairRingDepth) {
+                    d = 0;
+                    dph ^= 1u;
                 }
             }
+            if (!ok) break;
+            // ---- bias, conversion, and out through the warp's two boxes of 32 rows x 128 bytes
+            int tr, tc;
+            pair_tile(p, t, tr, tc);
+            const int row0 = tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows + g * 32;
+            const int col0 = tc * kPairCols + half * kPairWarpCols;
+            if (row0 >= p.rows) continue;
             if (p.staged) {
+                if (p.bias != nullptr) {
 #pragma unroll
-                for (int h = 0; h < kPairWarpCols / 32; ++h) {  // 32 columns a step
+                    for (int j = 0; j < kPairWarpCols / 2; ++j) {
+                        const int c = col0 + 2 * j;
+                        const float v0 = c < p.cols ? load_any(p.bias, p.bias_dtype, c) : 0.0f;
+                        const float v1 = c + 1 < p.cols ? load_any(p.bias, p.bias_dtype, c + 1) : 0.0f;
+                        acc[j] = pack2(lo2(acc[j]) + v0, hi2(acc[j]) + v1);
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < kPairWarpCols / 32; ++h) {  // a box: 32 columns of fp32, 64 of 16 bits
                     uint32_t w[32];
                     if (p.c_dtype == ST_F32) {
 #pragma unroll
@@ -737,30 +813,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     } else {
                         if (h & 1) continue;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            w[i] = pack_16(lo2(acc[(16 * h + i) % (kPairWarpCols / 2)]), hi2(acc[(16 * h + i) % (kPairWarpCols / 2)]),
-                                           p.c_dtype);
+                        for (int i = 0; i < 32; ++i) {
+                            const uint64_t v = acc[(16 * h + i) % (kPairWarpCols / 2)];
+                            w[i] = pack_16(lo2(v), hi2(v), p.c_dtype);
+                        }
                     }
-                    const int c = col0 + 32 * h;
-                    if (c >= p.cols || row0 >= p.rows) continue;
+                    if (col0 + 32 * h >= p.cols) continue;
                     if (lane == 0) bulk_wait_group_read<1>();  // the store that last used this box has read it
                     __syncwarp();
-                    const uint32_t at = box0 + static_cast<uint32_t>(box * kBoxBytes);
+                    const uint32_t at = smem_addr(my_boxes + box * kBoxBytes);
                     put_box_row(at, lane, w);
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&tmap_out, at, c, row0);
+                    if (lane == 0) {  // TMA clips the box at C's extents
+                        tma_store_2d(&tmap_out, at, col0 + 32 * h, row0);
                         bulk_commit_group();
                     }
                     box ^= 1;
                 }
-            } else if (row_ok) {
+            } else {  // 32 columns at a time through both boxes, then a row at a time with a lane per column
+                float *m = reinterpret_cast<float *>(my_boxes);
+                const int n = p.rows - row0 < 32 ? p.rows - row0 : 32;
 #pragma unroll
-                for (int j = 0; j < kPairWarpCols / 2; ++j) {
-                    const int c = col0 + 2 * j;
-                    if (c < p.cols) store_any(p.c, p.c_dtype, row * p.c_r + c, lo2(acc[j]));
-                    if (c + 1 < p.cols) store_any(p.c, p.c_dtype, row * p.c_r + c + 1, hi2(acc[j]));
+                for (int h = 0; h < kPairWarpCols / 32; ++h) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        m[lane * 33 + 2 * i] = lo2(acc[16 * h + i]);
+                        m[lane * 33 + 2 * i + 1] = hi2(acc[16 * h + i]);
+                    }
+                    __syncwarp();
+                    const int c = col0 + 32 * h + lane;
+                    if (c < p.cols) {
+                        const float add = p.bias != nullptr ? load_any(p.bias, p.bias_dtype, c) : 0.0f;
+                        for (int r = 0; r < n; ++r)
+                            store_any(p.c, p.c_dtype, (row0 + r) * p.c_r + c, p.bias != nullptr ? m[r * 33 + lane] + add : m[r * 33 + lane]);
+                    }
+                    __syncwarp();
                 }
             }
         }
@@ -852,7 +940,7 @@ int make_map_8(CUtensorMap *map, const void *base, int64_t inner, int64_t outer,
 
 template <int BN, bool R_MN, bool C_MN, bool CVEC>
 int launch_instance(const CUtensorMap &mr, const CUtensorMap &mc, const Fp8Params &p, cudaStream_t stream) {
-    using Cfg = Fp8Cfg<BN>;
+    using Cfg = Fp8Cfg<BN, CVEC>;
     auto kern = gemm_fp8_kernel<BN, R_MN, C_MN, CVEC>;
     static uint64_t attr_set = 0;  // one bit per device ordinal
     int dev = 0;
@@ -910,12 +998,12 @@ int launch_pair_instance(const CUtensorMap &mr, const CUtensorMap &mc, const CUt
     int dev = 0;
     ST_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !(attr_set & (1ull << dev))) {
-        ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg::kSmemBytes));
+        ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<CVEC>::kSmemBytes));
         if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
     }
     const int64_t tiles = static_cast<int64_t>(p.tiles_r) * p.tiles_c;
     const int64_t pairs = tiles < sm_count / 2 ? tiles : sm_count / 2;
-    ST_CUDA_TRY(launch_kernel(kern, static_cast<unsigned>(2 * pairs), kPairThreads, PairCfg::kSmemBytes, stream, mr, mc, mo, p));
+    ST_CUDA_TRY(launch_kernel(kern, static_cast<unsigned>(2 * pairs), kPairThreads, PairCfg<CVEC>::kSmemBytes, stream, mr, mc, mo, p));
     note_launch();
     const cudaError_t e = cudaPeekAtLastError();
     return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "gemm_fp8_pair_kernel launch");

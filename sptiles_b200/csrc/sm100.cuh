@@ -221,6 +221,20 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint
         : "memory");
 }
 
+// True in one lane of a converged warp.  A warp that keeps together and
+// issues its MMAs under this predicate holds their descriptors in uniform
+// registers; from one lane of a diverged warp four MMAs and their waits took
+// up to 766 cycles to issue, against the 512 that they run.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
 // Load 32 consecutive f32 columns of this thread's TMEM lane (32x32b shape:
 // thread t of the warp reads lane base+t).
 __device__ __forceinline__ void tmem_load_32(uint32_t taddr, uint32_t (&r)[32]) {
