@@ -87,6 +87,7 @@ constexpr int kDevAbortGemmProducer = 0x101;
 constexpr int kDevAbortGemmMma = 0x102;
 constexpr int kDevAbortGemmEpilogue = 0x103;
 constexpr int kDevAbortGemmStreamK = 0x104;  // a split tile's partial never arrived
+constexpr int kDevAbortNorm = 0x201;  // a row's copies never arrived
 constexpr int kDevAbortWaitCheckBarrier = 0x1f0;  // st_check_device_wait: mbarrier wait ran out
 constexpr int kDevAbortWaitCheckFlag = 0x1f1;     // st_check_device_wait: flag poll ran out
 
@@ -286,8 +287,10 @@ struct NormArgs {
     float *h_scale = nullptr;  // h is 8-bit: its scales per 1 x 128 block
     int64_t hs0 = 0, hs1 = 0;
     bool h_e5m2 = false, h_fp8 = false;
+    int *err = nullptr;  // set by the launcher
+    unsigned long long limit_ns = 0;
 };
-int launch_residual_norm(const NormArgs &args, int sm_count, cudaStream_t stream);
+int launch_residual_norm(const NormArgs &args, int sm_count, int *dev_err, uint64_t timeout_ns, cudaStream_t stream);
 
 struct NormBackwardArgs {
     int64_t rows, cols;

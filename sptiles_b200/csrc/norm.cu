@@ -20,12 +20,14 @@
 // The sums over rows are kept in registers by a fixed set of row groups, each
 // taking every G-th row, written once to a workspace and added in a fixed
 // order by a second launch: no atomics, the same bits on every run.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
 #include "common.h"
 #include "fp8.cuh"
+#include "sm100.cuh"
 
 namespace st {
 namespace {
@@ -158,6 +160,46 @@ struct RowGroup {
     __device__ __forceinline__ int64_t base(int v) const { return static_cast<int64_t>(v * warps + warp) * kChunk; }
 };
 
+// 8 elements of a row's normed copy, in the branch's type or as 8-bit blocks.
+template <typename TX, bool VEC>
+__device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int64_t base, int lane, const float (&h)[8]) {
+    if (!p.h_fp8) {
+        store8<TX, VEC>(static_cast<TX *>(p.h.p) + row * p.h.ld, base, lane, p.cols, h);
+        return;
+    }
+    // a chunk is two blocks of 128: VEC, 16 lanes each; otherwise the lanes' first and last four elements
+    const float limit = p.h_e5m2 ? 57344.0f : 448.0f;
+    uint32_t m[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m[VEC ? 0 : j / 4] = max(m[VEC ? 0 : j / 4], abs_bits(h[j]));
+    float inverse[2];
+#pragma unroll
+    for (int b = 0; b < (VEC ? 1 : 2); ++b) {
+#pragma unroll
+        for (int o = VEC ? 8 : 16; o > 0; o >>= 1) m[b] = max(m[b], __shfl_xor_sync(0xffffffffu, m[b], o));
+        const float scale = fp8_scale(m[b], limit);
+        inverse[b] = __fdiv_rn(1.0f, scale);
+        const int64_t block = base / 128 + (VEC ? lane / 16 : b);
+        if ((VEC ? lane % 16 : lane) == 0 && block * 128 < p.cols) p.h_scale[row * p.hs0 + block * p.hs1] = scale;
+    }
+    if constexpr (VEC) inverse[1] = inverse[0];
+    uint32_t q[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+        q[b] = to_fp8x4(__fmul_rn(h[4 * b], inverse[b]), __fmul_rn(h[4 * b + 1], inverse[b]),
+                        __fmul_rn(h[4 * b + 2], inverse[b]), __fmul_rn(h[4 * b + 3], inverse[b]), p.h_e5m2);
+    uint8_t *to = static_cast<uint8_t *>(p.h.p) + row * p.h.ld;
+    if (VEC && base + lane * 8 + 8 <= p.cols) {
+        *reinterpret_cast<uint2 *>(to + base + lane * 8) = make_uint2(q[0], q[1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t c = element<VEC>(base, lane, j);
+            if (c < p.cols) to[c] = static_cast<uint8_t>(q[j / 4] >> (8 * (j % 4)));
+        }
+    }
+}
+
 template <typename TX, typename TR, int VPT, bool VEC>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormArgs p, int warps) {
     pdl_wait();
@@ -225,42 +267,169 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormAr
             load8_of<TX, VEC>(p.pre, 0, base, g.lane, p.cols, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) r[v][j] *= inv * (w[j] + p.offset);
-            if (!p.h_fp8) {
-                store8<TX, VEC>(static_cast<TX *>(p.h.p) + row * p.h.ld, base, g.lane, p.cols, r[v]);
-                continue;
-            }
-            // a chunk is two blocks of 128: VEC, 16 lanes each; otherwise the lanes' first and last four elements
-            const float limit = p.h_e5m2 ? 57344.0f : 448.0f;
-            uint32_t m[2] = {0, 0};
+            store_normed<TX, VEC>(p, row, base, g.lane, r[v]);
+        }
+    }
+    pdl_trigger();
+}
+
+// ---------------------------------------------------------------- many rows on 16-byte boundaries
+// Persistent CTAs, each taking every G-th row: rows of x and r arrive by bulk
+// copies in a ring of shared memory, S rows ahead, so that what is in flight
+// does not depend on registers or on where the row before stands between its
+// two sums; the weights stay in registers over the rows, folded into one
+// factor per element and norm.
+struct RowRing {
+    uint32_t bar0;
+    uint8_t *data;
+    int stages, stage_bytes;
+    volatile int *abort_flag;
+    int *err;
+    uint64_t limit_ns;
+    __device__ __forceinline__ void init() const {
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < stages; ++s) mbar_init(bar0 + 8u * s, 1);
+            *abort_flag = 0;
+            fence_barrier_init();
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ uint8_t *stage(int s) const { return data + s * stage_bytes; }
+    // One thread: begin the copies of stage s (`bytes` in all).
+    __device__ __forceinline__ void expect(int s, uint32_t bytes) const { mbar_arrive_expect_tx(bar0 + 8u * s, bytes); }
+    __device__ __forceinline__ void copy(int s, int at, const void *src, uint32_t bytes) const {
+        bulk_load(smem_addr(data) + static_cast<uint32_t>(s * stage_bytes + at), src, bytes, bar0 + 8u * s);
+    }
+    // Every thread: a wait that ran out is recorded and lets the CTA run on
+    // (all later waits return at once), so that no barrier is missed.
+    __device__ __forceinline__ void wait(int s, uint32_t parity) const {
+        if (mbar_wait(bar0 + 8u * s, parity, abort_flag, limit_ns)) return;
+        if (*abort_flag == 0) atomicExch(err, kDevAbortNorm);
+        *abort_flag = 1;
+    }
+};
+
+constexpr int kMaxStages = 8;
+
+template <typename T>
+__device__ __forceinline__ void read8(const uint8_t *row, int64_t col, float (&f)[8]) {
+    uint4 w[sizeof(T) / 2];
+    const uint4 *src = reinterpret_cast<const uint4 *>(row + col * static_cast<int64_t>(sizeof(T)));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m[VEC ? 0 : j / 4] = max(m[VEC ? 0 : j / 4], abs_bits(r[v][j]));
-            float inverse[2];
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = src[i];
+    const T *e = reinterpret_cast<const T *>(w);
 #pragma unroll
-            for (int b = 0; b < (VEC ? 1 : 2); ++b) {
+    for (int j = 0; j < 8; ++j) f[j] = to_float(e[j]);
+}
+
+template <typename TX, typename TR, int VPT>
+__global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const NormArgs p, int warps, int stages) {
+    extern __shared__ __align__(128) uint8_t ring_smem[];
+    __shared__ float slots[2 * 3 * 32];
+    __shared__ uint64_t bars[kMaxStages];
+    __shared__ int aborted;
+    const RowGroup g(warps);
+    const int x_bytes = static_cast<int>(p.cols * sizeof(TX)), r_bytes = static_cast<int>(p.cols * sizeof(TR));
+    const int r_at = (x_bytes + 127) / 128 * 128;
+    const RowRing ring{smem_addr(bars), ring_smem, stages, r_at + (r_bytes + 127) / 128 * 128, &aborted, p.err, p.limit_ns};
+    ring.init();
+    pdl_wait();
+    auto fetch = [&](int s, int64_t row) {
+        ring.expect(s, static_cast<uint32_t>(x_bytes + r_bytes));
+        ring.copy(s, 0, static_cast<const TX *>(p.x.p) + row * p.x.ld, static_cast<uint32_t>(x_bytes));
+        ring.copy(s, r_at, static_cast<const TR *>(p.r.p) + row * p.r.ld, static_cast<uint32_t>(r_bytes));
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages; ++s)
+            if (g.first + s * g.step < p.rows) fetch(s, g.first + s * g.step);
+
+    const float inv_cols = 1.0f / static_cast<float>(p.cols);
+    // branch factor alpha * gate * (post + offset), norm factor pre + offset
+    float c1[VPT][8], c2[VPT][8];
 #pragma unroll
-                for (int o = VEC ? 8 : 16; o > 0; o >>= 1) m[b] = max(m[b], __shfl_xor_sync(0xffffffffu, m[b], o));
-                const float scale = fp8_scale(m[b], limit);
-                inverse[b] = __fdiv_rn(1.0f, scale);
-                const int64_t block = base / 128 + (VEC ? g.lane / 16 : b);
-                if ((VEC ? g.lane % 16 : g.lane) == 0 && block * 128 < p.cols)
-                    p.h_scale[row * p.hs0 + block * p.hs1] = scale;
-            }
-            if constexpr (VEC) inverse[1] = inverse[0];
-            uint32_t q[2];
+    for (int v = 0; v < VPT; ++v) {
+        float w[8];
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-                q[b] = to_fp8x4(__fmul_rn(r[v][4 * b], inverse[b]), __fmul_rn(r[v][4 * b + 1], inverse[b]),
-                                __fmul_rn(r[v][4 * b + 2], inverse[b]), __fmul_rn(r[v][4 * b + 3], inverse[b]), p.h_e5m2);
-            uint8_t *h = static_cast<uint8_t *>(p.h.p) + row * p.h.ld;
-            if (VEC && base + g.lane * 8 + 8 <= p.cols) {
-                *reinterpret_cast<uint2 *>(h + base + g.lane * 8) = make_uint2(q[0], q[1]);
+        for (int j = 0; j < 8; ++j) c1[v][j] = p.alpha;
+        if (p.post.p != nullptr) {
+            load8_of<TX, true>(p.post, 0, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c1[v][j] *= w[j] + p.offset;
+        }
+        if (p.gate_mode == kGateChannel) {
+            load8_of<TX, true>(p.gate, 0, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c1[v][j] *= w[j];
+        }
+        if (p.pre.p != nullptr) load8_of<TX, true>(p.pre, 0, g.base(v), g.lane, p.cols, c2[v]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c2[v][j] += p.offset;
+    }
+
+    int slot = 0, s = 0;
+    uint32_t ph = 0;
+    for (int64_t row = g.first; row < p.rows; row += g.step) {
+        float x[VPT][8], r[VPT][8];
+        float token = 1.0f;
+        if (p.gate_mode == kGateToken) token = load1_of<TX>(p.gate, row);
+        ring.wait(s, ph);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int64_t c = g.base(v) + g.lane * 8;
+            if (c < p.cols) {
+                read8<TX>(ring.stage(s), c, x[v]);
+                read8<TR>(ring.stage(s) + r_at, c, r[v]);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int64_t c = element<VEC>(base, g.lane, j);
-                    if (c < p.cols) h[c] = static_cast<uint8_t>(q[j / 4] >> (8 * (j % 4)));
-                }
+                for (int j = 0; j < 8; ++j) x[v][j] = r[v][j] = 0.0f;
             }
+        }
+        bool refill = row + stages * g.step < p.rows;  // once every thread has read the stage
+        auto refilled = [&] {
+            if (refill && threadIdx.x == 0) fetch(s, row + stages * g.step);
+            refill = false;
+        };
+        float inv = token;
+        if (p.post.p != nullptr) {
+            float sum[1] = {0.0f};
+#pragma unroll
+            for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[0] += x[v][j] * x[v][j];
+            row_sum(sum, g.warps, g.warp, g.lane, slots, slot);
+            refilled();
+            inv = token / sqrtf(sum[0] * inv_cols + p.eps);
+        }
+        float sum[1] = {0.0f};
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            if (p.gate_mode == kGateFull) {
+                float w[8];
+                load8_of<TX, true>(p.gate, row, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[v][j] *= w[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                r[v][j] += x[v][j] * inv * c1[v][j];
+                sum[0] += r[v][j] * r[v][j];
+            }
+            store8<TR, true>(static_cast<TR *>(p.r_out.p) + row * p.r_out.ld, g.base(v), g.lane, p.cols, r[v]);
+        }
+        if (p.pre.p != nullptr) {
+            row_sum(sum, g.warps, g.warp, g.lane, slots, slot);
+            refilled();
+            const float inv_r = 1.0f / sqrtf(sum[0] * inv_cols + p.eps);
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[v][j] *= inv_r * c2[v][j];
+                store_normed<TX, true>(p, row, g.base(v), g.lane, r[v]);
+            }
+        }
+        if (++s == stages) {
+            s = 0;
+            ph ^= 1u;
         }
     }
     pdl_trigger();
@@ -529,6 +698,39 @@ int forward_vpt(const NormArgs &p, const Shape &s, bool vec, cudaStream_t stream
     return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "residual_norm_kernel");
 }
 
+// Rows in flight of the ring kernels: as many stages of a row's bytes as fit beside the other CTAs of an SM.
+template <typename Kern, typename... Args>
+int launch_rows(Kern kern, uint64_t &attr_set, int threads, int stage_bytes, int64_t rows, int sm_count, cudaStream_t stream,
+                int *groups, Args... args) {
+    constexpr int kMostSmem = 200 * 1024;
+    int dev = 0;
+    ST_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !(attr_set & (1ull << dev))) {
+        ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
+        if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
+    }
+    const int per_sm = threads <= 256 ? 2 : 1;  // 128 registers a thread
+    int stages = kMostSmem / per_sm / stage_bytes;
+    stages = stages > 4 ? 4 : stages;
+    const int64_t ctas = rows < sm_count * per_sm ? rows : sm_count * per_sm;
+    if (groups != nullptr) *groups = static_cast<int>(ctas);
+    ST_CUDA_TRY(launch_kernel(kern, static_cast<unsigned>(ctas), threads, static_cast<size_t>(stages) * stage_bytes, stream,
+                              args..., stages));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "norm rows kernel");
+}
+
+int row_bytes(int64_t cols, size_t size) { return static_cast<int>((cols * size + 127) / 128 * 128); }
+
+template <typename TX, typename TR, int VPT>
+int forward_rows(const NormArgs &p, const Shape &s, int sm_count, cudaStream_t stream) {
+    static uint64_t attr_set = 0;  // one bit per device ordinal
+    return launch_rows(residual_norm_rows_kernel<TX, TR, VPT>, attr_set, s.threads,
+                       row_bytes(p.cols, sizeof(TX)) + row_bytes(p.cols, sizeof(TR)), p.rows, sm_count, stream, nullptr, p,
+                       s.warps);
+}
+
 template <typename TX, typename TR>
 int forward_typed(const NormArgs &p, int sm_count, cudaStream_t stream) {
     auto side = [](const NormView &v) { return v.dtype == ST_F32 ? sizeof(float) : sizeof(TX); };
@@ -539,6 +741,9 @@ int forward_typed(const NormArgs &p, int sm_count, cudaStream_t stream) {
                      (p.gate_mode == kGateToken ||
                       aligned_rows(p.gate, p.gate_mode == kGateFull ? p.rows : 1, side(p.gate), 16));
     const Shape s = shape_of(p.rows, p.cols, int64_t(1) << 30, p.rows < sm_count);
+    if (vec && p.x.p != nullptr && (p.post.p != nullptr || p.pre.p != nullptr) && p.cols % 8 == 0 && s.warps > 1 && s.vpt <= 2 &&
+        p.rows >= 2 * sm_count)
+        return s.vpt == 1 ? forward_rows<TX, TR, 1>(p, s, sm_count, stream) : forward_rows<TX, TR, 2>(p, s, sm_count, stream);
     if (s.vpt == 1) return forward_vpt<TX, TR, 1>(p, s, vec, stream);
     if (s.vpt == 2) return forward_vpt<TX, TR, 2>(p, s, vec, stream);
     return forward_vpt<TX, TR, 4>(p, s, vec, stream);
@@ -606,7 +811,10 @@ int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) 
 
 }  // namespace
 
-int launch_residual_norm(const NormArgs &p, int sm_count, cudaStream_t stream) {
+int launch_residual_norm(const NormArgs &args, int sm_count, int *dev_err, uint64_t timeout_ns, cudaStream_t stream) {
+    NormArgs p = args;
+    p.err = dev_err;
+    p.limit_ns = timeout_ns;
     if (p.rows == 0) return ST_OK;
     if (p.cols > kMaxCols) return fail(ST_ERR_UNSUPPORTED, "residual_norm: at most 16384 columns");
     const int tx = p.x.p != nullptr ? p.x.dtype : (p.h.p != nullptr && !p.h_fp8 ? p.h.dtype : p.r.dtype);

@@ -1668,7 +1668,7 @@ int st_residual_norm(st_ctx *ctx, const st_tensor *x_in, const st_tensor *residu
     ExecCtx x;
     ST_TRY(resolve_exec(ctx, exec, &x));
     DeviceGuard guard(x.dev->ordinal);
-    ST_TRY(launch_residual_norm(g, x.dev->sm_count, x.stream));
+    ST_TRY(launch_residual_norm(g, x.dev->sm_count, x.dev->dev_err, kDeviceWaitLimitNs, x.stream));
     return finish(x);
 }
 

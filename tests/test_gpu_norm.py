@@ -321,3 +321,23 @@ def test_norm_into_product():
     assert ((y.double() - want).abs() <= (128 + 4 + 5) * 2.0 ** -23 * mass).all()
     z = st.residual_norm(y[:, :n].to(BF16), torch.zeros(rows, n, device=DEV), torch.ones(n, device=DEV))
     assert torch.isfinite(z.residual).all() and z.normed is None
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("tx,tr", [(F32, F32), (F16, F16), (BF16, F32)], ids=["f32", "f16", "bf16_f32"])
+@pytest.mark.parametrize("rows,cols", [(700, 1024), (1601, 520), (500, 5000), (333, 8192)], ids=lambda v: str(v))
+def test_forward_many_rows(rows, cols, tx, tr, gate):
+    """Enough rows for every persistent CTA to take several, on 16-byte boundaries."""
+    d = inputs(rows, cols, tx, tr, gate, True, True, seed=3)
+    check_forward(d, quantize=True)
+    check_forward(d, offset=1.0)
+
+
+@pytest.mark.parametrize("post,pre", [(True, False), (False, True)])
+def test_forward_many_rows_parts(post, pre):
+    check_forward(inputs(900, 768, BF16, BF16, "channel", post, pre, seed=4))
+    d = inputs(900, 768, BF16, BF16, "channel", post, pre, seed=4)
+    g = dev(d)
+    want = st.residual_norm(g["x"], g["r"], g["post"], g["gate"], g["pre"])
+    got = st.residual_norm(g["x"], g["r"], g["post"], g["gate"], g["pre"], out=g["r"])  # in place
+    assert torch.equal(got.residual, want.residual) and got.residual is g["r"]
