@@ -169,16 +169,16 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
     }
     // a chunk is two blocks of 128: VEC, 16 lanes each; otherwise the lanes' first and last four elements
     const float limit = p.h_e5m2 ? 57344.0f : 448.0f;
-    uint32_t m[2] = {0, 0};
+    float m[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m[VEC ? 0 : j / 4] = max(m[VEC ? 0 : j / 4], abs_bits(h[j]));
+    for (int j = 0; j < 8; j += 2) m[VEC ? 0 : j / 4] = max_abs(m[VEC ? 0 : j / 4], h[j], h[j + 1]);
     float inverse[2];
 #pragma unroll
     for (int b = 0; b < (VEC ? 1 : 2); ++b) {
 #pragma unroll
-        for (int o = VEC ? 8 : 16; o > 0; o >>= 1) m[b] = max(m[b], __shfl_xor_sync(0xffffffffu, m[b], o));
+        for (int o = VEC ? 8 : 16; o > 0; o >>= 1) m[b] = max_abs(m[b], __shfl_xor_sync(0xffffffffu, m[b], o));
         const float scale = fp8_scale(m[b], limit);
-        inverse[b] = __fdiv_rn(1.0f, scale);
+        inverse[b] = __frcp_rn(scale);
         const int64_t block = base / 128 + (VEC ? lane / 16 : b);
         if ((VEC ? lane % 16 : lane) == 0 && block * 128 < p.cols) p.h_scale[row * p.hs0 + block * p.hs1] = scale;
     }
@@ -312,26 +312,62 @@ struct RowRing {
 constexpr int kMaxStages = 8;
 
 template <typename T>
-__device__ __forceinline__ void read8(const uint8_t *row, int64_t col, float (&f)[8]) {
+__device__ __forceinline__ void read8(const uint8_t *row, int col, uint64_t (&f)[4]) {
     uint4 w[sizeof(T) / 2];
-    const uint4 *src = reinterpret_cast<const uint4 *>(row + col * static_cast<int64_t>(sizeof(T)));
+    const uint4 *src = reinterpret_cast<const uint4 *>(row + col * static_cast<int>(sizeof(T)));
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = src[i];
-    const T *e = reinterpret_cast<const T *>(w);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = to_float(e[j]);
+    unpack8(w, f, T{});
 }
 
-template <typename TX, typename TR, int VPT>
-__global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const NormArgs p, int warps, int stages) {
+template <typename T>
+__device__ __forceinline__ void write8(T *dst, const uint64_t (&f)[4]) {
+    uint4 w[sizeof(T) / 2];
+    pack8(f, w, T{});
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4 *>(dst)[i] = w[i];
+}
+
+__device__ __forceinline__ uint64_t twice(float v) { return pack2(v, v); }
+
+// Sums of N values over the warps of a CTA (more than one warp); every thread
+// adds the warps' parts itself.
+template <int N>
+__device__ __forceinline__ void cta_sum(float (&v)[N], int warps, int warp, int lane, float4 *slots, int &slot) {
+    float *mine = reinterpret_cast<float *>(slots + slot * N * 4);
+    slot ^= 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) mine[i * 16 + warp] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (4 * q >= warps) break;
+            const float4 s = reinterpret_cast<const float4 *>(mine)[i * 4 + q];  // slots past the last warp stay 0
+            v[i] += (s.x + s.y) + (s.z + s.w);
+        }
+    }
+}
+
+template <typename TX, typename TR, int VPT, int MAX_THREADS>
+__global__ void __launch_bounds__(MAX_THREADS) residual_norm_rows_kernel(const NormArgs p, int warps, int stages) {
     extern __shared__ __align__(128) uint8_t ring_smem[];
-    __shared__ float slots[2 * 3 * 32];
+    __shared__ float4 slots[2 * 4];
     __shared__ uint64_t bars[kMaxStages];
     __shared__ int aborted;
     const RowGroup g(warps);
-    const int x_bytes = static_cast<int>(p.cols * sizeof(TX)), r_bytes = static_cast<int>(p.cols * sizeof(TR));
+    const int cols = static_cast<int>(p.cols);
+    const int x_bytes = cols * static_cast<int>(sizeof(TX)), r_bytes = cols * static_cast<int>(sizeof(TR));
     const int r_at = (x_bytes + 127) / 128 * 128;
     const RowRing ring{smem_addr(bars), ring_smem, stages, r_at + (r_bytes + 127) / 128 * 128, &aborted, p.err, p.limit_ns};
+    if (threadIdx.x < 32) reinterpret_cast<float *>(slots)[threadIdx.x] = 0.0f;
     ring.init();
     pdl_wait();
     auto fetch = [&](int s, int64_t row) {
@@ -344,87 +380,116 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
             if (g.first + s * g.step < p.rows) fetch(s, g.first + s * g.step);
 
     const float inv_cols = 1.0f / static_cast<float>(p.cols);
+    const bool has_post = p.post.p != nullptr, has_pre = p.pre.p != nullptr;
     // branch factor alpha * gate * (post + offset), norm factor pre + offset
-    float c1[VPT][8], c2[VPT][8];
+    uint64_t c1[VPT][4], c2[VPT][4];
+    int col[VPT];
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-        float w[8];
+        col[v] = static_cast<int>(g.base(v)) + g.lane * 8;
+        float f[8], w[8] = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) c1[v][j] = p.alpha;
-        if (p.post.p != nullptr) {
+        for (int j = 0; j < 8; ++j) f[j] = p.alpha;
+        if (has_post) {
             load8_of<TX, true>(p.post, 0, g.base(v), g.lane, p.cols, w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) c1[v][j] *= w[j] + p.offset;
+            for (int j = 0; j < 8; ++j) f[j] *= w[j] + p.offset;
         }
         if (p.gate_mode == kGateChannel) {
             load8_of<TX, true>(p.gate, 0, g.base(v), g.lane, p.cols, w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) c1[v][j] *= w[j];
+            for (int j = 0; j < 8; ++j) f[j] *= w[j];
         }
-        if (p.pre.p != nullptr) load8_of<TX, true>(p.pre, 0, g.base(v), g.lane, p.cols, c2[v]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) c2[v][j] += p.offset;
+        for (int j = 0; j < 4; ++j) c1[v][j] = pack2(f[2 * j], f[2 * j + 1]);
+        if (has_pre) load8_of<TX, true>(p.pre, 0, g.base(v), g.lane, p.cols, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c2[v][j] = pack2(w[2 * j] + p.offset, w[2 * j + 1] + p.offset);
     }
 
     int slot = 0, s = 0;
     uint32_t ph = 0;
     for (int64_t row = g.first; row < p.rows; row += g.step) {
-        float x[VPT][8], r[VPT][8];
+        uint64_t x[VPT][4], r[VPT][4];
         float token = 1.0f;
         if (p.gate_mode == kGateToken) token = load1_of<TX>(p.gate, row);
         ring.wait(s, ph);
+        const uint8_t *stage = ring.stage(s);
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            const int64_t c = g.base(v) + g.lane * 8;
-            if (c < p.cols) {
-                read8<TX>(ring.stage(s), c, x[v]);
-                read8<TR>(ring.stage(s) + r_at, c, r[v]);
+            if (col[v] < cols) {
+                read8<TX>(stage, col[v], x[v]);
+                read8<TR>(stage + r_at, col[v], r[v]);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[v][j] = r[v][j] = 0.0f;
+                for (int j = 0; j < 4; ++j) x[v][j] = r[v][j] = 0;
             }
         }
-        bool refill = row + stages * g.step < p.rows;  // once every thread has read the stage
+        bool refill = threadIdx.x == 0 && row + stages * g.step < p.rows;  // once every thread has read the stage
         auto refilled = [&] {
-            if (refill && threadIdx.x == 0) fetch(s, row + stages * g.step);
+            if (refill) fetch(s, row + stages * g.step);
             refill = false;
         };
         float inv = token;
-        if (p.post.p != nullptr) {
-            float sum[1] = {0.0f};
+        if (has_post) {
+            uint64_t a = 0;
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sum[0] += x[v][j] * x[v][j];
-            row_sum(sum, g.warps, g.warp, g.lane, slots, slot);
+                for (int j = 0; j < 4; ++j) a = fma2(x[v][j], x[v][j], a);
+            float sum[1] = {lo2(a) + hi2(a)};
+            cta_sum(sum, g.warps, g.warp, g.lane, slots, slot);
             refilled();
-            inv = token / sqrtf(sum[0] * inv_cols + p.eps);
+            inv = token * rsqrtf(sum[0] * inv_cols + p.eps);
         }
-        float sum[1] = {0.0f};
+        const uint64_t inv2 = twice(inv);
+        uint64_t a = 0;
+        TR *to = static_cast<TR *>(p.r_out.p) + row * p.r_out.ld;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             if (p.gate_mode == kGateFull) {
                 float w[8];
                 load8_of<TX, true>(p.gate, row, g.base(v), g.lane, p.cols, w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[v][j] *= w[j];
+                for (int j = 0; j < 4; ++j) x[v][j] = mul2(x[v][j], pack2(w[2 * j], w[2 * j + 1]));
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                r[v][j] += x[v][j] * inv * c1[v][j];
-                sum[0] += r[v][j] * r[v][j];
+            for (int j = 0; j < 4; ++j) {
+                r[v][j] = fma2(mul2(x[v][j], c1[v][j]), inv2, r[v][j]);
+                a = fma2(r[v][j], r[v][j], a);
             }
-            store8<TR, true>(static_cast<TR *>(p.r_out.p) + row * p.r_out.ld, g.base(v), g.lane, p.cols, r[v]);
+            if (col[v] < cols) write8<TR>(to + col[v], r[v]);
         }
-        if (p.pre.p != nullptr) {
-            row_sum(sum, g.warps, g.warp, g.lane, slots, slot);
+        if (has_pre) {
+            float sum[1] = {lo2(a) + hi2(a)};
+            cta_sum(sum, g.warps, g.warp, g.lane, slots, slot);
             refilled();
-            const float inv_r = 1.0f / sqrtf(sum[0] * inv_cols + p.eps);
+            const uint64_t inv_r = twice(rsqrtf(sum[0] * inv_cols + p.eps));
+            float top[VPT];
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
+                top[v] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) r[v][j] *= inv_r * c2[v][j];
-                store_normed<TX, true>(p, row, g.base(v), g.lane, r[v]);
+                for (int j = 0; j < 4; ++j) {
+                    r[v][j] = mul2(mul2(r[v][j], c2[v][j]), inv_r);
+                    top[v] = max_abs(top[v], lo2(r[v][j]), hi2(r[v][j]));
+                }
+                if (!p.h_fp8 && col[v] < cols) write8<TX>(static_cast<TX *>(p.h.p) + row * p.h.ld + col[v], r[v]);
+            }
+            if (p.h_fp8) {
+                uint8_t *h = static_cast<uint8_t *>(p.h.p) + row * p.h.ld;
+#pragma unroll
+                for (int v = 0; v < VPT; ++v) {  // 16 lanes hold a block of 128
+#pragma unroll
+                    for (int o = 8; o > 0; o >>= 1) top[v] = max_abs(top[v], __shfl_xor_sync(0xffffffffu, top[v], o));
+                    const float scale = fp8_scale(top[v], p.h_e5m2 ? 57344.0f : 448.0f);
+                    const float inverse = __frcp_rn(scale);
+                    if (col[v] < cols) {
+                        if (g.lane % 16 == 0) p.h_scale[row * p.hs0 + (col[v] >> 7) * p.hs1] = scale;
+                        *reinterpret_cast<uint2 *>(h + col[v]) =
+                            p.h_e5m2 ? to_fp8x8<true>(r[v], inverse) : to_fp8x8<false>(r[v], inverse);
+                    }
+                }
             }
         }
         if (++s == stages) {
@@ -723,10 +788,10 @@ int launch_rows(Kern kern, uint64_t &attr_set, int threads, int stage_bytes, int
 
 int row_bytes(int64_t cols, size_t size) { return static_cast<int>((cols * size + 127) / 128 * 128); }
 
-template <typename TX, typename TR, int VPT>
+template <typename TX, typename TR, int VPT, int MAX_THREADS>
 int forward_rows(const NormArgs &p, const Shape &s, int sm_count, cudaStream_t stream) {
     static uint64_t attr_set = 0;  // one bit per device ordinal
-    return launch_rows(residual_norm_rows_kernel<TX, TR, VPT>, attr_set, s.threads,
+    return launch_rows(residual_norm_rows_kernel<TX, TR, VPT, MAX_THREADS>, attr_set, s.threads,
                        row_bytes(p.cols, sizeof(TX)) + row_bytes(p.cols, sizeof(TR)), p.rows, sm_count, stream, nullptr, p,
                        s.warps);
 }
@@ -741,9 +806,10 @@ int forward_typed(const NormArgs &p, int sm_count, cudaStream_t stream) {
                      (p.gate_mode == kGateToken ||
                       aligned_rows(p.gate, p.gate_mode == kGateFull ? p.rows : 1, side(p.gate), 16));
     const Shape s = shape_of(p.rows, p.cols, int64_t(1) << 30, p.rows < sm_count);
-    if (vec && p.x.p != nullptr && (p.post.p != nullptr || p.pre.p != nullptr) && p.cols % 8 == 0 && s.warps > 1 && s.vpt <= 2 &&
+    if (vec && p.x.p != nullptr && p.r_out.p != nullptr && (p.post.p != nullptr || p.pre.p != nullptr) && p.cols % 8 == 0 && s.warps > 1 && s.vpt == 2 &&
         p.rows >= 2 * sm_count)
-        return s.vpt == 1 ? forward_rows<TX, TR, 1>(p, s, sm_count, stream) : forward_rows<TX, TR, 2>(p, s, sm_count, stream);
+        return s.threads <= 256 ? forward_rows<TX, TR, 2, 256>(p, s, sm_count, stream)
+                                : forward_rows<TX, TR, 2, 512>(p, s, sm_count, stream);
     if (s.vpt == 1) return forward_vpt<TX, TR, 1>(p, s, vec, stream);
     if (s.vpt == 2) return forward_vpt<TX, TR, 2>(p, s, vec, stream);
     return forward_vpt<TX, TR, 4>(p, s, vec, stream);

@@ -7,9 +7,8 @@
 // machine that computes them this way.  A NaN or infinity in a block makes
 // its scale NaN or infinite, and every product that reads the block NaN.
 //
-// One CTA takes a tile of 128 columns and up to 128 rows: 16 threads of 8
-// columns across, 16 rows down, the tile in registers between the maximum
-// and the conversion, so that the input is read once.
+// The input is read once and stays in registers between a block's maximum and
+// its conversion.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -21,174 +20,249 @@
 namespace st {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kTile = 128;
 
-template <typename T>
-struct Vec8 {
-    uint4 w[sizeof(T) / 2];  // 8 elements: one 16-byte word, two for fp32
-};
+// ---------------------------------------------------------------- 1 x 128 blocks on 16-byte rows
+// A warp takes four rows of 256 columns, 8 columns a lane: 2 KB of 16-bit
+// input in flight per warp, 16 lanes a block.  The four rows' maxima are
+// reduced together, each exchange halving the rows that a lane still carries
+// (5 shuffles for the 16 of four separate reductions), so that each lane ends
+// with one row's maximum and does one division pair for it.
+constexpr int kRowThreads = 128;
 
-template <typename T>
-__device__ __forceinline__ void unpack8(const Vec8<T> &v, float (&f)[8]) {
-    const T *e = reinterpret_cast<const T *>(&v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = to_float(e[j]);
-}
-
-enum : int { kRowBlocks = 0, kColumnBlocks = 1, kSquareBlocks = 2 };  // 1 x 128, 128 x 1, 128 x 128
-
-// NROWS rows per thread: 16 * NROWS rows a tile.  VEC: unit column stride
-// with rows on 16-byte boundaries of a and 8-byte boundaries of q; otherwise
-// a thread's columns are 16 apart, which keeps a warp's loads together.
-template <typename T, int MODE, int NROWS, bool VEC>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs p) {
+template <typename T, bool E5M2>
+__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const QuantizeArgs p, uint32_t chunks) {
     pdl_wait();
-    __shared__ uint32_t red[MODE == kColumnBlocks ? 16 * kTile : 16];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t col_tiles = (p.cols + kTile - 1) / kTile;
-    const int64_t tile_r = blockIdx.x / col_tiles, tile_c = blockIdx.x % col_tiles;
-    const int64_t r0 = tile_r * (16 * NROWS), c0 = tile_c * kTile;
-    const T *a = static_cast<const T *>(p.a);
-    auto column = [&](int j) { return c0 + (VEC ? tx * 8 + j : tx + 16 * j); };
-
-    float x[NROWS][8];
-    const bool whole = VEC && c0 + tx * 8 + 8 <= p.cols;
-    if (whole) {
-        Vec8<T> v[NROWS];
+    const uint32_t unit = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t rg = unit / chunks, chunk = unit - rg * chunks;
+    const int64_t row0 = static_cast<int64_t>(rg) * 4;
+    if (row0 >= p.rows) return;
+    const int lane = threadIdx.x & 31;
+    const int col = static_cast<int>(chunk) * 256 + lane * 8, cols = static_cast<int>(p.cols);
+    const int here = p.rows - row0 < 4 ? static_cast<int>(p.rows - row0) : 4;
+    const bool whole = col + 8 <= cols;
+    constexpr int kWords = static_cast<int>(sizeof(T) / 2);
+    const T *src = static_cast<const T *>(p.a) + row0 * p.sa0 + col;
+    uint4 raw[4][kWords];
 #pragma unroll
-        for (int i = 0; i < NROWS; ++i) {
-            const int64_t r = r0 + ty + 16 * i;
-            v[i] = Vec8<T>{};
-            if (r < p.rows) {
-                const uint4 *src = reinterpret_cast<const uint4 *>(a + r * p.sa0 + c0 + tx * 8);
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int w = 0; w < static_cast<int>(sizeof(T) / 2); ++w) v[i].w[w] = __ldcs(src + w);
-            }
-        }
+        for (int w = 0; w < kWords; ++w) raw[i][w] = make_uint4(0, 0, 0, 0);
+        if (i < here && whole) {
 #pragma unroll
-        for (int i = 0; i < NROWS; ++i) unpack8(v[i], x[i]);
-    } else {
+            for (int w = 0; w < kWords; ++w) raw[i][w] = __ldcs(reinterpret_cast<const uint4 *>(src + i * p.sa0) + w);
+        } else if (i < here) {
+            T *e = reinterpret_cast<T *>(raw[i]);
 #pragma unroll
-        for (int i = 0; i < NROWS; ++i) {
-            const int64_t r = r0 + ty + 16 * i;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int64_t c = column(j);
-                x[i][j] = r < p.rows && c < p.cols ? to_float(a[r * p.sa0 + c * p.sa1]) : 0.0f;
-            }
+            for (int j = 0; j < 8; ++j)
+                if (col + j < cols) e[j] = src[i * p.sa0 + j];
         }
     }
-
-    // maxima as bit patterns of |x|: order preserving, and a NaN wins
-    const float limit = p.e5m2 ? 57344.0f : 448.0f;
-    float inv[MODE == kColumnBlocks ? 8 : NROWS];
-    if constexpr (MODE == kRowBlocks) {
+    float m[4];
 #pragma unroll
-        for (int i = 0; i < NROWS; ++i) {
-            uint32_t m = 0;
+    for (int i = 0; i < 4; ++i) {
+        uint64_t f[4];
+        unpack8(raw[i], f, T{});
+        m[i] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, abs_bits(x[i][j]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float s = fp8_scale(m, limit);
-            inv[i] = __fdiv_rn(1.0f, s);
-            const int64_t r = r0 + ty + 16 * i;
-            if (tx == 0 && r < p.rows) p.scale[r * p.ss0 + tile_c * p.ss1] = s;
-        }
-    } else if constexpr (MODE == kColumnBlocks) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < NROWS; ++i) m = max(m, abs_bits(x[i][j]));
-            red[ty * kTile + static_cast<int>(column(j) - c0)] = m;
-        }
-        __syncthreads();
-        if (threadIdx.x < kTile) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int t = 0; t < 16; ++t) m = max(m, red[t * kTile + threadIdx.x]);
-            const float s = fp8_scale(m, limit);
-            const int64_t c = c0 + threadIdx.x;
-            if (c < p.cols) p.scale[tile_r * p.ss0 + c * p.ss1] = s;
-            red[threadIdx.x] = __float_as_uint(__fdiv_rn(1.0f, s));
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) inv[j] = __uint_as_float(red[static_cast<int>(column(j) - c0)]);
-    } else {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < NROWS; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, abs_bits(x[i][j]));
-        m = __reduce_max_sync(0xffffffffu, m);
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-        __syncthreads();
-        m = 0;
-#pragma unroll
-        for (int t = 0; t < kThreads / 32; ++t) m = max(m, red[t]);
-        const float s = fp8_scale(m, limit);
-        if (threadIdx.x == 0) p.scale[tile_r * p.ss0 + tile_c * p.ss1] = s;
-        const float v = __fdiv_rn(1.0f, s);
-#pragma unroll
-        for (int i = 0; i < NROWS; ++i) inv[i] = v;
+        for (int j = 0; j < 4; ++j) m[i] = max_abs(m[i], lo2(f[j]), hi2(f[j]));
     }
-
-    uint8_t *q = static_cast<uint8_t *>(p.q);
+    const bool up = lane & 8, odd = lane & 4;
+    float k0 = up ? m[2] : m[0], k1 = up ? m[3] : m[1];
+    k0 = max_abs(k0, __shfl_xor_sync(0xffffffffu, up ? m[0] : m[2], 8));
+    k1 = max_abs(k1, __shfl_xor_sync(0xffffffffu, up ? m[1] : m[3], 8));
+    float k = max_abs(odd ? k1 : k0, __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 4));
+    k = max_abs(k, __shfl_xor_sync(0xffffffffu, k, 2));
+    k = max_abs(k, __shfl_xor_sync(0xffffffffu, k, 1));
+    const float scale = fp8_scale(k, E5M2 ? 57344.0f : 448.0f);
+    const float inverse = __frcp_rn(scale);
+    const int mine = (lane >> 2) & 3, block = static_cast<int>(chunk) * 2 + (lane >> 4);
+    if ((lane & 3) == 0 && mine < here && block * kTile < cols) p.scale[(row0 + mine) * p.ss0 + block * p.ss1] = scale;
+    uint8_t *q = static_cast<uint8_t *>(p.q) + row0 * p.sq0 + col;
 #pragma unroll
-    for (int i = 0; i < NROWS; ++i) {
-        const int64_t r = r0 + ty + 16 * i;
-        if (r >= p.rows) continue;
-        uint32_t w[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float y[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (MODE == kColumnBlocks) y[j] = __fmul_rn(x[i][4 * h + j], inv[4 * h + j]);
-                else y[j] = __fmul_rn(x[i][4 * h + j], inv[i]);
-            }
-            w[h] = to_fp8x4(y[0], y[1], y[2], y[3], p.e5m2);
-        }
+    for (int i = 0; i < 4; ++i) {
+        const float inv = __shfl_sync(0xffffffffu, inverse, (lane & 16) | (i * 4));
+        uint64_t f[4];
+        unpack8(raw[i], f, T{});
+        const uint2 c = to_fp8x8<E5M2>(f, inv);
+        if (i >= here) continue;
         if (whole) {
-            *reinterpret_cast<uint2 *>(q + r * p.sq0 + c0 + tx * 8) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2 *>(q + i * p.sq0) = c;
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int64_t c = column(j);
-                if (c < p.cols) q[r * p.sq0 + c * p.sq1] = static_cast<uint8_t>(w[j / 4] >> (8 * (j % 4)));
-            }
+            for (int j = 0; j < 8; ++j)
+                if (col + j < cols) q[i * p.sq0 + j] = static_cast<uint8_t>((j < 4 ? c.x : c.y) >> (8 * (j % 4)));
         }
     }
     pdl_trigger();
 }
 
-template <typename T, int MODE, int NROWS>
-int launch_mode(const QuantizeArgs &p, bool vec, cudaStream_t stream) {
-    const int64_t grid = cdiv(p.rows, 16 * NROWS) * cdiv(p.cols, kTile);
-    if (grid > INT32_MAX) return fail(ST_ERR_UNSUPPORTED, "quantize_fp8: too many blocks");
-    const unsigned g = static_cast<unsigned>(grid);
-    if (vec) ST_CUDA_TRY(launch_kernel(quantize_kernel<T, MODE, NROWS, true>, g, kThreads, 0, stream, p));
-    else ST_CUDA_TRY(launch_kernel(quantize_kernel<T, MODE, NROWS, false>, g, kThreads, 0, stream, p));
+// ---------------------------------------------------------------- tiles of 128 columns
+// The other blocks, and any stride: a CTA takes 128 columns and 32 * NROWS
+// rows, 16 threads of 8 columns across, 32 rows down.
+constexpr int kTileThreads = 512;
+constexpr int kDown = kTileThreads / 16;
+
+enum : int { kRowBlocks = 0, kColumnBlocks = 1, kSquareBlocks = 2 };  // 1 x 128, 128 x 1, 128 x 128
+// How a thread reads its 8 columns: as 16-byte words (rows of a on 16-byte,
+// of q on 8-byte boundaries); one by one, 16 apart, so that neighbouring
+// threads read neighbouring elements; the same with any column stride.
+enum : int { kWordsAccess = 0, kUnitAccess = 1, kAnyAccess = 2 };
+
+template <typename T, int MODE, int NROWS, int ACCESS>
+__global__ void __launch_bounds__(kTileThreads) quantize_tiles_kernel(const QuantizeArgs p, uint32_t col_tiles) {
+    pdl_wait();
+    __shared__ float red[MODE == kColumnBlocks ? kDown * kTile : kTileThreads / 32];
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const uint32_t tile_r = blockIdx.x / col_tiles, tile_c = blockIdx.x - tile_r * col_tiles;
+    const int64_t r0 = static_cast<int64_t>(tile_r) * (kDown * NROWS) + ty;
+    const int c0 = static_cast<int>(tile_c) * kTile, left = static_cast<int>(p.cols) - c0;  // columns from c0 on
+    auto column = [&](int j) { return ACCESS == kWordsAccess ? tx * 8 + j : tx + 16 * j; };
+    const T *a = static_cast<const T *>(p.a) + c0 * p.sa1;
+    const bool whole = ACCESS == kWordsAccess && tx * 8 + 8 <= left;
+
+    uint64_t x[NROWS][4];
+#pragma unroll
+    for (int i = 0; i < NROWS; ++i) {
+        const int64_t r = r0 + kDown * i;
+        const T *row = a + r * p.sa0;
+        if (whole) {
+            constexpr int kWords = static_cast<int>(sizeof(T) / 2);
+            uint4 w[kWords];
+#pragma unroll
+            for (int k = 0; k < kWords; ++k)
+                w[k] = r < p.rows ? __ldcs(reinterpret_cast<const uint4 *>(row + tx * 8) + k) : make_uint4(0, 0, 0, 0);
+            unpack8(w, x[i], T{});
+        } else {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                f[j] = r < p.rows && column(j) < left ? to_float(row[ACCESS == kAnyAccess ? column(j) * p.sa1 : column(j)]) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i][j] = pack2(f[2 * j], f[2 * j + 1]);
+        }
+    }
+
+    const float limit = p.e5m2 ? 57344.0f : 448.0f;
+    float inv[MODE == kColumnBlocks ? 8 : NROWS];
+    if constexpr (MODE == kRowBlocks) {
+#pragma unroll
+        for (int i = 0; i < NROWS; ++i) {
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m = max_abs(m, lo2(x[i][j]), hi2(x[i][j]));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const float s = fp8_scale(m, limit);
+            inv[i] = __frcp_rn(s);
+            const int64_t r = r0 + kDown * i;
+            if (tx == 0 && r < p.rows) p.scale[r * p.ss0 + tile_c * p.ss1] = s;
+        }
+    } else if constexpr (MODE == kColumnBlocks) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NROWS; ++i) m = max_abs(m, j & 1 ? hi2(x[i][j / 2]) : lo2(x[i][j / 2]));
+            red[ty * kTile + column(j)] = m;
+        }
+        __syncthreads();
+        if (threadIdx.x < kTile) {
+            float m = 0.0f;
+#pragma unroll
+            for (int t = 0; t < kDown; t += 2)
+                m = max_abs(m, red[t * kTile + threadIdx.x], red[(t + 1) * kTile + threadIdx.x]);
+            const float s = fp8_scale(m, limit);
+            if (static_cast<int>(threadIdx.x) < left) p.scale[tile_r * p.ss0 + (c0 + static_cast<int>(threadIdx.x)) * p.ss1] = s;
+            red[threadIdx.x] = __frcp_rn(s);  // read by the others only after the barrier
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) inv[j] = red[column(j)];
+    } else {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NROWS; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m = max_abs(m, lo2(x[i][j]), hi2(x[i][j]));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+        __syncthreads();
+        m = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kTileThreads / 32; t += 2) m = max_abs(m, red[t], red[t + 1]);
+        const float s = fp8_scale(m, limit);
+        if (threadIdx.x == 0) p.scale[tile_r * p.ss0 + tile_c * p.ss1] = s;
+        const float v = __frcp_rn(s);
+#pragma unroll
+        for (int i = 0; i < NROWS; ++i) inv[i] = v;
+    }
+
+    uint8_t *q = static_cast<uint8_t *>(p.q) + c0 * p.sq1;
+#pragma unroll
+    for (int i = 0; i < NROWS; ++i) {
+        const int64_t r = r0 + kDown * i;
+        if (r >= p.rows) continue;
+        uint64_t y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            y[j] = MODE == kColumnBlocks ? mul2(x[i][j], pack2(inv[2 * j], inv[2 * j + 1])) : mul2(x[i][j], pack2(inv[i], inv[i]));
+        const uint2 c = p.e5m2 ? to_fp8x8<true>(y, 1.0f) : to_fp8x8<false>(y, 1.0f);
+        uint8_t *to = q + r * p.sq0;
+        if (whole) {
+            *reinterpret_cast<uint2 *>(to + tx * 8) = c;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (column(j) < left)
+                    to[ACCESS == kAnyAccess ? column(j) * p.sq1 : column(j)] =
+                        static_cast<uint8_t>((j < 4 ? c.x : c.y) >> (8 * (j % 4)));
+        }
+    }
+    pdl_trigger();
+}
+
+int checked(const char *what) {
     note_launch();
     const cudaError_t e = cudaPeekAtLastError();
-    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "quantize_kernel");
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), what);
+}
+
+template <typename T, int MODE, int NROWS>
+int launch_tiles(const QuantizeArgs &p, int access, cudaStream_t stream) {
+    const int64_t col_tiles = cdiv(p.cols, kTile), grid = cdiv(p.rows, kDown * NROWS) * col_tiles;
+    if (grid > INT32_MAX) return fail(ST_ERR_UNSUPPORTED, "quantize_fp8: too many blocks");
+    const unsigned g = static_cast<unsigned>(grid);
+    const uint32_t ct = static_cast<uint32_t>(col_tiles);
+    if (access == kWordsAccess)
+        ST_CUDA_TRY(launch_kernel(quantize_tiles_kernel<T, MODE, NROWS, kWordsAccess>, g, kTileThreads, 0, stream, p, ct));
+    else if (access == kUnitAccess)
+        ST_CUDA_TRY(launch_kernel(quantize_tiles_kernel<T, MODE, NROWS, kUnitAccess>, g, kTileThreads, 0, stream, p, ct));
+    else
+        ST_CUDA_TRY(launch_kernel(quantize_tiles_kernel<T, MODE, NROWS, kAnyAccess>, g, kTileThreads, 0, stream, p, ct));
+    return checked("quantize_tiles_kernel");
 }
 
 template <typename T>
 int launch_typed(const QuantizeArgs &p, cudaStream_t stream) {
-    const bool vec = p.sa1 == 1 && p.sq1 == 1 && reinterpret_cast<uintptr_t>(p.a) % 16 == 0 &&
-                     (p.rows == 1 || p.sa0 * static_cast<int64_t>(sizeof(T)) % 16 == 0) &&
-                     reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.rows == 1 || p.sq0 % 8 == 0);
-    if (p.block_rows == 1) {
-        // row blocks need no common tile: few rows stay spread over many CTAs
-        if (p.rows <= 1024) return launch_mode<T, kRowBlocks, 1>(p, vec, stream);
-        return launch_mode<T, kRowBlocks, 4>(p, vec, stream);
+    const bool unit = p.sa1 == 1 && p.sq1 == 1;
+    const bool words = unit && reinterpret_cast<uintptr_t>(p.a) % 16 == 0 &&
+                       (p.rows == 1 || p.sa0 * static_cast<int64_t>(sizeof(T)) % 16 == 0) &&
+                       reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.rows == 1 || p.sq0 % 8 == 0);
+    const int access = words ? kWordsAccess : unit ? kUnitAccess : kAnyAccess;
+    if (p.block_rows == 1 && words) {
+        const int64_t chunks = cdiv(p.cols, 256), units = cdiv(p.rows, 4) * chunks;
+        if (units > INT32_MAX) return fail(ST_ERR_UNSUPPORTED, "quantize_fp8: too many blocks");
+        const unsigned g = static_cast<unsigned>(cdiv(units, kRowThreads / 32));
+        const uint32_t ch = static_cast<uint32_t>(chunks);
+        if (p.e5m2) ST_CUDA_TRY(launch_kernel(quantize_rows_kernel<T, true>, g, kRowThreads, 0, stream, p, ch));
+        else ST_CUDA_TRY(launch_kernel(quantize_rows_kernel<T, false>, g, kRowThreads, 0, stream, p, ch));
+        return checked("quantize_rows_kernel");
     }
-    if (p.block_cols == 1) return launch_mode<T, kColumnBlocks, 8>(p, vec, stream);
-    return launch_mode<T, kSquareBlocks, 8>(p, vec, stream);
+    if (p.block_rows == 1) return launch_tiles<T, kRowBlocks, 1>(p, access, stream);
+    if (p.block_cols == 1) return launch_tiles<T, kColumnBlocks, 4>(p, access, stream);
+    return launch_tiles<T, kSquareBlocks, 4>(p, access, stream);
 }
 
 }  // namespace
