@@ -301,8 +301,11 @@ struct NormBackwardArgs {
     int gate_mode = kGateNone;
     NormView dx, dr, dgate;  // dgate: rows x cols (full) or float per row / column
     float *dpost = nullptr, *dpre = nullptr;
+    int *err = nullptr;  // set by the launcher
+    unsigned long long limit_ns = 0;
 };
 int64_t residual_norm_backward_workspace(int64_t rows, int64_t cols);
-int launch_residual_norm_backward(const NormBackwardArgs &args, void *workspace, int sm_count, cudaStream_t stream);
+int launch_residual_norm_backward(const NormBackwardArgs &args, void *workspace, int *dev_err, uint64_t timeout_ns,
+                                  cudaStream_t stream);
 
 }  // namespace st

@@ -330,11 +330,12 @@ __device__ __forceinline__ void write8(T *dst, const uint64_t (&f)[4]) {
 
 __device__ __forceinline__ uint64_t twice(float v) { return pack2(v, v); }
 
-// Sums of N values over the warps of a CTA (more than one warp); every thread
-// adds the warps' parts itself.
-template <int N>
+// Sums of N values over the warps of a CTA; every thread adds the warps'
+// parts itself.  MOST: the largest N of the kernel's calls, whose two buffers
+// `slots` holds.
+template <int MOST, int N>
 __device__ __forceinline__ void cta_sum(float (&v)[N], int warps, int warp, int lane, float4 *slots, int &slot) {
-    float *mine = reinterpret_cast<float *>(slots + slot * N * 4);
+    float *mine = reinterpret_cast<float *>(slots + slot * MOST * 4);
     slot ^= 1;
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -356,13 +357,32 @@ __device__ __forceinline__ void cta_sum(float (&v)[N], int warps, int warp, int 
     }
 }
 
-template <typename TX, typename TR, int VPT, int MAX_THREADS>
-__global__ void __launch_bounds__(MAX_THREADS) residual_norm_rows_kernel(const NormArgs p, int warps, int stages) {
+// Maxima of four blocks that 16 lanes hold each: every exchange halves the
+// blocks that a lane still carries, so a lane ends with the maximum of block
+// (lane >> 2) & 3 of its half warp.
+__device__ __forceinline__ float max_of_four(const float (&m)[4], int lane) {
+    const bool up = lane & 8, odd = lane & 4;
+    float k0 = up ? m[2] : m[0], k1 = up ? m[3] : m[1];
+    k0 = max_abs(k0, __shfl_xor_sync(0xffffffffu, up ? m[0] : m[2], 8));
+    k1 = max_abs(k1, __shfl_xor_sync(0xffffffffu, up ? m[1] : m[3], 8));
+    float k = max_abs(odd ? k1 : k0, __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 4));
+    k = max_abs(k, __shfl_xor_sync(0xffffffffu, k, 2));
+    return max_abs(k, __shfl_xor_sync(0xffffffffu, k, 1));
+}
+
+constexpr int kRowVecs = 4;  // chunks of 8 elements a thread: its share of the sums' and scales' cost stays small
+
+// x is read twice from its stage instead of being kept: at 128 registers with
+// both factors and r in them, 16 warps of an SM are at work.
+template <typename TX, typename TR>
+__global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const NormArgs p, int warps, int stages) {
+    constexpr int VPT = kRowVecs;
     extern __shared__ __align__(128) uint8_t ring_smem[];
     __shared__ float4 slots[2 * 4];
     __shared__ uint64_t bars[kMaxStages];
     __shared__ int aborted;
-    const RowGroup g(warps);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t first = blockIdx.x, step = gridDim.x;
     const int cols = static_cast<int>(p.cols);
     const int x_bytes = cols * static_cast<int>(sizeof(TX)), r_bytes = cols * static_cast<int>(sizeof(TR));
     const int r_at = (x_bytes + 127) / 128 * 128;
@@ -377,7 +397,7 @@ __global__ void __launch_bounds__(MAX_THREADS) residual_norm_rows_kernel(const N
     };
     if (threadIdx.x == 0)
         for (int s = 0; s < stages; ++s)
-            if (g.first + s * g.step < p.rows) fetch(s, g.first + s * g.step);
+            if (first + s * step < p.rows) fetch(s, first + s * step);
 
     const float inv_cols = 1.0f / static_cast<float>(p.cols);
     const bool has_post = p.post.p != nullptr, has_pre = p.pre.p != nullptr;
@@ -386,84 +406,79 @@ __global__ void __launch_bounds__(MAX_THREADS) residual_norm_rows_kernel(const N
     int col[VPT];
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-        col[v] = static_cast<int>(g.base(v)) + g.lane * 8;
+        const int base = (v * warps + warp) * kChunk;
+        col[v] = base + lane * 8;
         float f[8], w[8] = {};
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = p.alpha;
         if (has_post) {
-            load8_of<TX, true>(p.post, 0, g.base(v), g.lane, p.cols, w);
+            load8_of<TX, true>(p.post, 0, base, lane, p.cols, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] *= w[j] + p.offset;
         }
         if (p.gate_mode == kGateChannel) {
-            load8_of<TX, true>(p.gate, 0, g.base(v), g.lane, p.cols, w);
+            load8_of<TX, true>(p.gate, 0, base, lane, p.cols, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] *= w[j];
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) c1[v][j] = pack2(f[2 * j], f[2 * j + 1]);
-        if (has_pre) load8_of<TX, true>(p.pre, 0, g.base(v), g.lane, p.cols, w);
+        if (has_pre) load8_of<TX, true>(p.pre, 0, base, lane, p.cols, w);
 #pragma unroll
         for (int j = 0; j < 4; ++j) c2[v][j] = pack2(w[2 * j] + p.offset, w[2 * j + 1] + p.offset);
     }
 
     int slot = 0, s = 0;
     uint32_t ph = 0;
-    for (int64_t row = g.first; row < p.rows; row += g.step) {
-        uint64_t x[VPT][4], r[VPT][4];
+    for (int64_t row = first; row < p.rows; row += step) {
         float token = 1.0f;
         if (p.gate_mode == kGateToken) token = load1_of<TX>(p.gate, row);
         ring.wait(s, ph);
         const uint8_t *stage = ring.stage(s);
-#pragma unroll
-        for (int v = 0; v < VPT; ++v) {
-            if (col[v] < cols) {
-                read8<TX>(stage, col[v], x[v]);
-                read8<TR>(stage + r_at, col[v], r[v]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[v][j] = r[v][j] = 0;
-            }
-        }
-        bool refill = threadIdx.x == 0 && row + stages * g.step < p.rows;  // once every thread has read the stage
-        auto refilled = [&] {
-            if (refill) fetch(s, row + stages * g.step);
-            refill = false;
-        };
         float inv = token;
         if (has_post) {
             uint64_t a = 0;
 #pragma unroll
-            for (int v = 0; v < VPT; ++v)
+            for (int v = 0; v < VPT; ++v) {
+                if (col[v] >= cols) continue;
+                uint64_t x[4];
+                read8<TX>(stage, col[v], x);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) a = fma2(x[v][j], x[v][j], a);
+                for (int j = 0; j < 4; ++j) a = fma2(x[j], x[j], a);
+            }
             float sum[1] = {lo2(a) + hi2(a)};
-            cta_sum(sum, g.warps, g.warp, g.lane, slots, slot);
-            refilled();
+            cta_sum<1>(sum, warps, warp, lane, slots, slot);
             inv = token * rsqrtf(sum[0] * inv_cols + p.eps);
         }
         const uint64_t inv2 = twice(inv);
-        uint64_t a = 0;
+        uint64_t a = 0, r[VPT][4];
         TR *to = static_cast<TR *>(p.r_out.p) + row * p.r_out.ld;
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[v][j] = 0;
+            if (col[v] >= cols) continue;
+            uint64_t x[4];
+            read8<TX>(stage, col[v], x);
+            read8<TR>(stage + r_at, col[v], r[v]);
             if (p.gate_mode == kGateFull) {
                 float w[8];
-                load8_of<TX, true>(p.gate, row, g.base(v), g.lane, p.cols, w);
+                load8_of<TX, true>(p.gate, row, (v * warps + warp) * kChunk, lane, p.cols, w);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[v][j] = mul2(x[v][j], pack2(w[2 * j], w[2 * j + 1]));
+                for (int j = 0; j < 4; ++j) x[j] = mul2(x[j], pack2(w[2 * j], w[2 * j + 1]));
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                r[v][j] = fma2(mul2(x[v][j], c1[v][j]), inv2, r[v][j]);
+                r[v][j] = fma2(mul2(x[j], c1[v][j]), inv2, r[v][j]);
                 a = fma2(r[v][j], r[v][j], a);
             }
-            if (col[v] < cols) write8<TR>(to + col[v], r[v]);
+            write8<TR>(to + col[v], r[v]);
         }
+        float sum[1] = {lo2(a) + hi2(a)};
+        cta_sum<1>(sum, warps, warp, lane, slots, slot);
+        // every thread has read the stage: the next row that it is for may come in
+        if (threadIdx.x == 0 && row + stages * step < p.rows) fetch(s, row + stages * step);
         if (has_pre) {
-            float sum[1] = {lo2(a) + hi2(a)};
-            cta_sum(sum, g.warps, g.warp, g.lane, slots, slot);
-            refilled();
             const uint64_t inv_r = twice(rsqrtf(sum[0] * inv_cols + p.eps));
             float top[VPT];
 #pragma unroll
@@ -476,19 +491,18 @@ __global__ void __launch_bounds__(MAX_THREADS) residual_norm_rows_kernel(const N
                 }
                 if (!p.h_fp8 && col[v] < cols) write8<TX>(static_cast<TX *>(p.h.p) + row * p.h.ld + col[v], r[v]);
             }
-            if (p.h_fp8) {
+            if (p.h_fp8) {  // 16 lanes hold a block of 128
                 uint8_t *h = static_cast<uint8_t *>(p.h.p) + row * p.h.ld;
+                const float scale = fp8_scale(max_of_four(top, lane), p.h_e5m2 ? 57344.0f : 448.0f);
+                const float inverse = __frcp_rn(scale);
+                const int mine = (lane >> 2) & 3;
+                const int block = (mine * warps + warp) * 2 + (lane >> 4);
+                if ((lane & 3) == 0 && block * 128 < cols) p.h_scale[row * p.hs0 + block * p.hs1] = scale;
 #pragma unroll
-                for (int v = 0; v < VPT; ++v) {  // 16 lanes hold a block of 128
-#pragma unroll
-                    for (int o = 8; o > 0; o >>= 1) top[v] = max_abs(top[v], __shfl_xor_sync(0xffffffffu, top[v], o));
-                    const float scale = fp8_scale(top[v], p.h_e5m2 ? 57344.0f : 448.0f);
-                    const float inverse = __frcp_rn(scale);
-                    if (col[v] < cols) {
-                        if (g.lane % 16 == 0) p.h_scale[row * p.hs0 + (col[v] >> 7) * p.hs1] = scale;
-                        *reinterpret_cast<uint2 *>(h + col[v]) =
-                            p.h_e5m2 ? to_fp8x8<true>(r[v], inverse) : to_fp8x8<false>(r[v], inverse);
-                    }
+                for (int v = 0; v < VPT; ++v) {
+                    const float k = __shfl_sync(0xffffffffu, inverse, (lane & 16) | (v * 4));
+                    if (col[v] < cols)
+                        *reinterpret_cast<uint2 *>(h + col[v]) = p.h_e5m2 ? to_fp8x8<true>(r[v], k) : to_fp8x8<false>(r[v], k);
                 }
             }
         }
@@ -692,34 +706,245 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
     pdl_trigger();
 }
 
-// out[c] = sum over groups of sums[g][c], in a fixed order; blockIdx.y picks the plane.
-__global__ void __launch_bounds__(256) column_sums_kernel(const float *sums, int64_t groups, int64_t cols, float *out0,
-                                                          float *out1, float *out2) {
+// Backward for many rows on 16-byte boundaries, as residual_norm_rows_kernel:
+// a ring of rows of x, dh, r and dr', the factors and the sums over rows in
+// registers.  With X = x * inv_x and c1 = alpha * gate * (post + offset) (the
+// gate only where it is a channel's; a token's or element's is g), one sum
+// over rows S = sum dr * X * g serves dpost = alpha * gate * S and a channel's
+// dgate = alpha * (post + offset) * S, and one over the row, sum dr * X * c1
+// (times an element's g), the mean in dx and a token's dgate.
+constexpr int kBackVecs = 2;
+
+template <typename TX, typename TR>
+__global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kernel(const NormBackwardArgs p, int warps,
+                                                                                  const Planes planes, float *out,
+                                                                                  int stages) {
+    constexpr int VPT = kBackVecs;
+    extern __shared__ __align__(128) uint8_t ring_smem[];
+    __shared__ float4 slots[2 * 3 * 4];
+    __shared__ uint64_t bars[kMaxStages];
+    __shared__ int aborted;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t first = blockIdx.x, step = gridDim.x;
+    const int cols = static_cast<int>(p.cols);
+    const bool has_x = p.x.p != nullptr, has_post = p.post.p != nullptr, has_pre = p.pre.p != nullptr;
+    const bool has_dr = p.d_residual.p != nullptr;
+    const uint32_t x_bytes = static_cast<uint32_t>(cols) * sizeof(TX), r_bytes = static_cast<uint32_t>(cols) * sizeof(TR);
+    const int x_room = (x_bytes + 127) / 128 * 128, r_room = (r_bytes + 127) / 128 * 128;
+    const int dh_at = has_x ? x_room : 0, r_at = dh_at + (has_pre ? x_room : 0), dr_at = r_at + (has_pre ? r_room : 0);
+    const RowRing ring{smem_addr(bars), ring_smem, stages, dr_at + (has_dr ? r_room : 0), &aborted, p.err, p.limit_ns};
+    if (threadIdx.x < 32)
+        for (int i = 0; i < 3; ++i) reinterpret_cast<float *>(slots)[threadIdx.x + 32 * i] = 0.0f;
+    ring.init();
     pdl_wait();
-    float *out = blockIdx.y == 0 ? out0 : blockIdx.y == 1 ? out1 : out2;
-    __shared__ float part[8][33];
-    {
-        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-        const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
-        const float *src = sums + blockIdx.y * groups * cols + c;
-        float s = 0.0f;
-        if (c < cols)
-            for (int64_t i = ty; i < groups; i += 8) s += src[i * cols];
-        part[ty][tx] = s;
-        __syncthreads();
-        if (ty == 0 && c < cols) {
-#pragma unroll
-            for (int i = 1; i < 8; ++i) s += part[i][tx];
-            out[c] = s;
+    auto fetch = [&](int s, int64_t row) {
+        ring.expect(s, (has_x ? x_bytes : 0) + (has_pre ? x_bytes + r_bytes : 0) + (has_dr ? r_bytes : 0));
+        if (has_x) ring.copy(s, 0, static_cast<const TX *>(p.x.p) + row * p.x.ld, x_bytes);
+        if (has_pre) {
+            ring.copy(s, dh_at, static_cast<const TX *>(p.d_normed.p) + row * p.d_normed.ld, x_bytes);
+            ring.copy(s, r_at, static_cast<const TR *>(p.r.p) + row * p.r.ld, r_bytes);
         }
+        if (has_dr) ring.copy(s, dr_at, static_cast<const TR *>(p.d_residual.p) + row * p.d_residual.ld, r_bytes);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages; ++s)
+            if (first + s * step < p.rows) fetch(s, first + s * step);
+
+    const float inv_cols = 1.0f / static_cast<float>(p.cols);
+    uint64_t c1[VPT][4], c2[VPT][4], spre[VPT][4], spost[VPT][4];
+    int col[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int base = (v * warps + warp) * kChunk;
+        col[v] = base + lane * 8;
+        float f[8], w[8] = {};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = p.alpha;
+        if (has_post) {
+            load8_of<TX, true>(p.post, 0, base, lane, p.cols, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] *= w[j] + p.offset;
+        }
+        if (p.gate_mode == kGateChannel) {
+            load8_of<TX, true>(p.gate, 0, base, lane, p.cols, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] *= w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c1[v][j] = pack2(f[2 * j], f[2 * j + 1]);
+        if (has_pre) load8_of<TX, true>(p.pre, 0, base, lane, p.cols, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            c2[v][j] = pack2(w[2 * j] + p.offset, w[2 * j + 1] + p.offset);
+            spre[v][j] = spost[v][j] = 0;
+        }
+    }
+
+    int slot = 0, s = 0;
+    uint32_t ph = 0;
+    for (int64_t row = first; row < p.rows; row += step) {
+        float g = 1.0f;
+        if (p.gate_mode == kGateToken) g = load1_of<TX>(p.gate, row);
+        ring.wait(s, ph);
+        const uint8_t *stage = ring.stage(s);
+        float sum[3] = {0.0f, 0.0f, 0.0f};  // of r^2, r t and x^2
+        if (has_pre || has_post) {
+            uint64_t a[3] = {0, 0, 0};
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                if (col[v] >= cols) continue;
+                if (has_pre) {
+                    uint64_t r[4], dh[4];
+                    read8<TR>(stage + r_at, col[v], r);
+                    read8<TX>(stage + dh_at, col[v], dh);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        a[0] = fma2(r[j], r[j], a[0]);
+                        a[1] = fma2(r[j], mul2(dh[j], c2[v][j]), a[1]);
+                    }
+                }
+                if (has_post) {
+                    uint64_t x[4];
+                    read8<TX>(stage, col[v], x);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a[2] = fma2(x[j], x[j], a[2]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 3; ++i) sum[i] = lo2(a[i]) + hi2(a[i]);
+            cta_sum<3>(sum, warps, warp, lane, slots, slot);
+        }
+        const float inv_r = rsqrtf(sum[0] * inv_cols + p.eps);
+        const float inv_x = has_post ? rsqrtf(sum[2] * inv_cols + p.eps) : 1.0f;
+        const uint64_t inv_r2 = twice(inv_r), inv_x2 = twice(inv_x), less = twice(-inv_r * sum[1] * inv_cols);
+        uint64_t d[VPT][4], hat[VPT][4], e = 0;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[v][j] = hat[v][j] = 0;
+            if (col[v] >= cols) continue;
+            if (has_dr) read8<TR>(stage + dr_at, col[v], d[v]);
+            if (has_pre) {
+                uint64_t r[4], dh[4];
+                read8<TR>(stage + r_at, col[v], r);
+                read8<TX>(stage + dh_at, col[v], dh);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint64_t R = mul2(r[j], inv_r2);
+                    spre[v][j] = fma2(dh[j], R, spre[v][j]);
+                    d[v][j] = fma2(inv_r2, fma2(R, less, mul2(dh[j], c2[v][j])), d[v][j]);
+                }
+            }
+            if (p.dr.p != nullptr) write8<TR>(static_cast<TR *>(p.dr.p) + row * p.dr.ld + col[v], d[v]);
+            if (!has_x) continue;
+            read8<TX>(stage, col[v], hat[v]);
+            uint64_t gate[4] = {twice(g), twice(g), twice(g), twice(g)}, q[4];
+            if (p.gate_mode == kGateFull) {
+                float w[8];
+                load8_of<TX, true>(p.gate, row, (v * warps + warp) * kChunk, lane, p.cols, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) gate[j] = pack2(w[2 * j], w[2 * j + 1]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                hat[v][j] = mul2(hat[v][j], inv_x2);
+                q[j] = mul2(d[v][j], hat[v][j]);
+                spost[v][j] = fma2(q[j], gate[j], spost[v][j]);
+                q[j] = mul2(q[j], c1[v][j]);
+                e = p.gate_mode == kGateFull ? fma2(q[j], gate[j], e) : add2(q[j], e);
+                d[v][j] = mul2(mul2(d[v][j], c1[v][j]), gate[j]);
+            }
+            if (p.gate_mode == kGateFull) {
+                if (p.dgate.dtype == ST_F32) write8<float>(static_cast<float *>(p.dgate.p) + row * p.dgate.ld + col[v], q);
+                else write8<TX>(static_cast<TX *>(p.dgate.p) + row * p.dgate.ld + col[v], q);
+            }
+        }
+        float es[1] = {lo2(e) + hi2(e)};
+        cta_sum<3>(es, warps, warp, lane, slots, slot);
+        // every thread has read the stage: the next row that it is for may come in
+        if (threadIdx.x == 0 && row + stages * step < p.rows) fetch(s, row + stages * step);
+        if (has_x) {
+            if (p.gate_mode == kGateToken && threadIdx.x == 0) static_cast<float *>(p.dgate.p)[row * p.dgate.ld] = es[0];
+            const uint64_t minus = twice(has_post ? -g * es[0] * inv_cols : 0.0f);
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                if (col[v] >= cols) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[v][j] = mul2(inv_x2, fma2(hat[v][j], minus, d[v][j]));
+                write8<TX>(static_cast<TX *>(p.dx.p) + row * p.dx.ld + col[v], d[v]);
+            }
+        }
+        if (++s == stages) {
+            s = 0;
+            ph ^= 1u;
+        }
+    }
+
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        if (col[v] >= cols) continue;
+        if (planes.pre >= 0) write8<float>(out + (planes.pre * step + first) * p.cols + col[v], spre[v]);
+        if (planes.post >= 0) write8<float>(out + (planes.post * step + first) * p.cols + col[v], spost[v]);
     }
     pdl_trigger();
 }
 
-// Row groups of the backward kernel: each leaves one row of partial sums.
+// One sum over rows: out[c] = scale * (factor[c] + offset) * sum over groups
+// of sums[plane][g][c] (without a factor, scale * the sum).
+struct ColumnSum {
+    float *out = nullptr;
+    int plane = 0;
+    float scale = 1.0f, offset = 0.0f;
+    NormView factor;
+};
+struct ColumnSums {
+    ColumnSum sum[3];
+    int count = 0;
+};
+
+// In a fixed order: 8 threads a column, each every 8th group; blockIdx.y picks the sum.
+template <typename T>
+__global__ void __launch_bounds__(256) column_sums_kernel(const float *sums, int64_t groups, int64_t cols,
+                                                          const ColumnSums todo) {
+    pdl_wait();
+    const ColumnSum &o = todo.sum[blockIdx.y];
+    __shared__ float part[8][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
+    const float *src = sums + o.plane * groups * cols + c;
+    float s = 0.0f;
+    if (c < cols) {
+        int64_t i = ty;
+        for (; i + 24 < groups; i += 32) {  // four loads in flight
+            const float a = src[i * cols], b = src[(i + 8) * cols], d = src[(i + 16) * cols], e = src[(i + 24) * cols];
+            s += (a + b) + (d + e);
+        }
+        for (; i < groups; i += 8) s += src[i * cols];
+    }
+    part[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < cols) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += part[i][tx];
+        s *= o.scale;
+        if (o.factor.p != nullptr)
+            s *= (o.factor.dtype == ST_F32 ? static_cast<const float *>(o.factor.p)[c]
+                                           : to_float(static_cast<const T *>(o.factor.p)[c])) +
+                 o.offset;
+        o.out[c] = s;
+    }
+    pdl_trigger();
+}
+
+// Row groups of the backward kernels: each leaves one row of partial sums.
+// As many as CTAs of the ring kernel are at work, 16 warps an SM, and no
+// fewer than two an SM.
+constexpr int64_t kGroupSms = 148;
+
 int64_t backward_groups(int64_t rows, int64_t cols) {
-    const int64_t most = cols <= 2 * kChunk ? 148 * 16 : 148 * 2;
-    return rows < most ? rows : most;
+    const int64_t warps = cdiv(cols, kBackVecs * kChunk);
+    const int64_t per_sm = warps >= 8 ? 2 : 16 / warps;
+    return rows < kGroupSms * per_sm ? rows : kGroupSms * per_sm;
 }
 
 bool aligned_rows(const NormView &v, int64_t rows, size_t size, size_t to) {
@@ -774,9 +999,9 @@ int launch_rows(Kern kern, uint64_t &attr_set, int threads, int stage_bytes, int
         ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
         if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
     }
-    const int per_sm = threads <= 256 ? 2 : 1;  // 128 registers a thread
+    const int per_sm = kMaxThreads / threads;  // at 128 registers a thread
     int stages = kMostSmem / per_sm / stage_bytes;
-    stages = stages > 4 ? 4 : stages;
+    stages = stages > kMaxStages ? kMaxStages : stages;
     const int64_t ctas = rows < sm_count * per_sm ? rows : sm_count * per_sm;
     if (groups != nullptr) *groups = static_cast<int>(ctas);
     ST_CUDA_TRY(launch_kernel(kern, static_cast<unsigned>(ctas), threads, static_cast<size_t>(stages) * stage_bytes, stream,
@@ -788,12 +1013,13 @@ int launch_rows(Kern kern, uint64_t &attr_set, int threads, int stage_bytes, int
 
 int row_bytes(int64_t cols, size_t size) { return static_cast<int>((cols * size + 127) / 128 * 128); }
 
-template <typename TX, typename TR, int VPT, int MAX_THREADS>
-int forward_rows(const NormArgs &p, const Shape &s, int sm_count, cudaStream_t stream) {
+template <typename TX, typename TR>
+int forward_rows(const NormArgs &p, int sm_count, cudaStream_t stream) {
     static uint64_t attr_set = 0;  // one bit per device ordinal
-    return launch_rows(residual_norm_rows_kernel<TX, TR, VPT, MAX_THREADS>, attr_set, s.threads,
+    const int warps = static_cast<int>(cdiv(p.cols, kRowVecs * kChunk));
+    return launch_rows(residual_norm_rows_kernel<TX, TR>, attr_set, 32 * warps,
                        row_bytes(p.cols, sizeof(TX)) + row_bytes(p.cols, sizeof(TR)), p.rows, sm_count, stream, nullptr, p,
-                       s.warps);
+                       warps);
 }
 
 template <typename TX, typename TR>
@@ -806,10 +1032,8 @@ int forward_typed(const NormArgs &p, int sm_count, cudaStream_t stream) {
                      (p.gate_mode == kGateToken ||
                       aligned_rows(p.gate, p.gate_mode == kGateFull ? p.rows : 1, side(p.gate), 16));
     const Shape s = shape_of(p.rows, p.cols, int64_t(1) << 30, p.rows < sm_count);
-    if (vec && p.x.p != nullptr && p.r_out.p != nullptr && (p.post.p != nullptr || p.pre.p != nullptr) && p.cols % 8 == 0 && s.warps > 1 && s.vpt == 2 &&
-        p.rows >= 2 * sm_count)
-        return s.threads <= 256 ? forward_rows<TX, TR, 2, 256>(p, s, sm_count, stream)
-                                : forward_rows<TX, TR, 2, 512>(p, s, sm_count, stream);
+    if (vec && p.x.p != nullptr && p.r_out.p != nullptr && p.cols % 8 == 0 && p.cols > 2 * kChunk && p.rows >= 2 * sm_count)
+        return forward_rows<TX, TR>(p, sm_count, stream);
     if (s.vpt == 1) return forward_vpt<TX, TR, 1>(p, s, vec, stream);
     if (s.vpt == 2) return forward_vpt<TX, TR, 2>(p, s, vec, stream);
     return forward_vpt<TX, TR, 4>(p, s, vec, stream);
@@ -840,6 +1064,17 @@ int backward_vpt(const NormBackwardArgs &p, const Shape &s, bool vec, const Plan
                : backward_launch<TX, TR, VPT, false>(p, s, planes, sums, stream);
 }
 
+template <typename T>
+int finish_sums(const ColumnSums &todo, const float *sums, int64_t groups, int64_t cols, cudaStream_t stream) {
+    if (todo.count == 0) return ST_OK;
+    ST_CUDA_TRY(launch_kernel(column_sums_kernel<T>,
+                              dim3(static_cast<unsigned>(cdiv(cols, 32)), static_cast<unsigned>(todo.count)), 256, 0, stream,
+                              sums, groups, cols, todo));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "column_sums_kernel");
+}
+
 template <typename TX, typename TR>
 int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) {
     auto side = [](const NormView &v) { return v.dtype == ST_F32 ? sizeof(float) : sizeof(TX); };
@@ -851,28 +1086,41 @@ int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) 
         (p.gate_mode == kGateToken || p.gate_mode == kGateNone ||
          aligned_rows(p.gate, p.gate_mode == kGateFull ? p.rows : 1, side(p.gate), 16)) &&
         (p.gate_mode != kGateFull || aligned_rows(p.dgate, p.rows, side(p.dgate), 16)) && p.cols % 4 == 0;
-    Shape s = shape_of(p.rows, p.cols, backward_groups(p.rows, p.cols), false);
-    const int64_t groups = s.warps == 1 ? static_cast<int64_t>(s.ctas) * kRowsPerCta : s.ctas;
     Planes planes{-1, -1, -1, 0};
-    float *dst[3] = {nullptr, nullptr, nullptr};
+    ColumnSums todo;
+    const bool channel = p.gate_mode == kGateChannel;
+    if (vec && p.cols % 8 == 0 && p.cols <= kBackVecs * 8 * kMaxThreads && p.rows >= 2 * kGroupSms) {
+        if (p.dpre != nullptr) {
+            planes.pre = planes.count++;
+            todo.sum[todo.count++] = {p.dpre, planes.pre, 1.0f, 0.0f, NormView{}};
+        }
+        if (p.dpost != nullptr || channel) planes.post = planes.count++;
+        if (p.dpost != nullptr) todo.sum[todo.count++] = {p.dpost, planes.post, p.alpha, 0.0f, channel ? p.gate : NormView{}};
+        if (channel) todo.sum[todo.count++] = {static_cast<float *>(p.dgate.p), planes.post, p.alpha, p.offset, p.post};
+        static uint64_t attr_set = 0;  // one bit per device ordinal
+        const int warps = static_cast<int>(cdiv(p.cols, kBackVecs * kChunk));
+        const int stage = (p.x.p != nullptr ? row_bytes(p.cols, sizeof(TX)) : 0) +
+                          (p.pre.p != nullptr ? row_bytes(p.cols, sizeof(TX)) + row_bytes(p.cols, sizeof(TR)) : 0) +
+                          (p.d_residual.p != nullptr ? row_bytes(p.cols, sizeof(TR)) : 0);
+        int groups = 0;
+        ST_TRY(launch_rows(residual_norm_backward_rows_kernel<TX, TR>, attr_set, 32 * warps, stage, p.rows,
+                           static_cast<int>(kGroupSms), stream, &groups, p, warps, planes, sums));
+        return finish_sums<TX>(todo, sums, groups, p.cols, stream);
+    }
+    const Shape s = shape_of(p.rows, p.cols, backward_groups(p.rows, p.cols), false);
+    const int64_t groups = s.warps == 1 ? static_cast<int64_t>(s.ctas) * kRowsPerCta : s.ctas;
     auto keep = [&](int &plane, float *to) {
         if (to == nullptr) return;
-        plane = planes.count;
-        dst[planes.count++] = to;
+        plane = planes.count++;
+        todo.sum[todo.count++] = {to, plane, 1.0f, 0.0f, NormView{}};
     };
     keep(planes.pre, p.dpre);
     keep(planes.post, p.dpost);
-    if (p.gate_mode == kGateChannel) keep(planes.gate, static_cast<float *>(p.dgate.p));
+    if (channel) keep(planes.gate, static_cast<float *>(p.dgate.p));
     if (s.vpt == 1) ST_TRY((backward_vpt<TX, TR, 1>(p, s, vec, planes, sums, stream)));
     else if (s.vpt == 2) ST_TRY((backward_vpt<TX, TR, 2>(p, s, vec, planes, sums, stream)));
     else ST_TRY((backward_vpt<TX, TR, 4>(p, s, vec, planes, sums, stream)));
-    if (planes.count == 0) return ST_OK;
-    ST_CUDA_TRY(launch_kernel(column_sums_kernel,
-                              dim3(static_cast<unsigned>(cdiv(p.cols, 32)), static_cast<unsigned>(planes.count)), 256, 0,
-                              stream, sums, groups, p.cols, dst[0], dst[1], dst[2]));
-    note_launch();
-    const cudaError_t e = cudaPeekAtLastError();
-    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "column_sums_kernel");
+    return finish_sums<TX>(todo, sums, groups, p.cols, stream);
 }
 
 }  // namespace
@@ -898,8 +1146,11 @@ int64_t residual_norm_backward_workspace(int64_t rows, int64_t cols) {
     return 3 * groups * cols * static_cast<int64_t>(sizeof(float));
 }
 
-int launch_residual_norm_backward(const NormBackwardArgs &p, void *workspace, int sm_count, cudaStream_t stream) {
-    (void)sm_count;
+int launch_residual_norm_backward(const NormBackwardArgs &args, void *workspace, int *dev_err, uint64_t timeout_ns,
+                                  cudaStream_t stream) {
+    NormBackwardArgs p = args;
+    p.err = dev_err;
+    p.limit_ns = timeout_ns;
     if (p.cols > kMaxCols) return fail(ST_ERR_UNSUPPORTED, "residual_norm_backward: at most 16384 columns");
     float *sums = static_cast<float *>(workspace);
     if (p.rows == 0) {  // the sums over no rows

@@ -1744,7 +1744,7 @@ int st_residual_norm_backward(st_ctx *ctx, const st_tensor *d_residual, const st
     ExecCtx x;
     ST_TRY(resolve_exec(ctx, exec, &x));
     DeviceGuard guard(x.dev->ordinal);
-    ST_TRY(launch_residual_norm_backward(g, workspace, x.dev->sm_count, x.stream));
+    ST_TRY(launch_residual_norm_backward(g, workspace, x.dev->dev_err, kDeviceWaitLimitNs, x.stream));
     return finish(x);
 }
 

@@ -341,3 +341,28 @@ def test_forward_many_rows_parts(post, pre):
     want = st.residual_norm(g["x"], g["r"], g["post"], g["gate"], g["pre"])
     got = st.residual_norm(g["x"], g["r"], g["post"], g["gate"], g["pre"], out=g["r"])  # in place
     assert torch.equal(got.residual, want.residual) and got.residual is g["r"]
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("tx,tr", [(F32, F32), (F16, F16), (BF16, F32)], ids=["f32", "f16", "bf16_f32"])
+@pytest.mark.parametrize("rows,cols", [(700, 1024), (1601, 520), (500, 5000), (333, 8192), (2500, 264)], ids=lambda v: str(v))
+def test_backward_many_rows(rows, cols, tx, tr, gate):
+    check_backward(inputs(rows, cols, tx, tr, gate, True, True, seed=3), rows, cols, tx, tr, offset=0.5)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("post", [True, False], ids=["post", "nopost"])
+@pytest.mark.parametrize("pre", [True, False], ids=["pre", "nopre"])
+def test_backward_many_rows_parts(pre, post, gate):
+    check_backward(inputs(900, 768, BF16, BF16, gate, post, pre, seed=4), 900, 768, BF16, BF16)
+    if pre:
+        check_backward(inputs(900, 768, BF16, F32, gate, post, pre, seed=4), 900, 768, BF16, F32, d_residual=False)
+
+
+def test_backward_zero_token_gate():
+    """A token whose gate is 0 still gets the gate's gradient; its x gets none."""
+    for rows in (10, 700):
+        d = inputs(rows, 640, F32, F32, "token", True, True)
+        d["gate"][::2] = 0
+        got = check_backward(d, rows, 640, F32, F32)
+        assert (got.x[::2] == 0).all() and (got.gate[::2] != 0).all()
