@@ -31,6 +31,7 @@
 #include <mutex>
 
 #include "common.h"
+#include "fp8.cuh"
 #include "sm100.cuh"
 
 namespace st {
@@ -80,29 +81,12 @@ __device__ __forceinline__ uint32_t pack_16(float a, float b, int dtype) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// acc (two fp32) += v * s, one packed instruction
-__device__ __forceinline__ void fma2(uint64_t &acc, uint32_t v0, uint32_t v1, uint64_t s) {
-    asm("{\n\t.reg .b64 v;\n\t"
-        "mov.b64 v, {%1, %2};\n\t"
-        "fma.rn.f32x2 %0, v, %3, %0;\n\t}"
-        : "+l"(acc)
-        : "r"(v0), "r"(v1), "l"(s));
+// Load 8, 16 or 32 consecutive f32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_load_8(uint32_t taddr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
 }
-
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    return static_cast<uint64_t>(__float_as_uint(a)) | (static_cast<uint64_t>(__float_as_uint(b)) << 32);
-}
-
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
-__device__ __forceinline__ float lo2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
-__device__ __forceinline__ float hi2(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-
-// Load 16 consecutive f32 columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t *r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -111,71 +95,46 @@ __device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t *r) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
-
-// Wait for every load so far; the registers pass through, so that nothing
-// reads them before it.
-__device__ __forceinline__ void tmem_load_wait_16(uint32_t *r) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-}
-
-// acc[0..COLS) += accumulator columns at tm, times r_scale and the column
-// scales: cols[0] or, CVEC, one
-// of cols[] for each column.  STEP columns are multiplied while the next STEP
-// are read; `release` is called once the accumulator has been read.
-template <int COLS, bool CVEC, int STEP, typename Release>
-__device__ __forceinline__ void scale_and_add(uint64_t (&acc)[COLS / 2], uint32_t tm, float r_scale, const float *cols,
-                                              Release release) {
-    static_assert(COLS % STEP == 0 && STEP % 16 == 0, "whole steps");
-    constexpr int kSteps = COLS / STEP;
-    const float both = CVEC ? r_scale : r_scale * cols[0];
-    const uint64_t s2 = pack2(both, both);
-    uint32_t v[2][STEP];
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t *r) {
+    if constexpr (N == 8) {
+        tmem_load_8(taddr, r);
+    } else {
 #pragma unroll
-    for (int i = 0; i < STEP; i += 16) tmem_load_16(tm + i, v[0] + i);
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-        uint32_t *x = v[j & 1];
-#pragma unroll
-        for (int i = 0; i < STEP; i += 16) tmem_load_wait_16(x + i);
-        if (j + 1 < kSteps) {
-#pragma unroll
-            for (int i = 0; i < STEP; i += 16) tmem_load_16(tm + (j + 1) * STEP + i, v[(j + 1) & 1] + i);
-        } else {
-            release();
-        }
-#pragma unroll
-        for (int i = 0; i < STEP; i += 4) {
-            uint64_t &a0 = acc[(j * STEP + i) / 2], &a1 = acc[(j * STEP + i) / 2 + 1];
-            if constexpr (CVEC) {
-                const float4 c = *reinterpret_cast<const float4 *>(cols + j * STEP + i);
-                fma2(a0, x[i], x[i + 1], mul2(s2, pack2(c.x, c.y)));
-                fma2(a1, x[i + 2], x[i + 3], mul2(s2, pack2(c.z, c.w)));
-            } else {
-                fma2(a0, x[i], x[i + 1], s2);
-                fma2(a1, x[i + 2], x[i + 3], s2);
-            }
-        }
+        for (int i = 0; i < N; i += 16) tmem_load_16(taddr + i, r + i);
     }
 }
 
-// One warp brings the scales of a tile's blocks, ROWS for its rows and COLS
-// for its columns (CVEC), or one for each 128 columns, into a ring of shared
-// memory DEPTH blocks ahead of their use: a load by the scaling warps
-// themselves would cost them its latency in every block (92 us against 76 at
-// 4096^3, measured with one block of look-ahead).
+// Wait for every load so far; the registers pass through, so that nothing
+// reads them before it.
+template <int N>
+__device__ __forceinline__ void tmem_loaded(uint32_t *r) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                       "+r"(r[i + 6]), "+r"(r[i + 7])
+                     :
+                     : "memory");
+}
+
 __device__ __forceinline__ void copy_4_async(uint32_t dst, const float *src, bool valid) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
 
+// One warp brings the scales of a tile's blocks, ROWS for its rows and COLS
+// for its columns (CVEC), or one for each 128 columns, into a ring of shared
+// memory ahead of their use: a load by the scaling warps themselves would
+// cost them its latency in every block.  A slot holds the scales of kBatch
+// blocks, so that a slot's two barriers are passed once in kBatch blocks.
+constexpr int kBatch = 4;
+
 template <int ROWS, int COLS, bool CVEC, int DEPTH>
 struct ScaleRing {
+    static constexpr int kDepth = DEPTH;
     static constexpr int kCols = CVEC ? COLS : (COLS + 127) / 128;
-    static constexpr int kSlot = ROWS + (kCols + 3) / 4 * 4;  // floats; 16-byte aligned columns
-    static constexpr int kBytes = DEPTH * kSlot * 4;
+    static constexpr int kBlock = ROWS + (kCols + 3) / 4 * 4;  // floats; 16-byte aligned columns
+    static constexpr int kBytes = DEPTH * kBatch * kBlock * 4;
     static constexpr int kBars = 2 * DEPTH;
     float *slots;
     uint32_t bar0;  // full[DEPTH], empty[DEPTH]
@@ -187,8 +146,8 @@ struct ScaleRing {
             mbar_init(empty(d), readers);
         }
     }
-    __device__ __forceinline__ const float *rows(int d) const { return slots + d * kSlot; }
-    __device__ __forceinline__ const float *cols(int d) const { return slots + d * kSlot + ROWS; }
+    __device__ __forceinline__ const float *rows(int d, int i) const { return slots + (d * kBatch + i) * kBlock; }
+    __device__ __forceinline__ const float *cols(int d, int i) const { return rows(d, i) + ROWS; }
     // The scales of blocks [b0, b1) of the tile at row r0, column c0; false after an abort.
     __device__ __forceinline__ bool load(const Fp8Params &p, int r0, int c0, int b0, int b1, int lane, int &d, uint32_t &ph,
                                          const volatile int *abort_flag) const {
@@ -206,14 +165,17 @@ struct ScaleRing {
             ok_c[i] = j < kCols && c < p.cols;
             src_c[i] = p.cs + static_cast<int64_t>(ok_c[i] ? c >> p.cs_shift : 0) * p.cs_i;
         }
-        for (int b = b0; b < b1; ++b) {
+        for (int b = b0; b < b1; b += kBatch) {
             if (!__all_sync(0xffffffffu, mbar_wait(empty(d), ph ^ 1u, abort_flag, p.timeout_ns))) return false;
-            const uint32_t to_r = smem_addr(slots + d * kSlot) + 4u * lane, to_c = to_r + 4u * ROWS;
+            const int n = b1 - b < kBatch ? b1 - b : kBatch;
+            for (int k = 0; k < n; ++k) {
+                const uint32_t to_r = smem_addr(rows(d, k)) + 4u * lane, to_c = to_r + 4u * ROWS;
 #pragma unroll
-            for (int i = 0; i < ROWS / 32; ++i) copy_4_async(to_r + 128u * i, src_r[i] + b * p.rs_b, ok_r[i]);
+                for (int i = 0; i < ROWS / 32; ++i) copy_4_async(to_r + 128u * i, src_r[i] + (b + k) * p.rs_b, ok_r[i]);
 #pragma unroll
-            for (int i = 0; i < (kCols + 31) / 32; ++i)
-                if (lane + 32 * i < kCols) copy_4_async(to_c + 128u * i, src_c[i] + b * p.cs_b, ok_c[i]);
+                for (int i = 0; i < (kCols + 31) / 32; ++i)
+                    if (lane + 32 * i < kCols) copy_4_async(to_c + 128u * i, src_c[i] + (b + k) * p.cs_b, ok_c[i]);
+            }
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(d)) : "memory");
             if (++d == DEPTH) {
                 d = 0;
@@ -223,6 +185,88 @@ struct ScaleRing {
         return true;
     }
 };
+
+// What a scaling warp carries from tile to tile: the next accumulator and ring slot.
+struct ScalePosition {
+    int a = 0, d = 0;
+    uint32_t aph = 0, dph = 0;
+};
+
+// acc += the scaled sums of n blocks of a tile, for one row (TMEM lane) and
+// COLS columns from accumulator column t on (accumulator a lies a * STRIDE
+// further).  A warp passes every block, so a block's serial latency counts:
+// STEP columns are added while the next STEP are read, and the first ones of
+// the next block are asked for before the last ones of this block are added.
+// The sums are added one by one: a packed multiply-add of two needs its
+// operands in register pairs, and the moves that make them cost more than it
+// saves (eight warps reading and adding 128 columns each: 292 cycles, packed
+// 445).  released(a): accumulator a has been read.
+template <int COLS, int STEP, bool CVEC, int ACCS, int STRIDE, typename Ring, typename Full, typename Released>
+__device__ __forceinline__ bool scale_blocks(float (&acc)[COLS], int n, uint32_t t, int row, int col, const Ring &ring,
+                                             ScalePosition &at, Full tfull, Released released, int lane,
+                                             const volatile int *abort_flag, uint64_t limit_ns) {
+    constexpr int kSteps = COLS / STEP;
+    static_assert(kSteps % 2 == 0, "the two buffers keep their order from block to block");
+    uint32_t v[2][STEP];
+    auto arrived = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit_ns));
+    };
+    if (!arrived(tfull(at.a), at.aph)) return false;
+    tc_fence_after_sync();
+    tmem_load<STEP>(t + static_cast<uint32_t>(at.a * STRIDE), v[0]);
+    for (int b = 0; b < n; ++b) {
+        const int k = b % kBatch;
+        if (k == 0 && !arrived(ring.full(at.d), at.dph)) return false;
+        const float *cols = ring.cols(at.d, k) + col;
+        const float r_scale = ring.rows(at.d, k)[row];
+        const float both = CVEC ? r_scale : r_scale * cols[0];
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            uint32_t *x = v[j & 1];
+            tmem_loaded<STEP>(x);
+            if (j + 1 < kSteps) {
+                tmem_load<STEP>(t + static_cast<uint32_t>(at.a * STRIDE + (j + 1) * STEP), v[(j + 1) & 1]);
+            } else {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) released(at.a);
+                if (++at.a == ACCS) {
+                    at.a = 0;
+                    at.aph ^= 1u;
+                }
+                if (b + 1 < n) {
+                    if (!arrived(tfull(at.a), at.aph)) return false;
+                    tc_fence_after_sync();
+                    tmem_load<STEP>(t + static_cast<uint32_t>(at.a * STRIDE), v[0]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < STEP; i += 4) {
+                float *s = acc + j * STEP + i;
+                if constexpr (CVEC) {
+                    const float4 c = *reinterpret_cast<const float4 *>(cols + j * STEP + i);
+                    const uint64_t r2 = pack2(both, both), s0 = mul2(r2, pack2(c.x, c.y)), s1 = mul2(r2, pack2(c.z, c.w));
+                    s[0] = __fmaf_rn(__uint_as_float(x[i]), lo2(s0), s[0]);
+                    s[1] = __fmaf_rn(__uint_as_float(x[i + 1]), hi2(s0), s[1]);
+                    s[2] = __fmaf_rn(__uint_as_float(x[i + 2]), lo2(s1), s[2]);
+                    s[3] = __fmaf_rn(__uint_as_float(x[i + 3]), hi2(s1), s[3]);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) s[q] = __fmaf_rn(__uint_as_float(x[i + q]), both, s[q]);
+                }
+            }
+        }
+        if (k == kBatch - 1 || b + 1 == n) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ring.empty(at.d));
+            if (++at.d == Ring::kDepth) {
+                at.d = 0;
+                at.dph ^= 1u;
+            }
+        }
+    }
+    return true;
+}
 
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -247,10 +291,10 @@ struct Fp8Cfg {
     static constexpr int kStageBytes = kRowBytes + kColBytes;
     // BN 128 fills an SM's TMEM (4 x 128 columns) and shared memory alone;
     // narrower tiles leave room for two CTAs per SM
-    static constexpr int kStages = BN == 128 ? 6 : (BN == 64 ? 4 : (BN == 32 ? 5 : 6));
+    static constexpr int kStages = BN == 128 ? 6 : (BN == 64 ? 4 : 5);
     static constexpr int kAccs = 4;
     static constexpr int kTmemCols = kAccs * BN;
-    using Ring = ScaleRing<kTileRows, BN, CVEC, 4>;
+    using Ring = ScaleRing<kTileRows, BN, CVEC, 2>;
     static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + Ring::kBytes + 1024;
     static_assert(kSmemBytes <= (BN == 128 ? 232448 : 115712), "shared memory of one (two) CTAs per SM");
     static_assert(kStages * kStageBytes >= kPadRows * BN * 4, "the ring holds a tile's partial sums");
@@ -321,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     // scaling warps: TMEM lane = row of the tile
     const int g = warp & 3;
     const int row_in_tile = g * 32 + lane;
-    uint64_t acc[BN / 2];
+    float acc[BN];
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
@@ -406,35 +450,14 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     } else {
         // ------------------------------------------------ scaling
 #pragma unroll
-        for (int j = 0; j < BN / 2; ++j) acc[j] = 0;
-        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(g * 32) << 16);
-        int a = 0, d = 0;
-        uint32_t aph = 0, dph = 0;
-        for (int b = b0; b < b1; ++b) {
-            const bool ready = mbar_wait(ring.full(d), dph, abort_flag, p.timeout_ns) &&
-                               mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns);
-            if (!__all_sync(0xffffffffu, ready)) {
-                *abort_flag = 1;
-                if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
-                break;
-            }
-            tc_fence_after_sync();
-            scale_and_add<BN, CVEC, (BN >= 64 ? 32 : 16)>(acc, t_lane + static_cast<uint32_t>(a * BN),
-                                                          ring.rows(d)[row_in_tile], ring.cols(d), [&] {
-                                                              tc_fence_before_sync();
-                                                              __syncwarp();
-                                                              if (lane == 0) mbar_arrive(tempty_bar(a));
-                                                          });
-            __syncwarp();
-            if (lane == 0) mbar_arrive(ring.empty(d));
-            if (++a == Cfg::kAccs) {
-                a = 0;
-                aph ^= 1u;
-            }
-            if (++d == 4) {
-                d = 0;
-                dph ^= 1u;
-            }
+        for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
+        ScalePosition at;
+        const bool ok = scale_blocks<BN, (BN == 128 ? 32 : BN >= 32 ? 16 : 8), CVEC, Cfg::kAccs, BN>(
+            acc, b1 - b0, tmem_base + (static_cast<uint32_t>(g * 32) << 16), row_in_tile, 0, ring, at, tfull_bar,
+            [&](int a) { mbar_arrive_relaxed(tempty_bar(a)); }, lane, abort_flag, p.timeout_ns);
+        if (!ok) {
+            *abort_flag = 1;
+            if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
         }
     }
 
@@ -449,16 +472,15 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
             uint8_t *dst = static_cast<uint8_t *>(p.c) + (row * p.c_r + c0) * es;
             if (p.c_dtype == ST_F32) {
 #pragma unroll
-                for (int j = 0; j < BN / 2; j += 2)
-                    reinterpret_cast<float4 *>(dst)[j / 2] =
-                        make_float4(lo2(acc[j]), hi2(acc[j]), lo2(acc[j + 1]), hi2(acc[j + 1]));
+                for (int j = 0; j < BN; j += 4)
+                    reinterpret_cast<float4 *>(dst)[j / 4] = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
             } else {
 #pragma unroll
-                for (int j = 0; j < BN / 2; j += 4) {
+                for (int j = 0; j < BN; j += 8) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = pack_16(lo2(acc[j + i]), hi2(acc[j + i]), p.c_dtype);
-                    reinterpret_cast<uint4 *>(dst)[j / 4] = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int i = 0; i < 4; ++i) w[i] = pack_16(acc[j + 2 * i], acc[j + 2 * i + 1], p.c_dtype);
+                    reinterpret_cast<uint4 *>(dst)[j / 8] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
@@ -469,10 +491,7 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
         float *mine = reinterpret_cast<float *>(smem);
         if (scaler) {
 #pragma unroll
-            for (int j = 0; j < BN / 2; ++j) {
-                mine[(2 * j) * kPadRows + row_in_tile] = lo2(acc[j]);
-                mine[(2 * j + 1) * kPadRows + row_in_tile] = hi2(acc[j]);
-            }
+            for (int j = 0; j < BN; ++j) mine[j * kPadRows + row_in_tile] = acc[j];
         }
         __syncwarp();
         if (split > 1) cluster_sync();
@@ -539,7 +558,7 @@ constexpr int kPairFeedRegs = 56, kPairScaleRegs = 224;
 constexpr int kPairCols = 256;
 constexpr int kPairWarpCols = 128;  // columns of a scaling warp
 constexpr int kBoxBytes = 32 * 128;
-constexpr int kPairRingDepth = 8;
+constexpr int kPairRingDepth = 2;
 
 template <bool CVEC>
 struct PairCfg {
@@ -746,45 +765,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(half * kPairWarpCols);
         const uint32_t even_tempty0 = map_to_rank(tempty_bar(0), 0);
         uint8_t *my_boxes = boxes + e * 2 * kBoxBytes;
-        int a = 0, box = 0, d = 0;
-        uint32_t aph = 0, dph = 0;
+        int box = 0;
+        ScalePosition at;
         bool ok = true;
-        for (int t = pair; ok && t < tiles; t += pairs) {
-            uint64_t acc[kPairWarpCols / 2];
+        for (int t = pair; t < tiles; t += pairs) {
+            float acc[kPairWarpCols];
 #pragma unroll
-            for (int j = 0; j < kPairWarpCols / 2; ++j) acc[j] = 0;
-            for (int b = 0; b < p.k_blocks; ++b) {
-                const bool ready = mbar_wait(ring.full(d), dph, abort_flag, p.timeout_ns) &&
-                                   mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns);
-                if (!__all_sync(0xffffffffu, ready)) {
-                    *abort_flag = 1;
-                    if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
-                    ok = false;
-                    break;
-                }
-                tc_fence_after_sync();
-                scale_and_add<kPairWarpCols, CVEC, 32>(
-                    acc, t_lane + static_cast<uint32_t>(a * kPairCols), ring.rows(d)[g * 32 + lane],
-                    ring.cols(d) + half * (CVEC ? kPairWarpCols : 1), [&] {
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (rank == 0) mbar_arrive(tempty_bar(a));
-                            else mbar_arrive_cluster(even_tempty0 + 8u * a);
-                        }
-                    });
-                __syncwarp();
-                if (lane == 0) mbar_arrive(ring.empty(d));
-                if (++a == Cfg::kAccs) {
-                    a = 0;
-                    aph ^= 1u;
-                }
-                if (++d == kPairRingDepth) {
-                    d = 0;
-                    dph ^= 1u;
-                }
+            for (int j = 0; j < kPairWarpCols; ++j) acc[j] = 0.0f;
+            ok = scale_blocks<kPairWarpCols, 32, CVEC, Cfg::kAccs, kPairCols>(
+                acc, p.k_blocks, t_lane, g * 32 + lane, half * (CVEC ? kPairWarpCols : 1), ring, at, tfull_bar,
+                [&](int a) {
+                    if (rank == 0) mbar_arrive_relaxed(tempty_bar(a));
+                    else mbar_arrive_cluster_relaxed(even_tempty0 + 8u * a);
+                },
+                lane, abort_flag, p.timeout_ns);
+            if (!ok) {
+                *abort_flag = 1;
+                if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
+                break;
             }
-            if (!ok) break;
             // ---- bias, conversion, and out through the warp's two boxes of 32 rows x 128 bytes
             int tr, tc;
             pair_tile(p, t, tr, tc);
@@ -794,28 +793,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if (p.staged) {
                 if (p.bias != nullptr) {
 #pragma unroll
-                    for (int j = 0; j < kPairWarpCols / 2; ++j) {
-                        const int c = col0 + 2 * j;
-                        const float v0 = c < p.cols ? load_any(p.bias, p.bias_dtype, c) : 0.0f;
-                        const float v1 = c + 1 < p.cols ? load_any(p.bias, p.bias_dtype, c + 1) : 0.0f;
-                        acc[j] = pack2(lo2(acc[j]) + v0, hi2(acc[j]) + v1);
-                    }
+                    for (int j = 0; j < kPairWarpCols; ++j)
+                        acc[j] += col0 + j < p.cols ? load_any(p.bias, p.bias_dtype, col0 + j) : 0.0f;
                 }
 #pragma unroll
                 for (int h = 0; h < kPairWarpCols / 32; ++h) {  // a box: 32 columns of fp32, 64 of 16 bits
                     uint32_t w[32];
                     if (p.c_dtype == ST_F32) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            w[2 * i] = static_cast<uint32_t>(acc[16 * h + i]);
-                            w[2 * i + 1] = static_cast<uint32_t>(acc[16 * h + i] >> 32);
-                        }
+                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(acc[32 * h + i]);
                     } else {
                         if (h & 1) continue;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            const uint64_t v = acc[(16 * h + i) % (kPairWarpCols / 2)];
-                            w[i] = pack_16(lo2(v), hi2(v), p.c_dtype);
+                            const int j = (32 * h + 2 * i) % kPairWarpCols;
+                            w[i] = pack_16(acc[j], acc[j + 1], p.c_dtype);
                         }
                     }
                     if (col0 + 32 * h >= p.cols) continue;
@@ -837,10 +829,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                 for (int h = 0; h < kPairWarpCols / 32; ++h) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        m[lane * 33 + 2 * i] = lo2(acc[16 * h + i]);
-                        m[lane * 33 + 2 * i + 1] = hi2(acc[16 * h + i]);
-                    }
+                    for (int i = 0; i < 32; ++i) m[lane * 33 + i] = acc[32 * h + i];
                     __syncwarp();
                     const int c = col0 + 32 * h + lane;
                     if (c < p.cols) {
