@@ -485,46 +485,43 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
             }
         }
     } else {
-        // Every CTA's (partial) sums go into its own ring, which its MMAs have
-        // read, as [column][row]; then its share of the tile is added over the
-        // parts in order, with a warp's lanes along C's contiguous dimension.
-        float *mine = reinterpret_cast<float *>(smem);
+        // Each part owns BN / split columns of the tile: every CTA sends its
+        // sums to their owners' rings, [part][column][row], once all of the
+        // cluster's MMAs have read them; the owner adds its columns over the
+        // parts in order, a warp's lanes along C's contiguous dimension.
+        // (Stores do not wait; reading the others' parts cost a remote
+        // round trip for each few values.)
+        const int own = BN / split, own_shift = 31 - __clz(own);  // split is a power of two
+        __syncwarp();
+        if (split > 1) cluster_sync();
         if (scaler) {
+            const uint32_t mine = smem_addr(smem) + 4u * static_cast<uint32_t>(part * own * kPadRows + row_in_tile);
+            uint32_t to = mine;
 #pragma unroll
-            for (int j = 0; j < BN; ++j) mine[j * kPadRows + row_in_tile] = acc[j];
+            for (int j = 0; j < BN; ++j) {
+                if ((j & (own - 1)) == 0) to = split == 1 ? mine : map_to_rank(mine, static_cast<uint32_t>(j >> own_shift));
+                st_cluster_f32(to, acc[j]);
+                to += 4u * kPadRows;
+            }
         }
         __syncwarp();
         if (split > 1) cluster_sync();
         else __syncthreads();
         if (scaler) {
-            uint32_t at[8];
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                at[q] = split == 1 ? smem_addr(smem) : (q < split ? map_to_rank(smem_addr(smem), q) : 0);
-            auto put = [&](int r, int j) {  // row r, column j of the tile
-                if (r0 + r >= p.rows || c0 + j >= p.cols) return;
-                const uint32_t off = 4u * static_cast<uint32_t>(j * kPadRows + r);
+            const float *sums = reinterpret_cast<const float *>(smem);
+            const int first = (warp - 2) * 32 + lane;
+            const bool by_rows = p.c_c == 1;
+#pragma unroll 4
+            for (int e = first; e < own * kTileRows; e += 32 * kScaleWarps) {
+                const int r = by_rows ? e >> own_shift : e % kTileRows, j = by_rows ? e & (own - 1) : e / kTileRows;
                 float v = 0.0f;
-                if (split == 1) {
-                    v = mine[j * kPadRows + r];
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        if (q < split) v += ld_cluster_f32(at[q] + off);
-                }
-                if (p.bias != nullptr) v += load_any(p.bias, p.bias_dtype, p.bias_on_rows ? r0 + r : c0 + j);
-                store_any(p.c, p.c_dtype, (r0 + r) * p.c_r + (c0 + j) * p.c_c, v);
-            };
-            if (p.c_c == 1) {
-                for (int r = part * kScaleWarps + g; r < kTileRows; r += split * kScaleWarps)
-#pragma unroll
-                    for (int j = lane; j < BN; j += 32) put(r, j);
-            } else {
-                for (int j = part; j < BN; j += split) put(row_in_tile, j);
+                for (int q = 0; q < split; ++q) v += sums[(q * own + j) * kPadRows + r];
+                const int row = r0 + r, col = c0 + part * own + j;
+                if (row >= p.rows || col >= p.cols) continue;
+                if (p.bias != nullptr) v += load_any(p.bias, p.bias_dtype, p.bias_on_rows ? row : col);
+                store_any(p.c, p.c_dtype, row * p.c_r + col * p.c_c, v);
             }
         }
-        __syncwarp();
-        if (split > 1) cluster_sync();  // the others have read this CTA's part
     }
     tc_fence_before_sync();
     __syncthreads();

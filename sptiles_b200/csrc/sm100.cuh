@@ -456,11 +456,10 @@ __host__ __device__ constexpr uint32_t mma_idesc_f8(uint32_t a_format, uint32_t 
            (static_cast<uint32_t>(b_mn_major) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-// f32 in another CTA's shared memory of the cluster (shared::cluster address).
-__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-    return v;
+// Store f32 to another CTA's shared memory of the cluster (shared::cluster
+// address); seen there after a cluster barrier.
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
 }  // namespace st
