@@ -282,7 +282,6 @@ __device__ __forceinline__ void drain_ring(int issued, int stages, Bar bar, uint
 // ---------------------------------------------------------------- one CTA, 128 x BN tiles
 constexpr int kScaleWarps = 4;
 constexpr int kThreads = 32 * (3 + kScaleWarps);  // warps 0 TMA, 1 MMA, 2..5 scaling, 6 scales
-constexpr int kPadRows = kTileRows + 1;           // odd: a column's and a row's elements lie in different banks
 
 template <int BN, bool CVEC>
 struct Fp8Cfg {
@@ -297,7 +296,7 @@ struct Fp8Cfg {
     using Ring = ScaleRing<kTileRows, BN, CVEC, 2>;
     static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + Ring::kBytes + 1024;
     static_assert(kSmemBytes <= (BN == 128 ? 232448 : 115712), "shared memory of one (two) CTAs per SM");
-    static_assert(kStages * kStageBytes >= kPadRows * BN * 4, "the ring holds a tile's partial sums");
+    static_assert(kStages * kStageBytes >= kTileRows * (BN + 4 * 8) * 4, "the ring holds eight parts' sums of its columns");
 };
 
 // R_MN / C_MN: the operand is stored with its rows (columns) contiguous
@@ -485,41 +484,56 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
             }
         }
     } else {
-        // Each part owns BN / split columns of the tile: every CTA sends its
-        // sums to their owners' rings, [part][column][row], once all of the
-        // cluster's MMAs have read them; the owner adds its columns over the
-        // parts in order, a warp's lanes along C's contiguous dimension.
-        // (Stores do not wait; reading the others' parts cost a remote
-        // round trip for each few values.)
-        const int own = BN / split, own_shift = 31 - __clz(own);  // split is a power of two
+        // A part owns `own` columns of the tile (with many parts, the last
+        // ones none): every CTA sends its sums to their owners' rings, once
+        // all of the cluster's MMAs have read them, as [part][row][own + 4
+        // columns]; the owner adds its columns over the parts in order, a
+        // warp's lanes along C's contiguous dimension.  (Stores do not wait;
+        // reading the others' parts cost a remote round trip for every few
+        // values.)
+        const int own = BN / split < 4 ? 4 : BN / split, own_shift = 31 - __clz(own);  // split is a power of two
+        const int stride = own + 4;  // floats; rows on different banks
         __syncwarp();
         if (split > 1) cluster_sync();
         if (scaler) {
-            const uint32_t mine = smem_addr(smem) + 4u * static_cast<uint32_t>(part * own * kPadRows + row_in_tile);
-            uint32_t to = mine;
+            const uint32_t mine = smem_addr(smem) + 4u * static_cast<uint32_t>((part * kTileRows + row_in_tile) * stride);
 #pragma unroll
-            for (int j = 0; j < BN; ++j) {
-                if ((j & (own - 1)) == 0) to = split == 1 ? mine : map_to_rank(mine, static_cast<uint32_t>(j >> own_shift));
-                st_cluster_f32(to, acc[j]);
-                to += 4u * kPadRows;
+            for (int j = 0; j < BN; j += 4) {
+                const uint32_t to = (split == 1 ? mine : map_to_rank(mine, static_cast<uint32_t>(j >> own_shift))) +
+                                    4u * static_cast<uint32_t>(j & (own - 1));
+                st_cluster_v4(to, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
             }
         }
         __syncwarp();
         if (split > 1) cluster_sync();
         else __syncthreads();
-        if (scaler) {
-            const float *sums = reinterpret_cast<const float *>(smem);
-            const int first = (warp - 2) * 32 + lane;
+        if (scaler && part * own < BN) {
+            const float4 *sums = reinterpret_cast<const float4 *>(smem);
+            const int first = (warp - 2) * 32 + lane, quads = own / 4;
             const bool by_rows = p.c_c == 1;
-#pragma unroll 4
-            for (int e = first; e < own * kTileRows; e += 32 * kScaleWarps) {
-                const int r = by_rows ? e >> own_shift : e % kTileRows, j = by_rows ? e & (own - 1) : e / kTileRows;
-                float v = 0.0f;
-                for (int q = 0; q < split; ++q) v += sums[(q * own + j) * kPadRows + r];
-                const int row = r0 + r, col = c0 + part * own + j;
-                if (row >= p.rows || col >= p.cols) continue;
-                if (p.bias != nullptr) v += load_any(p.bias, p.bias_dtype, p.bias_on_rows ? row : col);
-                store_any(p.c, p.c_dtype, row * p.c_r + col * p.c_c, v);
+            // by rows: this thread's 4 columns of every (512 / own)th row; else all columns of one row
+            const int q0 = by_rows ? first & (quads - 1) : 0, r_first = by_rows ? first >> (own_shift - 2) : first;
+            const int dr = by_rows ? 4 * 128 / own : 0, dq = by_rows ? 0 : 1;
+#pragma unroll 2
+            for (int i = 0; i < quads; ++i) {
+                const int r = r_first + i * dr, quad = q0 + i * dq;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int q = 0; q < split; ++q) {
+                    const float4 x = sums[(q * kTileRows + r) * (stride / 4) + quad];
+                    v.x += x.x;
+                    v.y += x.y;
+                    v.z += x.z;
+                    v.w += x.w;
+                }
+                const int row = r0 + r, col = c0 + part * own + 4 * quad;
+                if (row >= p.rows) continue;
+                const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (col + k >= p.cols) continue;
+                    const float add = p.bias != nullptr ? load_any(p.bias, p.bias_dtype, p.bias_on_rows ? row : col + k) : 0.0f;
+                    store_any(p.c, p.c_dtype, row * p.c_r + (col + k) * p.c_c, p.bias != nullptr ? f[k] + add : f[k]);
+                }
             }
         }
     }

@@ -456,10 +456,11 @@ __host__ __device__ constexpr uint32_t mma_idesc_f8(uint32_t a_format, uint32_t 
            (static_cast<uint32_t>(b_mn_major) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
-// Store f32 to another CTA's shared memory of the cluster (shared::cluster
-// address); seen there after a cluster barrier.
-__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+// Store four f32 to another CTA's shared memory of the cluster
+// (shared::cluster address); seen there after a cluster barrier.
+__device__ __forceinline__ void st_cluster_v4(uint32_t cluster_addr, float a, float b, float c, float d) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(a), "f"(b), "f"(c), "f"(d)
+                 : "memory");
 }
 
 }  // namespace st
