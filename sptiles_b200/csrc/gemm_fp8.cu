@@ -299,6 +299,66 @@ struct Fp8Cfg {
     static_assert(kStages * kStageBytes >= kTileRows * (BN + 4 * 8) * 4, "the ring holds eight parts' sums of its columns");
 };
 
+// Thread `first` of 128: its share of 128 rows x `own` columns (a power of
+// two, 4 at least), added over the parts of sums [part][row][own + 4].  By
+// rows, 4 columns of every (512 / own)th row; else all columns of one row.
+template <typename T>
+__device__ __forceinline__ void store_sums(const Fp8Params &p, const float4 *sums, int first, int own, int own_shift,
+                                           int parts, int r0, int col0) {
+    const int quads = own / 4, pitch = own / 4 + 1;
+    const bool by_rows = p.c_c == 1;
+    const int quad0 = by_rows ? first & (quads - 1) : 0, r_first = by_rows ? first >> (own_shift - 2) : first;
+    const int dr = by_rows ? 4 * 128 / own : 0, dq = by_rows ? 0 : 1;
+    T *c = static_cast<T *>(p.c) + (r0 + r_first) * p.c_r + (col0 + 4 * quad0) * p.c_c;
+    const int64_t dc = by_rows ? dr * p.c_r : 4 * p.c_c;
+    const int left = p.cols - col0 - 4 * quad0;  // columns from this thread's first on
+    const bool four = by_rows && left >= 4 && reinterpret_cast<uintptr_t>(p.c) % (4 * sizeof(T)) == 0 && p.c_r % 4 == 0 &&
+                      col0 % 4 == 0;
+    // one bias for each column of a quad, or one for the row
+    float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias != nullptr) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = p.bias_on_rows ? r0 + r_first : col0 + 4 * quad0 + k;
+            if (i < (p.bias_on_rows ? p.rows : p.cols)) add[k] = load_any(p.bias, p.bias_dtype, i);
+        }
+    }
+#pragma unroll 2
+    for (int i = 0; i < quads; ++i, c += dc) {
+        const int r = r_first + i * dr, quad = quad0 + i * dq;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int q = 0; q < parts; ++q) {
+            const float4 x = sums[(q * kTileRows + r) * pitch + quad];
+            v.x += x.x;
+            v.y += x.y;
+            v.z += x.z;
+            v.w += x.w;
+        }
+        if (p.bias != nullptr) {
+            v.x += add[0];
+            v.y += add[1];
+            v.z += add[2];
+            v.w += add[3];
+        }
+        if (r0 + r >= p.rows) break;
+        T o[4];
+        from_float(v.x, o[0]);
+        from_float(v.y, o[1]);
+        from_float(v.z, o[2]);
+        from_float(v.w, o[3]);
+        if (four) {
+            struct alignas(4 * sizeof(T)) Four {
+                T v[4];
+            };
+            *reinterpret_cast<Four *>(c) = Four{{o[0], o[1], o[2], o[3]}};
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < left - 4 * i * dq) c[k * p.c_c] = o[k];
+        }
+    }
+}
+
 // R_MN / C_MN: the operand is stored with its rows (columns) contiguous
 // instead of K.  CVEC: the column scale differs inside the tile.
 template <int BN, bool R_MN, bool C_MN, bool CVEC>
@@ -509,32 +569,11 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
         else __syncthreads();
         if (scaler && part * own < BN) {
             const float4 *sums = reinterpret_cast<const float4 *>(smem);
-            const int first = (warp - 2) * 32 + lane, quads = own / 4;
-            const bool by_rows = p.c_c == 1;
-            // by rows: this thread's 4 columns of every (512 / own)th row; else all columns of one row
-            const int q0 = by_rows ? first & (quads - 1) : 0, r_first = by_rows ? first >> (own_shift - 2) : first;
-            const int dr = by_rows ? 4 * 128 / own : 0, dq = by_rows ? 0 : 1;
-#pragma unroll 2
-            for (int i = 0; i < quads; ++i) {
-                const int r = r_first + i * dr, quad = q0 + i * dq;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int q = 0; q < split; ++q) {
-                    const float4 x = sums[(q * kTileRows + r) * (stride / 4) + quad];
-                    v.x += x.x;
-                    v.y += x.y;
-                    v.z += x.z;
-                    v.w += x.w;
-                }
-                const int row = r0 + r, col = c0 + part * own + 4 * quad;
-                if (row >= p.rows) continue;
-                const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (col + k >= p.cols) continue;
-                    const float add = p.bias != nullptr ? load_any(p.bias, p.bias_dtype, p.bias_on_rows ? row : col + k) : 0.0f;
-                    store_any(p.c, p.c_dtype, row * p.c_r + (col + k) * p.c_c, p.bias != nullptr ? f[k] + add : f[k]);
-                }
-            }
+            const int first = (warp - 2) * 32 + lane;
+            const int col0 = c0 + part * own;
+            if (p.c_dtype == ST_F32) store_sums<float>(p, sums, first, own, own_shift, split, r0, col0);
+            else if (p.c_dtype == ST_F16) store_sums<__half>(p, sums, first, own, own_shift, split, r0, col0);
+            else store_sums<__nv_bfloat16>(p, sums, first, own, own_shift, split, r0, col0);
         }
     }
     tc_fence_before_sync();
