@@ -34,14 +34,13 @@ _FP8 = {torch.float8_e4m3fn: N.ST_E4M3, torch.float8_e5m2: N.ST_E5M2}
 _ALL_CODES = {**_CODES, **_FP8}
 
 _vp, _cp, _i32, _u64 = ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int32, ctypes.c_uint64
+_pack = _TENSOR_DESC.pack
 _fns: dict = {}
 
 
 def _fn(name: str, *args):
     """`name` from the native library; descriptors are passed as packed bytes."""
-    fn = _fns.get(name)
-    if fn is None:
-        fn = _fns[name] = ctypes.CFUNCTYPE(ctypes.c_int, *args)((name, N.lib()))
+    fn = _fns[name] = ctypes.CFUNCTYPE(ctypes.c_int, *args)((name, N.lib()))
     return fn
 
 
@@ -52,10 +51,10 @@ def _desc(t: torch.Tensor) -> bytes:
     if code is None:
         raise ValueError(f"unsupported dtype {t.dtype}")
     if len(shape) == 2:
-        return _TENSOR_DESC.pack(t.data_ptr() if shape[0] and shape[1] else 0, code, 2, shape[0], shape[1],
-                                 strides[0], strides[1])
+        r, c = shape
+        return _pack(t.data_ptr() if r and c else 0, code, 2, r, c, *strides)
     if len(shape) == 1:
-        return _TENSOR_DESC.pack(t.data_ptr() if shape[0] else 0, code, 1, shape[0], 0, strides[0], 0)
+        return _pack(t.data_ptr() if shape[0] else 0, code, 1, shape[0], 0, strides[0], 0)
     raise ValueError("tensors must be rank 1 or 2")
 
 
@@ -66,27 +65,31 @@ def _device_of(*tensors: torch.Tensor | None) -> int:
         if t is None:
             continue
         d = t.get_device()
-        if d < 0:
-            raise ValueError("Input tensors must be on a CUDA device.")
-        if dev is not None and d != dev:
-            raise ValueError("Input tensors must be on the same CUDA device.")
-        dev = d
+        if d != dev:
+            if d < 0:
+                raise ValueError("Input tensors must be on a CUDA device.")
+            if dev is not None:
+                raise ValueError("Input tensors must be on the same CUDA device.")
+            dev = d
     return dev
 
 
-def _empty_rows(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+# Outputs are made and described at once: their shapes and strides are known,
+# and a call's host time is mostly that of its tensors.
+def _new(like: torch.Tensor, rows: int, cols: int, s0: int, s1: int, dtype: torch.dtype) -> tuple[torch.Tensor, bytes]:
+    t = like.new_empty_strided((rows, cols), (s0, s1), dtype=dtype)
+    return t, _pack(t.data_ptr(), _ALL_CODES[dtype], 2, rows, cols, s0, s1)
+
+
+def _new_codes(like: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> tuple[torch.Tensor, bytes]:
     """[rows, cols] 8-bit codes, each row on a 16-byte boundary, where the tensor core's loads can start."""
-    ld = -(-cols // 16) * 16
-    t = torch.empty((rows, ld), dtype=dtype, device=device)
-    return t if ld == cols else t[:, :cols]
+    return _new(like, rows, cols, (cols + 15) // 16 * 16, 1, dtype)
 
 
-def _empty_scales(rows: int, cols: int, block: tuple[int, int], device: torch.device) -> torch.Tensor:
+def _new_scales(like: torch.Tensor, rows: int, cols: int, block_rows: int, block_cols: int) -> tuple[torch.Tensor, bytes]:
     """One scale per block, lying along the rows (columns) that have one each, as the product reads them."""
-    r, c = -(-rows // block[0]), -(-cols // block[1])
-    if block[0] == 1:
-        return torch.empty((c, r), dtype=torch.float32, device=device).t()
-    return torch.empty((r, c), dtype=torch.float32, device=device)
+    r, c = -(-rows // block_rows), -(-cols // block_cols)
+    return _new(like, r, c, 1, r, torch.float32) if block_rows == 1 else _new(like, r, c, c, 1, torch.float32)
 
 
 def quantize_fp8(A: torch.Tensor, *, block: tuple[int, int] = (1, BLOCK), dtype: torch.dtype = torch.float8_e4m3fn,
@@ -102,32 +105,35 @@ def quantize_fp8(A: torch.Tensor, *, block: tuple[int, int] = (1, BLOCK), dtype:
     16-byte boundaries, so it need not be contiguous.  A block with a NaN or
     an infinity gets a scale that is one, and a product that reads it is NaN.
     """
-    if A.dim() != 2:
+    shape = A.shape
+    if len(shape) != 2:
         raise ValueError("A must be a 2D tensor.")
-    if tuple(block) not in _BLOCKS:
-        raise ValueError(f"block must be one of {_BLOCKS}, got {tuple(block)}")
+    block = tuple(block)
+    if block not in _BLOCKS:
+        raise ValueError(f"block must be one of {_BLOCKS}, got {block}")
     if dtype not in _FP8:
         raise ValueError(f"dtype must be torch.float8_e4m3fn or torch.float8_e5m2, got {dtype}")
-    if out is not None and out.dtype != dtype:
-        raise ValueError(f"out must have dtype {dtype}, got {out.dtype}")
     dev = _device_of(A, out, scale_out)
-    rows, cols = A.shape
+    rows, cols = shape
     if out is None:
-        by_columns = A.stride(0) == 1 and A.stride(1) != 1 and cols > 1
-        out = _empty_rows(cols, rows, dtype, A.device).t() if by_columns else _empty_rows(rows, cols, dtype, A.device)
+        s0, s1 = A.stride()
+        if s0 == 1 and s1 != 1 and cols > 1:
+            out, dq = _new(A, rows, cols, 1, (rows + 15) // 16 * 16, dtype)
+        else:
+            out, dq = _new_codes(A, rows, cols, dtype)
+    else:
+        if out.dtype != dtype:
+            raise ValueError(f"out must have dtype {dtype}, got {out.dtype}")
+        dq = _desc(out)
     if scale_out is None:
-        scale_out = _empty_scales(rows, cols, block, A.device)
-    rc = _fn("st_quantize_fp8", _vp, _cp, _cp, _cp, _i32, _i32, _cp)(
-        context(dev), _desc(A), _desc(out), _desc(scale_out), block[0], block[1], _exec_desc(dev))
+        scale_out, ds = _new_scales(A, rows, cols, *block)
+    else:
+        ds = _desc(scale_out)
+    fn = _fns.get("st_quantize_fp8") or _fn("st_quantize_fp8", _vp, _cp, _cp, _cp, _i32, _i32, _cp)
+    rc = fn(context(dev), _desc(A), dq, ds, block[0], block[1], _exec_desc(dev))
     if rc != N.ST_OK:
         N.check(rc, "quantize_fp8")
     return out, scale_out
-
-
-def _on_16_bytes(t: torch.Tensor) -> bool:
-    """Whether the tensor core's loads address `t` in place (a copy is made otherwise)."""
-    s0, s1 = t.stride()
-    return t.data_ptr() % 16 == 0 and ((s1 == 1 and s0 > 0 and s0 % 16 == 0) or (s0 == 1 and s1 > 0 and s1 % 16 == 0))
 
 
 def matmul_fp8(A: torch.Tensor, B: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
@@ -152,20 +158,28 @@ def matmul_fp8(A: torch.Tensor, B: torch.Tensor, a_scale: torch.Tensor, b_scale:
                          f"must match K dimension of B ({sb[0]})")
     dev = _device_of(A, B, a_scale, b_scale, bias, out)
     if out is None:
-        out = torch.empty((sa[0], sb[1]), dtype=out_dtype, device=A.device)
+        if out_dtype not in _CODES:
+            raise ValueError(f"unsupported dtype {out_dtype}")
+        out, dc = _new(A, sa[0], sb[1], max(sb[1], 1), 1, out_dtype)
+    else:
+        dc = _desc(out)
     da, db = _desc(A), _desc(B)
     workspace, need = None, 0
-    if not (_on_16_bytes(A) and _on_16_bytes(B)):
+    # operands that the tensor core's loads cannot address in place are copied: ask how much room that takes
+    (a0, a1), (b0, b1) = A.stride(), B.stride()
+    if not ((a1 == 1 and a0 % 16 == 0 or a0 == 1 and a1 % 16 == 0) and (b1 == 1 and b0 % 16 == 0 or b0 == 1 and b1 % 16 == 0) and
+            a0 and a1 and b0 and b1 and (A.data_ptr() | B.data_ptr()) % 16 == 0):
         size = ctypes.c_uint64(0)
-        rc = _fn("st_matmul_fp8_workspace", _cp, _cp, _vp)(da, db, ctypes.addressof(size))
+        fn = _fns.get("st_matmul_fp8_workspace") or _fn("st_matmul_fp8_workspace", _cp, _cp, _vp)
+        rc = fn(da, db, ctypes.addressof(size))
         if rc != N.ST_OK:
             N.check(rc, "matmul_fp8")
         need = size.value
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=A.device)
-    rc = _fn("st_matmul_fp8", _vp, _cp, _cp, _cp, _cp, _cp, _cp, _vp, _u64, _cp)(
-        context(dev), da, db, _desc(a_scale), _desc(b_scale), None if bias is None else _desc(bias), _desc(out),
-        None if workspace is None else workspace.data_ptr(), need, _exec_desc(dev))
+    fn = _fns.get("st_matmul_fp8") or _fn("st_matmul_fp8", _vp, _cp, _cp, _cp, _cp, _cp, _cp, _vp, _u64, _cp)
+    rc = fn(context(dev), da, db, _desc(a_scale), _desc(b_scale), None if bias is None else _desc(bias), dc,
+            None if workspace is None else workspace.data_ptr(), need, _exec_desc(dev))
     if rc != N.ST_OK:
         N.check(rc, "matmul_fp8")
     return out

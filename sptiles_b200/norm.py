@@ -24,7 +24,8 @@ import torch
 
 from . import _native as N
 from .api import _exec_desc
-from .fp8 import _FP8, BLOCK, _cp, _desc, _device_of, _empty_rows, _empty_scales, _fn, _u64, _vp
+from .fp8 import (_ALL_CODES, _FP8, BLOCK, _cp, _desc, _device_of, _fn, _fns, _new, _new_codes, _new_scales, _pack, _u64,
+                  _vp)
 from .runtime import context
 
 _OPTIONS = struct.Struct("@fff")  # alpha, eps, weight_offset
@@ -65,32 +66,40 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, post_weight: t
     blocks of 1 x 128, as quantize_fp8 makes them (True: float8_e4m3fn).
     out: where the updated stream goes; ``residual`` itself is allowed.
     """
-    if residual.dim() != 2:
+    shape = residual.shape
+    if len(shape) != 2:
         raise ValueError("residual must be a 2D tensor.")
     dev = _device_of(residual, x, post_weight, gate, pre_weight, out)
-    rows, cols = residual.shape
-    if out is not None and x is None:
-        raise ValueError("out is the updated stream: without x there is none")
-    if x is not None and out is None:
-        out = torch.empty((rows, cols), dtype=residual.dtype, device=residual.device)
+    rows, cols = shape
+    d_out = d_normed = d_scale = normed = scale = None
+    if x is None:
+        if out is not None:
+            raise ValueError("out is the updated stream: without x there is none")
+    elif out is None:
+        out, d_out = _new(residual, rows, cols, max(cols, 1), 1, residual.dtype)
+    else:
+        d_out = _desc(out)
     if x is not None and out_dtype is not None and out_dtype != x.dtype:
         raise ValueError(f"out_dtype {out_dtype} differs from x's dtype {x.dtype}")
-    normed = scale = None
-    if quantize and pre_weight is None:
-        raise ValueError("quantize is for the normed copy: it needs pre_weight")
     if pre_weight is not None:
         if quantize:
             kind = torch.float8_e4m3fn if quantize is True else quantize
             if kind not in _FP8:
                 raise ValueError(f"quantize must be torch.float8_e4m3fn or torch.float8_e5m2, got {kind}")
-            normed = _empty_rows(rows, cols, kind, residual.device)
-            scale = _empty_scales(rows, cols, (1, BLOCK), residual.device)
+            normed, d_normed = _new_codes(residual, rows, cols, kind)
+            scale, d_scale = _new_scales(residual, rows, cols, 1, BLOCK)
         else:
             dtype = x.dtype if x is not None else out_dtype or residual.dtype
-            normed = torch.empty((rows, cols), dtype=dtype, device=residual.device)
-    rc = _fn("st_residual_norm", _vp, _cp, _cp, _cp, _cp, _cp, _cp, _cp, _cp, _cp, _cp)(
-        context(dev), _opt(x), _desc(residual), _opt(post_weight), _opt(gate), _opt(pre_weight), _opt(out), _opt(normed),
-        _opt(scale), _OPTIONS.pack(alpha, eps, weight_offset), _exec_desc(dev))
+            if dtype not in _ALL_CODES:
+                raise ValueError(f"unsupported dtype {dtype}")
+            normed, d_normed = _new(residual, rows, cols, max(cols, 1), 1, dtype)
+    elif quantize:
+        raise ValueError("quantize is for the normed copy: it needs pre_weight")
+    fn = _fns.get("st_residual_norm") or _fn("st_residual_norm", _vp, *[_cp] * 10)
+    rc = fn(context(dev), None if x is None else _desc(x), _desc(residual),
+            None if post_weight is None else _desc(post_weight), None if gate is None else _desc(gate),
+            None if pre_weight is None else _desc(pre_weight), d_out, d_normed, d_scale,
+            _OPTIONS.pack(alpha, eps, weight_offset), _exec_desc(dev))
     if rc != N.ST_OK:
         N.check(rc, "residual_norm")
     return ResidualNorm(residual if out is None else out, normed, scale)
@@ -112,30 +121,41 @@ def residual_norm_backward(d_residual: torch.Tensor | None, d_normed: torch.Tens
     like = d_residual if d_residual is not None else d_normed
     if like is None:
         raise ValueError("one of d_residual and d_normed must be given")
-    if like.dim() != 2:
+    shape = like.shape
+    if len(shape) != 2:
         raise ValueError("gradients must be 2D tensors.")
     dev = _device_of(like, d_normed, x, residual, post_weight, gate, pre_weight)
-    rows, cols = like.shape
-    device = like.device
+    rows, cols = shape
     stream = residual if residual is not None else like
-    dr = torch.empty((rows, cols), dtype=stream.dtype, device=device)
-    dx = torch.empty((rows, cols), dtype=x.dtype, device=device) if x is not None else None
-    dpost = torch.empty(cols, dtype=torch.float32, device=device) if post_weight is not None else None
-    dpre = torch.empty(cols, dtype=torch.float32, device=device) if pre_weight is not None else None
-    dgate = None
+    pitch = max(cols, 1)
+    for t in (stream, x):
+        if t is not None and t.dtype not in _ALL_CODES:
+            raise ValueError(f"unsupported dtype {t.dtype}")
+    dr, d_dr = _new(like, rows, cols, pitch, 1, stream.dtype)
+    dx, d_dx = (None, None) if x is None else _new(like, rows, cols, pitch, 1, x.dtype)
+    # the sums over rows are one allocation: dpost, dpre, dgate
+    sums = like.new_empty_strided((3, pitch), (pitch, 1), dtype=torch.float32)
+    base = sums.data_ptr()
+    dpost = dpre = dgate = d_dpost = d_dpre = d_dgate = None
+    if post_weight is not None:
+        dpost, d_dpost = sums[0, :cols], _pack(base, N.ST_F32, 1, cols, 0, 1, 0)
+    if pre_weight is not None:
+        dpre, d_dpre = sums[1, :cols], _pack(base + 4 * pitch, N.ST_F32, 1, cols, 0, 1, 0)
     if gate is not None:
         full = gate.dim() == 2 and gate.shape[0] == rows and gate.shape[1] == cols
-        dgate = torch.empty(gate.shape, dtype=gate.dtype if full else torch.float32, device=device)
+        dgate = torch.empty(gate.shape, dtype=gate.dtype if full else torch.float32, device=like.device)
+        d_dgate = _desc(dgate)
     size = ctypes.c_uint64(0)
-    rc = _fn("st_residual_norm_backward_workspace", ctypes.c_int64, ctypes.c_int64, _vp)(rows, cols,
-                                                                                        ctypes.addressof(size))
+    fn = _fns.get("st_residual_norm_backward_workspace") or _fn("st_residual_norm_backward_workspace", ctypes.c_int64,
+                                                               ctypes.c_int64, _vp)
+    rc = fn(rows, cols, ctypes.addressof(size))
     if rc != N.ST_OK:
         N.check(rc, "residual_norm_backward")
-    workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
-    rc = _fn("st_residual_norm_backward", _vp, *[_cp] * 12, _vp, _u64, _cp, _cp)(
-        context(dev), _opt(d_residual), _opt(d_normed), _opt(x), _opt(residual), _opt(post_weight), _opt(gate),
-        _opt(pre_weight), _opt(dx), _desc(dr), _opt(dpost), _opt(dgate), _opt(dpre), workspace.data_ptr(), size.value,
-        _OPTIONS.pack(alpha, eps, weight_offset), _exec_desc(dev))
+    workspace = like.new_empty_strided((size.value,), (1,), dtype=torch.uint8)
+    fn = _fns.get("st_residual_norm_backward") or _fn("st_residual_norm_backward", _vp, *[_cp] * 12, _vp, _u64, _cp, _cp)
+    rc = fn(context(dev), _opt(d_residual), _opt(d_normed), _opt(x), _opt(residual), _opt(post_weight), _opt(gate),
+            _opt(pre_weight), d_dx, d_dr, d_dpost, d_dgate, d_dpre, workspace.data_ptr(), size.value,
+            _OPTIONS.pack(alpha, eps, weight_offset), _exec_desc(dev))
     if rc != N.ST_OK:
         N.check(rc, "residual_norm_backward")
     return ResidualNormGrads(dx, dr, dpost, dgate, dpre)
