@@ -113,9 +113,21 @@ __device__ __forceinline__ void tmem_loaded(uint32_t *r) {
     for (int i = 0; i < N; i += 8)
         asm volatile("tcgen05.wait::ld.sync.aligned;"
                      : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
-                       "+r"(r[i + 6]), "+r"(r[i + 7])
-                     :
-                     : "memory");
+                       "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+
+// The four MMAs of a block, by one elected lane: descriptors of its first
+// 32 elements along K, each next one a fixed step further in the address
+// field (shared memory ends below 2^18, so the field does not overflow).
+template <bool R_MN, bool C_MN, bool PAIR>
+__device__ __forceinline__ void issue_block(uint32_t d_tmem, uint64_t dr, uint64_t dc, uint32_t idesc) {
+    // K-major: 32 bytes further along the 128-byte span; otherwise 32 K rows of 128 bytes
+    constexpr uint64_t kStepR = (R_MN ? kMmaK * 128 : kMmaK) >> 4, kStepC = (C_MN ? kMmaK * 128 : kMmaK) >> 4;
+#pragma unroll
+    for (int ks = 0; ks < kBlockK / kMmaK; ++ks) {
+        if constexpr (PAIR) tc_mma_f8_pair(d_tmem, dr + ks * kStepR, dc + ks * kStepC, idesc, ks != 0 ? 1u : 0u);
+        else tc_mma_f8(d_tmem, dr + ks * kStepR, dc + ks * kStepC, idesc, ks != 0 ? 1u : 0u);
+    }
 }
 
 __device__ __forceinline__ void copy_4_async(uint32_t dst, const float *src, bool valid) {
@@ -288,11 +300,12 @@ struct Fp8Cfg {
     static constexpr int kRowBytes = kTileRows * kBlockK;
     static constexpr int kColBytes = BN * kBlockK;
     static constexpr int kStageBytes = kRowBytes + kColBytes;
-    // BN 128 fills an SM's TMEM (4 x 128 columns) and shared memory alone;
-    // narrower tiles leave room for two CTAs per SM
-    static constexpr int kStages = BN == 128 ? 6 : (BN == 64 ? 4 : 5);
-    static constexpr int kAccs = 4;
-    static constexpr int kTmemCols = kAccs * BN;
+    // Stage and accumulator of a block have one index: the commit that hands
+    // over the accumulator frees the stage as well.  BN 128 fills an SM's
+    // TMEM (4 x 128 columns) alone; narrower tiles leave room for two CTAs.
+    static constexpr int kStages = BN >= 64 ? 4 : 5;
+    static constexpr int kTmemCols = BN == 16 ? 128 : BN == 32 ? 256 : kStages * BN;  // powers of two
+    static_assert(kStages * BN <= kTmemCols, "the accumulators fit");
     using Ring = ScaleRing<kTileRows, BN, CVEC, 2>;
     static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + Ring::kBytes + 1024;
     static_assert(kSmemBytes <= (BN == 128 ? 232448 : 115712), "shared memory of one (two) CTAs per SM");
@@ -370,28 +383,24 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::kStages * Cfg::kStageBytes);
-    constexpr int kBars = 2 * Cfg::kStages + 2 * Cfg::kAccs + 1;
+    constexpr int kBars = 3 * Cfg::kStages + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars + Ring::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t bar0 = smem_addr(bars);
-    auto full_bar = [&](int s) { return bar0 + 8u * s; };
-    auto empty_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };
-    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + a); };
-    auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + Cfg::kAccs + a); };
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };                        // loads landed
+    auto done_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };       // MMAs done: stage free, accumulator full
+    auto empty_bar = [&](int s) { return bar0 + 8u * (2 * Cfg::kStages + s); };  // accumulator read
     const uint32_t drain_bar = bar0 + 8u * (kBars - 1);
     const Ring ring{reinterpret_cast<float *>(smem + Cfg::kStages * Cfg::kStageBytes + kBarBytes), bar0 + 8u * kBars};
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
             mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), 1);
-        }
-        for (int a = 0; a < Cfg::kAccs; ++a) {
-            mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), kScaleWarps);
+            mbar_init(done_bar(s), 1);
+            mbar_init(empty_bar(s), kScaleWarps);
         }
         mbar_init(drain_bar, 1);
         ring.init(kScaleWarps);
@@ -429,12 +438,13 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
         if (lane == 0) {
-            const uint64_t pol = l2_policy_evict_last();
+            // rows that one column tile reads pass through L2 once
+            const uint64_t pol = l2_policy_evict_last(), row_pol = p.tiles_c > 1 ? pol : l2_policy_evict_first();
             int s = 0, issued = 0;
             uint32_t ph = 0;
             bool ok = true;
             for (int b = b0; b < b1; ++b, ++issued) {
-                if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
+                if (!mbar_wait(done_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
                     ok = false;
                     break;
                 }
@@ -442,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
                 const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
                 const uint32_t sc = sr + Cfg::kRowBytes;
                 const int k0 = b * kBlockK;
-                if constexpr (R_MN) tma_load_2d(sr, &tmap_r, full_bar(s), r0, k0, pol);
-                else tma_load_2d(sr, &tmap_r, full_bar(s), k0, r0, pol);
+                if constexpr (R_MN) tma_load_2d(sr, &tmap_r, full_bar(s), r0, k0, row_pol);
+                else tma_load_2d(sr, &tmap_r, full_bar(s), k0, r0, row_pol);
                 if constexpr (C_MN) tma_load_2d(sc, &tmap_c, full_bar(s), c0, k0, pol);
                 else tma_load_2d(sc, &tmap_c, full_bar(s), k0, c0, pol);
                 if (++s == Cfg::kStages) {
@@ -459,38 +469,28 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
         }
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
-        int s = 0, a = 0;
-        uint32_t ph = 0, aph = 0;
+        int s = 0;
+        uint32_t ph = 0;
         bool ok = true;
+        const uint64_t dr0 = smem_desc_sw128(smem_addr(smem), R_MN ? 128 * 128 : 16, 1024);
+        const uint64_t dc0 = smem_desc_sw128(smem_addr(smem) + Cfg::kRowBytes, C_MN ? 128 * 128 : 16, 1024);
         for (int b = b0; b < b1; ++b) {
-            const bool ready = mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns) &&
-                               mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns);
+            const bool ready = mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns) &&
+                               mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns);
             if (!__all_sync(0xffffffffu, ready)) {
                 ok = false;
                 break;
             }
             tc_fence_after_sync();
-            const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
-            const uint32_t sc = sr + Cfg::kRowBytes;
             if (elect_one()) {
-#pragma unroll
-                for (int ks = 0; ks < kBlockK / kMmaK; ++ks) {
-                    // K-major: 32 bytes further along the 128-byte span; otherwise 32 K rows of 128 bytes
-                    const uint64_t dr = smem_desc_sw128(sr + ks * (R_MN ? kMmaK * 128 : kMmaK), R_MN ? 128 * 128 : 16, 1024);
-                    const uint64_t dc = smem_desc_sw128(sc + ks * (C_MN ? kMmaK * 128 : kMmaK), C_MN ? 128 * 128 : 16, 1024);
-                    tc_mma_f8(tmem_base + static_cast<uint32_t>(a * BN), dr, dc, p.idesc, ks != 0 ? 1u : 0u);
-                }
-                tc_commit(empty_bar(s));
-                tc_commit(tfull_bar(a));
+                const uint64_t step = static_cast<uint64_t>(s) * (Cfg::kStageBytes >> 4);
+                issue_block<R_MN, C_MN, false>(tmem_base + static_cast<uint32_t>(s * BN), dr0 + step, dc0 + step, p.idesc);
+                tc_commit(done_bar(s));
             }
             __syncwarp();
             if (++s == Cfg::kStages) {
                 s = 0;
                 ph ^= 1u;
-            }
-            if (++a == Cfg::kAccs) {
-                a = 0;
-                aph ^= 1u;
             }
         }
         if (!ok) {
@@ -511,9 +511,9 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
 #pragma unroll
         for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
         ScalePosition at;
-        const bool ok = scale_blocks<BN, (BN == 128 ? 32 : BN >= 32 ? 16 : 8), CVEC, Cfg::kAccs, BN>(
-            acc, b1 - b0, tmem_base + (static_cast<uint32_t>(g * 32) << 16), row_in_tile, 0, ring, at, tfull_bar,
-            [&](int a) { mbar_arrive_relaxed(tempty_bar(a)); }, lane, abort_flag, p.timeout_ns);
+        const bool ok = scale_blocks<BN, (BN == 128 ? 32 : BN >= 32 ? 16 : 8), CVEC, Cfg::kStages, BN>(
+            acc, b1 - b0, tmem_base + (static_cast<uint32_t>(g * 32) << 16), row_in_tile, 0, ring, at, done_bar,
+            [&](int a) { mbar_arrive_relaxed(empty_bar(a)); }, lane, abort_flag, p.timeout_ns);
         if (!ok) {
             *abort_flag = 1;
             if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
@@ -749,29 +749,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 int s = 0, a = 0;
                 uint32_t ph = 0, aph = 0;
                 bool ok = true;
+                const uint64_t dr0 = smem_desc_sw128(smem_addr(smem), R_MN ? 128 * 128 : 16, 1024);
+                const uint64_t dc0 = smem_desc_sw128(smem_addr(smem) + Cfg::kRowBytes, C_MN ? 128 * 128 : 16, 1024);
                 for (int t = pair; ok && t < tiles; t += pairs) {
                     for (int b = 0; b < p.k_blocks; ++b) {
-                        const bool ready = mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns) &&
-                                           mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns);
+                        const bool ready = mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns) &&
+                                           mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns);
                         if (!__all_sync(0xffffffffu, ready)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after_sync();
-                        const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
-                        const uint32_t sc = sr + Cfg::kRowBytes;
                         if (elect_one()) {
-#pragma unroll
-                            for (int ks = 0; ks < kBlockK / kMmaK; ++ks) {
-                                const uint64_t dr =
-                                    smem_desc_sw128(sr + ks * (R_MN ? kMmaK * 128 : kMmaK), R_MN ? 128 * 128 : 16, 1024);
-                                const uint64_t dc =
-                                    smem_desc_sw128(sc + ks * (C_MN ? kMmaK * 128 : kMmaK), C_MN ? 128 * 128 : 16, 1024);
-                                tc_mma_f8_pair(tmem_base + static_cast<uint32_t>(a * kPairCols), dr, dc, p.idesc,
-                                               ks != 0 ? 1u : 0u);
-                            }
-                            tc_commit_pair_multicast(empty_bar(s), 3);
+                            const uint64_t step = static_cast<uint64_t>(s) * (Cfg::kStageBytes >> 4);
+                            issue_block<R_MN, C_MN, true>(tmem_base + static_cast<uint32_t>(a * kPairCols), dr0 + step,
+                                                          dc0 + step, p.idesc);
                             tc_commit_pair_multicast(tfull_bar(a), 3);
+                            tc_commit_pair_multicast(empty_bar(s), 3);
                         }
                         __syncwarp();
                         if (++s == Cfg::kStages) {
@@ -1099,6 +1093,47 @@ Access access_of(const Fp8Operand &o) {
     return {mn, true, ((mn ? o.rows : o.k) + 15) / 16 * 16};
 }
 
+// Tile shape and split of a product: the least estimated time, in SM cycles.
+// A wave of CTAs costs its blocks of K and what a CTA spends before and after
+// them, each about as measured on B200 (block: scaling included; alone, two
+// CTAs on an SM take 1.5 times as long; ends: prologue, first loads and the
+// store, with the exchange where a cluster shares a tile).
+struct Fp8Plan {
+    bool pair;
+    int bn, split;
+};
+
+Fp8Plan plan_fp8(int64_t rows, int64_t cols, int64_t k_blocks, bool k_major, int sm_count) {
+    Fp8Plan best{false, 128, 1};
+    double least = 1e300;
+    auto offer = [&](bool pair, int bn, int split, int64_t ctas, int64_t slots, double block, double ends) {
+        const double t = static_cast<double>(cdiv(ctas, slots)) * (static_cast<double>(cdiv(k_blocks, split)) * block + ends);
+        if (t < least) {
+            least = t;
+            best = Fp8Plan{pair, bn, split};
+        }
+    };
+    struct Shape {
+        int bn;
+        double block, ends, join;
+    };
+    static const Shape shapes[] = {{16, 350, 2300, 1700}, {32, 380, 2400, 2100}, {64, 450, 2700, 2800}, {128, 700, 3500, 7000}};
+    for (const Shape &s : shapes) {
+        // no narrower than the columns need, unless tiles of all of them would leave SMs idle
+        if (s.bn < 64 && s.bn < cols) continue;
+        if (s.bn < 128 && !k_major) continue;
+        const int64_t tiles = cdiv(rows, kTileRows) * cdiv(cols, s.bn);
+        const int per_sm = s.bn == 128 ? 1 : 2;
+        for (int split = 1; split <= 8 && split <= k_blocks; split *= 2) {
+            const int64_t ctas = tiles * split;
+            offer(false, s.bn, split, ctas, static_cast<int64_t>(sm_count) * per_sm,
+                  ctas > sm_count && per_sm == 2 ? 1.5 * s.block : s.block, s.ends + (split > 1 ? s.join : 0));
+        }
+    }
+    if (cols > 64) offer(true, 128, 1, cdiv(rows, 256) * cdiv(cols, 256), sm_count / 2, 1050, 7000);
+    return best;
+}
+
 int64_t copy_bytes(const Fp8Operand &o, const Access &a) {
     return a.copy ? ((a.mn ? o.k : o.rows) * a.ld + 255) / 256 * 256 : 0;
 }
@@ -1147,20 +1182,17 @@ int launch_gemm_fp8(const GemmFp8Args &g, void *workspace, int sm_count, int *de
     const bool swap = m <= 64 && m <= n && !acc[0].mn;
     const int ri = swap ? 1 : 0, ci = swap ? 0 : 1;
     const Fp8Operand &r = op[ri], &c = op[ci];
-    // 256 x 256 tiles of CTA pairs once they fill most of the pairs
-    const bool pair = !swap && n > 64 && cdiv(m, 256) * cdiv(n, 256) * 4 >= sm_count / 2 * 3;
-    int bn = 128;
-    if (!pair && !acc[ci].mn) bn = c.rows <= 16 ? 16 : c.rows <= 32 ? 32 : c.rows <= 64 ? 64 : 128;
+    const Fp8Plan plan = plan_fp8(r.rows, c.rows, cdiv(k, kBlockK), !acc[ci].mn, sm_count);
+    const bool pair = plan.pair;
+    const int bn = plan.bn;
     Fp8Params p{};
     p.rows = static_cast<int>(r.rows);
     p.cols = static_cast<int>(c.rows);
     p.k_blocks = static_cast<int>(cdiv(k, kBlockK));
     p.tiles_r = static_cast<int>(cdiv(r.rows, pair ? 2 * kTileRows : kTileRows));
     p.tiles_c = static_cast<int>(cdiv(c.rows, pair ? kPairCols : bn));
+    p.split = plan.split;
     const int64_t tiles = static_cast<int64_t>(p.tiles_r) * p.tiles_c;
-    const int64_t slots = static_cast<int64_t>(sm_count) * (bn == 128 ? 1 : 2);
-    p.split = 1;
-    while (!pair && p.split < 8 && tiles * p.split * 2 <= slots && p.k_blocks >= p.split * 2 * 2) p.split *= 2;
     if (tiles * p.split > INT32_MAX) return fail(ST_ERR_UNSUPPORTED, "matmul_fp8: too many output tiles");
     p.rs = static_cast<const float *>(r.scale);
     p.rs_i = r.scale_row;
