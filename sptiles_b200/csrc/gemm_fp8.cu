@@ -235,6 +235,16 @@ __device__ __forceinline__ bool scale_blocks(float (&acc)[COLS], int n, uint32_t
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
             uint32_t *x = v[j & 1];
+            // CVEC: the step's scales while its columns are on their way
+            uint64_t scales[CVEC ? STEP / 2 : 1];
+            if constexpr (CVEC) {
+#pragma unroll
+                for (int i = 0; i < STEP; i += 4) {
+                    const float4 c = *reinterpret_cast<const float4 *>(cols + j * STEP + i);
+                    scales[i / 2] = mul2(pack2(both, both), pack2(c.x, c.y));
+                    scales[i / 2 + 1] = mul2(pack2(both, both), pack2(c.z, c.w));
+                }
+            }
             tmem_loaded<STEP>(x);
             if (j + 1 < kSteps) {
                 tmem_load<STEP>(t + static_cast<uint32_t>(at.a * STRIDE + (j + 1) * STEP), v[(j + 1) & 1]);
@@ -252,21 +262,10 @@ __device__ __forceinline__ bool scale_blocks(float (&acc)[COLS], int n, uint32_t
                     tmem_load<STEP>(t + static_cast<uint32_t>(at.a * STRIDE), v[0]);
                 }
             }
+            float *s = acc + j * STEP;
 #pragma unroll
-            for (int i = 0; i < STEP; i += 4) {
-                float *s = acc + j * STEP + i;
-                if constexpr (CVEC) {
-                    const float4 c = *reinterpret_cast<const float4 *>(cols + j * STEP + i);
-                    const uint64_t r2 = pack2(both, both), s0 = mul2(r2, pack2(c.x, c.y)), s1 = mul2(r2, pack2(c.z, c.w));
-                    s[0] = __fmaf_rn(__uint_as_float(x[i]), lo2(s0), s[0]);
-                    s[1] = __fmaf_rn(__uint_as_float(x[i + 1]), hi2(s0), s[1]);
-                    s[2] = __fmaf_rn(__uint_as_float(x[i + 2]), lo2(s1), s[2]);
-                    s[3] = __fmaf_rn(__uint_as_float(x[i + 3]), hi2(s1), s[3]);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) s[q] = __fmaf_rn(__uint_as_float(x[i + q]), both, s[q]);
-                }
-            }
+            for (int i = 0; i < STEP; ++i)
+                s[i] = __fmaf_rn(__uint_as_float(x[i]), CVEC ? (i & 1 ? hi2(scales[i / 2]) : lo2(scales[i / 2])) : both, s[i]);
         }
         if (k == kBatch - 1 || b + 1 == n) {
             __syncwarp();
@@ -292,11 +291,14 @@ __device__ __forceinline__ void drain_ring(int issued, int stages, Bar bar, uint
 }
 
 // ---------------------------------------------------------------- one CTA, 128 x BN tiles
-constexpr int kScaleWarps = 4;
-constexpr int kThreads = 32 * (3 + kScaleWarps);  // warps 0 TMA, 1 MMA, 2..5 scaling, 6 scales
 
 template <int BN, bool CVEC>
 struct Fp8Cfg {
+    // warps 0 TMA, 1 MMA, 2.. scaling, the last one scales; two scaling warps
+    // share a quarter of the lanes where a tile has the columns for both
+    static constexpr int kScaleWarps = BN >= 64 ? 8 : 4;
+    static constexpr int kWarpCols = BN / (kScaleWarps / 4);
+    static constexpr int kThreads = 32 * (3 + kScaleWarps);
     static constexpr int kRowBytes = kTileRows * kBlockK;
     static constexpr int kColBytes = BN * kBlockK;
     static constexpr int kStageBytes = kRowBytes + kColBytes;
@@ -312,18 +314,19 @@ struct Fp8Cfg {
     static_assert(kStages * kStageBytes >= kTileRows * (BN + 4 * 8) * 4, "the ring holds eight parts' sums of its columns");
 };
 
-// Thread `first` of 128: its share of 128 rows x `own` columns (a power of
-// two, 4 at least), added over the parts of sums [part][row][own + 4].  By
-// rows, 4 columns of every (512 / own)th row; else all columns of one row.
-template <typename T>
+// Thread `first` of THREADS: its share of 128 rows x `own` columns (a power
+// of two, 4 at least), added over the parts of sums [part][row][own + 4].
+// By rows, the same 4 columns of every (4 THREADS / own)th row; else every
+// (THREADS / 128)th 4 columns of one row.
+template <typename T, int THREADS>
 __device__ __forceinline__ void store_sums(const Fp8Params &p, const float4 *sums, int first, int own, int own_shift,
                                            int parts, int r0, int col0) {
     const int quads = own / 4, pitch = own / 4 + 1;
     const bool by_rows = p.c_c == 1;
-    const int quad0 = by_rows ? first & (quads - 1) : 0, r_first = by_rows ? first >> (own_shift - 2) : first;
-    const int dr = by_rows ? 4 * 128 / own : 0, dq = by_rows ? 0 : 1;
+    const int quad0 = by_rows ? first & (quads - 1) : first >> 7, r_first = by_rows ? first >> (own_shift - 2) : first & 127;
+    const int dr = by_rows ? 4 * THREADS / own : 0, dq = by_rows ? 0 : THREADS / 128;
     T *c = static_cast<T *>(p.c) + (r0 + r_first) * p.c_r + (col0 + 4 * quad0) * p.c_c;
-    const int64_t dc = by_rows ? dr * p.c_r : 4 * p.c_c;
+    const int64_t dc = by_rows ? dr * p.c_r : 4 * dq * p.c_c;
     const int left = p.cols - col0 - 4 * quad0;  // columns from this thread's first on
     const bool four = by_rows && left >= 4 && reinterpret_cast<uintptr_t>(p.c) % (4 * sizeof(T)) == 0 && p.c_r % 4 == 0 &&
                       col0 % 4 == 0;
@@ -337,8 +340,9 @@ __device__ __forceinline__ void store_sums(const Fp8Params &p, const float4 *sum
         }
     }
 #pragma unroll 2
-    for (int i = 0; i < quads; ++i, c += dc) {
+    for (int i = 0;; ++i, c += dc) {
         const int r = r_first + i * dr, quad = quad0 + i * dq;
+        if (r >= kTileRows || quad >= quads || r0 + r >= p.rows) break;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int q = 0; q < parts; ++q) {
             const float4 x = sums[(q * kTileRows + r) * pitch + quad];
@@ -353,7 +357,6 @@ __device__ __forceinline__ void store_sums(const Fp8Params &p, const float4 *sum
             v.z += add[2];
             v.w += add[3];
         }
-        if (r0 + r >= p.rows) break;
         T o[4];
         from_float(v.x, o[0]);
         from_float(v.y, o[1]);
@@ -375,7 +378,7 @@ __device__ __forceinline__ void store_sums(const Fp8Params &p, const float4 *sum
 // R_MN / C_MN: the operand is stored with its rows (columns) contiguous
 // instead of K.  CVEC: the column scale differs inside the tile.
 template <int BN, bool R_MN, bool C_MN, bool CVEC>
-__global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
+__global__ void __launch_bounds__(Fp8Cfg<BN, CVEC>::kThreads, BN == 128 ? 1 : 2)
     gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
                     const Fp8Params p) {
     using Cfg = Fp8Cfg<BN, CVEC>;
@@ -400,10 +403,10 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
         for (int s = 0; s < Cfg::kStages; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(done_bar(s), 1);
-            mbar_init(empty_bar(s), kScaleWarps);
+            mbar_init(empty_bar(s), Cfg::kScaleWarps);
         }
         mbar_init(drain_bar, 1);
-        ring.init(kScaleWarps);
+        ring.init(Cfg::kScaleWarps);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -431,9 +434,10 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     const int b1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / split);
 
     // scaling warps: TMEM lane = row of the tile
-    const int g = warp & 3;
+    constexpr int kWarpCols = Cfg::kWarpCols;
+    const int g = warp & 3, col_in_tile = ((warp - 2) >> 2) * kWarpCols;
     const int row_in_tile = g * 32 + lane;
-    float acc[BN];
+    float acc[kWarpCols];
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
@@ -500,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
         if (elect_one()) tc_commit(drain_bar);
         __syncwarp();
         (void)mbar_wait(drain_bar, 0, abort_flag, p.timeout_ns);
-    } else if (warp == 2 + kScaleWarps) {
+    } else if (warp == 2 + Cfg::kScaleWarps) {
         // ------------------------------------------------ scales
         int d = 0;
         uint32_t dph = 0;
@@ -509,10 +513,11 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     } else {
         // ------------------------------------------------ scaling
 #pragma unroll
-        for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
+        for (int j = 0; j < kWarpCols; ++j) acc[j] = 0.0f;
         ScalePosition at;
-        const bool ok = scale_blocks<BN, (BN == 128 ? 32 : BN >= 32 ? 16 : 8), CVEC, Cfg::kStages, BN>(
-            acc, b1 - b0, tmem_base + (static_cast<uint32_t>(g * 32) << 16), row_in_tile, 0, ring, at, done_bar,
+        const bool ok = scale_blocks<kWarpCols, (kWarpCols >= 64 ? (CVEC ? 16 : 32) : BN == 32 ? 16 : 8), CVEC, Cfg::kStages, BN>(
+            acc, b1 - b0, tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(col_in_tile), row_in_tile,
+            CVEC ? col_in_tile : 0, ring, at, done_bar,
             [&](int a) { mbar_arrive_relaxed(empty_bar(a)); }, lane, abort_flag, p.timeout_ns);
         if (!ok) {
             *abort_flag = 1;
@@ -521,21 +526,21 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
     }
 
     // ------------------------------------------------ C
-    const bool scaler = warp >= 2 && warp < 2 + kScaleWarps;
+    const bool scaler = warp >= 2 && warp < 2 + Cfg::kScaleWarps;
     const int es = p.c_dtype == ST_F32 ? 4 : 2;
     const bool wide = split == 1 && p.c_c == 1 && c0 + BN <= p.cols && p.bias == nullptr &&
                       (reinterpret_cast<uintptr_t>(p.c) & 15u) == 0 && (p.c_r * es) % 16 == 0;
     if (wide) {  // whole 16-byte pieces of each row, straight from registers
         const int row = r0 + row_in_tile;
         if (scaler && row < p.rows) {
-            uint8_t *dst = static_cast<uint8_t *>(p.c) + (row * p.c_r + c0) * es;
+            uint8_t *dst = static_cast<uint8_t *>(p.c) + (row * p.c_r + c0 + col_in_tile) * es;
             if (p.c_dtype == ST_F32) {
 #pragma unroll
-                for (int j = 0; j < BN; j += 4)
+                for (int j = 0; j < kWarpCols; j += 4)
                     reinterpret_cast<float4 *>(dst)[j / 4] = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
             } else {
 #pragma unroll
-                for (int j = 0; j < BN; j += 8) {
+                for (int j = 0; j < kWarpCols; j += 8) {
                     uint32_t w[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) w[i] = pack_16(acc[j + 2 * i], acc[j + 2 * i + 1], p.c_dtype);
@@ -558,9 +563,10 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
         if (scaler) {
             const uint32_t mine = smem_addr(smem) + 4u * static_cast<uint32_t>((part * kTileRows + row_in_tile) * stride);
 #pragma unroll
-            for (int j = 0; j < BN; j += 4) {
-                const uint32_t to = (split == 1 ? mine : map_to_rank(mine, static_cast<uint32_t>(j >> own_shift))) +
-                                    4u * static_cast<uint32_t>(j & (own - 1));
+            for (int j = 0; j < kWarpCols; j += 4) {
+                const int col = col_in_tile + j;
+                const uint32_t to = (split == 1 ? mine : map_to_rank(mine, static_cast<uint32_t>(col >> own_shift))) +
+                                    4u * static_cast<uint32_t>(col & (own - 1));
                 st_cluster_v4(to, acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
             }
         }
@@ -571,9 +577,9 @@ __global__ void __launch_bounds__(kThreads, BN == 128 ? 1 : 2)
             const float4 *sums = reinterpret_cast<const float4 *>(smem);
             const int first = (warp - 2) * 32 + lane;
             const int col0 = c0 + part * own;
-            if (p.c_dtype == ST_F32) store_sums<float>(p, sums, first, own, own_shift, split, r0, col0);
-            else if (p.c_dtype == ST_F16) store_sums<__half>(p, sums, first, own, own_shift, split, r0, col0);
-            else store_sums<__nv_bfloat16>(p, sums, first, own, own_shift, split, r0, col0);
+            if (p.c_dtype == ST_F32) store_sums<float, 32 * Cfg::kScaleWarps>(p, sums, first, own, own_shift, split, r0, col0);
+            else if (p.c_dtype == ST_F16) store_sums<__half, 32 * Cfg::kScaleWarps>(p, sums, first, own, own_shift, split, r0, col0);
+            else store_sums<__nv_bfloat16, 32 * Cfg::kScaleWarps>(p, sums, first, own, own_shift, split, r0, col0);
         }
     }
     tc_fence_before_sync();
@@ -816,7 +822,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             float acc[kPairWarpCols];
 #pragma unroll
             for (int j = 0; j < kPairWarpCols; ++j) acc[j] = 0.0f;
-            ok = scale_blocks<kPairWarpCols, 32, CVEC, Cfg::kAccs, kPairCols>(
+            ok = scale_blocks<kPairWarpCols, CVEC ? 16 : 32, CVEC, Cfg::kAccs, kPairCols>(
                 acc, p.k_blocks, t_lane, g * 32 + lane, half * (CVEC ? kPairWarpCols : 1), ring, at, tfull_bar,
                 [&](int a) {
                     if (rank == 0) mbar_arrive_relaxed(tempty_bar(a));
@@ -984,7 +990,7 @@ int launch_instance(const CUtensorMap &mr, const CUtensorMap &mc, const Fp8Param
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.tiles_r) * p.tiles_c * p.split));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(Cfg::kThreads);
     cfg.dynamicSmemBytes = Cfg::kSmemBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
