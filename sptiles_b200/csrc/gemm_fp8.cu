@@ -160,9 +160,10 @@ struct ScaleRing {
     }
     __device__ __forceinline__ const float *rows(int d, int i) const { return slots + (d * kBatch + i) * kBlock; }
     __device__ __forceinline__ const float *cols(int d, int i) const { return rows(d, i) + ROWS; }
-    // The scales of blocks [b0, b1) of the tile at row r0, column c0; false after an abort.
-    __device__ __forceinline__ bool load(const Fp8Params &p, int r0, int c0, int b0, int b1, int lane, int &d, uint32_t &ph,
-                                         const volatile int *abort_flag) const {
+    // The scales of blocks b0, b0 + step, ... (count of them) of the tile at
+    // row r0, column c0; false after an abort.
+    __device__ __forceinline__ bool load(const Fp8Params &p, int r0, int c0, int b0, int step, int count, int lane, int &d,
+                                         uint32_t &ph, const volatile int *abort_flag) const {
         const float *src_r[ROWS / 32], *src_c[(kCols + 31) / 32];
         bool ok_r[ROWS / 32], ok_c[(kCols + 31) / 32];
 #pragma unroll
@@ -177,16 +178,17 @@ struct ScaleRing {
             ok_c[i] = j < kCols && c < p.cols;
             src_c[i] = p.cs + static_cast<int64_t>(ok_c[i] ? c >> p.cs_shift : 0) * p.cs_i;
         }
-        for (int b = b0; b < b1; b += kBatch) {
+        for (int done = 0; done < count; done += kBatch) {
             if (!__all_sync(0xffffffffu, mbar_wait(empty(d), ph ^ 1u, abort_flag, p.timeout_ns))) return false;
-            const int n = b1 - b < kBatch ? b1 - b : kBatch;
+            const int n = count - done < kBatch ? count - done : kBatch;
             for (int k = 0; k < n; ++k) {
+                const int b = b0 + (done + k) * step;
                 const uint32_t to_r = smem_addr(rows(d, k)) + 4u * lane, to_c = to_r + 4u * ROWS;
 #pragma unroll
-                for (int i = 0; i < ROWS / 32; ++i) copy_4_async(to_r + 128u * i, src_r[i] + (b + k) * p.rs_b, ok_r[i]);
+                for (int i = 0; i < ROWS / 32; ++i) copy_4_async(to_r + 128u * i, src_r[i] + b * p.rs_b, ok_r[i]);
 #pragma unroll
                 for (int i = 0; i < (kCols + 31) / 32; ++i)
-                    if (lane + 32 * i < kCols) copy_4_async(to_c + 128u * i, src_c[i] + (b + k) * p.cs_b, ok_c[i]);
+                    if (lane + 32 * i < kCols) copy_4_async(to_c + 128u * i, src_c[i] + b * p.cs_b, ok_c[i]);
             }
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(d)) : "memory");
             if (++d == DEPTH) {
@@ -430,8 +432,8 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, CVEC>::kThreads, BN == 128 ? 1 : 2)
     // neighbouring CTAs walk the row tiles of one column tile
     const int r0 = (tile % p.tiles_r) * kTileRows;
     const int c0 = (tile / p.tiles_r) * BN;
-    const int b0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * part / split);
-    const int b1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (part + 1) / split);
+    // blocks part, part + split, ...: a cluster's loads of a row lie next to each other
+    const int blocks = (p.k_blocks - part + split - 1) / split;
 
     // scaling warps: TMEM lane = row of the tile
     constexpr int kWarpCols = Cfg::kWarpCols;
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, CVEC>::kThreads, BN == 128 ? 1 : 2)
             int s = 0, issued = 0;
             uint32_t ph = 0;
             bool ok = true;
-            for (int b = b0; b < b1; ++b, ++issued) {
+            for (int b = part; b < p.k_blocks; b += split, ++issued) {
                 if (!mbar_wait(done_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
                     ok = false;
                     break;
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, CVEC>::kThreads, BN == 128 ? 1 : 2)
         bool ok = true;
         const uint64_t dr0 = smem_desc_sw128(smem_addr(smem), R_MN ? 128 * 128 : 16, 1024);
         const uint64_t dc0 = smem_desc_sw128(smem_addr(smem) + Cfg::kRowBytes, C_MN ? 128 * 128 : 16, 1024);
-        for (int b = b0; b < b1; ++b) {
+        for (int b = 0; b < blocks; ++b) {
             const bool ready = mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns) &&
                                mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns);
             if (!__all_sync(0xffffffffu, ready)) {
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, CVEC>::kThreads, BN == 128 ? 1 : 2)
         // ------------------------------------------------ scales
         int d = 0;
         uint32_t dph = 0;
-        if (!ring.load(p, r0, c0, b0, b1, lane, d, dph, abort_flag)) *abort_flag = 1;
+        if (!ring.load(p, r0, c0, part, split, blocks, lane, d, dph, abort_flag)) *abort_flag = 1;
         copies_done();
     } else {
         // ------------------------------------------------ scaling
@@ -516,7 +518,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, CVEC>::kThreads, BN == 128 ? 1 : 2)
         for (int j = 0; j < kWarpCols; ++j) acc[j] = 0.0f;
         ScalePosition at;
         const bool ok = scale_blocks<kWarpCols, (kWarpCols >= 64 ? (CVEC ? 16 : 32) : BN == 32 ? 16 : 8), CVEC, Cfg::kStages, BN>(
-            acc, b1 - b0, tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(col_in_tile), row_in_tile,
+            acc, blocks, tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(col_in_tile), row_in_tile,
             CVEC ? col_in_tile : 0, ring, at, done_bar,
             [&](int a) { mbar_arrive_relaxed(empty_bar(a)); }, lane, abort_flag, p.timeout_ns);
         if (!ok) {
@@ -799,8 +801,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             for (int t = pair; t < tiles; t += pairs) {
                 int tr, tc;
                 pair_tile(p, t, tr, tc);
-                if (!ring.load(p, tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows, tc * kPairCols, 0, p.k_blocks,
-                               lane, d, dph, abort_flag)) {
+                if (!ring.load(p, tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows, tc * kPairCols, 0, 1,
+                               p.k_blocks, lane, d, dph, abort_flag)) {
                     *abort_flag = 1;
                     break;
                 }
@@ -1099,44 +1101,43 @@ Access access_of(const Fp8Operand &o) {
     return {mn, true, ((mn ? o.rows : o.k) + 15) / 16 * 16};
 }
 
-// Tile shape and split of a product: the least estimated time, in SM cycles.
-// A wave of CTAs costs its blocks of K and what a CTA spends before and after
-// them, each about as measured on B200 (block: scaling included; alone, two
-// CTAs on an SM take 1.5 times as long; ends: prologue, first loads and the
-// store, with the exchange where a cluster shares a tile).
+// Tile shape and split of a product of one orientation: the least estimated
+// time.  A wave of CTAs costs its blocks of K and what a CTA spends outside
+// them; the figures are SM cycles fitted to B200 timings of 1 x 1024 x 4096 to
+// 8192^3 (within 10 % of most; e.g. 64 x 8192 x 8192 estimated 19.4 us on 128
+// columns and two parts, 21.3 on 64 columns and four, measured 20.6 and 22.7).
 struct Fp8Plan {
-    bool pair;
-    int bn, split;
+    bool pair = false;
+    int bn = 128, split = 1;
+    double cycles = 1e300;
 };
 
-Fp8Plan plan_fp8(int64_t rows, int64_t cols, int64_t k_blocks, bool k_major, int sm_count) {
-    Fp8Plan best{false, 128, 1};
-    double least = 1e300;
+Fp8Plan plan_fp8(int64_t rows, int64_t cols, int64_t k_blocks, bool k_major, bool column_scales, int sm_count) {
+    Fp8Plan best;
     auto offer = [&](bool pair, int bn, int split, int64_t ctas, int64_t slots, double block, double ends) {
         const double t = static_cast<double>(cdiv(ctas, slots)) * (static_cast<double>(cdiv(k_blocks, split)) * block + ends);
-        if (t < least) {
-            least = t;
-            best = Fp8Plan{pair, bn, split};
-        }
+        if (t < best.cycles) best = Fp8Plan{pair, bn, split, t};
     };
     struct Shape {
         int bn;
-        double block, ends, join;
+        double block, two, ends, join[3];  // a block alone on an SM, and beside another CTA; extra for 2, 4 and 8 parts
     };
-    static const Shape shapes[] = {{16, 350, 2300, 1700}, {32, 380, 2400, 2100}, {64, 450, 2700, 2800}, {128, 700, 3500, 7000}};
+    const Shape shapes[] = {{16, 600, 1000, 12000, {0, 0, 0}},
+                            {32, 700, 1050, 14000, {0, 0, 0}},
+                            {64, 1050, 1340, 18000, {0, 0, 5000}},
+                            {128, column_scales ? 890.0 : 620.0, 0, 9000, {7000, 11700, 16000}}};
     for (const Shape &s : shapes) {
-        // no narrower than the columns need, unless tiles of all of them would leave SMs idle
-        if (s.bn < 64 && s.bn < cols) continue;
-        if (s.bn < 128 && !k_major) continue;
+        if (s.bn < 128 && (!k_major || s.bn < (cols < 64 ? cols : 64))) continue;  // narrow boxes are K-major
         const int64_t tiles = cdiv(rows, kTileRows) * cdiv(cols, s.bn);
         const int per_sm = s.bn == 128 ? 1 : 2;
-        for (int split = 1; split <= 8 && split <= k_blocks; split *= 2) {
-            const int64_t ctas = tiles * split;
-            offer(false, s.bn, split, ctas, static_cast<int64_t>(sm_count) * per_sm,
-                  ctas > sm_count && per_sm == 2 ? 1.5 * s.block : s.block, s.ends + (split > 1 ? s.join : 0));
+        for (int parts = 0; parts <= 3 && (1 << parts) <= k_blocks; ++parts) {
+            const int64_t ctas = tiles << parts;
+            offer(false, s.bn, 1 << parts, ctas, static_cast<int64_t>(sm_count) * per_sm,
+                  ctas > sm_count && per_sm == 2 ? s.two : s.block, s.ends + (parts > 0 ? s.join[parts - 1] : 0));
         }
     }
-    if (cols > 64) offer(true, 128, 1, cdiv(rows, 256) * cdiv(cols, 256), sm_count / 2, 1050, 7000);
+    if (cols > 64)
+        offer(true, 128, 1, cdiv(rows, 256) * cdiv(cols, 256), sm_count / 2, column_scales ? 1480 : 1000, 11400);
     return best;
 }
 
@@ -1183,18 +1184,24 @@ int launch_gemm_fp8(const GemmFp8Args &g, void *workspace, int sm_count, int *de
         op[i].data = ws;
         ws += copy_bytes(op[i], acc[i]);
     }
-    // The smaller of M and N becomes the column operand where a tile of up
-    // to 64 columns covers it; its boxes are K-major.
-    const bool swap = m <= 64 && m <= n && !acc[0].mn;
+    // A becomes the row operand; or B does, where few rows of A then make a
+    // narrow tile's columns.
+    const int64_t k_blocks = cdiv(k, kBlockK);
+    Fp8Plan plan = plan_fp8(m, n, k_blocks, !acc[1].mn, g.b.scale_shift == 0, sm_count);
+    bool swap = false;
+    if (m <= 64 && !acc[0].mn) {
+        const Fp8Plan other = plan_fp8(n, m, k_blocks, true, true, sm_count);
+        swap = other.cycles < plan.cycles;
+        if (swap) plan = other;
+    }
     const int ri = swap ? 1 : 0, ci = swap ? 0 : 1;
     const Fp8Operand &r = op[ri], &c = op[ci];
-    const Fp8Plan plan = plan_fp8(r.rows, c.rows, cdiv(k, kBlockK), !acc[ci].mn, sm_count);
     const bool pair = plan.pair;
     const int bn = plan.bn;
     Fp8Params p{};
     p.rows = static_cast<int>(r.rows);
     p.cols = static_cast<int>(c.rows);
-    p.k_blocks = static_cast<int>(cdiv(k, kBlockK));
+    p.k_blocks = static_cast<int>(k_blocks);
     p.tiles_r = static_cast<int>(cdiv(r.rows, pair ? 2 * kTileRows : kTileRows));
     p.tiles_c = static_cast<int>(cdiv(c.rows, pair ? kPairCols : bn));
     p.split = plan.split;
