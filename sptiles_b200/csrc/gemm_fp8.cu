@@ -95,25 +95,35 @@ __device__ __forceinline__ void tmem_load_16(uint32_t taddr, uint32_t *r) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_load_x32(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
 template <int N>
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t *r) {
-    if constexpr (N == 8) {
-        tmem_load_8(taddr, r);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 16) tmem_load_16(taddr + i, r + i);
-    }
+    static_assert(N == 8 || N == 16 || N == 32, "one load");
+    if constexpr (N == 8) tmem_load_8(taddr, r);
+    else if constexpr (N == 16) tmem_load_16(taddr, r);
+    else tmem_load_x32(taddr, r);
 }
 
 // Wait for every load so far; the registers pass through, so that nothing
 // reads them before it.
 template <int N>
 __device__ __forceinline__ void tmem_loaded(uint32_t *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]));
 #pragma unroll
-    for (int i = 0; i < N; i += 8)
-        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                     : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
-                       "+r"(r[i + 6]), "+r"(r[i + 7]));
+    for (int i = 8; i < N; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                          "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
 // The four MMAs of a block, by one elected lane: descriptors of its first
