@@ -40,7 +40,7 @@ constexpr int64_t kMaxCols = 4 * kMaxThreads * 8;
 // Where a lane's 8 elements of a chunk lie.  VEC: next to each other;
 // otherwise 32 apart, so that a warp's scalar loads are contiguous.
 template <bool VEC>
-__device__ __forceinline__ int64_t element(int64_t base, int lane, int j) {
+__device__ __forceinline__ int element(int base, int lane, int j) {
     return VEC ? base + lane * 8 + j : base + lane + 32 * j;
 }
 
@@ -52,18 +52,22 @@ struct Raw8 {
 };
 
 template <typename T, bool VEC>
-__device__ __forceinline__ Raw8<T> load_raw(const NormView &view, int64_t r, int64_t base, int lane, int64_t cols) {
+__device__ __forceinline__ Raw8<T> load_raw(const NormView &view, int64_t r, int base, int lane, int cols) {
     Raw8<T> out;
     const T *row = static_cast<const T *>(view.p) + r * view.ld;
     if (VEC && base + lane * 8 + 8 <= cols) {
         const uint4 *src = reinterpret_cast<const uint4 *>(row + base + lane * 8);
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) out.w[i] = src[i];
+    } else if (!VEC && base + kChunk <= cols) {
+        T *e = reinterpret_cast<T *>(out.w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = row[base + lane + 32 * j];
     } else {
         T *e = reinterpret_cast<T *>(out.w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int64_t c = element<VEC>(base, lane, j);
+            const int c = element<VEC>(base, lane, j);
             if (c < cols) e[j] = row[c];
             else from_float(0.0f, e[j]);
         }
@@ -72,7 +76,7 @@ __device__ __forceinline__ Raw8<T> load_raw(const NormView &view, int64_t r, int
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *row, int64_t base, int lane, int64_t cols, float (&f)[8]) {
+__device__ __forceinline__ void load8(const T *row, int base, int lane, int cols, float (&f)[8]) {
     if (VEC && base + lane * 8 + 8 <= cols) {
         uint4 w[sizeof(T) / 2];
         const uint4 *src = reinterpret_cast<const uint4 *>(row + base + lane * 8);
@@ -81,17 +85,21 @@ __device__ __forceinline__ void load8(const T *row, int64_t base, int lane, int6
         const T *e = reinterpret_cast<const T *>(w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = to_float(e[j]);
+    } else if (!VEC && base + kChunk <= cols) {  // the whole warp is inside: no checks
+        row += base + lane;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = to_float(row[32 * j]);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int64_t c = element<VEC>(base, lane, j);
+            const int c = element<VEC>(base, lane, j);
             f[j] = c < cols ? to_float(row[c]) : 0.0f;
         }
     }
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T *row, int64_t base, int lane, int64_t cols, const float (&f)[8]) {
+__device__ __forceinline__ void store8(T *row, int base, int lane, int cols, const float (&f)[8]) {
     if (VEC && base + lane * 8 + 8 <= cols) {
         uint4 w[sizeof(T) / 2];
         T *e = reinterpret_cast<T *>(w);
@@ -100,10 +108,14 @@ __device__ __forceinline__ void store8(T *row, int64_t base, int lane, int64_t c
         uint4 *dst = reinterpret_cast<uint4 *>(row + base + lane * 8);
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) dst[i] = w[i];
+    } else if (!VEC && base + kChunk <= cols) {
+        row += base + lane;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) from_float(f[j], row[32 * j]);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int64_t c = element<VEC>(base, lane, j);
+            const int c = element<VEC>(base, lane, j);
             if (c < cols) from_float(f[j], row[c]);
         }
     }
@@ -111,7 +123,7 @@ __device__ __forceinline__ void store8(T *row, int64_t base, int lane, int64_t c
 
 // A weight or gate of type T or fp32.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8_of(const NormView &v, int64_t row, int64_t base, int lane, int64_t cols,
+__device__ __forceinline__ void load8_of(const NormView &v, int64_t row, int base, int lane, int cols,
                                          float (&f)[8]) {
     if (v.dtype == ST_F32) load8<float, VEC>(static_cast<const float *>(v.p) + row * v.ld, base, lane, cols, f);
     else load8<T, VEC>(static_cast<const T *>(v.p) + row * v.ld, base, lane, cols, f);
@@ -157,14 +169,14 @@ struct RowGroup {
         first = static_cast<int64_t>(blockIdx.x) * per_cta + (warps == 1 ? w : 0);
         step = static_cast<int64_t>(gridDim.x) * per_cta;
     }
-    __device__ __forceinline__ int64_t base(int v) const { return static_cast<int64_t>(v * warps + warp) * kChunk; }
+    __device__ __forceinline__ int base(int v) const { return (v * warps + warp) * kChunk; }
 };
 
 // 8 elements of a row's normed copy, in the branch's type or as 8-bit blocks.
 template <typename TX, bool VEC>
-__device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int64_t base, int lane, const float (&h)[8]) {
+__device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int base, int lane, int cols, const float (&h)[8]) {
     if (!p.h_fp8) {
-        store8<TX, VEC>(static_cast<TX *>(p.h.p) + row * p.h.ld, base, lane, p.cols, h);
+        store8<TX, VEC>(static_cast<TX *>(p.h.p) + row * p.h.ld, base, lane, cols, h);
         return;
     }
     // a chunk is two blocks of 128: VEC, 16 lanes each; otherwise the lanes' first and last four elements
@@ -179,8 +191,8 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
         for (int o = VEC ? 8 : 16; o > 0; o >>= 1) m[b] = max_abs(m[b], __shfl_xor_sync(0xffffffffu, m[b], o));
         const float scale = fp8_scale(m[b], limit);
         inverse[b] = __frcp_rn(scale);
-        const int64_t block = base / 128 + (VEC ? lane / 16 : b);
-        if ((VEC ? lane % 16 : lane) == 0 && block * 128 < p.cols) p.h_scale[row * p.hs0 + block * p.hs1] = scale;
+        const int block = base / 128 + (VEC ? lane / 16 : b);
+        if ((VEC ? lane % 16 : lane) == 0 && block * 128 < cols) p.h_scale[row * p.hs0 + block * p.hs1] = scale;
     }
     if constexpr (VEC) inverse[1] = inverse[0];
     uint32_t q[2];
@@ -189,59 +201,66 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
         q[b] = to_fp8x4(__fmul_rn(h[4 * b], inverse[b]), __fmul_rn(h[4 * b + 1], inverse[b]),
                         __fmul_rn(h[4 * b + 2], inverse[b]), __fmul_rn(h[4 * b + 3], inverse[b]), p.h_e5m2);
     uint8_t *to = static_cast<uint8_t *>(p.h.p) + row * p.h.ld;
-    if (VEC && base + lane * 8 + 8 <= p.cols) {
+    if (VEC && base + lane * 8 + 8 <= cols) {
         *reinterpret_cast<uint2 *>(to + base + lane * 8) = make_uint2(q[0], q[1]);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int64_t c = element<VEC>(base, lane, j);
-            if (c < p.cols) to[c] = static_cast<uint8_t>(q[j / 4] >> (8 * (j % 4)));
+            const int c = element<VEC>(base, lane, j);
+            if (c < cols) to[c] = static_cast<uint8_t>(q[j / 4] >> (8 * (j % 4)));
         }
     }
 }
 
+// Few rows, short ones, and any alignment: a CTA or a warp for each row.  All
+// of a row's reads, the weights among them, are under way before the first
+// sum where a thread has one chunk; longer rows read the weights when needed.
 template <typename TX, typename TR, int VPT, bool VEC>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormArgs p, int warps) {
+    constexpr bool kAhead = VPT == 1;
     pdl_wait();
     __shared__ float slots[2 * 3 * 32];
     const RowGroup g(warps);
+    const int cols = static_cast<int>(p.cols);
     const float inv_cols = 1.0f / static_cast<float>(p.cols);
+    const bool has_x = p.x.p != nullptr, has_post = p.post.p != nullptr, has_pre = p.pre.p != nullptr;
+    const bool wide_gate = p.gate_mode == kGateChannel || p.gate_mode == kGateFull;
     int slot = 0;
     for (int64_t row = g.first; row < p.rows; row += g.step) {
-        float r[VPT][8];
+        const int64_t gate_row = p.gate_mode == kGateFull ? row : 0;
+        float r[VPT][8], x[VPT][8], post[VPT][8], gate[VPT][8], pre[VPT][8];
+        float token = p.alpha;
+        if (p.gate_mode == kGateToken) token *= load1_of<TX>(p.gate, row);
 #pragma unroll
-        for (int v = 0; v < VPT; ++v)
-            load8<TR, VEC>(static_cast<const TR *>(p.r.p) + row * p.r.ld, g.base(v), g.lane, p.cols, r[v]);
-        if (p.x.p != nullptr) {
-            float x[VPT][8];
-#pragma unroll
-            for (int v = 0; v < VPT; ++v)
-                load8<TX, VEC>(static_cast<const TX *>(p.x.p) + row * p.x.ld, g.base(v), g.lane, p.cols, x[v]);
-            if (p.post.p != nullptr) {
+        for (int v = 0; v < VPT; ++v) {
+            if (has_x) load8<TX, VEC>(static_cast<const TX *>(p.x.p) + row * p.x.ld, g.base(v), g.lane, cols, x[v]);
+            load8<TR, VEC>(static_cast<const TR *>(p.r.p) + row * p.r.ld, g.base(v), g.lane, cols, r[v]);
+            if (kAhead && has_post) load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, cols, post[v]);
+            if (kAhead && wide_gate) load8_of<TX, VEC>(p.gate, gate_row, g.base(v), g.lane, cols, gate[v]);
+            if (kAhead && has_pre) load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, cols, pre[v]);
+        }
+        if (has_x) {
+            if (has_post) {
                 float s[1] = {0.0f};
 #pragma unroll
                 for (int v = 0; v < VPT; ++v)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) s[0] += x[v][j] * x[v][j];
                 row_sum(s, g.warps, g.warp, g.lane, slots, slot);
-                const float inv = 1.0f / sqrtf(s[0] * inv_cols + p.eps);
+                const float inv = rsqrtf(s[0] * inv_cols + p.eps);
 #pragma unroll
                 for (int v = 0; v < VPT; ++v) {
-                    float w[8];
-                    load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, p.cols, w);
+                    if (!kAhead) load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, cols, post[v]);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[v][j] *= inv * (w[j] + p.offset);
+                    for (int j = 0; j < 8; ++j) x[v][j] *= inv * (post[v][j] + p.offset);
                 }
             }
-            float token = p.alpha;
-            if (p.gate_mode == kGateToken) token *= load1_of<TX>(p.gate, row);
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                if (p.gate_mode == kGateChannel || p.gate_mode == kGateFull) {
-                    float w[8];
-                    load8_of<TX, VEC>(p.gate, p.gate_mode == kGateFull ? row : 0, g.base(v), g.lane, p.cols, w);
+                if (wide_gate) {
+                    if (!kAhead) load8_of<TX, VEC>(p.gate, gate_row, g.base(v), g.lane, cols, gate[v]);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[v][j] *= w[j];
+                    for (int j = 0; j < 8; ++j) x[v][j] *= gate[v][j];
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[v][j] += token * x[v][j];
@@ -250,24 +269,22 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormAr
         if (p.r_out.p != nullptr) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
-                store8<TR, VEC>(static_cast<TR *>(p.r_out.p) + row * p.r_out.ld, g.base(v), g.lane, p.cols, r[v]);
+                store8<TR, VEC>(static_cast<TR *>(p.r_out.p) + row * p.r_out.ld, g.base(v), g.lane, cols, r[v]);
         }
-        if (p.pre.p == nullptr) continue;
+        if (!has_pre) continue;
         float s[1] = {0.0f};
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
 #pragma unroll
             for (int j = 0; j < 8; ++j) s[0] += r[v][j] * r[v][j];
         row_sum(s, g.warps, g.warp, g.lane, slots, slot);
-        const float inv = 1.0f / sqrtf(s[0] * inv_cols + p.eps);
+        const float inv = rsqrtf(s[0] * inv_cols + p.eps);
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            const int64_t base = g.base(v);
-            float w[8];
-            load8_of<TX, VEC>(p.pre, 0, base, g.lane, p.cols, w);
+            if (!kAhead) load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, cols, pre[v]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r[v][j] *= inv * (w[j] + p.offset);
-            store_normed<TX, VEC>(p, row, base, g.lane, r[v]);
+            for (int j = 0; j < 8; ++j) r[v][j] *= inv * (pre[v][j] + p.offset);
+            store_normed<TX, VEC>(p, row, g.base(v), g.lane, cols, r[v]);
         }
     }
     pdl_trigger();
@@ -412,18 +429,18 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = p.alpha;
         if (has_post) {
-            load8_of<TX, true>(p.post, 0, base, lane, p.cols, w);
+            load8_of<TX, true>(p.post, 0, base, lane, cols, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] *= w[j] + p.offset;
         }
         if (p.gate_mode == kGateChannel) {
-            load8_of<TX, true>(p.gate, 0, base, lane, p.cols, w);
+            load8_of<TX, true>(p.gate, 0, base, lane, cols, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] *= w[j];
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) c1[v][j] = pack2(f[2 * j], f[2 * j + 1]);
-        if (has_pre) load8_of<TX, true>(p.pre, 0, base, lane, p.cols, w);
+        if (has_pre) load8_of<TX, true>(p.pre, 0, base, lane, cols, w);
 #pragma unroll
         for (int j = 0; j < 4; ++j) c2[v][j] = pack2(w[2 * j] + p.offset, w[2 * j + 1] + p.offset);
     }
@@ -463,7 +480,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
             read8<TR>(stage + r_at, col[v], r[v]);
             if (p.gate_mode == kGateFull) {
                 float w[8];
-                load8_of<TX, true>(p.gate, row, (v * warps + warp) * kChunk, lane, p.cols, w);
+                load8_of<TX, true>(p.gate, row, (v * warps + warp) * kChunk, lane, cols, w);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = mul2(x[j], pack2(w[2 * j], w[2 * j + 1]));
             }
@@ -554,6 +571,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
     const RowGroup g(warps);
     const float inv_cols = 1.0f / static_cast<float>(p.cols);
     const bool has_x = p.x.p != nullptr, has_post = p.post.p != nullptr, has_pre = p.pre.p != nullptr;
+    const int cols = static_cast<int>(p.cols);
     int slot = 0;
     Sums<VPT> sums(sums_smem);
     for (int i = 0; i < planes.count; ++i)
@@ -568,12 +586,12 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         float d[VPT][8];  // dr', then dr, then du
         if (has_x) {
 #pragma unroll
-            for (int v = 0; v < VPT; ++v) x[v] = load_raw<TX, VEC>(p.x, row, g.base(v), g.lane, p.cols);
+            for (int v = 0; v < VPT; ++v) x[v] = load_raw<TX, VEC>(p.x, row, g.base(v), g.lane, cols);
         }
         Raw8<TR> dres[VPT];
         if (p.d_residual.p != nullptr) {
 #pragma unroll
-            for (int v = 0; v < VPT; ++v) dres[v] = load_raw<TR, VEC>(p.d_residual, row, g.base(v), g.lane, p.cols);
+            for (int v = 0; v < VPT; ++v) dres[v] = load_raw<TR, VEC>(p.d_residual, row, g.base(v), g.lane, cols);
         }
         float s[3] = {0.0f, 0.0f, 0.0f};
         if (has_x && has_post) {
@@ -588,13 +606,13 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
             Raw8<TX> dh[VPT];
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                r[v] = load_raw<TR, VEC>(p.r, row, g.base(v), g.lane, p.cols);
-                dh[v] = load_raw<TX, VEC>(p.d_normed, row, g.base(v), g.lane, p.cols);
+                r[v] = load_raw<TR, VEC>(p.r, row, g.base(v), g.lane, cols);
+                dh[v] = load_raw<TX, VEC>(p.d_normed, row, g.base(v), g.lane, cols);
             }
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 float w[8];
-                load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, p.cols, w);
+                load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, cols, w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float rj = r[v][j];
@@ -603,12 +621,12 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
                 }
             }
             row_sum(s, g.warps, g.warp, g.lane, slots, slot);
-            const float inv = 1.0f / sqrtf(s[0] * inv_cols + p.eps);
+            const float inv = rsqrtf(s[0] * inv_cols + p.eps);
             const float mean = inv * s[1] * inv_cols;  // of t * R
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 float w[8], dw[8];
-                load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, p.cols, w);
+                load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, cols, w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float hat = r[v][j] * inv, dhj = dh[v][j];
@@ -624,7 +642,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
 #pragma unroll
                 for (int j = 0; j < 8; ++j) d[v][j] = 0.0f;
         }
-        if (has_post) inv_x = 1.0f / sqrtf(s[2] * inv_cols + p.eps);
+        if (has_post) inv_x = rsqrtf(s[2] * inv_cols + p.eps);
         if (p.d_residual.p != nullptr) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
@@ -634,7 +652,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         if (p.dr.p != nullptr) {
 #pragma unroll
             for (int v = 0; v < VPT; ++v)
-                store8<TR, VEC>(static_cast<TR *>(p.dr.p) + row * p.dr.ld, g.base(v), g.lane, p.cols, d[v]);
+                store8<TR, VEC>(static_cast<TR *>(p.dr.p) + row * p.dr.ld, g.base(v), g.lane, cols, d[v]);
         }
         if (!has_x) continue;
 
@@ -646,7 +664,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         for (int v = 0; v < VPT; ++v) {
             float w[8], gt[8], dw[8], dg[8];
             if (has_post) {
-                load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, p.cols, w);
+                load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, cols, w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) w[j] += p.offset;
             } else {
@@ -654,7 +672,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
                 for (int j = 0; j < 8; ++j) w[j] = 1.0f;
             }
             if (p.gate_mode == kGateChannel || p.gate_mode == kGateFull) {
-                load8_of<TX, VEC>(p.gate, p.gate_mode == kGateFull ? row : 0, g.base(v), g.lane, p.cols, gt);
+                load8_of<TX, VEC>(p.gate, p.gate_mode == kGateFull ? row : 0, g.base(v), g.lane, cols, gt);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) gt[j] = 1.0f;
@@ -672,9 +690,9 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
             if (planes.gate >= 0) sums.add(planes.gate, v, dg);
             if (p.gate_mode == kGateFull) {
                 if (p.dgate.dtype == ST_F32)
-                    store8<float, VEC>(static_cast<float *>(p.dgate.p) + row * p.dgate.ld, g.base(v), g.lane, p.cols, dg);
+                    store8<float, VEC>(static_cast<float *>(p.dgate.p) + row * p.dgate.ld, g.base(v), g.lane, cols, dg);
                 else
-                    store8<TX, VEC>(static_cast<TX *>(p.dgate.p) + row * p.dgate.ld, g.base(v), g.lane, p.cols, dg);
+                    store8<TX, VEC>(static_cast<TX *>(p.dgate.p) + row * p.dgate.ld, g.base(v), g.lane, cols, dg);
             }
         }
         if (has_post || p.gate_mode == kGateToken) row_sum(e, g.warps, g.warp, g.lane, slots, slot);
@@ -685,12 +703,12 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         for (int v = 0; v < VPT; ++v) {
             if (has_post) {
                 float w[8];
-                load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, p.cols, w);
+                load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, cols, w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     d[v][j] = inv_x * (d[v][j] * (w[j] + p.offset) - x[v][j] * inv_x * mean);
             }
-            store8<TX, VEC>(static_cast<TX *>(p.dx.p) + row * p.dx.ld, g.base(v), g.lane, p.cols, d[v]);
+            store8<TX, VEC>(static_cast<TX *>(p.dx.p) + row * p.dx.ld, g.base(v), g.lane, cols, d[v]);
         }
     }
 
@@ -700,7 +718,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         for (int v = 0; v < VPT; ++v) {
             const float4 a = sums.at(i, v, 0), b = sums.at(i, v, 1);
             const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            store8<float, VEC>(to, g.base(v), g.lane, p.cols, f);
+            store8<float, VEC>(to, g.base(v), g.lane, cols, f);
         }
     }
     pdl_trigger();
@@ -761,18 +779,18 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = p.alpha;
         if (has_post) {
-            load8_of<TX, true>(p.post, 0, base, lane, p.cols, w);
+            load8_of<TX, true>(p.post, 0, base, lane, cols, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] *= w[j] + p.offset;
         }
         if (p.gate_mode == kGateChannel) {
-            load8_of<TX, true>(p.gate, 0, base, lane, p.cols, w);
+            load8_of<TX, true>(p.gate, 0, base, lane, cols, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] *= w[j];
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) c1[v][j] = pack2(f[2 * j], f[2 * j + 1]);
-        if (has_pre) load8_of<TX, true>(p.pre, 0, base, lane, p.cols, w);
+        if (has_pre) load8_of<TX, true>(p.pre, 0, base, lane, cols, w);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             c2[v][j] = pack2(w[2 * j] + p.offset, w[2 * j + 1] + p.offset);
@@ -841,7 +859,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
             uint64_t gate[4] = {twice(g), twice(g), twice(g), twice(g)}, q[4];
             if (p.gate_mode == kGateFull) {
                 float w[8];
-                load8_of<TX, true>(p.gate, row, (v * warps + warp) * kChunk, lane, p.cols, w);
+                load8_of<TX, true>(p.gate, row, (v * warps + warp) * kChunk, lane, cols, w);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) gate[j] = pack2(w[2 * j], w[2 * j + 1]);
             }
