@@ -212,12 +212,13 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
     }
 }
 
-// Few rows, short ones, and any alignment: a CTA or a warp for each row.  All
-// of a row's reads, the weights among them, are under way before the first
-// sum where a thread has one chunk; longer rows read the weights when needed.
-template <typename TX, typename TR, int VPT, bool VEC>
-__global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const NormArgs p, int warps) {
-    constexpr bool kAhead = VPT == 1;
+// Few rows, short ones, and any alignment: a CTA or a warp for each row.
+// AHEAD: all of a row's reads, the weights among them, are under way before
+// the first sum, for few rows; many rows would rather have the registers
+// (64 a thread: 1025 x 2049 in 20 us with 13 warps at work on an SM).
+template <typename TX, typename TR, int VPT, bool VEC, bool AHEAD>
+__global__ void __launch_bounds__(kMaxThreads, VPT == 1 && !AHEAD ? 2 : 1) residual_norm_kernel(const NormArgs p, int warps) {
+    constexpr bool kAhead = AHEAD;
     pdl_wait();
     __shared__ float slots[2 * 3 * 32];
     const RowGroup g(warps);
@@ -975,13 +976,13 @@ struct Shape {
 };
 
 // `rows` rows of `cols` on up to `most` row groups.
-Shape shape_of(int64_t rows, int64_t cols, int64_t most, bool latency) {
+Shape shape_of(int64_t rows, int64_t cols, int64_t most, bool one_chunk) {
     Shape s;
     const int64_t chunks = cdiv(cols, kChunk);
     if (chunks <= 2) {
         s.vpt = static_cast<int>(chunks);
     } else {
-        s.vpt = latency && chunks <= 16 ? 1 : chunks <= 32 ? 2 : 4;
+        s.vpt = one_chunk && chunks <= 16 ? 1 : chunks <= 32 ? 2 : 4;
     }
     s.warps = static_cast<int>(cdiv(chunks, s.vpt));
     const int64_t groups = rows < most ? rows : most;
@@ -995,12 +996,12 @@ Shape shape_of(int64_t rows, int64_t cols, int64_t most, bool latency) {
     return s;
 }
 
-template <typename TX, typename TR, int VPT>
+template <typename TX, typename TR, int VPT, bool AHEAD>
 int forward_vpt(const NormArgs &p, const Shape &s, bool vec, cudaStream_t stream) {
     if (vec)
-        ST_CUDA_TRY(launch_kernel(residual_norm_kernel<TX, TR, VPT, true>, s.ctas, s.threads, 0, stream, p, s.warps));
+        ST_CUDA_TRY(launch_kernel(residual_norm_kernel<TX, TR, VPT, true, AHEAD>, s.ctas, s.threads, 0, stream, p, s.warps));
     else
-        ST_CUDA_TRY(launch_kernel(residual_norm_kernel<TX, TR, VPT, false>, s.ctas, s.threads, 0, stream, p, s.warps));
+        ST_CUDA_TRY(launch_kernel(residual_norm_kernel<TX, TR, VPT, false, AHEAD>, s.ctas, s.threads, 0, stream, p, s.warps));
     note_launch();
     const cudaError_t e = cudaPeekAtLastError();
     return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "residual_norm_kernel");
@@ -1049,12 +1050,16 @@ int forward_typed(const NormArgs &p, int sm_count, cudaStream_t stream) {
                      aligned_rows(p.post, 1, side(p.post), 16) && aligned_rows(p.pre, 1, side(p.pre), 16) &&
                      (p.gate_mode == kGateToken ||
                       aligned_rows(p.gate, p.gate_mode == kGateFull ? p.rows : 1, side(p.gate), 16));
-    const Shape s = shape_of(p.rows, p.cols, int64_t(1) << 30, p.rows < sm_count);
+    // one chunk a thread for few rows, whose latency counts, and for unaligned ones, whose single elements leave little in
+    // flight otherwise
+    const Shape s = shape_of(p.rows, p.cols, int64_t(1) << 30, p.rows < sm_count || !vec);
     if (vec && p.x.p != nullptr && p.r_out.p != nullptr && p.cols % 8 == 0 && p.cols > 2 * kChunk && p.rows >= 2 * sm_count)
         return forward_rows<TX, TR>(p, sm_count, stream);
-    if (s.vpt == 1) return forward_vpt<TX, TR, 1>(p, s, vec, stream);
-    if (s.vpt == 2) return forward_vpt<TX, TR, 2>(p, s, vec, stream);
-    return forward_vpt<TX, TR, 4>(p, s, vec, stream);
+    if (s.vpt == 1)
+        return p.rows < sm_count ? forward_vpt<TX, TR, 1, true>(p, s, vec, stream)
+                                 : forward_vpt<TX, TR, 1, false>(p, s, vec, stream);
+    if (s.vpt == 2) return forward_vpt<TX, TR, 2, false>(p, s, vec, stream);
+    return forward_vpt<TX, TR, 4, false>(p, s, vec, stream);
 }
 
 template <typename TX, typename TR, int VPT, bool VEC>
