@@ -291,6 +291,94 @@ __device__ __forceinline__ bool scale_blocks(float (&acc)[COLS], int n, uint32_t
     return true;
 }
 
+// Load 32 columns of 16 TMEM lanes: lane l gets, for each 8 columns, columns
+// 2 (l % 4) and + 1 of rows l / 4 and l / 4 + 8.
+__device__ __forceinline__ void tmem_load_16x32(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+// scale_blocks for scales that differ from column to column, with each
+// lane on 4 rows (l / 4 + 8 q) and every fourth pair of columns instead of
+// one row and all columns: then a lane needs a quarter of the column scales.
+// (A 16-byte shared-memory read that all lanes share still takes four
+// cycles: one row a lane, 8 warps reading 128 scales each kept shared memory
+// busy for 1024 cycles a block beside the MMAs' 512, and a block took 1480.)
+// Element (row l / 4 + 8 q, column 8 c + 2 (l % 4) + i) is acc[8 c + 2 q + i].
+template <int COLS, int ACCS, int STRIDE, typename Ring, typename Full, typename Released>
+__device__ __forceinline__ bool scale_blocks_by_column(float (&acc)[COLS], int n, uint32_t t, int row0, int col, const Ring &ring,
+                                                       ScalePosition &at, Full tfull, Released released, int lane,
+                                                       const volatile int *abort_flag, uint64_t limit_ns) {
+    constexpr int kSteps = COLS / 32;
+    static_assert(kSteps % 2 == 0, "the two buffers keep their order from block to block");
+    uint32_t v[2][32];  // 16 lanes, then the other 16
+    auto arrived = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit_ns));
+    };
+    auto ask = [&](uint32_t from, uint32_t *to) {
+        tmem_load_16x32(from, to);
+        tmem_load_16x32(from + (16u << 16), to + 16);
+    };
+    if (!arrived(tfull(at.a), at.aph)) return false;
+    tc_fence_after_sync();
+    ask(t + static_cast<uint32_t>(at.a * STRIDE), v[0]);
+    for (int b = 0; b < n; ++b) {
+        const int k = b % kBatch;
+        if (k == 0 && !arrived(ring.full(at.d), at.dph)) return false;
+        const float2 *cols = reinterpret_cast<const float2 *>(ring.cols(at.d, k) + col) + (lane & 3);
+        const float *rows = ring.rows(at.d, k) + row0 + (lane >> 2);
+        uint64_t r[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) r[q] = pack2(rows[8 * q], rows[8 * q]);
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            uint32_t *x = v[j & 1];
+            tmem_loaded<32>(x);
+            if (j + 1 < kSteps) {
+                ask(t + static_cast<uint32_t>(at.a * STRIDE + (j + 1) * 32), v[(j + 1) & 1]);
+            } else {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) released(at.a);
+                if (++at.a == ACCS) {
+                    at.a = 0;
+                    at.aph ^= 1u;
+                }
+                if (b + 1 < n) {
+                    if (!arrived(tfull(at.a), at.aph)) return false;
+                    tc_fence_after_sync();
+                    ask(t + static_cast<uint32_t>(at.a * STRIDE), v[0]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {  // 8 columns
+                const float2 pair = cols[4 * (4 * j + c)];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint64_t scale = mul2(r[q], pack2(pair.x, pair.y));
+                    const uint32_t *in = x + (q >> 1) * 16 + 4 * c + 2 * (q & 1);
+                    float *s = acc + 8 * (4 * j + c) + 2 * q;
+                    s[0] = __fmaf_rn(__uint_as_float(in[0]), lo2(scale), s[0]);
+                    s[1] = __fmaf_rn(__uint_as_float(in[1]), hi2(scale), s[1]);
+                }
+            }
+        }
+        if (k == kBatch - 1 || b + 1 == n) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ring.empty(at.d));
+            if (++at.d == Ring::kDepth) {
+                at.d = 0;
+                at.dph ^= 1u;
+            }
+        }
+    }
+    return true;
+}
+
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Bulk copies still in flight after `issued` of them through a ring of
@@ -653,6 +741,16 @@ __device__ __forceinline__ void put_box_row(uint32_t box, int lane, const uint32
     }
 }
 
+// 8 (4) bytes at byte `at` of a row of such a box.
+__device__ __forceinline__ void put_box_8(uint32_t box, int row, int at, uint32_t a, uint32_t b) {
+    const uint32_t to = box + static_cast<uint32_t>(row * 128 + (((at >> 4) ^ (row & 7)) << 4) + (at & 15));
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(a), "r"(b) : "memory");
+}
+__device__ __forceinline__ void put_box_4(uint32_t box, int row, int at, uint32_t a) {
+    const uint32_t to = box + static_cast<uint32_t>(row * 128 + (((at >> 4) ^ (row & 7)) << 4) + (at & 15));
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(a) : "memory");
+}
+
 // Row and column tile of tile t: 8 row tiles of a column tile after another,
 // so that the tiles in flight share their operands in L2.
 __device__ __forceinline__ void pair_tile(const Fp8Params &p, int t, int &tr, int &tc) {
@@ -834,13 +932,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             float acc[kPairWarpCols];
 #pragma unroll
             for (int j = 0; j < kPairWarpCols; ++j) acc[j] = 0.0f;
-            ok = scale_blocks<kPairWarpCols, CVEC ? 16 : 32, CVEC, Cfg::kAccs, kPairCols>(
-                acc, p.k_blocks, t_lane, g * 32 + lane, half * (CVEC ? kPairWarpCols : 1), ring, at, tfull_bar,
-                [&](int a) {
-                    if (rank == 0) mbar_arrive_relaxed(tempty_bar(a));
-                    else mbar_arrive_cluster_relaxed(even_tempty0 + 8u * a);
-                },
-                lane, abort_flag, p.timeout_ns);
+            auto released = [&](int a) {
+                if (rank == 0) mbar_arrive_relaxed(tempty_bar(a));
+                else mbar_arrive_cluster_relaxed(even_tempty0 + 8u * a);
+            };
+            if constexpr (CVEC)
+                ok = scale_blocks_by_column<kPairWarpCols, Cfg::kAccs, kPairCols>(acc, p.k_blocks, t_lane, g * 32,
+                                                                                  half * kPairWarpCols, ring, at, tfull_bar,
+                                                                                  released, lane, abort_flag, p.timeout_ns);
+            else
+                ok = scale_blocks<kPairWarpCols, 32, false, Cfg::kAccs, kPairCols>(acc, p.k_blocks, t_lane, g * 32 + lane, half,
+                                                                                   ring, at, tfull_bar, released, lane,
+                                                                                   abort_flag, p.timeout_ns);
             if (!ok) {
                 *abort_flag = 1;
                 if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
@@ -852,35 +955,59 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             const int row0 = tr * 2 * kTileRows + static_cast<int>(rank) * kTileRows + g * 32;
             const int col0 = tc * kPairCols + half * kPairWarpCols;
             if (row0 >= p.rows) continue;
-            if (p.staged) {
-                if (p.bias != nullptr) {
+            // CVEC: this lane's element e of 8 columns c lies at (row_of(e), col_of(c, e)); otherwise row `lane`, all columns
+            auto row_of = [&](int e) { return (lane >> 2) + 8 * (e >> 1); };
+            auto col_of = [&](int c, int e) { return 8 * c + 2 * (lane & 3) + (e & 1); };
+            if (p.bias != nullptr) {
 #pragma unroll
-                    for (int j = 0; j < kPairWarpCols; ++j)
-                        acc[j] += col0 + j < p.cols ? load_any(p.bias, p.bias_dtype, col0 + j) : 0.0f;
+                for (int j = 0; j < kPairWarpCols; ++j) {
+                    const int c = col0 + (CVEC ? col_of(j / 8, j % 8) : j);
+                    acc[j] += c < p.cols ? load_any(p.bias, p.bias_dtype, c) : 0.0f;
                 }
+            }
+            if (p.staged) {
 #pragma unroll
                 for (int h = 0; h < kPairWarpCols / 32; ++h) {  // a box: 32 columns of fp32, 64 of 16 bits
-                    uint32_t w[32];
-                    if (p.c_dtype == ST_F32) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(acc[32 * h + i]);
-                    } else {
-                        if (h & 1) continue;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int j = (32 * h + 2 * i) % kPairWarpCols;
-                            w[i] = pack_16(acc[j], acc[j + 1], p.c_dtype);
-                        }
-                    }
+                    if (p.c_dtype != ST_F32 && (h & 1)) continue;
                     if (col0 + 32 * h >= p.cols) continue;
                     if (lane == 0) bulk_wait_group_read<1>();  // the store that last used this box has read it
                     __syncwarp();
-                    const uint32_t at = smem_addr(my_boxes + box * kBoxBytes);
-                    put_box_row(at, lane, w);
+                    const uint32_t at_box = smem_addr(my_boxes + box * kBoxBytes);
+                    if constexpr (CVEC) {
+                        if (p.c_dtype == ST_F32) {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                                for (int e = 0; e < 8; e += 2)
+                                    put_box_8(at_box, row_of(e), 4 * (8 * c + 2 * (lane & 3)),
+                                              __float_as_uint(acc[32 * h + 8 * c + e]), __float_as_uint(acc[32 * h + 8 * c + e + 1]));
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c)
+#pragma unroll
+                                for (int e = 0; e < 8; e += 2) {
+                                    const int j = (32 * h + 8 * c + e) % kPairWarpCols;
+                                    put_box_4(at_box, row_of(e), 2 * (8 * c + 2 * (lane & 3)), pack_16(acc[j], acc[j + 1], p.c_dtype));
+                                }
+                        }
+                    } else {
+                        uint32_t w[32];
+                        if (p.c_dtype == ST_F32) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(acc[32 * h + i]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const int j = (32 * h + 2 * i) % kPairWarpCols;
+                                w[i] = pack_16(acc[j], acc[j + 1], p.c_dtype);
+                            }
+                        }
+                        put_box_row(at_box, lane, w);
+                    }
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {  // TMA clips the box at C's extents
-                        tma_store_2d(&tmap_out, at, col0 + 32 * h, row0);
+                        tma_store_2d(&tmap_out, at_box, col0 + 32 * h, row0);
                         bulk_commit_group();
                     }
                     box ^= 1;
@@ -891,14 +1018,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                 for (int h = 0; h < kPairWarpCols / 32; ++h) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) m[lane * 33 + i] = acc[32 * h + i];
+                    for (int i = 0; i < 32; ++i)
+                        m[CVEC ? row_of(i % 8) * 33 + col_of(i / 8, i % 8) : lane * 33 + i] = acc[32 * h + i];
                     __syncwarp();
                     const int c = col0 + 32 * h + lane;
-                    if (c < p.cols) {
-                        const float add = p.bias != nullptr ? load_any(p.bias, p.bias_dtype, c) : 0.0f;
-                        for (int r = 0; r < n; ++r)
-                            store_any(p.c, p.c_dtype, (row0 + r) * p.c_r + c, p.bias != nullptr ? m[r * 33 + lane] + add : m[r * 33 + lane]);
-                    }
+                    if (c < p.cols)
+                        for (int r = 0; r < n; ++r) store_any(p.c, p.c_dtype, (row0 + r) * p.c_r + c, m[r * 33 + lane]);
                     __syncwarp();
                 }
             }
