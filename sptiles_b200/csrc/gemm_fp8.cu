@@ -1272,7 +1272,7 @@ Fp8Plan plan_fp8(int64_t rows, int64_t cols, int64_t k_blocks, bool k_major, boo
         }
     }
     if (cols > 64)
-        offer(true, 128, 1, cdiv(rows, 256) * cdiv(cols, 256), sm_count / 2, column_scales ? 1480 : 1000, 11400);
+        offer(true, 128, 1, cdiv(rows, 256) * cdiv(cols, 256), sm_count / 2, column_scales ? 1400 : 980, 11400);
     return best;
 }
 

@@ -921,36 +921,42 @@ struct ColumnSums {
     int count = 0;
 };
 
-// In a fixed order: 8 threads a column, each every 8th group; blockIdx.y picks the sum.
+// In a fixed order: 32 threads a column, each every 32nd group, then a
+// shuffle over them.  blockIdx.y picks the plane, read once for all its sums.
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const float *sums, int64_t groups, int64_t cols,
-                                                          const ColumnSums todo) {
+__global__ void __launch_bounds__(1024) column_sums_kernel(const float *sums, int groups, int cols, const ColumnSums todo) {
     pdl_wait();
-    const ColumnSum &o = todo.sum[blockIdx.y];
-    __shared__ float part[8][33];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + tx;
-    const float *src = sums + o.plane * groups * cols + c;
+    __shared__ float part[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c = static_cast<int>(blockIdx.x) * 32 + lane;
+    const float *src = sums + static_cast<int64_t>(blockIdx.y) * groups * cols + c;
     float s = 0.0f;
     if (c < cols) {
-        int64_t i = ty;
-        for (; i + 24 < groups; i += 32) {  // four loads in flight
-            const float a = src[i * cols], b = src[(i + 8) * cols], d = src[(i + 16) * cols], e = src[(i + 24) * cols];
-            s += (a + b) + (d + e);
+        int i = warp;
+        for (; i + 96 < groups; i += 128) {  // four loads in flight
+            const float v0 = src[static_cast<int64_t>(i) * cols], v1 = src[static_cast<int64_t>(i + 32) * cols];
+            const float v2 = src[static_cast<int64_t>(i + 64) * cols], v3 = src[static_cast<int64_t>(i + 96) * cols];
+            s += (v0 + v1) + (v2 + v3);
         }
-        for (; i < groups; i += 8) s += src[i * cols];
+        for (; i < groups; i += 32) s += src[static_cast<int64_t>(i) * cols];
     }
-    part[ty][tx] = s;
+    part[warp][lane] = s;
     __syncthreads();
-    if (ty == 0 && c < cols) {
+    s = part[lane][warp];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) s += part[i][tx];
-        s *= o.scale;
-        if (o.factor.p != nullptr)
-            s *= (o.factor.dtype == ST_F32 ? static_cast<const float *>(o.factor.p)[c]
-                                           : to_float(static_cast<const T *>(o.factor.p)[c])) +
-                 o.offset;
-        o.out[c] = s;
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const int mine = static_cast<int>(blockIdx.x) * 32 + warp;
+    if (lane == 0 && mine < cols) {
+        for (int i = 0; i < todo.count; ++i) {
+            const ColumnSum &o = todo.sum[i];
+            if (o.plane != static_cast<int>(blockIdx.y)) continue;
+            float v = s * o.scale;
+            if (o.factor.p != nullptr)
+                v *= (o.factor.dtype == ST_F32 ? static_cast<const float *>(o.factor.p)[mine]
+                                               : to_float(static_cast<const T *>(o.factor.p)[mine])) +
+                     o.offset;
+            o.out[mine] = v;
+        }
     }
     pdl_trigger();
 }
@@ -1088,11 +1094,11 @@ int backward_vpt(const NormBackwardArgs &p, const Shape &s, bool vec, const Plan
 }
 
 template <typename T>
-int finish_sums(const ColumnSums &todo, const float *sums, int64_t groups, int64_t cols, cudaStream_t stream) {
+int finish_sums(const ColumnSums &todo, const float *sums, int planes, int64_t groups, int64_t cols, cudaStream_t stream) {
     if (todo.count == 0) return ST_OK;
     ST_CUDA_TRY(launch_kernel(column_sums_kernel<T>,
-                              dim3(static_cast<unsigned>(cdiv(cols, 32)), static_cast<unsigned>(todo.count)), 256, 0, stream,
-                              sums, groups, cols, todo));
+                              dim3(static_cast<unsigned>(cdiv(cols, 32)), static_cast<unsigned>(planes)), 1024, 0, stream, sums,
+                              static_cast<int>(groups), static_cast<int>(cols), todo));
     note_launch();
     const cudaError_t e = cudaPeekAtLastError();
     return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "column_sums_kernel");
@@ -1128,7 +1134,7 @@ int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) 
         int groups = 0;
         ST_TRY(launch_rows(residual_norm_backward_rows_kernel<TX, TR>, attr_set, 32 * warps, stage, p.rows,
                            static_cast<int>(kGroupSms), stream, &groups, p, warps, planes, sums));
-        return finish_sums<TX>(todo, sums, groups, p.cols, stream);
+        return finish_sums<TX>(todo, sums, planes.count, groups, p.cols, stream);
     }
     const Shape s = shape_of(p.rows, p.cols, backward_groups(p.rows, p.cols), false);
     const int64_t groups = s.warps == 1 ? static_cast<int64_t>(s.ctas) * kRowsPerCta : s.ctas;
@@ -1143,7 +1149,7 @@ int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) 
     if (s.vpt == 1) ST_TRY((backward_vpt<TX, TR, 1>(p, s, vec, planes, sums, stream)));
     else if (s.vpt == 2) ST_TRY((backward_vpt<TX, TR, 2>(p, s, vec, planes, sums, stream)));
     else ST_TRY((backward_vpt<TX, TR, 4>(p, s, vec, planes, sums, stream)));
-    return finish_sums<TX>(todo, sums, groups, p.cols, stream);
+    return finish_sums<TX>(todo, sums, planes.count, groups, p.cols, stream);
 }
 
 }  // namespace

@@ -17,6 +17,7 @@ keep nothing between calls and can be captured into a CUDA graph.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from typing import NamedTuple
 
@@ -44,6 +45,19 @@ class ResidualNormGrads(NamedTuple):
     post_weight: torch.Tensor | None  # float32 [cols]
     gate: torch.Tensor | None         # the gate's shape; float32, or the gate's dtype where it is [rows, cols]
     pre_weight: torch.Tensor | None   # float32 [cols]
+
+
+def _new_sums(like: torch.Tensor, cols: int) -> tuple[torch.Tensor, bytes]:
+    t = like.new_empty_strided((cols,), (1,), dtype=torch.float32)
+    return t, _pack(t.data_ptr(), N.ST_F32, 1, cols, 0, 1, 0)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(rows: int, cols: int) -> int:
+    """What residual_norm_backward needs for its sums over rows: a function of the extents alone."""
+    size = ctypes.c_uint64(0)
+    N.check(N.lib().st_residual_norm_backward_workspace(rows, cols, ctypes.byref(size)), "residual_norm_backward")
+    return size.value
 
 
 def _opt(t: torch.Tensor | None) -> bytes | None:
@@ -133,28 +147,26 @@ def residual_norm_backward(d_residual: torch.Tensor | None, d_normed: torch.Tens
             raise ValueError(f"unsupported dtype {t.dtype}")
     dr, d_dr = _new(like, rows, cols, pitch, 1, stream.dtype)
     dx, d_dx = (None, None) if x is None else _new(like, rows, cols, pitch, 1, x.dtype)
-    # the sums over rows are one allocation: dpost, dpre, dgate
-    sums = like.new_empty_strided((3, pitch), (pitch, 1), dtype=torch.float32)
-    base = sums.data_ptr()
     dpost = dpre = dgate = d_dpost = d_dpre = d_dgate = None
     if post_weight is not None:
-        dpost, d_dpost = sums[0, :cols], _pack(base, N.ST_F32, 1, cols, 0, 1, 0)
+        dpost, d_dpost = _new_sums(like, cols)
     if pre_weight is not None:
-        dpre, d_dpre = sums[1, :cols], _pack(base + 4 * pitch, N.ST_F32, 1, cols, 0, 1, 0)
+        dpre, d_dpre = _new_sums(like, cols)
     if gate is not None:
-        full = gate.dim() == 2 and gate.shape[0] == rows and gate.shape[1] == cols
-        dgate = torch.empty(gate.shape, dtype=gate.dtype if full else torch.float32, device=like.device)
-        d_dgate = _desc(dgate)
-    size = ctypes.c_uint64(0)
-    fn = _fns.get("st_residual_norm_backward_workspace") or _fn("st_residual_norm_backward_workspace", ctypes.c_int64,
-                                                               ctypes.c_int64, _vp)
-    rc = fn(rows, cols, ctypes.addressof(size))
-    if rc != N.ST_OK:
-        N.check(rc, "residual_norm_backward")
-    workspace = like.new_empty_strided((size.value,), (1,), dtype=torch.uint8)
+        if gate.dim() == 1:
+            dgate, d_dgate = _new_sums(like, gate.shape[0])
+        elif gate.dim() == 2:
+            g0, g1 = gate.shape
+            if gate.dtype not in _ALL_CODES:
+                raise ValueError(f"unsupported dtype {gate.dtype}")
+            dgate, d_dgate = _new(like, g0, g1, max(g1, 1), 1, gate.dtype if g0 == rows and g1 == cols else torch.float32)
+        else:
+            raise ValueError("gate must be rank 1 or 2")
+    size = _workspace_bytes(rows, cols)
+    workspace = like.new_empty_strided((size,), (1,), dtype=torch.uint8)
     fn = _fns.get("st_residual_norm_backward") or _fn("st_residual_norm_backward", _vp, *[_cp] * 12, _vp, _u64, _cp, _cp)
     rc = fn(context(dev), _opt(d_residual), _opt(d_normed), _opt(x), _opt(residual), _opt(post_weight), _opt(gate),
-            _opt(pre_weight), d_dx, d_dr, d_dpost, d_dgate, d_dpre, workspace.data_ptr(), size.value,
+            _opt(pre_weight), d_dx, d_dr, d_dpost, d_dgate, d_dpre, workspace.data_ptr(), size,
             _OPTIONS.pack(alpha, eps, weight_offset), _exec_desc(dev))
     if rc != N.ST_OK:
         N.check(rc, "residual_norm_backward")
