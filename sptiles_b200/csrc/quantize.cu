@@ -98,9 +98,12 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const Quanti
 }
 
 // ---------------------------------------------------------------- tiles of 128 columns
-// The other blocks, and any stride: a CTA takes 128 columns and 32 * NROWS
-// rows, 16 threads of 8 columns across, 32 rows down.
-constexpr int kTileThreads = 512;
+// The other blocks, and any stride: a CTA takes 128 columns and 16 * NROWS
+// rows, 16 threads of 8 columns across, 16 rows down.  The elements stay as
+// they were read and are unpacked twice: at 4 registers for 8 of 16 bits,
+// three such CTAs have 96 KB of an SM's reads under way (unpacked, two CTAs
+// of 512 threads took 64 us for 8192 x 8192; so 38, and 40 in 128 x 1 blocks).
+constexpr int kTileThreads = 256;
 constexpr int kDown = kTileThreads / 16;
 
 enum : int { kRowBlocks = 0, kColumnBlocks = 1, kSquareBlocks = 2 };  // 1 x 128, 128 x 1, 128 x 128
@@ -110,7 +113,8 @@ enum : int { kRowBlocks = 0, kColumnBlocks = 1, kSquareBlocks = 2 };  // 1 x 128
 enum : int { kWordsAccess = 0, kUnitAccess = 1, kAnyAccess = 2 };
 
 template <typename T, int MODE, int NROWS, int ACCESS>
-__global__ void __launch_bounds__(kTileThreads) quantize_tiles_kernel(const QuantizeArgs p, uint32_t col_tiles) {
+__global__ void __launch_bounds__(kTileThreads, NROWS == 2 ? 4 : ACCESS == kWordsAccess ? 3 : 2)
+    quantize_tiles_kernel(const QuantizeArgs p, uint32_t col_tiles) {
     pdl_wait();
     __shared__ float red[MODE == kColumnBlocks ? kDown * kTile : kTileThreads / 32];
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -121,25 +125,23 @@ __global__ void __launch_bounds__(kTileThreads) quantize_tiles_kernel(const Quan
     const T *a = static_cast<const T *>(p.a) + c0 * p.sa1;
     const bool whole = ACCESS == kWordsAccess && tx * 8 + 8 <= left;
 
-    uint64_t x[NROWS][4];
+    constexpr int kWords = static_cast<int>(sizeof(T) / 2);
+    uint4 raw[NROWS][kWords];
 #pragma unroll
     for (int i = 0; i < NROWS; ++i) {
         const int64_t r = r0 + kDown * i;
         const T *row = a + r * p.sa0;
-        if (whole) {
-            constexpr int kWords = static_cast<int>(sizeof(T) / 2);
-            uint4 w[kWords];
 #pragma unroll
-            for (int k = 0; k < kWords; ++k)
-                w[k] = r < p.rows ? __ldcs(reinterpret_cast<const uint4 *>(row + tx * 8) + k) : make_uint4(0, 0, 0, 0);
-            unpack8(w, x[i], T{});
+        for (int k = 0; k < kWords; ++k) raw[i][k] = make_uint4(0, 0, 0, 0);
+        if (r >= p.rows) continue;
+        if (whole) {
+#pragma unroll
+            for (int k = 0; k < kWords; ++k) raw[i][k] = __ldcs(reinterpret_cast<const uint4 *>(row + tx * 8) + k);
         } else {
-            float f[8];
+            T *e = reinterpret_cast<T *>(raw[i]);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                f[j] = r < p.rows && column(j) < left ? to_float(row[ACCESS == kAnyAccess ? column(j) * p.sa1 : column(j)]) : 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[i][j] = pack2(f[2 * j], f[2 * j + 1]);
+                if (column(j) < left) e[j] = row[ACCESS == kAnyAccess ? column(j) * p.sa1 : column(j)];
         }
     }
 
@@ -148,9 +150,11 @@ __global__ void __launch_bounds__(kTileThreads) quantize_tiles_kernel(const Quan
     if constexpr (MODE == kRowBlocks) {
 #pragma unroll
         for (int i = 0; i < NROWS; ++i) {
+            uint64_t x[4];
+            unpack8(raw[i], x, T{});
             float m = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) m = max_abs(m, lo2(x[i][j]), hi2(x[i][j]));
+            for (int j = 0; j < 4; ++j) m = max_abs(m, lo2(x[j]), hi2(x[j]));
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
             const float s = fp8_scale(m, limit);
@@ -159,13 +163,16 @@ __global__ void __launch_bounds__(kTileThreads) quantize_tiles_kernel(const Quan
             if (tx == 0 && r < p.rows) p.scale[r * p.ss0 + tile_c * p.ss1] = s;
         }
     } else if constexpr (MODE == kColumnBlocks) {
+        float m[8] = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float m = 0.0f;
+        for (int i = 0; i < NROWS; ++i) {
+            uint64_t x[4];
+            unpack8(raw[i], x, T{});
 #pragma unroll
-            for (int i = 0; i < NROWS; ++i) m = max_abs(m, j & 1 ? hi2(x[i][j / 2]) : lo2(x[i][j / 2]));
-            red[ty * kTile + column(j)] = m;
+            for (int j = 0; j < 8; ++j) m[j] = max_abs(m[j], j & 1 ? hi2(x[j / 2]) : lo2(x[j / 2]));
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) red[ty * kTile + column(j)] = m[j];
         __syncthreads();
         if (threadIdx.x < kTile) {
             float m = 0.0f;
@@ -182,9 +189,12 @@ __global__ void __launch_bounds__(kTileThreads) quantize_tiles_kernel(const Quan
     } else {
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NROWS; ++i)
+        for (int i = 0; i < NROWS; ++i) {
+            uint64_t x[4];
+            unpack8(raw[i], x, T{});
 #pragma unroll
-            for (int j = 0; j < 4; ++j) m = max_abs(m, lo2(x[i][j]), hi2(x[i][j]));
+            for (int j = 0; j < 4; ++j) m = max_abs(m, lo2(x[j]), hi2(x[j]));
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
@@ -204,10 +214,11 @@ __global__ void __launch_bounds__(kTileThreads) quantize_tiles_kernel(const Quan
     for (int i = 0; i < NROWS; ++i) {
         const int64_t r = r0 + kDown * i;
         if (r >= p.rows) continue;
-        uint64_t y[4];
+        uint64_t x[4], y[4];
+        unpack8(raw[i], x, T{});
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            y[j] = MODE == kColumnBlocks ? mul2(x[i][j], pack2(inv[2 * j], inv[2 * j + 1])) : mul2(x[i][j], pack2(inv[i], inv[i]));
+            y[j] = MODE == kColumnBlocks ? mul2(x[j], pack2(inv[2 * j], inv[2 * j + 1])) : mul2(x[j], pack2(inv[i], inv[i]));
         const uint2 c = p.e5m2 ? to_fp8x8<true>(y, 1.0f) : to_fp8x8<false>(y, 1.0f);
         uint8_t *to = q + r * p.sq0;
         if (whole) {
@@ -260,9 +271,9 @@ int launch_typed(const QuantizeArgs &p, cudaStream_t stream) {
         else ST_CUDA_TRY(launch_kernel(quantize_rows_kernel<T, false>, g, kRowThreads, 0, stream, p, ch));
         return checked("quantize_rows_kernel");
     }
-    if (p.block_rows == 1) return launch_tiles<T, kRowBlocks, 1>(p, access, stream);
-    if (p.block_cols == 1) return launch_tiles<T, kColumnBlocks, 4>(p, access, stream);
-    return launch_tiles<T, kSquareBlocks, 4>(p, access, stream);
+    if (p.block_rows == 1) return launch_tiles<T, kRowBlocks, 2>(p, access, stream);
+    if (p.block_cols == 1) return launch_tiles<T, kColumnBlocks, 8>(p, access, stream);
+    return launch_tiles<T, kSquareBlocks, 8>(p, access, stream);
 }
 
 }  // namespace
