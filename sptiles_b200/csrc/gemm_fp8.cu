@@ -1216,7 +1216,8 @@ int make_map_out(CUtensorMap *map, const GemmFp8Args &g) {
 }
 
 // How TMA can read a [rows, k] operand: directly along K or along its rows,
-// or after a copy (the strides 0 of a broadcast among the copies).
+// or after a copy (the overlapping rows of a broadcast or a window among the
+// copies).
 struct Access {
     bool mn;     // rows contiguous
     bool copy;   // through the workspace
@@ -1227,7 +1228,7 @@ Access access_of(const Fp8Operand &o) {
     const bool base = (reinterpret_cast<uintptr_t>(o.data) & 15u) == 0;
     auto fits = [&](int64_t unit, int64_t unit_extent, int64_t ld, int64_t outer) {
         return base && (unit == 1 || unit_extent == 1) &&
-               (outer == 1 || (ld > 0 && ld % 16 == 0 && ld < (int64_t(1) << 40)));
+               (outer == 1 || (ld >= unit_extent && ld % 16 == 0 && ld < (int64_t(1) << 40)));
     };
     auto stride = [](int64_t ld, int64_t outer, int64_t extent) { return outer == 1 ? (extent + 15) / 16 * 16 : ld; };
     if (fits(o.s_k, o.k, o.s_row, o.rows)) return {false, false, stride(o.s_row, o.rows, o.k)};

@@ -167,8 +167,9 @@ def matmul_fp8(A: torch.Tensor, B: torch.Tensor, a_scale: torch.Tensor, b_scale:
     workspace, need = None, 0
     # operands that the tensor core's loads cannot address in place are copied: ask how much room that takes
     (a0, a1), (b0, b1) = A.stride(), B.stride()
-    if not ((a1 == 1 and a0 % 16 == 0 or a0 == 1 and a1 % 16 == 0) and (b1 == 1 and b0 % 16 == 0 or b0 == 1 and b1 % 16 == 0) and
-            a0 and a1 and b0 and b1 and (A.data_ptr() | B.data_ptr()) % 16 == 0):
+    if not ((a1 == 1 and a0 % 16 == 0 and a0 >= sa[1] or a0 == 1 and a1 % 16 == 0 and a1 >= sa[0]) and
+            (b1 == 1 and b0 % 16 == 0 and b0 >= sb[1] or b0 == 1 and b1 % 16 == 0 and b1 >= sb[0]) and
+            (A.data_ptr() | B.data_ptr()) % 16 == 0):
         size = ctypes.c_uint64(0)
         fn = _fns.get("st_matmul_fp8_workspace") or _fn("st_matmul_fp8_workspace", _cp, _cp, _vp)
         rc = fn(da, db, ctypes.addressof(size))

@@ -106,6 +106,7 @@ def test_matmul_workspace():
     assert need(t2(16, 250, E4), t2(250, 32, E4, strides=(1, 256))) == 16 * 256
     assert need(t2(16, 256, E4, data=DATA + 8), k_major) == 16 * 256
     assert need(t2(16, 256, E4, strides=(0, 1)), k_major) == 16 * 256       # a broadcast row
+    assert need(t2(16, 256, E4, strides=(32, 1)), k_major) == 16 * 256      # overlapping rows
     assert need(t2(16, 256, E4, strides=(512, 2)), t2(256, 30, E4)) == 16 * 256 + 256 * 32
     assert need(t2(0, 256, E4, strides=(3, 1)), k_major) == 0
     refused(L.st_matmul_fp8_workspace(ref(t2(16, 256, F32)), ref(k_major), ctypes.byref(n)), BAD, "A and B must be")

@@ -7,7 +7,10 @@ magnitudes (a truncating adder), so a K-term element with its B blocks is
 within (K_block + B + 4) 2^-23 sum |a b| of the exact value -- a term passes
 at most its block's additions, the blocks' additions and the two scalings --
 and the result's rounding adds half a step, eps / 2 relative."""
-import numpy as np
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -206,6 +209,48 @@ def test_matmul_strided_broadcast_and_square_a():
     s1 = sa[:1].expand(2, -1)
     C = st.matmul_fp8(put(a)[:1].expand(140, -1), put(b).t(), s1.to(DEV), sb.t().to(DEV), out_dtype=torch.float32)
     check_product(C, one, b, s1, sb, None, torch.float32)
+
+
+def test_matmul_overlapping_rows():
+    """Rows of A that overlap (a window moving by 16) are copied, not read as a matrix of separate rows."""
+    a, b, sa, sb = make(1, 150, 2400)
+    line = put(a)[0]
+    _, _, sa, _ = make(100, 150, 800)
+    b, sb = b[:, :800], sb[:, :7]
+    C = st.matmul_fp8(line.as_strided((100, 800), (16, 1)), put(b).t(), sa.to(DEV), sb.t().to(DEV), out_dtype=torch.float32)
+    rows = torch.stack([a[0, 16 * i:16 * i + 800].float() for i in range(100)]).to(E4)
+    check_product(C, rows, b, sa, sb, None, torch.float32)
+
+
+def test_first_call_may_be_captured():
+    """In a process of its own: each operator's first call inside a graph capture."""
+    code = """
+import torch, sptiles_b200 as st
+dev = torch.device('cuda:0')
+torch.manual_seed(0)
+x = torch.randn(300, 1024, device=dev, dtype=torch.bfloat16)
+w = torch.randn(256, 1024, device=dev, dtype=torch.bfloat16)
+p = torch.ones(1024, device=dev, dtype=torch.bfloat16)
+s = torch.cuda.Stream()
+torch.cuda.synchronize()
+st.runtime.context(0)
+def step():
+    wq, ws = st.quantize_fp8(w, block=(128, 128))
+    f = st.residual_norm(x, x, p, p, p, quantize=True)
+    y = st.matmul_fp8(f.normed, wq.t(), f.scale, ws.t())
+    return y, *st.residual_norm_backward(x, x, x, f.residual, p, p, p)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    out = step()
+g.replay()
+torch.cuda.synchronize()
+want = step()
+assert all(torch.equal(a, b) for a, b in zip(out, want))
+print('captured')
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          cwd=str(Path(__file__).resolve().parents[1]))
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
 
 
 def test_matmul_output_view_and_edges():
