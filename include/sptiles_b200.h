@@ -267,9 +267,10 @@ int st_quantize_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *q, const s
  * with dY in blocks of 1 x 128, dX = dY @ W reads W [N, K] as it is stored;
  * with dY and X in blocks of 128 x 1 (tokens), dW = dY^T @ X reads both as
  * they are stored, through transposed views.  The same inputs give the same
- * bits.  An operand that neither starts on a 16-byte boundary nor has its
- * rows (or columns) 16 bytes apart is copied first, into `workspace`:
- * st_matmul_fp8_workspace gives the bytes, 0 where none is needed. */
+ * bits.  An operand is read in place if it starts on a 16-byte boundary and
+ * its rows (or its columns) are contiguous, a multiple of 16 bytes apart and
+ * do not overlap; any other is copied first, into `workspace` (16-byte
+ * aligned): st_matmul_fp8_workspace gives the bytes, 0 where none is needed. */
 int st_matmul_fp8_workspace(const st_tensor *a, const st_tensor *b, uint64_t *bytes);
 int st_matmul_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_tensor *a_scale,
                   const st_tensor *b_scale, const st_tensor *bias, const st_tensor *c, void *workspace,
@@ -295,8 +296,8 @@ int st_residual_norm(st_ctx *ctx, const st_tensor *x, const st_tensor *residual,
                      const st_exec *exec);
 /* The gradients of the call above at `residual`, its residual_out as stored:
  * d_residual and d_normed (either may be NULL) to dx, dr (the incoming
- * stream's; may be NULL), dpost, dpre (f32 [cols]; may be NULL) and dgate (the gate's shape: f32, or T where it is
- * [rows, cols]).  `workspace` holds partial sums over rows:
+ * stream's; may be NULL), dpost, dpre (f32 [cols]; may be NULL) and dgate
+ * (the gate's shape: f32, or T where it is [rows, cols]).  `workspace` holds partial sums over rows:
  * st_residual_norm_backward_workspace gives its bytes.  The same inputs give
  * the same bits. */
 int st_residual_norm_backward_workspace(int64_t rows, int64_t cols, uint64_t *bytes);

@@ -118,6 +118,20 @@ __device__ __forceinline__ uint2 to_fp8x8(const uint64_t (&f)[4], float scale) {
                       to_fp8x4<E5M2>(lo2(y[2]), hi2(y[2]), lo2(y[3]), hi2(y[3])));
 }
 
+// Maxima of four blocks that 16 lanes hold each: every exchange halves the
+// blocks that a lane still carries, so a lane ends with the maximum of block
+// (lane >> 2) & 3 of its half warp, after 5 shuffles for the 16 of four
+// separate reductions.
+__device__ __forceinline__ float max_of_four(const float (&m)[4], int lane) {
+    const bool up = lane & 8, odd = lane & 4;
+    float k0 = up ? m[2] : m[0], k1 = up ? m[3] : m[1];
+    k0 = max_abs(k0, __shfl_xor_sync(0xffffffffu, up ? m[0] : m[2], 8));
+    k1 = max_abs(k1, __shfl_xor_sync(0xffffffffu, up ? m[1] : m[3], 8));
+    float k = max_abs(odd ? k1 : k0, __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 4));
+    k = max_abs(k, __shfl_xor_sync(0xffffffffu, k, 2));
+    return max_abs(k, __shfl_xor_sync(0xffffffffu, k, 1));
+}
+
 // The scale of a block from its largest |value|, a NaN kept: see quantize.cu.
 constexpr float kFp8LeastScale = 1.1754943508222875e-38f;  // 2^-126
 __device__ __forceinline__ float fp8_scale(float top, float limit) {

@@ -381,15 +381,6 @@ __device__ __forceinline__ bool scale_blocks_by_column(float (&acc)[COLS], int n
 
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Bulk copies still in flight after `issued` of them through a ring of
-// barriers: wait (bounded, whatever the abort flag says) before leaving.
-template <typename Bar>
-__device__ __forceinline__ void drain_ring(int issued, int stages, Bar bar, uint64_t limit_ns) {
-    const volatile int never = 0;
-    for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
-        (void)mbar_wait(bar(i % stages), static_cast<uint32_t>(i / stages) & 1u, &never, limit_ns);
-}
-
 // ---------------------------------------------------------------- one CTA, 128 x BN tiles
 
 template <int BN, bool CVEC>
@@ -603,7 +594,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, CVEC>::kThreads, BN == 128 ? 1 : 2)
         }
         if (elect_one()) tc_commit(drain_bar);
         __syncwarp();
-        (void)mbar_wait(drain_bar, 0, abort_flag, p.timeout_ns);
+        drain_ring(1, 1, [&](int) { return drain_bar; }, p.timeout_ns);  // the MMAs read shared memory and write TMEM
     } else if (warp == 2 + Cfg::kScaleWarps) {
         // ------------------------------------------------ scales
         int d = 0;
@@ -628,7 +619,7 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, CVEC>::kThreads, BN == 128 ? 1 : 2)
     // ------------------------------------------------ C
     const bool scaler = warp >= 2 && warp < 2 + Cfg::kScaleWarps;
     const int es = p.c_dtype == ST_F32 ? 4 : 2;
-    const bool wide = split == 1 && p.c_c == 1 && c0 + BN <= p.cols && p.bias == nullptr &&
+    const bool wide = split == 1 && p.c_c == 1 && p.cols - c0 >= BN && p.bias == nullptr &&
                       (reinterpret_cast<uintptr_t>(p.c) & 15u) == 0 && (p.c_r * es) % 16 == 0;
     if (wide) {  // whole 16-byte pieces of each row, straight from registers
         const int row = r0 + row_in_tile;
@@ -900,7 +891,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 }
                 if (elect_one()) tc_commit_pair(drain_bar);
                 __syncwarp();
-                (void)mbar_wait(drain_bar, 0, abort_flag, p.timeout_ns);
+                drain_ring(1, 1, [&](int) { return drain_bar; }, p.timeout_ns);  // the MMAs read shared memory and write TMEM
             }
         } else if (warp == 2) {
             // -------------------------------------------- scales (both CTAs)

@@ -218,7 +218,6 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
 // (64 a thread: 1025 x 2049 in 20 us with 13 warps at work on an SM).
 template <typename TX, typename TR, int VPT, bool VEC, bool AHEAD>
 __global__ void __launch_bounds__(kMaxThreads, VPT == 1 && !AHEAD ? 2 : 1) residual_norm_kernel(const NormArgs p, int warps) {
-    constexpr bool kAhead = AHEAD;
     pdl_wait();
     __shared__ float slots[2 * 3 * 32];
     const RowGroup g(warps);
@@ -236,9 +235,9 @@ __global__ void __launch_bounds__(kMaxThreads, VPT == 1 && !AHEAD ? 2 : 1) resid
         for (int v = 0; v < VPT; ++v) {
             if (has_x) load8<TX, VEC>(static_cast<const TX *>(p.x.p) + row * p.x.ld, g.base(v), g.lane, cols, x[v]);
             load8<TR, VEC>(static_cast<const TR *>(p.r.p) + row * p.r.ld, g.base(v), g.lane, cols, r[v]);
-            if (kAhead && has_post) load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, cols, post[v]);
-            if (kAhead && wide_gate) load8_of<TX, VEC>(p.gate, gate_row, g.base(v), g.lane, cols, gate[v]);
-            if (kAhead && has_pre) load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, cols, pre[v]);
+            if (AHEAD && has_post) load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, cols, post[v]);
+            if (AHEAD && wide_gate) load8_of<TX, VEC>(p.gate, gate_row, g.base(v), g.lane, cols, gate[v]);
+            if (AHEAD && has_pre) load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, cols, pre[v]);
         }
         if (has_x) {
             if (has_post) {
@@ -251,7 +250,7 @@ __global__ void __launch_bounds__(kMaxThreads, VPT == 1 && !AHEAD ? 2 : 1) resid
                 const float inv = rsqrtf(s[0] * inv_cols + p.eps);
 #pragma unroll
                 for (int v = 0; v < VPT; ++v) {
-                    if (!kAhead) load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, cols, post[v]);
+                    if (!AHEAD) load8_of<TX, VEC>(p.post, 0, g.base(v), g.lane, cols, post[v]);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[v][j] *= inv * (post[v][j] + p.offset);
                 }
@@ -259,7 +258,7 @@ __global__ void __launch_bounds__(kMaxThreads, VPT == 1 && !AHEAD ? 2 : 1) resid
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 if (wide_gate) {
-                    if (!kAhead) load8_of<TX, VEC>(p.gate, gate_row, g.base(v), g.lane, cols, gate[v]);
+                    if (!AHEAD) load8_of<TX, VEC>(p.gate, gate_row, g.base(v), g.lane, cols, gate[v]);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) x[v][j] *= gate[v][j];
                 }
@@ -282,7 +281,7 @@ __global__ void __launch_bounds__(kMaxThreads, VPT == 1 && !AHEAD ? 2 : 1) resid
         const float inv = rsqrtf(s[0] * inv_cols + p.eps);
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
-            if (!kAhead) load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, cols, pre[v]);
+            if (!AHEAD) load8_of<TX, VEC>(p.pre, 0, g.base(v), g.lane, cols, pre[v]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) r[v][j] *= inv * (pre[v][j] + p.offset);
             store_normed<TX, VEC>(p, row, g.base(v), g.lane, cols, r[v]);
@@ -302,19 +301,29 @@ struct RowRing {
     uint8_t *data;
     int stages, stage_bytes;
     volatile int *abort_flag;
+    volatile int *issued;  // rows whose copies have begun
     int *err;
     uint64_t limit_ns;
     __device__ __forceinline__ void init() const {
         if (threadIdx.x == 0) {
             for (int s = 0; s < stages; ++s) mbar_init(bar0 + 8u * s, 1);
-            *abort_flag = 0;
+            *abort_flag = *issued = 0;
             fence_barrier_init();
         }
         __syncthreads();
     }
     __device__ __forceinline__ uint8_t *stage(int s) const { return data + s * stage_bytes; }
     // One thread: begin the copies of stage s (`bytes` in all).
-    __device__ __forceinline__ void expect(int s, uint32_t bytes) const { mbar_arrive_expect_tx(bar0 + 8u * s, bytes); }
+    __device__ __forceinline__ void expect(int s, uint32_t bytes) const {
+        *issued = *issued + 1;
+        mbar_arrive_expect_tx(bar0 + 8u * s, bytes);
+    }
+    // Thread 0: the stage may be filled again, unless a wait ran out before.
+    __device__ __forceinline__ bool open() const { return *abort_flag == 0; }
+    // Thread 0, at the end: after a wait that ran out, what was begun is still waited for.
+    __device__ __forceinline__ void drain() const {
+        if (*abort_flag != 0) drain_ring(*issued, stages, [&](int s) { return bar0 + 8u * s; }, limit_ns);
+    }
     __device__ __forceinline__ void copy(int s, int at, const void *src, uint32_t bytes) const {
         bulk_load(smem_addr(data) + static_cast<uint32_t>(s * stage_bytes + at), src, bytes, bar0 + 8u * s);
     }
@@ -375,19 +384,6 @@ __device__ __forceinline__ void cta_sum(float (&v)[N], int warps, int warp, int 
     }
 }
 
-// Maxima of four blocks that 16 lanes hold each: every exchange halves the
-// blocks that a lane still carries, so a lane ends with the maximum of block
-// (lane >> 2) & 3 of its half warp.
-__device__ __forceinline__ float max_of_four(const float (&m)[4], int lane) {
-    const bool up = lane & 8, odd = lane & 4;
-    float k0 = up ? m[2] : m[0], k1 = up ? m[3] : m[1];
-    k0 = max_abs(k0, __shfl_xor_sync(0xffffffffu, up ? m[0] : m[2], 8));
-    k1 = max_abs(k1, __shfl_xor_sync(0xffffffffu, up ? m[1] : m[3], 8));
-    float k = max_abs(odd ? k1 : k0, __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 4));
-    k = max_abs(k, __shfl_xor_sync(0xffffffffu, k, 2));
-    return max_abs(k, __shfl_xor_sync(0xffffffffu, k, 1));
-}
-
 constexpr int kRowVecs = 4;  // chunks of 8 elements a thread: its share of the sums' and scales' cost stays small
 
 // x is read twice from its stage instead of being kept: at 128 registers with
@@ -398,13 +394,13 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
     extern __shared__ __align__(128) uint8_t ring_smem[];
     __shared__ float4 slots[2 * 4];
     __shared__ uint64_t bars[kMaxStages];
-    __shared__ int aborted;
+    __shared__ int aborted, issued;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t first = blockIdx.x, step = gridDim.x;
     const int cols = static_cast<int>(p.cols);
     const int x_bytes = cols * static_cast<int>(sizeof(TX)), r_bytes = cols * static_cast<int>(sizeof(TR));
     const int r_at = (x_bytes + 127) / 128 * 128;
-    const RowRing ring{smem_addr(bars), ring_smem, stages, r_at + (r_bytes + 127) / 128 * 128, &aborted, p.err, p.limit_ns};
+    const RowRing ring{smem_addr(bars), ring_smem, stages, r_at + (r_bytes + 127) / 128 * 128, &aborted, &issued, p.err, p.limit_ns};
     if (threadIdx.x < 32) reinterpret_cast<float *>(slots)[threadIdx.x] = 0.0f;
     ring.init();
     pdl_wait();
@@ -495,7 +491,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
         float sum[1] = {lo2(a) + hi2(a)};
         cta_sum<1>(sum, warps, warp, lane, slots, slot);
         // every thread has read the stage: the next row that it is for may come in
-        if (threadIdx.x == 0 && row + stages * step < p.rows) fetch(s, row + stages * step);
+        if (threadIdx.x == 0 && row + stages * step < p.rows && ring.open()) fetch(s, row + stages * step);
         if (has_pre) {
             const uint64_t inv_r = twice(rsqrtf(sum[0] * inv_cols + p.eps));
             float top[VPT];
@@ -529,6 +525,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
             ph ^= 1u;
         }
     }
+    if (threadIdx.x == 0) ring.drain();
     pdl_trigger();
 }
 
@@ -742,7 +739,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
     extern __shared__ __align__(128) uint8_t ring_smem[];
     __shared__ float4 slots[2 * 3 * 4];
     __shared__ uint64_t bars[kMaxStages];
-    __shared__ int aborted;
+    __shared__ int aborted, issued;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t first = blockIdx.x, step = gridDim.x;
     const int cols = static_cast<int>(p.cols);
@@ -751,7 +748,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
     const uint32_t x_bytes = static_cast<uint32_t>(cols) * sizeof(TX), r_bytes = static_cast<uint32_t>(cols) * sizeof(TR);
     const int x_room = (x_bytes + 127) / 128 * 128, r_room = (r_bytes + 127) / 128 * 128;
     const int dh_at = has_x ? x_room : 0, r_at = dh_at + (has_pre ? x_room : 0), dr_at = r_at + (has_pre ? r_room : 0);
-    const RowRing ring{smem_addr(bars), ring_smem, stages, dr_at + (has_dr ? r_room : 0), &aborted, p.err, p.limit_ns};
+    const RowRing ring{smem_addr(bars), ring_smem, stages, dr_at + (has_dr ? r_room : 0), &aborted, &issued, p.err, p.limit_ns};
     if (threadIdx.x < 32)
         for (int i = 0; i < 3; ++i) reinterpret_cast<float *>(slots)[threadIdx.x + 32 * i] = 0.0f;
     ring.init();
@@ -881,7 +878,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
         float es[1] = {lo2(e) + hi2(e)};
         cta_sum<3>(es, warps, warp, lane, slots, slot);
         // every thread has read the stage: the next row that it is for may come in
-        if (threadIdx.x == 0 && row + stages * step < p.rows) fetch(s, row + stages * step);
+        if (threadIdx.x == 0 && row + stages * step < p.rows && ring.open()) fetch(s, row + stages * step);
         if (has_x) {
             if (p.gate_mode == kGateToken && threadIdx.x == 0) static_cast<float *>(p.dgate.p)[row * p.dgate.ld] = es[0];
             const uint64_t minus = twice(has_post ? -g * es[0] * inv_cols : 0.0f);
@@ -905,6 +902,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
         if (planes.pre >= 0) write8<float>(out + (planes.pre * step + first) * p.cols + col[v], spre[v]);
         if (planes.post >= 0) write8<float>(out + (planes.post * step + first) * p.cols + col[v], spost[v]);
     }
+    if (threadIdx.x == 0) ring.drain();
     pdl_trigger();
 }
 

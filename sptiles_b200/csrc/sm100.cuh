@@ -70,6 +70,15 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const v
     }
 }
 
+// Bulk copies still in flight after `issued` of them through a ring of
+// barriers: wait (bounded, whatever the abort flag says) before leaving.
+template <typename Bar>
+__device__ __forceinline__ void drain_ring(int issued, int stages, Bar bar, uint64_t limit_ns) {
+    const volatile int never = 0;
+    for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+        (void)mbar_wait(bar(i % stages), static_cast<uint32_t>(i / stages) & 1u, &never, limit_ns);
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");

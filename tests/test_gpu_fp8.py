@@ -367,3 +367,51 @@ def test_matmul_large_layouts(b_square, b_rows, a_rows):
     a, b, sa, sb = make(m, n, k, a_square=b_rows, b_square=b_square)
     C = st.matmul_fp8(put(a, a_rows), put(b, b_rows, aligned=a_rows).t(), sa.to(DEV), sb.t().contiguous().to(DEV), out_dtype=torch.float32)
     check_product(C, a, b, sa, sb, None, torch.float32)
+
+
+# ------------------------------------------------------------------ offsets past 32 bits
+def some_codes(rows, cols, seed):
+    """Codes below 2 in magnitude (so none is NaN), made on the GPU."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randint(0, 256, (rows, cols), generator=g, device=DEV, dtype=torch.uint8).bitwise_and_(0xBF).view(E4)
+
+
+@pytest.mark.parametrize("block", [(1, 128), (128, 1), (128, 128)], ids=["row", "column", "square"])
+def test_quantize_many_elements(block):
+    rows, cols, first = 140000, 16384, 139904
+    x = torch.randn(rows, cols, device=DEV, dtype=torch.bfloat16)
+    Q, S = st.quantize_fp8(x, block=block)
+    q, s = plain_quantize(x[first:].cpu(), block, E4)
+    same_codes(Q[first:], q)
+    assert torch.equal(S[-s.shape[0]:].cpu(), s)
+
+
+def test_quantize_longest_row():
+    cols = 2 ** 31 - 1
+    x = torch.zeros(1, cols, device=DEV, dtype=torch.bfloat16)
+    tail = torch.randn(1, 127 + 256, generator=gen(3)).to(torch.bfloat16)
+    x[:, -tail.shape[1]:] = tail.to(DEV)
+    Q, S = st.quantize_fp8(x)
+    q, s = plain_quantize(tail, (1, 128), E4)
+    same_codes(Q[:, -tail.shape[1]:], q)
+    assert torch.equal(S[:, -3:].cpu(), s) and (S[:, :-3] == 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("aligned", [True, False], ids=["aligned", "off"])
+def test_matmul_many_weights(aligned):
+    m, n, k, last = 3, 270000, 8192, 300
+    a, _, sa, _ = make(m, 1, k)
+    ld = k if aligned else k + 1
+    w = some_codes(1, n * ld, 1).as_strided((n, k), (ld, 1))
+    sb = torch.rand(n, k // 128, device=DEV)
+    C = st.matmul_fp8(put(a), w.t(), sa.to(DEV), sb.t(), out_dtype=torch.float32)
+    check_product(C[:, -last:], a, w[-last:].cpu(), sa, sb[-last:].cpu(), None, torch.float32)
+
+
+def test_matmul_many_results():
+    m, n, k, last = 33000, 66000, 128, 300
+    a, w = some_codes(m, k, 1), some_codes(n, k, 2)
+    sa, sb = torch.rand(m, 1, device=DEV), torch.rand(-(-n // 128), 1, device=DEV)
+    C = st.matmul_fp8(a, w.t(), sa, sb.t())
+    part = sb.repeat_interleave(128, 0)[:n][-last:]
+    check_product(C[-last:, -last:], a[-last:].cpu(), w[-last:].cpu(), sa[-last:].cpu(), part.cpu(), None, torch.bfloat16)

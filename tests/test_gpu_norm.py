@@ -366,3 +366,56 @@ def test_backward_zero_token_gate():
         d["gate"][::2] = 0
         got = check_backward(d, rows, 640, F32, F32)
         assert (got.x[::2] == 0).all() and (got.gate[::2] != 0).all()
+
+
+def test_many_elements():
+    """Offsets past 32 bits: the last rows of 2^31 and more elements."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for rows, cols in [(140000, 16384), (270000, 8192)]:
+        x, r, dr, dh = (torch.randn(rows, cols, generator=g, device=DEV, dtype=BF16) for _ in range(4))
+        w = torch.rand(cols, generator=g, device=DEV).to(BF16)
+        f = st.residual_norm(x, r, w, None, w, eps=EPS, quantize=True)
+        b = st.residual_norm_backward(dr, dh, x, r, w, None, w, eps=EPS)
+        last = {"x": x[-5:].cpu(), "r": r[-5:].cpu(), "post": w.cpu(), "pre": w.cpu(), "gate": None}
+        want, mass, h = forward64(dbl(last), 1.0, 0.0)
+        close(f.residual[-5:], want, mass, BF16)
+        same = st.residual_norm(x[-5:].clone(), r[-5:].clone(), w, None, w, eps=EPS, quantize=True)
+        back = [(v.normed[-5:].double() * v.scale[-5:].double().repeat_interleave(128, 1)).cpu() for v in (f, same)]
+        for v in back:  # half a step of e4m3, or of the block's smallest code, and the fp32 sums' REL
+            least = 2.0 ** -10 * f.scale[-5:].double().cpu().repeat_interleave(128, 1)
+            assert ((v - h).abs() <= 2.0 ** -4 * h.abs() + least + 8 * REL * (mass + h.abs())).all()
+        want, mass = backward64(dbl(last), dr[-5:].double().cpu(), dh[-5:].double().cpu(), 1.0, 0.0)
+        close(b.residual[-5:], want["residual"], mass["residual"], BF16)
+        close(b.x[-5:], want["x"], mass["x"], BF16)
+        del x, r, dr, dh, f, b
+
+
+def test_two_streams_at_once():
+    """Two training steps under way on two streams, each with tensors of its own, as one after the other."""
+    rows, cols = 900, 2048
+    sets = [dev(inputs(rows, cols, BF16, F32, "channel", True, True, seed=s)) for s in (0, 2)]
+    grads = [torch.randn(rows, cols, generator=gen(3 + s)).to(DEV) for s in (0, 1)]
+
+    def step(d, dr):
+        f = st.residual_norm(d["x"], d["r"], d["post"], d["gate"], d["pre"])
+        b = st.residual_norm_backward(dr, dr.to(BF16), d["x"], f.residual, d["post"], d["gate"], d["pre"])
+        return [f.residual, f.normed, *b]
+
+    want = [step(d, g) for d, g in zip(sets, grads)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(sets[i], grads[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
+
+
+def test_widest_rows():
+    """16384 columns in every type, where a row fills one stage of the ring."""
+    for tx, tr in [(F32, F32), (BF16, F32), (F16, F16)]:
+        check_forward(inputs(400, 16384, tx, tr, "channel", True, True, seed=1), quantize=True)
+        check_backward(inputs(320, 16384, tx, tr, "token", True, True, seed=1), 320, 16384, tx, tr)
