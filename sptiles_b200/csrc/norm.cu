@@ -296,47 +296,49 @@ __global__ void __launch_bounds__(kMaxThreads, VPT == 1 && !AHEAD ? 2 : 1) resid
 // does not depend on registers or on where the row before stands between its
 // two sums; the weights stay in registers over the rows, folded into one
 // factor per element and norm.
+constexpr int kMaxStages = 8;
+
 struct RowRing {
     uint32_t bar0;
     uint8_t *data;
     int stages, stage_bytes;
     volatile int *abort_flag;
-    volatile int *issued;  // rows whose copies have begun
     int *err;
     uint64_t limit_ns;
     __device__ __forceinline__ void init() const {
         if (threadIdx.x == 0) {
             for (int s = 0; s < stages; ++s) mbar_init(bar0 + 8u * s, 1);
-            *abort_flag = *issued = 0;
+            *abort_flag = 0;
             fence_barrier_init();
         }
         __syncthreads();
     }
     __device__ __forceinline__ uint8_t *stage(int s) const { return data + s * stage_bytes; }
     // One thread: begin the copies of stage s (`bytes` in all).
-    __device__ __forceinline__ void expect(int s, uint32_t bytes) const {
-        *issued = *issued + 1;
-        mbar_arrive_expect_tx(bar0 + 8u * s, bytes);
-    }
-    // Thread 0: the stage may be filled again, unless a wait ran out before.
-    __device__ __forceinline__ bool open() const { return *abort_flag == 0; }
-    // Thread 0, at the end: after a wait that ran out, what was begun is still waited for.
-    __device__ __forceinline__ void drain() const {
-        if (*abort_flag != 0) drain_ring(*issued, stages, [&](int s) { return bar0 + 8u * s; }, limit_ns);
-    }
+    __device__ __forceinline__ void expect(int s, uint32_t bytes) const { mbar_arrive_expect_tx(bar0 + 8u * s, bytes); }
     __device__ __forceinline__ void copy(int s, int at, const void *src, uint32_t bytes) const {
         bulk_load(smem_addr(data) + static_cast<uint32_t>(s * stage_bytes + at), src, bytes, bar0 + 8u * s);
+    }
+    // Thread 0: stages may be filled again, unless a wait ran out.
+    __device__ __forceinline__ bool open() const { return *abort_flag == 0; }
+    // Thread 0, at the end: after a wait that ran out, what is on its way is
+    // waited for.  A stage's current phase is not known then: one of the two
+    // waits returns at once, the other with the copies or, where none is under
+    // way, at its share of the limit.
+    __device__ __forceinline__ void drain() const {
+        if (open()) return;
+        const volatile int never = 0;
+        for (int q = 0; q < 2 * stages; ++q) (void)mbar_wait(bar0 + 8u * (q >> 1), q & 1u, &never, limit_ns / kMaxStages);
     }
     // Every thread: a wait that ran out is recorded and lets the CTA run on
     // (all later waits return at once), so that no barrier is missed.
     __device__ __forceinline__ void wait(int s, uint32_t parity) const {
         if (mbar_wait(bar0 + 8u * s, parity, abort_flag, limit_ns)) return;
-        if (*abort_flag == 0) atomicExch(err, kDevAbortNorm);
+        if (*abort_flag != 0) return;
+        atomicExch(err, kDevAbortNorm);
         *abort_flag = 1;
     }
 };
-
-constexpr int kMaxStages = 8;
 
 template <typename T>
 __device__ __forceinline__ void read8(const uint8_t *row, int col, uint64_t (&f)[4]) {
@@ -394,13 +396,13 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
     extern __shared__ __align__(128) uint8_t ring_smem[];
     __shared__ float4 slots[2 * 4];
     __shared__ uint64_t bars[kMaxStages];
-    __shared__ int aborted, issued;
+    __shared__ int aborted;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t first = blockIdx.x, step = gridDim.x;
     const int cols = static_cast<int>(p.cols);
     const int x_bytes = cols * static_cast<int>(sizeof(TX)), r_bytes = cols * static_cast<int>(sizeof(TR));
     const int r_at = (x_bytes + 127) / 128 * 128;
-    const RowRing ring{smem_addr(bars), ring_smem, stages, r_at + (r_bytes + 127) / 128 * 128, &aborted, &issued, p.err, p.limit_ns};
+    const RowRing ring{smem_addr(bars), ring_smem, stages, r_at + (r_bytes + 127) / 128 * 128, &aborted, p.err, p.limit_ns};
     if (threadIdx.x < 32) reinterpret_cast<float *>(slots)[threadIdx.x] = 0.0f;
     ring.init();
     pdl_wait();
@@ -739,7 +741,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
     extern __shared__ __align__(128) uint8_t ring_smem[];
     __shared__ float4 slots[2 * 3 * 4];
     __shared__ uint64_t bars[kMaxStages];
-    __shared__ int aborted, issued;
+    __shared__ int aborted;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t first = blockIdx.x, step = gridDim.x;
     const int cols = static_cast<int>(p.cols);
@@ -748,7 +750,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
     const uint32_t x_bytes = static_cast<uint32_t>(cols) * sizeof(TX), r_bytes = static_cast<uint32_t>(cols) * sizeof(TR);
     const int x_room = (x_bytes + 127) / 128 * 128, r_room = (r_bytes + 127) / 128 * 128;
     const int dh_at = has_x ? x_room : 0, r_at = dh_at + (has_pre ? x_room : 0), dr_at = r_at + (has_pre ? r_room : 0);
-    const RowRing ring{smem_addr(bars), ring_smem, stages, dr_at + (has_dr ? r_room : 0), &aborted, &issued, p.err, p.limit_ns};
+    const RowRing ring{smem_addr(bars), ring_smem, stages, dr_at + (has_dr ? r_room : 0), &aborted, p.err, p.limit_ns};
     if (threadIdx.x < 32)
         for (int i = 0; i < 3; ++i) reinterpret_cast<float *>(slots)[threadIdx.x + 32 * i] = 0.0f;
     ring.init();
