@@ -724,6 +724,13 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
     pdl_trigger();
 }
 
+// What a ring kernel's call has: every tensor, with no gate of a row's or with
+// one, is known to the compiler; any other set is looked up in each row.
+enum class Parts { kSome, kPlain, kToken, kFull };
+inline Parts whole(int gate_mode) {
+    return gate_mode == kGateToken ? Parts::kToken : gate_mode == kGateFull ? Parts::kFull : Parts::kPlain;
+}
+
 // Backward for many rows on 16-byte boundaries, as residual_norm_rows_kernel:
 // a ring of rows of x, dh, r and dr', the factors and the sums over rows in
 // registers.  With X = x * inv_x and c1 = alpha * gate * (post + offset) (the
@@ -733,11 +740,12 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
 // (times an element's g), the mean in dx and a token's dgate.
 constexpr int kBackVecs = 2;
 
-template <typename TX, typename TR>
+template <typename TX, typename TR, Parts PARTS>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kernel(const NormBackwardArgs p, int warps,
                                                                                   const Planes planes, float *out,
                                                                                   int stages) {
     constexpr int VPT = kBackVecs;
+    constexpr bool ALL = PARTS != Parts::kSome, PLAIN = PARTS == Parts::kPlain;
     extern __shared__ __align__(128) uint8_t ring_smem[];
     __shared__ float4 slots[2 * 3 * 4];
     __shared__ uint64_t bars[kMaxStages];
@@ -745,8 +753,10 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t first = blockIdx.x, step = gridDim.x;
     const int cols = static_cast<int>(p.cols);
-    const bool has_x = p.x.p != nullptr, has_post = p.post.p != nullptr, has_pre = p.pre.p != nullptr;
-    const bool has_dr = p.d_residual.p != nullptr;
+    const bool has_x = ALL || p.x.p != nullptr, has_post = ALL || p.post.p != nullptr, has_pre = ALL || p.pre.p != nullptr;
+    const bool has_dr = ALL || p.d_residual.p != nullptr;
+    const bool token = PARTS == Parts::kToken || (!ALL && p.gate_mode == kGateToken);
+    const bool full = PARTS == Parts::kFull || (!ALL && p.gate_mode == kGateFull);
     const uint32_t x_bytes = static_cast<uint32_t>(cols) * sizeof(TX), r_bytes = static_cast<uint32_t>(cols) * sizeof(TR);
     const int x_room = (x_bytes + 127) / 128 * 128, r_room = (r_bytes + 127) / 128 * 128;
     const int dh_at = has_x ? x_room : 0, r_at = dh_at + (has_pre ? x_room : 0), dr_at = r_at + (has_pre ? r_room : 0);
@@ -802,7 +812,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
     uint32_t ph = 0;
     for (int64_t row = first; row < p.rows; row += step) {
         float g = 1.0f;
-        if (p.gate_mode == kGateToken) g = load1_of<TX>(p.gate, row);
+        if (token) g = load1_of<TX>(p.gate, row);
         ring.wait(s, ph);
         const uint8_t *stage = ring.stage(s);
         float sum[3] = {0.0f, 0.0f, 0.0f};  // of r^2, r t and x^2
@@ -853,11 +863,11 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
                     d[v][j] = fma2(inv_r2, fma2(R, less, mul2(dh[j], c2[v][j])), d[v][j]);
                 }
             }
-            if (p.dr.p != nullptr) write8<TR>(static_cast<TR *>(p.dr.p) + row * p.dr.ld + col[v], d[v]);
+            if (ALL || p.dr.p != nullptr) write8<TR>(static_cast<TR *>(p.dr.p) + row * p.dr.ld + col[v], d[v]);
             if (!has_x) continue;
             read8<TX>(stage, col[v], hat[v]);
             uint64_t gate[4] = {twice(g), twice(g), twice(g), twice(g)}, q[4];
-            if (p.gate_mode == kGateFull) {
+            if (full) {
                 float w[8];
                 load8_of<TX, true>(p.gate, row, (v * warps + warp) * kChunk, lane, cols, w);
 #pragma unroll
@@ -867,12 +877,13 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
             for (int j = 0; j < 4; ++j) {
                 hat[v][j] = mul2(hat[v][j], inv_x2);
                 q[j] = mul2(d[v][j], hat[v][j]);
-                spost[v][j] = fma2(q[j], gate[j], spost[v][j]);
+                spost[v][j] = PLAIN ? add2(q[j], spost[v][j]) : fma2(q[j], gate[j], spost[v][j]);
                 q[j] = mul2(q[j], c1[v][j]);
-                e = p.gate_mode == kGateFull ? fma2(q[j], gate[j], e) : add2(q[j], e);
-                d[v][j] = mul2(mul2(d[v][j], c1[v][j]), gate[j]);
+                e = full ? fma2(q[j], gate[j], e) : add2(q[j], e);
+                d[v][j] = mul2(d[v][j], c1[v][j]);
+                if (!PLAIN) d[v][j] = mul2(d[v][j], gate[j]);
             }
-            if (p.gate_mode == kGateFull) {
+            if (full) {
                 if (p.dgate.dtype == ST_F32) write8<float>(static_cast<float *>(p.dgate.p) + row * p.dgate.ld + col[v], q);
                 else write8<TX>(static_cast<TX *>(p.dgate.p) + row * p.dgate.ld + col[v], q);
             }
@@ -882,8 +893,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
         // every thread has read the stage: the next row that it is for may come in
         if (threadIdx.x == 0 && row + stages * step < p.rows && ring.open()) fetch(s, row + stages * step);
         if (has_x) {
-            if (p.gate_mode == kGateToken && threadIdx.x == 0) static_cast<float *>(p.dgate.p)[row * p.dgate.ld] = es[0];
-            const uint64_t minus = twice(has_post ? -g * es[0] * inv_cols : 0.0f);
+            if (token && threadIdx.x == 0) static_cast<float *>(p.dgate.p)[row * p.dgate.ld] = es[0];
+            const uint64_t minus = twice(has_post ? (PLAIN ? -es[0] : -g * es[0]) * inv_cols : 0.0f);
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
                 if (col[v] >= cols) continue;
@@ -901,8 +912,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
         if (col[v] >= cols) continue;
-        if (planes.pre >= 0) write8<float>(out + (planes.pre * step + first) * p.cols + col[v], spre[v]);
-        if (planes.post >= 0) write8<float>(out + (planes.post * step + first) * p.cols + col[v], spost[v]);
+        if (ALL || planes.pre >= 0) write8<float>(out + (planes.pre * step + first) * p.cols + col[v], spre[v]);
+        if (ALL || planes.post >= 0) write8<float>(out + (planes.post * step + first) * p.cols + col[v], spost[v]);
     }
     if (threadIdx.x == 0) ring.drain();
     pdl_trigger();
@@ -1104,6 +1115,17 @@ int finish_sums(const ColumnSums &todo, const float *sums, int planes, int64_t g
     return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "column_sums_kernel");
 }
 
+template <typename TX, typename TR, Parts PARTS>
+int backward_rows(const NormBackwardArgs &p, const Planes &planes, float *sums, cudaStream_t stream, int *groups) {
+    static uint64_t attr_set = 0;  // one bit per device ordinal
+    const int warps = static_cast<int>(cdiv(p.cols, kBackVecs * kChunk));
+    const int stage = (p.x.p != nullptr ? row_bytes(p.cols, sizeof(TX)) : 0) +
+                      (p.pre.p != nullptr ? row_bytes(p.cols, sizeof(TX)) + row_bytes(p.cols, sizeof(TR)) : 0) +
+                      (p.d_residual.p != nullptr ? row_bytes(p.cols, sizeof(TR)) : 0);
+    return launch_rows(residual_norm_backward_rows_kernel<TX, TR, PARTS>, attr_set, 32 * warps, stage, p.rows,
+                       static_cast<int>(kGroupSms), stream, groups, p, warps, planes, sums);
+}
+
 template <typename TX, typename TR>
 int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) {
     auto side = [](const NormView &v) { return v.dtype == ST_F32 ? sizeof(float) : sizeof(TX); };
@@ -1126,14 +1148,15 @@ int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) 
         if (p.dpost != nullptr || channel) planes.post = planes.count++;
         if (p.dpost != nullptr) todo.sum[todo.count++] = {p.dpost, planes.post, p.alpha, 0.0f, channel ? p.gate : NormView{}};
         if (channel) todo.sum[todo.count++] = {static_cast<float *>(p.dgate.p), planes.post, p.alpha, p.offset, p.post};
-        static uint64_t attr_set = 0;  // one bit per device ordinal
-        const int warps = static_cast<int>(cdiv(p.cols, kBackVecs * kChunk));
-        const int stage = (p.x.p != nullptr ? row_bytes(p.cols, sizeof(TX)) : 0) +
-                          (p.pre.p != nullptr ? row_bytes(p.cols, sizeof(TX)) + row_bytes(p.cols, sizeof(TR)) : 0) +
-                          (p.d_residual.p != nullptr ? row_bytes(p.cols, sizeof(TR)) : 0);
+        const bool all = p.x.p != nullptr && p.post.p != nullptr && p.pre.p != nullptr && p.d_residual.p != nullptr &&
+                         p.dr.p != nullptr && planes.pre >= 0 && planes.post >= 0;
         int groups = 0;
-        ST_TRY(launch_rows(residual_norm_backward_rows_kernel<TX, TR>, attr_set, 32 * warps, stage, p.rows,
-                           static_cast<int>(kGroupSms), stream, &groups, p, warps, planes, sums));
+        switch (all ? whole(p.gate_mode) : Parts::kSome) {
+        case Parts::kSome: ST_TRY((backward_rows<TX, TR, Parts::kSome>(p, planes, sums, stream, &groups))); break;
+        case Parts::kPlain: ST_TRY((backward_rows<TX, TR, Parts::kPlain>(p, planes, sums, stream, &groups))); break;
+        case Parts::kToken: ST_TRY((backward_rows<TX, TR, Parts::kToken>(p, planes, sums, stream, &groups))); break;
+        case Parts::kFull: ST_TRY((backward_rows<TX, TR, Parts::kFull>(p, planes, sums, stream, &groups))); break;
+        }
         return finish_sums<TX>(todo, sums, planes.count, groups, p.cols, stream);
     }
     const Shape s = shape_of(p.rows, p.cols, backward_groups(p.rows, p.cols), false);
