@@ -1035,7 +1035,8 @@ int launch_rows(Kern kern, uint64_t &attr_set, int threads, int stage_bytes, int
         ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
         if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
     }
-    const int per_sm = kMaxThreads / threads;  // at 128 registers a thread
+    int per_sm = kMaxThreads / threads;  // at 128 registers a thread
+    while (per_sm > 1 && kMostSmem / per_sm / stage_bytes < 2) --per_sm;  // one stage a CTA leaves nothing in flight
     int stages = kMostSmem / per_sm / stage_bytes;
     stages = stages > kMaxStages ? kMaxStages : stages;
     const int64_t ctas = rows < sm_count * per_sm ? rows : sm_count * per_sm;
