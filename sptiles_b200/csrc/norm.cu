@@ -386,13 +386,21 @@ __device__ __forceinline__ void cta_sum(float (&v)[N], int warps, int warp, int 
     }
 }
 
+// What a ring kernel's call has: every tensor, with no gate of a row's or with
+// one, is known to the compiler; any other set is looked up in each row.
+enum class Parts { kSome, kPlain, kToken, kFull };
+inline Parts whole(int gate_mode) {
+    return gate_mode == kGateToken ? Parts::kToken : gate_mode == kGateFull ? Parts::kFull : Parts::kPlain;
+}
+
 constexpr int kRowVecs = 4;  // chunks of 8 elements a thread: its share of the sums' and scales' cost stays small
 
 // x is read twice from its stage instead of being kept: at 128 registers with
 // both factors and r in them, 16 warps of an SM are at work.
-template <typename TX, typename TR>
+template <typename TX, typename TR, Parts PARTS>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const NormArgs p, int warps, int stages) {
     constexpr int VPT = kRowVecs;
+    constexpr bool ALL = PARTS != Parts::kSome;
     extern __shared__ __align__(128) uint8_t ring_smem[];
     __shared__ float4 slots[2 * 4];
     __shared__ uint64_t bars[kMaxStages];
@@ -401,22 +409,27 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
     const int64_t first = blockIdx.x, step = gridDim.x;
     const int cols = static_cast<int>(p.cols);
     const int x_bytes = cols * static_cast<int>(sizeof(TX)), r_bytes = cols * static_cast<int>(sizeof(TR));
-    const int r_at = (x_bytes + 127) / 128 * 128;
-    const RowRing ring{smem_addr(bars), ring_smem, stages, r_at + (r_bytes + 127) / 128 * 128, &aborted, p.err, p.limit_ns};
+    const bool token_gate = PARTS == Parts::kToken || (!ALL && p.gate_mode == kGateToken);
+    const bool full_gate = PARTS == Parts::kFull || (!ALL && p.gate_mode == kGateFull);
+    const int gate_size = p.gate.dtype == ST_F32 ? 4 : static_cast<int>(sizeof(TX)), gate_bytes = full_gate ? cols * gate_size : 0;
+    const int r_at = (x_bytes + 127) / 128 * 128, gate_at = r_at + (r_bytes + 127) / 128 * 128;
+    const RowRing ring{smem_addr(bars), ring_smem, stages, gate_at + (gate_bytes + 127) / 128 * 128, &aborted, p.err, p.limit_ns};
     if (threadIdx.x < 32) reinterpret_cast<float *>(slots)[threadIdx.x] = 0.0f;
     ring.init();
     pdl_wait();
     auto fetch = [&](int s, int64_t row) {
-        ring.expect(s, static_cast<uint32_t>(x_bytes + r_bytes));
+        ring.expect(s, static_cast<uint32_t>(x_bytes + r_bytes + gate_bytes));
         ring.copy(s, 0, static_cast<const TX *>(p.x.p) + row * p.x.ld, static_cast<uint32_t>(x_bytes));
         ring.copy(s, r_at, static_cast<const TR *>(p.r.p) + row * p.r.ld, static_cast<uint32_t>(r_bytes));
+        if (full_gate)
+            ring.copy(s, gate_at, static_cast<const uint8_t *>(p.gate.p) + row * p.gate.ld * gate_size, static_cast<uint32_t>(gate_bytes));
     };
     if (threadIdx.x == 0)
         for (int s = 0; s < stages; ++s)
             if (first + s * step < p.rows) fetch(s, first + s * step);
 
     const float inv_cols = 1.0f / static_cast<float>(p.cols);
-    const bool has_post = p.post.p != nullptr, has_pre = p.pre.p != nullptr;
+    const bool has_post = ALL || p.post.p != nullptr, has_pre = ALL || p.pre.p != nullptr;
     // branch factor alpha * gate * (post + offset), norm factor pre + offset
     uint64_t c1[VPT][4], c2[VPT][4];
     int col[VPT];
@@ -448,7 +461,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
     uint32_t ph = 0;
     for (int64_t row = first; row < p.rows; row += step) {
         float token = 1.0f;
-        if (p.gate_mode == kGateToken) token = load1_of<TX>(p.gate, row);
+        if (token_gate) token = load1_of<TX>(p.gate, row);
         ring.wait(s, ph);
         const uint8_t *stage = ring.stage(s);
         float inv = token;
@@ -477,11 +490,12 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_rows_kernel(const N
             uint64_t x[4];
             read8<TX>(stage, col[v], x);
             read8<TR>(stage + r_at, col[v], r[v]);
-            if (p.gate_mode == kGateFull) {
-                float w[8];
-                load8_of<TX, true>(p.gate, row, (v * warps + warp) * kChunk, lane, cols, w);
+            if (full_gate) {
+                uint64_t gate[4];
+                if (gate_size == 4) read8<float>(stage + gate_at, col[v], gate);
+                else read8<TX>(stage + gate_at, col[v], gate);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = mul2(x[j], pack2(w[2 * j], w[2 * j + 1]));
+                for (int j = 0; j < 4; ++j) x[j] = mul2(x[j], gate[j]);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -724,13 +738,6 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
     pdl_trigger();
 }
 
-// What a ring kernel's call has: every tensor, with no gate of a row's or with
-// one, is known to the compiler; any other set is looked up in each row.
-enum class Parts { kSome, kPlain, kToken, kFull };
-inline Parts whole(int gate_mode) {
-    return gate_mode == kGateToken ? Parts::kToken : gate_mode == kGateFull ? Parts::kFull : Parts::kPlain;
-}
-
 // Backward for many rows on 16-byte boundaries, as residual_norm_rows_kernel:
 // a ring of rows of x, dh, r and dr', the factors and the sums over rows in
 // registers.  With X = x * inv_x and c1 = alpha * gate * (post + offset) (the
@@ -760,13 +767,17 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
     const uint32_t x_bytes = static_cast<uint32_t>(cols) * sizeof(TX), r_bytes = static_cast<uint32_t>(cols) * sizeof(TR);
     const int x_room = (x_bytes + 127) / 128 * 128, r_room = (r_bytes + 127) / 128 * 128;
     const int dh_at = has_x ? x_room : 0, r_at = dh_at + (has_pre ? x_room : 0), dr_at = r_at + (has_pre ? r_room : 0);
-    const RowRing ring{smem_addr(bars), ring_smem, stages, dr_at + (has_dr ? r_room : 0), &aborted, p.err, p.limit_ns};
+    const int gate_size = p.gate.dtype == ST_F32 ? 4 : static_cast<int>(sizeof(TX)), gate_at = dr_at + (has_dr ? r_room : 0);
+    const uint32_t gate_bytes = full ? static_cast<uint32_t>(cols * gate_size) : 0;
+    const RowRing ring{smem_addr(bars), ring_smem, stages, gate_at + static_cast<int>((gate_bytes + 127) / 128 * 128), &aborted, p.err, p.limit_ns};
     if (threadIdx.x < 32)
         for (int i = 0; i < 3; ++i) reinterpret_cast<float *>(slots)[threadIdx.x + 32 * i] = 0.0f;
     ring.init();
     pdl_wait();
     auto fetch = [&](int s, int64_t row) {
-        ring.expect(s, (has_x ? x_bytes : 0) + (has_pre ? x_bytes + r_bytes : 0) + (has_dr ? r_bytes : 0));
+        ring.expect(s, (has_x ? x_bytes : 0) + (has_pre ? x_bytes + r_bytes : 0) + (has_dr ? r_bytes : 0) + gate_bytes);
+        if (full)
+            ring.copy(s, gate_at, static_cast<const uint8_t *>(p.gate.p) + row * p.gate.ld * gate_size, gate_bytes);
         if (has_x) ring.copy(s, 0, static_cast<const TX *>(p.x.p) + row * p.x.ld, x_bytes);
         if (has_pre) {
             ring.copy(s, dh_at, static_cast<const TX *>(p.d_normed.p) + row * p.d_normed.ld, x_bytes);
@@ -868,10 +879,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_rows_kerne
             read8<TX>(stage, col[v], hat[v]);
             uint64_t gate[4] = {twice(g), twice(g), twice(g), twice(g)}, q[4];
             if (full) {
-                float w[8];
-                load8_of<TX, true>(p.gate, row, (v * warps + warp) * kChunk, lane, cols, w);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) gate[j] = pack2(w[2 * j], w[2 * j + 1]);
+                if (gate_size == 4) read8<float>(stage + gate_at, col[v], gate);
+                else read8<TX>(stage + gate_at, col[v], gate);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -1050,12 +1059,19 @@ int launch_rows(Kern kern, uint64_t &attr_set, int threads, int stage_bytes, int
 
 int row_bytes(int64_t cols, size_t size) { return static_cast<int>((cols * size + 127) / 128 * 128); }
 
-template <typename TX, typename TR>
+// Bytes of a row of the gate, where it has one of its own.
+int gate_row_bytes(const NormView &gate, int mode, int64_t cols, size_t size) {
+    return mode == kGateFull ? row_bytes(cols, gate.dtype == ST_F32 ? sizeof(float) : size) : 0;
+}
+
+template <typename TX, typename TR, Parts PARTS>
 int forward_rows(const NormArgs &p, int sm_count, cudaStream_t stream) {
     static uint64_t attr_set = 0;  // one bit per device ordinal
     const int warps = static_cast<int>(cdiv(p.cols, kRowVecs * kChunk));
-    return launch_rows(residual_norm_rows_kernel<TX, TR>, attr_set, 32 * warps,
-                       row_bytes(p.cols, sizeof(TX)) + row_bytes(p.cols, sizeof(TR)), p.rows, sm_count, stream, nullptr, p,
+    return launch_rows(residual_norm_rows_kernel<TX, TR, PARTS>, attr_set, 32 * warps,
+                       row_bytes(p.cols, sizeof(TX)) + row_bytes(p.cols, sizeof(TR)) +
+                           gate_row_bytes(p.gate, p.gate_mode, p.cols, sizeof(TX)),
+                       p.rows, sm_count, stream, nullptr, p,
                        warps);
 }
 
@@ -1072,7 +1088,12 @@ int forward_typed(const NormArgs &p, int sm_count, cudaStream_t stream) {
     // flight otherwise
     const Shape s = shape_of(p.rows, p.cols, int64_t(1) << 30, p.rows < sm_count || !vec);
     if (vec && p.x.p != nullptr && p.r_out.p != nullptr && p.cols % 8 == 0 && p.cols > 2 * kChunk && p.rows >= 2 * sm_count)
-        return forward_rows<TX, TR>(p, sm_count, stream);
+        switch (p.post.p != nullptr && p.pre.p != nullptr ? whole(p.gate_mode) : Parts::kSome) {
+        case Parts::kSome: return forward_rows<TX, TR, Parts::kSome>(p, sm_count, stream);
+        case Parts::kPlain: return forward_rows<TX, TR, Parts::kPlain>(p, sm_count, stream);
+        case Parts::kToken: return forward_rows<TX, TR, Parts::kToken>(p, sm_count, stream);
+        case Parts::kFull: return forward_rows<TX, TR, Parts::kFull>(p, sm_count, stream);
+        }
     if (s.vpt == 1)
         return p.rows < sm_count ? forward_vpt<TX, TR, 1, true>(p, s, vec, stream)
                                  : forward_vpt<TX, TR, 1, false>(p, s, vec, stream);
@@ -1122,7 +1143,8 @@ int backward_rows(const NormBackwardArgs &p, const Planes &planes, float *sums, 
     const int warps = static_cast<int>(cdiv(p.cols, kBackVecs * kChunk));
     const int stage = (p.x.p != nullptr ? row_bytes(p.cols, sizeof(TX)) : 0) +
                       (p.pre.p != nullptr ? row_bytes(p.cols, sizeof(TX)) + row_bytes(p.cols, sizeof(TR)) : 0) +
-                      (p.d_residual.p != nullptr ? row_bytes(p.cols, sizeof(TR)) : 0);
+                      (p.d_residual.p != nullptr ? row_bytes(p.cols, sizeof(TR)) : 0) +
+                      gate_row_bytes(p.gate, p.gate_mode, p.cols, sizeof(TX));
     return launch_rows(residual_norm_backward_rows_kernel<TX, TR, PARTS>, attr_set, 32 * warps, stage, p.rows,
                        static_cast<int>(kGroupSms), stream, groups, p, warps, planes, sums);
 }
