@@ -419,3 +419,31 @@ def test_widest_rows():
     for tx, tr in [(F32, F32), (BF16, F32), (F16, F16)]:
         check_forward(inputs(400, 16384, tx, tr, "channel", True, True, seed=1), quantize=True)
         check_backward(inputs(320, 16384, tx, tr, "token", True, True, seed=1), 320, 16384, tx, tr)
+
+
+@pytest.mark.parametrize("rows", [3, 700])
+def test_outputs_left_out_in_c(rows):
+    """The C calls without an updated stream, without dr and without the sums (then with no workspace)."""
+    from sptiles_b200.fp8 import _desc, _fn, _vp, _cp, _u64
+    from sptiles_b200.norm import _OPTIONS
+    from sptiles_b200.api import _exec_desc
+
+    cols = 1024
+    d = dev(inputs(rows, cols, BF16, F32, "token", True, True))
+    dr, dh = torch.randn(rows, cols, generator=gen(1)).to(DEV), torch.randn(rows, cols, generator=gen(2)).to(BF16).to(DEV)
+    want = st.residual_norm(d["x"], d["r"], d["post"], d["gate"], d["pre"], eps=EPS)
+    back = st.residual_norm_backward(dr, dh, d["x"], want.residual, d["post"], d["gate"], d["pre"], eps=EPS)
+    ctx, opt, ex = st.runtime.context(0), _OPTIONS.pack(1.0, EPS, 0.0), _exec_desc(0)
+    normed = torch.empty(rows, cols, dtype=BF16, device=DEV)
+    forward = _fn("st_residual_norm", _vp, *[_cp] * 10)
+    x, r, post, gate, pre = (_desc(d[k]) for k in ("x", "r", "post", "gate", "pre"))
+    assert forward(ctx, x, r, post, gate, pre, None, _desc(normed), None, opt, ex) == 0
+    dx, dgate = torch.empty_like(d["x"]), torch.empty(rows, 1, device=DEV)
+    backward = _fn("st_residual_norm_backward", _vp, *[_cp] * 12, _vp, _u64, _cp, _cp)
+    assert backward(ctx, _desc(dr), _desc(dh), x, _desc(want.residual), post, gate, pre, _desc(dx), None, None, _desc(dgate),
+                    None, None, 0, opt, ex) == 0
+    torch.cuda.synchronize()
+    # the same arithmetic in another instance of the kernel: one step of the type and the sums' bound apart at most
+    for got, ref, dtype in [(normed, want.normed, BF16), (dx, back.x, BF16), (dgate, back.gate, F32)]:
+        mass = ref.double().abs().cpu() + ref.double().abs().max().cpu()
+        close(got, ref.double().cpu(), mass, dtype, rel=REL + torch.finfo(dtype).eps / 2)
