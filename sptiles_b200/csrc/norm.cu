@@ -949,32 +949,42 @@ struct ColumnSums {
     int count = 0;
 };
 
-// In a fixed order: 32 threads a column, each every 32nd group, then a
-// shuffle over them (two planes of 296 groups of 4096 columns in 7.9 us).  blockIdx.y picks the plane, read once for all its sums.
-template <typename T>
+// In a fixed order: 1024 / W threads a column, each every (1024 / W)th group,
+// then a sum over them.  W columns a CTA: 32 (two planes of 296 groups of 4096
+// columns in 7.9 us), or 8, a sector, where that would leave half of the SMs
+// idle: narrow rows have many groups (backward of 65536 x 256 in 55.8 us with
+// 32, 52.8 with 8; 32768 x 512 in 65.0 and 62.1; but 16384 x 2048 in 72.3 and
+// 73.5).  blockIdx.y picks the plane, read once for all its sums.
+template <typename T, int W>
 __global__ void __launch_bounds__(1024) column_sums_kernel(const float *sums, int groups, int cols, const ColumnSums todo) {
     pdl_wait();
-    __shared__ float part[32][33];
+    constexpr int kRows = 1024 / W;
+    __shared__ float part[kRows][W + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = static_cast<int>(blockIdx.x) * 32 + lane;
+    const int at = static_cast<int>(threadIdx.x) % W, first = static_cast<int>(threadIdx.x) / W;
+    const int c = static_cast<int>(blockIdx.x) * W + at;
     const float *src = sums + static_cast<int64_t>(blockIdx.y) * groups * cols + c;
     float s = 0.0f;
     if (c < cols) {
-        int i = warp;
-        for (; i + 96 < groups; i += 128) {  // four loads in flight
-            const float v0 = src[static_cast<int64_t>(i) * cols], v1 = src[static_cast<int64_t>(i + 32) * cols];
-            const float v2 = src[static_cast<int64_t>(i + 64) * cols], v3 = src[static_cast<int64_t>(i + 96) * cols];
+        int i = first;
+        for (; i + 3 * kRows < groups; i += 4 * kRows) {  // four loads in flight
+            const float v0 = src[static_cast<int64_t>(i) * cols], v1 = src[static_cast<int64_t>(i + kRows) * cols];
+            const float v2 = src[static_cast<int64_t>(i + 2 * kRows) * cols], v3 = src[static_cast<int64_t>(i + 3 * kRows) * cols];
             s += (v0 + v1) + (v2 + v3);
         }
-        for (; i < groups; i += 32) s += src[static_cast<int64_t>(i) * cols];
+        for (; i < groups; i += kRows) s += src[static_cast<int64_t>(i) * cols];
     }
-    part[warp][lane] = s;
+    part[first][at] = s;
     __syncthreads();
-    s = part[lane][warp];
+    if (warp < W) {
+        s = 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const int mine = static_cast<int>(blockIdx.x) * 32 + warp;
-    if (lane == 0 && mine < cols) {
+        for (int k = 0; k < kRows; k += 32) s += part[k + lane][warp];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    }
+    const int mine = static_cast<int>(blockIdx.x) * W + warp;
+    if (lane == 0 && warp < W && mine < cols) {
         for (int i = 0; i < todo.count; ++i) {
             const ColumnSum &o = todo.sum[i];
             if (o.plane != static_cast<int>(blockIdx.y)) continue;
@@ -1137,9 +1147,10 @@ int backward_vpt(const NormBackwardArgs &p, const Shape &s, bool vec, const Plan
 template <typename T>
 int finish_sums(const ColumnSums &todo, const float *sums, int planes, int64_t groups, int64_t cols, cudaStream_t stream) {
     if (todo.count == 0) return ST_OK;
-    ST_CUDA_TRY(launch_kernel(column_sums_kernel<T>,
-                              dim3(static_cast<unsigned>(cdiv(cols, 32)), static_cast<unsigned>(planes)), 1024, 0, stream, sums,
-                              static_cast<int>(groups), static_cast<int>(cols), todo));
+    const bool narrow = cdiv(cols, 32) * planes < kGroupSms / 2 && groups > 32;
+    ST_CUDA_TRY(launch_kernel(narrow ? column_sums_kernel<T, 8> : column_sums_kernel<T, 32>,
+                              dim3(static_cast<unsigned>(cdiv(cols, narrow ? 8 : 32)), static_cast<unsigned>(planes)), 1024, 0,
+                              stream, sums, static_cast<int>(groups), static_cast<int>(cols), todo));
     note_launch();
     const cudaError_t e = cudaPeekAtLastError();
     return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "column_sums_kernel");
