@@ -218,7 +218,7 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
 // would rather have the registers (unaligned 1025 x 2049 with a full gate in
 // 11.8 us; inputs not in L2: 16.5, and 19.6 at 128 registers a thread).
 template <typename TX, typename TR, int VPT, bool VEC, bool AHEAD>
-__global__ void __launch_bounds__(kMaxThreads, VPT == 1 && !AHEAD ? 2 : 1) residual_norm_kernel(const NormArgs p, int warps) {
+__global__ void __launch_bounds__(VPT == 1 && !AHEAD ? 2 * kMaxThreads : kMaxThreads) residual_norm_kernel(const NormArgs p, int warps) {
     pdl_wait();
     __shared__ float slots[2 * 3 * 32];
     const RowGroup g(warps);
@@ -1019,14 +1019,14 @@ struct Shape {
     int vpt, warps, ctas, threads;
 };
 
-// `rows` rows of `cols` on up to `most` row groups.
-Shape shape_of(int64_t rows, int64_t cols, int64_t most, bool one_chunk) {
+// `rows` rows of `cols` on up to `most` row groups; a chunk a thread up to `one_chunk` of them.
+Shape shape_of(int64_t rows, int64_t cols, int64_t most, int one_chunk) {
     Shape s;
     const int64_t chunks = cdiv(cols, kChunk);
     if (chunks <= 2) {
         s.vpt = static_cast<int>(chunks);
     } else {
-        s.vpt = one_chunk && chunks <= 16 ? 1 : chunks <= 32 ? 2 : 4;
+        s.vpt = chunks <= one_chunk ? 1 : chunks <= 32 ? 2 : 4;
     }
     s.warps = static_cast<int>(cdiv(chunks, s.vpt));
     const int64_t groups = rows < most ? rows : most;
@@ -1103,8 +1103,9 @@ int forward_typed(const NormArgs &p, int sm_count, cudaStream_t stream) {
                      (p.gate_mode == kGateToken ||
                       aligned_rows(p.gate, p.gate_mode == kGateFull ? p.rows : 1, side(p.gate), 16));
     // one chunk a thread for few rows, whose latency counts, and for unaligned ones, whose single elements leave little in
-    // flight otherwise
-    const Shape s = shape_of(p.rows, p.cols, int64_t(1) << 30, p.rows < sm_count || !vec);
+    // flight otherwise: up to 4096 columns, 8192 of 16 bits (16001 x 4097 bf16 on an f32 stream, to 8 bits, 632 us with two,
+    // 493 with one; 4000 x 8191 f32 137 and 163)
+    const Shape s = shape_of(p.rows, p.cols, int64_t(1) << 30, p.rows < sm_count ? 16 : vec ? 0 : sizeof(TX) == 2 ? 32 : 16);
     if (vec && p.x.p != nullptr && p.r_out.p != nullptr && p.cols % 8 == 0 && p.cols > 2 * kChunk && p.rows >= 2 * sm_count)
         switch (p.post.p != nullptr && p.pre.p != nullptr ? whole(p.gate_mode) : Parts::kSome) {
         case Parts::kSome: return forward_rows<TX, TR, Parts::kSome>(p, sm_count, stream);
@@ -1201,7 +1202,7 @@ int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) 
         }
         return finish_sums<TX>(todo, sums, planes.count, groups, p.cols, stream);
     }
-    const Shape s = shape_of(p.rows, p.cols, backward_groups(p.rows, p.cols), false);
+    const Shape s = shape_of(p.rows, p.cols, backward_groups(p.rows, p.cols), 0);
     const int64_t groups = s.warps == 1 ? static_cast<int64_t>(s.ctas) * kRowsPerCta : s.ctas;
     auto keep = [&](int &plane, float *to) {
         if (to == nullptr) return;
