@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(VPT == 1 && !AHEAD ? 2 * kMaxThreads : kMaxThr
 // does not depend on registers or on where the row before stands between its
 // two sums; the weights stay in registers over the rows, folded into one
 // factor per element and norm.  Bound by DRAM, less what a row's two sums
-// keep waiting: 16384 x 4096 bf16 to 8-bit blocks in 80.2 us, 72.0 at the
-// copy rate.
+// keep waiting: 16384 x 4096 bf16 to 8-bit blocks in 80 to 84 us, 72.0 at
+// the copy rate.
 constexpr int kMaxStages = 8;
 
 struct RowRing {
@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
 // over rows S = sum dr * X * g serves dpost = alpha * gate * S and a channel's
 // dgate = alpha * (post + offset) * S, and one over the row, sum dr * X * c1
 // (times an element's g), the mean in dx and a token's dgate.  Bound by DRAM
-// and by issue slots (8192 x 4096 bf16 with its column sums in 72.0 us, 61.5
+// and by issue slots (8192 x 4096 bf16 with its column sums in 72 to 76 us, 61.5
 // at the copy rate; 64 registers a thread and twice the warps spilled: 113
 // against 95 then).
 constexpr int kBackVecs = 2;
