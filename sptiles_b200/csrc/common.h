@@ -281,6 +281,7 @@ enum : int { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateFull = 3 };
 struct NormArgs {
     int64_t rows, cols;
     float alpha, eps, offset;
+    int branch, stream;  // types of x, h and their gradients, and of the residual stream, as the caller has checked them
     NormView x, r, r_out, h;
     NormView post, pre, gate;  // post, pre and a channel gate: one row; a token gate: ld per row
     int gate_mode = kGateNone;
@@ -295,6 +296,7 @@ int launch_residual_norm(const NormArgs &args, int sm_count, int *dev_err, uint6
 struct NormBackwardArgs {
     int64_t rows, cols;
     float alpha, eps, offset;
+    int branch, stream;  // as in NormArgs
     NormView d_residual, d_normed;  // p null: absent
     NormView x, r;                  // the branch and the updated stream
     NormView post, pre, gate;

@@ -1226,10 +1226,9 @@ int launch_residual_norm(const NormArgs &args, int sm_count, int *dev_err, uint6
     p.limit_ns = timeout_ns;
     if (p.rows == 0) return ST_OK;
     if (p.cols > kMaxCols) return fail(ST_ERR_UNSUPPORTED, "residual_norm: at most 16384 columns");
-    const int tx = p.x.p != nullptr ? p.x.dtype : (p.h.p != nullptr && !p.h_fp8 ? p.h.dtype : p.r.dtype);
-    const bool wide = p.r.dtype == ST_F32;
-    if (tx == ST_F32) return forward_typed<float, float>(p, sm_count, stream);
-    if (tx == ST_F16)
+    const bool wide = p.stream == ST_F32;
+    if (p.branch == ST_F32) return forward_typed<float, float>(p, sm_count, stream);
+    if (p.branch == ST_F16)
         return wide ? forward_typed<__half, float>(p, sm_count, stream) : forward_typed<__half, __half>(p, sm_count, stream);
     return wide ? forward_typed<__nv_bfloat16, float>(p, sm_count, stream)
                 : forward_typed<__nv_bfloat16, __nv_bfloat16>(p, sm_count, stream);
@@ -1254,10 +1253,9 @@ int launch_residual_norm_backward(const NormBackwardArgs &args, void *workspace,
             if (out != nullptr) ST_CUDA_TRY(cudaMemsetAsync(out, 0, p.cols * sizeof(float), stream));
         return ST_OK;
     }
-    const int tx = p.x.p != nullptr ? p.x.dtype : (p.d_normed.p != nullptr ? p.d_normed.dtype : p.r.dtype);
-    const bool wide = (p.r.p != nullptr ? p.r.dtype : p.d_residual.dtype) == ST_F32;
-    if (tx == ST_F32) return backward_typed<float, float>(p, sums, stream);
-    if (tx == ST_F16)
+    const bool wide = p.stream == ST_F32;
+    if (p.branch == ST_F32) return backward_typed<float, float>(p, sums, stream);
+    if (p.branch == ST_F16)
         return wide ? backward_typed<__half, float>(p, sums, stream) : backward_typed<__half, __half>(p, sums, stream);
     return wide ? backward_typed<__nv_bfloat16, float>(p, sums, stream)
                 : backward_typed<__nv_bfloat16, __nv_bfloat16>(p, sums, stream);

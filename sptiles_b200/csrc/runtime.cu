@@ -1647,6 +1647,8 @@ int st_residual_norm(st_ctx *ctx, const st_tensor *x_in, const st_tensor *residu
     g.h_e5m2 = normed && normed->dtype == ST_E5M2;
     const int t = x_in ? x_in->dtype : (normed && !g.h_fp8 ? normed->dtype : residual->dtype);
     ST_TRY(check_norm_types("residual_norm", t, residual->dtype));
+    g.branch = t;
+    g.stream = residual->dtype;
     if (residual_out && residual_out->dtype != residual->dtype)
         return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm: residual and residual_out must have the same dtype");
     if (normed && !g.h_fp8 && normed->dtype != t)
@@ -1714,6 +1716,8 @@ int st_residual_norm_backward(st_ctx *ctx, const st_tensor *d_residual, const st
     const int t = x_in ? x_in->dtype : (d_normed ? d_normed->dtype : d_residual->dtype);
     const int s = residual && pre ? residual->dtype : (d_residual ? d_residual->dtype : t);
     ST_TRY(check_norm_types(what, t, s));
+    g.branch = t;
+    g.stream = s;
     if ((d_residual && d_residual->dtype != s) || (dr && dr->dtype != s) || (d_normed && d_normed->dtype != t) ||
         (dx && dx->dtype != t))
         return fail(ST_ERR_INVALID_ARGUMENT, "residual_norm_backward: a gradient must have the dtype of its tensor");

@@ -447,3 +447,36 @@ def test_outputs_left_out_in_c(rows):
     for got, ref, dtype in [(normed, want.normed, BF16), (dx, back.x, BF16), (dgate, back.gate, F32)]:
         mass = ref.double().abs().cpu() + ref.double().abs().max().cpu()
         close(got, ref.double().cpu(), mass, dtype, rel=REL + torch.finfo(dtype).eps / 2)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(7, 96), (5, 301), (700, 1024), (3, 12001)], ids=lambda v: str(v))
+def test_backward_of_the_stream_alone(rows, cols, dtype):
+    """d_residual and nothing else: the stream's gradient as it is, read and written in its own type.  d_residual is a
+    row block among others, so that a read in a wider type would bring in its neighbours; the updated stream, given or
+    not, does not matter without pre_weight."""
+    room = torch.randn(3 * rows, cols, generator=gen(rows)).to(dtype).to(DEV)
+    d = room[rows:2 * rows]
+    for residual in (None, torch.zeros(rows, cols, dtype=dtype, device=DEV)):
+        got = st.residual_norm_backward(d, None, None, residual)
+        assert got.residual.dtype == dtype and torch.equal(got.residual, d)
+        assert got.x is None and got.post_weight is None and got.gate is None and got.pre_weight is None
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [5, 700])
+def test_backward_of_the_stream_alone_writes_dr_only(rows, dtype):
+    """The same call in C with dr inside a larger array: nothing around it is written."""
+    from sptiles_b200.api import _exec_desc
+    from sptiles_b200.fp8 import _cp, _desc, _fn, _u64, _vp
+    from sptiles_b200.norm import _OPTIONS
+
+    cols = 1024
+    d = torch.randn(rows, cols, generator=gen(2)).to(dtype).to(DEV)
+    room = torch.full((3 * rows, cols), 3.0, dtype=dtype, device=DEV)
+    dr = room[rows:2 * rows]
+    backward = _fn("st_residual_norm_backward", _vp, *[_cp] * 12, _vp, _u64, _cp, _cp)
+    assert backward(st.runtime.context(0), _desc(d), *[None] * 7, _desc(dr), None, None, None, None, 0,
+                    _OPTIONS.pack(1.0, EPS, 0.0), _exec_desc(0)) == 0
+    assert torch.equal(dr, d)
+    assert (room[:rows] == 3.0).all() and (room[2 * rows:] == 3.0).all()
