@@ -58,7 +58,7 @@ struct Fp8Params {
     int c_dtype;
     const void *bias;
     int bias_dtype;
-    int bias_on_rows;
+    int bias_on_rows;  // B is the row operand: C's rows, contiguous, run along the tile's columns
     int staged;  // CTA pairs: C leaves by TMA stores
     uint32_t idesc;
     int *err;
@@ -418,7 +418,7 @@ template <typename T, int THREADS>
 __device__ __forceinline__ void store_sums(const Fp8Params &p, const float4 *sums, int first, int own, int own_shift,
                                            int parts, int r0, int col0) {
     const int quads = own / 4, pitch = own / 4 + 1;
-    const bool by_rows = p.c_c == 1;
+    const bool by_rows = !p.bias_on_rows;  // not c_c == 1: a C of one row may have unit strides both ways
     const int quad0 = by_rows ? first & (quads - 1) : first >> 7, r_first = by_rows ? first >> (own_shift - 2) : first & 127;
     const int dr = by_rows ? 4 * THREADS / own : 0, dq = by_rows ? 0 : THREADS / 128;
     T *c = static_cast<T *>(p.c) + (r0 + r_first) * p.c_r + (col0 + 4 * quad0) * p.c_c;

@@ -264,6 +264,28 @@ def test_matmul_output_view_and_edges():
         assert (room == 3.0).all()
 
 
+@pytest.mark.parametrize("n,k", [(20000, 130), (12000, 4200), (8000, 2100), (300, 4096)], ids=lambda v: str(v))
+def test_matmul_one_row_as_a_column(n, k):
+    """C [1, N] with unit strides both ways (a column's transpose), with a bias: the weights' rows in one, two, four and
+    eight parts."""
+    a, b, sa, sb = make(1, n, k)
+    bias = torch.randn(n, generator=gen(9))
+    room = torch.full((n + 2, 1), 3.0, device=DEV)
+    out = room[1:n + 1].t()
+    assert out.stride() == (1, 1)
+    st.matmul_fp8(put(a), put(b).t(), sa.to(DEV), sb.t().to(DEV), bias.to(DEV), out=out)
+    check_product(out, a, b, sa, sb, bias, torch.float32)
+    assert room[0] == 3.0 and room[-1] == 3.0
+
+
+@pytest.mark.parametrize("m", [1, 40, 64])
+def test_matmul_one_column(m):
+    a, b, sa, sb = make(m, 1, 2000)
+    bias = torch.randn(1, generator=gen(9))
+    C = st.matmul_fp8(put(a), put(b).t(), sa.to(DEV), sb.t().to(DEV), bias.to(DEV), out_dtype=torch.float32)
+    check_product(C, a, b, sa, sb, bias, torch.float32)
+
+
 def test_matmul_empty():
     z = torch.zeros
     A, B = z(4, 0, dtype=torch.uint8, device=DEV).view(E4), z(0, 6, dtype=torch.uint8, device=DEV).view(E4)
