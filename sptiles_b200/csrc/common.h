@@ -166,6 +166,9 @@ struct GemmArgs {
     bool c_preset = false;
     // fold split tiles in a fixed order (ST_EXEC_DETERMINISTIC)
     bool deterministic = false;
+    // the bytes from a row's end to the next 16-byte boundary are scratch of
+    // this call's: a TMA store of C may write them
+    bool c_padding = false;
     // ab_dtype ST_F32 with raw fp32 A [M, K] and B (K-major [N, K] or
     // N-contiguous [K, N]) and the true K: the CTA-pair kernel splits the
     // tiles into tf32 hi / lo itself (3xTF32); only when gemm_split_fp32_fits

@@ -2115,13 +2115,16 @@ int plan_gemm(int in_dtype, int64_t m, int64_t n, int64_t k, int sm_count, GemmP
 }
 
 // The TMA-store epilogue needs every C destination 16-byte aligned with a
-// row stride of a multiple of 16 bytes; other C views take the per-lane
-// direct stores.  Peer copies always go by TMA store (one asynchronous bulk
+// row stride of a multiple of 16 bytes, and rows that end on a 16-byte
+// boundary: a TMA store clips at whole 16-byte pieces, so what lies behind a
+// row's end in its last piece would be written too (with zeros).  Other C
+// views take the per-lane direct stores.  Peer copies always go by TMA store (one asynchronous bulk
 // store per box and destination instead of per-lane stores across NVLink);
 // a local C does unless SPTILES_B200_C_STORE=direct (or =tma) overrides it.
 bool c_store_staged(const GemmArgs &g) {
     const int ces = dtype_size(g.c_dtype);
     if ((g.ldc * ces) % 16 != 0) return false;
+    if ((g.n * ces) % 16 != 0 && !g.c_padding) return false;
     if (reinterpret_cast<uintptr_t>(g.c) % 16 != 0) return false;
     for (int d = 0; d < g.peers.n; ++d)
         if (reinterpret_cast<uintptr_t>(g.peers.base[d]) % 16 != 0) return false;

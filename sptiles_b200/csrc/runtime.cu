@@ -357,7 +357,7 @@ __global__ void fill_rows_kernel(void *c, int64_t ldc, int c_dtype, const void *
 }
 
 int matmul_device(const ExecCtx &x, const st_tensor &a, const st_tensor &b, const st_tensor *bias,
-                  const st_tensor &c, const PeerOutputs *peers = nullptr) {
+                  const st_tensor &c, const PeerOutputs *peers = nullptr, bool c_padding = false) {
     const int64_t M = a.shape[0], K = a.shape[1], N = b.shape[1];
     if (M == 0 || N == 0) return ST_OK;
     const void *bias_ptr = bias ? bias->data : nullptr;
@@ -373,6 +373,7 @@ int matmul_device(const ExecCtx &x, const st_tensor &a, const st_tensor &b, cons
     GemmArgs g{};
     if (peers) g.peers = *peers;
     g.deterministic = (x.flags & ST_EXEC_DETERMINISTIC) != 0;
+    g.c_padding = c_padding;
     g.c = c.data;
     g.ldc = c.strides[0];
     g.c_dtype = c.dtype;
@@ -676,7 +677,8 @@ int matmul_host_pipelined(const ExecCtx &x, const st_tensor &a, const st_tensor 
             vbias.shape[0] = c1 - c0;
             vbias.strides[0] = 1;
         }
-        return matmul_device(x, va, vb, bias ? &vbias : nullptr, vc);
+        // the last column block ends in the device copy's own padding, the others on 256 columns
+        return matmul_device(x, va, vb, bias ? &vbias : nullptr, vc, nullptr, true);
     };
     for (int64_t st = 0; st < steps; ++st) {
         const int64_t r0 = std::min(M, st * rows), r1 = std::min(M, (st + 1) * rows);

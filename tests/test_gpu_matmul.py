@@ -249,6 +249,27 @@ def test_operand_layouts(dtype):
     assert torch.all(out[:, n:] == 5.0)
 
 
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.float32, torch.float32), (torch.float16, torch.float32),
+                                             (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16)],
+                         ids=["f32", "f16_f32", "f16", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(130, 70, 64), (100, 33, 128), (1000, 513, 512), (2048, 1801, 512), (3000, 2501, 256)],
+                         ids=str)
+def test_output_rows_that_end_inside_16_bytes(m, n, k, dtype, out_dtype):
+    """C a view whose rows start on 16-byte boundaries and end inside a 16-byte piece: what lies behind each row stays,
+    also beside a row of NaN (0 * NaN is not added there either)."""
+    A, B = normal((m, k), 1.0, m, dtype), normal((k, n), 1.0, n, dtype)
+    A[m // 2] = float("nan")
+    per = 16 // torch.empty(0, dtype=out_dtype).element_size()
+    room = torch.full((m + 1, -(-n // per) * per), 3.0, dtype=out_dtype, device=DEV)
+    st.matmul(A, B, out=room[:m, :n])
+    rows = [r for r in range(m) if r != m // 2]
+    want = oracle_mm(A, B, rows=(0, 8))
+    tol = TOL[dtype] + torch.finfo(out_dtype).eps / 2 * (out_dtype != torch.float32)  # C's own rounding
+    assert rel_err(room[:8, :n].float().cpu().numpy(), want) <= tol
+    assert torch.isfinite(room[rows, :n]).all() and torch.isnan(room[m // 2, :n]).all()
+    assert torch.all(room[:, n:] == 3.0) and torch.all(room[m] == 3.0)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_output_dtypes_and_bias(dtype, out_dtype):
