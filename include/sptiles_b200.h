@@ -170,7 +170,9 @@ int st_grid_from_dispatch(const char *entry_name, const uint32_t dispatch[3], in
 /* ---- failure path check.  Runs one warp that waits, with the helpers the
  * GEMM kernels' bounded waits use, on something that never completes: an
  * mbarrier nothing arrives on (kind 0) or a GPU-scope flag nothing sets
- * (kind 1).  After limit_us (1 .. 10^7) it gives up, records its abort code
+ * (kind 1); or the norms' ring of rows with a row that never comes (kind 16),
+ * or a scaling warp of the 8-bit product whose scales never come, by rows
+ * (kind 17) or by columns (kind 18).  After limit_us (1 .. 10^7) it gives up, records its abort code
  * in the device's error word and returns; the next bounded host wait
  * (ST_EXEC_SYNC here, or st_sync) reports ST_ERR_DEVICE_ABORT and clears the
  * word, and the context stays usable.  Nothing faults or hangs.  No

@@ -95,6 +95,10 @@ constexpr int kDevAbortWaitCheckFlag = 0x1f1;     // st_check_device_wait: flag 
 // (kind 0) or a flag nothing sets (kind 1), then records its abort code in
 // dev_err and returns (diag.cu).
 int launch_wait_check(int kind, uint64_t limit_ns, int *dev_err, cudaStream_t stream);
+// The same for the norms' ring of rows (norm.cu) and a scaling warp of the
+// 8-bit product, by rows or by columns (gemm_fp8.cu), with their own codes.
+int launch_norm_wait_check(uint64_t limit_ns, int *dev_err, cudaStream_t stream);
+int launch_fp8_wait_check(bool by_column, uint64_t limit_ns, int *dev_err, cudaStream_t stream);
 
 // ---- launchers (implemented in vecadd.cu, gemm.cu, pack.cu) ----
 

@@ -245,7 +245,10 @@ __device__ __forceinline__ bool scale_blocks(float (&acc)[COLS], int n, uint32_t
     tmem_load<STEP>(t + static_cast<uint32_t>(at.a * STRIDE), v[0]);
     for (int b = 0; b < n; ++b) {
         const int k = b % kBatch;
-        if (k == 0 && !arrived(ring.full(at.d), at.dph)) return false;
+        if (k == 0 && !arrived(ring.full(at.d), at.dph)) {
+            tmem_loaded<STEP>(v[0]);  // the load under way lands before its registers serve anything else
+            return false;
+        }
         const float *cols = ring.cols(at.d, k) + col;
         const float r_scale = ring.rows(at.d, k)[row];
         const float both = CVEC ? r_scale : r_scale * cols[0];
@@ -333,7 +336,10 @@ __device__ __forceinline__ bool scale_blocks_by_column(float (&acc)[COLS], int n
     ask(t + static_cast<uint32_t>(at.a * STRIDE), v[0]);
     for (int b = 0; b < n; ++b) {
         const int k = b % kBatch;
-        if (k == 0 && !arrived(ring.full(at.d), at.dph)) return false;
+        if (k == 0 && !arrived(ring.full(at.d), at.dph)) {
+            tmem_loaded<32>(v[0]);  // as in scale_blocks
+            return false;
+        }
         const float2 *cols = reinterpret_cast<const float2 *>(ring.cols(at.d, k) + col) + (lane & 3);
         const float *rows = ring.rows(at.d, k) + row0 + (lane >> 2);
         uint64_t r[4];
@@ -382,6 +388,61 @@ __device__ __forceinline__ bool scale_blocks_by_column(float (&acc)[COLS], int n
         }
     }
     return true;
+}
+
+// One scaling warp on its way out (st_check_device_wait): its accumulator is
+// there, so its first columns are being read, and the block's scales never
+// come.  It waits for the read, frees its TMEM and returns.
+__device__ float g_checked_sum;  // so that what is read has a use
+
+template <bool BY_COLUMN>
+__global__ void __launch_bounds__(32) fp8_wait_check_kernel(uint64_t limit_ns, int *err) {
+    constexpr int kCols = BY_COLUMN ? 128 : 16;
+    using Ring = ScaleRing<kTileRows, kCols, true, 2>;
+    __shared__ __align__(16) float slots[Ring::kBytes / 4];
+    __shared__ __align__(8) uint64_t bars[1 + Ring::kBars];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    const int lane = static_cast<int>(threadIdx.x);
+    const uint32_t accumulated = smem_addr(bars);
+    const Ring ring{slots, accumulated + 8u};
+    if (lane == 0) {
+        mbar_init(accumulated, 1);
+        ring.init(1);
+        abort_flag = 0;
+        fence_barrier_init();
+        mbar_arrive(accumulated);
+    }
+    __syncwarp();
+    tmem_alloc(smem_addr(&tmem_slot), 128);
+    tmem_relinquish();
+    __syncwarp();
+    const uint32_t t = *static_cast<volatile uint32_t *>(&tmem_slot);
+    float acc[kCols];
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) {
+        acc[j] = 0.0f;
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(t + static_cast<uint32_t>(j)), "r"(0) : "memory");
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    ScalePosition at;
+    auto full = [&](int) { return accumulated; };
+    auto released = [](int) {};
+    bool ok;
+    if constexpr (BY_COLUMN)
+        ok = scale_blocks_by_column<kCols, 1, kCols>(acc, 1, t, 0, 0, ring, at, full, released, lane, &abort_flag, limit_ns);
+    else
+        ok = scale_blocks<kCols, 8, true, 1, kCols>(acc, 1, t, lane, 0, ring, at, full, released, lane, &abort_flag, limit_ns);
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) sum += acc[j];
+    if (ok) g_checked_sum = sum;
+    if (!ok && lane == 0) {
+        abort_flag = 1;
+        atomicExch(err, kDevAbortGemmEpilogue);
+    }
+    __syncwarp();
+    tmem_dealloc(t, 128);
 }
 
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
@@ -1294,6 +1355,14 @@ int launch_repack_8(const Fp8Operand &o, const Access &a, uint8_t *dst, int sm_c
 }
 
 }  // namespace
+
+int launch_fp8_wait_check(bool by_column, uint64_t limit_ns, int *dev_err, cudaStream_t stream) {
+    if (by_column) fp8_wait_check_kernel<true><<<1, 32, 0, stream>>>(limit_ns, dev_err);
+    else fp8_wait_check_kernel<false><<<1, 32, 0, stream>>>(limit_ns, dev_err);
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "fp8_wait_check_kernel launch");
+}
 
 int64_t gemm_fp8_workspace_bytes(const Fp8Operand &a, const Fp8Operand &b) {
     if (a.rows == 0 || b.rows == 0 || a.k == 0) return 0;

@@ -343,6 +343,27 @@ struct RowRing {
     }
 };
 
+// A ring whose first row comes and whose second never does (st_check_device_wait).
+__device__ float4 g_checked_row[8];
+
+__global__ void __launch_bounds__(64) norm_wait_check_kernel(uint64_t limit_ns, int *err) {
+    __shared__ __align__(128) uint8_t rows[2 * sizeof(g_checked_row)];
+    __shared__ uint64_t bars[2];
+    __shared__ int aborted;
+    constexpr uint32_t kBytes = sizeof(g_checked_row);
+    const RowRing ring{smem_addr(bars), rows, 2, static_cast<int>(kBytes), &aborted, err, limit_ns};
+    ring.init();
+    if (threadIdx.x == 0) {
+        ring.expect(0, kBytes);
+        ring.copy(0, 0, g_checked_row, kBytes);
+        ring.expect(1, kBytes);
+    }
+    ring.wait(0, 0);
+    ring.wait(1, 0);
+    __syncthreads();
+    if (threadIdx.x == 0) ring.drain();
+}
+
 template <typename T>
 __device__ __forceinline__ void read8(const uint8_t *row, int col, uint64_t (&f)[4]) {
     uint4 w[sizeof(T) / 2];
@@ -1219,6 +1240,13 @@ int backward_typed(const NormBackwardArgs &p, float *sums, cudaStream_t stream) 
 }
 
 }  // namespace
+
+int launch_norm_wait_check(uint64_t limit_ns, int *dev_err, cudaStream_t stream) {
+    norm_wait_check_kernel<<<1, 64, 0, stream>>>(limit_ns, dev_err);
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "norm_wait_check_kernel launch");
+}
 
 int launch_residual_norm(const NormArgs &args, int sm_count, int *dev_err, uint64_t timeout_ns, cudaStream_t stream) {
     NormArgs p = args;

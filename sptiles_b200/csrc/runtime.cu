@@ -1755,14 +1755,18 @@ int st_residual_norm_backward(st_ctx *ctx, const st_tensor *d_residual, const st
 }
 
 int st_check_device_wait(st_ctx *ctx, int32_t kind, uint32_t limit_us, const st_exec *exec) {
-    if (kind != 0 && kind != 1)
-        return fail(ST_ERR_INVALID_ARGUMENT, "st_check_device_wait: kind must be 0 (mbarrier) or 1 (flag)");
+    if (kind != 0 && kind != 1 && (kind < 16 || kind > 18))
+        return fail(ST_ERR_INVALID_ARGUMENT, "st_check_device_wait: kind must be 0 (mbarrier), 1 (flag), 16 (row ring of the "
+                                             "norms), 17 or 18 (scaling warp of the 8-bit product, by rows or by columns)");
     if (limit_us == 0 || limit_us > 10u * 1000 * 1000)
         return fail(ST_ERR_INVALID_ARGUMENT, "st_check_device_wait: limit_us must be in [1, 10^7]");
     ExecCtx x;
     ST_TRY(resolve_exec(ctx, exec, &x));
     DeviceGuard guard(x.dev->ordinal);
-    ST_TRY(launch_wait_check(kind, static_cast<uint64_t>(limit_us) * 1000, x.dev->dev_err, x.stream));
+    const uint64_t limit_ns = static_cast<uint64_t>(limit_us) * 1000;
+    if (kind < 16) ST_TRY(launch_wait_check(kind, limit_ns, x.dev->dev_err, x.stream));
+    else if (kind == 16) ST_TRY(launch_norm_wait_check(limit_ns, x.dev->dev_err, x.stream));
+    else ST_TRY(launch_fp8_wait_check(kind == 18, limit_ns, x.dev->dev_err, x.stream));
     return finish(x);
 }
 
