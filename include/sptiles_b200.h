@@ -265,6 +265,11 @@ int st_quantize_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *q, const s
  *   a_scale               f32 [M, ceil(K/128)] or, one scale for 128 rows, [ceil(M/128), ceil(K/128)]
  *   b_scale               f32 [ceil(K/128), N] or [ceil(K/128), ceil(N/128)]
  *   C                     f32, f16 or bf16, unit column stride;  bias: f32 or C's dtype
+ * A block's sum is multiplied by a_scale * b_scale, itself rounded to fp32:
+ * that product has to lie in fp32's normal range, 2^-126 <= |a_scale *
+ * b_scale| < 2^128, or be 0.  Below it loses bits (a block of zeros, whose
+ * sum is 0, still gives 0, whatever its scale), above it is infinite (and
+ * NaN where the block's sum is 0).
  * The sum over blocks is kept in fp32.  Gradients are calls of the same kind:
  * with dY in blocks of 1 x 128, dX = dY @ W reads W [N, K] as it is stored;
  * with dY and X in blocks of 128 x 1 (tokens), dW = dY^T @ X reads both as

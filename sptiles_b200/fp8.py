@@ -146,7 +146,9 @@ def matmul_fp8(A: torch.Tensor, B: torch.Tensor, a_scale: torch.Tensor, b_scale:
     are read in place; anything else is copied first).  a_scale: float32
     [M, ceil(K/128)], or [ceil(M/128), ceil(K/128)] with one scale for 128
     rows; b_scale: float32 [ceil(K/128), N] or [ceil(K/128), ceil(N/128)];
-    any strides.  Products are summed in fp32, block by block.  C is
+    any strides.  Products are summed in fp32, block by block, and a block's
+    sum is multiplied by a_scale * b_scale in fp32: keep that product within
+    2^-126 and 2^128 (a block of zeros gives 0 whatever its scale).  C is
     bfloat16, float16 or float32; bias (length N) is float32 or C's dtype.
     The same inputs give the same bits.
     """

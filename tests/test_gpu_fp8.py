@@ -310,6 +310,33 @@ def test_matmul_nan_stays_in_its_row_and_column():
     assert not bad.any()
 
 
+@pytest.mark.parametrize("b_square", [True, False], ids=["b128", "b1"])
+@pytest.mark.parametrize("m,n", [(3, 300), (150, 200), (2048, 1800)], ids=str)
+def test_matmul_scales_at_the_ends_of_their_range(m, n, b_square):
+    """Products of two scales down to 2^-126 and up to 2^90, from factors far apart and near each other: as exact as
+    any.  (300 products of codes up to 448 sum to less than 2^26, so 2^90 times that stays finite.)"""
+    k = 300
+    for ea, eb in [(-63, -63), (-126, 0), (0, -126), (-126, 60), (100, -126), (45, 45), (90, 0)]:
+        a, b, sa, sb = make(m, n, k, b_square=b_square)
+        sa, sb = torch.full_like(sa, 2.0 ** ea), torch.full_like(sb, 2.0 ** eb)
+        C = st.matmul_fp8(put(a), put(b).t(), sa.to(DEV), sb.t().to(DEV), out_dtype=torch.float32)
+        check_product(C, a, b, sa, sb, None, torch.float32)
+
+
+@pytest.mark.parametrize("b_square", [True, False], ids=["b128", "b1"])
+@pytest.mark.parametrize("m,n", [(3, 300), (150, 200), (2048, 1800)], ids=str)
+def test_matmul_blocks_of_zeros(m, n, b_square):
+    """Tokens and weights of zeros carry the least scale, 2^-126: their products with any other are 0."""
+    x, w = torch.randn(m, 300, generator=gen(1)), torch.randn(n, 300, generator=gen(2)) * 1e-3
+    x[m // 2], x[0, :128], w[:128] = 0, 0, 0
+    xq, xs = st.quantize_fp8(x.to(DEV))
+    wq, ws = st.quantize_fp8(w.to(DEV), block=(128, 128) if b_square else (1, 128))
+    assert xs[m // 2, 0] == 2.0 ** -126 and ws[0, 0] == 2.0 ** -126
+    C = st.matmul_fp8(xq, wq.t(), xs, ws.t(), out_dtype=torch.float32)
+    assert (C[m // 2] == 0).all() and (C[:, :128] == 0).all()
+    check_product(C, xq.cpu(), wq.cpu(), xs.cpu(), ws.cpu(), None, torch.float32)
+
+
 def test_matmul_same_bits_streams_and_graph():
     a, b, sa, sb = make(24, 1000, 4000)
     A, B, SA, SB = put(a, aligned=False), put(b).t(), sa.to(DEV), sb.t().to(DEV)
