@@ -480,3 +480,92 @@ def test_backward_of_the_stream_alone_writes_dr_only(rows, dtype):
                     _OPTIONS.pack(1.0, EPS, 0.0), _exec_desc(0)) == 0
     assert torch.equal(dr, d)
     assert (room[:rows] == 3.0).all() and (room[2 * rows:] == 3.0).all()
+
+
+# ------------------------------------------------------------------ weights and gates of another type than x
+def float32_sides(d, names):
+    return {k: v.float() if k in names and v is not None else v for k, v in d.items()}
+
+
+@pytest.mark.parametrize("names", [("gate",), ("post",), ("gate", "post", "pre")], ids="+".join)
+@pytest.mark.parametrize("gate", ["none", "channel", "row", "token", "full"])
+@pytest.mark.parametrize("tx,tr", [(F16, F16), (BF16, BF16), (BF16, F32)], ids=["f16", "bf16", "bf16_f32"])
+@pytest.mark.parametrize("rows,cols", [(5, 96), (4, 1101), (700, 1024), (333, 2056), (300, 4104)], ids=lambda v: str(v))
+def test_float32_gate_and_weights_beside_16_bits(rows, cols, tx, tr, gate, names):
+    """float32 gates and weights beside a 16-bit x, forward to both kinds of copies and backward, on the generic
+    kernels and on the rings; a gate's gradient comes in the gate's type."""
+    d = inputs(rows, cols, tx, tr, gate, True, True, seed=6)
+    g = gen(7)
+    d = float32_sides(d, names)
+    for k in names:  # values that 16 bits do not hold
+        if d[k] is not None:
+            d[k] = d[k] + 1e-4 * torch.randn(d[k].shape, generator=g)
+    check_forward(d)
+    check_forward(d, quantize=True, offset=0.5)
+    full = gate == "full" and d["gate"].dtype == F32
+    if not full:
+        check_backward(d, rows, cols, tx, tr, offset=0.5)
+        return
+    dr, dh = torch.randn(rows, cols, generator=g).to(tr), torch.randn(rows, cols, generator=g).to(tx)
+    c = dev(d)
+    got = st.residual_norm_backward(dr.to(DEV), dh.to(DEV), c["x"], c["r"], c["post"], c["gate"], c["pre"], alpha=0.7, eps=EPS)
+    want, mass = backward64(dbl(d), dr.double(), dh.double(), 0.7, 0.0)
+    close(got.gate, want["gate"], mass["gate"], F32)
+    close(got.x, want["x"], mass["x"], tx)
+    close(got.residual, want["residual"], mass["residual"], tr)
+    for value, name in ((got.post_weight, "post"), (got.pre_weight, "pre")):
+        close(value, want[name], mass[name], F32, rel=REL + (rows + 64) * 2.0 ** -24)
+
+
+# ------------------------------------------------------------------ NaN and infinities through the rings
+BAD_ROWS = {5: float("nan"), 297: float("inf"), 640: float("-inf")}
+
+
+def test_forward_ring_keeps_bad_rows_apart():
+    """Rows of NaN and infinity among rows that the same CTAs take before and after them: every other row has the bits
+    that it has without them, its 8-bit codes and scales too."""
+    for gate in ("none", "channel", "token", "full"):
+        d = inputs(900, 1024, BF16, F32, gate, True, True, seed=5)
+        for quantize in (False, True):
+            run = lambda v: st.residual_norm(v["x"], v["r"], v["post"], v["gate"], v["pre"], eps=EPS, quantize=quantize)  # noqa: E731
+            want = run(dev(d))
+            bad = dict(d, x=d["x"].clone(), r=d["r"].clone())
+            for i, (row, v) in enumerate(BAD_ROWS.items()):
+                bad["x" if i % 2 == 0 else "r"][row, 100 * i + 7] = v
+            got = run(dev(bad))
+            fine = torch.ones(900, dtype=torch.bool)
+            fine[list(BAD_ROWS)] = False
+            for a, b in zip(got, want):
+                if a is None:
+                    continue
+                a, b = (v.cpu().view(torch.uint8) if v.element_size() == 1 else v.cpu() for v in (a, b))
+                assert torch.equal(a[fine], b[fine])
+            assert torch.isnan(got.residual[5]).all()  # x's NaN is in its row's norm
+            assert not torch.isfinite(got.residual[297, 107]) and not torch.isfinite(got.residual[640, 207])
+            if quantize:  # what reads the blocks' codes and scales gets NaN where the row is bad
+                assert torch.isnan(got.scale[5]).all()
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+def test_backward_ring_keeps_bad_rows_apart(gate):
+    """The same backward: dx, dr and a row's own gate gradient of every other row keep their bits; sums over rows
+    are not finite in the columns that a bad row reaches."""
+    rows, cols = 900, 1024
+    d = inputs(rows, cols, BF16, F32, gate, True, True, seed=5)
+    dr, dh = torch.randn(rows, cols, generator=gen(1)), torch.randn(rows, cols, generator=gen(2)).to(BF16)
+    run = lambda v, p, q: st.residual_norm_backward(p.to(DEV), q.to(DEV), v["x"], v["r"], v["post"], v["gate"], v["pre"],  # noqa: E731
+                                                    eps=EPS)
+    want = run(dev(d), dr, dh)
+    x, p, q = d["x"].clone(), dr.clone(), dh.clone()
+    x[5, 7], p[297, 107], q[640, 207] = float("nan"), float("inf"), float("nan")
+    got = run(dev(dict(d, x=x)), p, q)
+    fine = torch.ones(rows, dtype=torch.bool)
+    fine[list(BAD_ROWS)] = False
+    own = [(got.x, want.x), (got.residual, want.residual)] + ([(got.gate, want.gate)] if gate in ("token", "full") else [])
+    for a, b in own:
+        assert torch.equal(a.cpu()[fine], b.cpu()[fine])
+    assert torch.isnan(got.x[5]).all() and torch.isfinite(got.residual[5]).all()
+    assert torch.isinf(got.residual[297, 107]) and torch.isnan(got.residual[640]).all()
+    assert torch.isnan(got.post_weight).all() and torch.isnan(got.pre_weight[207])
+    if gate == "channel":
+        assert torch.isnan(got.gate).all()
