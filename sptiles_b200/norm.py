@@ -83,6 +83,8 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, post_weight: t
     shape = residual.shape
     if len(shape) != 2:
         raise ValueError("residual must be a 2D tensor.")
+    if residual.dtype not in _ALL_CODES:
+        raise ValueError(f"unsupported dtype {residual.dtype}")
     dev = _device_of(residual, x, post_weight, gate, pre_weight, out)
     rows, cols = shape
     d_out = d_normed = d_scale = normed = scale = None

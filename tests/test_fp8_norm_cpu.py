@@ -200,6 +200,14 @@ def test_python_refusals():
         st.residual_norm_backward(None, None, x, None)
 
 
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int32, torch.bool])
+def test_python_refuses_a_residual_of_another_type(dtype):
+    r = torch.zeros(4, 128, dtype=dtype)
+    for x in (None, torch.zeros(4, 128), r):
+        with pytest.raises(ValueError, match="unsupported dtype"):
+            st.residual_norm(x, r, pre_weight=torch.ones(128))
+
+
 def test_older_calls_still_refuse_8_bit_types():
     from sptiles_b200 import api
 
