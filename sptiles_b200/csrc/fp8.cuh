@@ -18,8 +18,6 @@ __device__ __forceinline__ void from_float(float v, float &out) { out = v; }
 __device__ __forceinline__ void from_float(float v, __half &out) { out = __float2half_rn(v); }
 __device__ __forceinline__ void from_float(float v, __nv_bfloat16 &out) { out = __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
 // ---- pairs of fp32 in one register pair: the packed instructions halve the
 // issue slots of the row kernels, which were bound by them
 __device__ __forceinline__ uint64_t pack2(float a, float b) {

@@ -8,7 +8,8 @@
 // accumulator; the epilogue warps read each block's accumulator, multiply by
 // the block's two scales and add onto running sums in fp32 registers, while
 // the tensor core works on the next blocks in the other TMEM accumulators.
-// So the sum over blocks is a plain fp32 sum, whatever the scales are.
+// So the sum over blocks is a plain fp32 sum; the product of the two scales
+// is one too, and has to stay within fp32's normal range.
 //
 //   warp 0      TMA producer: one 128-byte-swizzled box of each operand per block
 //   warp 1      MMA issuer (owns the TMEM allocation)
@@ -17,15 +18,17 @@
 //   last warp   the blocks' scales, ahead of their use, into shared memory
 //
 // The kernel knows a row operand (128 rows a tile, the MMA's M) and a column
-// operand (BN columns, the MMA's N).  A call with few tokens makes the
-// weights the row operand and the tokens the columns, so that a tile reads
-// 128 rows of weights against 16 to 64 tokens and nothing is padded to 128
-// tokens.  When tiles alone would leave SMs idle, a cluster of up to 8 CTAs
+// operand (BN columns, the MMA's N).  With up to 64 tokens the weights may
+// become the row operand and the tokens the columns, so that a tile reads 128
+// rows of weights against 16 to 64 tokens and nothing is padded to 128
+// tokens; that is done where it is estimated to be faster (57 x 4109 x 4001
+// keeps its tokens as rows, 71 of a tile's 128 empty).  When tiles alone would leave SMs idle, a cluster of up to 8 CTAs
 // splits the blocks of one tile and adds its parts in a fixed order through
 // distributed shared memory.  Bound by the weights' bytes with few tokens:
-// 1 x 8192 x 8192 in 14.8 us (10.3 at the copy rate; about 5 us are launch,
+// 1 x 8192 x 8192 in 15.0 us (10.3 at the copy rate; about 5 us are launch,
 // the first load's latency, the cluster's exchange and the store, whatever
-// the size), 57 x 4109 x 4001 in 12.9, 1024^3 in 7.7.
+// the size), 57 x 4109 x 4001 in 14.1, 1024^3 in 10.8 a call and 7.2 in a
+// replayed graph.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -754,14 +757,14 @@ __global__ void __launch_bounds__(Fp8Cfg<BN, CVEC>::kThreads, BN == 128 ? 1 : 2)
 // operand, so a block of K costs an SM 32 KB of loads for 512 cycles of its
 // tensor core, half of what 128 x 128 tiles of one CTA take.  A block's
 // accumulator is 256 TMEM columns, two of them alternate.  (Two halves of 128
-// columns with four buffers would be handed over more finely, but an MMA of
-// 128 columns is bound by its operands' shared-memory reads: 369 cycles for
-// the 256 of its arithmetic.)  Eight scaling warps per CTA, two for each
+// columns with four buffers would be handed over more finely, but a block's
+// four MMAs of 128 columns take 369 cycles for the 256 of their arithmetic.)  Eight scaling warps per CTA, two for each
 // quarter of the lanes, hold 128 columns of running sums each in registers.
 // What bounds it is not the MMAs but reading their sums: 128 KB of TMEM a
 // block take eight warps 137 cycles alone and about 750 while the next
-// block's MMAs run, against the MMAs' 512.  8192^3 in 520 us (2116 TFLOP/s),
-// 4096 x 4096 x 16384 with a scale for each column in 448 (1226).
+// block's MMAs run, against the MMAs' 512; why they slow down is not known.
+// Calls back to back: 8192^3 in 605 us (1820 TFLOP/s), 4096 x 4096 x 16384
+// with a scale for each column in 462 (1190).
 //
 // full[s] lives in the even CTA and counts both CTAs' loads; the even CTA's
 // MMA warp commits empty[s] and tfull[a] to both CTAs; tempty[a] lives in
@@ -1103,7 +1106,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 }
 
 // Dense copy of a strided 8-bit [rows, cols] matrix, rows of `ld` bytes (a
-// multiple of 16; the padding is not written).  Unit column stride: 16 bytes
+// multiple of 16).  Whole 16-byte pieces are written, so the padding gets
+// bytes of no meaning; the tensor map ends at cols.  Unit column stride: 16 bytes
 // a thread, put together from the aligned words that hold them.
 __global__ void __launch_bounds__(256) repack_8_kernel(const uint8_t *__restrict__ src, int64_t s0, int64_t s1,
                                                        int64_t rows, int64_t cols, uint8_t *__restrict__ dst, int64_t ld) {

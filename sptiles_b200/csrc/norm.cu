@@ -216,7 +216,7 @@ __device__ __forceinline__ void store_normed(const NormArgs &p, int64_t row, int
 // AHEAD: all of a row's reads, the weights among them, are under way before
 // the first sum, for few rows (1 x 4096 in 3.6 us, latency alone); many rows
 // would rather have the registers (unaligned 1025 x 2049 with a full gate in
-// 11.8 us; inputs not in L2: 16.5, and 19.6 at 128 registers a thread).
+// 14.1 us a call; inputs not in L2: 16.5, and 19.6 at 128 registers a thread).
 template <typename TX, typename TR, int VPT, bool VEC, bool AHEAD>
 __global__ void __launch_bounds__(VPT == 1 && !AHEAD ? 2 * kMaxThreads : kMaxThreads) residual_norm_kernel(const NormArgs p, int warps) {
     pdl_wait();
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(VPT == 1 && !AHEAD ? 2 * kMaxThreads : kMaxThr
 // does not depend on registers or on where the row before stands between its
 // two sums; the weights stay in registers over the rows, folded into one
 // factor per element and norm.  Bound by DRAM, less what a row's two sums
-// keep waiting: 16384 x 4096 bf16 to 8-bit blocks in 80 to 84 us, 72.0 at
+// keep waiting: 16384 x 4096 bf16 to 8-bit blocks in 83 to 87 us, 72.0 at
 // the copy rate.
 constexpr int kMaxStages = 8;
 
@@ -413,7 +413,8 @@ __device__ __forceinline__ void cta_sum(float (&v)[N], int warps, int warp, int 
 // What a ring kernel's call has: every tensor, with no gate of a row's own or
 // with a token's or an element's, known to the compiler; any other set is
 // looked up in each row, which took the backward kernel a third of its issue
-// slots (8192 x 4096 bf16 94.6 us, 72.0 known; a token's gate 98.6 and 77.6).
+// slots (the kernel alone, 8192 x 4096 bf16 94.6 us, 72.0 known; a token's gate
+// 98.6 and 77.6).
 enum class Parts { kSome, kPlain, kToken, kFull };
 inline Parts whole(int gate_mode) {
     return gate_mode == kGateToken ? Parts::kToken : gate_mode == kGateFull ? Parts::kFull : Parts::kPlain;
@@ -771,7 +772,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
 // over rows S = sum dr * X * g serves dpost = alpha * gate * S and a channel's
 // dgate = alpha * (post + offset) * S, and one over the row, sum dr * X * c1
 // (times an element's g), the mean in dx and a token's dgate.  Bound by DRAM
-// and by issue slots (8192 x 4096 bf16 with its column sums in 72 to 76 us, 61.5
+// and by issue slots (8192 x 4096 bf16 with its column sums in 80 to 81 us, 61.5
 // at the copy rate; 64 registers a thread and twice the warps spilled: 113
 // against 95 then).
 constexpr int kBackVecs = 2;

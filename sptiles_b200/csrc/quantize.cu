@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const Quanti
 // rows, 16 threads of 8 columns across, 16 rows down.  The elements stay as
 // they were read and are unpacked twice: at 4 registers for 8 of 16 bits,
 // three such CTAs have 96 KB of an SM's reads under way (unpacked, two CTAs
-// of 512 threads took 64 us for 8192 x 8192; so 38, and 40 in 128 x 1 blocks).
+// of 512 threads took 64 us for 8192 x 8192; so 39, and 41 in 128 x 1 blocks).
 constexpr int kTileThreads = 256;
 constexpr int kDown = kTileThreads / 16;
 
