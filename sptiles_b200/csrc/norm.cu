@@ -974,9 +974,9 @@ struct ColumnSums {
 // In a fixed order: 1024 / W threads a column, each every (1024 / W)th group,
 // then a sum over them.  W columns a CTA: 32 (two planes of 296 groups of 4096
 // columns in 7.9 us), or 8, a sector, where that would leave half of the SMs
-// idle: narrow rows have many groups (backward of 65536 x 256 in 55.8 us with
-// 32, 52.8 with 8; 32768 x 512 in 65.0 and 62.1; but 16384 x 2048 in 72.3 and
-// 73.5).  blockIdx.y picks the plane, read once for all its sums.
+// idle: narrow rows have many groups (bf16 backward of 65536 x 256 in 55.8 us
+// with 32, 52.8 with 8; 32768 x 512 on an f32 stream in 65.0 and 62.1; but 16384
+// x 2048 in 72.3 and 73.5).  blockIdx.y picks the plane, read once for all its sums.
 template <typename T, int W>
 __global__ void __launch_bounds__(1024) column_sums_kernel(const float *sums, int groups, int cols, const ColumnSums todo) {
     pdl_wait();

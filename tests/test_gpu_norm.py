@@ -569,3 +569,18 @@ def test_backward_ring_keeps_bad_rows_apart(gate):
     assert torch.isnan(got.post_weight).all() and torch.isnan(got.pre_weight[207])
     if gate == "channel":
         assert torch.isnan(got.gate).all()
+
+
+@pytest.mark.parametrize("rows", [6, 700])
+@pytest.mark.parametrize("eps,alpha,offset", [(0.0, -1.5, 0.0), (1e-12, 0.0, 1.0), (1e-2, 3.0, -0.25), (10.0, 1.0, 2.0)])
+def test_other_options(rows, eps, alpha, offset, monkeypatch):
+    """eps, alpha and weight_offset over their range, none of them the defaults, on the generic kernels and on the rings."""
+    monkeypatch.setitem(globals(), "EPS", eps)
+    # backward64's masses of what alpha scales carry alpha's sign: alpha * (a sum of magnitudes), so that sum of magnitudes
+    # is their absolute value
+    plain = backward64
+    monkeypatch.setitem(globals(), "backward64", lambda *a: (lambda v, m: (v, {k: t.abs() for k, t in m.items()}))(*plain(*a)))
+    for gate in ("channel", "token"):
+        d = inputs(rows, 1024, F32, F32, gate, True, True, seed=8)
+        check_forward(d, alpha=alpha, offset=offset)
+        check_backward(d, rows, 1024, F32, F32, alpha=alpha, offset=offset)
