@@ -186,11 +186,11 @@ def run(state):
     return _run_forward(state) if state["case"]["direction"] == "forward" else _run_weights(state)
 
 
-def _power_of_two(top, limit):
-    """The least power of two p >= 2^-126 with limit * p >= top."""
+def _power_of_two(top, limit, least):
+    """The least power of two p >= 2^least with limit * p >= top."""
     fraction, exponent = torch.frexp(top.double() / limit)
     exponent = torch.where(fraction == 0.5, exponent - 1, exponent)
-    return torch.ldexp(torch.ones_like(fraction), exponent.clamp(min=-126)).float()
+    return torch.ldexp(torch.ones_like(fraction), exponent.clamp(min=least)).float()
 
 
 def _plain_blocks(x, block, amax):
@@ -200,11 +200,11 @@ def _plain_blocks(x, block, amax):
     top = wide.abs().amax(2)
     t = None
     if block == 16:
-        t = torch.where(amax > 0, _power_of_two(amax, 2688.0), torch.ones_like(amax))
+        t = torch.where(amax > 0, _power_of_two(amax, 2688.0, -126), torch.ones_like(amax))
         scale = (top / t / 6.0).clamp(max=448.0).to(torch.float8_e4m3fn).float()
         unit = scale * t
     else:
-        scale = unit = torch.where(top > 0, _power_of_two(top, 6.0), torch.full_like(top, 2.0 ** -127))
+        scale = unit = torch.where(top > 0, _power_of_two(top, 6.0, -127), torch.full_like(top, 2.0 ** -127))
     # a border between two levels times the unit is exact in fp32
     y, unit = wide.abs(), unit[:, :, None]
     index = torch.zeros(wide.shape, dtype=torch.int8, device=x.device)
