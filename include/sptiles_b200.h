@@ -50,6 +50,8 @@ extern "C" {
 #define ST_I32 3
 #define ST_E4M3 4 /* 8-bit floats: st_quantize_fp8, st_matmul_fp8 and the norms' 8-bit output only */
 #define ST_E5M2 5
+#define ST_E8M0 6   /* scales of 4-bit blocks: a power of two in a byte */
+#define ST_E2M1X2 7 /* two 4-bit floats a byte, the first in the low half: st_quantize_fp4 and its kin only */
 
 /* ---- binding kinds of st_param ---- */
 #define ST_PARAM_BUFFER 0 /* data pointer of one array (spirv StorageBuffer f32[]) */
@@ -282,6 +284,77 @@ int st_matmul_fp8_workspace(const st_tensor *a, const st_tensor *b, uint64_t *by
 int st_matmul_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_tensor *a_scale,
                   const st_tensor *b_scale, const st_tensor *bias, const st_tensor *c, void *workspace,
                   uint64_t workspace_bytes, const st_exec *exec);
+
+/* ---- 4-bit operands with a scale for each block of 16 or 32 ----
+ * No counterpart in the reference.  Device memory only.
+ *
+ * Elements are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two a
+ * byte: a tensor of ST_E2M1X2 counts bytes, so [rows, cols] elements are
+ * [rows, ceil(cols / 2)], along cols only.  A block lies along cols; its
+ * scale's type says how long it is:
+ *   ST_E4M3  16 elements, value = e2m1 * scale * tensor_scale
+ *   ST_E8M0  32 elements, value = e2m1 * scale, no tensor scale
+ * Scales are one byte each in a contiguous rank 1 tensor, in the order of the
+ * tensor core: [row / 128][block / 4][row % 32][row / 32 % 4][block % 4], so
+ * ceil(rows / 128) * ceil(blocks / 4) * 512 bytes, on a 16-byte boundary;
+ * those of rows and blocks that do not exist are to be 0.
+ *
+ * st_quantize_fp4: A (f32, f16 or bf16, any strides) to Q and scale.
+ *   ST_E4M3: tensor_scale (one f32, written) = least power of two t >= 2^-126 with 2688 t >= amax,
+ *            scale = e4m3(max|a| of the block / (6 t)), Q = e2m1(a / (scale t)); 0 where scale is 0
+ *   ST_E8M0: scale = least power of two >= 2^-127 with 6 scale >= max|a| of the block, Q = e2m1(a / scale)
+ * rounded to nearest even, saturating.  amax: one f32, the largest |a| to
+ * provide for (larger elements saturate), or NULL: then it is taken from A's
+ * finite elements, in a first pass.  A block with a NaN or an infinity gets
+ * the scale NaN.  Q has unit column stride.  workspace: st_quantize_fp4_workspace
+ * bytes, 4-byte aligned, where amax is to be taken.
+ * st_dequantize_fp4: the values back, as f32, f16 or bf16, out [rows, cols]
+ * with cols 2 * Q's columns, or one less. */
+int st_quantize_fp4_workspace(uint64_t *bytes);
+int st_quantize_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *q, const st_tensor *scale, const st_tensor *amax,
+                    const st_tensor *tensor_scale, void *workspace, uint64_t workspace_bytes, const st_exec *exec);
+int st_dequantize_fp4(st_ctx *ctx, const st_tensor *q, const st_tensor *scale, const st_tensor *tensor_scale,
+                      const st_tensor *out, const st_exec *exec);
+/* C = values(A) @ values(B) (+ bias): A [M, K/2] and B [K/2, N] bytes of
+ * ST_E2M1X2, scales of M and N rows and of one type; tensor scales one f32 or
+ * NULL (1; NULL with ST_E8M0).  C f32, f16 or bf16 [M, N] with unit column
+ * stride; bias f32 or C's dtype.  Sums are fp32; the tensor scales' product
+ * and the bias are applied in fp32.  The same inputs give the same bits.  An
+ * operand is read in place if its rows (B: columns) are contiguous along K, on
+ * 16-byte boundaries, and do not overlap; any other is copied first, into
+ * `workspace` (16-byte aligned, st_matmul_fp4_workspace bytes). */
+int st_matmul_fp4_workspace(const st_tensor *a, const st_tensor *b, uint64_t *bytes);
+int st_matmul_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_tensor *a_scale, const st_tensor *b_scale,
+                  const st_tensor *a_tensor_scale, const st_tensor *b_tensor_scale, const st_tensor *bias,
+                  const st_tensor *c, void *workspace, uint64_t workspace_bytes, const st_exec *exec);
+
+/* ---- products by groups of rows ----
+ * No counterpart in the reference.  Device memory only.
+ *
+ * ends (ST_I32, one per group, at most 1024, contiguous, on the device): group
+ * g is rows [ends[g - 1], ends[g]) of A, ends[-1] = 0; it may be empty.  An
+ * end below the one before it counts as that one, one beyond A's rows as
+ * their number.  No host code reads them.
+ * st_matmul_grouped: C[r, n] = sum_k A[r, k] B[g, k, n] for each row r of
+ * each group g.  A [R, K] and B, f16 or bf16 both, any strides; `b` is the
+ * first group's [K, N], the next one's lies b_group_stride elements further (0:
+ * one B for all).  C [R, N] f32, f16 or bf16, unit column stride.  Rows behind
+ * the last group are left as they are, or set to 0 with zero_rest.
+ * st_matmul_grouped_weights: D[g, k, n] = sum over g's rows of A[r, k] C[r, n],
+ * 0 for an empty group: the gradient of B where C is the gradient of the
+ * product.  `d` is the first group's [K, N], unit column stride; groups do not
+ * overlap.  (The gradient of A is st_matmul_grouped with B's transposed view.)
+ * Sums are fp32.  The same inputs give the same bits, whatever the other
+ * groups' rows hold.  An operand is read in place if it is contiguous along a
+ * dimension (A of st_matmul_grouped along K; both operands of the second form
+ * along their columns), with its rows and groups on 16-byte boundaries; any
+ * other is copied first, into `workspace` (16-byte aligned). */
+int st_matmul_grouped_workspace(const st_tensor *a, const st_tensor *b, int64_t b_group_stride, int64_t groups, uint64_t *bytes);
+int st_matmul_grouped(st_ctx *ctx, const st_tensor *a, const st_tensor *b, int64_t b_group_stride, const st_tensor *ends,
+                      const st_tensor *c, int32_t zero_rest, void *workspace, uint64_t workspace_bytes, const st_exec *exec);
+int st_matmul_grouped_weights_workspace(const st_tensor *a, const st_tensor *c, int64_t groups, uint64_t *bytes);
+int st_matmul_grouped_weights(st_ctx *ctx, const st_tensor *a, const st_tensor *c, const st_tensor *ends, const st_tensor *d,
+                              int64_t d_group_stride, void *workspace, uint64_t workspace_bytes, const st_exec *exec);
 
 /* ---- the norms after and before a block, its gate and residual scale ----
  * No counterpart in the reference.  Device memory only; tensors [rows, cols]

@@ -17,6 +17,8 @@ from .runtime import (  # noqa: F401
     shard_range, shutdown, stream_k_split, sync, tensor_1d_descriptor, tensor_2d_descriptor, tile_raster,
 )
 from .fp8 import matmul_fp8, quantize_fp8  # noqa: F401
+from .fp4 import Quantized4, dequantize_fp4, matmul_fp4, quantize_fp4  # noqa: F401
+from .grouped import matmul_grouped, matmul_grouped_weights  # noqa: F401
 from .norm import ResidualNorm, ResidualNormGrads, residual_norm, residual_norm_backward  # noqa: F401
 from .module import ModuleEntry, TileModule  # noqa: F401
 from ._native import DeviceAbort, NativeError, lib  # noqa: F401

@@ -25,7 +25,7 @@ ST_ERR_TIMEOUT = 7
 ST_ERR_DEVICE_ABORT = 8
 
 ST_F32, ST_F16, ST_BF16, ST_I32 = 0, 1, 2, 3
-ST_E4M3, ST_E5M2 = 4, 5
+ST_E4M3, ST_E5M2, ST_E8M0, ST_E2M1X2 = 4, 5, 6, 7
 ST_PARAM_BUFFER, ST_PARAM_I32 = 0, 1
 ST_MODULE_PARAM_BUFFER, ST_MODULE_PARAM_I32, ST_MODULE_PARAM_OTHER = 0, 1, 2
 ST_EXEC_SYNC, ST_EXEC_HOST_BUFFERS, ST_EXEC_DETERMINISTIC, ST_EXEC_ALL_DEVICES = 1, 2, 4, 8
@@ -37,7 +37,9 @@ EXPORTED = (
     "st_vector_add", "st_matmul", "st_vector_add_host", "st_matmul_host", "st_tile_raster",
     "st_matmul_plan", "st_stream_k_split", "st_shard_range", "st_matmul_static_scratch", "st_vector_fma", "st_cast",
     "st_quantize_fp8", "st_matmul_fp8_workspace", "st_matmul_fp8", "st_residual_norm",
-    "st_residual_norm_backward_workspace", "st_residual_norm_backward",
+    "st_quantize_fp4_workspace", "st_quantize_fp4", "st_dequantize_fp4", "st_matmul_fp4_workspace", "st_matmul_fp4",
+    "st_matmul_grouped_workspace", "st_matmul_grouped", "st_matmul_grouped_weights_workspace",
+    "st_matmul_grouped_weights", "st_residual_norm_backward_workspace", "st_residual_norm_backward",
     "st_ipc_handle", "st_ipc_open", "st_ipc_close", "st_matmul_allgather",
     "st_module_load", "st_module_load_file", "st_module_free", "st_module_version", "st_module_entry_count",
     "st_module_entry", "st_module_param", "st_launch_module", "st_check_device_wait",
@@ -121,6 +123,17 @@ def _declare(L: ctypes.CDLL) -> None:
         "st_quantize_fp8": ([vp, _P(StTensor), _P(StTensor), _P(StTensor), i32, i32, _P(StExec)], _c.c_int),
         "st_matmul_fp8_workspace": ([_P(StTensor), _P(StTensor), _P(u64)], _c.c_int),
         "st_matmul_fp8": ([vp] + [_P(StTensor)] * 6 + [vp, u64, _P(StExec)], _c.c_int),
+        "st_quantize_fp4_workspace": ([_P(u64)], _c.c_int),
+        "st_quantize_fp4": ([vp] + [_P(StTensor)] * 5 + [vp, u64, _P(StExec)], _c.c_int),
+        "st_dequantize_fp4": ([vp] + [_P(StTensor)] * 4 + [_P(StExec)], _c.c_int),
+        "st_matmul_fp4_workspace": ([_P(StTensor), _P(StTensor), _P(u64)], _c.c_int),
+        "st_matmul_fp4": ([vp] + [_P(StTensor)] * 8 + [vp, u64, _P(StExec)], _c.c_int),
+        "st_matmul_grouped_workspace": ([_P(StTensor), _P(StTensor), i64, i64, _P(u64)], _c.c_int),
+        "st_matmul_grouped": ([vp, _P(StTensor), _P(StTensor), i64, _P(StTensor), _P(StTensor), i32, vp, u64, _P(StExec)],
+                              _c.c_int),
+        "st_matmul_grouped_weights_workspace": ([_P(StTensor), _P(StTensor), i64, _P(u64)], _c.c_int),
+        "st_matmul_grouped_weights": ([vp, _P(StTensor), _P(StTensor), _P(StTensor), _P(StTensor), i64, vp, u64, _P(StExec)],
+                                      _c.c_int),
         "st_residual_norm": ([vp] + [_P(StTensor)] * 8 + [_P(StNormOptions), _P(StExec)], _c.c_int),
         "st_residual_norm_backward_workspace": ([i64, i64, _P(u64)], _c.c_int),
         "st_residual_norm_backward": ([vp] + [_P(StTensor)] * 12 + [vp, u64, _P(StNormOptions), _P(StExec)], _c.c_int),

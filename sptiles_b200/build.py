@@ -19,7 +19,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libsptiles_b200.so"
 SOURCES = ["runtime.cu", "vecadd.cu", "elementwise.cu", "gemm.cu", "pack.cu", "noalloc.cu", "module.cu", "diag.cu",
-           "quantize.cu", "gemm_fp8.cu", "norm.cu"]
+           "quantize.cu", "gemm_fp8.cu", "norm.cu", "quantize_fp4.cu", "gemm_fp4.cu", "gemm_grouped.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -278,6 +278,85 @@ struct QuantizeArgs {
 };
 int launch_quantize_fp8(const QuantizeArgs &args, cudaStream_t stream);
 
+// Dense copy of a strided byte matrix [rows, cols] into rows of `ld` bytes (a
+// multiple of 16; the padding gets bytes of no meaning).
+int launch_repack_8(const void *src, int64_t s0, int64_t s1, int64_t rows, int64_t cols, void *dst, int64_t ld,
+                    int sm_count, cudaStream_t stream);
+
+// ---- 4-bit operands with a scale per block of 16 or 32 along K (quantize_fp4.cu, gemm_fp4.cu)
+// Scales lie as [row / 128][block / 4][row % 32][row / 32 % 4][block % 4].
+inline int64_t fp4_scale_bytes(int64_t rows, int64_t blocks) { return cdiv(rows, 128) * cdiv(blocks, 4) * 512; }
+
+struct Quantize4Args {
+    const void *a;
+    int a_dtype;
+    int64_t sa0, sa1;
+    int64_t rows, cols;
+    bool wide;  // blocks of 32 with e8m0 scales; else 16 with e4m3
+    uint8_t *q;
+    int64_t sq0;  // bytes; two codes a byte along a row
+    uint8_t *scale;
+    const float *maxima = nullptr;  // the tensor's known maximum; null: taken from a
+    int n_maxima = 1;
+    float *tensor_scale = nullptr;  // blocks of 16: where the tensor's scale goes
+};
+int64_t quantize_fp4_workspace_bytes();
+int launch_quantize_fp4(const Quantize4Args &args, void *workspace, int sm_count, cudaStream_t stream);
+
+struct Dequantize4Args {
+    const uint8_t *q;
+    int64_t sq0, sq1;
+    int64_t rows, cols;
+    bool wide;
+    const uint8_t *scale;
+    const float *tensor_scale;  // or null
+    void *out;
+    int out_dtype;
+    int64_t so0, so1;
+};
+int launch_dequantize_fp4(const Dequantize4Args &args, int sm_count, cudaStream_t stream);
+
+// One operand as [rows, k]: A's rows are M, B's rows are N; k in bytes (two elements each).
+struct Fp4Operand {
+    const void *data;
+    int64_t rows, k;
+    int64_t s_row, s_k;
+    const void *scale;
+    const float *tensor_scale;  // or null
+};
+struct GemmFp4Args {
+    Fp4Operand a, b;
+    bool wide;
+    void *c;
+    int64_t ldc;
+    int c_dtype;
+    const void *bias;
+    int bias_dtype;
+};
+int64_t gemm_fp4_workspace_bytes(const Fp4Operand &a, const Fp4Operand &b);
+int launch_gemm_fp4(const GemmFp4Args &args, void *workspace, int sm_count, int *dev_err, uint64_t timeout_ns,
+                    cudaStream_t stream);
+
+// ---- products by groups of rows (gemm_grouped.cu); group g is rows [ends[g - 1], ends[g])
+constexpr int kGroupedMaxGroups = 1024;
+struct GroupedArgs {
+    bool weights;  // false: C [rows, n] = A [rows, k] @ B [groups, k, n];  true: C [groups, k, n] = A [rows, k]^T @ B [rows, n]
+    int dtype;     // ST_F16 or ST_BF16
+    int64_t groups, rows, k, n;
+    const int *ends;
+    const void *a;
+    int64_t a_s0, a_s1;
+    const void *b;
+    int64_t b_g, b_s0, b_s1;
+    void *c;
+    int64_t c_g, ldc;
+    int c_dtype;
+    bool zero_rest;  // rows of no group become 0
+};
+int64_t gemm_grouped_workspace_bytes(const GroupedArgs &args);
+int launch_gemm_grouped(const GroupedArgs &args, void *workspace, int sm_count, int *dev_err, uint64_t timeout_ns,
+                        cudaStream_t stream);
+
 // Norms around a block (norm.cu).  Strides in elements; unit column strides.
 struct NormView {
     void *p = nullptr;

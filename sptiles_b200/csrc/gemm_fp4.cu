@@ -1,0 +1,504 @@
+// gemm_fp4.cu -- matrix product of 4-bit operands (e2m1) with a scale for
+// each 16 (e4m3) or 32 (e8m0) elements along the contraction.
+//
+//   C[m, n] = ta tb sum_k (sa[m, k / block] A[m, k]) (sb[n, k / block] B[k, n])  (+ bias[n])
+//
+// The tensor core multiplies the scales in (tcgen05.mma with block_scale, 64
+// elements an instruction): they travel from shared memory to TMEM by
+// tcgen05.cp ahead of the MMAs that read them, in the order in which the
+// quantiser writes them, so that a stage's scales are one contiguous copy.
+// Sums are fp32; ta tb and the bias are applied in fp32 on the way out.
+//
+//   warp 0      TMA producer: 256 elements (128 bytes) of K of each operand a stage, and their scales
+//   warp 1      MMA issuer (owns the TMEM allocation)
+//   warps 2-5   C: TMEM -> registers, scale, bias, store
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <utility>
+
+#include "common.h"
+#include "fp8.cuh"
+#include "sm100.cuh"
+#include "tensor_map.h"
+
+namespace st {
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kBlockK = 128;     // bytes: 256 elements, one 128-byte swizzle span
+constexpr int kChunks = 4;       // MMAs of 64 elements in it
+constexpr int kAtomBytes = 512;  // scales of 128 rows and four blocks
+constexpr int kBarBytes = 512;
+
+struct Fp4Params {
+    int rows, cols;     // row operand x column operand
+    int k_blocks;       // of 256 elements
+    int k_chunks;       // of 64 elements
+    int quads;          // groups of four blocks: atoms of a row of tiles
+    int tiles_r, tiles_c, split;
+    const uint8_t *rs, *cs;    // scales of the row and the column operand
+    const float *ta, *tb;      // tensor scales, or null
+    void *c;
+    int64_t c_r, c_c;  // strides of C along the row and the column operand; one of them is 1
+    int c_dtype;
+    const void *bias;
+    int bias_dtype;
+    int bias_on_rows;  // B is the row operand: C's rows, contiguous, run along the tile's columns
+    uint32_t idesc[2];  // blocks of 32: the MMA of the lower and the upper two scales of a word
+    int *err;
+    unsigned long long timeout_ns;
+};
+
+__device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
+    if (dtype == ST_F32) return static_cast<const float *>(p)[i];
+    if (dtype == ST_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+
+__device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v) {
+    if (dtype == ST_F32) static_cast<float *>(p)[i] = v;
+    else if (dtype == ST_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Load 16 consecutive f32 columns of this thread's TMEM lane and wait for them.
+__device__ __forceinline__ void tmem_read_16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// ---------------------------------------------------------------- one CTA, 128 x BN tiles
+template <int BN>
+struct Fp4Cfg {
+    static constexpr int kOutWarps = 4;
+    static constexpr int kThreads = 32 * (2 + kOutWarps);
+    static constexpr int kRowBytes = kTileRows * kBlockK;
+    static constexpr int kColBytes = BN * kBlockK;
+    static constexpr int kScaleBytes = kChunks * kAtomBytes;  // of each operand (blocks of 32 use half)
+    static constexpr int kStageBytes = kRowBytes + kColBytes + 2 * kScaleBytes;
+    static constexpr int kStages = BN == 128 ? 5 : BN == 64 ? 3 : BN == 32 ? 4 : 5;
+    // A stage's scales have TMEM columns of their own: they are overwritten
+    // only after the MMAs that read them have freed the stage.
+    static constexpr int kStageCols = 2 * 4 * kChunks;
+    static constexpr int kScaleCol = BN;
+    static constexpr int kTmemCols = BN == 128 ? 512 : 256;
+    static_assert(kScaleCol + kStages * kStageCols <= kTmemCols, "the accumulator and the scales fit");
+    static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + 1024;
+    static_assert(kSmemBytes <= (BN == 128 ? 232448 : 115712), "shared memory of one (two) CTAs per SM");
+    static_assert(kStages * kStageBytes >= kTileRows * (BN + 4 * 8) * 4, "the ring holds eight parts' sums of its columns");
+};
+
+// Thread `first` of THREADS: its share of 128 rows x `own` columns (a power
+// of two, 4 at least), added over the parts of sums [part][row][own + 4],
+// times alpha.  By rows, the same 4 columns of every (4 THREADS / own)th row;
+// else every (THREADS / 128)th 4 columns of one row.
+template <typename T, int THREADS>
+__device__ __forceinline__ void store_parts(const Fp4Params &p, const float4 *sums, float alpha, int first, int own,
+                                            int own_shift, int parts, int r0, int col0) {
+    const int quads = own / 4, pitch = own / 4 + 1;
+    const bool by_rows = !p.bias_on_rows;  // not c_c == 1: a C of one row may have unit strides both ways
+    const int quad0 = by_rows ? first & (quads - 1) : first >> 7, r_first = by_rows ? first >> (own_shift - 2) : first & 127;
+    const int dr = by_rows ? 4 * THREADS / own : 0, dq = by_rows ? 0 : THREADS / 128;
+    T *c = static_cast<T *>(p.c) + (r0 + r_first) * p.c_r + (col0 + 4 * quad0) * p.c_c;
+    const int64_t dc = by_rows ? dr * p.c_r : 4 * dq * p.c_c;
+    const int left = p.cols - col0 - 4 * quad0;  // columns from this thread's first on
+    const bool four = by_rows && left >= 4 && reinterpret_cast<uintptr_t>(p.c) % (4 * sizeof(T)) == 0 && p.c_r % 4 == 0 &&
+                      col0 % 4 == 0;
+    // one bias for each column of a quad, or one for the row
+    float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias != nullptr) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = p.bias_on_rows ? r0 + r_first : col0 + 4 * quad0 + k;
+            if (i < (p.bias_on_rows ? p.rows : p.cols)) add[k] = load_any(p.bias, p.bias_dtype, i);
+        }
+    }
+#pragma unroll 2
+    for (int i = 0;; ++i, c += dc) {
+        const int r = r_first + i * dr, quad = quad0 + i * dq;
+        if (r >= kTileRows || quad >= quads || r0 + r >= p.rows) break;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int q = 0; q < parts; ++q) {
+            const float4 x = sums[(q * kTileRows + r) * pitch + quad];
+            v.x += x.x;
+            v.y += x.y;
+            v.z += x.z;
+            v.w += x.w;
+        }
+        T o[4];
+        from_float(__fmaf_rn(v.x, alpha, add[0]), o[0]);
+        from_float(__fmaf_rn(v.y, alpha, add[1]), o[1]);
+        from_float(__fmaf_rn(v.z, alpha, add[2]), o[2]);
+        from_float(__fmaf_rn(v.w, alpha, add[3]), o[3]);
+        if (four) {
+            struct alignas(4 * sizeof(T)) Four {
+                T v[4];
+            };
+            *reinterpret_cast<Four *>(c) = Four{{o[0], o[1], o[2], o[3]}};
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < left - 4 * i * dq) c[k * p.c_c] = o[k];
+        }
+    }
+}
+
+template <int BN, bool WIDE>
+__global__ void __launch_bounds__(Fp4Cfg<BN>::kThreads, BN == 128 ? 1 : 2)
+    gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
+                    const Fp4Params p) {
+    using Cfg = Fp4Cfg<BN>;
+    constexpr int kAtoms = WIDE ? 2 : 4;  // of a stage and an operand
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::kStages * Cfg::kStageBytes);
+    constexpr int kBars = 2 * Cfg::kStages + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t bar0 = smem_addr(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };                   // loads landed
+    auto empty_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };  // MMAs done
+    const uint32_t done_bar = bar0 + 8u * (kBars - 1);                       // all of the tile's MMAs done
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Cfg::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_map(&tmap_r);
+        tma_prefetch_map(&tmap_c);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_addr(tmem_slot), Cfg::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_begin();  // nothing above touches global memory
+
+    const int split = p.split;
+    const int part = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int tile = static_cast<int>(blockIdx.x) / split;
+    // neighbouring CTAs walk the row tiles of one column tile
+    const int tr = tile % p.tiles_r, tc = tile / p.tiles_r;
+    const int r0 = tr * kTileRows, c0 = tc * BN;
+    // blocks part, part + split, ...: a cluster's loads of a row lie next to each other
+    const int blocks = (p.k_blocks - part + split - 1) / split;
+
+    if (warp == 0) {
+        // ------------------------------------------------ TMA producer
+        if (lane == 0) {
+            // rows that one column tile reads pass through L2 once
+            const uint64_t pol = l2_policy_evict_last(), row_pol = p.tiles_c > 1 ? pol : l2_policy_evict_first();
+            const uint8_t *rs = p.rs + static_cast<int64_t>(tr) * p.quads * kAtomBytes;
+            const uint8_t *cs = p.cs + static_cast<int64_t>(c0 / 128) * p.quads * kAtomBytes;
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int b = part; b < p.k_blocks; b += split, ++issued) {
+                if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
+                    ok = false;
+                    break;
+                }
+                const int left = p.quads - b * kAtoms;
+                const uint32_t scale_bytes = static_cast<uint32_t>(left < kAtoms ? left : kAtoms) * kAtomBytes;
+                mbar_arrive_expect_tx(full_bar(s), Cfg::kRowBytes + Cfg::kColBytes + 2 * scale_bytes);
+                const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
+                const uint32_t sc = sr + Cfg::kRowBytes, ss = sc + Cfg::kColBytes;
+                tma_load_2d(sr, &tmap_r, full_bar(s), b * kBlockK, r0, row_pol);
+                tma_load_2d(sc, &tmap_c, full_bar(s), b * kBlockK, c0, pol);
+                bulk_load(ss, rs + static_cast<int64_t>(b) * kAtoms * kAtomBytes, scale_bytes, full_bar(s));
+                bulk_load(ss + Cfg::kScaleBytes, cs + static_cast<int64_t>(b) * kAtoms * kAtomBytes, scale_bytes, full_bar(s));
+                if (++s == Cfg::kStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                atomicExch(p.err, kDevAbortGemmProducer);
+            }
+            drain_ring(issued, Cfg::kStages, full_bar, p.timeout_ns);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issuer
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int i = 0; i < blocks; ++i) {
+            if (!__all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after_sync();
+            if (elect_one()) {
+                const int left = p.k_chunks - (part + i * split) * kChunks, n = left < kChunks ? left : kChunks;
+                const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
+                const uint32_t sc = sr + Cfg::kRowBytes, ss = sc + Cfg::kColBytes;
+                const uint32_t tr_s = tmem_base + static_cast<uint32_t>(Cfg::kScaleCol + s * Cfg::kStageCols);
+                const uint32_t tc_s = tr_s + 4 * kChunks;
+                const uint64_t dr = smem_desc_sw128(sr, 16, 1024), dc = smem_desc_sw128(sc, 16, 1024);
+                const uint64_t dsr = smem_desc_scales(ss), dsc = smem_desc_scales(ss + Cfg::kScaleBytes);
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j) {
+                    if (j >= n) break;
+                    const uint32_t atom = static_cast<uint32_t>(WIDE ? j / 2 : j);
+                    if (!WIDE || j % 2 == 0) {
+                        tmem_copy_scales(tr_s + 4 * atom, dsr + atom * (kAtomBytes >> 4));
+                        tmem_copy_scales(tc_s + 4 * atom, dsc + atom * (kAtomBytes >> 4));
+                    }
+                    tc_mma_fp4<WIDE ? 2 : 4>(tmem_base, dr + j * 2u, dc + j * 2u, p.idesc[WIDE ? j % 2 : 0], tr_s + 4 * atom,
+                                             tc_s + 4 * atom, i + j != 0 ? 1u : 0u);
+                }
+                tc_commit(empty_bar(s));
+            }
+            __syncwarp();
+            if (++s == Cfg::kStages) {
+                s = 0;
+                ph ^= 1u;
+            }
+        }
+        if (!ok) {
+            *abort_flag = 1;
+            atomicExch(p.err, kDevAbortGemmMma);
+        }
+        if (elect_one()) tc_commit(done_bar);
+        __syncwarp();
+        drain_ring(1, 1, [&](int) { return done_bar; }, p.timeout_ns);  // the MMAs read shared memory and write TMEM
+    }
+
+    // ------------------------------------------------ C
+    const int g = warp & 3, row_in_tile = g * 32 + lane;
+    const bool out = warp >= 2;
+    if (out) {
+        if (!__all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag, p.timeout_ns))) {
+            *abort_flag = 1;
+            if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
+        }
+        tc_fence_after_sync();
+    }
+    const float alpha = (p.ta != nullptr ? *p.ta : 1.0f) * (p.tb != nullptr ? *p.tb : 1.0f);
+    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(g * 32) << 16);
+    // A part owns `own` columns of the tile (with many parts, the last ones
+    // none): every CTA sends its sums to their owners' rings, once all of the
+    // cluster's MMAs have read them, as [part][row][own + 4 columns]; the
+    // owner adds its columns over the parts in order, a warp's lanes along C's
+    // contiguous dimension.
+    const int own = BN / split < 4 ? 4 : BN / split, own_shift = 31 - __clz(own);  // split is a power of two
+    const int stride = own + 4;  // floats; rows on different banks
+    __syncwarp();
+    if (split > 1) cluster_sync();
+    if (out) {
+        const uint32_t mine = smem_addr(smem) + 4u * static_cast<uint32_t>((part * kTileRows + row_in_tile) * stride);
+#pragma unroll
+        for (int c = 0; c < BN; c += 16) {
+            uint32_t v[16];
+            tmem_read_16(t_lane + static_cast<uint32_t>(c), v);
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                const int col = c + j;
+                const uint32_t to = (split == 1 ? mine : map_to_rank(mine, static_cast<uint32_t>(col >> own_shift))) +
+                                    4u * static_cast<uint32_t>(col & (own - 1));
+                st_cluster_v4(to, __uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]),
+                              __uint_as_float(v[j + 3]));
+            }
+        }
+    }
+    __syncwarp();
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+    if (out && part * own < BN) {
+        const float4 *sums = reinterpret_cast<const float4 *>(smem);
+        const int first = (warp - 2) * 32 + lane;
+        const int col0 = c0 + part * own;
+        constexpr int kOut = 32 * Cfg::kOutWarps;
+        if (p.c_dtype == ST_F32) store_parts<float, kOut>(p, sums, alpha, first, own, own_shift, split, r0, col0);
+        else if (p.c_dtype == ST_F16) store_parts<__half, kOut>(p, sums, alpha, first, own, own_shift, split, r0, col0);
+        else store_parts<__nv_bfloat16, kOut>(p, sums, alpha, first, own, own_shift, split, r0, col0);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    }
+}
+
+__global__ void __launch_bounds__(256) fill_bias_kernel(void *c, int64_t ldc, int c_dtype, const void *bias, int bias_dtype,
+                                                        int64_t m, int64_t n) {
+    pdl_wait();
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < m * n;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / n, q = i - r * n;
+        store_any(c, c_dtype, r * ldc + q, bias ? load_any(bias, bias_dtype, q) : 0.0f);
+    }
+    pdl_trigger();
+}
+
+// ---------------------------------------------------------------- host side
+int make_map_4(CUtensorMap *map, const char *what, const void *base, int64_t k_bytes, int64_t rows, int64_t ld, int box_rows) {
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k_bytes), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+    const cuuint32_t box[2] = {kBlockK, static_cast<cuuint32_t>(box_rows)};
+    return make_tensor_map(map, what, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box);
+}
+
+template <int BN, bool WIDE>
+int launch_instance(const CUtensorMap &mr, const CUtensorMap &mc, const Fp4Params &p, cudaStream_t stream) {
+    using Cfg = Fp4Cfg<BN>;
+    auto kern = gemm_fp4_kernel<BN, WIDE>;
+    static uint64_t attr_set = 0;  // one bit per device ordinal
+    int dev = 0;
+    ST_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !(attr_set & (1ull << dev))) {
+        ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
+        if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.tiles_r) * p.tiles_c * p.split));
+    cfg.blockDim = dim3(Cfg::kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (p.split > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = static_cast<unsigned>(p.split);
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    ST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mr, mc, p));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "gemm_fp4_kernel launch");
+}
+
+template <int BN>
+int launch_tile(const CUtensorMap &mr, const CUtensorMap &mc, const Fp4Params &p, bool wide, cudaStream_t stream) {
+    return wide ? launch_instance<BN, true>(mr, mc, p, stream) : launch_instance<BN, false>(mr, mc, p, stream);
+}
+
+// TMA reads an operand in place if its rows lie along K on 16-byte boundaries
+// and do not overlap; any other is copied first.
+struct Access {
+    bool copy;
+    int64_t ld;  // bytes between rows
+};
+
+Access access_of(const Fp4Operand &o) {
+    const bool fits = reinterpret_cast<uintptr_t>(o.data) % 16 == 0 && (o.s_k == 1 || o.k == 1) &&
+                      (o.rows == 1 || (o.s_row >= o.k && o.s_row % 16 == 0 && o.s_row < (int64_t(1) << 40)));
+    return {!fits, fits && o.rows > 1 ? o.s_row : (o.k + 15) / 16 * 16};
+}
+
+int64_t copy_bytes(const Fp4Operand &o, const Access &a) { return a.copy ? (o.rows * a.ld + 255) / 256 * 256 : 0; }
+
+struct Fp4Plan {
+    int bn = 128, split = 1;
+};
+
+Fp4Plan plan_fp4(int64_t rows, int64_t cols, int64_t k_blocks, int sm_count) {
+    Fp4Plan best;
+    best.bn = cols <= 16 ? 16 : cols <= 32 ? 32 : cols <= 64 ? 64 : 128;
+    const int64_t tiles = cdiv(rows, kTileRows) * cdiv(cols, best.bn), slots = static_cast<int64_t>(sm_count) * (best.bn == 128 ? 1 : 2);
+    while (best.split < 8 && tiles * best.split * 2 <= slots && best.split * 4 <= k_blocks) best.split *= 2;
+    return best;
+}
+
+}  // namespace
+
+int64_t gemm_fp4_workspace_bytes(const Fp4Operand &a, const Fp4Operand &b) {
+    if (a.rows == 0 || b.rows == 0 || a.k == 0) return 0;
+    return copy_bytes(a, access_of(a)) + copy_bytes(b, access_of(b));
+}
+
+int launch_gemm_fp4(const GemmFp4Args &g, void *workspace, int sm_count, int *dev_err, uint64_t timeout_ns,
+                    cudaStream_t stream) {
+    const int64_t m = g.a.rows, n = g.b.rows, k = g.a.k;
+    if (m == 0 || n == 0) return ST_OK;
+    if (k == 0) {
+        ST_CUDA_TRY(launch_kernel(fill_bias_kernel, static_cast<unsigned>(sm_count), 256, 0, stream, g.c, g.ldc,
+                                  g.c_dtype, g.bias, g.bias_dtype, m, n));
+        note_launch();
+        const cudaError_t e = cudaPeekAtLastError();
+        return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "fill_bias_kernel");
+    }
+    Fp4Operand op[2] = {g.a, g.b};
+    Access acc[2] = {access_of(g.a), access_of(g.b)};
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    for (int i = 0; i < 2; ++i) {
+        if (!acc[i].copy) continue;
+        ST_TRY(launch_repack_8(op[i].data, op[i].s_row, op[i].s_k, op[i].rows, op[i].k, ws, acc[i].ld, sm_count, stream));
+        op[i].data = ws;
+        ws += copy_bytes(op[i], acc[i]);
+    }
+    const int64_t k_blocks = cdiv(k, kBlockK);
+    // few rows of A make the columns of a narrow tile, against 128 rows of B
+    const bool swap = m <= 64;
+    const int ri = swap ? 1 : 0, ci = swap ? 0 : 1;
+    const Fp4Operand &r = op[ri], &c = op[ci];
+    const Fp4Plan plan = plan_fp4(r.rows, c.rows, k_blocks, sm_count);
+    Fp4Params p{};
+    p.rows = static_cast<int>(r.rows);
+    p.cols = static_cast<int>(c.rows);
+    p.k_blocks = static_cast<int>(k_blocks);
+    p.k_chunks = static_cast<int>(cdiv(k, 32));
+    p.quads = static_cast<int>(cdiv(cdiv(k, g.wide ? 16 : 8), 4));
+    p.tiles_r = static_cast<int>(cdiv(r.rows, kTileRows));
+    p.tiles_c = static_cast<int>(cdiv(c.rows, plan.bn));
+    p.split = plan.split;
+    if (static_cast<int64_t>(p.tiles_r) * p.tiles_c * p.split > INT32_MAX)
+        return fail(ST_ERR_UNSUPPORTED, "matmul_fp4: too many output tiles");
+    p.rs = static_cast<const uint8_t *>(r.scale);
+    p.cs = static_cast<const uint8_t *>(c.scale);
+    p.ta = g.a.tensor_scale;
+    p.tb = g.b.tensor_scale;
+    p.c = g.c;
+    p.c_r = swap ? 1 : g.ldc;
+    p.c_c = swap ? g.ldc : 1;
+    p.c_dtype = g.c_dtype;
+    p.bias = g.bias;
+    p.bias_dtype = g.bias_dtype;
+    p.bias_on_rows = swap;
+    for (uint32_t i = 0; i < 2; ++i) p.idesc[i] = mma_idesc_fp4(g.wide, 2 * i, kTileRows, static_cast<uint32_t>(plan.bn));
+    p.err = dev_err;
+    p.timeout_ns = timeout_ns;
+    CUtensorMap mr, mc;
+    ST_TRY(make_map_4(&mr, "a 4-bit operand", r.data, k, r.rows, acc[ri].ld, kTileRows));
+    ST_TRY(make_map_4(&mc, "a 4-bit operand", c.data, k, c.rows, acc[ci].ld, plan.bn));
+    switch (plan.bn) {
+    case 16: return launch_tile<16>(mr, mc, p, g.wide, stream);
+    case 32: return launch_tile<32>(mr, mc, p, g.wide, stream);
+    case 64: return launch_tile<64>(mr, mc, p, g.wide, stream);
+    default: return launch_tile<128>(mr, mc, p, g.wide, stream);
+    }
+}
+
+}  // namespace st

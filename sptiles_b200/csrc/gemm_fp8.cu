@@ -1346,19 +1346,24 @@ int64_t copy_bytes(const Fp8Operand &o, const Access &a) {
     return a.copy ? ((a.mn ? o.k : o.rows) * a.ld + 255) / 256 * 256 : 0;
 }
 
-int launch_repack_8(const Fp8Operand &o, const Access &a, uint8_t *dst, int sm_count, cudaStream_t stream) {
+int copy_operand(const Fp8Operand &o, const Access &a, uint8_t *dst, int sm_count, cudaStream_t stream) {
     const int64_t outer = a.mn ? o.k : o.rows, inner = a.mn ? o.rows : o.k;
     const int64_t s0 = a.mn ? o.s_k : o.s_row, s1 = a.mn ? o.s_row : o.s_k;
-    int64_t grid = cdiv(outer * (a.ld / 16), 256);
+    return launch_repack_8(o.data, s0, s1, outer, inner, dst, a.ld, sm_count, stream);
+}
+
+}  // namespace
+
+int launch_repack_8(const void *src, int64_t s0, int64_t s1, int64_t rows, int64_t cols, void *dst, int64_t ld,
+                    int sm_count, cudaStream_t stream) {
+    int64_t grid = cdiv(rows * (ld / 16), 256);
     if (grid > static_cast<int64_t>(sm_count) * 8) grid = static_cast<int64_t>(sm_count) * 8;
-    ST_CUDA_TRY(launch_kernel(repack_8_kernel, static_cast<unsigned>(grid), 256, 0, stream,
-                              static_cast<const uint8_t *>(o.data), s0, inner == 1 ? int64_t(1) : s1, outer, inner, dst, a.ld));
+    ST_CUDA_TRY(launch_kernel(repack_8_kernel, static_cast<unsigned>(grid), 256, 0, stream, static_cast<const uint8_t *>(src), s0,
+                              cols == 1 ? int64_t(1) : s1, rows, cols, static_cast<uint8_t *>(dst), ld));
     note_launch();
     const cudaError_t e = cudaPeekAtLastError();
     return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "repack_8_kernel");
 }
-
-}  // namespace
 
 int launch_fp8_wait_check(bool by_column, uint64_t limit_ns, int *dev_err, cudaStream_t stream) {
     if (by_column) fp8_wait_check_kernel<true><<<1, 32, 0, stream>>>(limit_ns, dev_err);
@@ -1389,7 +1394,7 @@ int launch_gemm_fp8(const GemmFp8Args &g, void *workspace, int sm_count, int *de
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     for (int i = 0; i < 2; ++i) {
         if (!acc[i].copy) continue;
-        ST_TRY(launch_repack_8(op[i], acc[i], ws, sm_count, stream));
+        ST_TRY(copy_operand(op[i], acc[i], ws, sm_count, stream));
         op[i].data = ws;
         ws += copy_bytes(op[i], acc[i]);
     }

@@ -951,6 +951,126 @@ int set_scale(const st_tensor *t, const char *name, bool is_b, Fp8Operand *o) {
     return ST_OK;
 }
 
+// ---- 4-bit blocks
+int check_codes(const st_tensor *t, const char *name) {
+    ST_TRY(check_matrix(t, name));
+    if (t->dtype != ST_E2M1X2) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be ST_E2M1X2");
+    if (t->shape[0] > INT32_MAX / 2 || t->shape[1] > INT32_MAX / 2)
+        return fail(ST_ERR_UNSUPPORTED, std::string(name) + ": elements of a row or column must fit in int32");
+    return ST_OK;
+}
+
+// The scales of `rows` rows of `bytes` bytes of codes.
+int check_fp4_scale(const st_tensor *t, const char *name, int64_t rows, int64_t bytes) {
+    if (!t) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " is null");
+    if (t->dtype != ST_E4M3 && t->dtype != ST_E8M0)
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be ST_E4M3 (blocks of 16) or ST_E8M0 (blocks of 32)");
+    const int64_t need = fp4_scale_bytes(rows, cdiv(bytes, t->dtype == ST_E8M0 ? 16 : 8));
+    if (t->rank != 1 || t->shape[0] != need || (need > 1 && t->strides[0] != 1))
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be contiguous, with " + std::to_string(need) +
+                                                 " scales: [ceil(rows / 128)][ceil(blocks / 4)][32][4][4]");
+    if (need > 0 && !t->data) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " has a null data pointer");
+    if (need > 0 && !aligned16(t->data)) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must start on a 16-byte boundary");
+    return ST_OK;
+}
+
+// One f32 on the device, or null.
+int scalar_of(const st_tensor *t, const char *name, float **out) {
+    *out = nullptr;
+    if (!t) return ST_OK;
+    if (t->dtype != ST_F32 || t->rank != 1 || t->shape[0] != 1 || !t->data)
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be one ST_F32");
+    *out = static_cast<float *>(t->data);
+    return ST_OK;
+}
+
+int check_fp4_operands(const st_tensor *a, const st_tensor *b) {
+    ST_TRY(check_codes(a, "A"));
+    ST_TRY(check_codes(b, "B"));
+    if (a->shape[1] != b->shape[0])
+        return fail(ST_ERR_INVALID_ARGUMENT, "Incompatible matrices: K dimension of A (" + std::to_string(a->shape[1]) +
+                                                 " bytes) must match K dimension of B (" + std::to_string(b->shape[0]) + ")");
+    return ST_OK;
+}
+
+Fp4Operand fp4_operand(const st_tensor &t, bool is_b) {
+    Fp4Operand o{};
+    o.data = t.data;
+    o.rows = t.shape[is_b ? 1 : 0];
+    o.k = t.shape[is_b ? 0 : 1];
+    o.s_row = t.strides[is_b ? 1 : 0];
+    o.s_k = t.strides[is_b ? 0 : 1];
+    return o;
+}
+
+int check_workspace(const char *what, int64_t need, const void *workspace, uint64_t bytes, uintptr_t align) {
+    if (need <= 0) return ST_OK;
+    if (!workspace || bytes < static_cast<uint64_t>(need))
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(what) + " needs a workspace of " + std::to_string(need) + " bytes");
+    if (reinterpret_cast<uintptr_t>(workspace) % align != 0)
+        return fail(ST_ERR_INVALID_ARGUMENT, "workspace must be " + std::to_string(align) + "-byte aligned");
+    return ST_OK;
+}
+
+// ---- products by groups of rows
+int check_ends(const st_tensor *t) {
+    if (!t) return fail(ST_ERR_INVALID_ARGUMENT, "ends is null");
+    if (t->dtype != ST_I32 || t->rank != 1) return fail(ST_ERR_INVALID_ARGUMENT, "ends must be rank 1 of ST_I32");
+    if (t->shape[0] < 0) return fail(ST_ERR_INVALID_ARGUMENT, "ends has a negative extent");
+    if (t->shape[0] > kGroupedMaxGroups)
+        return fail(ST_ERR_UNSUPPORTED, "at most " + std::to_string(kGroupedMaxGroups) + " groups, got " + std::to_string(t->shape[0]));
+    if (t->shape[0] > 1 && t->strides[0] != 1) return fail(ST_ERR_INVALID_ARGUMENT, "ends must be contiguous");
+    if (t->shape[0] > 0 && !t->data) return fail(ST_ERR_INVALID_ARGUMENT, "ends has a null data pointer");
+    return ST_OK;
+}
+
+// A [rows, k] and, for one group, B [k, n] (weights: B [rows, n]).
+int grouped_operands(const char *what, const st_tensor *a, const st_tensor *b, const char *b_name, bool weights, int64_t groups,
+                     int64_t b_group_stride, GroupedArgs *g) {
+    ST_TRY(check_matrix(a, "A"));
+    st_tensor shape_of_b{};
+    if (b && !weights && groups == 0) {  // no matrix, but the extents of one
+        shape_of_b = *b;
+        shape_of_b.data = &shape_of_b;
+        b = &shape_of_b;
+    }
+    ST_TRY(check_matrix(b, b_name));
+    if (a->dtype == ST_F32 && b->dtype == ST_F32)
+        return fail(ST_ERR_UNSUPPORTED, std::string(what) + ": operands must be ST_F16 or ST_BF16");
+    if ((a->dtype != ST_F16 && a->dtype != ST_BF16) || a->dtype != b->dtype)
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(what) + ": A and " + b_name + " must both be ST_F16 or both ST_BF16");
+    if (weights && a->shape[0] != b->shape[0])
+        return fail(ST_ERR_INVALID_ARGUMENT, "A and C must have the same rows, got " + std::to_string(a->shape[0]) + " and " +
+                                                 std::to_string(b->shape[0]));
+    if (!weights && a->shape[1] != b->shape[0])
+        return fail(ST_ERR_INVALID_ARGUMENT, "Incompatible matrices: K dimension of A (" + std::to_string(a->shape[1]) +
+                                                 ") must match K dimension of B (" + std::to_string(b->shape[0]) + ")");
+    if (b_group_stride < 0) return fail(ST_ERR_INVALID_ARGUMENT, std::string(b_name) + " has a negative group stride");
+    g->weights = weights;
+    g->dtype = a->dtype;
+    g->groups = groups;
+    g->rows = a->shape[0];
+    g->k = a->shape[1];
+    g->n = b->shape[1];
+    g->a = a->data;
+    g->a_s0 = a->strides[0];
+    g->a_s1 = a->strides[1];
+    g->b = b->data;
+    g->b_g = b_group_stride;
+    g->b_s0 = b->strides[0];
+    g->b_s1 = b->strides[1];
+    return ST_OK;
+}
+
+int check_grouped_output(const st_tensor *c, const char *name, int64_t rows, int64_t cols) {
+    ST_TRY(check_matrix(c, name));
+    if (c->shape[0] != rows || c->shape[1] != cols)
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be [" + std::to_string(rows) + ", " + std::to_string(cols) + "]");
+    if (!is_float(c->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be ST_F32, ST_F16 or ST_BF16");
+    if (!unit_columns(*c)) return fail(ST_ERR_UNSUPPORTED, std::string(name) + " must have unit column stride");
+    return check_output(*c, name);
+}
+
 // A tensor of the norms: [rows, cols] with unit column stride.
 int norm_view(const st_tensor *t, const char *name, int64_t rows, int64_t cols, bool output, NormView *out) {
     if (!t) return ST_OK;
@@ -1619,6 +1739,205 @@ int st_matmul_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
     ST_TRY(resolve_exec(ctx, exec, &x));
     DeviceGuard guard(x.dev->ordinal);
     ST_TRY(launch_gemm_fp8(g, workspace, x.dev->sm_count, x.dev->dev_err, kDeviceWaitLimitNs, x.stream));
+    return finish(x);
+}
+
+int st_quantize_fp4_workspace(uint64_t *bytes) {
+    if (!bytes) return fail(ST_ERR_INVALID_ARGUMENT, "bytes is null");
+    *bytes = static_cast<uint64_t>(quantize_fp4_workspace_bytes());
+    return ST_OK;
+}
+
+int st_quantize_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *q, const st_tensor *scale, const st_tensor *amax,
+                    const st_tensor *tensor_scale, void *workspace, uint64_t workspace_bytes, const st_exec *exec) {
+    ST_TRY(check_matrix(a, "A"));
+    ST_TRY(check_codes(q, "Q"));
+    if (!is_float(a->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp4: A must be ST_F32, ST_F16 or ST_BF16");
+    if (q->shape[0] != a->shape[0] || q->shape[1] != cdiv(a->shape[1], 2))
+        return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp4: Q must be [rows, ceil(cols / 2)] = [" + std::to_string(a->shape[0]) + ", " +
+                                                 std::to_string(cdiv(a->shape[1], 2)) + "]");
+    if (!unit_columns(*q)) return fail(ST_ERR_UNSUPPORTED, "quantize_fp4: Q must have unit column stride");
+    ST_TRY(check_output(*q, "Q"));
+    ST_TRY(check_fp4_scale(scale, "scale", q->shape[0], q->shape[1]));
+    Quantize4Args g{};
+    float *known = nullptr;
+    ST_TRY(scalar_of(amax, "amax", &known));
+    ST_TRY(scalar_of(tensor_scale, "tensor_scale", &g.tensor_scale));
+    g.wide = scale->dtype == ST_E8M0;
+    if (g.wide && (amax || tensor_scale))
+        return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp4: amax and tensor_scale go with ST_E4M3 scales");
+    if (!g.wide && !tensor_scale) return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp4: ST_E4M3 scales need tensor_scale");
+    if (!g.wide && !known && a->shape[0] > 0 && a->shape[1] > 0)
+        ST_TRY(check_workspace("quantize_fp4", quantize_fp4_workspace_bytes(), workspace, workspace_bytes, 4));
+    g.a = a->data;
+    g.a_dtype = a->dtype;
+    g.sa0 = a->strides[0];
+    g.sa1 = a->strides[1];
+    g.rows = a->shape[0];
+    g.cols = a->shape[1];
+    g.q = static_cast<uint8_t *>(q->data);
+    g.sq0 = q->strides[0];
+    g.scale = static_cast<uint8_t *>(scale->data);
+    g.maxima = known;
+    ExecCtx x;
+    ST_TRY(resolve_exec(ctx, exec, &x));
+    DeviceGuard guard(x.dev->ordinal);
+    ST_TRY(launch_quantize_fp4(g, workspace, x.dev->sm_count, x.stream));
+    return finish(x);
+}
+
+int st_dequantize_fp4(st_ctx *ctx, const st_tensor *q, const st_tensor *scale, const st_tensor *tensor_scale,
+                      const st_tensor *out, const st_exec *exec) {
+    ST_TRY(check_codes(q, "Q"));
+    ST_TRY(check_matrix(out, "out"));
+    ST_TRY(check_fp4_scale(scale, "scale", q->shape[0], q->shape[1]));
+    if (!is_float(out->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, "dequantize_fp4: out must be ST_F32, ST_F16 or ST_BF16");
+    if (out->shape[0] != q->shape[0] || cdiv(out->shape[1], 2) != q->shape[1])
+        return fail(ST_ERR_INVALID_ARGUMENT, "dequantize_fp4: out must be [" + std::to_string(q->shape[0]) + ", " +
+                                                 std::to_string(2 * q->shape[1]) + "], or a column less");
+    ST_TRY(check_output(*out, "out"));
+    Dequantize4Args g{};
+    float *t = nullptr;
+    ST_TRY(scalar_of(tensor_scale, "tensor_scale", &t));
+    g.wide = scale->dtype == ST_E8M0;
+    if (g.wide && t) return fail(ST_ERR_INVALID_ARGUMENT, "dequantize_fp4: tensor_scale goes with ST_E4M3 scales");
+    g.q = static_cast<const uint8_t *>(q->data);
+    g.sq0 = q->strides[0];
+    g.sq1 = q->shape[1] > 1 ? q->strides[1] : 1;
+    g.rows = out->shape[0];
+    g.cols = out->shape[1];
+    g.scale = static_cast<const uint8_t *>(scale->data);
+    g.tensor_scale = t;
+    g.out = out->data;
+    g.out_dtype = out->dtype;
+    g.so0 = out->strides[0];
+    g.so1 = out->shape[1] > 1 ? out->strides[1] : 1;
+    ExecCtx x;
+    ST_TRY(resolve_exec(ctx, exec, &x));
+    DeviceGuard guard(x.dev->ordinal);
+    ST_TRY(launch_dequantize_fp4(g, x.dev->sm_count, x.stream));
+    return finish(x);
+}
+
+int st_matmul_fp4_workspace(const st_tensor *a, const st_tensor *b, uint64_t *bytes) {
+    if (!bytes) return fail(ST_ERR_INVALID_ARGUMENT, "bytes is null");
+    ST_TRY(check_fp4_operands(a, b));
+    *bytes = static_cast<uint64_t>(gemm_fp4_workspace_bytes(fp4_operand(*a, false), fp4_operand(*b, true)));
+    return ST_OK;
+}
+
+int st_matmul_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_tensor *a_scale, const st_tensor *b_scale,
+                  const st_tensor *a_tensor_scale, const st_tensor *b_tensor_scale, const st_tensor *bias,
+                  const st_tensor *c, void *workspace, uint64_t workspace_bytes, const st_exec *exec) {
+    ST_TRY(check_fp4_operands(a, b));
+    GemmFp4Args g{};
+    g.a = fp4_operand(*a, false);
+    g.b = fp4_operand(*b, true);
+    ST_TRY(check_fp4_scale(a_scale, "a_scale", g.a.rows, g.a.k));
+    ST_TRY(check_fp4_scale(b_scale, "b_scale", g.b.rows, g.b.k));
+    if (a_scale->dtype != b_scale->dtype)
+        return fail(ST_ERR_INVALID_ARGUMENT, "matmul_fp4: a_scale and b_scale must have one type");
+    g.wide = a_scale->dtype == ST_E8M0;
+    g.a.scale = a_scale->data;
+    g.b.scale = b_scale->data;
+    float *t = nullptr;
+    ST_TRY(scalar_of(a_tensor_scale, "a_tensor_scale", &t));
+    g.a.tensor_scale = t;
+    ST_TRY(scalar_of(b_tensor_scale, "b_tensor_scale", &t));
+    g.b.tensor_scale = t;
+    if (g.wide && (a_tensor_scale || b_tensor_scale))
+        return fail(ST_ERR_INVALID_ARGUMENT, "matmul_fp4: tensor scales go with ST_E4M3 scales");
+    ST_TRY(check_matrix(c, "C"));
+    if (c->shape[0] != g.a.rows || c->shape[1] != g.b.rows)
+        return fail(ST_ERR_INVALID_ARGUMENT, "C must be [M, N] = [" + std::to_string(g.a.rows) + ", " +
+                                                 std::to_string(g.b.rows) + "]");
+    if (!is_float(c->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, "C must be ST_F32, ST_F16 or ST_BF16");
+    if (!unit_columns(*c)) return fail(ST_ERR_UNSUPPORTED, "C must have unit column stride");
+    ST_TRY(check_output(*c, "C"));
+    if (bias) {
+        if (bias->rank != 1 || bias->shape[0] != g.b.rows)
+            return fail(ST_ERR_INVALID_ARGUMENT, "bias must have N elements");
+        if (bias->dtype != ST_F32 && (bias->dtype != c->dtype || !is_float(bias->dtype)))
+            return fail(ST_ERR_INVALID_ARGUMENT, "bias must be ST_F32 or C's dtype");
+        if (bias->shape[0] > 1 && bias->strides[0] != 1) return fail(ST_ERR_UNSUPPORTED, "bias must be contiguous");
+        if (bias->shape[0] > 0 && !bias->data) return fail(ST_ERR_INVALID_ARGUMENT, "bias has a null data pointer");
+        g.bias = bias->data;
+        g.bias_dtype = bias->dtype;
+    }
+    ST_TRY(check_workspace("matmul_fp4", gemm_fp4_workspace_bytes(g.a, g.b), workspace, workspace_bytes, 16));
+    g.c = c->data;
+    g.ldc = c->strides[0];
+    g.c_dtype = c->dtype;
+    ExecCtx x;
+    ST_TRY(resolve_exec(ctx, exec, &x));
+    DeviceGuard guard(x.dev->ordinal);
+    ST_TRY(launch_gemm_fp4(g, workspace, x.dev->sm_count, x.dev->dev_err, kDeviceWaitLimitNs, x.stream));
+    return finish(x);
+}
+
+int st_matmul_grouped_workspace(const st_tensor *a, const st_tensor *b, int64_t b_group_stride, int64_t groups, uint64_t *bytes) {
+    if (!bytes) return fail(ST_ERR_INVALID_ARGUMENT, "bytes is null");
+    if (groups < 0 || groups > kGroupedMaxGroups) return fail(ST_ERR_INVALID_ARGUMENT, "groups must be in [0, 1024]");
+    GroupedArgs g{};
+    ST_TRY(grouped_operands("matmul_grouped", a, b, "B", false, groups, b_group_stride, &g));
+    *bytes = static_cast<uint64_t>(gemm_grouped_workspace_bytes(g));
+    return ST_OK;
+}
+
+int st_matmul_grouped(st_ctx *ctx, const st_tensor *a, const st_tensor *b, int64_t b_group_stride, const st_tensor *ends,
+                      const st_tensor *c, int32_t zero_rest, void *workspace, uint64_t workspace_bytes, const st_exec *exec) {
+    ST_TRY(check_ends(ends));
+    GroupedArgs g{};
+    ST_TRY(grouped_operands("matmul_grouped", a, b, "B", false, ends->shape[0], b_group_stride, &g));
+    ST_TRY(check_grouped_output(c, "C", g.rows, g.n));
+    ST_TRY(check_workspace("matmul_grouped", gemm_grouped_workspace_bytes(g), workspace, workspace_bytes, 16));
+    g.ends = static_cast<const int *>(ends->data);
+    g.c = c->data;
+    g.ldc = c->strides[0];
+    g.c_dtype = c->dtype;
+    g.zero_rest = zero_rest != 0;
+    ExecCtx x;
+    ST_TRY(resolve_exec(ctx, exec, &x));
+    DeviceGuard guard(x.dev->ordinal);
+    ST_TRY(launch_gemm_grouped(g, workspace, x.dev->sm_count, x.dev->dev_err, kDeviceWaitLimitNs, x.stream));
+    return finish(x);
+}
+
+int st_matmul_grouped_weights_workspace(const st_tensor *a, const st_tensor *c, int64_t groups, uint64_t *bytes) {
+    if (!bytes) return fail(ST_ERR_INVALID_ARGUMENT, "bytes is null");
+    if (groups < 0 || groups > kGroupedMaxGroups) return fail(ST_ERR_INVALID_ARGUMENT, "groups must be in [0, 1024]");
+    GroupedArgs g{};
+    ST_TRY(grouped_operands("matmul_grouped_weights", a, c, "C", true, groups, 0, &g));
+    *bytes = static_cast<uint64_t>(gemm_grouped_workspace_bytes(g));
+    return ST_OK;
+}
+
+int st_matmul_grouped_weights(st_ctx *ctx, const st_tensor *a, const st_tensor *c, const st_tensor *ends, const st_tensor *d,
+                              int64_t d_group_stride, void *workspace, uint64_t workspace_bytes, const st_exec *exec) {
+    ST_TRY(check_ends(ends));
+    GroupedArgs g{};
+    ST_TRY(grouped_operands("matmul_grouped_weights", a, c, "C", true, ends->shape[0], 0, &g));
+    st_tensor shape_of_d{};
+    if (d && g.groups == 0) {  // no matrix, but the extents of one
+        shape_of_d = *d;
+        shape_of_d.data = &shape_of_d;
+        d = &shape_of_d;
+    }
+    ST_TRY(check_grouped_output(d, "D", g.k, g.n));
+    const int64_t span = g.k > 0 && g.n > 0 ? (g.k - 1) * d->strides[0] + g.n : 0;
+    if (g.groups > 1 && d_group_stride < span)
+        return fail(ST_ERR_INVALID_ARGUMENT, "D has overlapping groups: their stride is " + std::to_string(d_group_stride) +
+                                                 ", one spans " + std::to_string(span) + " elements");
+    ST_TRY(check_workspace("matmul_grouped_weights", gemm_grouped_workspace_bytes(g), workspace, workspace_bytes, 16));
+    g.ends = static_cast<const int *>(ends->data);
+    g.c = d->data;
+    g.c_g = d_group_stride;
+    g.ldc = d->strides[0];
+    g.c_dtype = d->dtype;
+    ExecCtx x;
+    ST_TRY(resolve_exec(ctx, exec, &x));
+    DeviceGuard guard(x.dev->ordinal);
+    ST_TRY(launch_gemm_grouped(g, workspace, x.dev->sm_count, x.dev->dev_err, kDeviceWaitLimitNs, x.stream));
     return finish(x);
 }
 

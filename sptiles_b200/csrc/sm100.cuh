@@ -96,6 +96,16 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map
         : "memory");
 }
 
+// 3D tiled load, as above; c1 and c2 may lie outside of the tensor (zeros).
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t c0, int32_t c1,
+                                            int32_t c2, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+        : "memory");
+}
+
 // 2D tiled store of one shared-memory box to global memory (this GPU's or a
 // peer's through an IPC mapping), tracked by the issuing thread's bulk
 // async-groups.  Same alignment rule on c0 as the load; c0, c1 >= 0.
@@ -234,6 +244,39 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+
+// 4-bit operands (e2m1, both K-major, K = 64 per instruction) with a scale
+// for each 16 (SCALES 4: e4m3) or 32 (SCALES 2: e8m0) elements along K, read
+// from TMEM, f32 accumulator.  sfa, sfb: TMEM columns of the scales as
+// tmem_copy_scales brings them.
+template <int SCALES>
+__device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    static_assert(SCALES == 4 || SCALES == 2, "scales per row and instruction");
+    if constexpr (SCALES == 4)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+
+// 512 bytes of scales (128 rows x 4 along K, in the order [row % 32][row /
+// 32][4]) from shared memory into four TMEM columns: 32 lanes of 16 bytes,
+// repeated for the four lane quarters.  Ordered before the MMAs that the same
+// thread issues after it.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 // True in one lane of a converged warp.  A warp that keeps together and
@@ -463,6 +506,27 @@ __host__ __device__ constexpr uint32_t mma_idesc_f8(uint32_t a_format, uint32_t 
                                                     bool b_mn_major, uint32_t m, uint32_t n) {
     return (1u << 4) | (a_format << 7) | (b_format << 10) | (static_cast<uint32_t>(a_mn_major) << 15) |
            (static_cast<uint32_t>(b_mn_major) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// The same for block-scaled 4-bit operands (both e2m1, K-major).  e8m0: the
+// scales' type; scale_byte: which byte of a TMEM word holds an instruction's
+// first scale (0, or 2 for the upper two of four).
+//   bits 4-5 B's scale byte; 7-9 and 10-11 element format (1 = e2m1); 17-22
+//   N >> 3; 23 scale type (0 = e4m3, 1 = e8m0); 24-28 M >> 4; 29-30 A's scale byte.
+__host__ __device__ constexpr uint32_t mma_idesc_fp4(bool e8m0, uint32_t scale_byte, uint32_t m, uint32_t n) {
+    return (scale_byte << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (static_cast<uint32_t>(e8m0) << 23) |
+           ((m >> 4) << 24) | (scale_byte << 29);
+}
+
+// Shared-memory matrix descriptor without swizzle, for tmem_copy_scales: 8
+// rows of 16 bytes lie together, the next 8 rows 128 bytes further.
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>(128u >> 4) << 16;
+    d |= static_cast<uint64_t>(128u >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    return d;
 }
 
 // Store four f32 to another CTA's shared memory of the cluster

@@ -1,0 +1,319 @@
+"""4-bit blocks and their product on the GPU against plain computations.
+
+The quantiser is compared bit for bit with a float64 computation on the CPU:
+a tensor scale and an e8m0 scale are powers of two and a code's border times
+the scale has at most seven bits, so every comparison below is exact.  Products
+of integers whose sums stay below 2^24 of their least step are exact in fp32
+and compared for equality.  Other products: each fp32 addition is off by at
+most 2^-23 of the sum of the terms' magnitudes (a truncating adder), so a
+K-term sum by (K + 4) 2^-23 sum |a b|, the tensor scales' product included; the
+result's rounding adds half a step, eps / 2 relative."""
+import pytest
+import torch
+
+import sptiles_b200 as st
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+E4, E8, CODES = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.float4_e2m1fn_x2
+LEVELS = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+BLOCK = {E4: 16, E8: 32}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ------------------------------------------------------------------ plain forms
+def nearest(y, levels):
+    """Index of the level nearest to y >= 0; ties to the even index; above the last, the last."""
+    lv = torch.tensor(levels, dtype=torch.float64)
+    hi = torch.searchsorted(lv, y.contiguous()).clamp(max=len(levels) - 1)
+    lo = (hi - 1).clamp(min=0)
+    up, down = lv[hi] - y, y - lv[lo]
+    return torch.where((up < down) | ((up == down) & (hi % 2 == 0)), hi, lo)
+
+
+E4M3 = [m * 2.0 ** -9 for m in range(8)] + [(8 + m) * 2.0 ** (e - 10) for e in range(1, 16) for m in range(8)][:-1]
+
+
+def least_power(top, limit, least):
+    e = least
+    while limit * 2.0 ** e < top:
+        e += 1
+    return e
+
+
+def plain_quantize(x, scale_dtype, amax=None):
+    """(codes 0..15 [rows, cols], scale bytes [rows, blocks], tensor scale) in float64."""
+    x = x.double()
+    rows, cols = x.shape
+    b = BLOCK[scale_dtype]
+    parts = torch.nn.functional.pad(x, (0, -cols % b)).view(rows, -1, b)
+    top = parts.abs().amax(2)
+    bad = ~torch.isfinite(top)
+    if b == 16:
+        m = x[torch.isfinite(x)].abs().max().item() if amax is None else amax
+        t = 2.0 ** least_power(m, 2688.0, -126) if m > 0 else 1.0
+        byte = nearest(torch.where(bad, 0.0, top) / (6 * t), E4M3)
+        unit = torch.tensor(E4M3, dtype=torch.float64)[byte] * t
+        byte = torch.where(bad, 0x7f, byte)
+    else:
+        t = None
+        e = torch.tensor([[least_power(0.0 if not torch.isfinite(v) else v.item(), 6.0, -127) for v in row] for row in top])
+        byte, unit = torch.where(bad, 255, e + 127), torch.pow(torch.tensor(2.0, dtype=torch.float64), e.double())
+    live = unit > 0
+    q = torch.where(bad[:, :, None], 0.0, parts) / torch.where(live, unit, 1.0)[:, :, None]
+    code = nearest(q.abs(), LEVELS) + 8 * torch.signbit(parts)
+    code = torch.where(live[:, :, None], code, code & 8)
+    return code.view(rows, -1)[:, :cols], byte, t, bad.repeat_interleave(b, 1)[:, :cols]
+
+
+def tiled(byte):
+    rows, blocks = byte.shape
+    byte = torch.nn.functional.pad(byte.to(torch.uint8), (0, -blocks % 4, 0, -rows % 128))
+    return byte.view(-(-rows // 128), 4, 32, -(-blocks // 4), 4).permute(0, 3, 2, 1, 4).contiguous()
+
+
+def untiled(scale, rows, blocks):
+    byte = scale.view(torch.uint8).cpu()
+    i, j = byte.shape[:2]
+    return byte.permute(0, 3, 2, 1, 4).reshape(128 * i, 4 * j)[:rows, :blocks]
+
+
+def split(codes, cols):
+    byte = codes.view(torch.uint8).cpu()
+    return torch.stack((byte & 15, byte >> 4), 2).flatten(1), cols
+
+
+def check_quantize(x, scale_dtype, amax=None, where=None):
+    got = st.quantize_fp4(x.to(DEV) if where is None else where, scale_dtype=scale_dtype,
+                          amax=None if amax is None else torch.tensor(amax, device=DEV))
+    code, byte, t, bad = plain_quantize(x, scale_dtype, amax)
+    rows, cols = x.shape
+    assert got.codes.dtype == CODES and got.codes.shape == (rows, (cols + 1) // 2) and got.scale.dtype == scale_dtype
+    assert (got.tensor_scale is None) == (t is None)
+    if t is not None:
+        assert got.tensor_scale.item() == t
+    assert torch.equal(got.scale.view(torch.uint8).cpu(), tiled(byte))  # zeros where no row or block is
+    halves, _ = split(got.codes, cols)
+    assert (halves[:, cols:] == 0).all()
+    assert torch.equal(torch.where(bad, 0, halves[:, :cols].long()), torch.where(bad, 0, code.long()))
+    return got
+
+
+SRC = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.mark.parametrize("scale_dtype", [E4, E8], ids=["16", "32"])
+@pytest.mark.parametrize("src", SRC, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 16), (3, 33), (127, 64), (128, 128), (130, 257), (301, 136), (5, 4096)])
+def test_quantize_bits(rows, cols, src, scale_dtype):
+    x = (torch.randn(rows, cols, generator=gen(rows + cols)) * torch.exp(2 * torch.randn(rows, 1, generator=gen(7)))).to(src)
+    check_quantize(x, scale_dtype)
+
+
+@pytest.mark.parametrize("scale_dtype", [E4, E8], ids=["16", "32"])
+@pytest.mark.parametrize("src", SRC, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("view", ["transposed", "transposed offset", "strided", "offset", "broadcast", "broadcast column"])
+def test_quantize_views(view, src, scale_dtype):
+    base = torch.randn(301, 406, generator=gen(3)).to(src)
+    cut = {"transposed": lambda t: t.t(), "transposed offset": lambda t: t[1:, 1:].t(), "strided": lambda t: t[::2, ::3],
+           "offset": lambda t: t[1:, 1:], "broadcast": lambda t: t[:1].expand(140, -1),
+           "broadcast column": lambda t: t[:, :1].expand(-1, 50)}[view]
+    check_quantize(cut(base), scale_dtype, where=cut(base.to(DEV)))
+
+
+@pytest.mark.parametrize("src", SRC, ids=["f32", "f16", "bf16"])
+def test_quantize_borders(src):
+    """Every border between two codes times every scale mantissa, and the elements next to it."""
+    borders = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]
+    rows = []
+    for m in range(8, 16):
+        s = torch.tensor(m / 8, dtype=src)
+        at = torch.tensor(borders, dtype=src) * s
+        inf, zero = torch.tensor(float("inf"), dtype=src), torch.tensor(0.0, dtype=src)
+        if src == torch.bfloat16:  # no nextafter: one step of its bits
+            near = (at.view(torch.int16) + 1).view(src), (at.view(torch.int16) - 1).view(src)
+        else:
+            near = torch.nextafter(at.float(), inf.float()).to(src) if src == torch.float32 else (at.view(torch.int16) + 1).view(src), \
+                torch.nextafter(at.float(), zero.float()) if src == torch.float32 else (at.view(torch.int16) - 1).view(src)
+        for v in (at, *near):
+            for sign in (1, -1):
+                row = torch.zeros(16, dtype=src)
+                row[:7], row[15] = sign * v, 6 * s
+                rows.append(row)
+    x = torch.stack(rows)
+    x = torch.cat((x, 448 * x / 1.75), 1) if src == torch.float32 else x
+    check_quantize(x, E4, amax=2688.0)
+    check_quantize(x, E4, amax=2688.0, where=x.t().contiguous().to(DEV).t())
+    check_quantize(x.repeat(1, 2), E8)
+
+
+def test_quantize_extremes():
+    """Zero, subnormal, huge, infinite and NaN blocks; saturation at a known maximum; tensors near the ends of fp32."""
+    x = torch.zeros(8, 64)
+    x[1, 5], x[2], x[3, 0], x[4, 40] = 1e-45, 3e38, float("inf"), float("nan")
+    x[5, :4], x[6], x[7] = torch.tensor([448.0, 17.0, 19.0, -21.0]), -0.0, 2.0 ** -130
+    for dtype in (E4, E8):
+        check_quantize(x, dtype)
+        check_quantize(x[[0, 1, 5, 6, 7]] * 2.0 ** -100, dtype)
+        check_quantize(x[[0, 6]], dtype)
+        check_quantize(torch.randn(40, 100, generator=gen(5)) * 2.0 ** -120, dtype)
+        check_quantize(torch.randn(40, 100, generator=gen(5)) * 2.0 ** 124, dtype)
+    got = check_quantize(torch.tensor([[100.0] * 16 + [1.0] * 16]), E4, amax=8.0)
+    back = st.dequantize_fp4(got.codes, got.scale, got.tensor_scale, out_dtype=torch.float32)
+    assert back[0, 0].item() == 6 * 448 * got.tensor_scale.item() < 100.0
+    bad = st.dequantize_fp4(*check_quantize(x, E4))
+    assert torch.isnan(bad[3, :16]).all() and torch.isnan(bad[4, 32:48]).all() and not torch.isnan(bad[4, 48:]).any()
+
+
+def test_quantize_empty():
+    for shape in [(0, 5), (5, 0), (0, 0)]:
+        for dtype in (E4, E8):
+            q = st.quantize_fp4(torch.empty(shape, device=DEV), scale_dtype=dtype)
+            assert q.codes.shape == (shape[0], (shape[1] + 1) // 2)
+            assert q.scale.shape == (-(-shape[0] // 128), -(-(-(-shape[1] // BLOCK[dtype])) // 4), 32, 4, 4)
+            assert q.tensor_scale is None or q.tensor_scale.item() == 1.0
+            assert st.dequantize_fp4(*q, cols=shape[1]).shape == shape
+
+
+def test_quantize_large():
+    """A tensor whose second pass walks many units a thread, and whose maximum lies in its last element."""
+    x = torch.randn(4096, 2050, generator=gen(1)).to(torch.bfloat16)
+    x[-1, -1] = 300.0
+    got = st.quantize_fp4(x.to(DEV))
+    assert got.tensor_scale.item() == 0.125
+    take = [0, 1, 127, 128, 2047, 4095]
+    code, byte, t, _ = plain_quantize(x[take], E4, amax=300.0)
+    assert torch.equal(split(got.codes, 2050)[0][take][:, :2050].long(), code.long())
+    assert torch.equal(untiled(got.scale, 4096, 129)[take].long(), byte.long())
+
+
+# ------------------------------------------------------------------ back to values
+def values(code, byte, t, scale_dtype):
+    level = torch.tensor(LEVELS + [-v for v in LEVELS], dtype=torch.float64)[code.long()]
+    scale = byte.to(torch.uint8).view(scale_dtype).double().repeat_interleave(BLOCK[scale_dtype], 1)[:, : code.shape[1]]
+    return level * scale * (1.0 if t is None else t)
+
+
+@pytest.mark.parametrize("scale_dtype", [E4, E8], ids=["16", "32"])
+@pytest.mark.parametrize("cols", [1, 15, 31, 64, 333])
+def test_dequantize(cols, scale_dtype):
+    x = torch.randn(140, cols, generator=gen(cols))
+    q = st.quantize_fp4(x.to(DEV), scale_dtype=scale_dtype)
+    code, byte, t, _ = plain_quantize(x, scale_dtype)
+    want = values(code, byte, t, scale_dtype)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):  # one rounding; exact in the first two
+        assert torch.equal(st.dequantize_fp4(*q, cols=cols, out_dtype=dtype).cpu(), want.float().to(dtype))
+    wide = st.dequantize_fp4(*q, out_dtype=torch.float32)
+    assert wide.shape == (140, cols + cols % 2) and (cols % 2 == 0 or (wide[:, -1] == 0).all())
+    for turned in (q.codes.view(torch.uint8).t().contiguous().t(), q.codes.contiguous()):
+        assert torch.equal(st.dequantize_fp4(turned, *q[1:], cols=cols, out_dtype=torch.float32).cpu(), want.float())
+
+
+def test_dequantize_any_tensor_scale():
+    q = st.quantize_fp4(torch.randn(3, 48, generator=gen(1)).to(DEV))
+    t = torch.tensor([0.3], device=DEV)
+    code = split(q.codes, 48)[0]
+    want = values(code, untiled(q.scale, 3, 3), None, E4)
+    unit = (want.float() != 0)
+    got = st.dequantize_fp4(q.codes, q.scale, t, out_dtype=torch.float32).cpu()
+    # scale * t and its product with the code: two roundings of half a step
+    assert ((got.double() - want * t.cpu().double()).abs() <= 2.0 ** -23 * (want * 0.3).abs() * 1.0001)[unit].all()
+
+
+# ------------------------------------------------------------------ the product
+def random_operand(rows, cols, scale_dtype, seed):
+    """Codes and scales at random, with the values they stand for; scales 0.5, 1 or 2."""
+    g = gen(seed)
+    b = BLOCK[scale_dtype]
+    code = torch.randint(0, 16, (rows, cols), generator=g)
+    power = torch.randint(-1, 2, (rows, -(-cols // b)), generator=g)
+    byte = torch.pow(2.0, power).to(scale_dtype).view(torch.uint8)
+    padded = torch.nn.functional.pad(code, (0, cols % 2)).to(torch.uint8)
+    return padded[:, 0::2] | (padded[:, 1::2] << 4), tiled(byte).view(scale_dtype), values(code, byte, None, scale_dtype)
+
+
+def aligned(codes):
+    """Rows on 16-byte boundaries, as quantize_fp4 lays them out."""
+    room = torch.full((codes.shape[0], (codes.shape[1] + 15) // 16 * 16), 0x77, dtype=torch.uint8, device=DEV)
+    room[:, : codes.shape[1]] = codes.to(DEV)
+    return room[:, : codes.shape[1]].view(CODES)
+
+
+SHAPES = [(1, 1, 1), (1, 128, 64), (1, 500, 2048), (2, 129, 33), (16, 256, 256), (17, 100, 130), (33, 515, 512), (64, 128, 4096),
+          (65, 127, 63), (128, 128, 1000), (200, 300, 255), (257, 129, 257), (300, 513, 96), (1000, 520, 1111), (1, 4100, 6000)]
+
+
+@pytest.mark.parametrize("scale_dtype", [E4, E8], ids=["16", "32"])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_product_exact(m, n, k, scale_dtype):
+    qa, sa, va = random_operand(m, k, scale_dtype, 1)
+    qb, sb, vb = random_operand(n, k, scale_dtype, 2)
+    want = (va @ vb.t()).float()
+    a, b, sa, sb = aligned(qa), aligned(qb).t(), sa.to(DEV), sb.to(DEV)
+    assert torch.equal(st.matmul_fp4(a, b, sa, sb, out_dtype=torch.float32).cpu(), want)
+    # operands off every boundary, and stored across K: copied first
+    off = torch.zeros(qa.shape[0], qa.shape[1] + 1, dtype=torch.uint8, device=DEV)[:, 1:]
+    off.copy_(qa)
+    assert torch.equal(st.matmul_fp4(off, qb.t().contiguous().to(DEV), sa, sb, out_dtype=torch.float32).cpu(), want)
+    bias = torch.randint(-8, 8, (n,), generator=gen(3)).float()
+    got = st.matmul_fp4(a, b, sa, sb, bias.to(DEV), out_dtype=torch.float32)
+    assert torch.equal(got.cpu(), want + bias)
+    for dtype in (torch.bfloat16, torch.float16):
+        got = st.matmul_fp4(a, b, sa, sb, bias.to(dtype).to(DEV), out_dtype=dtype)
+        assert torch.equal(got.cpu(), (want + bias).to(dtype))
+    if scale_dtype == E4:
+        t = torch.tensor(0.25, device=DEV), torch.tensor([4.0], device=DEV)
+        got = st.matmul_fp4(a, b, sa, sb, bias.to(DEV), a_tensor_scale=t[0], out_dtype=torch.float32)
+        assert torch.equal(got.cpu(), 0.25 * want + bias)
+        got = st.matmul_fp4(a, b, sa, sb, a_tensor_scale=t[0], b_tensor_scale=t[1], out_dtype=torch.float32)
+        assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("scale_dtype", [E4, E8], ids=["16", "32"])
+@pytest.mark.parametrize("m,n,k", [(3, 700, 900), (130, 257, 1025), (1024, 512, 2048)])
+def test_product_of_quantised(m, n, k, scale_dtype):
+    """What quantize_fp4 makes, multiplied, against float64 on the values it stands for."""
+    x = torch.randn(m, k, generator=gen(1)) * torch.exp(torch.randn(m, 1, generator=gen(2)))
+    w = torch.randn(n, k, generator=gen(3))
+    xq, wq = (st.quantize_fp4(t.to(torch.bfloat16).to(DEV), scale_dtype=scale_dtype) for t in (x, w))
+    vx, vw = (st.dequantize_fp4(*q, cols=k, out_dtype=torch.float32).double() for q in (xq, wq))
+    want, size = vx @ vw.t(), vx.abs() @ vw.abs().t()
+    ts = {} if scale_dtype == E8 else dict(a_tensor_scale=xq.tensor_scale, b_tensor_scale=wq.tensor_scale)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = st.matmul_fp4(xq.codes, wq.codes.t(), xq.scale, wq.scale, out_dtype=dtype, **ts).double()
+        slack = (k + 4) * 2.0 ** -23 * size
+        assert ((got - want).abs() <= slack + torch.finfo(dtype).eps / 2 * (want.abs() + slack)).all()
+
+
+def test_product_nan_stays_in_its_row_and_column():
+    x, w = torch.randn(40, 128, generator=gen(1)), torch.randn(300, 128, generator=gen(2))
+    x[7, 100], w[129, 3] = float("nan"), float("inf")
+    for dtype in (E4, E8):
+        a, b = st.quantize_fp4(x.to(DEV), scale_dtype=dtype), st.quantize_fp4(w.to(DEV), scale_dtype=dtype)
+        c = st.matmul_fp4(a.codes, b.codes.t(), a.scale, b.scale, out_dtype=torch.float32)
+        nan = torch.isnan(c)
+        assert nan[7].all() and nan[:, 129].all()
+        nan[7] = nan[:, 129] = False
+        assert not nan.any()
+
+
+def test_product_empty_and_given_output():
+    for m, n, k in [(0, 5, 64), (5, 0, 64), (5, 7, 0)]:
+        qa, sa, _ = random_operand(m, k, E4, 1)
+        qb, sb, _ = random_operand(n, k, E4, 2)
+        bias = torch.arange(n, dtype=torch.float32, device=DEV)
+        c = st.matmul_fp4(qa.to(DEV), qb.to(DEV).t(), sa.to(DEV), sb.to(DEV), bias)
+        assert c.shape == (m, n) and torch.equal(c.float(), bias.expand(m, n))
+    for m, n in [(70, 200), (1, 333), (300, 260)]:
+        qa, sa, va = random_operand(m, 320, E4, 1)
+        qb, sb, vb = random_operand(n, 320, E4, 2)
+        for dtype in (torch.float32, torch.bfloat16):
+            room = torch.full((m + 2, n + 9), 7.0, dtype=dtype, device=DEV)
+            out = room[1 : m + 1, 3 : n + 3]
+            assert st.matmul_fp4(aligned(qa), aligned(qb).t(), sa.to(DEV), sb.to(DEV), out=out) is out
+            assert torch.equal(out.cpu(), (va @ vb.t()).to(dtype))
+            out.fill_(7.0)
+            assert (room == 7).all()
