@@ -50,7 +50,7 @@ constexpr int kMaxGroups = kGroupedMaxGroups;
 constexpr int kBK = 64;  // elements of the contraction a stage: 128 bytes, one swizzle span
 constexpr int kMmaK = 16;
 constexpr int kBarBytes = 512;
-constexpr int kPitch = 36;  // floats of a staged row of 32: 16-byte reads and writes without bank conflicts
+constexpr int kOutWarps = 4;  // warps that take C out, one for each quarter of the TMEM lanes
 
 struct GroupedParams {
     const int *ends;
@@ -63,10 +63,18 @@ struct GroupedParams {
     int64_t c_g, ldc;    // weights: D's strides of groups and rows
     int c_dtype;
     int zero_rest;       // rows of no group are set to 0
+    int r_by_64, c_by_64;  // the operand's map splits its columns in 64s, so that one box holds two of them
     int reads;           // there is something to sum over: the maps are valid
     uint32_t idesc;
     int *err;
     unsigned long long timeout_ns;
+};
+
+// Maps of the column operand with boxes of 32, 64, 96 and 128 rows: a stage's
+// rows come in one box.  (Four boxes of 32 cost more than one of 128: 16384 x
+// 4096 x 4096 421 us against 355.)  The second form uses the first one only.
+struct ColumnMaps {
+    CUtensorMap by32[4];
 };
 
 // ends[g] clipped to [ends[g - 1], rows], and the tiles up to and with group g.
@@ -139,7 +147,7 @@ struct TileWalk {
         out.rows = rows;
         if constexpr (WEIGHTS) {
             out.c0 = c * COLS;
-            out.cols = p.n - out.c0 < COLS ? p.n - out.c0 : COLS;
+            out.cols = p.k - out.c0 < COLS ? p.k - out.c0 : COLS;
             out.blocks = (rows + kBK - 1) / kBK;
         } else {
             const int even = ((rows + tiles_c - 1) / tiles_c + 15) / 16 * 16;  // columns of the group's tiles
@@ -152,45 +160,38 @@ struct TileWalk {
     }
 };
 
-// A warp's 32 x 32 values, staged [row][kPitch], to C: `rows` x `cols` of them
-// are inside.  c points at the first one.  16-byte pieces where C allows.
-template <typename T>
-__device__ __forceinline__ void store_box(T *c, int64_t ldc, const float *box, int rows, int cols, bool wide, int lane) {
-    constexpr int kPer = 16 / static_cast<int>(sizeof(T)), kLanes = 32 / kPer;  // elements a piece, pieces a row
-    if (wide && cols >= 32) {
-        const int piece = lane % kLanes;
+// 128 columns (64s of a swizzle span each) x 64 rows of an operand that lies
+// along its columns.  y and z: the map's other coordinates.  (Two boxes a
+// stage and operand instead of one: weights of 4096 x 4096 from 16384 rows
+// 433 us, in one 367.)
+template <bool PAIR>
+__device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap *map, uint32_t bar, int col, int y, int z, bool by_64,
+                                             uint64_t pol) {
+    if (by_64) {
+        if constexpr (PAIR) tma_load_4d_pair(dst, map, bar, 0, y, z, col / 64, pol);
+        else tma_load_4d(dst, map, bar, 0, y, z, col / 64, pol);
+    } else {
 #pragma unroll
-        for (int r = lane / kLanes; r < 32; r += 32 / kLanes) {
-            if (r >= rows) break;
-            alignas(16) T o[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer; i += 4) {
-                const float4 v = *reinterpret_cast<const float4 *>(box + r * kPitch + piece * kPer + i);
-                from_float(v.x, o[i]);
-                from_float(v.y, o[i + 1]);
-                from_float(v.z, o[i + 2]);
-                from_float(v.w, o[i + 3]);
-            }
-            *reinterpret_cast<uint4 *>(c + r * ldc + piece * kPer) = *reinterpret_cast<const uint4 *>(o);
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (PAIR) tma_load_3d_pair(dst + i * 64 * 128, map, bar, col + 64 * i, y, z, pol);
+            else tma_load_3d(dst + i * 64 * 128, map, bar, col + 64 * i, y, z, pol);
         }
-    } else if (lane < cols) {
-        for (int r = 0; r < rows && r < 32; ++r) from_float(box[r * kPitch + lane], c[r * ldc + lane]);
     }
 }
 
-// A warp's 32 TMEM lanes, `cols` columns of them, to C.  ACROSS: the lanes lie
-// along C's rows (n) and the columns are rows of C; else the lanes are rows of C.
-// `at`: the element of lane 0 and column 0; `lanes` of the lanes are inside C.
-// zero: there was nothing to sum.
-template <bool ACROSS>
-__device__ __forceinline__ void store_tile(const GroupedParams &p, int64_t at, uint32_t taddr, float *box, int lanes, int cols,
-                                           bool zero, int lane) {
-    const int es = p.c_dtype == ST_F32 ? 4 : 2;
-    const int64_t next = (ACROSS ? 32 * p.ldc : 32) * es;  // bytes from 32 columns to the next
-    uint8_t *base = static_cast<uint8_t *>(p.c) + at * es;
-    const bool wide = reinterpret_cast<uintptr_t>(base) % 16 == 0 && p.ldc * es % 16 == 0;
-#pragma unroll 1
-    for (int c = 0; c < cols; c += 32, base += next) {
+// ---- C.  The TMEM lanes lie along C's rows and the columns are rows of C, so
+// that a register of a warp is 32 neighbouring elements, stored as they are.
+// (Through shared memory and 16-byte stores, or TMA stores, was slower: the
+// loads' way into the SM is what bounds the kernels.  Weights of 32 x 2048 x
+// 4096 f32 from 16384 rows 318 us by TMA stores, 293 by 16-byte stores.)
+//
+// `cols` columns of a warp's 32 TMEM lanes.  at: the element of C of lane 0 and column 0; `lanes` of the lanes are inside.  zero:
+// there was nothing to sum.  released(): the accumulator has been read.
+template <typename T, typename Released>
+__device__ __forceinline__ void store_tile(const GroupedParams &p, int64_t at, uint32_t taddr, int lanes, int cols, bool zero,
+                                           int lane, Released released) {
+    if (lanes <= 0) cols = 0;
+    for (int c = 0; c < cols; c += 32) {
         uint32_t v[32];
         if (!zero) {
             tmem_load_32(taddr + static_cast<uint32_t>(c), v);
@@ -199,21 +200,27 @@ __device__ __forceinline__ void store_tile(const GroupedParams &p, int64_t at, u
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0u;
         }
-        __syncwarp();  // the last 32 columns have left the box
-        if constexpr (ACROSS) {
+        if (c + 32 >= cols) released();
+        if (lane >= lanes) continue;
+        T *to = static_cast<T *>(p.c) + at + c * p.ldc + lane;
+        if (cols - c >= 32) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) box[i * kPitch + lane] = __uint_as_float(v[i]);
+            for (int i = 0; i < 32; ++i, to += p.ldc) from_float(__uint_as_float(v[i]), *to);
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<uint4 *>(box + lane * kPitch + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            for (int i = 0; i < 32; ++i, to += p.ldc)
+                if (i < cols - c) from_float(__uint_as_float(v[i]), *to);
         }
-        __syncwarp();
-        const int rows = ACROSS ? cols - c : lanes, width = ACROSS ? lanes : cols - c;
-        if (p.c_dtype == ST_F32) store_box(reinterpret_cast<float *>(base), p.ldc, box, rows, width, wide, lane);
-        else if (p.c_dtype == ST_F16) store_box(reinterpret_cast<__half *>(base), p.ldc, box, rows, width, wide, lane);
-        else store_box(reinterpret_cast<__nv_bfloat16 *>(base), p.ldc, box, rows, width, wide, lane);
     }
+    if (cols <= 0) released();
+}
+
+template <typename Released>
+__device__ __forceinline__ void store_any_tile(const GroupedParams &p, int64_t at, uint32_t taddr, int lanes, int cols, bool zero,
+                                               int lane, Released released) {
+    if (p.c_dtype == ST_F32) store_tile<float>(p, at, taddr, lanes, cols, zero, lane, released);
+    else if (p.c_dtype == ST_F16) store_tile<__half>(p, at, taddr, lanes, cols, zero, lane, released);
+    else store_tile<__nv_bfloat16>(p, at, taddr, lanes, cols, zero, lane, released);
 }
 
 // Rows [first, p.rows) of C, which belong to no group, become 0.
@@ -231,29 +238,26 @@ __device__ __forceinline__ void zero_rows(const GroupedParams &p, int first, int
 template <int BN>
 struct GroupedCfg {
     static constexpr int kRows = 128;
-    static constexpr int kOutWarps = 4;
     static constexpr int kThreads = 32 * (2 + kOutWarps);
     static constexpr int kRowBytes = kRows * kBK * 2;
     static constexpr int kColBytes = BN * kBK * 2;
     static constexpr int kStageBytes = kRowBytes + kColBytes;
     static constexpr int kStages = BN == 128 ? 6 : 9;
     static constexpr int kTmemCols = 2 * BN;
-    static constexpr int kBoxBytes = 32 * kPitch * 4;
     static constexpr int kSmemBytes =
-        kStages * kStageBytes + kOutWarps * kBoxBytes + static_cast<int>(sizeof(GroupTable)) + kBarBytes + 1024;
+        kStages * kStageBytes + static_cast<int>(sizeof(GroupTable)) + kBarBytes + 1024;
     static_assert(kSmemBytes <= 232448, "over the per-block shared memory limit");
 };
 
 template <int BN, bool WEIGHTS, bool R_MN>
 __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
-    gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
+    gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ ColumnMaps maps_c,
                         const GroupedParams p) {
     using Cfg = GroupedCfg<BN>;
     static_assert(!WEIGHTS || R_MN, "both operands of the second form lie along their columns");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *boxes = smem + Cfg::kStages * Cfg::kStageBytes;
-    GroupTable &table = *reinterpret_cast<GroupTable *>(boxes + Cfg::kOutWarps * Cfg::kBoxBytes);
+    GroupTable &table = *reinterpret_cast<GroupTable *>(smem + Cfg::kStages * Cfg::kStageBytes);
     uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(&table) + sizeof(GroupTable));
     constexpr int kBars = 2 * Cfg::kStages + 5;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
@@ -275,7 +279,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), Cfg::kOutWarps);
+            mbar_init(tempty_bar(a), kOutWarps);
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
     }
     if (warp == 0 && lane == 0 && p.reads) {
         tma_prefetch_map(&tmap_r);
-        tma_prefetch_map(&tmap_c);
+        tma_prefetch_map(&maps_c.by32[0]);
     }
     if (warp == 1) {
         tmem_alloc(smem_addr(tmem_slot), Cfg::kTmemCols);
@@ -306,7 +310,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
             uint32_t ph = 0;
             bool ok = true;
             while (ok && walk.next(table, p, tile)) {
-                const int boxes_c = (tile.cols + 31) / 32;
+                const int high = (tile.cols + 31) / 32;  // rows of the column operand's box, in 32
                 for (int b = 0; b < tile.blocks; ++b, ++issued) {
                     if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
                         ok = false;
@@ -317,22 +321,18 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
                     if constexpr (WEIGHTS) {
                         mbar_arrive_expect_tx(fb, Cfg::kStageBytes);
                         const int left = tile.rows - b * kBK, y = left < kBK ? left - kBK : 0, z = tile.first + b * kBK;
-#pragma unroll
-                        for (int i = 0; i < Cfg::kRows / 64; ++i)
-                            tma_load_3d(sr + i * 64 * 128, &tmap_r, fb, tile.r0 + 64 * i, y, z, pol);
-#pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) tma_load_3d(sc + i * 64 * 128, &tmap_c, fb, tile.c0 + 64 * i, y, z, pol);
+                        static_assert(!WEIGHTS || BN == 128, "columns in two 64s");
+                        load_columns<false>(sr, &tmap_r, fb, tile.r0, y, z, p.r_by_64, pol);
+                        load_columns<false>(sc, &maps_c.by32[0], fb, tile.c0, y, z, p.c_by_64, pol);
                     } else {
-                        mbar_arrive_expect_tx(fb, static_cast<uint32_t>(Cfg::kRowBytes + boxes_c * 32 * 128));
+                        mbar_arrive_expect_tx(fb, static_cast<uint32_t>(Cfg::kRowBytes + high * 32 * 128));
                         const int g = p.b_groups ? tile.group : 0;
                         if constexpr (R_MN) {
-#pragma unroll
-                            for (int i = 0; i < Cfg::kRows / 64; ++i)
-                                tma_load_3d(sr + i * 64 * 128, &tmap_r, fb, tile.r0 + 64 * i, b * kBK, g, pol);
+                            load_columns<false>(sr, &tmap_r, fb, tile.r0, b * kBK, g, p.r_by_64, pol);
                         } else {
                             tma_load_3d(sr, &tmap_r, fb, b * kBK, tile.r0, g, pol);
                         }
-                        for (int i = 0; i < boxes_c; ++i) tma_load_2d(sc + i * 32 * 128, &tmap_c, fb, b * kBK, tile.c0 + 32 * i, pol);
+                        tma_load_2d(sc, &maps_c.by32[high - 1], fb, b * kBK, tile.c0, pol);
                     }
                     if (++s == Cfg::kStages) {
                         s = 0;
@@ -396,7 +396,6 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
     } else {
         // ------------------------------------------------ C
         const int g = warp & 3;
-        float *box = reinterpret_cast<float *>(boxes + g * Cfg::kBoxBytes);
         int a = 0;
         uint32_t aph = 0;
         while (walk.next(table, p, tile)) {
@@ -409,24 +408,22 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
                 }
                 tc_fence_after_sync();
             }
-            const int lanes = (WEIGHTS ? p.k : p.n) - tile.r0 - 32 * g;
-            const int64_t at = WEIGHTS ? tile.group * p.c_g + (tile.r0 + 32 * g) * p.ldc + tile.c0
-                                       : tile.c0 * p.ldc + tile.r0 + 32 * g;
-            if (lanes > 0)
-                store_tile<!WEIGHTS>(p, at, tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(a * BN), box,
-                                     lanes < 32 ? lanes : 32, tile.cols, zero, lane);
-            if (!zero) {
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(tempty_bar(a));
-                if (++a == 2) {
-                    a = 0;
-                    aph ^= 1u;
-                }
+            const int r = tile.r0 + 32 * g;
+            const int64_t at = (WEIGHTS ? tile.group * p.c_g : 0) + tile.c0 * p.ldc + r;
+            store_any_tile(p, at, tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(a * BN), p.n - r,
+                           tile.cols, zero, lane, [&] {
+                               if (zero) return;
+                               tc_fence_before_sync();
+                               __syncwarp();
+                               if (lane == 0) mbar_arrive(tempty_bar(a));
+                           });
+            if (!zero && ++a == 2) {
+                a = 0;
+                aph ^= 1u;
             }
         }
         if (!WEIGHTS && p.zero_rest)
-            zero_rows<32 * Cfg::kOutWarps>(p, p.groups > 0 ? table.row_end[p.groups - 1] : 0, (warp - 2) * 32 + lane);
+            zero_rows<32 * kOutWarps>(p, p.groups > 0 ? table.row_end[p.groups - 1] : 0, (warp - 2) * 32 + lane);
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -447,29 +444,26 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
 // even CTA and counts the pair's warps that read accumulators.
 struct GroupedPairCfg {
     static constexpr int kRows = 256, kCols = 256;
-    static constexpr int kOutWarps = 4;
     static constexpr int kThreads = 32 * (2 + kOutWarps);
     static constexpr int kRowBytes = 128 * kBK * 2;
     static constexpr int kColBytes = 128 * kBK * 2;
     static constexpr int kStageBytes = kRowBytes + kColBytes;
     static constexpr int kStages = 6;
     static constexpr int kTmemCols = 2 * kCols;
-    static constexpr int kBoxBytes = 32 * kPitch * 4;
     static constexpr int kSmemBytes =
-        kStages * kStageBytes + kOutWarps * kBoxBytes + static_cast<int>(sizeof(GroupTable)) + kBarBytes + 1024;
+        kStages * kStageBytes + static_cast<int>(sizeof(GroupTable)) + kBarBytes + 1024;
     static_assert(kSmemBytes <= 232448, "over the per-block shared memory limit");
 };
 
 template <bool WEIGHTS, bool R_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThreads, 1)
-    gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
+    gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ ColumnMaps maps_c,
                              const GroupedParams p) {
     using Cfg = GroupedPairCfg;
     static_assert(!WEIGHTS || R_MN, "both operands of the second form lie along their columns");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *boxes = smem + Cfg::kStages * Cfg::kStageBytes;
-    GroupTable &table = *reinterpret_cast<GroupTable *>(boxes + Cfg::kOutWarps * Cfg::kBoxBytes);
+    GroupTable &table = *reinterpret_cast<GroupTable *>(smem + Cfg::kStages * Cfg::kStageBytes);
     uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(&table) + sizeof(GroupTable));
     constexpr int kBars = 2 * Cfg::kStages + 5;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
@@ -492,7 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), 2 * Cfg::kOutWarps);
+            mbar_init(tempty_bar(a), 2 * kOutWarps);
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -500,7 +494,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
     }
     if (warp == 0 && lane == 0 && p.reads) {
         tma_prefetch_map(&tmap_r);
-        tma_prefetch_map(&tmap_c);
+        tma_prefetch_map(&maps_c.by32[0]);
     }
     if (warp == 1) {
         tmem_alloc_pair(smem_addr(tmem_slot), Cfg::kTmemCols);
@@ -526,8 +520,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
             uint32_t ph = 0;
             bool ok = true;
             while (ok && walk.next(table, p, tile)) {
-                // each CTA brings half of the tile's columns (rows of A), in boxes of 32
-                const int half_c = (tile.cols + 15) / 16 * 8, boxes_c = (half_c + 31) / 32;
+                // each CTA brings half of the tile's columns (rows of A)
+                const int half_c = (tile.cols + 15) / 16 * 8, high = (half_c + 31) / 32;
                 for (int b = 0; b < tile.blocks; ++b, ++issued) {
                     if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
                         ok = false;
@@ -538,25 +532,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
                     if constexpr (WEIGHTS) {
                         if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * Cfg::kStageBytes);
                         const int left = tile.rows - b * kBK, y = left < kBK ? left - kBK : 0, z = tile.first + b * kBK;
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            tma_load_3d_pair(sr + i * 64 * 128, &tmap_r, fb, tile.r0 + half + 64 * i, y, z, pol);
-                            tma_load_3d_pair(sc + i * 64 * 128, &tmap_c, fb, tile.c0 + half + 64 * i, y, z, pol);
-                        }
+                        load_columns<true>(sr, &tmap_r, fb, tile.r0 + half, y, z, p.r_by_64, pol);
+                        load_columns<true>(sc, &maps_c.by32[0], fb, tile.c0 + half, y, z, p.c_by_64, pol);
                     } else {
                         if (rank == 0)
-                            mbar_arrive_expect_tx(full_bar(s), static_cast<uint32_t>(2 * (Cfg::kRowBytes + boxes_c * 32 * 128)));
+                            mbar_arrive_expect_tx(full_bar(s), static_cast<uint32_t>(2 * (Cfg::kRowBytes + high * 32 * 128)));
                         const int g = p.b_groups ? tile.group : 0;
                         if constexpr (R_MN) {
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-                                tma_load_3d_pair(sr + i * 64 * 128, &tmap_r, fb, tile.r0 + half + 64 * i, b * kBK, g, pol);
+                            load_columns<true>(sr, &tmap_r, fb, tile.r0 + half, b * kBK, g, p.r_by_64, pol);
                         } else {
                             tma_load_3d_pair(sr, &tmap_r, fb, b * kBK, tile.r0 + half, g, pol);
                         }
-                        const int c0 = tile.c0 + static_cast<int>(rank) * half_c;
-                        for (int i = 0; i < boxes_c; ++i)
-                            tma_load_2d_pair(sc + i * 32 * 128, &tmap_c, fb, b * kBK, c0 + 32 * i, pol);
+                        tma_load_2d_pair(sc, &maps_c.by32[high - 1], fb, b * kBK, tile.c0 + static_cast<int>(rank) * half_c, pol);
                     }
                     if (++s == Cfg::kStages) {
                         s = 0;
@@ -624,7 +611,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
         // ------------------------------------------------ C (both CTAs)
         const int g = warp & 3, row = static_cast<int>(rank) * 128 + 32 * g;
         const uint32_t even_tempty0 = map_to_rank(tempty_bar(0), 0);
-        float *box = reinterpret_cast<float *>(boxes + g * Cfg::kBoxBytes);
         int a = 0;
         uint32_t aph = 0;
         while (walk.next(table, p, tile)) {
@@ -637,26 +623,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
                 }
                 tc_fence_after_sync();
             }
-            const int lanes = (WEIGHTS ? p.k : p.n) - tile.r0 - row;
-            const int64_t at = WEIGHTS ? tile.group * p.c_g + (tile.r0 + row) * p.ldc + tile.c0 : tile.c0 * p.ldc + tile.r0 + row;
-            if (lanes > 0)
-                store_tile<!WEIGHTS>(p, at, tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(a * Cfg::kCols),
-                                     box, lanes < 32 ? lanes : 32, tile.cols, zero, lane);
-            if (!zero) {
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) {
-                    if (rank == 0) mbar_arrive(tempty_bar(a));
-                    else mbar_arrive_cluster(even_tempty0 + 8u * a);
-                }
-                if (++a == 2) {
-                    a = 0;
-                    aph ^= 1u;
-                }
+            const int r = tile.r0 + row;
+            const int64_t at = (WEIGHTS ? tile.group * p.c_g : 0) + tile.c0 * p.ldc + r;
+            store_any_tile(p, at, tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(a * Cfg::kCols), p.n - r,
+                           tile.cols, zero, lane, [&] {
+                               if (zero) return;
+                               tc_fence_before_sync();
+                               __syncwarp();
+                               if (lane == 0) {
+                                   if (rank == 0) mbar_arrive(tempty_bar(a));
+                                   else mbar_arrive_cluster(even_tempty0 + 8u * a);
+                               }
+                           });
+            if (!zero && ++a == 2) {
+                a = 0;
+                aph ^= 1u;
             }
         }
         if (!WEIGHTS && p.zero_rest)
-            zero_rows<32 * Cfg::kOutWarps>(p, p.groups > 0 ? table.row_end[p.groups - 1] : 0, (warp - 2) * 32 + lane);
+            zero_rows<32 * kOutWarps>(p, p.groups > 0 ? table.row_end[p.groups - 1] : 0, (warp - 2) * 32 + lane);
     }
     tc_fence_before_sync();
     __syncwarp();
@@ -764,8 +749,20 @@ int make_map_16(CUtensorMap *map, int dtype, const char *what, int rank, const v
                            data, dims, strides, box);
 }
 
+// (column, y, z) for load_columns: whole 64s as (column in a 64, y, z, 64), any other as three dimensions.
+int make_map_columns(CUtensorMap *map, int *by_64, int dtype, const char *what, const void *data, int64_t cols, int64_t y, int64_t z,
+                     int64_t sy, int64_t sz) {
+    *by_64 = cols % 64 == 0;
+    if (!*by_64) return make_map_16(map, dtype, what, 3, data, cols, y, z, sy, sz, 64, kBK);
+    const cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(y), static_cast<cuuint64_t>(z), static_cast<cuuint64_t>(cols / 64)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(sy * 2), static_cast<cuuint64_t>(sz * 2), 128};
+    const cuuint32_t box[4] = {64, kBK, 1, 2};
+    return make_tensor_map(map, what, dtype == ST_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, data,
+                           dims, strides, box);
+}
+
 template <int BN, bool WEIGHTS, bool R_MN>
-int launch_instance(const CUtensorMap &mr, const CUtensorMap &mc, const GroupedParams &p, int64_t most_tiles, int sm_count,
+int launch_instance(const CUtensorMap &mr, const ColumnMaps &mc, const GroupedParams &p, int64_t most_tiles, int sm_count,
                     cudaStream_t stream) {
     using Cfg = GroupedCfg<BN>;
     auto kern = gemm_grouped_kernel<BN, WEIGHTS, R_MN>;
@@ -782,7 +779,7 @@ int launch_instance(const CUtensorMap &mr, const CUtensorMap &mc, const GroupedP
 }
 
 template <bool WEIGHTS, bool R_MN>
-int launch_pair_instance(const CUtensorMap &mr, const CUtensorMap &mc, const GroupedParams &p, int64_t most_tiles, int sm_count,
+int launch_pair_instance(const CUtensorMap &mr, const ColumnMaps &mc, const GroupedParams &p, int64_t most_tiles, int sm_count,
                          cudaStream_t stream) {
     using Cfg = GroupedPairCfg;
     auto kern = gemm_grouped_pair_kernel<WEIGHTS, R_MN>;
@@ -796,6 +793,34 @@ int launch_pair_instance(const CUtensorMap &mr, const CUtensorMap &mc, const Gro
     const int64_t pairs = most_tiles < 1 ? 1 : most_tiles < sm_count / 2 ? most_tiles : sm_count / 2;
     ST_CUDA_TRY(launch_kernel(kern, static_cast<unsigned>(2 * pairs), Cfg::kThreads, Cfg::kSmemBytes, stream, mr, mc, p));
     return checked("gemm_grouped_pair_kernel");
+}
+
+// Tile shape: the least estimated time for groups of equal size (what the ends
+// hold is not known here).  A stage of 64 along the contraction costs an SM its
+// MMAs or its loads, whichever is longer; the figures are SM cycles.
+struct GroupedPlan {
+    bool pair = false;
+    int cols = 128;  // most columns of a tile
+    double cycles = 1e300;
+};
+
+GroupedPlan plan_grouped(const GroupedArgs &g, int sm_count) {
+    const int64_t met = g.groups < 1 ? 1 : !g.weights && g.rows < g.groups ? (g.rows > 0 ? g.rows : 1) : g.groups;
+    const int64_t per_group = cdiv(g.rows > 0 ? g.rows : 1, met);
+    GroupedPlan best;
+    auto offer = [&](bool pair, int cols) {
+        const int64_t extent = g.weights ? g.k : per_group, tiles_c = cdiv(extent, cols);
+        const double c = g.weights ? cols : static_cast<double>(cdiv(cdiv(extent, tiles_c), 16) * 16);
+        const int64_t tiles = met * tiles_c * cdiv(g.n, pair ? 256 : 128);
+        const double mma = 2 * c, load = 256 + (pair ? c : 2 * c);
+        const double t = static_cast<double>(cdiv(tiles, pair ? sm_count / 2 : sm_count)) *
+                         (static_cast<double>(cdiv(g.weights ? per_group : g.k, kBK)) * (mma > load ? mma : load) + 3000);
+        if (t < best.cycles) best = GroupedPlan{pair, cols, t};
+    };
+    if (!g.weights) offer(false, 32);
+    offer(false, 128);
+    offer(true, GroupedPairCfg::kCols);
+    return best;
 }
 
 }  // namespace
@@ -822,17 +847,16 @@ int launch_gemm_grouped(const GroupedArgs &g, void *workspace, int sm_count, int
     p.zero_rest = g.zero_rest;
     p.err = dev_err;
     p.timeout_ns = timeout_ns;
-    // rows of the group, on average: the columns of a tile
-    const int64_t per_group = cdiv(g.rows, g.groups > 0 ? g.groups : 1), extent_r = g.weights ? g.k : g.n;
-    const bool pair = extent_r > 128 && (g.weights ? g.n > 128 : per_group > 64);
-    const int rows = pair ? GroupedPairCfg::kRows : 128;
-    const int cols = pair ? GroupedPairCfg::kCols : g.weights || per_group > 32 ? 128 : 32;
-    p.tiles_r = static_cast<int>(cdiv(extent_r, rows));
-    p.tiles_c = static_cast<int>(cdiv(g.n, cols));
+    const GroupedPlan plan = plan_grouped(g, sm_count);
+    const bool pair = plan.pair;
+    const int rows = pair ? GroupedPairCfg::kRows : 128, cols = plan.cols;
+    p.tiles_r = static_cast<int>(cdiv(g.n, rows));
+    p.tiles_c = static_cast<int>(cdiv(g.k, cols));
     const int64_t most = g.weights ? g.groups * p.tiles_r * p.tiles_c
                                    : (cdiv(g.rows, cols) + (g.groups < g.rows ? g.groups : g.rows)) * p.tiles_r;
     if (most > INT32_MAX / 2) return fail(ST_ERR_UNSUPPORTED, "matmul_grouped: too many output tiles");
-    CUtensorMap mr{}, mc{};
+    CUtensorMap mr{};
+    ColumnMaps mc{};
     Operands o{};
     o.b_mn = g.weights;
     // with nothing to sum over (k = 0, no groups, or no rows) no operand is read
@@ -844,11 +868,12 @@ int launch_gemm_grouped(const GroupedArgs &g, void *workspace, int sm_count, int
         if (g.weights) {
             // (column, position in a step of 64 rows, the step's first row): positions reach behind the last
             // row in the map's extents, but no step's box does
-            ST_TRY(make_map_16(&mr, g.dtype, "A", 3, o.a.data, g.k, kBK, g.rows, o.a.so, o.a.so, 64, kBK));
-            ST_TRY(make_map_16(&mc, g.dtype, "C", 3, o.b.data, g.n, kBK, g.rows, o.b.so, o.b.so, 64, kBK));
+            ST_TRY(make_map_columns(&mr, &p.r_by_64, g.dtype, "C", o.b.data, g.n, kBK, g.rows, o.b.so, o.b.so));
+            ST_TRY(make_map_columns(&mc.by32[0], &p.c_by_64, g.dtype, "A", o.a.data, g.k, kBK, g.rows, o.a.so, o.a.so));
         } else {
-            ST_TRY(make_map_16(&mc, g.dtype, "A", 2, o.a.data, g.k, g.rows, 1, o.a.so, 0, kBK, 32));
-            if (o.b_mn) ST_TRY(make_map_16(&mr, g.dtype, "B", 3, o.b.data, g.n, g.k, o.b.groups, o.b.so, o.b.sg, 64, kBK));
+            for (int i = 0; i < 4; ++i)
+                ST_TRY(make_map_16(&mc.by32[i], g.dtype, "A", 2, o.a.data, g.k, g.rows, 1, o.a.so, 0, kBK, 32 * (i + 1)));
+            if (o.b_mn) ST_TRY(make_map_columns(&mr, &p.r_by_64, g.dtype, "B", o.b.data, g.n, g.k, o.b.groups, o.b.so, o.b.sg));
             else ST_TRY(make_map_16(&mr, g.dtype, "B", 3, o.b.data, g.k, g.n, o.b.groups, o.b.so, o.b.sg, kBK, 128));
         }
         p.b_groups = o.b_groups;

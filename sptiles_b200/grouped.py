@@ -58,6 +58,13 @@ def _workspace(name: str, like: torch.Tensor, da: bytes, db: bytes, *args: int) 
     return (torch.empty(need, dtype=torch.uint8, device=like.device) if need else None), need
 
 
+def _on_16(t: torch.Tensor) -> bool:
+    """Read in place as it is: contiguous rows, everything on 16-byte boundaries (16-bit elements)."""
+    st = t.stride()
+    return (st[-1] == 1 and st[-2] % 8 == 0 and st[-2] >= t.shape[-1] and t.data_ptr() % 16 == 0 and
+            (len(st) == 2 or st[0] % 8 == 0 and st[0] > 0))
+
+
 def matmul_grouped(A: torch.Tensor, B: torch.Tensor, ends: torch.Tensor, *, out_dtype: torch.dtype | None = None,
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """C [T, N]: C[r] = A[r] @ B[g] for the rows r of each group g.
@@ -88,7 +95,9 @@ def matmul_grouped(A: torch.Tensor, B: torch.Tensor, ends: torch.Tensor, *, out_
         out, dc = _new(A, rows, cols, max(cols, 1), 1, out_dtype)
     else:
         dc = _desc(out)
-    workspace, need = _workspace("st_matmul_grouped_workspace", A, da, db, stride, groups)
+    workspace, need = None, 0
+    if not (_on_16(A) and (_on_16(B) or _on_16(B.transpose(1, 2)))):
+        workspace, need = _workspace("st_matmul_grouped_workspace", A, da, db, stride, groups)
     fn = _fns.get("st_matmul_grouped") or _fn("st_matmul_grouped", _vp, _cp, _cp, _i64, _cp, _cp, _i32, _vp, _u64, _cp)
     rc = fn(context(dev), da, db, stride, de, dc, fresh, None if workspace is None else workspace.data_ptr(), need,
             _exec_desc(dev))
@@ -121,7 +130,9 @@ def matmul_grouped_weights(A: torch.Tensor, C: torch.Tensor, ends: torch.Tensor,
             raise ValueError(f"unsupported dtype {out_dtype}")
         out = A.new_empty((groups, A.shape[1], C.shape[1]), dtype=out_dtype)
     dd, stride = _stack_desc(out, groups, "out")
-    workspace, need = _workspace("st_matmul_grouped_weights_workspace", A, da, dc, groups)
+    workspace, need = None, 0
+    if not (_on_16(A) and _on_16(C)):
+        workspace, need = _workspace("st_matmul_grouped_weights_workspace", A, da, dc, groups)
     fn = _fns.get("st_matmul_grouped_weights") or _fn("st_matmul_grouped_weights", _vp, _cp, _cp, _cp, _cp, _i64, _vp, _u64, _cp)
     rc = fn(context(dev), da, dc, de, dd, stride, None if workspace is None else workspace.data_ptr(), need, _exec_desc(dev))
     if rc != N.ST_OK:
