@@ -345,6 +345,290 @@ __global__ void __launch_bounds__(Fp4Cfg<BN>::kThreads, BN == 128 ? 1 : 2)
     }
 }
 
+// ---------------------------------------------------------------- CTA pairs, 256 x 256 tiles
+// The large products.  A pair of CTAs (cta_group::2) computes 256 x 256 of C,
+// B's columns as its rows, so that the TMEM lanes lie along C's rows and C is
+// stored from registers as it is: each CTA holds 128 rows of the row operand
+// and 128 of the column operand, and the scales of its rows and of all columns.
+//
+// TMEM: two accumulators of 256 columns and the scales do not fit 512 columns,
+// so the accumulators share 96: [0, 256) and [160, 416).  A tile's shared
+// columns are read first, and the next tile's MMAs start when that is done.
+// The scales of a stage (48 columns) have two places behind them, taken in
+// turn; a place is written again once the MMAs that read it are done.
+//
+// full[s] lives in the even CTA and counts both CTAs' loads; the even CTA's
+// MMA warp commits empty[s] and tfull to both CTAs; tfree lives in the even CTA
+// and counts the pair's warps that have read the shared columns.
+struct Fp4PairCfg {
+    static constexpr int kRows = 256, kCols = 256;
+    static constexpr int kOutWarps = 8;
+    static constexpr int kThreads = 32 * (2 + kOutWarps);
+    static constexpr int kRowBytes = 128 * kBlockK;
+    static constexpr int kColBytes = 128 * kBlockK;
+    static constexpr int kRowScaleBytes = kChunks * kAtomBytes;
+    static constexpr int kColScaleBytes = 2 * kChunks * kAtomBytes;
+    static constexpr int kStageBytes = kRowBytes + kColBytes + kRowScaleBytes + kColScaleBytes;
+    static constexpr int kStages = 5;
+    static constexpr int kAccStep = 160;
+    static constexpr int kScaleCol = kAccStep + kCols, kScaleCols = 12 * kChunks;
+    static constexpr int kTmemCols = 512;
+    static_assert(kScaleCol + 2 * kScaleCols <= kTmemCols, "accumulators and scales fit");
+    static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + 1024;
+    static_assert(kSmemBytes <= 232448, "over the per-block shared memory limit");
+};
+
+// First row and column of tile t: 8 column tiles of a row tile after another,
+// so that the tiles in flight share their operands in L2.
+__device__ __forceinline__ void pair_tile(const Fp4Params &p, int t, int &r0, int &c0) {
+    constexpr int kBand = 8;
+    const int in_band = kBand * p.tiles_r;
+    const int first = t / in_band * kBand;
+    const int high = p.tiles_c - first < kBand ? p.tiles_c - first : kBand;
+    c0 = (first + t % in_band % high) * Fp4PairCfg::kCols;
+    r0 = t % in_band / high * Fp4PairCfg::kRows;
+}
+
+// 32 columns (rows of C) of a warp's lanes (its columns): alpha, bias, store.
+template <typename T>
+__device__ __forceinline__ void store_columns(T *to, int64_t ldc, const uint32_t (&v)[32], int cols, float alpha, float add) {
+    if (cols >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i, to += ldc) from_float(__fmaf_rn(__uint_as_float(v[i]), alpha, add), *to);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i, to += ldc)
+            if (i < cols) from_float(__fmaf_rn(__uint_as_float(v[i]), alpha, add), *to);
+    }
+}
+
+template <bool WIDE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp4PairCfg::kThreads, 1)
+    gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
+                         const __grid_constant__ CUtensorMap tmap_rs, const __grid_constant__ CUtensorMap tmap_cs,
+                         const Fp4Params p) {
+    using Cfg = Fp4PairCfg;
+    constexpr int kAtoms = WIDE ? 2 : 4;  // of a stage and 128 rows
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::kStages * Cfg::kStageBytes);
+    constexpr int kBars = 2 * Cfg::kStages + 6;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
+    const int tiles = p.tiles_r * p.tiles_c;
+    const uint32_t bar0 = smem_addr(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };
+    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + a); };
+    auto place_bar = [&](int i) { return bar0 + 8u * (2 * Cfg::kStages + 2 + i); };
+    const uint32_t tfree_bar = bar0 + 8u * (2 * Cfg::kStages + 4);
+    const uint32_t drain_bar = bar0 + 8u * (kBars - 1);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Cfg::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(tfull_bar(i), 1);
+            mbar_init(place_bar(i), 1);
+        }
+        mbar_init(tfree_bar, 2 * Cfg::kOutWarps);
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_map(&tmap_r);
+        tma_prefetch_map(&tmap_c);
+        tma_prefetch_map(&tmap_rs);
+        tma_prefetch_map(&tmap_cs);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_addr(tmem_slot), Cfg::kTmemCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_begin();  // nothing above touches global memory
+
+    if (warp == 0) {
+        // ------------------------------------------------ TMA producer (both CTAs)
+        if (lane == 0) {
+            const uint64_t pol = l2_policy_evict_last();
+            const uint32_t even_full0 = map_to_rank(full_bar(0), 0);
+            constexpr uint32_t kBytes = Cfg::kRowBytes + Cfg::kColBytes + 3 * kAtoms * kAtomBytes;
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                int r0, c0;
+                pair_tile(p, t, r0, c0);
+                const int half = static_cast<int>(rank) * 128;
+                for (int b = 0; b < p.k_blocks; ++b, ++issued) {
+                    if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * kBytes);
+                    const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes), sc = sr + Cfg::kRowBytes;
+                    const uint32_t srs = sc + Cfg::kColBytes, scs = srs + Cfg::kRowScaleBytes, fb = even_full0 + 8u * s;
+                    tma_load_2d_pair(sr, &tmap_r, fb, b * kBlockK, r0 + half, pol);
+                    tma_load_2d_pair(sc, &tmap_c, fb, b * kBlockK, c0 + half, pol);
+                    tma_load_3d_pair(srs, &tmap_rs, fb, 0, b * kAtoms, (r0 + half) / 128, pol);
+                    tma_load_3d_pair(scs, &tmap_cs, fb, 0, b * kAtoms, c0 / 128, pol);
+                    if (++s == Cfg::kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                atomicExch(p.err, kDevAbortGemmProducer);
+            }
+            if (rank == 0) drain_ring(issued, Cfg::kStages, full_bar, p.timeout_ns);  // both CTAs' copies
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issuer (even CTA)
+        if (rank == 0) {
+            int s = 0, a = 0, place = 0;
+            uint32_t ph = 0, fph = 0, pph = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                // the last tile's shared columns have been read (and so has the whole one before it)
+                if (!__all_sync(0xffffffffu, mbar_wait(tfree_bar, fph ^ 1u, abort_flag, p.timeout_ns))) {
+                    ok = false;
+                    break;
+                }
+                fph ^= 1u;
+                const uint32_t acc = tmem_base + static_cast<uint32_t>(a * Cfg::kAccStep);
+                for (int b = 0; b < p.k_blocks; ++b) {
+                    const bool ready = mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns) &&
+                                       mbar_wait(place_bar(place), pph ^ 1u, abort_flag, p.timeout_ns);
+                    if (!__all_sync(0xffffffffu, ready)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    if (elect_one()) {
+                        const int left = p.k_chunks - b * kChunks, n = left < kChunks ? left : kChunks;
+                        const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes), sc = sr + Cfg::kRowBytes;
+                        const uint32_t srs = sc + Cfg::kColBytes, scs = srs + Cfg::kRowScaleBytes;
+                        const uint32_t tr_s = tmem_base + static_cast<uint32_t>(Cfg::kScaleCol + place * Cfg::kScaleCols);
+                        const uint32_t tc_s = tr_s + 4 * kChunks;
+                        const uint64_t dr = smem_desc_sw128(sr, 16, 1024), dc = smem_desc_sw128(sc, 16, 1024);
+                        const uint64_t drs = smem_desc_scales(srs), dcs = smem_desc_scales(scs);
+#pragma unroll
+                        for (uint32_t i = 0; i < kAtoms; ++i) {
+                            tmem_copy_scales_pair(tr_s + 4 * i, drs + i * (kAtomBytes >> 4));
+                            tmem_copy_scales_pair(tc_s + 8 * i, dcs + i * (kAtomBytes >> 4));
+                            tmem_copy_scales_pair(tc_s + 8 * i + 4, dcs + (kAtoms + i) * (kAtomBytes >> 4));
+                        }
+#pragma unroll
+                        for (int j = 0; j < kChunks; ++j) {
+                            const uint32_t atom = static_cast<uint32_t>(WIDE ? j / 2 : j);
+                            if (j < n)
+                                tc_mma_fp4_pair<WIDE ? 2 : 4>(acc, dr + j * 2u, dc + j * 2u, p.idesc[WIDE ? j % 2 : 0], tr_s + 4 * atom,
+                                                              tc_s + 8 * atom, b + j != 0 ? 1u : 0u);
+                        }
+                        tc_commit_pair_multicast(empty_bar(s), 3);
+                        tc_commit_pair(place_bar(place));
+                        if (b + 1 == p.k_blocks) tc_commit_pair_multicast(tfull_bar(a), 3);
+                    }
+                    __syncwarp();
+                    if (++s == Cfg::kStages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                    place ^= 1;
+                    if (place == 0) pph ^= 1u;
+                }
+                a ^= 1;
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                if (lane == 0) atomicExch(p.err, kDevAbortGemmMma);
+            }
+            if (elect_one()) tc_commit_pair(drain_bar);
+            __syncwarp();
+            drain_ring(1, 1, [&](int) { return drain_bar; }, p.timeout_ns);  // the MMAs read shared memory and write TMEM
+        }
+    } else {
+        // ------------------------------------------------ C (both CTAs)
+        const int g = warp & 3, side = (warp - 2) >> 2;  // two warps for each quarter of the lanes
+        const uint32_t even_tfree = map_to_rank(tfree_bar, 0);
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(g * 32) << 16);
+        const float alpha = (p.ta != nullptr ? *p.ta : 1.0f) * (p.tb != nullptr ? *p.tb : 1.0f);
+        int a = 0;
+        uint32_t aph = 0;
+        for (int t = pair; t < tiles; t += pairs) {
+            int r0, c0;
+            pair_tile(p, t, r0, c0);
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns))) {
+                *abort_flag = 1;
+                if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
+                break;
+            }
+            tc_fence_after_sync();
+            const uint32_t acc = t_lane + static_cast<uint32_t>(a * Cfg::kAccStep);
+            const int row = r0 + static_cast<int>(rank) * 128 + 32 * g + lane;  // of the row operand: a column of C
+            const float add = p.bias != nullptr && row < p.rows ? load_any(p.bias, p.bias_dtype, row) : 0.0f;
+            // this warp's four 32s of columns, the shared ones (160 to 255, or 0 to 95) first
+            const int first = a == 0 ? 5 : 0;
+#pragma unroll 1
+            for (int step = 0; step < 4; step += 2) {
+                // shared: 0 and 1 of them by side 0, 2 by side 1 with the first of the others; then two each
+                const int i0 = side == 0 ? (step == 0 ? 0 : 3) : (step == 0 ? 2 : 6), i1 = side == 0 ? (step == 0 ? 1 : 4) : (step == 0 ? 5 : 7);
+                const int at0 = 32 * ((first + i0) % 8), at1 = 32 * ((first + i1) % 8);
+                uint32_t v[2][32];
+                tmem_load_32(acc + static_cast<uint32_t>(at0), v[0]);
+                tmem_load_32(acc + static_cast<uint32_t>(at1), v[1]);
+                tmem_load_wait();
+                if (step == 0) {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (rank == 0) mbar_arrive(tfree_bar);
+                        else mbar_arrive_cluster(even_tfree);
+                    }
+                }
+                if (row < p.rows) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int col = c0 + (h == 0 ? at0 : at1), left = p.cols - col;
+                        if (left <= 0) continue;
+                        const int64_t at = col * p.c_c + row;
+                        if (p.c_dtype == ST_F32) store_columns(static_cast<float *>(p.c) + at, p.c_c, v[h], left, alpha, add);
+                        else if (p.c_dtype == ST_F16) store_columns(static_cast<__half *>(p.c) + at, p.c_c, v[h], left, alpha, add);
+                        else store_columns(static_cast<__nv_bfloat16 *>(p.c) + at, p.c_c, v[h], left, alpha, add);
+                    }
+                }
+                __syncwarp();  // TMEM is read by whole warps
+            }
+            a ^= 1;
+            if (a == 0) aph ^= 1u;
+        }
+    }
+
+    tc_fence_before_sync();
+    __syncwarp();
+    cluster_sync();  // all MMAs retired, all TMEM reads done, no remote arrival pending
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    }
+}
+
 __global__ void __launch_bounds__(256) fill_bias_kernel(void *c, int64_t ldc, int c_dtype, const void *bias, int bias_dtype,
                                                         int64_t m, int64_t n) {
     pdl_wait();
@@ -405,6 +689,35 @@ int launch_tile(const CUtensorMap &mr, const CUtensorMap &mc, const Fp4Params &p
     return wide ? launch_instance<BN, true>(mr, mc, p, stream) : launch_instance<BN, false>(mr, mc, p, stream);
 }
 
+// An operand's scales, [row / 128][block / 4] of 512 bytes, in boxes of a stage's of `tiles` times 128 rows.
+int make_map_scales(CUtensorMap *map, const void *base, int64_t rows, int64_t quads, int atoms, int tiles) {
+    const cuuint64_t dims[3] = {kAtomBytes / 4, static_cast<cuuint64_t>(quads), static_cast<cuuint64_t>(cdiv(rows, 128))};
+    const cuuint64_t strides[2] = {kAtomBytes, static_cast<cuuint64_t>(quads) * kAtomBytes};
+    const cuuint32_t box[3] = {kAtomBytes / 4, static_cast<cuuint32_t>(atoms), static_cast<cuuint32_t>(tiles)};
+    return make_tensor_map(map, "scales of a 4-bit operand", CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, base, dims, strides, box,
+                           CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <bool WIDE>
+int launch_pair(const CUtensorMap &mr, const CUtensorMap &mc, const CUtensorMap &mrs, const CUtensorMap &mcs, const Fp4Params &p,
+                int sm_count, cudaStream_t stream) {
+    auto kern = gemm_fp4_pair_kernel<WIDE>;
+    static uint64_t attr_set = 0;  // one bit per device ordinal
+    int dev = 0;
+    ST_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !(attr_set & (1ull << dev))) {
+        ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp4PairCfg::kSmemBytes));
+        if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
+    }
+    const int64_t tiles = static_cast<int64_t>(p.tiles_r) * p.tiles_c;
+    const int64_t pairs = tiles < sm_count / 2 ? tiles : sm_count / 2;
+    ST_CUDA_TRY(launch_kernel(kern, static_cast<unsigned>(2 * pairs), Fp4PairCfg::kThreads, Fp4PairCfg::kSmemBytes, stream, mr, mc, mrs,
+                              mcs, p));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "gemm_fp4_pair_kernel launch");
+}
+
 // TMA reads an operand in place if its rows lie along K on 16-byte boundaries
 // and do not overlap; any other is copied first.
 struct Access {
@@ -421,11 +734,16 @@ Access access_of(const Fp4Operand &o) {
 int64_t copy_bytes(const Fp4Operand &o, const Access &a) { return a.copy ? (o.rows * a.ld + 255) / 256 * 256 : 0; }
 
 struct Fp4Plan {
+    bool pair = false, swap = false;  // swap: B is the row operand
     int bn = 128, split = 1;
 };
 
-Fp4Plan plan_fp4(int64_t rows, int64_t cols, int64_t k_blocks, int sm_count) {
+Fp4Plan plan_fp4(int64_t m, int64_t n, int64_t k_blocks, int sm_count) {
     Fp4Plan best;
+    best.pair = m > 128 && n > 128 && cdiv(m, 256) * cdiv(n, 256) * 4 >= sm_count;
+    best.swap = best.pair || m <= 64;
+    if (best.pair) return best;
+    const int64_t rows = best.swap ? n : m, cols = best.swap ? m : n;
     best.bn = cols <= 16 ? 16 : cols <= 32 ? 32 : cols <= 64 ? 64 : 128;
     const int64_t tiles = cdiv(rows, kTileRows) * cdiv(cols, best.bn), slots = static_cast<int64_t>(sm_count) * (best.bn == 128 ? 1 : 2);
     while (best.split < 8 && tiles * best.split * 2 <= slots && best.split * 4 <= k_blocks) best.split *= 2;
@@ -460,19 +778,18 @@ int launch_gemm_fp4(const GemmFp4Args &g, void *workspace, int sm_count, int *de
         ws += copy_bytes(op[i], acc[i]);
     }
     const int64_t k_blocks = cdiv(k, kBlockK);
-    // few rows of A make the columns of a narrow tile, against 128 rows of B
-    const bool swap = m <= 64;
+    const Fp4Plan plan = plan_fp4(m, n, k_blocks, sm_count);
+    const bool swap = plan.swap;
     const int ri = swap ? 1 : 0, ci = swap ? 0 : 1;
     const Fp4Operand &r = op[ri], &c = op[ci];
-    const Fp4Plan plan = plan_fp4(r.rows, c.rows, k_blocks, sm_count);
     Fp4Params p{};
     p.rows = static_cast<int>(r.rows);
     p.cols = static_cast<int>(c.rows);
     p.k_blocks = static_cast<int>(k_blocks);
     p.k_chunks = static_cast<int>(cdiv(k, 32));
     p.quads = static_cast<int>(cdiv(cdiv(k, g.wide ? 16 : 8), 4));
-    p.tiles_r = static_cast<int>(cdiv(r.rows, kTileRows));
-    p.tiles_c = static_cast<int>(cdiv(c.rows, plan.bn));
+    p.tiles_r = static_cast<int>(cdiv(r.rows, plan.pair ? Fp4PairCfg::kRows : kTileRows));
+    p.tiles_c = static_cast<int>(cdiv(c.rows, plan.pair ? Fp4PairCfg::kCols : plan.bn));
     p.split = plan.split;
     if (static_cast<int64_t>(p.tiles_r) * p.tiles_c * p.split > INT32_MAX)
         return fail(ST_ERR_UNSUPPORTED, "matmul_fp4: too many output tiles");
@@ -487,12 +804,22 @@ int launch_gemm_fp4(const GemmFp4Args &g, void *workspace, int sm_count, int *de
     p.bias = g.bias;
     p.bias_dtype = g.bias_dtype;
     p.bias_on_rows = swap;
-    for (uint32_t i = 0; i < 2; ++i) p.idesc[i] = mma_idesc_fp4(g.wide, 2 * i, kTileRows, static_cast<uint32_t>(plan.bn));
+    for (uint32_t i = 0; i < 2; ++i)
+        p.idesc[i] = plan.pair ? mma_idesc_fp4(g.wide, 2 * i, Fp4PairCfg::kRows, Fp4PairCfg::kCols)
+                               : mma_idesc_fp4(g.wide, 2 * i, kTileRows, static_cast<uint32_t>(plan.bn));
     p.err = dev_err;
     p.timeout_ns = timeout_ns;
     CUtensorMap mr, mc;
     ST_TRY(make_map_4(&mr, "a 4-bit operand", r.data, k, r.rows, acc[ri].ld, kTileRows));
-    ST_TRY(make_map_4(&mc, "a 4-bit operand", c.data, k, c.rows, acc[ci].ld, plan.bn));
+    ST_TRY(make_map_4(&mc, "a 4-bit operand", c.data, k, c.rows, acc[ci].ld, plan.pair ? 128 : plan.bn));
+    if (plan.pair) {
+        CUtensorMap mrs, mcs;
+        const int atoms = g.wide ? 2 : 4;
+        ST_TRY(make_map_scales(&mrs, r.scale, r.rows, p.quads, atoms, 1));
+        ST_TRY(make_map_scales(&mcs, c.scale, c.rows, p.quads, atoms, 2));
+        return g.wide ? launch_pair<true>(mr, mc, mrs, mcs, p, sm_count, stream)
+                      : launch_pair<false>(mr, mc, mrs, mcs, p, sm_count, stream);
+    }
     switch (plan.bn) {
     case 16: return launch_tile<16>(mr, mc, p, g.wide, stream);
     case 32: return launch_tile<32>(mr, mc, p, g.wide, stream);

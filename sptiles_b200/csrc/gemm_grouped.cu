@@ -50,7 +50,7 @@ constexpr int kMaxGroups = kGroupedMaxGroups;
 constexpr int kBK = 64;  // elements of the contraction a stage: 128 bytes, one swizzle span
 constexpr int kMmaK = 16;
 constexpr int kBarBytes = 512;
-constexpr int kOutWarps = 4;  // warps that take C out, one for each quarter of the TMEM lanes
+constexpr int kOutWarps = 8;  // warps that take C out, two for each quarter of the TMEM lanes
 
 struct GroupedParams {
     const int *ends;
@@ -185,13 +185,14 @@ __device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap *ma
 // loads' way into the SM is what bounds the kernels.  Weights of 32 x 2048 x
 // 4096 f32 from 16384 rows 318 us by TMA stores, 293 by 16-byte stores.)
 //
-// `cols` columns of a warp's 32 TMEM lanes.  at: the element of C of lane 0 and column 0; `lanes` of the lanes are inside.  zero:
+// A warp's share (every other 32) of `cols` columns of 32 TMEM lanes.  at: the element of C of lane 0 and column 0; `lanes` of the lanes are inside.  zero:
 // there was nothing to sum.  released(): the accumulator has been read.
 template <typename T, typename Released>
 __device__ __forceinline__ void store_tile(const GroupedParams &p, int64_t at, uint32_t taddr, int lanes, int cols, bool zero,
                                            int lane, Released released) {
     if (lanes <= 0) cols = 0;
-    for (int c = 0; c < cols; c += 32) {
+    const int half = (static_cast<int>(threadIdx.x >> 5) - 2) >> 2;  // of the two warps of a quarter
+    for (int c = 32 * half; c < cols; c += 64) {
         uint32_t v[32];
         if (!zero) {
             tmem_load_32(taddr + static_cast<uint32_t>(c), v);
@@ -200,19 +201,21 @@ __device__ __forceinline__ void store_tile(const GroupedParams &p, int64_t at, u
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0u;
         }
-        if (c + 32 >= cols) released();
-        if (lane >= lanes) continue;
-        T *to = static_cast<T *>(p.c) + at + c * p.ldc + lane;
-        if (cols - c >= 32) {
+        if (c + 64 >= cols) released();
+        if (lane < lanes) {
+            T *to = static_cast<T *>(p.c) + at + c * p.ldc + lane;
+            if (cols - c >= 32) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i, to += p.ldc) from_float(__uint_as_float(v[i]), *to);
-        } else {
+                for (int i = 0; i < 32; ++i, to += p.ldc) from_float(__uint_as_float(v[i]), *to);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i, to += p.ldc)
-                if (i < cols - c) from_float(__uint_as_float(v[i]), *to);
+                for (int i = 0; i < 32; ++i, to += p.ldc)
+                    if (i < cols - c) from_float(__uint_as_float(v[i]), *to);
+            }
         }
+        __syncwarp();  // TMEM is read by whole warps
     }
-    if (cols <= 0) released();
+    if (32 * half >= cols) released();  // no share in this tile
 }
 
 template <typename Released>

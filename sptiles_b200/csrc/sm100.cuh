@@ -280,12 +280,41 @@ __device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t a_desc, uin
             : "memory");
 }
 
+// The same by a pair of CTAs: M = 256, each CTA with its own 128 rows' scales
+// of A and those of all columns of B in its TMEM.
+template <int SCALES>
+__device__ __forceinline__ void tc_mma_fp4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    static_assert(SCALES == 4 || SCALES == 2, "scales per row and instruction");
+    if constexpr (SCALES == 4)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+                d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+
 // 512 bytes of scales (128 rows x 4 along K, in the order [row % 32][row /
 // 32][4]) from shared memory into four TMEM columns: 32 lanes of 16 bytes,
 // repeated for the four lane quarters.  Ordered before the MMAs that the same
 // thread issues after it.
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// In both CTAs of a pair, each from its own shared memory at the descriptor's
+// address into its own TMEM; issued once, by the even CTA.
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 // True in one lane of a converged warp.  A warp that keeps together and

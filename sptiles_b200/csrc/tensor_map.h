@@ -26,15 +26,16 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     return fn;
 }
 
-// 128-byte-swizzled boxes of a tensor of `rank` dimensions, the first one
+// Boxes (128-byte-swizzled, unless told otherwise) of a tensor of `rank` dimensions, the first one
 // contiguous; strides in bytes, of the second dimension on.
 inline int make_tensor_map(CUtensorMap *map, const char *what, CUtensorMapDataType type, int rank, const void *base,
-                           const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+                           const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+                           CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     auto fn = tensor_map_encoder();
     if (!fn) return fail(ST_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
     const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
     const CUresult r = fn(map, type, static_cast<cuuint32_t>(rank), const_cast<void *>(base), dims, strides, box, ones,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return fail(ST_ERR_INVALID_ARGUMENT, std::string("cuTensorMapEncodeTiled rejected ") + what + " (error " +

@@ -288,6 +288,25 @@ def test_product_of_quantised(m, n, k, scale_dtype):
         assert ((got - want).abs() <= slack + torch.finfo(dtype).eps / 2 * (want.abs() + slack)).all()
 
 
+@pytest.mark.parametrize("scale_dtype", [E4, E8], ids=["16", "32"])
+@pytest.mark.parametrize("m,n,k", [(1500, 1700, 64), (2311, 1025, 700), (1024, 2560, 1601), (300, 5000, 33), (4100, 258, 2048),
+                                   (2560, 4096, 512)])
+def test_product_exact_large(m, n, k, scale_dtype):
+    """Many tiles: each CTA pair has several, cut at C's edges in both directions."""
+    qa, sa, va = random_operand(m, k, scale_dtype, 1)
+    qb, sb, vb = random_operand(n, k, scale_dtype, 2)
+    want = (va.to(DEV) @ vb.to(DEV).t()).float()
+    a, b, sa, sb = aligned(qa), aligned(qb).t(), sa.to(DEV), sb.to(DEV)
+    bias = torch.randint(-8, 8, (n,), generator=gen(3)).float().to(DEV)
+    assert torch.equal(st.matmul_fp4(a, b, sa, sb, out_dtype=torch.float32), want)
+    assert torch.equal(st.matmul_fp4(a, b, sa, sb, bias), (want + bias).to(torch.bfloat16))
+    room = torch.full((m + 2, n + 5), 7.0, dtype=torch.float16, device=DEV)
+    st.matmul_fp4(a, b, sa, sb, bias, out=room[1 : m + 1, 2 : n + 2])
+    assert torch.equal(room[1 : m + 1, 2 : n + 2], (want + bias).to(torch.float16))
+    room[1 : m + 1, 2 : n + 2] = 7.0
+    assert (room == 7).all()
+
+
 def test_product_nan_stays_in_its_row_and_column():
     x, w = torch.randn(40, 128, generator=gen(1)), torch.randn(300, 128, generator=gen(2))
     x[7, 100], w[129, 3] = float("nan"), float("inf")
