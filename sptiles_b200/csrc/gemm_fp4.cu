@@ -351,15 +351,21 @@ __global__ void __launch_bounds__(Fp4Cfg<BN>::kThreads, BN == 128 ? 1 : 2)
 // stored from registers as it is: each CTA holds 128 rows of the row operand
 // and 128 of the column operand, and the scales of its rows and of all columns.
 //
-// TMEM: two accumulators of 256 columns and the scales do not fit 512 columns,
-// so the accumulators share 96: [0, 256) and [160, 416).  A tile's shared
-// columns are read first, and the next tile's MMAs start when that is done.
-// The scales of a stage (48 columns) have two places behind them, taken in
-// turn; a place is written again once the MMAs that read it are done.
+// TMEM: a tile's sums take 256 columns, the scales of each stage 48 of their
+// own behind them (so that they are written again only after the MMAs that read
+// them have freed the stage).  There is no room for a second accumulator: eight
+// warps take a tile's sums into registers at once, and the next tile's MMAs
+// start when they have.
+//
+// What bounds the kernel is the warp that issues: a stage's 12 scale copies, 4
+// MMAs and their barriers take it about as long as the 512 cycles of the MMAs.
+// So it keeps together, its operands in uniform registers (the warp's index and
+// the TMEM address are broadcast for that), and asks for the next stage's
+// barrier before it issues this one's MMAs.
 //
 // full[s] lives in the even CTA and counts both CTAs' loads; the even CTA's
 // MMA warp commits empty[s] and tfull to both CTAs; tfree lives in the even CTA
-// and counts the pair's warps that have read the shared columns.
+// and counts the pair's warps that have taken a tile's sums.
 struct Fp4PairCfg {
     static constexpr int kRows = 256, kCols = 256;
     static constexpr int kOutWarps = 8;
@@ -370,10 +376,9 @@ struct Fp4PairCfg {
     static constexpr int kColScaleBytes = 2 * kChunks * kAtomBytes;
     static constexpr int kStageBytes = kRowBytes + kColBytes + kRowScaleBytes + kColScaleBytes;
     static constexpr int kStages = 5;
-    static constexpr int kAccStep = 160;
-    static constexpr int kScaleCol = kAccStep + kCols, kScaleCols = 12 * kChunks;
+    static constexpr int kScaleCol = kCols, kScaleCols = 12 * kChunks;
     static constexpr int kTmemCols = 512;
-    static_assert(kScaleCol + 2 * kScaleCols <= kTmemCols, "accumulators and scales fit");
+    static_assert(kScaleCol + kStages * kScaleCols <= kTmemCols, "the accumulator and the scales fit");
     static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + 1024;
     static_assert(kSmemBytes <= 232448, "over the per-block shared memory limit");
 };
@@ -412,11 +417,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp4PairCfg::kThreads
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + Cfg::kStages * Cfg::kStageBytes);
-    constexpr int kBars = 2 * Cfg::kStages + 6;
+    constexpr int kBars = 2 * Cfg::kStages + 3;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
@@ -424,9 +429,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp4PairCfg::kThreads
     const uint32_t bar0 = smem_addr(bars);
     auto full_bar = [&](int s) { return bar0 + 8u * s; };
     auto empty_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };
-    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + a); };
-    auto place_bar = [&](int i) { return bar0 + 8u * (2 * Cfg::kStages + 2 + i); };
-    const uint32_t tfree_bar = bar0 + 8u * (2 * Cfg::kStages + 4);
+    const uint32_t tfull_bar = bar0 + 8u * (2 * Cfg::kStages), tfree_bar = tfull_bar + 8u;
     const uint32_t drain_bar = bar0 + 8u * (kBars - 1);
 
     if (threadIdx.x == 0) {
@@ -434,10 +437,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp4PairCfg::kThreads
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(tfull_bar(i), 1);
-            mbar_init(place_bar(i), 1);
-        }
+        mbar_init(tfull_bar, 1);
         mbar_init(tfree_bar, 2 * Cfg::kOutWarps);
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -457,7 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp4PairCfg::kThreads
     __syncthreads();
     cluster_sync();
     tc_fence_after_sync();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     pdl_begin();  // nothing above touches global memory
 
     if (warp == 0) {
@@ -500,59 +500,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp4PairCfg::kThreads
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer (even CTA)
         if (rank == 0) {
-            int s = 0, a = 0, place = 0;
-            uint32_t ph = 0, fph = 0, pph = 0;
-            bool ok = true;
+            const uint32_t ring = smem_addr(smem);
+            const uint64_t dr0 = smem_desc_sw128(ring, 16, 1024), dc0 = smem_desc_sw128(ring + Cfg::kRowBytes, 16, 1024);
+            const uint64_t drs0 = smem_desc_scales(ring + Cfg::kRowBytes + Cfg::kColBytes);
+            const uint64_t dcs0 = smem_desc_scales(ring + Cfg::kRowBytes + Cfg::kColBytes + Cfg::kRowScaleBytes);
+            int s = 0;
+            uint32_t ph = 0, fph = 0;
+            bool ok = true, there = false;  // there: this lane has seen stage s filled
             for (int t = pair; ok && t < tiles; t += pairs) {
-                // the last tile's shared columns have been read (and so has the whole one before it)
+                // the last tile's sums have been taken
                 if (!__all_sync(0xffffffffu, mbar_wait(tfree_bar, fph ^ 1u, abort_flag, p.timeout_ns))) {
                     ok = false;
                     break;
                 }
                 fph ^= 1u;
-                const uint32_t acc = tmem_base + static_cast<uint32_t>(a * Cfg::kAccStep);
                 for (int b = 0; b < p.k_blocks; ++b) {
-                    const bool ready = mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns) &&
-                                       mbar_wait(place_bar(place), pph ^ 1u, abort_flag, p.timeout_ns);
-                    if (!__all_sync(0xffffffffu, ready)) {
+                    if (!__all_sync(0xffffffffu, there || mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns))) {
                         ok = false;
                         break;
                     }
                     tc_fence_after_sync();
+                    const int next = s + 1 == Cfg::kStages ? 0 : s + 1;
+                    const uint32_t next_ph = next == 0 ? ph ^ 1u : ph;
+                    there = mbar_try_now(full_bar(next), next_ph);
                     if (elect_one()) {
-                        const int left = p.k_chunks - b * kChunks, n = left < kChunks ? left : kChunks;
-                        const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes), sc = sr + Cfg::kRowBytes;
-                        const uint32_t srs = sc + Cfg::kColBytes, scs = srs + Cfg::kRowScaleBytes;
-                        const uint32_t tr_s = tmem_base + static_cast<uint32_t>(Cfg::kScaleCol + place * Cfg::kScaleCols);
+                        const int left = p.k_chunks - b * kChunks;
+                        const uint64_t step = static_cast<uint64_t>(s) * (Cfg::kStageBytes >> 4);
+                        const uint32_t tr_s = tmem_base + static_cast<uint32_t>(Cfg::kScaleCol + s * Cfg::kScaleCols);
                         const uint32_t tc_s = tr_s + 4 * kChunks;
-                        const uint64_t dr = smem_desc_sw128(sr, 16, 1024), dc = smem_desc_sw128(sc, 16, 1024);
-                        const uint64_t drs = smem_desc_scales(srs), dcs = smem_desc_scales(scs);
 #pragma unroll
                         for (uint32_t i = 0; i < kAtoms; ++i) {
-                            tmem_copy_scales_pair(tr_s + 4 * i, drs + i * (kAtomBytes >> 4));
-                            tmem_copy_scales_pair(tc_s + 8 * i, dcs + i * (kAtomBytes >> 4));
-                            tmem_copy_scales_pair(tc_s + 8 * i + 4, dcs + (kAtoms + i) * (kAtomBytes >> 4));
+                            tmem_copy_scales_pair(tr_s + 4 * i, drs0 + step + i * (kAtomBytes >> 4));
+                            tmem_copy_scales_pair(tc_s + 8 * i, dcs0 + step + i * (kAtomBytes >> 4));
+                            tmem_copy_scales_pair(tc_s + 8 * i + 4, dcs0 + step + (kAtoms + i) * (kAtomBytes >> 4));
                         }
 #pragma unroll
                         for (int j = 0; j < kChunks; ++j) {
                             const uint32_t atom = static_cast<uint32_t>(WIDE ? j / 2 : j);
-                            if (j < n)
-                                tc_mma_fp4_pair<WIDE ? 2 : 4>(acc, dr + j * 2u, dc + j * 2u, p.idesc[WIDE ? j % 2 : 0], tr_s + 4 * atom,
-                                                              tc_s + 8 * atom, b + j != 0 ? 1u : 0u);
+                            if (j == 0 || j < left)
+                                tc_mma_fp4_pair<WIDE ? 2 : 4>(tmem_base, dr0 + step + j * 2u, dc0 + step + j * 2u,
+                                                              p.idesc[WIDE ? j % 2 : 0], tr_s + 4 * atom, tc_s + 8 * atom,
+                                                              j != 0 || b != 0 ? 1u : 0u);
                         }
                         tc_commit_pair_multicast(empty_bar(s), 3);
-                        tc_commit_pair(place_bar(place));
-                        if (b + 1 == p.k_blocks) tc_commit_pair_multicast(tfull_bar(a), 3);
+                        if (b + 1 == p.k_blocks) tc_commit_pair_multicast(tfull_bar, 3);
                     }
                     __syncwarp();
-                    if (++s == Cfg::kStages) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
-                    place ^= 1;
-                    if (place == 0) pph ^= 1u;
+                    s = next;
+                    ph = next_ph;
                 }
-                a ^= 1;
             }
             if (!ok) {
                 *abort_flag = 1;
@@ -568,54 +564,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp4PairCfg::kThreads
         const uint32_t even_tfree = map_to_rank(tfree_bar, 0);
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(g * 32) << 16);
         const float alpha = (p.ta != nullptr ? *p.ta : 1.0f) * (p.tb != nullptr ? *p.tb : 1.0f);
-        int a = 0;
-        uint32_t aph = 0;
-        for (int t = pair; t < tiles; t += pairs) {
+        uint32_t fph = 0;
+        for (int t = pair; t < tiles; t += pairs, fph ^= 1u) {
             int r0, c0;
             pair_tile(p, t, r0, c0);
-            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(a), aph, abort_flag, p.timeout_ns))) {
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar, fph, abort_flag, p.timeout_ns))) {
                 *abort_flag = 1;
                 if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
                 break;
             }
             tc_fence_after_sync();
-            const uint32_t acc = t_lane + static_cast<uint32_t>(a * Cfg::kAccStep);
-            const int row = r0 + static_cast<int>(rank) * 128 + 32 * g + lane;  // of the row operand: a column of C
-            const float add = p.bias != nullptr && row < p.rows ? load_any(p.bias, p.bias_dtype, row) : 0.0f;
-            // this warp's four 32s of columns, the shared ones (160 to 255, or 0 to 95) first
-            const int first = a == 0 ? 5 : 0;
-#pragma unroll 1
-            for (int step = 0; step < 4; step += 2) {
-                // shared: 0 and 1 of them by side 0, 2 by side 1 with the first of the others; then two each
-                const int i0 = side == 0 ? (step == 0 ? 0 : 3) : (step == 0 ? 2 : 6), i1 = side == 0 ? (step == 0 ? 1 : 4) : (step == 0 ? 5 : 7);
-                const int at0 = 32 * ((first + i0) % 8), at1 = 32 * ((first + i1) % 8);
-                uint32_t v[2][32];
-                tmem_load_32(acc + static_cast<uint32_t>(at0), v[0]);
-                tmem_load_32(acc + static_cast<uint32_t>(at1), v[1]);
-                tmem_load_wait();
-                if (step == 0) {
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (rank == 0) mbar_arrive(tfree_bar);
-                        else mbar_arrive_cluster(even_tfree);
-                    }
-                }
-                if (row < p.rows) {
+            uint32_t v[4][32];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int col = c0 + (h == 0 ? at0 : at1), left = p.cols - col;
-                        if (left <= 0) continue;
-                        const int64_t at = col * p.c_c + row;
-                        if (p.c_dtype == ST_F32) store_columns(static_cast<float *>(p.c) + at, p.c_c, v[h], left, alpha, add);
-                        else if (p.c_dtype == ST_F16) store_columns(static_cast<__half *>(p.c) + at, p.c_c, v[h], left, alpha, add);
-                        else store_columns(static_cast<__nv_bfloat16 *>(p.c) + at, p.c_c, v[h], left, alpha, add);
-                    }
-                }
-                __syncwarp();  // TMEM is read by whole warps
+            for (int i = 0; i < 4; ++i) tmem_load_32(t_lane + static_cast<uint32_t>(128 * side + 32 * i), v[i]);
+            tmem_load_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (rank == 0) mbar_arrive(tfree_bar);
+                else mbar_arrive_cluster(even_tfree);
             }
-            a ^= 1;
-            if (a == 0) aph ^= 1u;
+            const int row = r0 + static_cast<int>(rank) * 128 + 32 * g + lane;  // of the row operand: a column of C
+            if (row < p.rows) {
+                const float add = p.bias != nullptr ? load_any(p.bias, p.bias_dtype, row) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int col = c0 + 128 * side + 32 * i, left = p.cols - col;
+                    if (left <= 0) break;
+                    const int64_t to = col * p.c_c + row;
+                    if (p.c_dtype == ST_F32) store_columns(static_cast<float *>(p.c) + to, p.c_c, v[i], left, alpha, add);
+                    else if (p.c_dtype == ST_F16) store_columns(static_cast<__half *>(p.c) + to, p.c_c, v[i], left, alpha, add);
+                    else store_columns(static_cast<__nv_bfloat16 *>(p.c) + to, p.c_c, v[i], left, alpha, add);
+                }
+            }
+            __syncwarp();  // TMEM is read by whole warps
         }
     }
 
