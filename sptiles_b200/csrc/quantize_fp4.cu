@@ -21,6 +21,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 #include <utility>
 
 #include "common.h"
@@ -75,25 +76,46 @@ __device__ __forceinline__ float block_max(float m, float *shared) {
 }
 
 // ---------------------------------------------------------------- the tensor's largest |a|
-// One maximum per CTA; the quantiser's CTAs reduce them.
+// One maximum per CTA; the quantiser's CTAs reduce them.  A NaN loses every
+// comparison; a maximum that comes out infinite is taken again over the finite
+// elements.
+__device__ __forceinline__ float max_of_word(float m, const uint4 &w, float) {
+    m = fmaxf(fmaxf(m, fabsf(__uint_as_float(w.x))), fabsf(__uint_as_float(w.y)));
+    return fmaxf(fmaxf(m, fabsf(__uint_as_float(w.z))), fabsf(__uint_as_float(w.w)));
+}
+template <typename T2>
+__device__ __forceinline__ T2 max_of_word2(T2 m, const uint4 &w) {
+    const T2 *e = reinterpret_cast<const T2 *>(&w);
+    return __hmax2(__hmax2(m, __hmax2(__habs2(e[0]), __habs2(e[1]))), __hmax2(__habs2(e[2]), __habs2(e[3])));
+}
+__device__ __forceinline__ __half2 max_of_word(__half2 m, const uint4 &w, __half) { return max_of_word2(m, w); }
+__device__ __forceinline__ __nv_bfloat162 max_of_word(__nv_bfloat162 m, const uint4 &w, __nv_bfloat16) { return max_of_word2(m, w); }
+__device__ __forceinline__ float start_of(float) { return 0.0f; }
+__device__ __forceinline__ __half2 start_of(__half) { return __float2half2_rn(0.0f); }
+__device__ __forceinline__ __nv_bfloat162 start_of(__nv_bfloat16) { return __float2bfloat162_rn(0.0f); }
+__device__ __forceinline__ float end_of(float m) { return m; }
+__device__ __forceinline__ float end_of(__half2 m) { return fmaxf(__low2float(m), __high2float(m)); }
+__device__ __forceinline__ float end_of(__nv_bfloat162 m) { return fmaxf(__low2float(m), __high2float(m)); }
+
 template <typename T, bool WORDS>
 __global__ void __launch_bounds__(kThreads) amax_kernel(const T *a, int64_t s0, int64_t s1, int64_t rows, int64_t cols,
                                                         float *maxima) {
     pdl_wait();
     __shared__ float shared[kWarps];
-    float m = 0.0f;
-    constexpr int kVec = 16 / static_cast<int>(sizeof(T));
-    const int64_t per_row = WORDS ? cols / kVec : cols;
-    const int64_t total = rows * per_row, stride = static_cast<int64_t>(gridDim.x) * kThreads;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    float m = 0.0f;
     if constexpr (WORDS) {
+        constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kAtOnce = 8;
+        const int64_t per_row = cols / kVec, total = rows * per_row;
         // the row and column of a stride's step, so that the loop divides nothing
         const int64_t dr = stride / per_row, dc = stride - dr * per_row;
         int64_t r = first / per_row, c = first - r * per_row;
-        for (int64_t i = first; i < total; i += 4 * stride) {
-            uint4 w[4];
+        auto most = start_of(T{});
+        for (int64_t i = first; i < total; i += kAtOnce * stride) {
+            uint4 w[kAtOnce];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < kAtOnce; ++j) {
                 w[j] = make_uint4(0, 0, 0, 0);
                 if (i + j * stride < total) w[j] = *reinterpret_cast<const uint4 *>(a + r * s0 + c * kVec);
                 r += dr;
@@ -104,21 +126,26 @@ __global__ void __launch_bounds__(kThreads) amax_kernel(const T *a, int64_t s0, 
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const T *e = reinterpret_cast<const T *>(&w[j]);
-#pragma unroll
-                for (int k = 0; k < kVec; ++k) m = finite_abs(m, to_float(e[k]));
-            }
+            for (int j = 0; j < kAtOnce; ++j) most = max_of_word(most, w[j], T{});
         }
+        m = end_of(most);
         const int64_t tail = per_row * kVec, left = cols - tail;  // the columns behind the last whole word
-        for (int64_t i = first; i < rows * left; i += stride) m = finite_abs(m, to_float(a[i / left * s0 + tail + i % left]));
+        for (int64_t i = first; i < rows * left; i += stride) m = fmaxf(m, fabsf(to_float(a[i / left * s0 + tail + i % left])));
     } else {
-        for (int64_t i = first; i < total; i += stride) {
+        for (int64_t i = first; i < rows * cols; i += stride) {
             const int64_t r = i / cols;
-            m = finite_abs(m, to_float(a[r * s0 + (i - r * cols) * s1]));
+            m = fmaxf(m, fabsf(to_float(a[r * s0 + (i - r * cols) * s1])));
         }
     }
     m = block_max(m, shared);
+    if (m == INFINITY) {
+        m = 0.0f;
+        for (int64_t i = first; i < rows * cols; i += stride) {
+            const int64_t r = i / cols;
+            m = finite_abs(m, to_float(a[r * s0 + (i - r * cols) * s1]));
+        }
+        m = block_max(m, shared);
+    }
     if (threadIdx.x == 0) maxima[blockIdx.x] = m;
     pdl_trigger();
 }
@@ -159,7 +186,9 @@ __device__ __forceinline__ BlockScale block_scale(float top, const Unit &u) {
         if (e < -127) e = -127;
         return BlockScale{static_cast<uint32_t>(e + 127), power_of_two(e), power_of_two(-e)};
     } else {
-        const uint32_t byte = __nv_cvt_float_to_fp8(__fdiv_rn(top * u.inverse, 6.0f), __NV_SATFINITE, __NV_E4M3);
+        // a sixth, correctly rounded: the product with the rounded inverse, corrected by its residual (see codes8)
+        const float y = top * u.inverse, r = 1.0f / 6.0f, q = y * r;
+        const uint32_t byte = __nv_cvt_float_to_fp8(__fmaf_rn(__fmaf_rn(q, -6.0f, y), r, q), __NV_SATFINITE, __NV_E4M3);
         const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
         if (s == 0.0f) return BlockScale{0u, 0.0f, 0.0f};
         return BlockScale{byte, s * u.t, __frcp_rn(s) * u.inverse};
@@ -213,30 +242,6 @@ __device__ __forceinline__ int64_t scale_at(int64_t row, int64_t b, int64_t quad
     return ((row >> 7) * quads + (b >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (b & 3);
 }
 
-// Sixteen elements of one row from column c on (of the view's columns) as
-// fp32 pairs; zeros behind the edge.
-template <typename T>
-__device__ __forceinline__ void load16_words(const T *src, int64_t left, uint64_t (&x)[2][4]) {
-    constexpr int kWords = static_cast<int>(sizeof(T) / 2);
-    uint4 w[2][kWords];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int k = 0; k < kWords; ++k) w[h][k] = make_uint4(0, 0, 0, 0);
-        if (left >= 8 * h + 8) {
-#pragma unroll
-            for (int k = 0; k < kWords; ++k) w[h][k] = __ldcs(reinterpret_cast<const uint4 *>(src + 8 * h) + k);
-        } else {
-            T *e = reinterpret_cast<T *>(w[h]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (8 * h + j < left) e[j] = src[8 * h + j];
-        }
-    }
-    unpack8(w[0], x[0], T{});
-    unpack8(w[1], x[1], T{});
-}
-
 // The 8 bytes of 16 codes, or those of the first n elements.
 __device__ __forceinline__ void store_codes(uint8_t *to, uint32_t lo, uint32_t hi, int64_t left, bool words) {
     if (left >= 16 && words) {
@@ -277,26 +282,48 @@ __device__ __forceinline__ void quantize_unit(const Quantize4Args &p, const Unit
 }
 
 // ---------------------------------------------------------------- rows on 16-byte boundaries
-// A lane takes 16 elements of a row, a CTA walks the tensor from its end: the
-// maximum has just passed over it from the start, and the end is still in L2.
-// Rows are padded to 128 and a row's blocks to four, as the scales are.
+// A lane takes 16 columns of two rows, whose reads are under way together.  The
+// CTAs walk the tensor from its end: the maximum has just passed over it from
+// the start, and the end is still in L2.  Rows are padded to 128 and a row's
+// blocks to four, as the scales are.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) quantize4_rows_kernel(const Quantize4Args p, int64_t units, int64_t quads,
-                                                                  bool words) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3)
+    quantize4_rows_kernel(const Quantize4Args p, uint32_t units, uint32_t across, uint32_t chunks, int64_t quads, bool words) {
     pdl_wait();
     __shared__ float shared[kWarps];
     const Unit u = WIDE ? Unit{1.0f, 1.0f, 1.0f} : tensor_unit(p, shared);
-    const int64_t padded = (p.rows + 127) / 128 * 128, total = padded * units, chunks = cdiv_dev(total, 32);
-    const int lane = threadIdx.x & 31;
-    for (int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < chunks;
-         w += static_cast<int64_t>(gridDim.x) * kWarps) {
-        const int64_t i = (chunks - 1 - w) * 32 + lane;
-        const bool here = i < total;
-        // units of a row are a multiple of the lanes of one scale word, so a word's lanes lie in one row
-        const int64_t row = here ? i / units : 0, unit = here ? i - row * units : 0;
-        uint64_t x[2][4] = {};
-        if (here && row < p.rows) load16_words(static_cast<const T *>(p.a) + row * p.sa0 + unit * 16, p.cols - unit * 16, x);
-        quantize_unit<WIDE>(p, u, x, row, unit, quads, here, words);
+    constexpr int kWords = static_cast<int>(sizeof(T) / 2);
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t w = blockIdx.x * kWarps + (threadIdx.x >> 5); w < chunks; w += gridDim.x * kWarps) {
+        const uint32_t at = chunks - 1 - w, pair = at / across, unit = (at - pair * across) * 32 + lane;
+        const int64_t row0 = static_cast<int64_t>(pair) * 2;
+        const int left = static_cast<int>(p.cols) - static_cast<int>(unit) * 16;  // columns from this lane's first on
+        const T *src = static_cast<const T *>(p.a) + row0 * p.sa0 + unit * 16;
+        uint4 raw[2][2][kWords];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int k = 0; k < kWords; ++k) raw[i][h][k] = make_uint4(0, 0, 0, 0);
+                if (row0 + i >= p.rows) continue;
+                if (left >= 8 * h + 8) {
+#pragma unroll
+                    for (int k = 0; k < kWords; ++k) raw[i][h][k] = __ldcs(reinterpret_cast<const uint4 *>(src + i * p.sa0 + 8 * h) + k);
+                } else {
+                    T *e = reinterpret_cast<T *>(raw[i][h]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (8 * h + j < left) e[j] = src[i * p.sa0 + 8 * h + j];
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint64_t x[2][4];
+            unpack8(raw[i][0], x[0], T{});
+            unpack8(raw[i][1], x[1], T{});
+            quantize_unit<WIDE>(p, u, x, row0 + i, unit, quads, unit < units, words);
+        }
     }
     pdl_trigger();
 }
@@ -344,131 +371,250 @@ __global__ void __launch_bounds__(kThreads) quantize4_any_kernel(const Quantize4
 }
 
 // ---------------------------------------------------------------- stored by columns (rows contiguous)
-// A lane takes ROWS neighbouring rows and the four blocks of one scale word,
-// so that a read of the warp is 32 * ROWS neighbouring elements and a row's
-// codes leave as whole 32-byte (64-byte) sectors.
-template <typename T, bool WIDE, int ROWS>
-__global__ void __launch_bounds__(kThreads) quantize4_columns_kernel(const Quantize4Args p, int64_t quads, bool words) {
+// A CTA takes 128 bytes of neighbouring rows and 8 units of 16 (of 32) columns
+// into shared memory, where a warp finds a unit's elements of all the rows;
+// the codes go through shared memory too, and leave as whole rows of the tile.
+// (Each lane reading its rows' elements from global memory and storing 8 bytes
+// a row took 255 us for 8192 x 8192 bf16.)
+template <typename T, bool WIDE>
+struct ColumnTile {
+    static constexpr int kSpan = WIDE ? 32 : 16;  // columns of a block and a warp
+    static constexpr int kCols = 8 * kSpan;
+    static constexpr int kPer = 4 / static_cast<int>(sizeof(T));  // rows of a lane
+    static constexpr int kRows = 32 * kPer;
+    static constexpr int kPitch = 128 + 16;             // bytes of a column's rows
+    static constexpr int kCodePitch = kCols / 2 + 4;    // bytes of a row's codes; a lane's rows lie on other banks than its neighbours'
+    uint8_t in[kCols * kPitch];
+    uint8_t codes[kRows * kCodePitch];
+    uint8_t scales[kRows * 8];
+};
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kThreads) quantize4_columns_kernel(const Quantize4Args p, int64_t quads, bool in_words, bool words) {
+    using Tile = ColumnTile<T, WIDE>;
     pdl_wait();
     __shared__ float shared[kWarps];
+    extern __shared__ __align__(16) uint8_t tile_bytes[];
+    Tile &tile = *reinterpret_cast<Tile *>(tile_bytes);
     const Unit u = WIDE ? Unit{1.0f, 1.0f, 1.0f} : tensor_unit(p, shared);
-    constexpr int kSpan = WIDE ? 128 : 64, kUnits = kSpan / 16;
-    const int64_t padded = (p.rows + 127) / 128 * 128, groups = padded / (32 * ROWS), chunks = groups * quads;
-    const int lane = threadIdx.x & 31;
-    for (int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < chunks;
-         w += static_cast<int64_t>(gridDim.x) * kWarps) {
-        const int64_t at = chunks - 1 - w, quad = at / groups, row0 = (at - quad * groups) * 32 * ROWS + lane * ROWS;
-        uint32_t codes[ROWS][2 * kUnits], scales[ROWS];
+    const int64_t groups = (p.rows + 127) / 128 * (128 / Tile::kRows), total = groups * cdiv_dev(quads, 2);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+        const int64_t at = total - 1 - w, across = at / groups, row0 = (at - across * groups) * Tile::kRows, col0 = across * Tile::kCols;
+        const T *src = static_cast<const T *>(p.a) + row0 + col0 * p.sa1;
+        const int rows = p.rows - row0 < Tile::kRows ? static_cast<int>(p.rows - row0) : Tile::kRows;
+        const int cols = p.cols - col0 < Tile::kCols ? static_cast<int>(p.cols - col0) : Tile::kCols;
+        // 16 bytes of a column a thread, 8 threads a column
+        constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kSteps = Tile::kCols / 32;
+        if (in_words) {
+            const int r = (threadIdx.x & 7) * kVec;
+            uint4 v[kSteps];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) scales[r] = 0;
-        float tops[ROWS];
-        uint64_t x[ROWS][WIDE ? 4 : 2][4];
-        constexpr int kStep = WIDE ? 2 : 1;  // units of a block
+            for (int j = 0; j < kSteps; ++j) {
+                const int c = static_cast<int>(threadIdx.x >> 3) + 32 * j;
+                v[j] = make_uint4(0, 0, 0, 0);
+                if (c < cols && r + kVec <= rows) {
+                    v[j] = __ldcs(reinterpret_cast<const uint4 *>(src + r + c * p.sa1));
+                } else if (c < cols) {
+                    T *e = reinterpret_cast<T *>(&v[j]);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-#pragma unroll
-            for (int s = 0; s < kStep; ++s) {
-                T v[ROWS][16];
-                const int64_t c0 = quad * kSpan + (b * kStep + s) * 16;
-                const T *src = static_cast<const T *>(p.a) + row0 + c0 * p.sa1;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-#pragma unroll
-                    for (int r = 0; r < ROWS; ++r) from_float(0.0f, v[r][j]);
-                    if (c0 + j < p.cols) {
-                        if (ROWS == 2 && row0 + 1 < p.rows) {
-                            const uint32_t both = __ldcs(reinterpret_cast<const uint32_t *>(src + j * p.sa1));
-                            *reinterpret_cast<uint16_t *>(&v[0][j]) = static_cast<uint16_t>(both);
-                            *reinterpret_cast<uint16_t *>(&v[ROWS - 1][j]) = static_cast<uint16_t>(both >> 16);
-                        } else if (row0 < p.rows) {
-                            v[0][j] = src[j * p.sa1];
-                        }
-                    }
+                    for (int i = 0; i < kVec; ++i)
+                        if (r + i < rows) e[i] = src[r + i + c * p.sa1];
                 }
-#pragma unroll
-                for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            x[r][2 * s + h][j] = mul2(pack2(to_float(v[r][8 * h + 2 * j]), to_float(v[r][8 * h + 2 * j + 1])),
-                                                      pack2(u.lift, u.lift));
             }
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-                tops[r] = max_abs8(max_abs8(0.0f, x[r][0]), x[r][1]);
-                if constexpr (WIDE) tops[r] = max_abs8(max_abs8(tops[r], x[r][2]), x[r][3]);
-                const BlockScale s = block_scale<WIDE>(tops[r], u);
-                scales[r] |= s.byte << (8 * b);
+            for (int j = 0; j < kSteps; ++j)
+                *reinterpret_cast<uint4 *>(tile.in + ((threadIdx.x >> 3) + 32 * j) * Tile::kPitch + (threadIdx.x & 7) * 16) = v[j];
+        } else {  // a column a warp at a time, an element a lane
 #pragma unroll
-                for (int h = 0; h < 2 * kStep; ++h) codes[r][2 * kStep * b + h] = codes8<WIDE>(x[r][h], s);
+            for (int j0 = 0; j0 < Tile::kSpan; j0 += 8) {
+                T v[8][Tile::kPer];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int i = 0; i < Tile::kPer; ++i) {
+                        const int c = warp * Tile::kSpan + j0 + j, r = lane + 32 * i;
+                        from_float(0.0f, v[j][i]);
+                        if (c < cols && r < rows) v[j][i] = src[r + c * p.sa1];
+                    }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int i = 0; i < Tile::kPer; ++i)
+                        *reinterpret_cast<T *>(tile.in + (warp * Tile::kSpan + j0 + j) * Tile::kPitch + (lane + 32 * i) * sizeof(T)) = v[j][i];
             }
         }
+        __syncthreads();
+        // rows kPer lane, ... of the block of this warp
+        float top[Tile::kPer];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            const int64_t row = row0 + r;
-            *reinterpret_cast<uint32_t *>(p.scale + scale_at(row, quad * 4, quads)) = scales[r];
-            if (row >= p.rows) continue;
-            uint8_t *to = p.q + row * p.sq0 + quad * (kSpan / 2);
+        for (int i = 0; i < Tile::kPer; ++i) top[i] = 0.0f;
+        const uint8_t *mine = tile.in + warp * Tile::kSpan * Tile::kPitch + lane * 4;
 #pragma unroll
-            for (int k = 0; k < kUnits; ++k) {
-                const int64_t left = p.cols - quad * kSpan - 16 * k;
-                if (left > 0) store_codes(to + 8 * k, codes[r][2 * k], codes[r][2 * k + 1], left, words);
+        for (int j = 0; j < Tile::kSpan; ++j) {
+            const uint32_t word = *reinterpret_cast<const uint32_t *>(mine + j * Tile::kPitch);
+#pragma unroll
+            for (int i = 0; i < Tile::kPer; ++i) top[i] = max_abs(top[i], to_float(reinterpret_cast<const T *>(&word)[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < Tile::kPer; ++i) {
+            const BlockScale b = block_scale<WIDE>(WIDE ? top[i] : top[i] * u.lift, u);
+            const int r = lane * Tile::kPer + i;
+            tile.scales[r * 8 + warp] = static_cast<uint8_t>(b.byte);
+#pragma unroll
+            for (int j = 0; j < Tile::kSpan; j += 8) {
+                uint64_t x[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const uint32_t w0 = *reinterpret_cast<const uint32_t *>(mine + (j + 2 * h) * Tile::kPitch);
+                    const uint32_t w1 = *reinterpret_cast<const uint32_t *>(mine + (j + 2 * h + 1) * Tile::kPitch);
+                    x[h] = pack2(to_float(reinterpret_cast<const T *>(&w0)[i]), to_float(reinterpret_cast<const T *>(&w1)[i]));
+                    if (!WIDE && u.lift != 1.0f) x[h] = mul2(x[h], pack2(u.lift, u.lift));
+                }
+                *reinterpret_cast<uint32_t *>(tile.codes + r * Tile::kCodePitch + (warp * Tile::kSpan + j) / 2) = codes8<WIDE>(x, b);
+            }
+        }
+        __syncthreads();
+        constexpr int kPieces = Tile::kCols / 32;  // 16 bytes of codes each
+        const int bytes = (cols + 1) / 2;
+        for (int i = threadIdx.x; i < Tile::kRows * kPieces; i += kThreads) {
+            const int r = i / kPieces, q = i - r * kPieces, n = bytes - 16 * q;
+            if (r >= rows || n <= 0) continue;
+            const uint8_t *from = tile.codes + r * Tile::kCodePitch + 16 * q;
+            uint8_t *to = p.q + (row0 + r) * p.sq0 + col0 / 2 + 16 * q;
+            if (n >= 16 && words) {
+                const uint32_t *f = reinterpret_cast<const uint32_t *>(from);
+                *reinterpret_cast<uint4 *>(to) = make_uint4(f[0], f[1], f[2], f[3]);
+            } else {
+                for (int j = 0; j < 16 && j < n; ++j) to[j] = from[j];
+            }
+        }
+        for (int i = threadIdx.x; i < Tile::kRows * 2; i += kThreads) {
+            const int64_t quad = across * 2 + i / Tile::kRows;
+            const int r = i % Tile::kRows;
+            if (quad < quads)
+                *reinterpret_cast<uint32_t *>(p.scale + scale_at(row0 + r, 4 * quad, quads)) =
+                    *reinterpret_cast<const uint32_t *>(tile.scales + r * 8 + 4 * (i / Tile::kRows));
+        }
+        __syncthreads();  // the tile's next contents
+    }
+    pdl_trigger();
+}
+
+// ---------------------------------------------------------------- back to values
+__device__ __forceinline__ float scale_value(uint32_t byte, bool wide) {
+    if (wide) return byte == 255u ? NAN : power_of_two(static_cast<int>(byte) - 127);
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+}
+__device__ __forceinline__ float2 two_codes(uint32_t byte) {
+    return __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1)));
+}
+
+// The values of 16 codes.
+__device__ __forceinline__ void values16(uint64_t (&f)[2][4], uint2 code, float unit) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 v = two_codes((h ? code.y : code.x) >> (8 * j) & 0xffu);
+            f[h][j] = mul2(pack2(v.x, v.y), pack2(unit, unit));
+        }
+}
+
+// A lane takes 16 columns of four rows.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) dequantize4_words_kernel(const Dequantize4Args p, uint32_t across, uint32_t chunks,
+                                                                        int64_t quads) {
+    pdl_wait();
+    const float t = p.tensor_scale != nullptr ? *p.tensor_scale : 1.0f;
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t w = blockIdx.x * kWarps + (threadIdx.x >> 5); w < chunks; w += gridDim.x * kWarps) {
+        const uint32_t group = w / across, unit = (w - group * across) * 32 + lane;
+        const int64_t row0 = static_cast<int64_t>(group) * 4;
+        const int left = static_cast<int>(p.cols) - static_cast<int>(unit) * 16;
+        if (left <= 0) continue;
+        uint2 code[4];
+        uint32_t byte[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            code[i] = make_uint2(0, 0);
+            byte[i] = 0;
+            if (row0 + i >= p.rows) continue;
+            const uint8_t *q = p.q + (row0 + i) * p.sq0 + unit * 8;
+            if (left >= 16) {
+                code[i] = __ldcs(reinterpret_cast<const uint2 *>(q));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (2 * j < left) (j < 4 ? code[i].x : code[i].y) |= static_cast<uint32_t>(q[j]) << (8 * (j & 3));
+            }
+            byte[i] = p.scale[scale_at(row0 + i, p.wide ? unit >> 1 : unit, quads)];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (row0 + i >= p.rows) break;
+            uint64_t f[2][4];
+            values16(f, code[i], scale_value(byte[i], p.wide) * t);
+            T *out = static_cast<T *>(p.out) + (row0 + i) * p.so0 + unit * 16;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (left >= 8 * h + 8) {
+                    constexpr int kWords = static_cast<int>(sizeof(T) / 2);
+                    uint4 o[kWords];
+                    pack8(f[h], o, T{});
+#pragma unroll
+                    for (int k = 0; k < kWords; ++k) reinterpret_cast<uint4 *>(out + 8 * h)[k] = o[k];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (8 * h + j < left) from_float(j & 1 ? hi2(f[h][j / 2]) : lo2(f[h][j / 2]), out[8 * h + j]);
+                }
             }
         }
     }
     pdl_trigger();
 }
 
-// ---------------------------------------------------------------- back to values
-// A thread per 16 codes.
+// Any strides, unit ones among them: a lane's 16 values are turned in shared
+// memory, so that neighbouring lanes store neighbouring elements.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) dequantize4_kernel(const Dequantize4Args p, int64_t units, int64_t quads, bool words,
-                                                               bool out_words) {
+__global__ void __launch_bounds__(kThreads) dequantize4_any_kernel(const Dequantize4Args p, uint32_t across, int64_t chunks,
+                                                                   int64_t quads, bool words) {
     pdl_wait();
+    __shared__ float turned[kWarps][32 * 17];
     const float t = p.tensor_scale != nullptr ? *p.tensor_scale : 1.0f;
-    const int64_t total = p.rows * units, stride = static_cast<int64_t>(gridDim.x) * kThreads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += stride) {
-        const int64_t row = i / units, unit = i - row * units, left = p.cols - unit * 16;
-        const uint8_t *q = p.q + row * p.sq0 + unit * 8 * p.sq1;
-        uint32_t code[2] = {0, 0};
-        if (left >= 16 && words) {
-            const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(q));
-            code[0] = v.x;
-            code[1] = v.y;
-        } else {
+    const uint32_t lane = threadIdx.x & 31;
+    float *mine = turned[threadIdx.x >> 5];
+    for (int64_t w = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < chunks;
+         w += static_cast<int64_t>(gridDim.x) * kWarps) {
+        const int64_t row = w / across;
+        const uint32_t chunk = static_cast<uint32_t>(w - row * across), unit = chunk * 32 + lane;
+        const int left = static_cast<int>(p.cols) - static_cast<int>(unit) * 16;
+        uint2 code = make_uint2(0, 0);
+        uint32_t byte = 0;
+        if (left > 0) {
+            const uint8_t *q = p.q + row * p.sq0 + unit * 8 * p.sq1;
+            if (left >= 16 && words) {
+                code = __ldcs(reinterpret_cast<const uint2 *>(q));
+            } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (2 * j < left) code[j / 4] |= static_cast<uint32_t>(q[j * p.sq1]) << (8 * (j & 3));
+                for (int j = 0; j < 8; ++j)
+                    if (2 * j < left) (j < 4 ? code.x : code.y) |= static_cast<uint32_t>(q[j * p.sq1]) << (8 * (j & 3));
+            }
+            byte = p.scale[scale_at(row, p.wide ? unit >> 1 : unit, quads)];
         }
-        const uint32_t byte = p.scale[scale_at(row, p.wide ? unit >> 1 : unit, quads)];
-        float s;
-        if (p.wide) s = byte == 255u ? NAN : power_of_two(static_cast<int>(byte) - 127);
-        else s = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
-        const float unit_scale = s * t;
         uint64_t f[2][4];
+        values16(f, code, scale_value(byte, p.wide) * t);
+        __syncwarp();
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int j = 0; j < 16; ++j) mine[17 * lane + j] = j & 1 ? hi2(f[j / 8][j % 8 / 2]) : lo2(f[j / 8][j % 8 / 2]);
+        __syncwarp();
+        T *out = static_cast<T *>(p.out) + row * p.so0 + static_cast<int64_t>(chunk) * 512 * p.so1;
+        const int here = static_cast<int>(p.cols) - static_cast<int>(chunk) * 512;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const __half2_raw v = __nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(code[h] >> (8 * j)), __NV_E2M1);
-                const float2 w = __half22float2(__half2(v));
-                f[h][j] = mul2(pack2(w.x, w.y), pack2(unit_scale, unit_scale));
-            }
-        T *out = static_cast<T *>(p.out) + row * p.so0 + unit * 16 * p.so1;
-        if (left >= 16 && out_words) {
-            constexpr int kWords = static_cast<int>(sizeof(T) / 2);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint4 w[kWords];
-                pack8(f[h], w, T{});
-#pragma unroll
-                for (int k = 0; k < kWords; ++k) reinterpret_cast<uint4 *>(out + 8 * h)[k] = w[k];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (j < left) from_float(j & 1 ? hi2(f[j / 8][j % 8 / 2]) : lo2(f[j / 8][j % 8 / 2]), out[j * p.so1]);
+        for (int j = 0; j < 16; ++j) {
+            const int c = 32 * j + static_cast<int>(lane);
+            if (c < here) from_float(mine[c + c / 16], out[c * p.so1]);
         }
     }
     pdl_trigger();
@@ -478,6 +624,18 @@ int checked(const char *what) {
     note_launch();
     const cudaError_t e = cudaPeekAtLastError();
     return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), what);
+}
+
+// CTAs for `work` of them, as many as are resident at once at most.
+template <typename Kernel, typename... Instance>
+unsigned resident_grid(Kernel kern, int64_t work, int sm_count, size_t smem) {
+    static int per_sm = 0;  // the same on every device of this architecture
+    if (per_sm == 0) {
+        int n = 0;
+        per_sm = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, kThreads, smem) == cudaSuccess && n > 0 ? n : 2;
+    }
+    const int64_t most = static_cast<int64_t>(sm_count) * per_sm;
+    return static_cast<unsigned>(work < 1 ? 1 : work < most ? work : most);
 }
 
 // CTAs for `work` of them, at most `per_sm` on each SM.
@@ -501,7 +659,7 @@ int launch_amax(Quantize4Args &p, float *maxima, int sm_count, cudaStream_t stre
     const T *a = static_cast<const T *>(p.a);
     constexpr int kVec = 16 / static_cast<int>(sizeof(T));
     const bool words = (s1 == 1 || cols == 1) && cols >= kVec && on16(a, s0, rows, sizeof(T));
-    unsigned grid = grid_of(cdiv(rows * cols, kThreads * (words ? 4 * kVec : 4)), sm_count, kAmaxPerSm);
+    unsigned grid = grid_of(cdiv(rows * cols, kThreads * (words ? 8 * kVec : 4)), sm_count, kAmaxPerSm);
     if (grid > kMostMaxima) grid = kMostMaxima;
     if (words) ST_CUDA_TRY(launch_kernel(amax_kernel<T, true>, grid, kThreads, 0, stream, a, s0, s1, rows, cols, maxima));
     else ST_CUDA_TRY(launch_kernel(amax_kernel<T, false>, grid, kThreads, 0, stream, a, s0, s1, rows, cols, maxima));
@@ -511,30 +669,49 @@ int launch_amax(Quantize4Args &p, float *maxima, int sm_count, cudaStream_t stre
 }
 
 template <typename T, bool WIDE>
+int launch_columns(const Quantize4Args &p, int64_t quads, int sm_count, cudaStream_t stream) {
+    using Tile = ColumnTile<T, WIDE>;
+    auto kern = quantize4_columns_kernel<T, WIDE>;
+    if constexpr (sizeof(Tile) > 48 * 1024) {
+        static uint64_t attr_set = 0;  // one bit per device ordinal
+        int dev = 0;
+        ST_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev < 0 || dev >= 64 || !(attr_set & (1ull << dev))) {
+            ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Tile)));
+            if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
+        }
+    }
+    const bool in_words = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && (p.cols == 1 || p.sa1 * static_cast<int64_t>(sizeof(T)) % 16 == 0);
+    const bool words = on16(p.q, p.sq0, p.rows, 1);
+    const int64_t work = cdiv(p.rows, 128) * (128 / Tile::kRows) * cdiv(quads, 2);
+    const unsigned grid = resident_grid<decltype(kern), T, std::bool_constant<WIDE>>(kern, work, sm_count, sizeof(Tile));
+    ST_CUDA_TRY(launch_kernel(kern, grid, kThreads, sizeof(Tile), stream, p, quads, in_words, words));
+    return checked("quantize4_columns_kernel");
+}
+
+template <typename T, bool WIDE>
 int launch_quantize(const Quantize4Args &p, int sm_count, cudaStream_t stream) {
     const int64_t blocks = cdiv(p.cols, WIDE ? 32 : 16), quads = cdiv(blocks, 4), units = quads * (WIDE ? 8 : 4);
     const int64_t padded = cdiv(p.rows, 128) * 128;
-    const bool words = reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.rows == 1 || p.sq0 % 8 == 0);
     if (p.cols == 1 || p.sa1 == 1) {
         if (on16(p.a, p.sa0, p.rows, sizeof(T))) {
-            const unsigned grid = grid_of(cdiv(padded * units, kThreads), sm_count, 8);
-            ST_CUDA_TRY(launch_kernel(quantize4_rows_kernel<T, WIDE>, grid, kThreads, 0, stream, p, units, quads, words));
+            const bool words = reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.rows == 1 || p.sq0 % 8 == 0);
+            const int64_t across = cdiv(units, 32), chunks = padded / 2 * across;
+            if (chunks > INT32_MAX) return fail(ST_ERR_UNSUPPORTED, "quantize_fp4: too many blocks");
+            auto kern = quantize4_rows_kernel<T, WIDE>;
+            const unsigned grid = resident_grid<decltype(kern), T, std::bool_constant<WIDE>>(kern, cdiv(chunks, kWarps), sm_count, 0);
+            ST_CUDA_TRY(launch_kernel(kern, grid, kThreads, 0, stream, p, static_cast<uint32_t>(units), static_cast<uint32_t>(across),
+                                      static_cast<uint32_t>(chunks), quads, words));
             return checked("quantize4_rows_kernel");
         }
     } else if (p.sa0 == 1 && p.rows > 1) {
-        const bool two = sizeof(T) == 2 && reinterpret_cast<uintptr_t>(p.a) % 4 == 0 && p.sa1 % 2 == 0;
-        const unsigned grid = grid_of(cdiv(padded / (two ? 64 : 32) * quads, kWarps), sm_count, 8);
-        if constexpr (sizeof(T) == 2) {
-            if (two) {
-                ST_CUDA_TRY(launch_kernel(quantize4_columns_kernel<T, WIDE, 2>, grid, kThreads, 0, stream, p, quads, words));
-                return checked("quantize4_columns_kernel");
-            }
-        }
-        ST_CUDA_TRY(launch_kernel(quantize4_columns_kernel<T, WIDE, 1>, grid, kThreads, 0, stream, p, quads, words));
-        return checked("quantize4_columns_kernel");
+        return launch_columns<T, WIDE>(p, quads, sm_count, stream);
     }
-    const unsigned grid = grid_of(cdiv(padded * cdiv(units, 32), kWarps), sm_count, 8);
-    ST_CUDA_TRY(launch_kernel(quantize4_any_kernel<T, WIDE>, grid, kThreads, 0, stream, p, units, quads, words));
+    const bool words = reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.rows == 1 || p.sq0 % 8 == 0);
+    auto kern = quantize4_any_kernel<T, WIDE>;
+    const unsigned grid =
+        resident_grid<decltype(kern), T, std::bool_constant<WIDE>, int>(kern, cdiv(padded * cdiv(units, 32), kWarps), sm_count, 0);
+    ST_CUDA_TRY(launch_kernel(kern, grid, kThreads, 0, stream, p, units, quads, words));
     return checked("quantize4_any_kernel");
 }
 
@@ -547,12 +724,20 @@ int launch_typed(Quantize4Args p, float *maxima, int sm_count, cudaStream_t stre
 
 template <typename T>
 int launch_dequantize(const Dequantize4Args &p, int sm_count, cudaStream_t stream) {
-    const int64_t units = cdiv(p.cols, 16), quads = cdiv(cdiv(p.cols, p.wide ? 32 : 16), 4);
+    const int64_t quads = cdiv(cdiv(p.cols, p.wide ? 32 : 16), 4);
     const bool words = p.sq1 == 1 && reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.rows == 1 || p.sq0 % 8 == 0);
-    const bool out_words = p.so1 == 1 && on16(p.out, p.so0, p.rows, sizeof(T));
-    const unsigned grid = grid_of(cdiv(p.rows * units, kThreads), sm_count, 8);
-    ST_CUDA_TRY(launch_kernel(dequantize4_kernel<T>, grid, kThreads, 0, stream, p, units, quads, words, out_words));
-    return checked("dequantize4_kernel");
+    const int64_t across = cdiv(p.cols, 512);
+    if (words && p.so1 == 1 && on16(p.out, p.so0, p.rows, sizeof(T)) && cdiv(p.rows, 4) * across <= INT32_MAX) {
+        const int64_t chunks = cdiv(p.rows, 4) * across;
+        auto kern = dequantize4_words_kernel<T>;
+        const unsigned grid = resident_grid<decltype(kern), T>(kern, cdiv(chunks, kWarps), sm_count, 0);
+        ST_CUDA_TRY(launch_kernel(kern, grid, kThreads, 0, stream, p, static_cast<uint32_t>(across), static_cast<uint32_t>(chunks), quads));
+        return checked("dequantize4_words_kernel");
+    }
+    auto kern = dequantize4_any_kernel<T>;
+    const unsigned grid = resident_grid<decltype(kern), T, int>(kern, cdiv(p.rows * across, kWarps), sm_count, 0);
+    ST_CUDA_TRY(launch_kernel(kern, grid, kThreads, 0, stream, p, static_cast<uint32_t>(across), p.rows * across, quads, words));
+    return checked("dequantize4_any_kernel");
 }
 
 }  // namespace
