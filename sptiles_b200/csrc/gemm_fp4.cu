@@ -11,7 +11,11 @@
 //
 //   warp 0      TMA producer: 256 elements (128 bytes) of K of each operand a stage, and their scales
 //   warp 1      MMA issuer (owns the TMEM allocation)
-//   warps 2-5   C: TMEM -> registers, scale, bias, store
+//   warps 2..   C: TMEM -> registers, scale, bias, store
+//
+// CTA pairs on 256 x 256 tiles, unless there are few rows of A or few tiles of
+// a long K: then 128 x 16, 32 or 64 tiles of one CTA, two of them on an SM,
+// and a cluster of up to 8 that splits the K of a tile.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -86,15 +90,15 @@ struct Fp4Cfg {
     static constexpr int kColBytes = BN * kBlockK;
     static constexpr int kScaleBytes = kChunks * kAtomBytes;  // of each operand (blocks of 32 use half)
     static constexpr int kStageBytes = kRowBytes + kColBytes + 2 * kScaleBytes;
-    static constexpr int kStages = BN == 128 ? 5 : BN == 64 ? 3 : BN == 32 ? 4 : 5;
+    static constexpr int kStages = BN == 64 ? 3 : BN == 32 ? 4 : 5;
     // A stage's scales have TMEM columns of their own: they are overwritten
     // only after the MMAs that read them have freed the stage.
     static constexpr int kStageCols = 2 * 4 * kChunks;
     static constexpr int kScaleCol = BN;
-    static constexpr int kTmemCols = BN == 128 ? 512 : 256;
+    static constexpr int kTmemCols = 256;
     static_assert(kScaleCol + kStages * kStageCols <= kTmemCols, "the accumulator and the scales fit");
     static constexpr int kSmemBytes = kStages * kStageBytes + kBarBytes + 1024;
-    static_assert(kSmemBytes <= (BN == 128 ? 232448 : 115712), "shared memory of one (two) CTAs per SM");
+    static_assert(kSmemBytes <= 115712, "shared memory of two CTAs per SM");
     static_assert(kStages * kStageBytes >= kTileRows * (BN + 4 * 8) * 4, "the ring holds eight parts' sums of its columns");
 };
 
@@ -154,7 +158,7 @@ __device__ __forceinline__ void store_parts(const Fp4Params &p, const float4 *su
 }
 
 template <int BN, bool WIDE>
-__global__ void __launch_bounds__(Fp4Cfg<BN>::kThreads, BN == 128 ? 1 : 2)
+__global__ void __launch_bounds__(Fp4Cfg<BN>::kThreads, 2)
     gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ CUtensorMap tmap_c,
                     const Fp4Params p) {
     using Cfg = Fp4Cfg<BN>;
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN>::kThreads, BN == 128 ? 1 : 2)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
     const uint32_t bar0 = smem_addr(bars);
     auto full_bar = [&](int s) { return bar0 + 8u * s; };                   // loads landed
@@ -193,7 +197,7 @@ __global__ void __launch_bounds__(Fp4Cfg<BN>::kThreads, BN == 128 ? 1 : 2)
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     pdl_begin();  // nothing above touches global memory
 
     const int split = p.split;
@@ -241,7 +245,12 @@ __global__ void __launch_bounds__(Fp4Cfg<BN>::kThreads, BN == 128 ? 1 : 2)
             drain_ring(issued, Cfg::kStages, full_bar, p.timeout_ns);
         }
     } else if (warp == 1) {
-        // ------------------------------------------------ MMA issuer
+        // ------------------------------------------------ MMA issuer (see the pair's)
+        const uint32_t ring = smem_addr(smem), scales = ring + Cfg::kRowBytes + Cfg::kColBytes;
+        const uint64_t dr0 = smem_desc_sw128(ring, 16, 1024), dc0 = smem_desc_sw128(ring + Cfg::kRowBytes, 16, 1024);
+        const uint64_t drs0 = smem_desc_scales(scales), dcs0 = smem_desc_scales(scales + Cfg::kScaleBytes);
+        // a tile of 64 columns may begin in the middle of 128 columns' scales: two TMEM columns of 32 further
+        const uint32_t middle = BN == 64 && (c0 & 64) ? 2u : 0u;
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
@@ -252,23 +261,21 @@ __global__ void __launch_bounds__(Fp4Cfg<BN>::kThreads, BN == 128 ? 1 : 2)
             }
             tc_fence_after_sync();
             if (elect_one()) {
-                const int left = p.k_chunks - (part + i * split) * kChunks, n = left < kChunks ? left : kChunks;
-                const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes);
-                const uint32_t sc = sr + Cfg::kRowBytes, ss = sc + Cfg::kColBytes;
+                const int left = p.k_chunks - (part + i * split) * kChunks;
+                const uint64_t step = static_cast<uint64_t>(s) * (Cfg::kStageBytes >> 4);
                 const uint32_t tr_s = tmem_base + static_cast<uint32_t>(Cfg::kScaleCol + s * Cfg::kStageCols);
                 const uint32_t tc_s = tr_s + 4 * kChunks;
-                const uint64_t dr = smem_desc_sw128(sr, 16, 1024), dc = smem_desc_sw128(sc, 16, 1024);
-                const uint64_t dsr = smem_desc_scales(ss), dsc = smem_desc_scales(ss + Cfg::kScaleBytes);
+#pragma unroll
+                for (uint32_t a = 0; a < kAtoms; ++a) {  // the last block's may be stale: no MMA reads those
+                    tmem_copy_scales(tr_s + 4 * a, drs0 + step + a * (kAtomBytes >> 4));
+                    tmem_copy_scales(tc_s + 4 * a, dcs0 + step + a * (kAtomBytes >> 4));
+                }
 #pragma unroll
                 for (int j = 0; j < kChunks; ++j) {
-                    if (j >= n) break;
                     const uint32_t atom = static_cast<uint32_t>(WIDE ? j / 2 : j);
-                    if (!WIDE || j % 2 == 0) {
-                        tmem_copy_scales(tr_s + 4 * atom, dsr + atom * (kAtomBytes >> 4));
-                        tmem_copy_scales(tc_s + 4 * atom, dsc + atom * (kAtomBytes >> 4));
-                    }
-                    tc_mma_fp4<WIDE ? 2 : 4>(tmem_base, dr + j * 2u, dc + j * 2u, p.idesc[WIDE ? j % 2 : 0], tr_s + 4 * atom,
-                                             tc_s + 4 * atom, i + j != 0 ? 1u : 0u);
+                    if (j == 0 || j < left)
+                        tc_mma_fp4<WIDE ? 2 : 4>(tmem_base, dr0 + step + j * 2u, dc0 + step + j * 2u, p.idesc[WIDE ? j % 2 : 0],
+                                                 tr_s + 4 * atom, tc_s + middle + 4 * atom, i + j != 0 ? 1u : 0u);
                 }
                 tc_commit(empty_bar(s));
             }
@@ -715,20 +722,45 @@ Access access_of(const Fp4Operand &o) {
 
 int64_t copy_bytes(const Fp4Operand &o, const Access &a) { return a.copy ? (o.rows * a.ld + 255) / 256 * 256 : 0; }
 
+// Kernel, tile and split of a product: the least estimated time.  The figures
+// are microseconds fitted to B200 timings of 1 x 1024 x 1024 to 4096 x 4096 x
+// 1024 and 1 x 4096 x 16384 (within 15 %; 1 x 8192 x 8192 estimated 8.3 on 16
+// columns and four parts, measured 8.4; 1024 x 512 x 8192 10.9 on 64 columns
+// and four parts, 13.6 by pairs, measured 12.4 and 13.5).
 struct Fp4Plan {
     bool pair = false, swap = false;  // swap: B is the row operand
-    int bn = 128, split = 1;
+    int bn = 64, split = 1;
+    double us = 1e300;
 };
 
 Fp4Plan plan_fp4(int64_t m, int64_t n, int64_t k_blocks, int sm_count) {
     Fp4Plan best;
-    best.pair = m > 128 && n > 128 && cdiv(m, 256) * cdiv(n, 256) * 4 >= sm_count;
-    best.swap = best.pair || m <= 64;
-    if (best.pair) return best;
-    const int64_t rows = best.swap ? n : m, cols = best.swap ? m : n;
-    best.bn = cols <= 16 ? 16 : cols <= 32 ? 32 : cols <= 64 ? 64 : 128;
-    const int64_t tiles = cdiv(rows, kTileRows) * cdiv(cols, best.bn), slots = static_cast<int64_t>(sm_count) * (best.bn == 128 ? 1 : 2);
-    while (best.split < 8 && tiles * best.split * 2 <= slots && best.split * 4 <= k_blocks) best.split *= 2;
+    {
+        const int64_t waves = cdiv(cdiv(n, 256) * cdiv(m, 256), sm_count / 2);
+        best.pair = best.swap = true;
+        best.us = 3.7 + static_cast<double>(waves) * (0.3 * static_cast<double>(k_blocks) + 0.3);
+    }
+    struct Shape {
+        int bn;
+        double ends, block, two, join[4];  // a block of K alone on an SM, and beside another CTA; extra for 1 to 8 parts
+    };
+    const Shape shapes[] = {{16, 3.9, 0.30, 0.42, {0, 0.8, 1.0, 1.6}},
+                            {32, 4.2, 0.33, 0.45, {0, 0.8, 1.2, 2.0}},
+                            {64, 4.8, 0.31, 0.36, {0, 2.0, 3.2, 5.0}}};
+    for (int swap = 0; swap < 2; ++swap) {
+        const int64_t rows = swap ? n : m, cols = swap ? m : n;
+        for (const Shape &s : shapes) {
+            if (s.bn < 64 && cols > s.bn) continue;  // a column tile's scales begin with 64 or 128 of them
+            const int64_t tiles = cdiv(rows, kTileRows) * cdiv(cols, s.bn);
+            for (int parts = 0; parts <= 3 && (1 << parts) <= k_blocks; ++parts) {
+                const int64_t ctas = tiles << parts, rounds = cdiv(ctas, 2 * static_cast<int64_t>(sm_count));
+                if (rounds > 1 && parts > 0) break;
+                const double block = ctas > sm_count ? s.two : s.block;
+                const double us = static_cast<double>(rounds) * (s.ends + s.join[parts] + block * static_cast<double>(cdiv(k_blocks, int64_t(1) << parts)));
+                if (us < best.us) best = Fp4Plan{false, swap != 0, s.bn, 1 << parts, us};
+            }
+        }
+    }
     return best;
 }
 
@@ -805,8 +837,7 @@ int launch_gemm_fp4(const GemmFp4Args &g, void *workspace, int sm_count, int *de
     switch (plan.bn) {
     case 16: return launch_tile<16>(mr, mc, p, g.wide, stream);
     case 32: return launch_tile<32>(mr, mc, p, g.wide, stream);
-    case 64: return launch_tile<64>(mr, mc, p, g.wide, stream);
-    default: return launch_tile<128>(mr, mc, p, g.wide, stream);
+    default: return launch_tile<64>(mr, mc, p, g.wide, stream);
     }
 }
 
