@@ -63,6 +63,7 @@ struct GroupedParams {
     int64_t c_g, ldc;    // weights: D's strides of groups and rows
     int c_dtype;
     int zero_rest;       // rows of no group are set to 0
+    int split;           // CTAs of a cluster that share a tile
     int r_by_64, c_by_64;  // the operand's map splits its columns in 64s, so that one box holds two of them
     int reads;           // there is something to sum over: the maps are valid
     uint32_t idesc;
@@ -252,7 +253,9 @@ struct GroupedCfg {
     static_assert(kSmemBytes <= 232448, "over the per-block shared memory limit");
 };
 
-template <int BN, bool WEIGHTS, bool R_MN>
+// SPLIT: a cluster of p.split CTAs takes one tile, each every split-th step of
+// its contraction; the sums are added in order through distributed shared memory.
+template <int BN, bool WEIGHTS, bool R_MN, bool SPLIT>
 __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
     gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmap_r, const __grid_constant__ ColumnMaps maps_c,
                         const GroupedParams p) {
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // uniform registers for what follows from it
     const int lane = threadIdx.x & 31;
     const uint32_t bar0 = smem_addr(bars);
     auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -301,10 +304,13 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-    TileWalk<WEIGHTS, Cfg::kRows, BN> walk(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+    const int split = SPLIT ? p.split : 1, part = SPLIT ? static_cast<int>(cluster_rank()) : 0;
+    using Walk = TileWalk<WEIGHTS, Cfg::kRows, BN>;
+    Walk walk(static_cast<int>(blockIdx.x) / split, static_cast<int>(gridDim.x) / split);
     Tile tile;
+    auto my_blocks = [&](const Tile &of) { return SPLIT ? (of.blocks - part + split - 1) / split : of.blocks; };
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
         if (lane == 0) {
@@ -314,7 +320,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
             bool ok = true;
             while (ok && walk.next(table, p, tile)) {
                 const int high = (tile.cols + 31) / 32;  // rows of the column operand's box, in 32
-                for (int b = 0; b < tile.blocks; ++b, ++issued) {
+                for (int b = part; b < tile.blocks; b += split, ++issued) {
                     if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
                         ok = false;
                         break;
@@ -355,13 +361,14 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
         uint32_t ph = 0, aph = 0;
         bool ok = true;
         while (ok && walk.next(table, p, tile)) {
-            if (tile.blocks == 0) continue;
+            const int blocks = my_blocks(tile);
+            if (blocks == 0) continue;
             const uint32_t idesc = p.idesc | static_cast<uint32_t>(WEIGHTS ? BN / 8 : (tile.cols + 15) / 16 * 2) << 17;
             if (!__all_sync(0xffffffffu, mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns))) {
                 ok = false;
                 break;
             }
-            for (int b = 0; b < tile.blocks; ++b) {
+            for (int b = 0; b < blocks; ++b) {
                 if (!__all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, abort_flag, p.timeout_ns))) {
                     ok = false;
                     break;
@@ -376,7 +383,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
                         tc_mma<false>(tmem_base + static_cast<uint32_t>(a * BN), dr + j * ((R_MN ? kMmaK * 128 : 32) >> 4),
                                       dc + j * ((WEIGHTS ? kMmaK * 128 : 32) >> 4), idesc, (b | j) != 0 ? 1u : 0u);
                     tc_commit(empty_bar(s));
-                    if (b + 1 == tile.blocks) tc_commit(tfull_bar(a));
+                    if (b + 1 == blocks) tc_commit(tfull_bar(a));
                 }
                 __syncwarp();
                 if (++s == Cfg::kStages) {
@@ -396,7 +403,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
         if (elect_one()) tc_commit(drain_bar);
         __syncwarp();
         drain_ring(1, 1, [&](int) { return drain_bar; }, p.timeout_ns);  // the MMAs read shared memory and write TMEM
-    } else {
+    } else if constexpr (!SPLIT) {
         // ------------------------------------------------ C
         const int g = warp & 3;
         int a = 0;
@@ -425,9 +432,63 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
                 aph ^= 1u;
             }
         }
-        if (!WEIGHTS && p.zero_rest)
-            zero_rows<32 * kOutWarps>(p, p.groups > 0 ? table.row_end[p.groups - 1] : 0, (warp - 2) * 32 + lane);
     }
+    if constexpr (SPLIT) {
+        // ------------------------------------------------ C of the cluster's tile
+        Walk again(static_cast<int>(blockIdx.x) / split, static_cast<int>(gridDim.x) / split);
+        const bool any = again.next(table, p, tile);
+        const int g = warp & 3, half = (warp - 2) >> 2;
+        const bool out = warp >= 2, zero = !any || my_blocks(tile) == 0;
+        if (out && !zero) {
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(0), 0, abort_flag, p.timeout_ns))) {
+                *abort_flag = 1;
+                if (lane == 0) atomicExch(p.err, kDevAbortGemmEpilogue);
+            }
+            tc_fence_after_sync();
+        }
+        __syncwarp();
+        cluster_sync();  // every MMA of the cluster has read its ring
+        // a part owns `own` columns of the tile and gets them as [part][column][128 lanes]
+        const int own = BN / split, own_shift = 31 - __clz(own);  // split is a power of two
+        if (out && any) {
+            const uint32_t mine = smem_addr(smem) + 4u * static_cast<uint32_t>(part * own * 128 + 32 * g + lane);
+            for (int c = 32 * half; c < tile.cols; c += 64) {
+                uint32_t v[32];
+                if (!zero) {
+                    tmem_load_32(tmem_base + (static_cast<uint32_t>(g * 32) << 16) + static_cast<uint32_t>(c), v);
+                    tmem_load_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = 0u;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int col = c + i;
+                    const uint32_t to = map_to_rank(mine, static_cast<uint32_t>(col >> own_shift));
+                    st_cluster_f32(to + 512u * static_cast<uint32_t>(col & (own - 1)), __uint_as_float(v[i]));
+                }
+                __syncwarp();
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+        if (out && any) {
+            const int id = (warp - 2) * 32 + lane, n = tile.r0 + (id & 127);
+            const float *sums = reinterpret_cast<const float *>(smem) + (id & 127);
+            const int64_t at = (WEIGHTS ? tile.group * p.c_g : 0) + tile.c0 * p.ldc + n;
+            if (n < p.n)
+                for (int j = id >> 7; j < own && part * own + j < tile.cols; j += kOutWarps / 4) {
+                    float v = 0.0f;
+                    for (int q = 0; q < split; ++q) v += sums[(q * own + j) * 128];
+                    const int64_t to = at + (part * own + j) * p.ldc;
+                    if (p.c_dtype == ST_F32) static_cast<float *>(p.c)[to] = v;
+                    else if (p.c_dtype == ST_F16) from_float(v, static_cast<__half *>(p.c)[to]);
+                    else from_float(v, static_cast<__nv_bfloat16 *>(p.c)[to]);
+                }
+        }
+    }
+    if (!WEIGHTS && p.zero_rest && warp >= 2)
+        zero_rows<32 * kOutWarps>(p, p.groups > 0 ? table.row_end[p.groups - 1] : 0, (warp - 2) * 32 + lane);
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 1) {
@@ -472,7 +533,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const uint32_t bar0 = smem_addr(bars);
@@ -509,7 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
     __syncthreads();
     cluster_sync();
     tc_fence_after_sync();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
     TileWalk<WEIGHTS, Cfg::kRows, Cfg::kCols> walk(static_cast<int>(blockIdx.x >> 1), static_cast<int>(gridDim.x >> 1));
     Tile tile;
@@ -656,17 +717,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
     }
 }
 
-// Dense copy of strided 16-bit matrices, one for each group: rows of `ld`
-// elements (a multiple of 8), padding columns zeroed.
+// Dense copy of strided 16-bit matrices, one for each group, into rows of `ld`
+// elements (a multiple of 8), padding columns zeroed: 8 elements a thread, put
+// together from the aligned words that hold them where they lie together.
 __global__ void __launch_bounds__(256) repack_groups_kernel(const uint16_t *__restrict__ src, int64_t sg, int64_t s0, int64_t s1,
                                                             int64_t groups, int64_t rows, int64_t cols, uint16_t *__restrict__ dst,
                                                             int64_t ld) {
     pdl_wait();
-    const int64_t per_group = rows * ld, total = groups * per_group;
+    const int64_t per_row = ld / 8, total = groups * rows * per_row;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t g = i / per_group, j = i - g * per_group, r = j / ld, c = j - r * ld;
-        dst[i] = c < cols ? src[g * sg + r * s0 + c * s1] : static_cast<uint16_t>(0);
+        const int64_t line = i / per_row, c = (i - line * per_row) * 8, g = line / rows, r = line - g * rows;
+        const uint16_t *from = src + g * sg + r * s0 + c * s1;
+        const int n = cols - c < 8 ? static_cast<int>(cols - c) : 8;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (s1 == 1) {
+            const uint32_t *words = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t(3));
+            const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(from) >> 1) & 1, have = (odd + n + 1) / 2;
+            uint32_t x[5];
+#pragma unroll
+            for (int j = 0; j < 5; ++j) x[j] = j < have ? words[j] : 0u;  // only words with an element of the row
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = __funnelshift_r(x[j], x[j + 1], 16 * odd);
+                if (2 * j + 1 >= n) w[j] = 2 * j < n ? w[j] & 0xffffu : 0u;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) w[j / 2] |= static_cast<uint32_t>(from[j * s1]) << (16 * (j % 2));
+        }
+        reinterpret_cast<uint4 *>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
     pdl_trigger();
 }
@@ -701,8 +782,8 @@ Matrices layout(const void *data, int64_t groups, int64_t outer, int64_t inner, 
 
 int copy_in(Matrices &m, uint8_t *&ws, int sm_count, cudaStream_t stream) {
     if (m.copy) {
-        const int64_t ld = (m.inner + 7) / 8 * 8, total = m.groups * m.outer * ld;
-        const int64_t grid = cdiv(total, 256 * 8) < sm_count * 8 ? cdiv(total, 256 * 8) : sm_count * 8;
+        const int64_t ld = (m.inner + 7) / 8 * 8, work = cdiv(m.groups * m.outer * (ld / 8), 256), most = static_cast<int64_t>(sm_count) * 8;
+        const int64_t grid = work < most ? work : most;
         ST_CUDA_TRY(launch_kernel(repack_groups_kernel, static_cast<unsigned>(grid), 256, 0, stream,
                                   static_cast<const uint16_t *>(m.data), m.sg, m.so, m.si, m.groups, m.outer, m.inner,
                                   reinterpret_cast<uint16_t *>(ws), ld));
@@ -764,11 +845,11 @@ int make_map_columns(CUtensorMap *map, int *by_64, int dtype, const char *what, 
                            dims, strides, box);
 }
 
-template <int BN, bool WEIGHTS, bool R_MN>
+template <int BN, bool WEIGHTS, bool R_MN, bool SPLIT>
 int launch_instance(const CUtensorMap &mr, const ColumnMaps &mc, const GroupedParams &p, int64_t most_tiles, int sm_count,
                     cudaStream_t stream) {
     using Cfg = GroupedCfg<BN>;
-    auto kern = gemm_grouped_kernel<BN, WEIGHTS, R_MN>;
+    auto kern = gemm_grouped_kernel<BN, WEIGHTS, R_MN, SPLIT>;
     static uint64_t attr_set = 0;  // one bit per device ordinal
     int dev = 0;
     ST_CUDA_TRY(cudaGetDevice(&dev));
@@ -776,9 +857,35 @@ int launch_instance(const CUtensorMap &mr, const ColumnMaps &mc, const GroupedPa
         ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
         if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
     }
-    const int64_t ctas = most_tiles < 1 ? 1 : most_tiles < sm_count ? most_tiles : sm_count;
-    ST_CUDA_TRY(launch_kernel(kern, static_cast<unsigned>(ctas), Cfg::kThreads, Cfg::kSmemBytes, stream, mr, mc, p));
+    const int64_t tiles = most_tiles < 1 ? 1 : most_tiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(SPLIT ? tiles * p.split : tiles < sm_count ? tiles : sm_count));
+    cfg.blockDim = dim3(Cfg::kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (SPLIT) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = static_cast<unsigned>(p.split);
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    ST_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mr, mc, p));
     return checked("gemm_grouped_kernel");
+}
+
+template <int BN, bool WEIGHTS, bool R_MN>
+int launch_single(const CUtensorMap &mr, const ColumnMaps &mc, const GroupedParams &p, int64_t most_tiles, int sm_count,
+                  cudaStream_t stream) {
+    return p.split > 1 ? launch_instance<BN, WEIGHTS, R_MN, true>(mr, mc, p, most_tiles, sm_count, stream)
+                       : launch_instance<BN, WEIGHTS, R_MN, false>(mr, mc, p, most_tiles, sm_count, stream);
 }
 
 template <bool WEIGHTS, bool R_MN>
@@ -798,31 +905,42 @@ int launch_pair_instance(const CUtensorMap &mr, const ColumnMaps &mc, const Grou
     return checked("gemm_grouped_pair_kernel");
 }
 
-// Tile shape: the least estimated time for groups of equal size (what the ends
-// hold is not known here).  A stage of 64 along the contraction costs an SM its
-// MMAs or its loads, whichever is longer; the figures are SM cycles.
+// Most tiles that there can be, however the ends divide the rows.
+int64_t most_tiles(const GroupedArgs &g, int64_t tiles_r, int cols) {
+    return tiles_r * (g.weights ? g.groups * cdiv(g.k, cols) : cdiv(g.rows, cols) + (g.groups < g.rows ? g.groups : g.rows));
+}
+
+// Tile shape and split: the least estimated time for groups of equal size (what
+// the ends hold is not known here).  A stage of 64 along the contraction costs
+// an SM its MMAs or its loads, whichever is longer; the figures are SM cycles.
 struct GroupedPlan {
     bool pair = false;
     int cols = 128;  // most columns of a tile
+    int split = 1;
     double cycles = 1e300;
 };
 
 GroupedPlan plan_grouped(const GroupedArgs &g, int sm_count) {
     const int64_t met = g.groups < 1 ? 1 : !g.weights && g.rows < g.groups ? (g.rows > 0 ? g.rows : 1) : g.groups;
-    const int64_t per_group = cdiv(g.rows > 0 ? g.rows : 1, met);
+    const int64_t per_group = cdiv(g.rows > 0 ? g.rows : 1, met), blocks = cdiv(g.weights ? per_group : g.k, kBK);
     GroupedPlan best;
-    auto offer = [&](bool pair, int cols) {
+    auto offer = [&](bool pair, int cols, int split) {
         const int64_t extent = g.weights ? g.k : per_group, tiles_c = cdiv(extent, cols);
         const double c = g.weights ? cols : static_cast<double>(cdiv(cdiv(extent, tiles_c), 16) * 16);
-        const int64_t tiles = met * tiles_c * cdiv(g.n, pair ? 256 : 128);
+        const int64_t tiles_r = cdiv(g.n, pair ? 256 : 128);
+        if (split > 1 && (split > blocks || most_tiles(g, tiles_r, cols) * split > 4 * static_cast<int64_t>(sm_count))) return;
         const double mma = 2 * c, load = 256 + (pair ? c : 2 * c);
-        const double t = static_cast<double>(cdiv(tiles, pair ? sm_count / 2 : sm_count)) *
-                         (static_cast<double>(cdiv(g.weights ? per_group : g.k, kBK)) * (mma > load ? mma : load) + 3000);
-        if (t < best.cycles) best = GroupedPlan{pair, cols, t};
+        const double join[] = {0, 2500, 3500, 5000};
+        const double t = static_cast<double>(cdiv(met * tiles_c * tiles_r * split, pair ? sm_count / 2 : sm_count)) *
+                         (static_cast<double>(cdiv(blocks, split)) * (mma > load ? mma : load) + 3000 +
+                          join[split == 8 ? 3 : split / 2]);
+        if (t < best.cycles) best = GroupedPlan{pair, cols, split, t};
     };
-    if (!g.weights) offer(false, 32);
-    offer(false, 128);
-    offer(true, GroupedPairCfg::kCols);
+    for (int split = 1; split <= 8; split *= 2) {
+        if (!g.weights) offer(false, 32, split);
+        offer(false, 128, split);
+    }
+    offer(true, GroupedPairCfg::kCols, 1);
     return best;
 }
 
@@ -855,8 +973,8 @@ int launch_gemm_grouped(const GroupedArgs &g, void *workspace, int sm_count, int
     const int rows = pair ? GroupedPairCfg::kRows : 128, cols = plan.cols;
     p.tiles_r = static_cast<int>(cdiv(g.n, rows));
     p.tiles_c = static_cast<int>(cdiv(g.k, cols));
-    const int64_t most = g.weights ? g.groups * p.tiles_r * p.tiles_c
-                                   : (cdiv(g.rows, cols) + (g.groups < g.rows ? g.groups : g.rows)) * p.tiles_r;
+    p.split = plan.split;
+    const int64_t most = most_tiles(g, p.tiles_r, cols);
     if (most > INT32_MAX / 2) return fail(ST_ERR_UNSUPPORTED, "matmul_grouped: too many output tiles");
     CUtensorMap mr{};
     ColumnMaps mc{};
@@ -888,12 +1006,12 @@ int launch_gemm_grouped(const GroupedArgs &g, void *workspace, int sm_count, int
         return o.b_mn ? launch_pair_instance<false, true>(mr, mc, p, most, sm_count, stream)
                       : launch_pair_instance<false, false>(mr, mc, p, most, sm_count, stream);
     }
-    if (g.weights) return launch_instance<128, true, true>(mr, mc, p, most, sm_count, stream);
+    if (g.weights) return launch_single<128, true, true>(mr, mc, p, most, sm_count, stream);
     if (cols == 32)
-        return o.b_mn ? launch_instance<32, false, true>(mr, mc, p, most, sm_count, stream)
-                      : launch_instance<32, false, false>(mr, mc, p, most, sm_count, stream);
-    return o.b_mn ? launch_instance<128, false, true>(mr, mc, p, most, sm_count, stream)
-                  : launch_instance<128, false, false>(mr, mc, p, most, sm_count, stream);
+        return o.b_mn ? launch_single<32, false, true>(mr, mc, p, most, sm_count, stream)
+                      : launch_single<32, false, false>(mr, mc, p, most, sm_count, stream);
+    return o.b_mn ? launch_single<128, false, true>(mr, mc, p, most, sm_count, stream)
+                  : launch_single<128, false, false>(mr, mc, p, most, sm_count, stream);
 }
 
 }  // namespace st

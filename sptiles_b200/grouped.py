@@ -58,11 +58,12 @@ def _workspace(name: str, like: torch.Tensor, da: bytes, db: bytes, *args: int) 
     return (torch.empty(need, dtype=torch.uint8, device=like.device) if need else None), need
 
 
-def _on_16(t: torch.Tensor) -> bool:
-    """Read in place as it is: contiguous rows, everything on 16-byte boundaries (16-bit elements)."""
-    st = t.stride()
-    return (st[-1] == 1 and st[-2] % 8 == 0 and st[-2] >= t.shape[-1] and t.data_ptr() % 16 == 0 and
-            (len(st) == 2 or st[0] % 8 == 0 and st[0] > 0))
+def _on_16(t: torch.Tensor, rows: int, cols: int) -> bool:
+    """Whether matrices [..., rows, cols] (dimension numbers) of 16-bit elements are read in place: contiguous rows,
+    everything on 16-byte boundaries."""
+    s = t.stride()
+    return (s[cols] == 1 and s[rows] % 8 == 0 and s[rows] >= t.shape[cols] and t.data_ptr() % 16 == 0 and
+            (len(s) == 2 or s[0] % 8 == 0 and s[0] > 0))
 
 
 def matmul_grouped(A: torch.Tensor, B: torch.Tensor, ends: torch.Tensor, *, out_dtype: torch.dtype | None = None,
@@ -96,7 +97,7 @@ def matmul_grouped(A: torch.Tensor, B: torch.Tensor, ends: torch.Tensor, *, out_
     else:
         dc = _desc(out)
     workspace, need = None, 0
-    if not (_on_16(A) and (_on_16(B) or _on_16(B.transpose(1, 2)))):
+    if not (_on_16(A, 0, 1) and (_on_16(B, 2, 1) or _on_16(B, 1, 2))):
         workspace, need = _workspace("st_matmul_grouped_workspace", A, da, db, stride, groups)
     fn = _fns.get("st_matmul_grouped") or _fn("st_matmul_grouped", _vp, _cp, _cp, _i64, _cp, _cp, _i32, _vp, _u64, _cp)
     rc = fn(context(dev), da, db, stride, de, dc, fresh, None if workspace is None else workspace.data_ptr(), need,
@@ -131,7 +132,7 @@ def matmul_grouped_weights(A: torch.Tensor, C: torch.Tensor, ends: torch.Tensor,
         out = A.new_empty((groups, A.shape[1], C.shape[1]), dtype=out_dtype)
     dd, stride = _stack_desc(out, groups, "out")
     workspace, need = None, 0
-    if not (_on_16(A) and _on_16(C)):
+    if not (_on_16(A, 0, 1) and _on_16(C, 0, 1)):
         workspace, need = _workspace("st_matmul_grouped_weights_workspace", A, da, dc, groups)
     fn = _fns.get("st_matmul_grouped_weights") or _fn("st_matmul_grouped_weights", _vp, _cp, _cp, _cp, _cp, _i64, _vp, _u64, _cp)
     rc = fn(context(dev), da, dc, de, dd, stride, None if workspace is None else workspace.data_ptr(), need, _exec_desc(dev))

@@ -55,6 +55,9 @@ CASES = [
     (129, 1001, 515, [64, 129]), (513, 40, 1000, [128, 256, 384, 512, 513]), (40, 512, 384, list(range(1, 41))),
     (70, 96, 80, [100]), (70, 96, 80, [30, 10, 200, 5]), (70, 96, 80, [-5, 40]), (2000, 136, 264, [1000, 1000, 1999]),
 ]
+# a long contraction and few tiles: clusters split it; and groups of several tiles of CTA pairs
+CASES += [(40, 4096, 200, [7, 40]), (3, 8192, 64, [3]), (200, 2049, 130, [150, 200]), (3000, 64, 72, [3000]), (5000, 40, 136, [4000, 4001]),
+          (1300, 320, 1032, [700, 700, 1299]), (2600, 72, 776, [2113, 2600])]
 IDS = [f"{r}x{k}x{n}-{len(e)}" for r, k, n, e in CASES]
 
 
