@@ -227,14 +227,16 @@ __device__ __forceinline__ void store_any_tile(const GroupedParams &p, int64_t a
     else store_tile<__nv_bfloat16>(p, at, taddr, lanes, cols, zero, lane, released);
 }
 
-// Rows [first, p.rows) of C, which belong to no group, become 0.
+// Rows [first, p.rows) of C, which belong to no group, become 0: a row a CTA.
 template <int THREADS>
 __device__ __forceinline__ void zero_rows(const GroupedParams &p, int first, int thread) {
-    const int64_t total = static_cast<int64_t>(p.rows - first) * p.n;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * THREADS + thread; i < total; i += static_cast<int64_t>(gridDim.x) * THREADS) {
-        const int64_t at = (first + i / p.n) * p.ldc + i % p.n;
-        if (p.c_dtype == ST_F32) static_cast<float *>(p.c)[at] = 0.0f;
-        else static_cast<uint16_t *>(p.c)[at] = 0;
+    const int es = p.c_dtype == ST_F32 ? 4 : 2;
+    const bool wide = reinterpret_cast<uintptr_t>(p.c) % 16 == 0 && p.ldc * es % 16 == 0;
+    for (int64_t r = first + static_cast<int64_t>(blockIdx.x); r < p.rows; r += gridDim.x) {
+        uint8_t *row = static_cast<uint8_t *>(p.c) + r * p.ldc * es;
+        const int64_t bytes = static_cast<int64_t>(p.n) * es, whole = wide ? bytes / 16 * 16 : 0;
+        for (int64_t i = 16 * thread; i < whole; i += 16 * THREADS) *reinterpret_cast<uint4 *>(row + i) = make_uint4(0, 0, 0, 0);
+        for (int64_t i = whole + 2 * thread; i < bytes; i += 2 * THREADS) *reinterpret_cast<uint16_t *>(row + i) = 0;
     }
 }
 

@@ -955,8 +955,8 @@ int set_scale(const st_tensor *t, const char *name, bool is_b, Fp8Operand *o) {
 int check_codes(const st_tensor *t, const char *name) {
     ST_TRY(check_matrix(t, name));
     if (t->dtype != ST_E2M1X2) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be ST_E2M1X2");
-    if (t->shape[0] > INT32_MAX / 2 || t->shape[1] > INT32_MAX / 2)
-        return fail(ST_ERR_UNSUPPORTED, std::string(name) + ": elements of a row or column must fit in int32");
+    if (t->shape[0] > INT32_MAX / 4 || t->shape[1] > INT32_MAX / 4)
+        return fail(ST_ERR_UNSUPPORTED, std::string(name) + ": at most " + std::to_string(INT32_MAX / 4) + " bytes a row or column");
     return ST_OK;
 }
 

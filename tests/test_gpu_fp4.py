@@ -8,6 +8,10 @@ and compared for equality.  Other products: each fp32 addition is off by at
 most 2^-23 of the sum of the terms' magnitudes (a truncating adder), so a
 K-term sum by (K + 4) 2^-23 sum |a b|, the tensor scales' product included; the
 result's rounding adds half a step, eps / 2 relative."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -336,3 +340,121 @@ def test_product_empty_and_given_output():
             assert torch.equal(out.cpu(), (va @ vb.t()).to(dtype))
             out.fill_(7.0)
             assert (room == 7).all()
+
+
+# ------------------------------------------------------------------ streams, graphs, long tensors
+def test_same_bits_streams_and_graphs():
+    """Quantisers of both kinds into a product: two graphs with workspaces of their own, side by side."""
+    x, w = torch.randn(300, 1000, generator=gen(1)).to(DEV), torch.randn(700, 1000, generator=gen(2)).to(DEV)
+
+    def step():
+        out = []
+        for dtype in (E4, E8):
+            a, b = st.quantize_fp4(x[:, 1:], scale_dtype=dtype), st.quantize_fp4(w.t()[1:].t(), scale_dtype=dtype)
+            out += [a.scale.view(torch.uint8), st.matmul_fp4(a.codes[1:], b.codes.t(), st.quantize_fp4(x[1:, 1:], scale_dtype=dtype).scale, b.scale),
+                    st.dequantize_fp4(*b, cols=999)]
+        return out
+
+    first = step()
+    assert all(torch.equal(a, b) for a, b in zip(first, step()))
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(side):
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                out = step()
+            graphs.append((g, out))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for (g, _), s in zip(graphs, (side, other)):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for _, out in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(first, out))
+
+
+def test_first_call_may_be_captured():
+    """In a process of its own: each operator's first call inside a graph capture."""
+    code = """
+import torch, sptiles_b200 as st
+dev = torch.device('cuda:0')
+torch.manual_seed(0)
+x = torch.randn(300, 1024, device=dev, dtype=torch.bfloat16)
+w = torch.randn(4, 256, 1024, device=dev, dtype=torch.bfloat16)
+ends = torch.tensor([10, 10, 250, 290], device=dev, dtype=torch.int32)
+s = torch.cuda.Stream()
+torch.cuda.synchronize()
+st.runtime.context(0)
+def step():
+    xq, wq = st.quantize_fp4(x), st.quantize_fp4(w[0])
+    y = st.matmul_fp4(xq.codes, wq.codes.t(), xq.scale, wq.scale, a_tensor_scale=xq.tensor_scale, b_tensor_scale=wq.tensor_scale)
+    z = st.matmul_grouped(x, w.transpose(1, 2), ends)
+    return y, z, st.dequantize_fp4(*xq), st.matmul_grouped_weights(z, x, ends)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=s):
+    out = step()
+g.replay()
+torch.cuda.synchronize()
+want = step()
+assert all(torch.equal(a, b) for a, b in zip(out, want))
+print('captured')
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          cwd=str(Path(__file__).resolve().parents[1]))
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
+
+
+def some_codes(rows, cols, seed):
+    return torch.randint(0, 256, (rows, cols), generator=torch.Generator(DEV).manual_seed(seed), device=DEV, dtype=torch.uint8)
+
+
+@pytest.mark.parametrize("scale_dtype", [E4, E8], ids=["16", "32"])
+@pytest.mark.parametrize("stored", ["rows", "columns", "off"])
+def test_quantize_many_elements(stored, scale_dtype):
+    """More than 2^31 elements; the last rows against the plain form."""
+    rows, cols, first = 140000, 16384, 139904
+    if stored == "columns":
+        x = torch.randn(cols, rows, device=DEV, dtype=torch.bfloat16).t()
+    else:
+        x = torch.randn(rows, cols + (stored == "off"), device=DEV, dtype=torch.bfloat16)[:, -cols:]
+    amax = torch.tensor(8.0, device=DEV) if scale_dtype == E4 else None
+    got = st.quantize_fp4(x, scale_dtype=scale_dtype, amax=amax)
+    code, byte, t, _ = plain_quantize(x[first:].cpu(), scale_dtype, 8.0)
+    assert torch.equal(split(got.codes[first:], cols)[0].long(), code.long())
+    assert torch.equal(untiled(got.scale[first // 128 :], rows - first, byte.shape[1]).long(), byte.long())
+    back = st.dequantize_fp4(*got)
+    assert torch.equal(back[first:].cpu(), values(code, byte, t, scale_dtype).to(torch.bfloat16))
+
+
+def test_maximum_of_many_elements():
+    x = torch.zeros(140000, 16384, device=DEV, dtype=torch.bfloat16)
+    x[139999, 16383], x[0, 0] = 2689.0 * 4, float("inf")
+    # 10756 lies 4 above 10752, bf16's numbers there 64 apart: it is 10752 = 2688 * 4 that is stored
+    assert x[139999, 16383].item() == 2688 * 4
+    assert st.quantize_fp4(x).tensor_scale.item() == 4.0
+
+
+@pytest.mark.parametrize("aligned", [True, False], ids=["aligned", "off"])
+def test_product_many_weights(aligned):
+    m, n, kb, last = 3, 270000, 16384, 300
+    ld = kb if aligned else kb + 1
+    w = some_codes(1, n * ld, 1).as_strided((n, kb), (ld, 1))
+    qa, sa, va = random_operand(m, 2 * kb, E4, 2)
+    sb = torch.full((-(-n // 128), kb // 32, 32, 4, 4), 1.0, device=DEV).to(E4)
+    c = st.matmul_fp4(qa.to(DEV), w.t(), sa.to(DEV), sb, out_dtype=torch.float32)
+    vb = values(split(w[-last:].cpu(), 2 * kb)[0], torch.full((last, kb // 8), 0x38), None, E4)
+    assert torch.equal(c[:, -last:].cpu(), (va @ vb.t()).float())
+
+
+def test_product_many_results():
+    m, n, k, last = 33000, 66000, 128, 300
+    a, b = some_codes(m, k // 2, 1), some_codes(n, k // 2, 2)
+    one = lambda rows: torch.ones(-(-rows // 128), 2, 32, 4, 4, device=DEV).to(E4)  # noqa: E731
+    c = st.matmul_fp4(a, b.t(), one(m), one(n))
+    ones = torch.full((last, k // 16), 0x38)
+    va, vb = (values(split(t[-last:].cpu(), k)[0], ones, None, E4) for t in (a, b))
+    assert torch.equal(c[-last:, -last:].cpu(), (va @ vb.t()).float().to(torch.bfloat16))

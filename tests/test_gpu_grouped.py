@@ -214,3 +214,146 @@ def test_gradients_against_autograd():
     near(st.matmul_grouped(xd, wd.transpose(1, 2), e, out_dtype=F32), y.detach(), 96, plain(x.abs(), w.abs().transpose(1, 2), ends))
     near(st.matmul_grouped(dyd, wd, e, out_dtype=F32), gx, 64, plain(dy.abs(), w.abs(), ends))
     near(st.matmul_grouped_weights(dyd, xd, e, out_dtype=F32), gw, 130, plain_weights(dy.abs(), x.abs(), ends))
+
+
+# ------------------------------------------------------------------ streams, graphs, long tensors
+def test_one_graph_serves_any_ends():
+    """The ends are read by the kernels: a captured step follows them when they change between replays."""
+    rows, groups = 700, 9
+    x, w = ints(1, rows, 128), ints(2, groups, 192, 128)
+    xd, wd, e = x.to(BF16).to(DEV), w.to(BF16).to(DEV), device_ends([0] * groups)
+    dy = ints(3, rows, 192).to(BF16).to(DEV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        y = st.matmul_grouped(xd, wd.transpose(1, 2), e, out_dtype=F32)
+        dw = st.matmul_grouped_weights(dy, xd, e, out_dtype=F32)
+    for seed in range(6):
+        cut = sorted(torch.randint(0, rows + 1, (groups - 1,), generator=gen(seed)).tolist()) + [rows - 50 * (seed % 2)]
+        ends = [min(c, cut[-1]) for c in cut]
+        e.copy_(device_ends(ends))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y.cpu(), plain(x, w.transpose(1, 2), ends).float())
+        assert torch.equal(dw.cpu(), plain_weights(dy.cpu().float(), x, ends).float())
+
+
+def test_two_streams_at_once():
+    ends = [100, 101, 330, 400]
+    sets = [[torch.randn(*s, generator=gen(10 * i + j)).to(BF16).to(DEV) for j, s in enumerate([(400, 264), (4, 200, 264), (400, 200)])]
+            for i in range(2)]
+    e = device_ends(ends)
+
+    def step(d):
+        return [st.matmul_grouped(d[0], d[1].transpose(1, 2), e), st.matmul_grouped(d[2], d[1], e),
+                st.matmul_grouped(d[0][:, 1:], d[1].transpose(1, 2)[:, 1:], e), st.matmul_grouped_weights(d[2], d[0][:, 1:], e)]
+
+    want = [step(d) for d in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(sets[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
+
+
+@pytest.mark.parametrize("order", ["n", "k"])
+def test_many_weights(order):
+    """A stack of more than 2^31 elements; the last groups against the plain form."""
+    groups, k, n, rows = 34, 8192, 8192, 40
+    b = torch.randint(-4, 5, (groups, k, n), device=DEV, dtype=torch.int8, generator=torch.Generator(DEV).manual_seed(1)).to(BF16)
+    if order == "k":
+        b = b.transpose(1, 2)
+    ends = [0] * (groups - 2) + [17, rows]
+    a = ints(2, rows, k)
+    got = st.matmul_grouped(a.to(BF16).to(DEV), b, device_ends(ends), out_dtype=F32)
+    for g, (i, j) in list(enumerate(parts(ends, rows)))[-2:]:
+        assert torch.equal(got[i:j, -300:].cpu(), (a[i:j].double() @ b[g][:, -300:].cpu().double()).float())
+
+
+def test_many_results():
+    rows, n, k = 140000, 16384, 16
+    a, b = ints(1, rows, k), ints(2, 3, k, n)
+    ends = [5, 139000, 139900]
+    got = st.matmul_grouped(a.to(F16).to(DEV), b.to(F16).to(DEV), device_ends(ends))
+    assert torch.equal(got[138000:139000].cpu(), (a[138000:139000] @ b[1]).to(F16))
+    assert torch.equal(got[139000:139900].cpu(), (a[139000:139900] @ b[2]).to(F16)) and (got[139900:] == 0).all()
+    c = ints(3, 40, 8192)
+    a = ints(4, 40, 8192)
+    got = st.matmul_grouped_weights(a.to(F16).to(DEV), c.to(F16).to(DEV), device_ends([0] * 32 + [40, 40]))
+    assert (got[33] == 0).all() and torch.equal(got[32, -100:].cpu(), (a.t()[-100:] @ c).to(F16))
+
+
+# ------------------------------------------------------------------ together
+def test_experts_layer_forward_and_backward():
+    """A block of a network: norm, routed experts, a shared 4-bit expert, their sum back into the stream; and the
+    experts' gradients.  Each stage is compared with float64 on what the stage before it gave."""
+    tokens, hidden, inner, experts = 300, 256, 384, 6
+    g = gen(7)
+    r = torch.randn(tokens, hidden, generator=g)
+    pre = torch.rand(hidden, generator=g) + 0.5
+    w1, w2 = (torch.randn(experts, o, i, generator=g).to(BF16) / i ** 0.5 for o, i in ((inner, hidden), (hidden, inner)))
+    shared = torch.randn(hidden, hidden, generator=g).to(BF16) / hidden ** 0.5
+    choice = torch.randint(0, experts, (tokens,), generator=g)
+    choice[choice == 2] = 3  # an expert without a token
+    order = torch.argsort(choice, stable=True).to(DEV)
+    ends_host = torch.cumsum(torch.bincount(choice, minlength=experts), 0).tolist()
+    e = device_ends(ends_host)
+    w1d, w2d = w1.to(DEV), w2.to(DEV)
+    s4 = st.quantize_fp4(shared.to(DEV))
+
+    f = st.residual_norm(None, r.to(BF16).to(DEV), pre_weight=pre.to(BF16).to(DEV), eps=1e-6)
+    h = f.normed[order]
+    u = st.matmul_grouped(h, w1d.transpose(1, 2), e, out_dtype=F32)
+    v = torch.relu(u).square().to(BF16)
+    y = st.matmul_grouped(v, w2d.transpose(1, 2), e, out_dtype=F32)
+    h4 = st.quantize_fp4(f.normed)
+    z = st.matmul_fp4(h4.codes, s4.codes.t(), h4.scale, s4.scale, a_tensor_scale=h4.tensor_scale, b_tensor_scale=s4.tensor_scale, out_dtype=F32)
+    out = torch.empty_like(y)
+    out[order] = y
+    stream = st.residual_norm((out + z).to(BF16), f.residual).residual
+
+    dy = torch.randn(tokens, hidden, generator=g).to(BF16).to(DEV)[order]
+    dv = st.matmul_grouped(dy, w2d, e, out_dtype=F32)
+    dw2 = st.matmul_grouped_weights(dy, v, e, out_dtype=F32)
+    du = (dv * 2 * torch.relu(u)).to(BF16)
+    dh = st.matmul_grouped(du, w1d, e, out_dtype=F32)
+    dw1 = st.matmul_grouped_weights(du, h, e, out_dtype=F32)
+
+    def near(got, want, size, terms):
+        slack = (terms + 4) * 2.0 ** -23 * size
+        assert ((got.cpu().double() - want).abs() <= slack + 2.0 ** -24 * (want.abs() + slack)).all()
+
+    def rows(got, a, b):
+        a, b = a.cpu(), b.cpu()
+        near(got, plain(a, b, ends_host), plain(a.abs(), b.abs(), ends_host), a.shape[1])
+
+    def sums(got, a, c):
+        a, c = a.cpu(), c.cpu()
+        near(got, plain_weights(a, c, ends_host), plain_weights(a.abs(), c.abs(), ends_host), tokens)
+
+    rows(u, h, w1d.transpose(1, 2))
+    rows(y, v, w2d.transpose(1, 2))
+    rows(dv, dy, w2d)
+    rows(dh, du, w1d)
+    sums(dw2, dy, v)
+    sums(dw1, du, h)
+    assert (dw1[2] == 0).all() and (dw2[2] == 0).all()
+    vh, vs = (st.dequantize_fp4(*q, out_dtype=F32).cpu().double() for q in (h4, s4))
+    near(z, vh @ vs.t(), vh.abs() @ vs.abs().t(), hidden)
+    want = f.residual.cpu().float() + (out + z).to(BF16).cpu().float()
+    assert torch.equal(stream.cpu(), want.to(BF16))
+    # a weight's gradient against differences of the layer's output, in float64
+    step, at = 2.0 ** -6, (0, 3, 5)
+    moved = []
+    for sign in (1, -1):
+        w = w2.double()
+        w[at] += sign * step
+        moved.append((plain(v.cpu(), w.transpose(1, 2), ends_host) * dy.cpu().double()).sum())
+    slope, size = (moved[0] - moved[1]) / (2 * step), plain_weights(dy.cpu().abs(), v.cpu().abs(), ends_host)[at]
+    assert abs(slope - dw2[at].item()) <= (tokens + 4) * 2.0 ** -23 * size + 2.0 ** -24 * abs(slope) + 1e-9 * abs(moved[0])
