@@ -311,6 +311,21 @@ def test_product_exact_large(m, n, k, scale_dtype):
     assert (room == 7).all()
 
 
+@pytest.mark.parametrize("m", [127, 300])
+@pytest.mark.parametrize("scale_dtype", [E4, E8], ids=["16", "32"])
+def test_product_every_scale(scale_dtype, m):
+    """Each finite scale, subnormal ones among them, against a block of ones: a row's sum is its scale times the block's length."""
+    b = BLOCK[scale_dtype]
+    byte = torch.arange(m) % 127 if scale_dtype == E4 else 40 + torch.arange(m) % 170
+    scale = byte.to(torch.uint8).view(scale_dtype).double()
+    ones = torch.full((m, b // 2), 0x22, dtype=torch.uint8, device=DEV)
+    one = torch.full((1, 1), 0x38 if scale_dtype == E4 else 127)
+    sa, sb = tiled(byte[:, None]).view(scale_dtype).to(DEV), tiled(one.expand(40, 1)).view(scale_dtype).to(DEV)
+    want = (scale * b).float()[:, None].expand(m, 40)
+    assert torch.equal(st.matmul_fp4(ones, ones[:40].t(), sa, sb, out_dtype=torch.float32).cpu(), want)
+    assert torch.equal(st.matmul_fp4(ones[:40], ones.t(), sb, sa, out_dtype=torch.float32).cpu(), want.t())
+
+
 def test_product_nan_stays_in_its_row_and_column():
     x, w = torch.randn(40, 128, generator=gen(1)), torch.randn(300, 128, generator=gen(2))
     x[7, 100], w[129, 3] = float("nan"), float("inf")

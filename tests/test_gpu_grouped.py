@@ -57,7 +57,7 @@ CASES = [
 ]
 # a long contraction and few tiles: clusters split it; and groups of several tiles of CTA pairs
 CASES += [(40, 4096, 200, [7, 40]), (3, 8192, 64, [3]), (200, 2049, 130, [150, 200]), (3000, 64, 72, [3000]), (5000, 40, 136, [4000, 4001]),
-          (1300, 320, 1032, [700, 700, 1299]), (2600, 72, 776, [2113, 2600])]
+          (1300, 320, 1032, [700, 700, 1299]), (2600, 72, 776, [2113, 2600]), (2700, 136, 4104, [1, 18, 18, 340, 2641])]
 IDS = [f"{r}x{k}x{n}-{len(e)}" for r, k, n, e in CASES]
 
 
