@@ -178,20 +178,26 @@ struct BlockScale {
     float unit, inverse;
 };
 
+__device__ __forceinline__ float approximate_inverse(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
 template <bool WIDE>  // blocks of 32
 __device__ __forceinline__ BlockScale block_scale(float top, const Unit &u) {
-    if (!(top < INFINITY)) return BlockScale{WIDE ? 0xffu : 0x7fu, 0.0f, 0.0f};
+    const bool finite = top < INFINITY;
     if constexpr (WIDE) {
-        int e = top > 0.0f ? least_power(top, 1.5f, 2) : -127;
+        int e = least_power(top, 1.5f, 2);
         if (e < -127) e = -127;
-        return BlockScale{static_cast<uint32_t>(e + 127), power_of_two(e), power_of_two(-e)};
+        return finite ? BlockScale{static_cast<uint32_t>(e + 127), power_of_two(e), power_of_two(-e)} : BlockScale{0xffu, 0.0f, 0.0f};
     } else {
         // a sixth, correctly rounded: the product with the rounded inverse, corrected by its residual (see codes8)
         const float y = top * u.inverse, r = 1.0f / 6.0f, q = y * r;
         const uint32_t byte = __nv_cvt_float_to_fp8(__fmaf_rn(__fmaf_rn(q, -6.0f, y), r, q), __NV_SATFINITE, __NV_E4M3);
         const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
-        if (s == 0.0f) return BlockScale{0u, 0.0f, 0.0f};
-        return BlockScale{byte, s * u.t, __frcp_rn(s) * u.inverse};
+        const bool live = finite && s > 0.0f;
+        return BlockScale{finite ? byte : 0x7fu, live ? s * u.t : 0.0f, live ? approximate_inverse(s) * u.inverse : 0.0f};
     }
 }
 
@@ -211,8 +217,12 @@ __device__ __forceinline__ uint32_t to_fp4x8(const uint64_t (&f)[4]) {
 }
 
 // The codes of eight elements.  Blocks of 16: the quotient by s t is the
-// product with the rounded inverse, corrected once by its residual (Markstein
-// 1990), so that an element on a border between two codes is found there.  It
+// product with the inverse, corrected once by its residual (Markstein 1990), so
+// that an element on a border between two codes is found there.  (s has four
+// bits, so a quotient by it is a thirtieth of a step or more from the middle
+// between two fp32 numbers, unless it is on it; the corrected product is off by
+// about 2^-45 of itself, so it rounds like the quotient although the inverse is
+// only good to a step.)  It
 // is taken with the opposite sign, which is turned at the end: so a zero keeps
 // the sign that x - x would lose.
 template <bool WIDE>
@@ -237,9 +247,11 @@ __device__ __forceinline__ float max_abs8(float m, const uint64_t (&x)[4]) {
     return m;
 }
 
-// Where the scale of block b (of `quads` groups of four a row) of a row lies.
-__device__ __forceinline__ int64_t scale_at(int64_t row, int64_t b, int64_t quads) {
-    return ((row >> 7) * quads + (b >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (b & 3);
+// Where the scale of block b (of `quads` groups of four a row) of a row lies:
+// below 2^32, as a tensor that fits the GPU has fewer blocks.
+__device__ __forceinline__ uint32_t scale_at(int64_t row, int64_t b, int64_t quads) {
+    const uint32_t r = static_cast<uint32_t>(row), k = static_cast<uint32_t>(b);
+    return ((r >> 7) * static_cast<uint32_t>(quads) + (k >> 2)) * 512u + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (k & 3u);
 }
 
 // The 8 bytes of 16 codes, or those of the first n elements.
@@ -257,7 +269,7 @@ __device__ __forceinline__ void store_codes(uint8_t *to, uint32_t lo, uint32_t h
 // A lane holds 16 elements of a row, consecutive lanes consecutive ones: their
 // codes, and four lanes' (blocks of 32: eight lanes') scales as one word.
 // row / unit name the 16 elements; every lane of the warp comes here.
-template <bool WIDE>
+template <bool WIDE, bool WHOLE>
 __device__ __forceinline__ void quantize_unit(const Quantize4Args &p, const Unit &u, uint64_t (&x)[2][4], int64_t row,
                                               int64_t unit, int64_t quads, bool here, bool words) {
     if (!WIDE && u.lift != 1.0f) {
@@ -276,7 +288,11 @@ __device__ __forceinline__ void quantize_unit(const Quantize4Args &p, const Unit
     word |= __shfl_down_sync(0xffffffffu, word, 2 * step) << 16;
     if (!here) return;
     const int64_t left = p.cols - unit * 16;
-    if (row < p.rows && left > 0) store_codes(p.q + row * p.sq0 + unit * 8, lo, hi, left, words);
+    if (row < p.rows && left > 0) {
+        uint8_t *to = p.q + row * p.sq0 + unit * 8;
+        if constexpr (WHOLE) *reinterpret_cast<uint2 *>(to) = make_uint2(lo, hi);
+        else store_codes(to, lo, hi, left, words);
+    }
     const int64_t block = WIDE ? unit >> 1 : unit;
     if ((WIDE ? unit & 7 : unit & 3) == 0) *reinterpret_cast<uint32_t *>(p.scale + scale_at(row, block, quads)) = word;
 }
@@ -286,7 +302,8 @@ __device__ __forceinline__ void quantize_unit(const Quantize4Args &p, const Unit
 // CTAs walk the tensor from its end: the maximum has just passed over it from
 // the start, and the end is still in L2.  Rows are padded to 128 and a row's
 // blocks to four, as the scales are.
-template <typename T, bool WIDE>
+// WHOLE: rows are a multiple of 16 columns, their codes on 8-byte boundaries.
+template <typename T, bool WIDE, bool WHOLE>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3)
     quantize4_rows_kernel(const Quantize4Args p, uint32_t units, uint32_t across, uint32_t chunks, int64_t quads, bool words) {
     pdl_wait();
@@ -301,28 +318,29 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3)
         const T *src = static_cast<const T *>(p.a) + row0 * p.sa0 + unit * 16;
         uint4 raw[2][2][kWords];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+            const bool here = row0 + i < p.rows && left > 0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int k = 0; k < kWords; ++k) raw[i][h][k] = make_uint4(0, 0, 0, 0);
-                if (row0 + i >= p.rows) continue;
-                if (left >= 8 * h + 8) {
+                if (here && (WHOLE || left >= 8 * h + 8)) {
 #pragma unroll
                     for (int k = 0; k < kWords; ++k) raw[i][h][k] = __ldcs(reinterpret_cast<const uint4 *>(src + i * p.sa0 + 8 * h) + k);
-                } else {
+                } else if (!WHOLE && here) {
                     T *e = reinterpret_cast<T *>(raw[i][h]);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (8 * h + j < left) e[j] = src[i * p.sa0 + 8 * h + j];
                 }
             }
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             uint64_t x[2][4];
             unpack8(raw[i][0], x[0], T{});
             unpack8(raw[i][1], x[1], T{});
-            quantize_unit<WIDE>(p, u, x, row0 + i, unit, quads, unit < units, words);
+            quantize_unit<WIDE, WHOLE>(p, u, x, row0 + i, unit, quads, unit < units, words);
         }
     }
     pdl_trigger();
@@ -365,7 +383,7 @@ __global__ void __launch_bounds__(kThreads) quantize4_any_kernel(const Quantize4
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[h][j] = pack2(mine[17 * lane + 8 * h + 2 * j], mine[17 * lane + 8 * h + 2 * j + 1]);
         const int64_t unit = first / 16 + lane;
-        quantize_unit<WIDE>(p, u, x, row, unit, quads, unit < units, words);
+        quantize_unit<WIDE, false>(p, u, x, row, unit, quads, unit < units, words);
     }
     pdl_trigger();
 }
@@ -702,10 +720,15 @@ int launch_quantize(const Quantize4Args &p, int sm_count, cudaStream_t stream) {
             const bool words = reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.rows == 1 || p.sq0 % 8 == 0);
             const int64_t across = cdiv(units, 32), chunks = padded / 2 * across;
             if (chunks > INT32_MAX) return fail(ST_ERR_UNSUPPORTED, "quantize_fp4: too many blocks");
-            auto kern = quantize4_rows_kernel<T, WIDE>;
-            const unsigned grid = resident_grid<decltype(kern), T, std::bool_constant<WIDE>>(kern, cdiv(chunks, kWarps), sm_count, 0);
-            ST_CUDA_TRY(launch_kernel(kern, grid, kThreads, 0, stream, p, static_cast<uint32_t>(units), static_cast<uint32_t>(across),
-                                      static_cast<uint32_t>(chunks), quads, words));
+            auto go = [&](auto kern, auto whole) -> int {
+                const unsigned grid = resident_grid<decltype(kern), T, std::bool_constant<WIDE>, decltype(whole)>(kern, cdiv(chunks, kWarps),
+                                                                                                                  sm_count, 0);
+                ST_CUDA_TRY(launch_kernel(kern, grid, kThreads, 0, stream, p, static_cast<uint32_t>(units), static_cast<uint32_t>(across),
+                                          static_cast<uint32_t>(chunks), quads, words));
+                return ST_OK;
+            };
+            if (words && p.cols % 16 == 0) ST_TRY(go(quantize4_rows_kernel<T, WIDE, true>, std::true_type{}));
+            else ST_TRY(go(quantize4_rows_kernel<T, WIDE, false>, std::false_type{}));
             return checked("quantize4_rows_kernel");
         }
     } else if (p.sa0 == 1 && p.rows > 1) {
