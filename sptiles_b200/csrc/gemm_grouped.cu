@@ -253,6 +253,7 @@ struct GroupedCfg {
     static constexpr int kSmemBytes =
         kStages * kStageBytes + static_cast<int>(sizeof(GroupTable)) + kBarBytes + 1024;
     static_assert(kSmemBytes <= 232448, "over the per-block shared memory limit");
+    static_assert(kStages * kStageBytes >= kRows * (BN + 4 * 8) * 4, "the ring holds eight parts' sums of its columns");
 };
 
 // SPLIT: a cluster of p.split CTAs takes one tile, each every split-th step of
@@ -450,10 +451,11 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
         }
         __syncwarp();
         cluster_sync();  // every MMA of the cluster has read its ring
-        // a part owns `own` columns of the tile and gets them as [part][column][128 lanes]
-        const int own = BN / split, own_shift = 31 - __clz(own);  // split is a power of two
+        // A part owns `own` columns of the tile and gets them as [part][128 lanes][own + 4 columns].  (As [column][lane],
+        // one value a lane and store, the exchange of 64 columns between two parts took 5 us more.)
+        const int own = BN / split, own_shift = 31 - __clz(own), pitch = own + 4;  // split is a power of two
         if (out && any) {
-            const uint32_t mine = smem_addr(smem) + 4u * static_cast<uint32_t>(part * own * 128 + 32 * g + lane);
+            const uint32_t mine = smem_addr(smem) + 4u * static_cast<uint32_t>((part * 128 + 32 * g + lane) * pitch);
             for (int c = 32 * half; c < tile.cols; c += 64) {
                 uint32_t v[32];
                 if (!zero) {
@@ -464,10 +466,10 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
                     for (int i = 0; i < 32; ++i) v[i] = 0u;
                 }
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
+                for (int i = 0; i < 32; i += 4) {
                     const int col = c + i;
-                    const uint32_t to = map_to_rank(mine, static_cast<uint32_t>(col >> own_shift));
-                    st_cluster_f32(to + 512u * static_cast<uint32_t>(col & (own - 1)), __uint_as_float(v[i]));
+                    st_cluster_v4(map_to_rank(mine, static_cast<uint32_t>(col >> own_shift)) + 4u * static_cast<uint32_t>(col & (own - 1)),
+                                  __uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
                 }
                 __syncwarp();
             }
@@ -476,16 +478,26 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
         cluster_sync();
         if (out && any) {
             const int id = (warp - 2) * 32 + lane, n = tile.r0 + (id & 127);
-            const float *sums = reinterpret_cast<const float *>(smem) + (id & 127);
+            const float *sums = reinterpret_cast<const float *>(smem) + (id & 127) * pitch;
             const int64_t at = (WEIGHTS ? tile.group * p.c_g : 0) + tile.c0 * p.ldc + n;
             if (n < p.n)
-                for (int j = id >> 7; j < own && part * own + j < tile.cols; j += kOutWarps / 4) {
-                    float v = 0.0f;
-                    for (int q = 0; q < split; ++q) v += sums[(q * own + j) * 128];
-                    const int64_t to = at + (part * own + j) * p.ldc;
-                    if (p.c_dtype == ST_F32) static_cast<float *>(p.c)[to] = v;
-                    else if (p.c_dtype == ST_F16) from_float(v, static_cast<__half *>(p.c)[to]);
-                    else from_float(v, static_cast<__nv_bfloat16 *>(p.c)[to]);
+                for (int j = 4 * (id >> 7); j < own && part * own + j < tile.cols; j += kOutWarps) {
+                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int q = 0; q < split; ++q) {
+                        const float4 x = *reinterpret_cast<const float4 *>(sums + q * 128 * pitch + j);
+                        v[0] += x.x;
+                        v[1] += x.y;
+                        v[2] += x.z;
+                        v[3] += x.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (part * own + j + i >= tile.cols) break;
+                        const int64_t to = at + (part * own + j + i) * p.ldc;
+                        if (p.c_dtype == ST_F32) static_cast<float *>(p.c)[to] = v[i];
+                        else if (p.c_dtype == ST_F16) from_float(v[i], static_cast<__half *>(p.c)[to]);
+                        else from_float(v[i], static_cast<__nv_bfloat16 *>(p.c)[to]);
+                    }
                 }
         }
     }
@@ -913,30 +925,39 @@ int64_t most_tiles(const GroupedArgs &g, int64_t tiles_r, int cols) {
 }
 
 // Tile shape and split: the least estimated time for groups of equal size (what
-// the ends hold is not known here).  A stage of 64 along the contraction costs
-// an SM its MMAs or its loads, whichever is longer; the figures are SM cycles.
+// the ends hold is not known here).  The figures are microseconds fitted to
+// B200 timings of 1 x 4096 x 1024 to 16384 rows on 32 groups of 4096 x 4096: a
+// stage of 64 along the contraction, which few columns of a tile leave bound by
+// the SM's loads; a tile's way out, beside the next tile's stages; the join of
+// parts.  (32 rows of 8192 x 512, in a replayed graph: 33 us on 32 columns, with
+// 8 parts estimated 10.8, measured 10.3.)
 struct GroupedPlan {
     bool pair = false;
     int cols = 128;  // most columns of a tile
     int split = 1;
-    double cycles = 1e300;
+    double us = 1e300;
 };
 
 GroupedPlan plan_grouped(const GroupedArgs &g, int sm_count) {
     const int64_t met = g.groups < 1 ? 1 : !g.weights && g.rows < g.groups ? (g.rows > 0 ? g.rows : 1) : g.groups;
     const int64_t per_group = cdiv(g.rows > 0 ? g.rows : 1, met), blocks = cdiv(g.weights ? per_group : g.k, kBK);
+    constexpr double kLaunch = 2.5;
     GroupedPlan best;
     auto offer = [&](bool pair, int cols, int split) {
-        const int64_t extent = g.weights ? g.k : per_group, tiles_c = cdiv(extent, cols);
+        const int64_t extent = g.weights ? g.k : per_group, tiles_c = cdiv(extent, cols), tiles_r = cdiv(g.n, pair ? 256 : 128);
         const double c = g.weights ? cols : static_cast<double>(cdiv(cdiv(extent, tiles_c), 16) * 16);
-        const int64_t tiles_r = cdiv(g.n, pair ? 256 : 128);
-        if (split > 1 && (split > blocks || most_tiles(g, tiles_r, cols) * split > 4 * static_cast<int64_t>(sm_count))) return;
-        const double mma = 2 * c, load = 256 + (pair ? c : 2 * c);
-        const double join[] = {0, 2500, 3500, 5000};
-        const double t = static_cast<double>(cdiv(met * tiles_c * tiles_r * split, pair ? sm_count / 2 : sm_count)) *
-                         (static_cast<double>(cdiv(blocks, split)) * (mma > load ? mma : load) + 3000 +
-                          join[split == 8 ? 3 : split / 2]);
-        if (t < best.cycles) best = GroupedPlan{pair, cols, split, t};
+        const double stage = pair ? (c > 168 ? 0.00125 * c : 0.21) : 0.235 + 0.0004 * c, out = pair ? 0.5 + 0.006 * c : 0.4 + 0.006 * c;
+        const double sums = static_cast<double>(cdiv(blocks, split)) * stage;
+        double us;
+        if (split > 1) {  // every tile that there can be has a cluster, met or not
+            const double join[2][3] = {{3.8, 4.5, 4.5}, {6.2, 6.2, 7.5}};
+            const int64_t at_once = split == 8 ? 120 : split == 4 ? 140 : sm_count, ctas = most_tiles(g, tiles_r, cols) * split;
+            if (split > blocks || ctas > 4 * at_once) return;
+            us = static_cast<double>(cdiv(ctas, at_once)) * (kLaunch + sums + join[cols == 128][split == 2 ? 0 : split == 4 ? 1 : 2]);
+        } else {
+            us = kLaunch + static_cast<double>(cdiv(met * tiles_c * tiles_r, pair ? sm_count / 2 : sm_count)) * (sums > out ? sums : out) + out;
+        }
+        if (us < best.us) best = GroupedPlan{pair, cols, split, us};
     };
     for (int split = 1; split <= 8; split *= 2) {
         if (!g.weights) offer(false, 32, split);

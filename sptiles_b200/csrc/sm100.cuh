@@ -598,11 +598,8 @@ __device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
     return d;
 }
 
-// Store an f32 (below: four) to another CTA's shared memory of the cluster
+// Store four f32 to another CTA's shared memory of the cluster
 // (shared::cluster address); seen there after a cluster barrier.
-__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float a) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(a) : "memory");
-}
 __device__ __forceinline__ void st_cluster_v4(uint32_t cluster_addr, float a, float b, float c, float d) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "f"(a), "f"(b), "f"(c), "f"(d)
                  : "memory");
