@@ -46,6 +46,12 @@
 namespace st {
 namespace {
 
+// Measured, bf16: one group of 16384 rows of 4096 x 4096 340 to 355 us (1540 to
+// 1618 TFLOP/s), 32 unequal groups of them 410 over 20 calls and 505 over seconds
+// under the power cap (the tensor pipe 85 % busy); 64 rows on 64 groups of 2048 x
+// 4096 96 us, bound by the weights' bytes (92 at the copy rate); the gradient of
+// 32 x 2048 x 4096 in f32 from 16384 rows 281 to 356 (194), bound by its stores
+// beside the loads.
 constexpr int kMaxGroups = kGroupedMaxGroups;
 constexpr int kBK = 64;  // elements of the contraction a stage: 128 bytes, one swizzle span
 constexpr int kMmaK = 16;

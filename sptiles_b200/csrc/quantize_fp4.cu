@@ -13,6 +13,10 @@
 // scale NaN, and what is computed from it is NaN; t is taken over the finite
 // elements.
 //
+// Bound by DRAM: 8192 x 8192 bf16 in 29 us in blocks of 16 with a known maximum
+// and in 26 in blocks of 32 (26.2 at the copy rate); the maximum's own pass takes
+// 28; back to values 32 (26.2).
+//
 // Scales leave in the order in which the tensor core takes them:
 // [row / 128][block / 4][row % 32][row / 32 % 4][block % 4], one byte each,
 // zeros where a row or a block of that grid does not exist.

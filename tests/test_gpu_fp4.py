@@ -357,6 +357,29 @@ def test_product_empty_and_given_output():
             assert (room == 7).all()
 
 
+@pytest.mark.parametrize("scale_dtype", [E4, E8], ids=["16", "32"])
+def test_layer_forward_and_gradients(scale_dtype):
+    """y = x W^T and its gradients, each operand quantised along what is summed over, transposed views as they are
+    stored; each product against float64 on the values that its operands' codes stand for."""
+    tokens, n, k = 200, 136, 260
+    x, w, dy = (torch.randn(*s, generator=gen(i)).to(torch.bfloat16).to(DEV) for i, s in enumerate([(tokens, k), (n, k), (tokens, n)]))
+
+    def product(a, b):
+        qa, qb = st.quantize_fp4(a, scale_dtype=scale_dtype), st.quantize_fp4(b, scale_dtype=scale_dtype)
+        got = st.matmul_fp4(qa.codes, qb.codes.t(), qa.scale, qb.scale, a_tensor_scale=qa.tensor_scale, b_tensor_scale=qb.tensor_scale,
+                            out_dtype=torch.float32).double()
+        va, vb = (st.dequantize_fp4(*q, cols=t.shape[1], out_dtype=torch.float32).double() for q, t in ((qa, a), (qb, b)))
+        # a code is at most half a step off, a step at most a third of the block's largest value; e8m0 scales up to twice
+        assert ((va - a.double()).abs().amax() <= a.double().abs().amax() / 3).item()
+        slack = (a.shape[1] + 4) * 2.0 ** -23 * (va.abs() @ vb.abs().t())
+        assert ((got - va @ vb.t()).abs() <= slack * (1 + 2.0 ** -24) + 2.0 ** -24 * (va @ vb.t()).abs()).all()
+        return got
+
+    assert product(x, w).shape == (tokens, n)          # y
+    assert product(dy, w.t()).shape == (tokens, k)     # dx
+    assert product(dy.t(), x.t()).shape == (n, k)      # dW
+
+
 # ------------------------------------------------------------------ streams, graphs, long tensors
 def test_same_bits_streams_and_graphs():
     """Quantisers of both kinds into a product: two graphs with workspaces of their own, side by side."""
