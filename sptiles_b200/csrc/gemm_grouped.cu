@@ -19,8 +19,8 @@
 //
 // First form: B's columns are the rows of a tile and the group's rows its
 // columns, 16 to 256 of them: N is a field of the MMA's descriptor, so a group
-// is cut into tiles of equal size in steps of 16 and nothing is padded to 128
-// or 256 rows (16384 rows on 32 groups of 4096 x 4096, between 60 and 2400
+// is cut into tiles of equal size in steps of 16 (32 for a pair of CTAs, whose
+// M = 256 takes no other) and nothing is padded to 128 or 256 rows (16384 rows on 32 groups of 4096 x 4096, between 60 and 2400
 // rows each: 647 us with a group's rows as M).  The last columns of a tile may
 // be rows of the next group, or what an earlier tile left in shared memory:
 // columns of a product do not mix, and those are not stored.
@@ -135,6 +135,8 @@ struct Tile {
 // Tiles in order; each role walks them for itself.  ROWS, COLS: a tile's most.
 template <bool WEIGHTS, int ROWS, int COLS>
 struct TileWalk {
+    static constexpr int kStep = ROWS == 256 ? 32 : 16;  // of the MMA's N
+    static __device__ __forceinline__ uint32_t idesc_n(int cols) { return static_cast<uint32_t>((cols + kStep - 1) / kStep * (kStep / 8)) << 17; }
     int t, step, g = 0;
     __device__ __forceinline__ TileWalk(int first, int step) : t(first), step(step) {}
     __device__ __forceinline__ bool next(const GroupTable &table, const GroupedParams &p, Tile &out) {
@@ -157,7 +159,7 @@ struct TileWalk {
             out.cols = p.k - out.c0 < COLS ? p.k - out.c0 : COLS;
             out.blocks = (rows + kBK - 1) / kBK;
         } else {
-            const int even = ((rows + tiles_c - 1) / tiles_c + 15) / 16 * 16;  // columns of the group's tiles
+            const int even = ((rows + tiles_c - 1) / tiles_c + kStep - 1) / kStep * kStep;  // columns of the group's tiles
             out.c0 = begin + c * even;
             out.cols = rows - c * even < even ? rows - c * even : even;
             out.blocks = (p.k + kBK - 1) / kBK;
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
         while (ok && walk.next(table, p, tile)) {
             const int blocks = my_blocks(tile);
             if (blocks == 0) continue;
-            const uint32_t idesc = p.idesc | static_cast<uint32_t>(WEIGHTS ? BN / 8 : (tile.cols + 15) / 16 * 2) << 17;
+            const uint32_t idesc = p.idesc | Walk::idesc_n(WEIGHTS ? BN : tile.cols);
             if (!__all_sync(0xffffffffu, mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns))) {
                 ok = false;
                 break;
@@ -592,7 +594,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
     tc_fence_after_sync();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-    TileWalk<WEIGHTS, Cfg::kRows, Cfg::kCols> walk(static_cast<int>(blockIdx.x >> 1), static_cast<int>(gridDim.x >> 1));
+    using Walk = TileWalk<WEIGHTS, Cfg::kRows, Cfg::kCols>;
+    Walk walk(static_cast<int>(blockIdx.x >> 1), static_cast<int>(gridDim.x >> 1));
     Tile tile;
     if (warp == 0) {
         // ------------------------------------------------ TMA producer (both CTAs)
@@ -605,7 +608,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
             bool ok = true;
             while (ok && walk.next(table, p, tile)) {
                 // each CTA brings half of the tile's columns (rows of A)
-                const int half_c = (tile.cols + 15) / 16 * 8, high = (half_c + 31) / 32;
+                const int half_c = (tile.cols + 31) / 32 * 16, high = (half_c + 31) / 32;
                 for (int b = 0; b < tile.blocks; ++b, ++issued) {
                     if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.timeout_ns)) {
                         ok = false;
@@ -649,7 +652,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
             bool ok = true;
             while (ok && walk.next(table, p, tile)) {
                 if (tile.blocks == 0) continue;
-                const uint32_t idesc = p.idesc | static_cast<uint32_t>(WEIGHTS ? Cfg::kCols / 8 : (tile.cols + 15) / 16 * 2) << 17;
+                const uint32_t idesc = p.idesc | Walk::idesc_n(WEIGHTS ? Cfg::kCols : tile.cols);
                 if (!__all_sync(0xffffffffu, mbar_wait(tempty_bar(a), aph ^ 1u, abort_flag, p.timeout_ns))) {
                     ok = false;
                     break;
@@ -951,7 +954,7 @@ GroupedPlan plan_grouped(const GroupedArgs &g, int sm_count) {
     GroupedPlan best;
     auto offer = [&](bool pair, int cols, int split) {
         const int64_t extent = g.weights ? g.k : per_group, tiles_c = cdiv(extent, cols), tiles_r = cdiv(g.n, pair ? 256 : 128);
-        const double c = g.weights ? cols : static_cast<double>(cdiv(cdiv(extent, tiles_c), 16) * 16);
+        const double c = g.weights ? cols : static_cast<double>(cdiv(cdiv(extent, tiles_c), pair ? 32 : 16) * (pair ? 32 : 16));
         const double stage = pair ? (c > 168 ? 0.00125 * c : 0.21) : 0.235 + 0.0004 * c, out = pair ? 0.5 + 0.006 * c : 0.4 + 0.006 * c;
         const double sums = static_cast<double>(cdiv(blocks, split)) * stage;
         double us;

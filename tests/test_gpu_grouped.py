@@ -84,6 +84,21 @@ def test_rows_exact(rows, k, n, ends, layout):
     assert got.dtype == dtype and torch.equal(got.cpu(), want.float().to(dtype))
 
 
+@pytest.mark.parametrize("order", ["n", "k"])
+def test_tiles_of_every_size(order):
+    """Groups on both sides of each step of a tile's columns, for one CTA and for pairs."""
+    sizes = [1, 15, 16, 17, 31, 32, 33, 48, 49, 63, 64, 65, 95, 97, 127, 128, 129, 145, 160, 161, 191, 193, 224, 225, 240, 241, 255, 256,
+             257, 273, 300, 511]
+    ends = [sum(sizes[: i + 1]) for i in range(len(sizes))]
+    a = ints(3, ends[-1], 264)
+    for n in (72, 2056):
+        b = ints(4, len(ends), 264, n)
+        bd = b.to(BF16).to(DEV)
+        bd = bd if order == "n" else bd.transpose(1, 2).contiguous().transpose(1, 2)
+        got = st.matmul_grouped(a.to(BF16).to(DEV), bd, device_ends(ends), out_dtype=F32)
+        assert torch.equal(got.cpu(), plain(a, b, ends).float())
+
+
 @pytest.mark.parametrize("rows,k,n,ends", CASES, ids=IDS)
 def test_weights_exact(rows, k, n, ends):
     a, c = ints(1, rows, k), ints(2, rows, n)
