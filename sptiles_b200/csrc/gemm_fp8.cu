@@ -922,6 +922,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     atomicExch(p.err, kDevAbortGemmProducer);
                 }
                 if (rank == 0) drain_ring(issued, Cfg::kStages, full_bar, p.timeout_ns);  // both CTAs' copies
+                else drain_ring(issued, Cfg::kStages, empty_bar, p.timeout_ns);  // the even CTA's arrivals here
             }
         } else if (warp == 1) {
             // -------------------------------------------- MMA issuer (even CTA)
