@@ -348,7 +348,8 @@ int st_matmul_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
  * groups' rows hold.  An operand is read in place if it is contiguous along a
  * dimension (A of st_matmul_grouped along K; both operands of the second form
  * along their columns), with its rows and groups on 16-byte boundaries; any
- * other is copied first, into `workspace` (16-byte aligned). */
+ * other is copied first, into `workspace` (16-byte aligned).  Every buffer starts
+ * on a boundary of its elements; extents below 2^30. */
 int st_matmul_grouped_workspace(const st_tensor *a, const st_tensor *b, int64_t b_group_stride, int64_t groups, uint64_t *bytes);
 int st_matmul_grouped(st_ctx *ctx, const st_tensor *a, const st_tensor *b, int64_t b_group_stride, const st_tensor *ends,
                       const st_tensor *c, int32_t zero_rest, void *workspace, uint64_t workspace_bytes, const st_exec *exec);

@@ -960,6 +960,14 @@ int check_codes(const st_tensor *t, const char *name) {
     return ST_OK;
 }
 
+// A load or store of an element off its boundary is a fault of the device.
+int check_elements(const st_tensor &t, const char *name) {
+    const size_t es = dtype_size(t.dtype);
+    if (es > 1 && reinterpret_cast<uintptr_t>(t.data) % es != 0)
+        return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must start on a boundary of its elements");
+    return ST_OK;
+}
+
 // The scales of `rows` rows of `bytes` bytes of codes.
 int check_fp4_scale(const st_tensor *t, const char *name, int64_t rows, int64_t bytes) {
     if (!t) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " is null");
@@ -980,6 +988,7 @@ int scalar_of(const st_tensor *t, const char *name, float **out) {
     if (!t) return ST_OK;
     if (t->dtype != ST_F32 || t->rank != 1 || t->shape[0] != 1 || !t->data)
         return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be one ST_F32");
+    ST_TRY(check_elements(*t, name));
     *out = static_cast<float *>(t->data);
     return ST_OK;
 }
@@ -1021,7 +1030,7 @@ int check_ends(const st_tensor *t) {
         return fail(ST_ERR_UNSUPPORTED, "at most " + std::to_string(kGroupedMaxGroups) + " groups, got " + std::to_string(t->shape[0]));
     if (t->shape[0] > 1 && t->strides[0] != 1) return fail(ST_ERR_INVALID_ARGUMENT, "ends must be contiguous");
     if (t->shape[0] > 0 && !t->data) return fail(ST_ERR_INVALID_ARGUMENT, "ends has a null data pointer");
-    return ST_OK;
+    return check_elements(*t, "ends");
 }
 
 // A [rows, k] and, for one group, B [k, n] (weights: B [rows, n]).
@@ -1046,6 +1055,10 @@ int grouped_operands(const char *what, const st_tensor *a, const st_tensor *b, c
         return fail(ST_ERR_INVALID_ARGUMENT, "Incompatible matrices: K dimension of A (" + std::to_string(a->shape[1]) +
                                                  ") must match K dimension of B (" + std::to_string(b->shape[0]) + ")");
     if (b_group_stride < 0) return fail(ST_ERR_INVALID_ARGUMENT, std::string(b_name) + " has a negative group stride");
+    for (const int64_t extent : {a->shape[0], a->shape[1], b->shape[1]})  // sums of an extent and a tile's stay in int32
+        if (extent > INT32_MAX / 2) return fail(ST_ERR_UNSUPPORTED, std::string(what) + ": extents of at most " + std::to_string(INT32_MAX / 2));
+    ST_TRY(check_elements(*a, "A"));
+    if (b != &shape_of_b) ST_TRY(check_elements(*b, b_name));
     g->weights = weights;
     g->dtype = a->dtype;
     g->groups = groups;
@@ -1068,6 +1081,7 @@ int check_grouped_output(const st_tensor *c, const char *name, int64_t rows, int
         return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be [" + std::to_string(rows) + ", " + std::to_string(cols) + "]");
     if (!is_float(c->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, std::string(name) + " must be ST_F32, ST_F16 or ST_BF16");
     if (!unit_columns(*c)) return fail(ST_ERR_UNSUPPORTED, std::string(name) + " must have unit column stride");
+    ST_TRY(check_elements(*c, name));
     return check_output(*c, name);
 }
 
@@ -1753,6 +1767,7 @@ int st_quantize_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *q, const s
     ST_TRY(check_matrix(a, "A"));
     ST_TRY(check_codes(q, "Q"));
     if (!is_float(a->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp4: A must be ST_F32, ST_F16 or ST_BF16");
+    ST_TRY(check_elements(*a, "A"));
     if (q->shape[0] != a->shape[0] || q->shape[1] != cdiv(a->shape[1], 2))
         return fail(ST_ERR_INVALID_ARGUMENT, "quantize_fp4: Q must be [rows, ceil(cols / 2)] = [" + std::to_string(a->shape[0]) + ", " +
                                                  std::to_string(cdiv(a->shape[1], 2)) + "]");
@@ -1795,6 +1810,7 @@ int st_dequantize_fp4(st_ctx *ctx, const st_tensor *q, const st_tensor *scale, c
     if (out->shape[0] != q->shape[0] || cdiv(out->shape[1], 2) != q->shape[1])
         return fail(ST_ERR_INVALID_ARGUMENT, "dequantize_fp4: out must be [" + std::to_string(q->shape[0]) + ", " +
                                                  std::to_string(2 * q->shape[1]) + "], or a column less");
+    ST_TRY(check_elements(*out, "out"));
     ST_TRY(check_output(*out, "out"));
     Dequantize4Args g{};
     float *t = nullptr;
@@ -1853,6 +1869,7 @@ int st_matmul_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
                                                  std::to_string(g.b.rows) + "]");
     if (!is_float(c->dtype)) return fail(ST_ERR_INVALID_ARGUMENT, "C must be ST_F32, ST_F16 or ST_BF16");
     if (!unit_columns(*c)) return fail(ST_ERR_UNSUPPORTED, "C must have unit column stride");
+    ST_TRY(check_elements(*c, "C"));
     ST_TRY(check_output(*c, "C"));
     if (bias) {
         if (bias->rank != 1 || bias->shape[0] != g.b.rows)
@@ -1861,6 +1878,7 @@ int st_matmul_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
             return fail(ST_ERR_INVALID_ARGUMENT, "bias must be ST_F32 or C's dtype");
         if (bias->shape[0] > 1 && bias->strides[0] != 1) return fail(ST_ERR_UNSUPPORTED, "bias must be contiguous");
         if (bias->shape[0] > 0 && !bias->data) return fail(ST_ERR_INVALID_ARGUMENT, "bias has a null data pointer");
+        ST_TRY(check_elements(*bias, "bias"));
         g.bias = bias->data;
         g.bias_dtype = bias->dtype;
     }

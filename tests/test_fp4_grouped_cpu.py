@@ -218,3 +218,25 @@ def test_other_calls_refuse_4_bit_types():
     refused(N.lib().st_quantize_fp8(None, ref(t2(10, 300)), ref(t2(10, 300, Q4)), ref(t2(10, 3)), 1, 128, None), BAD, "Q must be")
     refused(N.lib().st_matmul_fp8(None, ref(t2(16, 256, Q4)), ref(t2(256, 32, Q4)), ref(t2(16, 2)), ref(t2(2, 32)), None, ref(t2(16, 32)),
                                   None, 0, None), BAD, "A and B must be")
+
+
+# ------------------------------------------------------------------ addresses and extents that a kernel could not take
+@pytest.mark.parametrize("call,kw,name", [
+    (quantize, dict(a=t2(10, 300, data=DATA + 2)), "A"), (quantize, dict(a=t2(10, 300, BF16, data=DATA + 1)), "A"),
+    (quantize, dict(amax=t1(1, data=DATA + 1)), "amax"), (quantize, dict(t=t1(1, data=DATA + 2)), "tensor_scale"),
+    (dequantize, dict(out=t2(10, 300, BF16, data=DATA + 1)), "out"), (dequantize, dict(t=t1(1, data=DATA + 2)), "tensor_scale"),
+    (product, dict(c=t2(16, 32, BF16, data=DATA + 1)), "C"), (product, dict(bias=t1(32, data=DATA + 2)), "bias"),
+    (product, dict(tb=t1(1, data=DATA + 1)), "b_tensor_scale"),
+    (grouped, dict(a=t2(16, 64, F16, data=DATA + 1)), "A"), (grouped, dict(b=t2(64, 32, F16, data=DATA + 1)), "B"),
+    (grouped, dict(ends=t1(4, I32, data=DATA + 2)), "ends"), (grouped, dict(c=t2(16, 32, data=DATA + 2)), "C"),
+    (weights, dict(c=t2(16, 32, F16, data=DATA + 1)), "C"), (weights, dict(d=t2(64, 32, data=DATA + 2)), "D"),
+])
+def test_elements_off_their_boundary(call, kw, name):
+    refused(call(**kw), BAD, name + " must start on a boundary of its elements")
+
+
+@pytest.mark.parametrize("extent", [2**30, 2**31 - 1])
+def test_extents_near_int32(extent):
+    refused(grouped(a=t2(extent, 64, F16), c=t2(extent, 32)), NOT, "extents of at most")
+    refused(grouped(b=t2(64, extent, F16), c=t2(16, extent)), NOT, "extents of at most")
+    refused(weights(a=t2(extent, 64, F16), c=t2(extent, 32, F16)), NOT, "extents of at most")
