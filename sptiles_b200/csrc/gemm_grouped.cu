@@ -47,9 +47,9 @@ namespace st {
 namespace {
 
 // Measured, bf16: one group of 16384 rows of 4096 x 4096 340 to 355 us (1540 to
-// 1618 TFLOP/s), 32 unequal groups of them 410 over 20 calls and 505 over seconds
+// 1618 TFLOP/s), 32 unequal groups of them 410 over 20 calls and 515 over seconds
 // under the power cap (the tensor pipe 85 % busy); 64 rows on 64 groups of 2048 x
-// 4096 96 us, bound by the weights' bytes (92 at the copy rate); the gradient of
+// 4096 98 us, bound by the weights' bytes (92 at the copy rate); the gradient of
 // 32 x 2048 x 4096 in f32 from 16384 rows 281 to 356 (194), bound by its stores
 // beside the loads.
 constexpr int kMaxGroups = kGroupedMaxGroups;
@@ -744,23 +744,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
 // Dense copy of strided 16-bit matrices, one for each group, into rows of `ld`
 // elements (a multiple of 8), padding columns zeroed: 8 elements a thread, put
 // together from the aligned words that hold them where they lie together.
-__global__ void __launch_bounds__(256) repack_groups_kernel(const uint16_t *__restrict__ src, int64_t sg, int64_t s0, int64_t s1,
-                                                            int64_t groups, int64_t rows, int64_t cols, uint16_t *__restrict__ dst,
-                                                            int64_t ld) {
+struct Repack {
+    const uint16_t *src;
+    int64_t sg, s0, s1;  // element strides of groups, rows and columns
+    int64_t groups, rows, cols;
+    uint16_t *dst;
+    int64_t ld;
+};
+// Both operands' copies in one launch, one for each blockIdx.y (1003 rows on 7 groups of 1001 x 515, both off their
+// boundaries: 19.4 us a call in two launches, 18.5 in one).
+struct Repacks {
+    Repack of[2];
+};
+
+__global__ void __launch_bounds__(256) repack_groups_kernel(const __grid_constant__ Repacks both) {
     pdl_wait();
-    const int64_t per_row = ld / 8, total = groups * rows * per_row;
+    const Repack &m = both.of[blockIdx.y];
+    const int64_t per_row = m.ld / 8, total = m.groups * m.rows * per_row;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t line = i / per_row, c = (i - line * per_row) * 8, g = line / rows, r = line - g * rows;
-        const uint16_t *from = src + g * sg + r * s0 + c * s1;
-        const int n = cols - c < 8 ? static_cast<int>(cols - c) : 8;
+        const int64_t line = i / per_row, c = (i - line * per_row) * 8, g = line / m.rows, r = line - g * m.rows;
+        const uint16_t *from = m.src + g * m.sg + r * m.s0 + c * m.s1;
+        const int n = m.cols - c < 8 ? static_cast<int>(m.cols - c) : 8;
         uint32_t w[4] = {0, 0, 0, 0};
-        if (s1 == 1) {
+        if (m.s1 == 1) {
             const uint32_t *words = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t(3));
             const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(from) >> 1) & 1, have = (odd + n + 1) / 2;
             uint32_t x[5];
 #pragma unroll
-            for (int j = 0; j < 5; ++j) x[j] = j < have ? words[j] : 0u;  // only words with an element of the row
+            for (int j = 0; j < 5; ++j) x[j] = j < have ? __ldg(words + j) : 0u;  // only words with an element of the row
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 w[j] = __funnelshift_r(x[j], x[j + 1], 16 * odd);
@@ -769,9 +781,9 @@ __global__ void __launch_bounds__(256) repack_groups_kernel(const uint16_t *__re
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (j < n) w[j / 2] |= static_cast<uint32_t>(from[j * s1]) << (16 * (j % 2));
+                if (j < n) w[j / 2] |= static_cast<uint32_t>(__ldg(from + j * m.s1)) << (16 * (j % 2));
         }
-        reinterpret_cast<uint4 *>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4 *>(m.dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
     pdl_trigger();
 }
@@ -804,24 +816,32 @@ Matrices layout(const void *data, int64_t groups, int64_t outer, int64_t inner, 
     return m;
 }
 
-int copy_in(Matrices &m, uint8_t *&ws, int sm_count, cudaStream_t stream) {
-    if (m.copy) {
-        const int64_t ld = (m.inner + 7) / 8 * 8, work = cdiv(m.groups * m.outer * (ld / 8), 256), most = static_cast<int64_t>(sm_count) * 8;
-        const int64_t grid = work < most ? work : most;
-        ST_CUDA_TRY(launch_kernel(repack_groups_kernel, static_cast<unsigned>(grid), 256, 0, stream,
-                                  static_cast<const uint16_t *>(m.data), m.sg, m.so, m.si, m.groups, m.outer, m.inner,
-                                  reinterpret_cast<uint16_t *>(ws), ld));
-        ST_TRY(checked("repack_groups_kernel"));
-        m.data = ws;
-        ws += m.copied();
-        m.so = ld;
-        m.sg = m.outer * ld;
+// The operands as the maps take them, copied where they have to be.
+int copy_in(Matrices &a, Matrices &b, uint8_t *ws, int sm_count, cudaStream_t stream) {
+    Repacks copies{};
+    int n = 0;
+    int64_t work = 0;
+    for (Matrices *m : {&a, &b}) {
+        if (m->copy) {
+            const int64_t ld = (m->inner + 7) / 8 * 8, mine = cdiv(m->groups * m->outer * (ld / 8), 256);
+            copies.of[n++] = Repack{static_cast<const uint16_t *>(m->data), m->sg, m->so, m->si, m->groups, m->outer, m->inner,
+                                    reinterpret_cast<uint16_t *>(ws), ld};
+            work = mine > work ? mine : work;
+            m->data = ws;
+            ws += m->copied();
+            m->so = ld;
+            m->sg = m->outer * ld;
+        }
+        m->si = 1;
+        // strides that are never used still have to be valid ones
+        if (m->outer == 1) m->so = (m->inner + 7) / 8 * 8;
+        if (m->groups == 1) m->sg = (m->outer * m->so + 7) / 8 * 8;
     }
-    m.si = 1;
-    // strides that are never used still have to be valid ones
-    if (m.outer == 1) m.so = (m.inner + 7) / 8 * 8;
-    if (m.groups == 1) m.sg = (m.outer * m.so + 7) / 8 * 8;
-    return ST_OK;
+    if (n == 0) return ST_OK;
+    const int64_t most = static_cast<int64_t>(sm_count) * 8;
+    const dim3 grid(static_cast<unsigned>(work < most ? work : most), static_cast<unsigned>(n));
+    ST_CUDA_TRY(launch_kernel(repack_groups_kernel, grid, 256, 0, stream, copies));
+    return checked("repack_groups_kernel");
 }
 
 struct Operands {
@@ -1016,9 +1036,7 @@ int launch_gemm_grouped(const GroupedArgs &g, void *workspace, int sm_count, int
     // with nothing to sum over (k = 0, no groups, or no rows) no operand is read
     if (g.rows > 0 && g.k > 0 && g.groups > 0) {
         o = operands_of(g);
-        uint8_t *ws = static_cast<uint8_t *>(workspace);
-        ST_TRY(copy_in(o.a, ws, sm_count, stream));
-        ST_TRY(copy_in(o.b, ws, sm_count, stream));
+        ST_TRY(copy_in(o.a, o.b, static_cast<uint8_t *>(workspace), sm_count, stream));
         if (g.weights) {
             // (column, position in a step of 64 rows, the step's first row): positions reach behind the last
             // row in the map's extents, but no step's box does
