@@ -25,11 +25,10 @@
 // be rows of the next group, or what an earlier tile left in shared memory:
 // columns of a product do not mix, and those are not stored.
 //
-// Second form: the rows are what is summed over, so a group's last, shorter
-// step must read zeros beside its own rows: the row dimension of the tensor
-// map is split in two of equal stride, (position in the step, first row of the
-// step), and a step of n < 64 rows starts at position n - 64, whose first
-// 64 - n rows lie outside of the map and read as zeros.
+// Second form: the rows are what is summed over, and a group's last, shorter
+// step of n < 64 rows brings rows of the next group too.  It takes ceil(n / 16)
+// MMAs of 16 rows, and of the last one's rows those behind the group are set to
+// zero in shared memory first, in both operands (a product with a NaN is one).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -168,6 +167,26 @@ struct TileWalk {
         return true;
     }
 };
+
+// The step's rows that belong to the group, and whether its last MMA meets others.
+struct Step {
+    int mmas;
+    bool mixed;
+    __device__ __forceinline__ explicit Step(int left) : mmas(left < kBK ? (left + kMmaK - 1) / kMmaK : kBK / kMmaK), mixed(left < kBK && left % kMmaK != 0) {}
+};
+
+// By a warp: rows from `left` on of its last MMA become 0 in a stage, 2 x 128
+// columns in 64s of 64 rows, and the tensor core sees it.  (A swizzled row's
+// units stay within its 128 bytes.)
+__device__ __forceinline__ void zero_behind(uint32_t stage, int left, int lane) {
+    const int units = (kMmaK - left % kMmaK) * 4 * 8;  // of 16 bytes
+    for (int i = lane; i < units; i += 32) {
+        const int line = i >> 3, row = left + (line >> 2);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage + (line & 3) * (64 * 128) + row * 128 + (i & 7) * 16), "r"(0) : "memory");
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
 
 // 128 columns (64s of a swizzle span each) x 64 rows of an operand that lies
 // along its columns.  y and z: the map's other coordinates.  (Two boxes a
@@ -340,10 +359,9 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
                     const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes), sc = sr + Cfg::kRowBytes;
                     if constexpr (WEIGHTS) {
                         mbar_arrive_expect_tx(fb, Cfg::kStageBytes);
-                        const int left = tile.rows - b * kBK, y = left < kBK ? left - kBK : 0, z = tile.first + b * kBK;
                         static_assert(!WEIGHTS || BN == 128, "columns in two 64s");
-                        load_columns<false>(sr, &tmap_r, fb, tile.r0, y, z, p.r_by_64, pol);
-                        load_columns<false>(sc, &maps_c.by32[0], fb, tile.c0, y, z, p.c_by_64, pol);
+                        load_columns<false>(sr, &tmap_r, fb, tile.r0, tile.first + b * kBK, 0, p.r_by_64, pol);
+                        load_columns<false>(sc, &maps_c.by32[0], fb, tile.c0, tile.first + b * kBK, 0, p.c_by_64, pol);
                     } else {
                         mbar_arrive_expect_tx(fb, static_cast<uint32_t>(Cfg::kRowBytes + high * 32 * 128));
                         const int g = p.b_groups ? tile.group : 0;
@@ -384,6 +402,8 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
                     ok = false;
                     break;
                 }
+                const Step step(WEIGHTS ? tile.rows - (part + b * split) * kBK : kBK);
+                if (WEIGHTS && step.mixed) zero_behind(smem_addr(smem + s * Cfg::kStageBytes), tile.rows % kBK, lane);
                 tc_fence_after_sync();
                 if (elect_one()) {
                     const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes), sc = sr + Cfg::kRowBytes;
@@ -391,8 +411,9 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
                     const uint64_t dc = smem_desc_sw128(sc, WEIGHTS ? 64 * 128 : 16, 1024);
 #pragma unroll
                     for (int j = 0; j < kBK / kMmaK; ++j)
-                        tc_mma<false>(tmem_base + static_cast<uint32_t>(a * BN), dr + j * ((R_MN ? kMmaK * 128 : 32) >> 4),
-                                      dc + j * ((WEIGHTS ? kMmaK * 128 : 32) >> 4), idesc, (b | j) != 0 ? 1u : 0u);
+                        if (!WEIGHTS || j < step.mmas)
+                            tc_mma<false>(tmem_base + static_cast<uint32_t>(a * BN), dr + j * ((R_MN ? kMmaK * 128 : 32) >> 4),
+                                          dc + j * ((WEIGHTS ? kMmaK * 128 : 32) >> 4), idesc, (b | j) != 0 ? 1u : 0u);
                     tc_commit(empty_bar(s));
                     if (b + 1 == blocks) tc_commit(tfull_bar(a));
                 }
@@ -527,7 +548,10 @@ __global__ void __launch_bounds__(GroupedCfg<BN>::kThreads, 1)
 //
 // full[s] lives in the even CTA and counts both CTAs' loads; the even CTA's
 // MMA warp commits empty[s] and tfull[a] to both CTAs; tempty[a] lives in the
-// even CTA and counts the pair's warps that read accumulators.
+// even CTA and counts the pair's warps that read accumulators.  A step whose
+// rows are mixed (second form): the odd CTA's loads complete its own landed[s],
+// its second warp sets the rows behind the group to zero and arrives at the even
+// CTA's cleared[s].
 struct GroupedPairCfg {
     static constexpr int kRows = 256, kCols = 256;
     static constexpr int kThreads = 32 * (2 + kOutWarps);
@@ -551,7 +575,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     GroupTable &table = *reinterpret_cast<GroupTable *>(smem + Cfg::kStages * Cfg::kStageBytes);
     uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(&table) + sizeof(GroupTable));
-    constexpr int kBars = 2 * Cfg::kStages + 5;
+    constexpr int kBars = 4 * Cfg::kStages + 5;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -563,12 +587,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
     auto empty_bar = [&](int s) { return bar0 + 8u * (Cfg::kStages + s); };
     auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + a); };
     auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * Cfg::kStages + 2 + a); };
+    auto landed_bar = [&](int s) { return bar0 + 8u * (2 * Cfg::kStages + 4 + s); };
+    auto cleared_bar = [&](int s) { return bar0 + 8u * (3 * Cfg::kStages + 4 + s); };
     const uint32_t drain_bar = bar0 + 8u * (kBars - 1);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
+            mbar_init(landed_bar(s), 1);
+            mbar_init(cleared_bar(s), 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull_bar(a), 1);
@@ -604,7 +632,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
             const uint32_t even_full0 = map_to_rank(full_bar(0), 0);
             const int half = static_cast<int>(rank) * 128;
             int s = 0, issued = 0;
-            uint32_t ph = 0;
+            uint32_t ph = 0, uses = 0, landed_ph = 0;  // a bit for each landed[s]: waited for, and its next parity
             bool ok = true;
             while (ok && walk.next(table, p, tile)) {
                 // each CTA brings half of the tile's columns (rows of A)
@@ -617,10 +645,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
                     const uint32_t fb = even_full0 + 8u * s;
                     const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes), sc = sr + Cfg::kRowBytes;
                     if constexpr (WEIGHTS) {
-                        if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * Cfg::kStageBytes);
-                        const int left = tile.rows - b * kBK, y = left < kBK ? left - kBK : 0, z = tile.first + b * kBK;
-                        load_columns<true>(sr, &tmap_r, fb, tile.r0 + half, y, z, p.r_by_64, pol);
-                        load_columns<true>(sc, &maps_c.by32[0], fb, tile.c0 + half, y, z, p.c_by_64, pol);
+                        const Step step(tile.rows - b * kBK);
+                        const int y = tile.first + b * kBK;
+                        uint32_t bar = fb;
+                        if (rank == 0) {
+                            mbar_arrive_expect_tx(full_bar(s), step.mixed ? Cfg::kStageBytes : 2 * Cfg::kStageBytes);
+                        } else if (step.mixed) {
+                            bar = landed_bar(s);
+                            mbar_arrive_expect_tx(bar, Cfg::kStageBytes);
+                            uses |= 1u << s;
+                            landed_ph ^= 1u << s;
+                        }
+                        load_columns<true>(sr, &tmap_r, bar, tile.r0 + half, y, 0, p.r_by_64, pol);
+                        load_columns<true>(sc, &maps_c.by32[0], bar, tile.c0 + half, y, 0, p.c_by_64, pol);
                     } else {
                         if (rank == 0)
                             mbar_arrive_expect_tx(full_bar(s), static_cast<uint32_t>(2 * (Cfg::kRowBytes + high * 32 * 128)));
@@ -644,12 +681,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
             }
             if (rank == 0) drain_ring(issued, Cfg::kStages, full_bar, p.timeout_ns);  // both CTAs' copies
             else drain_ring(issued, Cfg::kStages, empty_bar, p.timeout_ns);  // the even CTA's arrivals here
+            if constexpr (WEIGHTS) {
+                const volatile int never = 0;
+                for (int i = 0; i < Cfg::kStages; ++i)  // copies that landed[i] counts
+                    if (uses >> i & 1u) (void)mbar_wait(landed_bar(i), (landed_ph >> i & 1u) ^ 1u, &never, p.timeout_ns);
+            }
         }
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer (even CTA)
         if (rank == 0) {
             int s = 0, a = 0;
-            uint32_t ph = 0, aph = 0;
+            uint32_t ph = 0, aph = 0, cleared_ph = 0;  // a bit for each cleared[s]
             bool ok = true;
             while (ok && walk.next(table, p, tile)) {
                 if (tile.blocks == 0) continue;
@@ -663,6 +705,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
                         ok = false;
                         break;
                     }
+                    const Step step(WEIGHTS ? tile.rows - b * kBK : kBK);
+                    if (WEIGHTS && step.mixed) {
+                        zero_behind(smem_addr(smem + s * Cfg::kStageBytes), tile.rows % kBK, lane);
+                        if (!__all_sync(0xffffffffu, mbar_wait_cluster(cleared_bar(s), cleared_ph >> s & 1u, abort_flag, p.timeout_ns))) {
+                            ok = false;
+                            break;
+                        }
+                        cleared_ph ^= 1u << s;
+                    }
                     tc_fence_after_sync();
                     if (elect_one()) {
                         const uint32_t sr = smem_addr(smem + s * Cfg::kStageBytes), sc = sr + Cfg::kRowBytes;
@@ -670,9 +721,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
                         const uint64_t dc = smem_desc_sw128(sc, WEIGHTS ? 64 * 128 : 16, 1024);
 #pragma unroll
                         for (int j = 0; j < kBK / kMmaK; ++j)
-                            tc_mma_pair<false>(tmem_base + static_cast<uint32_t>(a * Cfg::kCols),
-                                               dr + j * ((R_MN ? kMmaK * 128 : 32) >> 4),
-                                               dc + j * ((WEIGHTS ? kMmaK * 128 : 32) >> 4), idesc, (b | j) != 0 ? 1u : 0u);
+                            if (!WEIGHTS || j < step.mmas)
+                                tc_mma_pair<false>(tmem_base + static_cast<uint32_t>(a * Cfg::kCols),
+                                                   dr + j * ((R_MN ? kMmaK * 128 : 32) >> 4),
+                                                   dc + j * ((WEIGHTS ? kMmaK * 128 : 32) >> 4), idesc, (b | j) != 0 ? 1u : 0u);
                         tc_commit_pair_multicast(empty_bar(s), 3);
                         if (b + 1 == tile.blocks) tc_commit_pair_multicast(tfull_bar(a), 3);
                     }
@@ -694,6 +746,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
             if (elect_one()) tc_commit_pair(drain_bar);
             __syncwarp();
             drain_ring(1, 1, [&](int) { return drain_bar; }, p.timeout_ns);  // the MMAs read shared memory and write TMEM
+        } else if constexpr (WEIGHTS) {
+            // -------------------------------------------- zeros behind a group's last rows (odd CTA)
+            const uint32_t even_cleared0 = map_to_rank(cleared_bar(0), 0);
+            int s = 0;
+            uint32_t landed_ph = 0;
+            bool ok = true;
+            while (ok && walk.next(table, p, tile)) {
+                for (int b = 0; b < tile.blocks; ++b) {
+                    if (Step(tile.rows - b * kBK).mixed) {
+                        if (!__all_sync(0xffffffffu, mbar_wait(landed_bar(s), landed_ph >> s & 1u, abort_flag, p.timeout_ns))) {
+                            ok = false;
+                            break;
+                        }
+                        landed_ph ^= 1u << s;
+                        zero_behind(smem_addr(smem + s * Cfg::kStageBytes), tile.rows % kBK, lane);
+                        if (lane == 0) mbar_arrive_cluster_release(even_cleared0 + 8u * s);
+                    }
+                    if (++s == Cfg::kStages) s = 0;
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                if (lane == 0) atomicExch(p.err, kDevAbortGemmMma);
+            }
+            __syncwarp();
         }
     } else {
         // ------------------------------------------------ C (both CTAs)
@@ -1038,10 +1115,8 @@ int launch_gemm_grouped(const GroupedArgs &g, void *workspace, int sm_count, int
         o = operands_of(g);
         ST_TRY(copy_in(o.a, o.b, static_cast<uint8_t *>(workspace), sm_count, stream));
         if (g.weights) {
-            // (column, position in a step of 64 rows, the step's first row): positions reach behind the last
-            // row in the map's extents, but no step's box does
-            ST_TRY(make_map_columns(&mr, &p.r_by_64, g.dtype, "C", o.b.data, g.n, kBK, g.rows, o.b.so, o.b.so));
-            ST_TRY(make_map_columns(&mc.by32[0], &p.c_by_64, g.dtype, "A", o.a.data, g.k, kBK, g.rows, o.a.so, o.a.so));
+            ST_TRY(make_map_columns(&mr, &p.r_by_64, g.dtype, "C", o.b.data, g.n, g.rows, 1, o.b.so, o.b.sg));
+            ST_TRY(make_map_columns(&mc.by32[0], &p.c_by_64, g.dtype, "A", o.a.data, g.k, g.rows, 1, o.a.so, o.a.sg));
         } else {
             for (int i = 0; i < 4; ++i)
                 ST_TRY(make_map_16(&mc.by32[i], g.dtype, "A", 2, o.a.data, g.k, g.rows, 1, o.a.so, 0, kBK, 32 * (i + 1)));

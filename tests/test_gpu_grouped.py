@@ -112,6 +112,21 @@ def test_weights_exact(rows, k, n, ends):
     assert torch.equal(st.matmul_grouped_weights(*turned, device_ends(ends), out_dtype=F32).cpu(), want.float())
 
 
+@pytest.mark.parametrize("k,n", [(72, 136), (264, 520), (1032, 2056)])
+def test_weights_last_steps(k, n):
+    """Last steps of 1 to 64 rows, beside rows of other groups that hold NaN and infinities."""
+    sizes = [s for i in range(1, 65) for s in (i if i % 2 else 64 + i, 1 + i % 5)]
+    ends = [sum(sizes[: i + 1]) for i in range(len(sizes))]
+    a, c = ints(5, ends[-1] + 9, k), ints(6, ends[-1] + 9, n)
+    want = plain_weights(a, c, ends)
+    for i, (x, y) in enumerate(parts(ends, a.shape[0])):
+        if i % 2:
+            a[x:y], c[x:y] = float("nan"), float("inf")
+    a[ends[-1]:], c[ends[-1]:] = float("inf"), float("nan")
+    got = st.matmul_grouped_weights(a.to(BF16).to(DEV), c.to(BF16).to(DEV), device_ends(ends), out_dtype=F32).cpu()
+    assert torch.equal(got[::2], want[::2].float()) and got[1::2].isnan().all()
+
+
 def test_other_groups_do_not_matter():
     """NaN and infinities in one group's rows, in its matrix and behind the last group stay there."""
     ends = [70, 133, 200, 260]
