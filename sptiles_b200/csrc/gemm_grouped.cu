@@ -12,8 +12,8 @@
 //
 //   warp 0      TMA producer
 //   warp 1      MMA issuer (owns the TMEM allocation)
-//   warps 2-5   C: TMEM -> registers -> shared memory -> rows of C, while the
-//               MMAs of the next tile fill the other accumulator
+//   warps 2-9   C: TMEM -> registers -> columns of a tile, while the MMAs of
+//               the next tile fill the other accumulator
 //
 // The kernels know a row operand (the MMA's M) and a column operand (its N).
 //
@@ -49,7 +49,7 @@ namespace {
 // 1618 TFLOP/s), 32 unequal groups of them 410 over 20 calls and 515 over seconds
 // under the power cap (the tensor pipe 85 % busy); 64 rows on 64 groups of 2048 x
 // 4096 98 us, bound by the weights' bytes (92 at the copy rate); the gradient of
-// 32 x 2048 x 4096 in f32 from 16384 rows 281 to 356 (194), bound by its stores
+// 32 x 2048 x 4096 in f32 from 16384 rows 364 to 374 (194), bound by its stores
 // beside the loads.
 constexpr int kMaxGroups = kGroupedMaxGroups;
 constexpr int kBK = 64;  // elements of the contraction a stage: 128 bytes, one swizzle span

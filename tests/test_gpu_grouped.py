@@ -127,6 +127,18 @@ def test_weights_last_steps(k, n):
     assert torch.equal(got[::2], want[::2].float()) and got[1::2].isnan().all()
 
 
+def test_weights_last_steps_on_pairs():
+    sizes = [7, 900, 17, 880, 33, 850, 48, 840, 63, 830, 500, 517, 530, 547, 575, 600]
+    ends = [sum(sizes[: i + 1]) for i in range(len(sizes))]
+    a, c = ints(7, ends[-1], 520), ints(8, ends[-1], 1032)
+    want = plain_weights(a, c, ends)
+    for i, (x, y) in enumerate(parts(ends, a.shape[0])):
+        if i % 2:
+            a[x:y], c[x:y] = float("inf"), float("nan")
+    got = st.matmul_grouped_weights(a.to(F16).to(DEV), c.to(F16).to(DEV), device_ends(ends), out_dtype=F32).cpu()
+    assert torch.equal(got[::2], want[::2].float()) and got[1::2].isnan().all()
+
+
 def test_other_groups_do_not_matter():
     """NaN and infinities in one group's rows, in its matrix and behind the last group stay there."""
     ends = [70, 133, 200, 260]
