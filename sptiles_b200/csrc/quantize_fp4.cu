@@ -81,8 +81,8 @@ __device__ __forceinline__ float block_max(float m, float *shared) {
 
 // ---------------------------------------------------------------- the tensor's largest |a|
 // One maximum per CTA; the quantiser's CTAs reduce them.  A NaN loses every
-// comparison; a maximum that comes out infinite is taken again over the finite
-// elements.
+// comparison; a CTA whose maximum comes out infinite takes it again, over the
+// finite ones of the elements that it has read.
 __device__ __forceinline__ float max_of_word(float m, const uint4 &w, float) {
     m = fmaxf(fmaxf(m, fabsf(__uint_as_float(w.x))), fabsf(__uint_as_float(w.y)));
     return fmaxf(fmaxf(m, fabsf(__uint_as_float(w.z))), fabsf(__uint_as_float(w.w)));
@@ -142,11 +142,23 @@ __global__ void __launch_bounds__(kThreads) amax_kernel(const T *a, int64_t s0, 
         }
     }
     m = block_max(m, shared);
-    if (m == INFINITY) {
+    if (m == INFINITY) {  // the elements of this CTA again: of the same words, as no other CTA has seen them
         m = 0.0f;
-        for (int64_t i = first; i < rows * cols; i += stride) {
-            const int64_t r = i / cols;
-            m = finite_abs(m, to_float(a[r * s0 + (i - r * cols) * s1]));
+        if constexpr (WORDS) {
+            constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+            const int64_t per_row = cols / kVec, tail = per_row * kVec, left = cols - tail;
+            for (int64_t i = first; i < rows * per_row; i += stride) {
+                const int64_t r = i / per_row;
+                const uint4 w = *reinterpret_cast<const uint4 *>(a + r * s0 + (i - r * per_row) * kVec);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) m = finite_abs(m, to_float(reinterpret_cast<const T *>(&w)[j]));
+            }
+            for (int64_t i = first; i < rows * left; i += stride) m = finite_abs(m, to_float(a[i / left * s0 + tail + i % left]));
+        } else {
+            for (int64_t i = first; i < rows * cols; i += stride) {
+                const int64_t r = i / cols;
+                m = finite_abs(m, to_float(a[r * s0 + (i - r * cols) * s1]));
+            }
         }
         m = block_max(m, shared);
     }

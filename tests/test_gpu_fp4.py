@@ -496,3 +496,26 @@ def test_product_many_results():
     ones = torch.full((last, k // 16), 0x38)
     va, vb = (values(split(t[-last:].cpu(), k)[0], ones, None, E4) for t in (a, b))
     assert torch.equal(c[-last:, -last:].cpu(), (va @ vb.t()).float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("src", SRC, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout", ["rows", "columns behind the last word", "transposed", "strided"])
+def test_maximum_beside_infinities(layout, src):
+    """The largest finite element counts wherever it lies, also among the elements that a CTA takes together with an infinity."""
+    rows, cols = 2050, 4096
+    base = torch.empty(rows, cols + 8, dtype=src, device=DEV).uniform_(-1, 1)
+    x = {"rows": base[:, :cols], "columns behind the last word": base[:, : cols + 3], "transposed": base[:, :cols].t(),
+         "strided": base[:, ::2]}[layout]
+    odd = base.shape[1] // 2 - 1 if layout == "strided" else x.shape[1] - 1
+    last = (x.shape[0] - 1, odd)
+    # 2000 and 1500: a CTA's first 16-byte words hold the first 1024 elements of f32, or 2048 of 16 bits
+    first = [(j, 0) if layout == "transposed" else (0, j) for j in (1, 255, 256, 300, 777, 1023, 1500, 2000)]
+    for at in [*first, (1, 1), (3, odd), (odd % x.shape[0], 7), last]:
+        for bad in (float("inf"), float("-inf")):
+            kept = x[at].clone(), x[0, 0].clone()
+            x[at], x[0, 0] = 1000.0, bad
+            assert st.quantize_fp4(x).tensor_scale.item() == 0.5, at  # 2688 / 2 >= 1000 > 2688 / 4
+            x[at], x[0, 0] = kept
+    x[::7, ::5] = float("inf")
+    x[last] = 1000.0
+    assert st.quantize_fp4(x).tensor_scale.item() == 0.5
