@@ -101,6 +101,33 @@ __device__ __forceinline__ float end_of(float m) { return m; }
 __device__ __forceinline__ float end_of(__half2 m) { return fmaxf(__low2float(m), __high2float(m)); }
 __device__ __forceinline__ float end_of(__nv_bfloat162 m) { return fmaxf(__low2float(m), __high2float(m)); }
 
+// A thread's maximum over the finite ones of the elements that amax_kernel has
+// it read: of the same words, as no other CTA has seen them.  (Its loops
+// unrolled it takes registers from the first pass: 8192 x 8192 f32 93 -> 95 us a call.)
+template <typename T, bool WORDS>
+__device__ __forceinline__ float finite_max(const T *a, int64_t s0, int64_t s1, int64_t rows, int64_t cols, int64_t first, int64_t stride) {
+    float m = 0.0f;
+    if constexpr (WORDS) {
+        constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+        const int64_t per_row = cols / kVec, tail = per_row * kVec, left = cols - tail;
+#pragma unroll 1
+        for (int64_t i = first; i < rows * per_row; i += stride) {
+            const T *word = a + i / per_row * s0 + i % per_row * kVec;
+#pragma unroll 1
+            for (int j = 0; j < kVec; ++j) m = finite_abs(m, to_float(word[j]));
+        }
+#pragma unroll 1
+        for (int64_t i = first; i < rows * left; i += stride) m = finite_abs(m, to_float(a[i / left * s0 + tail + i % left]));
+    } else {
+#pragma unroll 1
+        for (int64_t i = first; i < rows * cols; i += stride) {
+            const int64_t r = i / cols;
+            m = finite_abs(m, to_float(a[r * s0 + (i - r * cols) * s1]));
+        }
+    }
+    return m;
+}
+
 template <typename T, bool WORDS>
 __global__ void __launch_bounds__(kThreads) amax_kernel(const T *a, int64_t s0, int64_t s1, int64_t rows, int64_t cols,
                                                         float *maxima) {
@@ -142,26 +169,7 @@ __global__ void __launch_bounds__(kThreads) amax_kernel(const T *a, int64_t s0, 
         }
     }
     m = block_max(m, shared);
-    if (m == INFINITY) {  // the elements of this CTA again: of the same words, as no other CTA has seen them
-        m = 0.0f;
-        if constexpr (WORDS) {
-            constexpr int kVec = 16 / static_cast<int>(sizeof(T));
-            const int64_t per_row = cols / kVec, tail = per_row * kVec, left = cols - tail;
-            for (int64_t i = first; i < rows * per_row; i += stride) {
-                const int64_t r = i / per_row;
-                const uint4 w = *reinterpret_cast<const uint4 *>(a + r * s0 + (i - r * per_row) * kVec);
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) m = finite_abs(m, to_float(reinterpret_cast<const T *>(&w)[j]));
-            }
-            for (int64_t i = first; i < rows * left; i += stride) m = finite_abs(m, to_float(a[i / left * s0 + tail + i % left]));
-        } else {
-            for (int64_t i = first; i < rows * cols; i += stride) {
-                const int64_t r = i / cols;
-                m = finite_abs(m, to_float(a[r * s0 + (i - r * cols) * s1]));
-            }
-        }
-        m = block_max(m, shared);
-    }
+    if (m == INFINITY) m = block_max(finite_max<T, WORDS>(a, s0, s1, rows, cols, first, stride), shared);
     if (threadIdx.x == 0) maxima[blockIdx.x] = m;
     pdl_trigger();
 }
