@@ -178,7 +178,23 @@ __global__ void __launch_bounds__(kThreads) amax_kernel(const T *a, int64_t s0, 
 struct Unit {
     float t, inverse;   // a power of two and its inverse, both times (over) lift
     float lift;         // elements are multiplied by it first: 1, or 2^100 for tensors so small that t / 448 is subnormal
+    float usual;        // a block with a larger maximum (or a NaN) goes through limit_top and limit8
 };
+
+// What blocks beyond u.usual take first.  8192 t is more than three times what
+// t provides for: from there on the block's scale is the largest one and the
+// element's code too, whatever is above, so that elements are taken as 8192 t
+// (infinite for the largest t) and nothing behind this overflows.  Then the lift.
+__device__ __forceinline__ float most_of(const Unit &u) { return u.lift != 1.0f ? u.t * (8192.0f * 0x1p-100f) : u.t * 8192.0f; }
+__device__ __forceinline__ float limit_top(float top, const Unit &u) {
+    return top < INFINITY ? fminf(top, most_of(u)) * u.lift : top;  // infinity and NaN stay
+}
+__device__ __forceinline__ void limit8(uint64_t (&x)[4], const Unit &u) {
+    const float most = most_of(u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        x[j] = mul2(pack2(fminf(fmaxf(lo2(x[j]), -most), most), fminf(fmaxf(hi2(x[j]), -most), most)), pack2(u.lift, u.lift));
+}
 
 __device__ __forceinline__ Unit tensor_unit(const Quantize4Args &p, float *shared) {
     float m = 0.0f;
@@ -191,7 +207,8 @@ __device__ __forceinline__ Unit tensor_unit(const Quantize4Args &p, float *share
     }
     if (p.tensor_scale != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *p.tensor_scale = power_of_two(e);
     const int lift = e < -100 ? 100 : 0;
-    return Unit{power_of_two(e + lift), power_of_two(-e - lift), power_of_two(lift)};
+    const float t = power_of_two(e + lift);
+    return Unit{t, power_of_two(-e - lift), power_of_two(lift), lift ? -1.0f : t * 8192.0f};
 }
 
 // ---------------------------------------------------------------- one block
@@ -296,14 +313,16 @@ __device__ __forceinline__ void store_codes(uint8_t *to, uint32_t lo, uint32_t h
 template <bool WIDE, bool WHOLE>
 __device__ __forceinline__ void quantize_unit(const Quantize4Args &p, const Unit &u, uint64_t (&x)[2][4], int64_t row,
                                               int64_t unit, int64_t quads, bool here, bool words) {
-    if (!WIDE && u.lift != 1.0f) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[h][j] = mul2(x[h][j], pack2(u.lift, u.lift));
-    }
     float top = max_abs8(max_abs8(0.0f, x[0]), x[1]);
-    if constexpr (WIDE) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    if constexpr (WIDE) {
+        top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    } else {
+        if (!(top <= u.usual)) {
+            top = limit_top(top, u);
+            limit8(x[0], u);
+            limit8(x[1], u);
+        }
+    }
     const BlockScale b = block_scale<WIDE>(top, u);
     const uint32_t lo = codes8<WIDE>(x[0], b), hi = codes8<WIDE>(x[1], b);
     // one byte from each of four blocks, to the first of their lanes
@@ -332,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3)
     quantize4_rows_kernel(const Quantize4Args p, uint32_t units, uint32_t across, uint32_t chunks, int64_t quads, bool words) {
     pdl_wait();
     __shared__ float shared[kWarps];
-    const Unit u = WIDE ? Unit{1.0f, 1.0f, 1.0f} : tensor_unit(p, shared);
+    const Unit u = WIDE ? Unit{1.0f, 1.0f, 1.0f, INFINITY} : tensor_unit(p, shared);
     constexpr int kWords = static_cast<int>(sizeof(T) / 2);
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t w = blockIdx.x * kWarps + (threadIdx.x >> 5); w < chunks; w += gridDim.x * kWarps) {
@@ -379,7 +398,7 @@ __global__ void __launch_bounds__(kThreads) quantize4_any_kernel(const Quantize4
     pdl_wait();
     __shared__ float shared[kWarps];
     __shared__ float turned[kWarps][32 * 17];
-    const Unit u = WIDE ? Unit{1.0f, 1.0f, 1.0f} : tensor_unit(p, shared);
+    const Unit u = WIDE ? Unit{1.0f, 1.0f, 1.0f, INFINITY} : tensor_unit(p, shared);
     const int64_t padded = (p.rows + 127) / 128 * 128, per_row = cdiv_dev(units, 32), chunks = padded * per_row;
     const int lane = threadIdx.x & 31;
     float *mine = turned[threadIdx.x >> 5];
@@ -439,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, WIDE && sizeof(T) == 2 ? 2 : 4)
     __shared__ float shared[kWarps];
     extern __shared__ __align__(16) uint8_t tile_bytes[];
     Tile &tile = *reinterpret_cast<Tile *>(tile_bytes);
-    const Unit u = WIDE ? Unit{1.0f, 1.0f, 1.0f} : tensor_unit(p, shared);
+    const Unit u = WIDE ? Unit{1.0f, 1.0f, 1.0f, INFINITY} : tensor_unit(p, shared);
     const int64_t groups = (p.rows + 127) / 128 * (128 / Tile::kRows), total = groups * cdiv_dev(quads, 2);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // tile w from the end: its first row and column, and how many of each are inside
@@ -520,22 +539,27 @@ __global__ void __launch_bounds__(kThreads, WIDE && sizeof(T) == 2 ? 2 : 4)
 #pragma unroll
         for (int i = 0; i < Tile::kPer; ++i) {
             auto value = [&](int j) { return to_float(reinterpret_cast<const T *>(&word[j])[i]); };
+            uint64_t x[Tile::kSpan / 8][4];
             float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < Tile::kSpan; j += 2) top = max_abs(top, value(j), value(j + 1));
-            const BlockScale b = block_scale<WIDE>(WIDE ? top : top * u.lift, u);
+            for (int j = 0; j < Tile::kSpan; j += 8) {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) x[j / 8][h] = pack2(value(j + 2 * h), value(j + 2 * h + 1));
+                top = max_abs8(top, x[j / 8]);
+            }
+            if constexpr (!WIDE) {
+                if (!(top <= u.usual)) {
+                    top = limit_top(top, u);
+                    limit8(x[0], u);
+                    limit8(x[1], u);
+                }
+            }
+            const BlockScale b = block_scale<WIDE>(top, u);
             const int r = lane * Tile::kPer + i;
             tile.scales[r * 8 + warp] = static_cast<uint8_t>(b.byte);
 #pragma unroll
-            for (int j = 0; j < Tile::kSpan; j += 8) {
-                uint64_t x[4];
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    x[h] = pack2(value(j + 2 * h), value(j + 2 * h + 1));
-                    if (!WIDE && u.lift != 1.0f) x[h] = mul2(x[h], pack2(u.lift, u.lift));
-                }
-                *reinterpret_cast<uint32_t *>(tile.codes + r * Tile::kCodePitch + (warp * Tile::kSpan + j) / 2) = codes8<WIDE>(x, b);
-            }
+            for (int j = 0; j < Tile::kSpan; j += 8)
+                *reinterpret_cast<uint32_t *>(tile.codes + r * Tile::kCodePitch + (warp * Tile::kSpan + j) / 2) = codes8<WIDE>(x[j / 8], b);
         }
         __syncthreads();
         constexpr int kPieces = Tile::kCols / 32;  // 16 bytes of codes each

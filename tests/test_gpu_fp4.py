@@ -519,3 +519,30 @@ def test_maximum_beside_infinities(layout, src):
     x[::7, ::5] = float("inf")
     x[last] = 1000.0
     assert st.quantize_fp4(x).tensor_scale.item() == 0.5
+
+
+@pytest.mark.parametrize("src", SRC, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout", ["whole rows", "rows", "columns", "columns off", "strided"])
+@pytest.mark.parametrize("amax", [0.0, 1e-38, 1e-30, 1e-20, 1.0, 8.0])
+def test_quantize_far_above_the_maximum(amax, layout, src):
+    """Elements however far above a known maximum saturate with their sign; those beside them are as they are without."""
+    most = torch.finfo(src).max
+    x = torch.randn(40, 96 if layout == "whole rows" else 91, generator=gen(11)) * max(amax, 2.0 ** -126)
+    for i, v in enumerate([4.0, -4.0, 1e9, -1e9, most, -most, 2.0 ** 28, -3.0 * 2.0 ** 60]):
+        x[i, 3 * i], x[i, 40], x[8 + i, 50] = v, -v, v
+    x[20, :16], x[21, 16:32] = most, -most
+    x[22, 5], x[22, 6] = float("inf"), most
+    x[23, 33], x[23, 34] = float("nan"), -most
+    x = x.clamp(-most, most).where(torch.isfinite(x), x).to(src)
+    turned = x.t().contiguous()
+    off = torch.zeros(turned.shape[0], 41, dtype=src)
+    off[:, 1:] = turned
+    wide = torch.zeros(40, 2 * x.shape[1], dtype=src)
+    wide[:, ::2] = x
+    where = {"whole rows": lambda: x.to(DEV), "rows": lambda: x.to(DEV), "columns": lambda: turned.to(DEV).t(),
+             "columns off": lambda: off.to(DEV)[:, 1:].t(), "strided": lambda: wide.to(DEV)[:, ::2]}[layout]()
+    got = check_quantize(x, E4, amax=torch.tensor(amax).item(), where=where)
+    back = st.dequantize_fp4(got.codes, got.scale, got.tensor_scale, cols=x.shape[1], out_dtype=torch.float32).cpu()
+    fine = torch.isfinite(x.float())
+    assert torch.isfinite(back[fine.view(40, -1).all(1)]).all()
+    assert (back[20, :16] > 0).all() and (back[21, 16:32] < 0).all()
