@@ -288,11 +288,13 @@ __device__ __forceinline__ float max_abs8(float m, const uint64_t (&x)[4]) {
     return m;
 }
 
-// Where the scale of block b (of `quads` groups of four a row) of a row lies:
-// below 2^32, as a tensor that fits the GPU has fewer blocks.
-__device__ __forceinline__ uint32_t scale_at(int64_t row, int64_t b, int64_t quads) {
+// Where the scale of block b (of `quads` groups of four a row) of a row lies.
+// A row's blocks are padded to four and the rows to 128, so that one row of
+// 2^29 elements has 2^32 bytes of scales: only the count of 512 bytes, of
+// which no GPU has 2^32, and the place inside of them are 32 bits.
+__device__ __forceinline__ int64_t scale_at(int64_t row, int64_t b, int64_t quads) {
     const uint32_t r = static_cast<uint32_t>(row), k = static_cast<uint32_t>(b);
-    return ((r >> 7) * static_cast<uint32_t>(quads) + (k >> 2)) * 512u + (r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (k & 3u);
+    return static_cast<int64_t>((r >> 7) * static_cast<uint32_t>(quads) + (k >> 2)) * 512 + ((r & 31u) * 16u + ((r >> 5) & 3u) * 4u + (k & 3u));
 }
 
 // The 8 bytes of 16 codes, or those of the first n elements.

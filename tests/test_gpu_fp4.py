@@ -546,3 +546,31 @@ def test_quantize_far_above_the_maximum(amax, layout, src):
     fine = torch.isfinite(x.float())
     assert torch.isfinite(back[fine.view(40, -1).all(1)]).all()
     assert (back[20, :16] > 0).all() and (back[21, 16:32] < 0).all()
+
+
+@pytest.mark.parametrize("layout", ["rows", "columns", "strided"])
+def test_scales_beyond_32_bits(layout):
+    """A row of 2^29 elements, padded to 128, has 2^32 bytes of scales: both ends of longer ones against the same columns alone."""
+    rows, cols, cut = 2, 2 ** 29 + 4096, 4096
+    shape = {"rows": (rows, cols), "columns": (cols, rows), "strided": (rows, 2 * cols)}[layout]
+    x = torch.empty(shape, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(1))
+    x = {"rows": x, "columns": x.t(), "strided": x[:, ::2]}[layout]
+    amax = torch.tensor(8.0, device=DEV)
+    got = st.quantize_fp4(x, amax=amax)
+    assert got.scale.numel() > 2 ** 32
+    back = st.dequantize_fp4(*got)
+    quads, half = cut // 64, cut // 2  # groups of four scales, bytes of codes
+    for first, quad in [(0, 0), (cols - cut, got.scale.shape[1] - quads)]:
+        alone = st.quantize_fp4(x[:, first : first + cut], amax=amax)
+        assert torch.equal(got.scale[:, quad : quad + quads].view(torch.uint8), alone.scale.view(torch.uint8))
+        assert torch.equal(got.codes[:, first // 2 : first // 2 + half].view(torch.uint8), alone.codes.view(torch.uint8))
+        assert torch.equal(back[:, first : first + cut], st.dequantize_fp4(*alone))
+    del back
+    # ones at both ends and zeros between them, the last columns' scales 2: the product is exact
+    codes, scale = got.codes.view(torch.uint8), got.scale.view(torch.uint8)
+    codes.zero_()
+    codes[:, :half], codes[:, -half:] = 0x22, 0x22
+    scale.fill_(0x38)
+    scale[:, -quads:] = 0x40
+    c = st.matmul_fp4(codes, codes.t(), got.scale, got.scale, out_dtype=torch.float32)
+    assert torch.equal(c, torch.full((rows, rows), cut * 1.0 + cut * 4.0, device=DEV))
