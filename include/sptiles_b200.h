@@ -319,7 +319,9 @@ int st_dequantize_fp4(st_ctx *ctx, const st_tensor *q, const st_tensor *scale, c
  * ST_E2M1X2, scales of M and N rows and of one type; tensor scales one f32 or
  * NULL (1; NULL with ST_E8M0).  C f32, f16 or bf16 [M, N] with unit column
  * stride; bias f32 or C's dtype.  Sums are fp32; the tensor scales' product
- * and the bias are applied in fp32.  The same inputs give the same bits.  An
+ * (where it leaves fp32's normal range one scale after the other, so that a
+ * result within that range is right) and the bias are applied in fp32.  The
+ * same inputs give the same bits.  An
  * operand is read in place if its rows (B: columns) are contiguous along K, on
  * 16-byte boundaries, and do not overlap; any other is copied first, into
  * `workspace` (16-byte aligned, st_matmul_fp4_workspace bytes). */

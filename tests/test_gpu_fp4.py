@@ -574,3 +574,28 @@ def test_scales_beyond_32_bits(layout):
     scale[:, -quads:] = 0x40
     c = st.matmul_fp4(codes, codes.t(), got.scale, got.scale, out_dtype=torch.float32)
     assert torch.equal(c, torch.full((rows, rows), cut * 1.0 + cut * 4.0, device=DEV))
+
+
+@pytest.mark.parametrize("m,n", [(1, 300), (40, 300), (200, 130), (2048, 2560)])
+@pytest.mark.parametrize("ta,tb", [(-70, -70), (-80, -76), (-126, -30), (-30, -126), (65, 65), (117, 15), (15, 117), (117, 20), (20, 117),
+                                   (-126, 117)])
+def test_product_of_far_tensor_scales(ta, tb, m, n):
+    """Tensor scales whose product leaves fp32's range, where the result does not; a sum of nothing stays 0.
+
+    Sums and scales are powers of two, or those times 49, so a result is exact, or, of 117 and 20, 2^-7 2^137: infinite in fp32."""
+    k, up = 2048, ta + tb < 0
+    qa, qb = torch.zeros(m, k, dtype=torch.uint8), torch.zeros(n, k, dtype=torch.uint8)
+    qa[::2], qb[::3] = 2, 2  # rows of ones and of zeros
+    byte = 0x7e if up else 1  # 448 and 2^-9: sums of 2048 * 448^2, about 2^28.6, or of 2^11 * 2^-18
+    sa, sb = (tiled(torch.full((r, k // 16), byte)).view(E4).to(DEV) for r in (m, n))
+    scale = [torch.tensor(2.0 ** e, device=DEV) for e in (ta, tb)]
+    a, b = ((q[:, 0::2] | q[:, 1::2] << 4).to(DEV) for q in (qa, qb))
+    one = k * (448.0 ** 2 if up else 2.0 ** -18)
+    want = torch.outer((qa[:, 0] == 2).double(), (qb[:, 0] == 2).double()) * one * 2.0 ** ta * 2.0 ** tb
+    step = 2.0 ** -149 if 0 < abs(one * 2.0 ** ta * 2.0 ** tb) < 2.0 ** -126 else 0.0  # below that fp32 is a grid of its own
+    got = st.matmul_fp4(a, b.t(), sa, sb, a_tensor_scale=scale[0], b_tensor_scale=scale[1], out_dtype=torch.float32).cpu().double()
+    want = want.float().double()
+    assert ((got == want) | ((got - want).abs() <= step)).all()
+    bias = torch.full((n,), 0.0, device=DEV)
+    assert torch.equal(st.matmul_fp4(a, b.t(), sa, sb, bias, a_tensor_scale=scale[0], b_tensor_scale=scale[1],
+                                     out_dtype=torch.float32).cpu().double(), got)
