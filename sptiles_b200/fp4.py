@@ -30,19 +30,23 @@ from .api import _CODES, _exec_desc
 from .fp8 import _cp, _desc, _device_of, _fn, _fns, _new, _pack, _u64, _vp
 from .runtime import context
 
-_BLOCK = {torch.float8_e4m3fn: 16, torch.float8_e8m0fnu: 32}
-_SCALE_CODES = {torch.float8_e4m3fn: N.ST_E4M3, torch.float8_e8m0fnu: N.ST_E8M0}
-_CODE_TYPES = (torch.float4_e2m1fn_x2, torch.uint8)
+_BLOCK = {torch.float8_e4m3fn: 16}
+_SCALE_CODES = {torch.float8_e4m3fn: N.ST_E4M3}
+# An older torch lacks the two types: codes are uint8 there, and blocks of 32 are not to be had.
+if hasattr(torch, "float8_e8m0fnu"):
+    _BLOCK[torch.float8_e8m0fnu] = 32
+    _SCALE_CODES[torch.float8_e8m0fnu] = N.ST_E8M0
+_CODES_TYPE = getattr(torch, "float4_e2m1fn_x2", torch.uint8)
 
 
 class Quantized4(NamedTuple):
-    codes: torch.Tensor                # float4_e2m1fn_x2 [rows, ceil(cols / 2)]
+    codes: torch.Tensor                # float4_e2m1fn_x2 [rows, ceil(cols / 2)] (uint8 with a torch that lacks the type)
     scale: torch.Tensor                # [ceil(rows / 128), ceil(blocks / 4), 32, 4, 4], see quantize_fp4
     tensor_scale: torch.Tensor | None  # float32, one element (None for blocks of 32)
 
 
 def _codes_desc(t: torch.Tensor, name: str) -> bytes:
-    if t.dtype not in _CODE_TYPES:
+    if t.dtype != _CODES_TYPE and t.dtype != torch.uint8:
         raise ValueError(f"{name} must have dtype torch.float4_e2m1fn_x2 (or torch.uint8), got {t.dtype}")
     if t.dim() != 2:
         raise ValueError(f"{name} must be a 2D tensor.")
@@ -115,7 +119,7 @@ def quantize_fp4(A: torch.Tensor, *, scale_dtype: torch.dtype = torch.float8_e4m
     rows, cols = A.shape
     width = (cols + 1) // 2
     pitch = (width + 15) // 16 * 16
-    codes = A.new_empty_strided((rows, width), (pitch, 1), dtype=torch.float4_e2m1fn_x2)
+    codes = A.new_empty_strided((rows, width), (pitch, 1), dtype=_CODES_TYPE)
     scale = A.new_empty(_scale_shape(rows, width, block), dtype=scale_dtype)
     n = scale.numel()
     t = workspace = None

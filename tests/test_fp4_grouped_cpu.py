@@ -1,6 +1,9 @@
 """Refusals of the 4-bit and grouped calls, without a GPU: every argument is
 checked before the context and the device are looked at."""
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -240,3 +243,29 @@ def test_extents_near_int32(extent):
     refused(grouped(a=t2(extent, 64, F16), c=t2(extent, 32)), NOT, "extents of at most")
     refused(grouped(b=t2(64, extent, F16), c=t2(16, extent)), NOT, "extents of at most")
     refused(weights(a=t2(extent, 64, F16), c=t2(extent, 32, F16)), NOT, "extents of at most")
+
+
+def test_a_torch_without_the_small_types():
+    """The package imports and keeps its other calls; 4-bit codes are uint8 and blocks of 32 are refused."""
+    code = """
+import torch
+for name in ("float4_e2m1fn_x2", "float8_e8m0fnu"):
+    delattr(torch, name)
+import sptiles_b200 as st
+x = torch.zeros(2, 32)
+for call, word in [(lambda: st.matmul(x, x), "K"), (lambda: st.quantize_fp4(x, scale_dtype=torch.uint8), "scale_dtype"),
+                   (lambda: st.quantize_fp4(x), "CUDA"),
+                   (lambda: st.dequantize_fp4(x.to(torch.uint8), torch.zeros(1, 1, 32, 4, 4, dtype=torch.uint8)), "scale must have"),
+                   (lambda: st.dequantize_fp4(x.to(torch.uint8), torch.zeros(1, 1, 32, 4, 4).to(torch.float8_e4m3fn)), "CUDA"),
+                   (lambda: st.dequantize_fp4(x, x), "codes must have")]:
+    try:
+        call()
+    except (ValueError, RuntimeError) as e:
+        assert word.lower() in str(e).lower(), (word, e)
+    else:
+        raise SystemExit("not refused: " + word)
+print("kept")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          cwd=str(Path(__file__).resolve().parents[1]))
+    assert done.returncode == 0 and "kept" in done.stdout, done.stdout + done.stderr
