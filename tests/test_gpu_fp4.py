@@ -599,3 +599,16 @@ def test_product_of_far_tensor_scales(ta, tb, m, n):
     bias = torch.full((n,), 0.0, device=DEV)
     assert torch.equal(st.matmul_fp4(a, b.t(), sa, sb, bias, a_tensor_scale=scale[0], b_tensor_scale=scale[1],
                                      out_dtype=torch.float32).cpu().double(), got)
+
+
+@pytest.mark.parametrize("m,n", [(128, 40), (1280, 1536)])
+@pytest.mark.parametrize("high", [False, True], ids=["low", "high"])
+def test_product_every_e8m0_scale(high, m, n):
+    """All 255 powers of two, 2^-127 (a subnormal of fp32) and 2^127 among them, against 2^64 or 2^-64 in the other operand."""
+    byte = torch.arange(m) % 128 + (127 if high else 0)
+    other = 127 - 64 if high else 127 + 64
+    ones = torch.full((max(m, n), 16), 0x22, dtype=torch.uint8, device=DEV)
+    sa, sb = tiled(byte[:, None]).view(E8).to(DEV), tiled(torch.full((n, 1), other)).view(E8).to(DEV)
+    want = (32 * torch.pow(torch.tensor(2.0, dtype=torch.float64), byte - 127.0 + other - 127.0)).float()[:, None].expand(m, n)
+    assert torch.equal(st.matmul_fp4(ones[:m], ones[:n].t(), sa, sb, out_dtype=torch.float32).cpu(), want)
+    assert torch.equal(st.matmul_fp4(ones[:n], ones[:m].t(), sb, sa, out_dtype=torch.float32).cpu(), want.t())
