@@ -344,7 +344,8 @@ int st_matmul_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
  * the last group are left as they are, or set to 0 with zero_rest.
  * st_matmul_grouped_weights: D[g, k, n] = sum over g's rows of A[r, k] C[r, n],
  * 0 for an empty group: the gradient of B where C is the gradient of the
- * product.  `d` is the first group's [K, N], unit column stride; groups do not
+ * product.  `d` is the first group's [K, N], unit column stride; the groups lie
+ * one behind the other, or their rows in turn ([K, groups, N]), and do not
  * overlap.  (The gradient of A is st_matmul_grouped with B's transposed view.)
  * Sums are fp32.  The same inputs give the same bits, whatever the other
  * groups' rows hold.  An operand is read in place if it is contiguous along a

@@ -1943,7 +1943,9 @@ int st_matmul_grouped_weights(st_ctx *ctx, const st_tensor *a, const st_tensor *
     }
     ST_TRY(check_grouped_output(d, "D", g.k, g.n));
     const int64_t span = g.k > 0 && g.n > 0 ? (g.k - 1) * d->strides[0] + g.n : 0;
-    if (g.groups > 1 && d_group_stride < span)
+    // one group behind the other, or the groups' rows in turn ([K, G, N])
+    const bool in_turn = g.groups > 1 && d_group_stride >= g.n && (d->strides[0] - g.n) / (g.groups - 1) >= d_group_stride;
+    if (g.groups > 1 && d_group_stride < span && !in_turn)
         return fail(ST_ERR_INVALID_ARGUMENT, "D has overlapping groups: their stride is " + std::to_string(d_group_stride) +
                                                  ", one spans " + std::to_string(span) + " elements");
     ST_TRY(check_workspace("matmul_grouped_weights", gemm_grouped_workspace_bytes(g), workspace, workspace_bytes, 16));

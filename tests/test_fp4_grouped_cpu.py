@@ -269,3 +269,10 @@ print("kept")
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
                           cwd=str(Path(__file__).resolve().parents[1]))
     assert done.returncode == 0 and "kept" in done.stdout, done.stdout + done.stderr
+
+
+def test_weights_of_groups_in_turn():
+    """Results [K, groups, N] do not overlap and get past that check, to the workspace's; a row too short for all groups does."""
+    for stride, row, word in [(32, 128, "workspace"), (40, 152, "workspace"), (32, 127, "overlapping groups"), (31, 128, "overlapping groups"),
+                              (40, 151, "overlapping groups")]:
+        refused(weights(a=t2(16, 64, F16, strides=(1, 16)), d=t2(64, 32, strides=(row, 1)), stride=stride), BAD, word)

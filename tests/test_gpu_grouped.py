@@ -399,3 +399,15 @@ def test_experts_layer_forward_and_backward():
         moved.append((plain(v.cpu(), w.transpose(1, 2), ends_host) * dy.cpu().double()).sum())
     slope, size = (moved[0] - moved[1]) / (2 * step), plain_weights(dy.cpu().abs(), v.cpu().abs(), ends_host)[at]
     assert abs(slope - dw2[at].item()) <= (tokens + 4) * 2.0 ** -23 * size + 2.0 ** -24 * abs(slope) + 1e-9 * abs(moved[0])
+
+
+@pytest.mark.parametrize("rows,k,n,ends", [(130, 72, 136, [1, 1, 129, 130]), (1300, 320, 1032, [700, 700, 1299])])
+@pytest.mark.parametrize("pad", [0, 5])
+def test_weights_of_groups_in_turn(pad, rows, k, n, ends):
+    """Results laid out [K, groups, N]: each where it belongs, what lies between them as it was."""
+    a, c = ints(1, rows, k), ints(2, rows, n)
+    room = torch.full((k, len(ends), n + pad), 7.0, device=DEV)
+    out = room[:, :, :n].transpose(0, 1)
+    st.matmul_grouped_weights(a.to(BF16).to(DEV), c.to(BF16).to(DEV), device_ends(ends), out=out)
+    assert torch.equal(out.cpu(), plain_weights(a, c, ends).float())
+    assert (room[:, :, n:] == 7).all()
