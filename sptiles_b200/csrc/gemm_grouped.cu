@@ -1026,9 +1026,12 @@ int launch_pair_instance(const CUtensorMap &mr, const ColumnMaps &mc, const Grou
     return checked("gemm_grouped_pair_kernel");
 }
 
-// Most tiles that there can be, however the ends divide the rows.
+// Most tiles that there can be, however the ends divide the rows: m groups of a
+// row each, and a tile more for each `cols` of the other rows.
 int64_t most_tiles(const GroupedArgs &g, int64_t tiles_r, int cols) {
-    return tiles_r * (g.weights ? g.groups * cdiv(g.k, cols) : cdiv(g.rows, cols) + (g.groups < g.rows ? g.groups : g.rows));
+    if (g.weights) return tiles_r * g.groups * cdiv(g.k, cols);
+    const int64_t m = g.groups < g.rows ? g.groups : g.rows;
+    return tiles_r * ((g.rows - m) / cols + m);
 }
 
 // Tile shape and split: the least estimated time for groups of equal size (what
