@@ -765,15 +765,7 @@ template <typename T, bool WIDE>
 int launch_columns(const Quantize4Args &p, int64_t quads, int sm_count, cudaStream_t stream) {
     using Tile = ColumnTile<T, WIDE>;
     auto kern = quantize4_columns_kernel<T, WIDE>;
-    if constexpr (sizeof(Tile) > 48 * 1024) {
-        static uint64_t attr_set = 0;  // one bit per device ordinal
-        int dev = 0;
-        ST_CUDA_TRY(cudaGetDevice(&dev));
-        if (dev < 0 || dev >= 64 || !(attr_set & (1ull << dev))) {
-            ST_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Tile)));
-            if (dev >= 0 && dev < 64) attr_set |= 1ull << dev;
-        }
-    }
+    static_assert(sizeof(Tile) <= 48 * 1024, "shared memory that a kernel has without asking");
     const bool in_words = reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && (p.cols == 1 || p.sa1 * static_cast<int64_t>(sizeof(T)) % 16 == 0);
     const bool words = on16(p.q, p.sq0, p.rows, 1);
     const int64_t work = cdiv(p.rows, 128) * (128 / Tile::kRows) * cdiv(quads, 2);
