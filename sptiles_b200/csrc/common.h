@@ -282,6 +282,9 @@ int launch_quantize_fp8(const QuantizeArgs &args, cudaStream_t stream);
 // multiple of 16; the padding gets bytes of no meaning).
 int launch_repack_8(const void *src, int64_t s0, int64_t s1, int64_t rows, int64_t cols, void *dst, int64_t ld,
                     int sm_count, cudaStream_t stream);
+// C = bias (or 0) in every row: a product over nothing.
+int launch_fill_bias(void *c, int64_t ldc, int c_dtype, const void *bias, int bias_dtype, int64_t m, int64_t n, int sm_count,
+                     cudaStream_t stream);
 
 // ---- 4-bit operands with a scale per block of 16 or 32 along K (quantize_fp4.cu, gemm_fp4.cu)
 // Scales lie as [row / 128][block / 4][row % 32][row / 32 % 4][block % 4].

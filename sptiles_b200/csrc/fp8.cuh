@@ -1,5 +1,5 @@
 // fp8.cuh -- element conversions and packed fp32 arithmetic shared by the
-// 8-bit quantiser, the 8-bit matmul and the norms.
+// quantisers, the 8- and 4-bit matmuls, the products by groups and the norms.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -7,6 +7,8 @@
 #include <cuda_fp8.h>
 
 #include <cstdint>
+
+#include "common.h"
 
 namespace st {
 
@@ -17,6 +19,19 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162f
 __device__ __forceinline__ void from_float(float v, float &out) { out = v; }
 __device__ __forceinline__ void from_float(float v, __half &out) { out = __float2half_rn(v); }
 __device__ __forceinline__ void from_float(float v, __nv_bfloat16 &out) { out = __float2bfloat16_rn(v); }
+
+// Element i of a tensor of type `dtype` (ST_F32, ST_F16 or ST_BF16).
+__device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
+    if (dtype == ST_F32) return static_cast<const float *>(p)[i];
+    if (dtype == ST_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+
+__device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v) {
+    if (dtype == ST_F32) static_cast<float *>(p)[i] = v;
+    else if (dtype == ST_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+}
 
 // ---- pairs of fp32 in one register pair: the packed instructions halve the
 // issue slots of the row kernels, which were bound by them

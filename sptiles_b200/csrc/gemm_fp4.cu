@@ -60,18 +60,6 @@ struct Fp4Params {
     unsigned long long timeout_ns;
 };
 
-__device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
-    if (dtype == ST_F32) return static_cast<const float *>(p)[i];
-    if (dtype == ST_F16) return __half2float(static_cast<const __half *>(p)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
-
-__device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v) {
-    if (dtype == ST_F32) static_cast<float *>(p)[i] = v;
-    else if (dtype == ST_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
-}
-
 // The tensor scales' product, by which sums are multiplied.  Where it leaves
 // fp32's normal range, a result need not: then one scale after the other,
 // first the one that leads away from that end of the range.
@@ -641,17 +629,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp4PairCfg::kThreads
     }
 }
 
-__global__ void __launch_bounds__(256) fill_bias_kernel(void *c, int64_t ldc, int c_dtype, const void *bias, int bias_dtype,
-                                                        int64_t m, int64_t n) {
-    pdl_wait();
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < m * n;
-         i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / n, q = i - r * n;
-        store_any(c, c_dtype, r * ldc + q, bias ? load_any(bias, bias_dtype, q) : 0.0f);
-    }
-    pdl_trigger();
-}
-
 // ---------------------------------------------------------------- host side
 int make_map_4(CUtensorMap *map, const char *what, const void *base, int64_t k_bytes, int64_t rows, int64_t ld, int box_rows) {
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k_bytes), static_cast<cuuint64_t>(rows)};
@@ -798,13 +775,7 @@ int launch_gemm_fp4(const GemmFp4Args &g, void *workspace, int sm_count, int *de
                     cudaStream_t stream) {
     const int64_t m = g.a.rows, n = g.b.rows, k = g.a.k;
     if (m == 0 || n == 0) return ST_OK;
-    if (k == 0) {
-        ST_CUDA_TRY(launch_kernel(fill_bias_kernel, static_cast<unsigned>(sm_count), 256, 0, stream, g.c, g.ldc,
-                                  g.c_dtype, g.bias, g.bias_dtype, m, n));
-        note_launch();
-        const cudaError_t e = cudaPeekAtLastError();
-        return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "fill_bias_kernel");
-    }
+    if (k == 0) return launch_fill_bias(g.c, g.ldc, g.c_dtype, g.bias, g.bias_dtype, m, n, sm_count, stream);
     Fp4Operand op[2] = {g.a, g.b};
     Access acc[2] = {access_of(g.a), access_of(g.b)};
     uint8_t *ws = static_cast<uint8_t *>(workspace);

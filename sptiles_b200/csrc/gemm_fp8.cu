@@ -30,17 +30,16 @@
 // the size), 57 x 4109 x 4001 in 14.1, 1024^3 in 10.8 a call and 7.2 in a
 // replayed graph.
 #include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
-#include <mutex>
 
 #include "common.h"
 #include "fp8.cuh"
 #include "sm100.cuh"
+#include "tensor_map.h"
 
 namespace st {
 namespace {
@@ -67,18 +66,6 @@ struct Fp8Params {
     int *err;
     unsigned long long timeout_ns;
 };
-
-__device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
-    if (dtype == ST_F32) return static_cast<const float *>(p)[i];
-    if (dtype == ST_F16) return __half2float(static_cast<const __half *>(p)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
-
-__device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v) {
-    if (dtype == ST_F32) static_cast<float *>(p)[i] = v;
-    else if (dtype == ST_F16) static_cast<__half *>(p)[i] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
-}
 
 __device__ __forceinline__ uint32_t pack_16(float a, float b, int dtype) {
     if (dtype == ST_F16) {
@@ -1150,34 +1137,12 @@ __global__ void __launch_bounds__(256) fill_bias_kernel(void *c, int64_t ldc, in
 }
 
 // ---------------------------------------------------------------- host side
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-    });
-    return fn;
-}
-
 // 128-byte-swizzled box of 128 bytes x `box_rows` of a byte matrix whose rows are `ld` bytes apart
 int make_map_8(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld, int box_rows) {
-    auto fn = encode_fn();
-    if (!fn) return fail(ST_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
-    cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
-    cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
-    cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-        return fail(ST_ERR_INVALID_ARGUMENT, "cuTensorMapEncodeTiled rejected an 8-bit operand (error " +
-                                                 std::to_string(static_cast<int>(r)) + ")");
-    return ST_OK;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+    const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+    return make_tensor_map(map, "an 8-bit operand", CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box);
 }
 
 template <int BN, bool R_MN, bool C_MN, bool CVEC>
@@ -1263,7 +1228,7 @@ int launch_pair(const CUtensorMap &mr, const CUtensorMap &mc, const CUtensorMap 
 
 // 32-row box of 128 bytes of C
 int make_map_out(CUtensorMap *map, const GemmFp8Args &g) {
-    auto fn = encode_fn();
+    auto fn = tensor_map_encoder();
     if (!fn) return fail(ST_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
     const int es = static_cast<int>(dtype_size(g.c_dtype));
     const CUtensorMapDataType dt = g.c_dtype == ST_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
@@ -1366,6 +1331,14 @@ int launch_repack_8(const void *src, int64_t s0, int64_t s1, int64_t rows, int64
     return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "repack_8_kernel");
 }
 
+int launch_fill_bias(void *c, int64_t ldc, int c_dtype, const void *bias, int bias_dtype, int64_t m, int64_t n, int sm_count,
+                     cudaStream_t stream) {
+    ST_CUDA_TRY(launch_kernel(fill_bias_kernel, static_cast<unsigned>(sm_count), 256, 0, stream, c, ldc, c_dtype, bias, bias_dtype, m, n));
+    note_launch();
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "fill_bias_kernel");
+}
+
 int launch_fp8_wait_check(bool by_column, uint64_t limit_ns, int *dev_err, cudaStream_t stream) {
     if (by_column) fp8_wait_check_kernel<true><<<1, 32, 0, stream>>>(limit_ns, dev_err);
     else fp8_wait_check_kernel<false><<<1, 32, 0, stream>>>(limit_ns, dev_err);
@@ -1384,11 +1357,7 @@ int launch_gemm_fp8(const GemmFp8Args &g, void *workspace, int sm_count, int *de
     const int64_t m = g.a.rows, n = g.b.rows, k = g.a.k;
     if (m == 0 || n == 0) return ST_OK;
     if (k == 0) {
-        ST_CUDA_TRY(launch_kernel(fill_bias_kernel, static_cast<unsigned>(sm_count), 256, 0, stream, g.c, g.ldc,
-                                  g.c_dtype, g.bias, g.bias_dtype, m, n));
-        note_launch();
-        const cudaError_t e = cudaPeekAtLastError();
-        return e == cudaSuccess ? ST_OK : cuda_fail(cudaGetLastError(), "fill_bias_kernel");
+        return launch_fill_bias(g.c, g.ldc, g.c_dtype, g.bias, g.bias_dtype, m, n, sm_count, stream);
     }
     Fp8Operand op[2] = {g.a, g.b};
     Access acc[2] = {access_of(g.a), access_of(g.b)};
