@@ -308,8 +308,9 @@ int st_matmul_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
  * finite elements, in a first pass.  A block with a NaN or an infinity gets
  * the scale NaN.  Q has unit column stride.  workspace: st_quantize_fp4_workspace
  * bytes, 4-byte aligned, where amax is to be taken.
- * st_dequantize_fp4: the values back, as f32, f16 or bf16, out [rows, cols]
- * with cols 2 * Q's columns, or one less. */
+ * st_dequantize_fp4: the values back, the product of code, scale and tensor
+ * scale rounded to fp32 and that to out's type, f32, f16 or bf16; out [rows,
+ * cols] with cols 2 * Q's columns, or one less. */
 int st_quantize_fp4_workspace(uint64_t *bytes);
 int st_quantize_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *q, const st_tensor *scale, const st_tensor *amax,
                     const st_tensor *tensor_scale, void *workspace, uint64_t workspace_bytes, const st_exec *exec);

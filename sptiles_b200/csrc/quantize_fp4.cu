@@ -591,23 +591,29 @@ __global__ void __launch_bounds__(kThreads, WIDE && sizeof(T) == 2 ? 2 : 4)
 }
 
 // ---------------------------------------------------------------- back to values
-__device__ __forceinline__ float scale_value(uint32_t byte, bool wide) {
-    if (wide) return byte == 255u ? NAN : power_of_two(static_cast<int>(byte) - 127);
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+// What a block's codes are multiplied by: an e4m3 scale in f16, where its
+// product with a code is exact (6 bits, 2^-10 to 2688), then the tensor's scale
+// in fp32, the one rounding; an e8m0 scale in fp32.
+struct Back {
+    __half2 scale;
+    float factor;
+};
+__device__ __forceinline__ Back back_of(uint32_t byte, bool wide, float t) {
+    if (wide) return Back{__float2half2_rn(1.0f), byte == 255u ? NAN : power_of_two(static_cast<int>(byte) - 127)};
+    return Back{__half2half2(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3))), t};
 }
-__device__ __forceinline__ float2 two_codes(uint32_t byte) {
-    return __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1)));
+__device__ __forceinline__ uint64_t two_values(uint32_t byte, const Back &b) {
+    const __half2 code = __half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1));
+    const float2 v = __half22float2(__hmul2(code, b.scale));
+    return mul2(pack2(v.x, v.y), pack2(b.factor, b.factor));
 }
 
 // The values of 16 codes.
-__device__ __forceinline__ void values16(uint64_t (&f)[2][4], uint2 code, float unit) {
+__device__ __forceinline__ void values16(uint64_t (&f)[2][4], uint2 code, const Back &b) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 v = two_codes((h ? code.y : code.x) >> (8 * j) & 0xffu);
-            f[h][j] = mul2(pack2(v.x, v.y), pack2(unit, unit));
-        }
+        for (int j = 0; j < 4; ++j) f[h][j] = two_values((h ? code.y : code.x) >> (8 * j) & 0xffu, b);
 }
 
 // A lane takes 8 columns of eight rows, whose reads are under way together; its
@@ -645,13 +651,10 @@ __global__ void __launch_bounds__(kThreads, 4) dequantize4_words_kernel(const De
 #pragma unroll
         for (int i = 0; i < kRows; ++i, out += p.so0) {
             if (row0 + i >= p.rows) break;
-            const float unit = scale_value(byte[i], p.wide) * t;
+            const Back b = back_of(byte[i], p.wide, t);
             uint64_t f[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 v = two_codes(code[i] >> (8 * j) & 0xffu);
-                f[j] = mul2(pack2(v.x, v.y), pack2(unit, unit));
-            }
+            for (int j = 0; j < 4; ++j) f[j] = two_values(code[i] >> (8 * j) & 0xffu, b);
             if (left >= 8) {
                 constexpr int kWords = static_cast<int>(sizeof(T) / 2);
                 uint4 o[kWords];
@@ -697,7 +700,7 @@ __global__ void __launch_bounds__(kThreads) dequantize4_any_kernel(const Dequant
             byte = p.scale[scale_at(row, p.wide ? unit >> 1 : unit, quads)];
         }
         uint64_t f[2][4];
-        values16(f, code, scale_value(byte, p.wide) * t);
+        values16(f, code, back_of(byte, p.wide, t));
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < 16; ++j) mine[17 * lane + j] = j & 1 ? hi2(f[j / 8][j % 8 / 2]) : lo2(f[j / 8][j % 8 / 2]);

@@ -140,9 +140,10 @@ def quantize_fp4(A: torch.Tensor, *, scale_dtype: torch.dtype = torch.float8_e4m
 
 def dequantize_fp4(codes: torch.Tensor, scale: torch.Tensor, tensor_scale: torch.Tensor | None = None, *,
                    cols: int | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values of 4-bit blocks, code * scale * tensor_scale, rounded once to out_dtype.
+    """The values of 4-bit blocks: code * scale * tensor_scale, rounded to fp32 and that to out_dtype.
 
-    codes, scale and tensor_scale as quantize_fp4 makes them (codes of any
+    (In fp32 it is exact where tensor_scale is a power of two, as quantize_fp4
+    makes it, and the result within fp32's normal range.)  codes, scale and tensor_scale as quantize_fp4 makes them (codes of any
     strides; uint8 is taken as well); ``cols`` where the last byte of a row
     holds one element only.
     """

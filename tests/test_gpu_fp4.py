@@ -612,3 +612,18 @@ def test_product_every_e8m0_scale(high, m, n):
     want = (32 * torch.pow(torch.tensor(2.0, dtype=torch.float64), byte - 127.0 + other - 127.0)).float()[:, None].expand(m, n)
     assert torch.equal(st.matmul_fp4(ones[:m], ones[:n].t(), sa, sb, out_dtype=torch.float32).cpu(), want)
     assert torch.equal(st.matmul_fp4(ones[:n], ones[:m].t(), sb, sa, out_dtype=torch.float32).cpu(), want.t())
+
+
+@pytest.mark.parametrize("layout", ["words", "columns"])
+@pytest.mark.parametrize("t", [0.3, 1 / 3, 3e-42, 2.0 ** 120, 2.0 ** 122])
+def test_dequantize_rounds_once(t, layout):
+    """Each finite scale times each code times a tensor scale of any size, to fp32: the exact product of 30 bits, rounded once."""
+    byte = torch.arange(127)[:, None]
+    code = torch.arange(16).repeat(127, 1)
+    packed = (code[:, 0::2] | code[:, 1::2] << 4).to(torch.uint8).to(DEV)
+    packed = packed if layout == "words" else packed.t().contiguous().t()
+    ts = torch.tensor(t, dtype=torch.float32)
+    got = st.dequantize_fp4(packed, tiled(byte).view(E4).to(DEV), ts.to(DEV), out_dtype=torch.float32).cpu()
+    want = values(code, byte, None, E4) * ts.double()
+    assert torch.equal(got, want.float())
+    assert torch.equal(torch.signbit(got), torch.signbit(want))
