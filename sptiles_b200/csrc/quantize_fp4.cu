@@ -13,9 +13,10 @@
 // scale NaN, and what is computed from it is NaN; t is taken over the finite
 // elements.
 //
-// Bound by DRAM: 8192 x 8192 bf16 in 29 us in blocks of 16 with a known maximum
-// and in 26 in blocks of 32 (26.2 at the copy rate); the maximum's own pass takes
-// 28; back to values 32 (26.2).
+// Bound by DRAM: 8192 x 8192 bf16 in 33 us in blocks of 16 with a known maximum
+// and in 30 in blocks of 32 (26.2 at the copy rate); the maximum's own pass takes
+// 25; back to values 32 (26.2).  (A replayed graph over three inputs; over one,
+// part of which stays in L2, 29 and 26.)
 //
 // Scales leave in the order in which the tensor core takes them:
 // [row / 128][block / 4][row % 32][row / 32 % 4][block % 4], one byte each,
@@ -498,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, WIDE && sizeof(T) == 2 ? 2 : 4)
         }
     };
     // blocks of 32 of 16 bits, which fill the registers of two CTAs anyway, read the next tile beside this one's work
-    // (8192 x 8192 bf16 43 -> 36 us; blocks of 16, with four CTAs an SM, 41 -> 44)
+    // (8192 x 8192 bf16 43 -> 36 us; blocks of 16, with four CTAs an SM, 41 -> 44, over one input)
     constexpr bool kAhead = WIDE && sizeof(T) == 2;
     uint4 v[kSteps];
     if (kAhead && in_words && blockIdx.x < total) read(place(blockIdx.x), v);
@@ -594,32 +595,39 @@ __global__ void __launch_bounds__(kThreads, WIDE && sizeof(T) == 2 ? 2 : 4)
 // What a block's codes are multiplied by: an e4m3 scale in f16, where its
 // product with a code is exact (6 bits, 2^-10 to 2688), then the tensor's scale
 // in fp32, the one rounding; an e8m0 scale in fp32.
+template <bool WIDE>
 struct Back {
     __half2 scale;
     float factor;
+    __device__ __forceinline__ Back(uint32_t byte, float t) {
+        if constexpr (WIDE) {
+            factor = byte == 255u ? NAN : power_of_two(static_cast<int>(byte) - 127);
+        } else {
+            scale = __half2half2(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+            factor = t;
+        }
+    }
+    __device__ __forceinline__ uint64_t two(uint32_t byte) const {
+        __half2 code = __half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1));
+        if constexpr (!WIDE) code = __hmul2(code, scale);
+        const float2 v = __half22float2(code);
+        return mul2(pack2(v.x, v.y), pack2(factor, factor));
+    }
 };
-__device__ __forceinline__ Back back_of(uint32_t byte, bool wide, float t) {
-    if (wide) return Back{__float2half2_rn(1.0f), byte == 255u ? NAN : power_of_two(static_cast<int>(byte) - 127)};
-    return Back{__half2half2(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3))), t};
-}
-__device__ __forceinline__ uint64_t two_values(uint32_t byte, const Back &b) {
-    const __half2 code = __half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(byte), __NV_E2M1));
-    const float2 v = __half22float2(__hmul2(code, b.scale));
-    return mul2(pack2(v.x, v.y), pack2(b.factor, b.factor));
-}
 
 // The values of 16 codes.
-__device__ __forceinline__ void values16(uint64_t (&f)[2][4], uint2 code, const Back &b) {
+template <bool WIDE>
+__device__ __forceinline__ void values16(uint64_t (&f)[2][4], uint2 code, const Back<WIDE> &b) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[h][j] = two_values((h ? code.y : code.x) >> (8 * j) & 0xffu, b);
+        for (int j = 0; j < 4; ++j) f[h][j] = b.two((h ? code.y : code.x) >> (8 * j) & 0xffu);
 }
 
 // A lane takes 8 columns of eight rows, whose reads are under way together; its
 // values of a row are 16 bytes of 16 bits, so that a warp's store is whole
 // sectors (16 columns a lane: 42 us for 8192 x 8192 bf16, so 33).
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 4) dequantize4_words_kernel(const Dequantize4Args p, uint32_t across, uint32_t chunks,
                                                                         int64_t quads) {
     pdl_wait();
@@ -632,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 4) dequantize4_words_kernel(const De
         const int left = static_cast<int>(p.cols) - static_cast<int>(part) * 8;
         if (left <= 0) continue;
         const uint8_t *q = p.q + row0 * p.sq0 + part * 4;
-        const uint8_t *scale = p.scale + scale_at(row0, p.wide ? part >> 2 : part >> 1, quads);  // the next row's 16 bytes on
+        const uint8_t *scale = p.scale + scale_at(row0, WIDE ? part >> 2 : part >> 1, quads);  // the next row's 16 bytes on
         uint32_t code[kRows], byte[kRows];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
@@ -651,10 +659,10 @@ __global__ void __launch_bounds__(kThreads, 4) dequantize4_words_kernel(const De
 #pragma unroll
         for (int i = 0; i < kRows; ++i, out += p.so0) {
             if (row0 + i >= p.rows) break;
-            const Back b = back_of(byte[i], p.wide, t);
+            const Back<WIDE> b(byte[i], t);
             uint64_t f[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = two_values(code[i] >> (8 * j) & 0xffu, b);
+            for (int j = 0; j < 4; ++j) f[j] = b.two(code[i] >> (8 * j) & 0xffu);
             if (left >= 8) {
                 constexpr int kWords = static_cast<int>(sizeof(T) / 2);
                 uint4 o[kWords];
@@ -673,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 4) dequantize4_words_kernel(const De
 
 // Any strides, unit ones among them: a lane's 16 values are turned in shared
 // memory, so that neighbouring lanes store neighbouring elements.
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) dequantize4_any_kernel(const Dequantize4Args p, uint32_t across, int64_t chunks,
                                                                    int64_t quads, bool words) {
     pdl_wait();
@@ -697,10 +705,10 @@ __global__ void __launch_bounds__(kThreads) dequantize4_any_kernel(const Dequant
                 for (int j = 0; j < 8; ++j)
                     if (2 * j < left) (j < 4 ? code.x : code.y) |= static_cast<uint32_t>(q[j * p.sq1]) << (8 * (j & 3));
             }
-            byte = p.scale[scale_at(row, p.wide ? unit >> 1 : unit, quads)];
+            byte = p.scale[scale_at(row, WIDE ? unit >> 1 : unit, quads)];
         }
         uint64_t f[2][4];
-        values16(f, code, back_of(byte, p.wide, t));
+        values16(f, code, Back<WIDE>(byte, t));
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < 16; ++j) mine[17 * lane + j] = j & 1 ? hi2(f[j / 8][j % 8 / 2]) : lo2(f[j / 8][j % 8 / 2]);
@@ -815,20 +823,20 @@ int launch_typed(Quantize4Args p, float *maxima, int sm_count, cudaStream_t stre
     return launch_quantize<T, false>(p, sm_count, stream);
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 int launch_dequantize(const Dequantize4Args &p, int sm_count, cudaStream_t stream) {
-    const int64_t quads = cdiv(cdiv(p.cols, p.wide ? 32 : 16), 4);
+    const int64_t quads = cdiv(cdiv(p.cols, WIDE ? 32 : 16), 4);
     const bool words = p.sq1 == 1 && reinterpret_cast<uintptr_t>(p.q) % 8 == 0 && (p.rows == 1 || p.sq0 % 8 == 0);
     if (words && p.so1 == 1 && on16(p.out, p.so0, p.rows, sizeof(T)) && cdiv(p.rows, 8) * cdiv(p.cols, 256) <= INT32_MAX) {
         const int64_t across = cdiv(p.cols, 256), chunks = cdiv(p.rows, 8) * across;
-        auto kern = dequantize4_words_kernel<T>;
-        const unsigned grid = resident_grid<decltype(kern), T>(kern, cdiv(chunks, kWarps), sm_count, 0);
+        auto kern = dequantize4_words_kernel<T, WIDE>;
+        const unsigned grid = resident_grid<decltype(kern), T, std::bool_constant<WIDE>>(kern, cdiv(chunks, kWarps), sm_count, 0);
         ST_CUDA_TRY(launch_kernel(kern, grid, kThreads, 0, stream, p, static_cast<uint32_t>(across), static_cast<uint32_t>(chunks), quads));
         return checked("dequantize4_words_kernel");
     }
     const int64_t across = cdiv(p.cols, 512);
-    auto kern = dequantize4_any_kernel<T>;
-    const unsigned grid = resident_grid<decltype(kern), T, int>(kern, cdiv(p.rows * across, kWarps), sm_count, 0);
+    auto kern = dequantize4_any_kernel<T, WIDE>;
+    const unsigned grid = resident_grid<decltype(kern), T, std::bool_constant<WIDE>, int>(kern, cdiv(p.rows * across, kWarps), sm_count, 0);
     ST_CUDA_TRY(launch_kernel(kern, grid, kThreads, 0, stream, p, static_cast<uint32_t>(across), p.rows * across, quads, words));
     return checked("dequantize4_any_kernel");
 }
@@ -856,9 +864,9 @@ int launch_quantize_fp4(const Quantize4Args &p, void *workspace, int sm_count, c
 int launch_dequantize_fp4(const Dequantize4Args &p, int sm_count, cudaStream_t stream) {
     if (p.rows == 0 || p.cols == 0) return ST_OK;
     switch (p.out_dtype) {
-    case ST_F32: return launch_dequantize<float>(p, sm_count, stream);
-    case ST_F16: return launch_dequantize<__half>(p, sm_count, stream);
-    default: return launch_dequantize<__nv_bfloat16>(p, sm_count, stream);
+    case ST_F32: return p.wide ? launch_dequantize<float, true>(p, sm_count, stream) : launch_dequantize<float, false>(p, sm_count, stream);
+    case ST_F16: return p.wide ? launch_dequantize<__half, true>(p, sm_count, stream) : launch_dequantize<__half, false>(p, sm_count, stream);
+    default: return p.wide ? launch_dequantize<__nv_bfloat16, true>(p, sm_count, stream) : launch_dequantize<__nv_bfloat16, false>(p, sm_count, stream);
     }
 }
 
