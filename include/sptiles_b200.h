@@ -304,7 +304,7 @@ int st_matmul_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
  *            scale = e4m3(max|a| of the block / (6 t)), Q = e2m1(a / (scale t)); 0 where scale is 0
  *   ST_E8M0: scale = least power of two >= 2^-127 with 6 scale >= max|a| of the block, Q = e2m1(a / scale)
  * rounded to nearest even, saturating.  amax: one f32, the largest |a| to
- * provide for (larger elements saturate), or NULL: then it is taken from A's
+ * provide for (larger elements saturate with their sign), or NULL: then it is taken from A's
  * finite elements, in a first pass.  A block with a NaN or an infinity gets
  * the scale NaN.  Q has unit column stride.  workspace: st_quantize_fp4_workspace
  * bytes, 4-byte aligned, where amax is to be taken.
@@ -348,8 +348,9 @@ int st_matmul_fp4(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
  * product.  `d` is the first group's [K, N], unit column stride; the groups lie
  * one behind the other, or their rows in turn ([K, groups, N]), and do not
  * overlap.  (The gradient of A is st_matmul_grouped with B's transposed view.)
- * Sums are fp32.  The same inputs give the same bits, whatever the other
- * groups' rows hold.  An operand is read in place if it is contiguous along a
+ * Sums are fp32 as the tensor core adds them, truncating: within (K + 4) 2^-23
+ * of the sum of the terms' magnitudes.  The same inputs give the same bits,
+ * whatever the other groups' rows hold.  An operand is read in place if it is contiguous along a
  * dimension (A of st_matmul_grouped along K; both operands of the second form
  * along their columns), with its rows and groups on 16-byte boundaries; any
  * other is copied first, into `workspace` (16-byte aligned).  Every buffer starts

@@ -16,8 +16,8 @@
 // CTA pairs on 256 x 256 tiles, unless there are few rows of A or few tiles of
 // a long K: then 128 x 16, 32 or 64 tiles of one CTA, two of them on an SM,
 // and a cluster of up to 8 that splits the K of a tile.  8192^3 in 197 us over 20
-// calls (5580 TFLOP/s) and 229 over seconds, under the power cap; 1024^3 in 5.3
-// in a replayed graph, 1 x 8192 x 8192 in 8.4 to 8.9 (5.8 at the copy rate).
+// calls (5580 TFLOP/s) and 229 to 243 over seconds, under the power cap; 1024^3 in
+// 5.6 in a replayed graph, 1 x 8192 x 8192 in 8.4 to 9.7 (5.8 at the copy rate).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

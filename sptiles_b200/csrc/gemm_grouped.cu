@@ -45,12 +45,12 @@
 namespace st {
 namespace {
 
-// Measured, bf16: one group of 16384 rows of 4096 x 4096 340 to 355 us (1540 to
-// 1618 TFLOP/s), 32 unequal groups of them 410 over 20 calls and 515 over seconds
-// under the power cap (the tensor pipe 85 % busy); 64 rows on 64 groups of 2048 x
-// 4096 98 us, bound by the weights' bytes (92 at the copy rate); the gradient of
-// 32 x 2048 x 4096 in f32 from 16384 rows 364 to 374 (194), bound by its stores
-// beside the loads.
+// Measured, bf16: one group of 16384 rows of 4096 x 4096 340 to 400 us (1370 to
+// 1618 TFLOP/s), 32 unequal groups of them 410 to 470 over 20 calls and 510 to 545
+// over seconds under the power cap (the tensor pipe 85 % busy); 64 rows on 64
+// groups of 2048 x 4096 98 us, bound by the weights' bytes (92 at the copy rate);
+// the gradient of 32 x 2048 x 4096 from 16384 rows in f32 295 on a cool card to 400
+// (194), in bf16 235 to 260 (165: the products), bound by its stores beside the loads.
 constexpr int kMaxGroups = kGroupedMaxGroups;
 constexpr int kBK = 64;  // elements of the contraction a stage: 128 bytes, one swizzle span
 constexpr int kMmaK = 16;
@@ -208,10 +208,10 @@ __device__ __forceinline__ void load_columns(uint32_t dst, const CUtensorMap *ma
 }
 
 // ---- C.  The TMEM lanes lie along C's rows and the columns are rows of C, so
-// that a register of a warp is 32 neighbouring elements, stored as they are.
-// (Through shared memory and 16-byte stores, or TMA stores, was slower: the
-// loads' way into the SM is what bounds the kernels.  Weights of 32 x 2048 x
-// 4096 f32 from 16384 rows 318 us by TMA stores, 293 by 16-byte stores.)
+// that a register of a warp is 32 neighbouring elements, stored as they are, at
+// any alignment.  (An earlier form of the kernels stored through shared memory, by
+// TMA or 16 bytes a lane, for no gain; that was within what boxes differ by and has
+// not been tried in this form.)
 //
 // A warp's share (every other 32) of `cols` columns of 32 TMEM lanes.  at: the element of C of lane 0 and column 0; `lanes` of the lanes are inside.  zero:
 // there was nothing to sum.  released(): the accumulator has been read.

@@ -93,7 +93,7 @@ def quantize_fp4(A: torch.Tensor, *, scale_dtype: torch.dtype = torch.float8_e4m
     of two t >= 2^-126 with 2688 t >= amax, a block's scale is
     e4m3(max|a| / (6 t)), its codes e2m1(a / (scale t)).  ``amax`` (one
     float32 on the device) is the largest |a| to provide for, larger elements
-    saturate; left out, it is taken from A's finite elements in a first pass.
+    saturate with their sign, however large; left out, it is taken from A's finite elements in a first pass.
     scale_dtype float8_e8m0fnu, blocks of 32: a block's scale is the least
     power of two >= 2^-127 with 6 scale >= max|a|, its codes e2m1(a / scale).
 
@@ -143,9 +143,10 @@ def dequantize_fp4(codes: torch.Tensor, scale: torch.Tensor, tensor_scale: torch
     """The values of 4-bit blocks: code * scale * tensor_scale, rounded to fp32 and that to out_dtype.
 
     (In fp32 it is exact where tensor_scale is a power of two, as quantize_fp4
-    makes it, and the result within fp32's normal range.)  codes, scale and tensor_scale as quantize_fp4 makes them (codes of any
-    strides; uint8 is taken as well); ``cols`` where the last byte of a row
-    holds one element only.
+    makes it, and the result lies in fp32's normal range.)  codes, scale and
+    tensor_scale as quantize_fp4 makes them, or any other tensor scale (codes
+    of any strides; uint8 is taken as well); ``cols`` where the last byte of a
+    row holds one element only.
     """
     dq = _codes_desc(codes, "codes")
     if out_dtype not in _CODES:
@@ -176,9 +177,10 @@ def matmul_fp4(A: torch.Tensor, B: torch.Tensor, a_scale: torch.Tensor, b_scale:
     boundaries are read in place, anything else is copied first.  a_scale and
     b_scale have one dtype, which says the blocks' length; entries of theirs
     that belong to no block must be 0 (or at least finite).  The sum is fp32;
-    it is multiplied by a_tensor_scale * b_tensor_scale, the bias (length N;
-    float32 or C's dtype) is added, and the result rounded once to C's dtype,
-    bfloat16, float16 or float32.  The same inputs give the same bits.
+    it is multiplied by a_tensor_scale * b_tensor_scale (by one after the other
+    where that product leaves fp32's normal range), the bias (length N; float32
+    or C's dtype) is added, and the result rounded once to C's dtype, bfloat16,
+    float16 or float32.  The same inputs give the same bits.
     """
     da, db = _codes_desc(A, "A"), _codes_desc(B, "B")
     (m, ka), (kb, n) = A.shape, B.shape

@@ -74,7 +74,10 @@ def matmul_grouped(A: torch.Tensor, B: torch.Tensor, ends: torch.Tensor, *, out_
     gradient of A is this call with B's transposed view).  ends [G], int32 on
     the device, at most 1024 of them: group g is rows [ends[g - 1], ends[g]); groups
     may be empty, and an end out of order counts as the nearest one in order.
-    Sums are fp32; C is out_dtype, A's type by default.  Rows behind the last
+    Sums are fp32 as the tensor core adds them, truncating: within (K + 4) 2^-23
+    of the sum of the terms' magnitudes (for K = 1001 1.2e-6 of the result as a
+    whole, where fp32 operations that round have 0.5e-6), then one rounding to
+    C's type, out_dtype, by default A's.  Rows behind the last
     group are 0 in a new C, and left as they were in ``out``.  The same inputs
     give the same bits.  Operands off 16-byte boundaries are copied first.
     """
@@ -113,9 +116,11 @@ def matmul_grouped_weights(A: torch.Tensor, C: torch.Tensor, ends: torch.Tensor,
 
     A [T, K] and C [T, N], both float16 or both bfloat16, any strides; ends as
     in matmul_grouped.  With C the gradient of matmul_grouped's result, D is
-    that of its B (of B's transposed view with A and C exchanged).  Sums are
-    fp32; D is out_dtype, A's type by default.  The same inputs give the same
-    bits.  Operands off 16-byte boundaries are copied first.
+    that of its B (of B's transposed view with A and C exchanged).  Sums as in
+    matmul_grouped, over a group's rows; D is out_dtype, A's type by default,
+    and ``out`` a stack of any layout whose columns lie together and whose groups
+    do not overlap ([K, G, N] transposed among them).  The same inputs give the
+    same bits.  Operands off 16-byte boundaries are copied first.
     """
     if A.dim() != 2 or C.dim() != 2:
         raise ValueError("A and C must be 2D tensors.")
