@@ -305,7 +305,8 @@ int st_matmul_fp8(st_ctx *ctx, const st_tensor *a, const st_tensor *b, const st_
  *   ST_E8M0: scale = least power of two >= 2^-127 with 6 scale >= max|a| of the block, Q = e2m1(a / scale)
  * rounded to nearest even, saturating.  amax: one f32, the largest |a| to
  * provide for (larger elements saturate with their sign), or NULL: then it is taken from A's
- * finite elements, in a first pass.  A block with a NaN or an infinity gets
+ * finite elements, in a first pass; 0, an infinity or a NaN makes tensor_scale
+ * 1; not tensor_scale's own place.  A block with a NaN or an infinity gets
  * the scale NaN.  Q has unit column stride.  workspace: st_quantize_fp4_workspace
  * bytes, 4-byte aligned, where amax is to be taken.
  * st_dequantize_fp4: the values back, the product of code, scale and tensor

@@ -93,7 +93,8 @@ def quantize_fp4(A: torch.Tensor, *, scale_dtype: torch.dtype = torch.float8_e4m
     of two t >= 2^-126 with 2688 t >= amax, a block's scale is
     e4m3(max|a| / (6 t)), its codes e2m1(a / (scale t)).  ``amax`` (one
     float32 on the device) is the largest |a| to provide for, larger elements
-    saturate with their sign, however large; left out, it is taken from A's finite elements in a first pass.
+    saturate with their sign, however large (0, an infinity or a NaN makes the
+    tensor_scale 1); left out, it is taken from A's finite elements in a first pass.
     scale_dtype float8_e8m0fnu, blocks of 32: a block's scale is the least
     power of two >= 2^-127 with 6 scale >= max|a|, its codes e2m1(a / scale).
 

@@ -627,3 +627,14 @@ def test_dequantize_rounds_once(t, layout):
     want = values(code, byte, None, E4) * ts.double()
     assert torch.equal(got, want.float())
     assert torch.equal(torch.signbit(got), torch.signbit(want))
+
+
+@pytest.mark.parametrize("amax", [0.0, float("inf"), float("-inf"), float("nan")])
+def test_quantize_a_maximum_that_says_nothing(amax):
+    """The tensor's scale is 1."""
+    x = torch.randn(5, 100, generator=gen(1)) * 1000
+    got = st.quantize_fp4(x.to(DEV), amax=torch.tensor(amax, device=DEV))
+    want = st.quantize_fp4(x.to(DEV), amax=torch.tensor(2688.0, device=DEV))
+    assert got.tensor_scale.item() == 1.0
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.uint8) if a.dim() else a, b.view(torch.uint8) if b.dim() else b)
